@@ -381,6 +381,83 @@ int trn_calibration_copy(const void* src, void* dst, int64_t bytes, void* stream
  */
 int trn_calibration_mfma(const void* operands, float* sink, int32_t iters, int32_t n_workgroups, void* stream);
 
+/*
+ * An 8-bit key/value cache: OCP e4m3 codes [batch, n_kv_heads, capacity, head_dim] with a float scale for each head and block of 32, 64 or 128
+ * tokens, [batch, n_kv_heads, ceil(capacity / block)] with unit innermost stride: key j stands for k[j] * k_scale[j / block].  Scales are not
+ * negative.  The sequences of a batch have lengths of their own, read on the device when a launch runs, so that a captured step may be
+ * replayed on caches that have grown.
+ *   lengths   nullable int32 [batch]: the keys of each sequence, this step's new ones among them (NULL: capacity).  Taken into [0, capacity].
+ *   counts    nullable int32 [batch]: its new tokens, of at most as many as the call has rows for (NULL: all); new token i is at position
+ *             lengths[b] - counts[b] + i.  Rows from counts[b] on are padding: neither read nor written.
+ * Neither has a counterpart in the reference, whose caches are fp16 tensors of one length (ref_rms.py:72-73, convert_eval_rms.py:146-147).
+ * Strides of codes are in bytes and multiples of 16, that of a token at most 2^24; head_dim 64 or 128; capacity at most 2^26.
+ */
+typedef struct trn_cache8 {
+    void* k; void* v; float* k_scale; float* v_scale;
+    const int32_t* lengths; const int32_t* counts;
+    int32_t batch, n_kv_heads, capacity, head_dim, block;
+    int64_t k_stride_b, k_stride_h, k_stride_s;
+    int64_t v_stride_b, v_stride_h, v_stride_s;
+    int64_t ks_stride_b, ks_stride_h, vs_stride_b, vs_stride_h;      /* of the scales, in floats */
+} trn_cache8;
+
+/*
+ * New keys and values k, v [batch, n_kv_heads, tokens, head_dim] (fp16, strided) into the cache: the quantising form of the cache append
+ * of ref_rms.py:72-73.  A block's scale is the least power of two s with |x| <= 448 s for its finite values, 2^-32 at least; a code is x * (1 / s) rounded to
+ * nearest even, infinities and NaN become NaN.  A block that holds earlier tokens keeps its scale unless the new ones need a larger one:
+ * the codes that are there are then multiplied by old / new and rounded again (between powers of two: exactly, but for those that
+ * become subnormal).  Nothing else of the cache is written.  k and v must not overlap the cache.
+ */
+int trn_cache8_append_f16(const trn_cache8* cache, const void* k, const void* v, int32_t tokens,
+                          int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_s,
+                          int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_s, void* stream);
+
+/*
+ * o = softmax(scale * q k^T) v over an 8-bit cache: trn_attn_fwd_f16 for q, o [batch, n_q_heads, seq_q, head_dim] fp16 (o on 8 bytes), GQA / MQA.
+ * causal: query i sees the keys j <= lengths[b] - counts[b] + i.  A query that sees no key gets zeros (lse -inf).
+ *   lse           nullable float [batch, n_q_heads, seq_q] contiguous, natural log.
+ *   weights_out   nullable float [batch, n_kv_heads, capacity] contiguous: weights_in (nullable: zeros) plus the attention weight that each key gets,
+ *                 summed over the queries and the query heads of its KV head; keys from lengths[b] on are left as they are.  weights_in may be
+ *                 weights_out: a running sum, as eviction by accumulated weight takes it.  Deterministic: no atomics.
+ *   workspace     trn_cache8_attn_workspace_bytes(...) bytes, 256-byte aligned, no initial contents: the keys of a head are then shared out over
+ *                 workgroups.  May be NULL or smaller without weights_out: a workgroup then walks over all of a row tile's keys; with weights_out
+ *                 it is TRN_E_SCRATCH.  One call at a time may use it.
+ */
+int64_t trn_cache8_attn_workspace_bytes(const trn_cache8* cache, int32_t n_q_heads, int32_t seq_q, int32_t with_weights);
+int trn_cache8_attn_f16(const trn_cache8* cache, const void* q, void* o, int32_t n_q_heads, int32_t seq_q,
+                        int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_s,
+                        int64_t o_stride_b, int64_t o_stride_h, int64_t o_stride_s,
+                        float scale, int32_t causal, float* lse, const float* weights_in, float* weights_out,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Eviction from a cache by accumulated attention weight -- what the key scores of KeyFormer and RoCo are for (ref_rms.py:171-179, 249-280; the
+ * reference stops at the scores).  Of the n = lengths[b] keys of a sequence the last min(recent, n, keep) stay, and of the others those with the
+ * largest weights, min(n, keep) keys in all; ties go to the earlier key, NaN counts as the smallest.  They move to the front in their order.
+ *   weights     float, or fp16 with weights_half, [batch, n_weight_rows, keys] contiguous; n_weight_rows a multiple of n_kv_heads: a KV head's are its
+ *               rows' sum, added in 64 bits and rounded once to float (KeyFormer's C_out has a row for each query head).
+ *   k, v        fp16 (code_bytes 2) or e4m3 codes (1) [batch, n_kv_heads, keys, head_dim]; k_out, v_out [.., keep (or more), head_dim].  An output may be its
+ *               input, with the same strides; otherwise no output may overlap K or V.  Rows from the new length on are left as they are.
+ *   *_scale     8 bits only: float [batch, n_kv_heads, ceil(keys / block)], the outputs over ceil(keep / block) blocks; an output may be its input.  A block
+ *               of the result has the largest of the scales that its rows come with; codes of rows with a smaller one are multiplied by the
+ *               ratio and rounded again.
+ *   weights_out nullable: the kept keys' weights [batch, n_weight_rows, keep], or weights itself, whose places behind the new length and
+ *               before the old one are then set to zero.
+ *   kept        int32 [batch, n_kv_heads, keep]: the kept keys' old positions, ascending, then -1.
+ *   new_lengths nullable int32 [batch]: min(n, keep); may be lengths.
+ *   workspace   trn_cache_evict_workspace_bytes(desc) bytes, 256-byte aligned, no initial contents.
+ * Strides are in elements (codes: bytes), not negative, multiples of 16 bytes; batch, head, token.
+ */
+typedef struct trn_cache_evict_desc {
+    int32_t batch, n_kv_heads, n_weight_rows, keys, head_dim, code_bytes, block, keep, recent, weights_half;
+    int64_t k_stride[3], v_stride[3], k_out_stride[3], v_out_stride[3];
+    int64_t k_scale_stride[2], v_scale_stride[2], k_scale_out_stride[2], v_scale_out_stride[2];
+} trn_cache_evict_desc;
+int64_t trn_cache_evict_workspace_bytes(const trn_cache_evict_desc* desc);
+int trn_cache_evict(const trn_cache_evict_desc* desc, const void* k, const void* v, void* k_out, void* v_out, const float* k_scale, const float* v_scale,
+                    float* k_scale_out, float* v_scale_out, const void* weights, void* weights_out, const int32_t* lengths,
+                    int32_t* kept, int32_t* new_lengths, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

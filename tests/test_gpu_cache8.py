@@ -1,0 +1,360 @@
+"""8-bit caches on the GPU: the quantising append, attention over them and the key weights, against the definitions in 64 bits.  Codes and scales are
+held to equality; outputs to the bounds that oracle/cache8.py derives."""
+import math
+
+import pytest
+import torch
+
+from oracle import cache8 as ref
+from triton_amd import _lib, modules, ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+SPOIL = 0x7f          # a NaN code: what lies behind a sequence's end must not matter
+
+
+def _cpu(t):
+    return t.detach().cpu()
+
+
+def _cache(B, H, S, D, block, seed, lengths, layout="head", spread=1.0, spoil=True):
+    """Codes, scales and their CPU copies; everything behind a sequence's keys is NaN."""
+    g = torch.Generator().manual_seed(seed)
+    blocks = -(-S // block)
+    out = []
+    for _ in range(2):
+        codes = ref.encode((torch.randn(B, H, S, D, generator=g) * 100.0).clamp(-448, 448))
+        scale = torch.exp2(torch.randint(-3, 4, (B, H, blocks), generator=g).float() * spread - 6.0)
+        if spoil:
+            for b, n in enumerate(lengths):
+                codes[b, :, n:] = SPOIL
+                scale[b, :, -(-n // block):] = math.nan
+        if layout == "token":          # [B, S, H, D] memory
+            dev = torch.empty(B, S, H, D, dtype=torch.uint8, device=DEV).permute(0, 2, 1, 3)
+        elif layout == "padded":       # rows further apart than they are long
+            dev = torch.full((B, H, S, D + 32), SPOIL, dtype=torch.uint8, device=DEV)[..., 16:16 + D]
+        else:
+            dev = torch.empty(B, H, S, D, dtype=torch.uint8, device=DEV)
+        dev.copy_(codes)
+        sdev = scale.to(DEV) if layout == "head" else torch.zeros(B, H, blocks + 3, device=DEV)[..., :blocks].copy_(scale)
+        out += [codes, scale, dev, sdev]
+    return out
+
+
+def _ints(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+APPENDS = [
+    # B, H, D, new, capacity, block, keys of each sequence with the new ones, new tokens of each
+    (1, 8, 128, 1, 64, 64, [1], [1]),                            # the first token
+    (2, 2, 64, 1, 100, 32, [33, 64], [1, 1]),                    # one that opens a block, one that fills it
+    (3, 3, 128, 5, 300, 64, [62, 66, 300], [5, 3, 5]),           # inside a block, across a border, up to the capacity's end
+    (2, 1, 64, 40, 129, 128, [40, 129], [40, 40]),
+    (2, 2, 128, 300, 512, 32, [300, 411], [300, 217]),
+    (4, 2, 64, 7, 65, 64, [0, 3, 65, 7], [0, 7, 0, 2]),          # no token; more new tokens than keys; nothing new
+    (1, 71, 64, 16, 80, 64, [79], [16]),
+]
+
+
+@pytest.mark.parametrize("case", APPENDS, ids=lambda c: f"B{c[0]}H{c[1]}D{c[2]}M{c[3]}S{c[4]}b{c[5]}")
+@pytest.mark.parametrize("layout", ["head", "token", "padded"])
+@pytest.mark.parametrize("size", [1.0, 3e-5, 4000.0])
+def test_append(case, layout, size):
+    B, H, D, M, S, block, lengths, counts = case
+    k8, ks, dk8, dks, v8, vs, dv8, dvs = _cache(B, H, S, D, block, 1, [max(0, n - c) for n, c in zip(lengths, counts)], layout)
+    g = torch.Generator().manual_seed(7)
+    rows = [(torch.randn(B, H, M, D, generator=g) * size * torch.exp(torch.randn(B, H, M, 1, generator=g))).half() for _ in range(2)]
+    dev = [torch.empty(B, M, H, D, dtype=torch.float16, device=DEV).permute(0, 2, 1, 3).copy_(r) if layout == "token" else r.to(DEV) for r in rows]
+    ops.cache8_append(*dev, dk8, dv8, dks, dvs, lengths=_ints(lengths), counts=_ints(counts), block=block)
+    for x, codes, scale, dc, ds in ((rows[0], k8, ks, dk8, dks), (rows[1], v8, vs, dv8, dvs)):
+        want, ws = ref.append(x, codes, scale, lengths, counts, block)
+        assert torch.equal(torch.nan_to_num(_cpu(ds), nan=-1.0), torch.nan_to_num(ws, nan=-1.0))
+        assert torch.equal(_cpu(dc), want)
+
+
+def test_append_without_lengths_takes_the_last_rows_and_float8_tensors():
+    B, H, D, M, S, block = 2, 2, 128, 9, 70, 32
+    k8, ks, dk8, dks, v8, vs, dv8, dvs = _cache(B, H, S, D, block, 3, [S, S])
+    g = torch.Generator().manual_seed(8)
+    rows = [torch.randn(B, H, M, D, generator=g).half() for _ in range(2)]
+    ops.cache8_append(rows[0].to(DEV), rows[1].to(DEV), dk8.view(torch.float8_e4m3fn), dv8.view(torch.float8_e4m3fn), dks, dvs, block=block)
+    for x, codes, scale, dc, ds in ((rows[0], k8, ks, dk8, dks), (rows[1], v8, vs, dv8, dvs)):
+        want, ws = ref.append(x, codes, scale, [S] * B, [M] * B, block)
+        assert torch.equal(_cpu(ds), ws) and torch.equal(_cpu(dc), want)
+
+
+def test_append_of_what_is_not_finite_and_of_the_type_s_ends():
+    B, H, D, M, S, block = 1, 1, 64, 6, 64, 64
+    x = torch.zeros(B, H, M, D, dtype=torch.float16)
+    x[0, 0, 0, :4] = torch.tensor([math.inf, -math.inf, math.nan, 1.0]).half()
+    x[0, 0, 1, :4] = torch.tensor([65504.0, -65504.0, 2.0 ** -24, -(2.0 ** -24)]).half()
+    x[0, 0, 2, :4] = torch.tensor([448.0, 464.0, 480.0, -0.0]).half()
+    for rows in ([0], [1], [2], [3], [0, 1], [2, 3], list(range(6))):
+        part = x[:, :, rows]
+        k8, ks, dk8, dks, v8, vs, dv8, dvs = _cache(B, H, S, D, block, 4, [0])
+        ops.cache8_append(part.to(DEV), part.to(DEV), dk8, dv8, dks, dvs, lengths=_ints([len(rows)]))
+        want, ws = ref.append(part, k8, ks, [len(rows)], [len(rows)], block)
+        assert torch.equal(_cpu(dks), ws)
+        got = _cpu(dk8)
+        nan = torch.isnan(ref.decode(want))
+        assert torch.equal(torch.isnan(ref.decode(got)), nan) and torch.equal(got[~nan], want[~nan])
+
+
+def test_appends_one_by_one_grow_the_scale():
+    """A block filled token by token, each larger than all before: codes are what repeated rescaling of the definition gives."""
+    B, H, D, S, block = 1, 2, 128, 64, 64
+    k8, ks, dk8, dks, v8, vs, dv8, dvs = _cache(B, H, S, D, block, 5, [0])
+    g = torch.Generator().manual_seed(9)
+    for n in range(1, 65):
+        x = (torch.randn(B, H, 1, D, generator=g) * 1.2 ** n * 1e-3).half()
+        ops.cache8_append(x.to(DEV), x.to(DEV), dk8, dv8, dks, dvs, lengths=_ints([n]))
+        k8, ks = ref.append(x, k8, ks, [n], [1], block)
+    assert torch.equal(_cpu(dk8), k8) and torch.equal(_cpu(dks), ks)
+
+
+ATTNS = [
+    # B, Hq, Hkv, D, queries, capacity, block, lengths, counts, causal
+    (1, 32, 8, 128, 1, 70, 64, [70], [1], True),
+    (2, 4, 1, 64, 1, 40, 32, [1, 33], [1, 1], True),             # one key; a tile and one more
+    (3, 2, 2, 128, 3, 100, 32, [0, 2, 100], [3, 3, 2], True),    # no key at all; fewer keys than queries; a padded query
+    (2, 8, 2, 128, 9, 300, 64, [300, 129], [9, 1], True),        # 36 rows: two tiles
+    (1, 71, 1, 64, 5, 500, 128, [437], [5], True),
+    (2, 6, 2, 64, 4, 160, 64, [160, 31], [4, 0], False),         # all keys for all; no query
+    (1, 2, 1, 128, 70, 130, 64, [130], [70], True),              # a prompt's diagonal
+    (1, 1, 1, 64, 33, 33, 32, [33], [33], True),
+    (1, 8, 8, 128, 1, 2500, 64, [2431], [1], True),              # split over workgroups
+    (2, 16, 4, 64, 2, 3000, 128, [3000, 1777], [2, 2], False),
+    (1, 4, 2, 128, 1, 1100, 32, [1100], [1], True),
+]
+
+
+def _check(got, want, tol, name):
+    bad = (got.double() - want).abs() > tol
+    assert not bad.any(), f"{name}: {int(bad.sum())} of {bad.numel()} off, worst {float(((got.double() - want).abs() / tol.clamp(min=1e-30)).max()):.3g} of the bound"
+
+
+def _attend(case, layout="head", spread=1.0, seed=11, size=1.0, spoil=True, edit=None):
+    B, Hq, Hkv, D, M, S, block, lengths, counts, causal = case
+    k8, ks, dk8, dks, v8, vs, dv8, dvs = _cache(B, Hkv, S, D, block, seed, lengths, layout, spread, spoil)
+    if edit:
+        edit(k8, ks, v8, vs)
+        dk8.copy_(k8), dks.copy_(ks), dv8.copy_(v8), dvs.copy_(vs)
+    g = torch.Generator().manual_seed(seed + 1)
+    q = (torch.randn(B, Hq, M, D, generator=g) * size).half()
+    if layout == "token":
+        dq = torch.empty(B, M, Hq, D, dtype=torch.float16, device=DEV).permute(0, 2, 1, 3).copy_(q)
+        o = torch.full((B, M, Hq, D), 7.0, dtype=torch.float16, device=DEV).permute(0, 2, 1, 3)
+    else:
+        dq, o = q.to(DEV), torch.full((B, Hq, M, D), 7.0, dtype=torch.float16, device=DEV)
+    lse = torch.full((B, Hq, M), 7.0, device=DEV)
+    w_in = torch.rand(B, Hkv, S, generator=g)
+    w_out = torch.full((B, Hkv, S), 7.0, device=DEV)
+    ws = torch.full((ops.cache8_attention_workspace_bytes(dq, dk8, True),), 0xff, dtype=torch.uint8, device=DEV)
+    ops.cache8_attention(dq, dk8, dv8, dks, dvs, o, None, causal, _ints(lengths), _ints(counts), lse, w_in.to(DEV), w_out, block, ws)
+    want, wlse, w, tol, wtol, ltol = ref.attention(q, k8, v8, ks, vs, D ** -0.5, causal, lengths, counts, block)
+    there = torch.arange(M)[None, None, :] < torch.tensor([min(c, M) for c in counts])[:, None, None]
+    there = there.expand(B, Hq, M)
+    return dict(o=_cpu(o), lse=_cpu(lse), w=_cpu(w_out), w_in=w_in, want=want, wlse=wlse, ww=w, tol=tol, wtol=wtol, ltol=ltol, there=there, q=dq, k8=dk8, v8=dv8, ks=dks, vs=dvs, ws=ws)
+
+
+def _hold(r, lengths):
+    there = r["there"]
+    assert torch.equal(r["o"][~there], torch.full_like(r["o"][~there], 7.0)), "outputs of queries that are not there"
+    assert (r["lse"][~there] == 7.0).all()
+    nan = torch.isnan(r["want"]) & there[..., None]
+    assert torch.equal(torch.isnan(r["o"]) & there[..., None], nan)
+    fine = there[..., None].expand_as(nan) & ~nan
+    _check(r["o"][fine], r["want"][fine], r["tol"][fine], "o")
+    empty = there & torch.isinf(r["wlse"])
+    assert (r["lse"][empty] == -math.inf).all() and (r["o"][empty] == 0).all()
+    some = there & torch.isfinite(r["wlse"])
+    _check(r["lse"][some], r["wlse"][some], r["ltol"][some], "lse")
+    for b, n in enumerate(lengths):
+        assert (r["w"][b, :, n:] == 7.0).all(), "weights behind the last key"
+        total = r["w_in"][b, :, :n].double() + r["ww"][b, :, :n]
+        ok = torch.isfinite(total)
+        _check(r["w"][b, :, :n][ok], total[ok], (r["wtol"][b, :, :n] + 2.0 ** -23 * total.abs())[ok], "weights")
+
+
+@pytest.mark.parametrize("case", ATTNS, ids=lambda c: f"B{c[0]}q{c[1]}kv{c[2]}D{c[3]}M{c[4]}S{c[5]}b{c[6]}c{int(c[9])}")
+@pytest.mark.parametrize("layout", ["head", "token", "padded"])
+def test_attention_and_weights(case, layout):
+    _hold(_attend(case, layout), case[7])
+
+
+@pytest.mark.parametrize("spread", [0.0, 4.0])
+@pytest.mark.parametrize("case", [ATTNS[3], ATTNS[8], ATTNS[6]], ids=["tiles", "split", "prompt"])
+def test_scales_that_differ_by_powers_and_by_nothing(case, spread):
+    _hold(_attend(case, spread=spread, size=0.3), case[7])
+
+
+def test_any_scale_and_none():
+    """Scales that are no powers of two, and blocks of zeros whose scale is zero (their keys count in the sum)."""
+    def edit(k8, ks, v8, vs):
+        ks *= 1.37; vs *= 0.77
+        ks[:, :, 0] = 0.0
+        vs[:, 0, 1] = 0.0
+    case = ATTNS[3]
+    _hold(_attend(case, edit=edit), case[7])
+
+
+def test_large_scores_and_a_single_key_that_takes_all():
+    case = ATTNS[8]
+    r = _attend(case, size=40.0)
+    _hold(r, case[7])
+
+
+@pytest.mark.parametrize("case", [ATTNS[6], ATTNS[7], ATTNS[3]], ids=["prompt", "tile", "chunk"])
+def test_nan_of_a_key_reaches_only_the_queries_that_see_it(case):
+    def edit(k8, ks, v8, vs):
+        n = case[7][0]
+        v8[0, 0, n - 2, 5] = 0x7f
+        v8[0, 0, n - 20, 40] = 0xff
+    r = _attend(case, edit=edit)
+    assert torch.isnan(r["want"]).any() and torch.isfinite(r["want"][r["there"]]).any()
+    _hold(r, case[7])
+
+
+def test_nan_in_a_key_code():
+    case = ATTNS[6]
+    def edit(k8, ks, v8, vs):
+        k8[0, 0, case[7][0] - 30, 3] = 0x7f
+    r = _attend(case, edit=edit)
+    nan = torch.isnan(r["want"])
+    assert nan.any() and not nan.all()
+    there = r["there"][..., None].expand_as(nan)
+    assert torch.equal(torch.isnan(r["o"])[there], nan[there])
+    _check(r["o"][there & ~nan], r["want"][there & ~nan], r["tol"][there & ~nan], "o")
+
+
+def test_without_a_workspace_lse_or_weights():
+    case = ATTNS[8]
+    r = _attend(case)
+    B, Hq, Hkv, D, M, S, block, lengths, counts, causal = case
+    o = torch.zeros(B, Hq, M, D, dtype=torch.float16, device=DEV)
+    ops.cache8_attention(r["q"], r["k8"], r["v8"], r["ks"], r["vs"], o, None, causal, _ints(lengths), _ints(counts), block=block)
+    _check(_cpu(o), r["want"], r["tol"], "o")
+
+
+def test_weights_add_up_in_place():
+    case = ATTNS[3]
+    B, Hq, Hkv, D, M, S, block, lengths, counts, causal = case
+    r = _attend(case)
+    w = r["w_in"].to(DEV)
+    for _ in range(2):
+        ops.cache8_attention(r["q"], r["k8"], r["v8"], r["ks"], r["vs"], torch.empty_like(r["q"]), None, causal, _ints(lengths), _ints(counts), None, w, w, block, r["ws"])
+    for b, n in enumerate(lengths):
+        total = r["w_in"][b, :, :n].double() + 2 * r["ww"][b, :, :n]
+        _check(_cpu(w)[b, :, :n], total, 2 * r["wtol"][b, :, :n] + 2.0 ** -22 * total.abs(), "weights")
+        assert torch.equal(_cpu(w)[b, :, n:], r["w_in"][b, :, n:])
+
+
+def test_a_long_cache_past_two_gigabytes_of_offsets():
+    """Rows 64 KB apart: the last of 40000 keys lies 2.6 GB behind the first."""
+    B, Hq, Hkv, D, M, S, block, pitch = 1, 2, 1, 64, 1, 40000, 128, 1 << 16
+    g = torch.Generator().manual_seed(5)
+    store = torch.empty(2, S, pitch, dtype=torch.uint8, device=DEV)
+    codes = [ref.encode((torch.randn(1, 1, S, D, generator=g) * 30.0).clamp(-448, 448)) for _ in range(2)]
+    dev = []
+    for i in range(2):
+        t = store[i, :, 32:32 + D][None, None]
+        t.copy_(codes[i])
+        dev.append(t)
+    scale = [torch.full((1, 1, -(-S // block)), 2.0 ** -5) for _ in range(2)]
+    q = torch.randn(B, Hq, M, D, generator=g).half()
+    o = torch.zeros(B, Hq, M, D, dtype=torch.float16, device=DEV)
+    ws = torch.empty(ops.cache8_attention_workspace_bytes(q, dev[0]), dtype=torch.uint8, device=DEV)
+    ops.cache8_attention(q.to(DEV), dev[0], dev[1], scale[0].to(DEV), scale[1].to(DEV), o, block=block, workspace=ws)
+    want, _, _, tol, _, _ = ref.attention(q, codes[0], codes[1], scale[0], scale[1], D ** -0.5, True, [S], [1], block)
+    _check(_cpu(o), want, tol, "o")
+
+
+def test_the_same_bits_again():
+    case = ATTNS[8]
+    a, b = _attend(case), _attend(case)
+    assert torch.equal(a["o"], b["o"]) and torch.equal(a["w"], b["w"]) and torch.equal(a["lse"], b["lse"])
+
+
+def test_captured_and_replayed_on_a_cache_that_grows():
+    """A step of append and attention with weights, captured once and replayed while `lengths` grow on the device."""
+    B, Hq, Hkv, D, S, block = 2, 8, 2, 128, 700, 64
+    lengths = [600, 65]
+    k8, ks, dk8, dks, v8, vs, dv8, dvs = _cache(B, Hkv, S, D, block, 21, lengths)
+    g = torch.Generator().manual_seed(22)
+    app, att = modules.get("append8", "cache", block=block), modules.get("weights8", "cache", block=block)
+    k, v = (torch.zeros(B, Hkv, 1, D, dtype=torch.float16, device=DEV) for _ in range(2))
+    q, o = (torch.zeros(B, Hq, 1, D, dtype=torch.float16, device=DEV) for _ in range(2))
+    w = torch.zeros(B, Hkv, S, device=DEV)
+    n = _ints(lengths)
+
+    def step():
+        n.add_(1)
+        app.forward(k, dk8, dks, v, dv8, dvs, None, n)
+        att.forward(dk8, dks, o, q, dv8, dvs, None, n, w, w)
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        att.forward(dk8, dks, o, q, dv8, dvs, None, n, None, torch.zeros_like(w))      # (its workspace)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        step()
+    side.synchronize()
+    ww = torch.zeros(B, Hkv, S, dtype=torch.float64)
+    slack = torch.zeros(B, Hkv, S, dtype=torch.float64)
+    for t in range(6):
+        rows = [torch.randn(B, h, 1, D, generator=g).half() for h in (Hkv, Hkv, Hq)]
+        for dst, src in zip((k, v, q), rows):
+            dst.copy_(src)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        lengths = [x + 1 for x in lengths]
+        k8, ks = ref.append(rows[0], k8, ks, lengths, [1, 1], block)
+        v8, vs = ref.append(rows[1], v8, vs, lengths, [1, 1], block)
+        want, _, got_w, tol, wtol, _ = ref.attention(rows[2], k8, v8, ks, vs, D ** -0.5, True, lengths, [1, 1], block)
+        _check(_cpu(o), want, tol, f"o of step {t}")
+        ww += got_w
+        slack += wtol + 2.0 ** -23 * ww
+        _check(_cpu(w), ww, slack, f"weights of step {t}")
+        assert torch.equal(_cpu(dk8)[0, :, :lengths[0]], k8[0, :, :lengths[0]])
+
+
+def test_first_call_inside_a_capture_is_refused():
+    k8, ks, dk8, dks, v8, vs, dv8, dvs = _cache(1, 2, 64, 64, 64, 31, [64])
+    q = torch.zeros(1, 2, 1, 64, dtype=torch.float16, device=DEV)
+    att = modules.get("weights8", "cache")
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side), pytest.raises(RuntimeError, match="eagerly"):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            att.forward(dk8, dks, q, q.clone(), dv8, dvs, None, None, None, torch.zeros(1, 2, 64, device=DEV))
+
+
+def test_refusals():
+    k8, ks, dk8, dks, v8, vs, dv8, dvs = _cache(1, 2, 64, 64, 64, 31, [64])
+    q = torch.zeros(1, 4, 1, 64, dtype=torch.float16, device=DEV)
+    o = torch.zeros_like(q)
+    good = dict(q=q, k8=dk8, v8=dv8, k_scale=dks, v_scale=dvs, o=o)
+    ops.cache8_attention(**good)
+
+    def bad(error=ValueError, **kw):
+        with pytest.raises(error):
+            ops.cache8_attention(**{**good, **kw})
+    bad(q=q.float()); bad(o=o[:, :2]); bad(q=q[:, :3], o=o[:, :3]); bad(k8=dk8.float()); bad(v8=dv8[:, :, :32]); bad(block=48); bad(block=32)
+    bad(k_scale=dks.half()); bad(k_scale=dks[..., :0]); bad(lengths=torch.zeros(1, dtype=torch.int64, device=DEV)); bad(lengths=torch.zeros(2, dtype=torch.int32, device=DEV))
+    bad(counts=torch.zeros(1, dtype=torch.int32)); bad(weights=torch.zeros(1, 2, 64, device=DEV)); bad(weights_out=torch.zeros(1, 4, 64, device=DEV))
+    bad(lse=torch.zeros(1, 4, 2, device=DEV)); bad(workspace=torch.zeros(4, device=DEV)); bad(q=q.cpu())
+    bad(_lib.TrnError, scale=0.0); bad(_lib.TrnError, scale=math.nan); bad(_lib.TrnError, weights_out=torch.zeros(1, 2, 64, device=DEV))
+    wide = torch.zeros(1, 4, 1, 72, dtype=torch.float16, device=DEV)[..., 4:68]
+    bad(_lib.TrnError, q=wide)
+    k = torch.zeros(1, 2, 1, 64, dtype=torch.float16, device=DEV)
+    ops.cache8_append(k, k, dk8, dv8, dks, dvs)
+    for kw in (dict(k=k.float()), dict(k=k[:, :1]), dict(v=torch.zeros(1, 2, 2, 64, dtype=torch.float16, device=DEV)), dict(block=16)):
+        with pytest.raises(ValueError):
+            ops.cache8_append(**{**dict(k=k, v=k, k8=dk8, v8=dv8, k_scale=dks, v_scale=dvs), **kw})
+    with pytest.raises(_lib.TrnError):      # rows that share memory
+        ops.cache8_append(torch.zeros(1, 2, 1, 64, dtype=torch.float16, device=DEV), k, dk8[:, :1].expand(1, 2, 64, 64), dv8, dks, dvs)
+    ops.cache8_append(k[:, :, :0], k[:, :, :0], dk8, dv8, dks, dvs)
+    ops.cache8_attention(**{**good, "q": q[:, :, :0], "o": o[:, :, :0]})

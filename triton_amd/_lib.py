@@ -20,6 +20,7 @@ EXPORTS = (
     "trn_attn_fwd_noalloc_f16", "trn_attn_fwd_kernel_name", "trn_attn_colmeanstd_f16", "trn_attn_fwd_probs_f16",
     "trn_attn_fwd_stats_half_f16", "trn_attn_fwd_stats_ws_f16", "trn_attn_stats_workspace_bytes",
     "trn_attn_key_scores_f16", "trn_attn_key_scores_workspace_bytes", "trn_attn_qknorm_f16", "trn_attn_qknorm_workspace_bytes",
+    "trn_cache8_append_f16", "trn_cache8_attn_workspace_bytes", "trn_cache8_attn_f16", "trn_cache_evict_workspace_bytes", "trn_cache_evict",
 )
 
 
@@ -46,6 +47,25 @@ class AttnDesc(C.Structure):
         ("noise_stride_b", C.c_int64), ("noise_stride_h", C.c_int64), ("noise_stride_s", C.c_int64),
         ("tau", C.c_float),
     ]
+
+
+class Cache8(C.Structure):
+    """Mirror of `trn_cache8`."""
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+        ("lengths", C.c_void_p), ("counts", C.c_void_p),
+        ("batch", C.c_int32), ("n_kv_heads", C.c_int32), ("capacity", C.c_int32), ("head_dim", C.c_int32), ("block", C.c_int32),
+        ("k_stride_b", C.c_int64), ("k_stride_h", C.c_int64), ("k_stride_s", C.c_int64),
+        ("v_stride_b", C.c_int64), ("v_stride_h", C.c_int64), ("v_stride_s", C.c_int64),
+        ("ks_stride_b", C.c_int64), ("ks_stride_h", C.c_int64), ("vs_stride_b", C.c_int64), ("vs_stride_h", C.c_int64),
+    ]
+
+
+class CacheEvictDesc(C.Structure):
+    """Mirror of `trn_cache_evict_desc`."""
+    _fields_ = [(n, C.c_int32) for n in ("batch", "n_kv_heads", "n_weight_rows", "keys", "head_dim", "code_bytes", "block", "keep", "recent", "weights_half")] + \
+        [(n, C.c_int64 * 3) for n in ("k_stride", "v_stride", "k_out_stride", "v_out_stride")] + \
+        [(n, C.c_int64 * 2) for n in ("k_scale_stride", "v_scale_stride", "k_scale_out_stride", "v_scale_out_stride")]
 
 
 _lib: Optional[C.CDLL] = None
@@ -115,6 +135,16 @@ def load() -> C.CDLL:
     lib.trn_attn_colmeanstd_f16.argtypes = [C.POINTER(AttnDesc), vp, vp, vp, vp, vp, vp]
     lib.trn_prenorm_qkv_f16.restype = C.c_int
     lib.trn_prenorm_qkv_f16.argtypes = [vp] * 8 + [i64] * 15 + [f32, i32, vp]
+    lib.trn_cache8_append_f16.restype = C.c_int
+    lib.trn_cache8_append_f16.argtypes = [C.POINTER(Cache8), vp, vp, i32] + [i64] * 6 + [vp]
+    lib.trn_cache8_attn_workspace_bytes.restype = C.c_int64
+    lib.trn_cache8_attn_workspace_bytes.argtypes = [C.POINTER(Cache8), i32, i32, i32]
+    lib.trn_cache8_attn_f16.restype = C.c_int
+    lib.trn_cache8_attn_f16.argtypes = [C.POINTER(Cache8), vp, vp, i32, i32] + [i64] * 6 + [f32, i32, vp, vp, vp, vp, i64, vp]
+    lib.trn_cache_evict_workspace_bytes.restype = C.c_int64
+    lib.trn_cache_evict_workspace_bytes.argtypes = [C.POINTER(CacheEvictDesc)]
+    lib.trn_cache_evict.restype = C.c_int
+    lib.trn_cache_evict.argtypes = [C.POINTER(CacheEvictDesc)] + [vp] * 14 + [i64, vp]
     lib.trn_calibration_copy.restype = C.c_int
     lib.trn_calibration_copy.argtypes = [vp, vp, i64, vp]
     lib.trn_calibration_mfma.restype = C.c_int

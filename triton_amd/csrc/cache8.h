@@ -1,0 +1,48 @@
+// Shared by the kernels of the 8-bit key/value cache: e4m3 codes [batch, KV heads, capacity, head_dim] and a float32 scale for each
+// head and block of 32, 64 or 128 tokens.
+#pragma once
+#include "common.h"
+
+namespace trn {
+
+// The least scale, and that of a block without a number in it: fp16's smallest number is 2^-24, e4m3's largest 1.75 * 2^8.
+constexpr float kScaleFloor = 0x1p-32f;
+
+// The keys of a sequence (its new tokens among them) and its new tokens, as they stand on the device; nothing outside the cache or the
+// launch is ever addressed by them.
+__device__ __forceinline__ int keys_of(const int32_t* lengths, int b, int capacity) { return lengths ? min(max(lengths[b], 0), capacity) : capacity; }
+__device__ __forceinline__ int tokens_of(const int32_t* counts, int b, int tokens) { return counts ? min(max(counts[b], 0), tokens) : tokens; }
+
+// The smallest power of two by which a finite magnitude comes to no more than 448, at least the floor.
+__device__ __forceinline__ float scale_for(float amax) {
+    const uint32_t u = __float_as_uint(amax);
+    const int e = (int)(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);       // (448 = 1.75 * 2^8)
+    return fmaxf(__uint_as_float((uint32_t)max(e, 1) << 23), kScaleFloor);
+}
+
+// Four codes as four fp16 values: every e4m3 number is one of fp16.
+__device__ __forceinline__ half4_t half_of_codes(uint32_t w) {
+    const auto lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, false), hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, true);
+    return half4_t{(half_t)lo[0], (half_t)lo[1], (half_t)hi[0], (half_t)hi[1]};
+}
+__device__ __forceinline__ half8_t half_of_codes(uint32_t a, uint32_t b) {
+    const half4_t x = half_of_codes(a), y = half_of_codes(b);
+    return half8_t{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+}
+// Four floats as codes, rounded to nearest even; anything past 464, and NaN, becomes NaN.
+__device__ __forceinline__ uint32_t codes_of(float a, float b, float c, float d) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+    return (uint32_t)w;
+}
+// ... of codes that are worth `ratio` times as much on another scale.
+__device__ __forceinline__ uint32_t recoded(uint32_t w, float ratio) {
+    const half4_t h = half_of_codes(w);
+    return codes_of((float)h[0] * ratio, (float)h[1] * ratio, (float)h[2] * ratio, (float)h[3] * ratio);
+}
+
+inline bool block_ok(int block) { return block == 32 || block == 64 || block == 128; }
+// The checks of a cache that every entry point makes; base pointers, and strides of axes with more than one element.
+int cache8_check(const trn_cache8* c);
+
+}  // namespace trn

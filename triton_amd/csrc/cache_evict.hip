@@ -1,0 +1,317 @@
+// Eviction from a key/value cache by accumulated attention weight: of each sequence and KV head the `recent` last keys and those of the
+// largest weight among the others, `keep` in all, gathered to the front in their order.
+//
+// Two launches.  Selection: a workgroup has one head of a sequence.  The weights of its query heads are added up in 64 bits and rounded
+// once to fp32, turned into integers that order as they do, and the smallest one kept is found by digits of 11, 11 and 10 bits, counted in
+// LDS; ties are filled up from the front.  A last pass numbers the kept keys in order.  Move: rows of K and V, 16 bytes a lane.  Into
+// another cache, workgroups share the rows; within the same one, a workgroup has a 64-byte column of all of a head's rows and
+// moves them front to back: a row goes to its own place or one before it, so what a step overwrites has been read by this step or an
+// earlier one, and columns never meet.
+//
+// 8-bit caches: a block of the shortened cache takes the largest of the scales that its rows come with; codes of rows with a smaller
+// one are multiplied by the ratio, which between powers of two only rounds what leaves e4m3's normal numbers.
+#include "cache8.h"
+
+namespace trn {
+
+struct EvictArgs {
+    const void* k; const void* v; void* k_out; void* v_out;
+    const float *ks, *vs; float *ks_out, *vs_out;
+    const void* w; void* w_out;
+    const int32_t* lengths; int32_t *kept, *new_lengths;
+    int B, Hkv, Hw, S, keep, recent, bshift, w_half, in_place[2];
+    int64_t st[2][3], ot[2][3];        // strides of K and V in bytes, given and kept
+    int64_t sst[2][2], sot[2][2];      // ... of their scales
+    uint32_t* order;                   // [B Hkv][S]
+    float* ratio;                      // [2][B Hkv][keep]
+    int32_t* now;                      // [2][B]: keys that stay, and that there were
+    int chunks, cols;                  // move: workgroups of a head's rows and columns
+    Div by_hkv, by_chunks, by_cols;
+};
+
+// Larger numbers first, NaN last of all.
+__device__ __forceinline__ uint32_t order_of(float x) {
+    const uint32_t u = __float_as_uint(x);
+    if (x != x) return 0;
+    return u & 0x80000000u ? ~u : u | 0x80000000u;       // (0xff800000's complement, of -inf, is 0x7fffff: above NaN's)
+}
+
+__global__ __launch_bounds__(1024) void cache_evict_select_kernel(const EvictArgs a) {
+    __shared__ int bins[2048];
+    __shared__ int waves[16], s_digit, s_above, s_base, s_ties;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int bh = blockIdx.x, b = a.by_hkv.of(bh), h = bh - b * a.Hkv;
+    const int n = keys_of(a.lengths, b, a.S), stay = min(n, a.keep);
+    const int late = min(a.recent, stay), early = n - late;              // the last `late` keys stay in any case
+    int want = stay - late;                                              // ... and so many of the first `early`
+    int32_t* kept = a.kept + (int64_t)bh * a.keep;
+    uint32_t* order = a.order + (int64_t)bh * a.S;
+    const int per = a.Hw / a.Hkv;
+
+    uint32_t least = 0; int ties = 0;         // kept: order > least, and the first `ties` of those equal to it
+    if (want < early && want > 0) {
+        for (int j = tid; j < early; j += 1024) {
+            double s = 0.0;
+            const int64_t at = ((int64_t)b * a.Hw + h * per) * a.S + j;
+            for (int g = 0; g < per; ++g)
+                s += a.w_half ? (double)(float)static_cast<const half_t*>(a.w)[at + (int64_t)g * a.S] : (double)static_cast<const float*>(a.w)[at + (int64_t)g * a.S];
+            order[j] = order_of((float)s);
+        }
+        int rest = want;
+        for (int pass = 0; pass < 3; ++pass) {
+            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+            for (int i = tid; i < 2048; i += 1024) bins[i] = 0;
+            __syncthreads();
+            for (int j = tid; j < early; j += 1024) {
+                const uint32_t u = order[j];
+                if (pass == 0 || (u >> (shift + bits)) == (least >> (shift + bits))) atomicAdd(&bins[(u >> shift) & ((1 << bits) - 1)], 1);
+            }
+            __syncthreads();
+            // from the top: thread i has the bins 2047 - 2 i and one below
+            const int hi = bins[2047 - 2 * tid], lo = bins[2046 - 2 * tid];
+            int sum = hi + lo;
+#pragma unroll
+            for (int m = 1; m < 64; m <<= 1) { const int x = __shfl_up(sum, m, 64); if (lane >= m) sum += x; }
+            if (lane == 63) waves[wave] = sum;
+            __syncthreads();
+            int before = sum - hi - lo;
+            for (int i = 0; i < wave; ++i) before += waves[i];
+            if (before < rest && before + hi + lo >= rest) {
+                const bool first = before + hi >= rest;
+                s_digit = first ? 2047 - 2 * tid : 2046 - 2 * tid;
+                s_above = first ? before : before + hi;
+            }
+            __syncthreads();
+            least |= (uint32_t)s_digit << shift;
+            rest -= s_above;
+            __syncthreads();
+        }
+        ties = rest;
+    }
+    const bool all = want >= early;
+    // in order, 1024 keys at a time
+    if (tid == 0) { s_base = 0; s_ties = 0; }
+    __syncthreads();
+    if (want > 0) {
+        for (int j0 = 0; j0 < early; j0 += 1024) {
+            const int j = j0 + tid;
+            const uint32_t u = j < early && !all ? order[j] : 0;
+            const bool tie = j < early && !all && u == least;
+            const uint64_t tb = __ballot(tie);
+            if (lane == 0) waves[wave] = __popcll(tb);
+            __syncthreads();
+            int t_before = s_ties + __popcll(tb & ((1ull << lane) - 1)), t_all = 0;
+            for (int i = 0; i < 16; ++i) { if (i < wave) t_before += waves[i]; t_all += waves[i]; }
+            const bool take = j < early && (all || u > least || (tie && t_before < ties));
+            const uint64_t kb = __ballot(take);
+            __syncthreads();
+            if (lane == 0) waves[wave] = __popcll(kb);
+            __syncthreads();
+            int at = s_base + __popcll(kb & ((1ull << lane) - 1)), k_all = 0;
+            for (int i = 0; i < 16; ++i) { if (i < wave) at += waves[i]; k_all += waves[i]; }
+            if (take) kept[at] = j;
+            __syncthreads();
+            if (tid == 0) { s_base += k_all; s_ties += t_all; }
+            __syncthreads();
+        }
+    }
+    for (int i = tid; i < late; i += 1024) kept[want + i] = early + i;
+    for (int i = stay + tid; i < a.keep; i += 1024) kept[i] = -1;
+    if (h == 0 && tid == 0) { a.now[b] = stay; a.now[a.B + b] = n; }
+    if (!a.ratio) return;
+    // 8 bits: new scales, and what each kept row's codes are to be multiplied by
+    __syncthreads();
+    for (int kv = 0; kv < 2; ++kv) {
+        const float* s = (kv ? a.vs : a.ks) + b * a.sst[kv][0] + h * a.sst[kv][1];
+        float* so = (kv ? a.vs_out : a.ks_out) + b * a.sot[kv][0] + h * a.sot[kv][1];
+        float* ratio = a.ratio + ((int64_t)kv * a.B * a.Hkv + bh) * a.keep;
+        for (int i = tid; i < stay; i += 1024) ratio[i] = s[kept[i] >> a.bshift];
+        __syncthreads();      // (the scales may be written where they were read)
+        const int block = 1 << a.bshift;
+        for (int i0 = wave * block; i0 < stay; i0 += 16 * block) {
+            float top = 0.f;
+            for (int i = i0 + lane; i < min(i0 + block, stay); i += 64) top = fmaxf(top, ratio[i]);
+#pragma unroll
+            for (int m = 32; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
+            for (int i = i0 + lane; i < min(i0 + block, stay); i += 64) ratio[i] = top > 0.f ? ratio[i] / top : 1.f;
+            if (lane == 0) so[i0 >> a.bshift] = top;
+        }
+        __syncthreads();
+    }
+}
+
+// blockIdx.y: 0 K, 1 V; blockIdx.x: (head of a sequence, chunk of rows, column).  W: 16-byte pieces of a row; in place a workgroup has 4 of
+// them, as a column, and all rows.
+template <bool BITS8>
+__global__ __launch_bounds__(256) void cache_evict_move_kernel(const EvictArgs a, int row_pieces, int piece_shift, int rows_per_chunk) {
+    const int kv = blockIdx.y;
+    const int u = a.by_cols.of(blockIdx.x), col = blockIdx.x - u * a.cols;
+    const int bh = a.by_chunks.of(u), chunk = u - bh * a.chunks;
+    const int b = a.by_hkv.of(bh), h = bh - b * a.Hkv;
+    const int stay = a.now[b];
+    const int32_t* kept = a.kept + (int64_t)bh * a.keep;
+    const char* src = (const char*)(kv ? a.v : a.k) + b * a.st[kv][0] + h * a.st[kv][1];
+    char* dst = (char*)(kv ? a.v_out : a.k_out) + b * a.ot[kv][0] + h * a.ot[kv][1];
+    const float* ratio = BITS8 ? a.ratio + ((int64_t)kv * a.B * a.Hkv + bh) * a.keep : nullptr;
+    const int sub = threadIdx.x & (row_pieces - 1), r0 = threadIdx.x >> piece_shift, step = 256 >> piece_shift;
+    const int off = (col * row_pieces + sub) * 16;
+    const int from = chunk * rows_per_chunk, to = min(stay, from + rows_per_chunk);
+    constexpr int NB = 4;      // rows of a lane on their way at once
+    for (int i0 = from; i0 < to; i0 += NB * step) {
+        uint4_t x[NB]; float f[NB];
+#pragma unroll
+        for (int e = 0; e < NB; ++e) {
+            const int i = i0 + e * step + r0;
+            if (i < to) {
+                x[e] = *reinterpret_cast<const uint4_t*>(src + (int64_t)kept[i] * a.st[kv][2] + off);
+                if (BITS8) f[e] = ratio[i];
+            }
+        }
+        if (a.in_place[kv]) __syncthreads();      // (waits for the loads as well: what this step overwrites has been read)
+#pragma unroll
+        for (int e = 0; e < NB; ++e) {
+            const int i = i0 + e * step + r0;
+            if (i < to) {
+                if (BITS8 && f[e] != 1.f) x[e] = uint4_t{recoded(x[e].x, f[e]), recoded(x[e].y, f[e]), recoded(x[e].z, f[e]), recoded(x[e].w, f[e])};
+                *reinterpret_cast<uint4_t*>(dst + (int64_t)i * a.ot[kv][2] + off) = x[e];
+            }
+        }
+    }
+}
+
+// The weights of the kept keys, a workgroup for each row of them; and the new lengths.
+__global__ __launch_bounds__(1024) void cache_evict_weights_kernel(const EvictArgs a) {
+    const int row = blockIdx.x, b = row / a.Hw, hw = row - b * a.Hw;
+    const int stay = a.now[b];
+    if (hw == 0 && threadIdx.x == 0 && a.new_lengths) a.new_lengths[b] = stay;
+    if (!a.w_out) return;
+    const int32_t* kept = a.kept + ((int64_t)b * a.Hkv + hw / (a.Hw / a.Hkv)) * a.keep;
+    const int64_t from = (int64_t)row * a.S;
+    // (w_out may be w, whose rows are S apart, or a tensor of its own with rows of `keep`)
+    const int64_t to = a.w_out == a.w ? from : (int64_t)row * a.keep;
+    for (int i0 = 0; i0 < stay; i0 += 1024) {
+        const int i = i0 + threadIdx.x;
+        float x = 0.f;
+        if (i < stay) x = a.w_half ? (float)static_cast<const half_t*>(a.w)[from + kept[i]] : static_cast<const float*>(a.w)[from + kept[i]];
+        __syncthreads();
+        if (i < stay) {
+            if (a.w_half) static_cast<half_t*>(a.w_out)[to + i] = (half_t)x;
+            else static_cast<float*>(a.w_out)[to + i] = x;
+        }
+    }
+    // (the places that new keys will take have gathered nothing)
+    if (a.w_out == a.w) {
+        const int n = a.now[a.B + b];
+        for (int i = stay + threadIdx.x; i < n; i += 1024) {
+            if (a.w_half) static_cast<half_t*>(a.w_out)[to + i] = (half_t)0.f;
+            else static_cast<float*>(a.w_out)[to + i] = 0.f;
+        }
+    }
+}
+
+struct EvictSizes { int64_t order, ratio, now, bytes; };
+static EvictSizes evict_sizes(const trn_cache_evict_desc* e) {
+    auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
+    EvictSizes s;
+    const int64_t heads = (int64_t)e->batch * e->n_kv_heads;
+    s.order = 0;
+    s.ratio = up(heads * e->keys * 4);
+    s.now = s.ratio + (e->code_bytes == 1 ? up(2 * heads * e->keep * 4) : 0);
+    s.bytes = s.now + up((int64_t)e->batch * 8);
+    return s;
+}
+
+// The bytes that a tensor [batch, heads, rows, width] spans from its base (strides in bytes, not negative).
+static int64_t span(const int64_t* st, int64_t b, int64_t h, int64_t rows, int64_t width) { return (b - 1) * st[0] + (h - 1) * st[1] + (rows - 1) * st[2] + width; }
+static bool apart(const void* x, int64_t nx, const void* y, int64_t ny) {
+    const uintptr_t p = (uintptr_t)x, q = (uintptr_t)y;
+    return p + (uint64_t)nx <= q || q + (uint64_t)ny <= p;
+}
+
+}  // namespace trn
+
+extern "C" int64_t trn_cache_evict_workspace_bytes(const trn_cache_evict_desc* e) {
+    if (!e || e->batch <= 0 || e->n_kv_heads <= 0 || e->keys <= 0 || e->keep <= 0) return 0;
+    return trn::evict_sizes(e).bytes;
+}
+
+extern "C" int trn_cache_evict(const trn_cache_evict_desc* e, const void* k, const void* v, void* k_out, void* v_out, const float* k_scale,
+                               const float* v_scale, float* k_scale_out, float* v_scale_out, const void* weights, void* weights_out,
+                               const int32_t* lengths, int32_t* kept, int32_t* new_lengths, void* workspace, int64_t workspace_bytes,
+                               void* stream) {
+    using namespace trn;
+    if (!e) return TRN_E_NULL;
+    if (e->batch < 0 || e->n_kv_heads <= 0 || e->n_weight_rows <= 0 || e->n_weight_rows % e->n_kv_heads || e->keys <= 0 || e->keep <= 0 || e->recent < 0 || e->recent > e->keep) return TRN_E_SHAPE;
+    if (e->code_bytes != 1 && e->code_bytes != 2) return TRN_E_UNSUPPORTED;
+    if (e->head_dim != 64 && e->head_dim != 128) return TRN_E_UNSUPPORTED;
+    const bool bits8 = e->code_bytes == 1;
+    if (bits8 && !block_ok(e->block)) return TRN_E_UNSUPPORTED;
+    if (e->keys > (1 << 26) || e->keep > (1 << 26)) return TRN_E_UNSUPPORTED;
+    if (e->batch == 0) return TRN_OK;
+    if (!k || !v || !k_out || !v_out || !weights || !kept || !workspace) return TRN_E_NULL;
+    if (bits8 && (!k_scale || !v_scale || !k_scale_out || !v_scale_out)) return TRN_E_NULL;
+    for (const void* p : {k, v, (const void*)k_out, (const void*)v_out}) if (!aligned16(p)) return TRN_E_ALIGN;
+    if ((uintptr_t)workspace & 255) return TRN_E_ALIGN;
+    const EvictSizes sz = evict_sizes(e);
+    if (workspace_bytes < sz.bytes) return TRN_E_SCRATCH;
+    EvictArgs a;
+    a.k = k; a.v = v; a.k_out = k_out; a.v_out = v_out; a.ks = k_scale; a.vs = v_scale; a.ks_out = k_scale_out; a.vs_out = v_scale_out;
+    a.w = weights; a.w_out = weights_out; a.lengths = lengths; a.kept = kept; a.new_lengths = new_lengths;
+    a.B = e->batch; a.Hkv = e->n_kv_heads; a.Hw = e->n_weight_rows; a.S = e->keys; a.keep = e->keep; a.recent = e->recent;
+    a.w_half = e->weights_half != 0;
+    a.bshift = e->block == 32 ? 5 : e->block == 64 ? 6 : 7;
+    const int width = e->head_dim * e->code_bytes;
+    const int64_t* in[2] = {e->k_stride, e->v_stride};
+    const int64_t* out[2] = {e->k_out_stride, e->v_out_stride};
+    const int rows_out = e->keep < e->keys ? e->keep : e->keys;
+    for (int i = 0; i < 2; ++i) {
+        for (int j = 0; j < 3; ++j) {
+            a.st[i][j] = in[i][j] * e->code_bytes; a.ot[i][j] = out[i][j] * e->code_bytes;
+            if (in[i][j] < 0 || out[i][j] < 0) return TRN_E_STRIDE;
+            if ((a.st[i][j] | a.ot[i][j]) & 15) return TRN_E_ALIGN;
+        }
+        if ((in[i][2] < e->head_dim && e->keys > 1) || (out[i][2] < e->head_dim && rows_out > 1)) return TRN_E_STRIDE;
+        if ((e->batch > 1 && !out[i][0]) || (e->n_kv_heads > 1 && !out[i][1])) return TRN_E_STRIDE;
+        const void* x = i ? v : k;
+        const void* y = i ? v_out : k_out;
+        const int64_t nx = span(a.st[i], e->batch, e->n_kv_heads, e->keys, width), ny = span(a.ot[i], e->batch, e->n_kv_heads, rows_out, width);
+        a.in_place[i] = x == y;
+        if (x == y) {       // the same cache, shortened
+            for (int j = 0; j < 3; ++j)
+                if (a.st[i][j] != a.ot[i][j]) return TRN_E_STRIDE;
+        } else if (!apart(x, nx, y, ny)) return TRN_E_UNSUPPORTED;
+        const void* other = i ? k : v;
+        if (!apart(other, span(a.st[1 - i], e->batch, e->n_kv_heads, e->keys, width), y, ny)) return TRN_E_UNSUPPORTED;
+    }
+    if (!apart(k_out, span(a.ot[0], e->batch, e->n_kv_heads, rows_out, width), v_out, span(a.ot[1], e->batch, e->n_kv_heads, rows_out, width))) return TRN_E_UNSUPPORTED;
+    if (weights_out && weights_out != weights) {
+        const int64_t rows = (int64_t)e->batch * e->n_weight_rows, size = e->weights_half ? 2 : 4;
+        if (!apart(weights, rows * e->keys * size, weights_out, rows * e->keep * size)) return TRN_E_UNSUPPORTED;
+    }
+    a.sst[0][0] = e->k_scale_stride[0]; a.sst[0][1] = e->k_scale_stride[1]; a.sst[1][0] = e->v_scale_stride[0]; a.sst[1][1] = e->v_scale_stride[1];
+    a.sot[0][0] = e->k_scale_out_stride[0]; a.sot[0][1] = e->k_scale_out_stride[1]; a.sot[1][0] = e->v_scale_out_stride[0]; a.sot[1][1] = e->v_scale_out_stride[1];
+    a.order = (uint32_t*)workspace;
+    a.ratio = bits8 ? (float*)((char*)workspace + sz.ratio) : nullptr;
+    a.now = (int32_t*)((char*)workspace + sz.now);
+    const int64_t heads = (int64_t)e->batch * e->n_kv_heads;
+    if (heads > 0x7fffffff || (int64_t)e->batch * e->n_weight_rows > 0x7fffffff) return TRN_E_SHAPE;
+    a.by_hkv = Div(e->n_kv_heads);
+    const hipStream_t s = (hipStream_t)stream;
+    hipLaunchKernelGGL(cache_evict_select_kernel, dim3((unsigned)heads), dim3(1024), 0, s, a);
+    // rows shared out, or in columns of 64 bytes
+    const bool columns = a.in_place[0] || a.in_place[1];
+    const int pieces = width / 16, row_pieces = columns ? 4 : pieces;
+    int shift = 0;
+    while ((1 << shift) < row_pieces) ++shift;
+    const int rows_per_chunk = columns ? rows_out : 4 * (256 / row_pieces);
+    a.cols = pieces / row_pieces;
+    a.chunks = (rows_out + rows_per_chunk - 1) / rows_per_chunk;
+    if (heads * a.chunks * a.cols > 0x7fffffffLL) return TRN_E_SHAPE;
+    a.by_cols = Div(a.cols); a.by_chunks = Div(a.chunks);
+    const dim3 grid((unsigned)(heads * a.chunks * a.cols), 2);
+    if (bits8) hipLaunchKernelGGL((cache_evict_move_kernel<true>), grid, dim3(256), 0, s, a, row_pieces, shift, rows_per_chunk);
+    else hipLaunchKernelGGL((cache_evict_move_kernel<false>), grid, dim3(256), 0, s, a, row_pieces, shift, rows_per_chunk);
+    if (weights_out || new_lengths)
+        hipLaunchKernelGGL(cache_evict_weights_kernel, dim3((unsigned)(e->batch * e->n_weight_rows)), dim3(1024), 0, s, a);
+    return hipGetLastError() == hipSuccess ? TRN_OK : TRN_E_LAUNCH;
+}

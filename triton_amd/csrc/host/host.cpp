@@ -14,6 +14,7 @@
 #include <Python.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/core/Tensor.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <algorithm>
 #include <cmath>
@@ -167,6 +168,7 @@ at::Tensor workspace(Workspaces* w, const char* name, at::IntArrayRef shape, c10
     return r;
 }
 Workspaces* ws_arg(PyObject* o);
+PyTypeObject* workspaces_type();
 // Size at which a workspace of so many bytes is kept: the next power of two from 1 MB on, so that lengths share one (by exact
 // size each length met would keep its own; all of them together are at most twice the largest).
 int64_t kept_bytes(int64_t need) {
@@ -498,6 +500,192 @@ bool f_gmlp_forward(Args a, Py_ssize_t n) {               // workspaces, silu, O
     return true;
 }
 
+// ---------------------------------------------------------------------------------------------- 8-bit caches, eviction
+// Launches go to the device of the tensors, which need not be the current one.
+struct OnDevice {
+    int was;
+    explicit OnDevice(int dev) : was((int)c10::hip::current_device()) { if (dev != was) c10::hip::set_device((c10::DeviceIndex)dev); else was = -1; }
+    ~OnDevice() { if (was >= 0) c10::hip::set_device((c10::DeviceIndex)was); }
+};
+void on(const View& t, const char* n, const View& first) { NEED(t.cuda && t.dev == first.dev, "%s: expected a tensor on the device of the others", n); }
+void dims4(const View& t, const char* n, int64_t b, int64_t h, int64_t s, int64_t d) {
+    NEED(t.dim == 4 && t.s[0] == b && t.s[1] == h && t.s[2] == s && t.s[3] == d, "%s %s: expected (%lld, %lld, %lld, %lld)", n, t.shape().c_str(),
+         (long long)b, (long long)h, (long long)s, (long long)d);
+}
+void unit4(const View& t, const char* n) { NEED(t.s[t.dim - 1] == 1 || t.unit(), "%s: innermost stride must be 1", n); }
+const int32_t* batch_ints(const OptView& t, const char* n, int64_t b, const View& first) {
+    if (!t.given) return nullptr;
+    on(t.v, n, first);
+    NEED(t.v.dt == c10::ScalarType::Int && t.v.dim == 1 && t.v.s[0] == b && t.v.contiguous(), "%s: expected contiguous int32 (%lld,)", n, (long long)b);
+    return reinterpret_cast<const int32_t*>(t.v.p);
+}
+bool codes(const View& t) { return t.dt == c10::ScalarType::Byte || t.dt == c10::ScalarType::Float8_e4m3fn; }
+void scales_of(const View& t, const char* n, int64_t b, int64_t h, int64_t blocks, bool more, const View& first) {
+    on(t, n, first);
+    NEED(t.f32(), "%s: expected float32, got %s", n, c10::toString(t.dt));
+    NEED(t.dim == 3 && t.s[0] == b && t.s[1] == h && (more ? t.s[2] >= blocks : t.s[2] == blocks), "%s %s: expected (%lld, %lld, %lld)", n, t.shape().c_str(),
+         (long long)b, (long long)h, (long long)blocks);
+    unit4(t, n);
+}
+int whole(PyObject* o, const char* n) {
+    const long long x = PyLong_AsLongLong(o);
+    if (x == -1 && PyErr_Occurred()) throw PyErrSet{};
+    NEED(x >= INT32_MIN && x <= INT32_MAX, "%s: out of range", n);
+    return (int)x;
+}
+
+trn_cache8 cache8_of(const View& k8, const View& ks, const View& v8, const View& vs, const OptView& lengths, const OptView& counts, int block) {
+    NEED(k8.cuda, "k8: expected a GPU tensor");
+    NEED(block == 32 || block == 64 || block == 128, "block: expected 32, 64 or 128, got %d", block);
+    NEED(k8.dim == 4, "k8: expected [batch, heads, capacity, head_dim], got %s", k8.shape().c_str());
+    NEED(codes(k8) && codes(v8), "k8, v8: expected float8_e4m3fn or uint8 tensors");
+    const int64_t B = k8.s[0], H = k8.s[1], S = k8.s[2], D = k8.s[3], blocks = (S + block - 1) / block;
+    NEED(B <= INT32_MAX && H <= INT32_MAX && S <= INT32_MAX, "k8 %s: too large", k8.shape().c_str());
+    dims4(v8, "v8", B, H, S, D);
+    on(v8, "v8", k8);
+    unit4(k8, "k8"); unit4(v8, "v8");
+    scales_of(ks, "k_scale", B, H, blocks, false, k8); scales_of(vs, "v_scale", B, H, blocks, false, k8);
+    trn_cache8 c{};
+    c.k = k8.p; c.v = v8.p; c.k_scale = (float*)ks.p; c.v_scale = (float*)vs.p;
+    c.lengths = batch_ints(lengths, "lengths", B, k8); c.counts = batch_ints(counts, "counts", B, k8);
+    c.batch = (int32_t)B; c.n_kv_heads = (int32_t)H; c.capacity = (int32_t)S; c.head_dim = (int32_t)D; c.block = block;
+    c.k_stride_b = k8.st[0]; c.k_stride_h = k8.st[1]; c.k_stride_s = k8.st[2];
+    c.v_stride_b = v8.st[0]; c.v_stride_h = v8.st[1]; c.v_stride_s = v8.st[2];
+    c.ks_stride_b = ks.st[0]; c.ks_stride_h = ks.st[1]; c.vs_stride_b = vs.st[0]; c.vs_stride_h = vs.st[1];
+    return c;
+}
+
+bool f_cache8_append(Args a, Py_ssize_t n) {              // block, K, K8, K_scale, V, V8, V_scale, counts | None, lengths | None
+    count(n, 9, "cache8_append");
+    const View k = arg(a[1], "k"), k8 = arg(a[2], "k8"), v = arg(a[4], "v"), v8 = arg(a[5], "v8");
+    const trn_cache8 c = cache8_of(k8, arg(a[3], "k_scale"), v8, arg(a[6], "v_scale"), opt(a[8], "lengths"), opt(a[7], "counts"), whole(a[0], "block"));
+    dev_half(k, "k"); dev_half(v, "v");
+    on(k, "k", k8); on(v, "v", k8);
+    NEED(k.dim == 4 && k.s[2] <= INT32_MAX, "k %s: expected [batch, heads, tokens, head_dim]", k.shape().c_str());
+    dims4(k, "k", k8.s[0], k8.s[1], k.s[2], k8.s[3]);
+    dims4(v, "v", k8.s[0], k8.s[1], k.s[2], k8.s[3]);
+    const OnDevice here(k8.dev);
+    CALL(trn_cache8_append_f16, &c, k.p, v.p, (int32_t)k.s[2], k.st[0], k.st[1], k.st[2], v.st[0], v.st[1], v.st[2], stream_of(k8));
+    return true;
+}
+
+// The attention, with a workspace of the module's or the caller's.
+bool f_cache8_attention(Args a, Py_ssize_t n) {
+    // workspaces | workspace | None, scale | None, causal, block, K8, K_scale, O, Q, V8, V_scale, counts | None, lengths | None, lse | None,
+    // weights | None, weights_out | None
+    count(n, 15, "cache8_attention");
+    const View k8 = arg(a[4], "k8"), o = arg(a[6], "o"), q = arg(a[7], "q"), v8 = arg(a[8], "v8");
+    const trn_cache8 c = cache8_of(k8, arg(a[5], "k_scale"), v8, arg(a[9], "v_scale"), opt(a[11], "lengths"), opt(a[10], "counts"), whole(a[3], "block"));
+    dev_half(q, "q"); dev_half(o, "o");
+    on(q, "q", k8); on(o, "o", k8);
+    NEED(q.dim == 4 && q.s[0] == k8.s[0] && q.s[3] == k8.s[3] && q.s[1] > 0 && k8.s[1] > 0 && q.s[1] % k8.s[1] == 0 && q.s[1] <= INT32_MAX && q.s[2] <= INT32_MAX,
+         "q %s does not match k8 %s", q.shape().c_str(), k8.shape().c_str());
+    NEED(same_shape(o, q), "o %s must equal q %s", o.shape().c_str(), q.shape().c_str());
+    const OptView lse = opt(a[12], "lse"), w = opt(a[13], "weights"), wo = opt(a[14], "weights_out");
+    if (lse.given) {
+        dev_float(lse.v, "lse"); on(lse.v, "lse", k8);
+        NEED(lse.v.dim == 3 && lse.v.s[0] == q.s[0] && lse.v.s[1] == q.s[1] && lse.v.s[2] == q.s[2] && lse.v.contiguous(), "lse: expected contiguous float32 (%lld, %lld, %lld)",
+             (long long)q.s[0], (long long)q.s[1], (long long)q.s[2]);
+    }
+    NEED(!w.given || wo.given, "weights given without weights_out");
+    for (const OptView* t : {&w, &wo}) {
+        if (!t->given) continue;
+        const char* nm = t == &w ? "weights" : "weights_out";
+        on(t->v, nm, k8);
+        NEED(t->v.f32() && t->v.dim == 3 && t->v.s[0] == k8.s[0] && t->v.s[1] == k8.s[1] && t->v.s[2] == k8.s[2] && t->v.contiguous(),
+             "%s: expected contiguous float32 (%lld, %lld, %lld)", nm, (long long)k8.s[0], (long long)k8.s[1], (long long)k8.s[2]);
+    }
+    at::Tensor kept;
+    void* ws = nullptr;
+    int64_t bytes = 0;
+    if (Py_TYPE(a[0]) == workspaces_type()) {
+        if (const int64_t need = trn_cache8_attn_workspace_bytes(&c, (int32_t)q.s[1], (int32_t)q.s[2], wo.given)) {
+            kept = workspace(ws_arg(a[0]), "attn8", {kept_bytes(need)}, c10::ScalarType::Byte, k8.dev);
+            ws = kept.data_ptr(); bytes = kept_bytes(need);
+        }
+    } else if (const OptView given = opt(a[0], "workspace"); given.given) {
+        on(given.v, "workspace", k8);
+        NEED(given.v.contiguous() && given.v.dt == c10::ScalarType::Byte, "workspace: expected a contiguous uint8 GPU tensor");
+        ws = given.v.p; bytes = given.v.numel();
+    }
+    const OnDevice here(k8.dev);
+    CALL(trn_cache8_attn_f16, &c, q.p, o.p, (int32_t)q.s[1], (int32_t)q.s[2], q.st[0], q.st[1], q.st[2], o.st[0], o.st[1], o.st[2],
+         (float)scale_of(a[1], q.s[3]), flag(a[2]) ? 1 : 0, (float*)lse.p(), (const float*)w.p(), (float*)wo.p(), ws, bytes, stream_of(k8));
+    return true;
+}
+
+bool f_cache_evict(Args a, Py_ssize_t n) {
+    // workspaces | workspace, keep, recent, block, K, K_out, K_scale | None, K_scale_out | None, V, V_out, V_scale | None, V_scale_out | None,
+    // kept, lengths | None, new_lengths | None, weights, weights_out | None
+    count(n, 17, "cache_evict");
+    const View k = arg(a[4], "k"), ko = arg(a[5], "k_out"), v = arg(a[8], "v"), vo = arg(a[9], "v_out"), kept = arg(a[12], "kept"), w = arg(a[15], "weights");
+    const OptView ks = opt(a[6], "k_scale"), kso = opt(a[7], "k_scale_out"), vs = opt(a[10], "v_scale"), vso = opt(a[11], "v_scale_out"),
+                  lengths = opt(a[13], "lengths"), fresh = opt(a[14], "new_lengths"), wo = opt(a[16], "weights_out");
+    trn_cache_evict_desc e{};
+    NEED(k.cuda && k.dim == 4, "k: expected a GPU tensor [batch, heads, keys, head_dim], got %s", k.shape().c_str());
+    const bool bits8 = codes(k);
+    NEED(bits8 || k.half(), "k: expected float16, float8_e4m3fn or uint8, got %s", c10::toString(k.dt));
+    const int64_t B = k.s[0], H = k.s[1], S = k.s[2], D = k.s[3];
+    NEED(B <= INT32_MAX && H <= INT32_MAX && S <= INT32_MAX, "k %s: too large", k.shape().c_str());
+    e.keep = whole(a[1], "keep"); e.recent = whole(a[2], "recent"); e.block = whole(a[3], "block");
+    NEED(e.keep > 0 && e.recent >= 0 && e.recent <= e.keep, "keep %d, recent %d: expected 0 <= recent <= keep, keep > 0", e.keep, e.recent);
+    const int64_t rows = std::min<int64_t>(e.keep, S);
+    dims4(v, "v", B, H, S, D);
+    for (const View* t : {&v, &ko, &vo}) {
+        const char* nm = t == &v ? "v" : t == &ko ? "k_out" : "v_out";
+        on(*t, nm, k);
+        NEED(bits8 ? codes(*t) : t->half(), "%s: expected the type of k", nm);
+        unit4(*t, nm);
+        NEED(t->dim == 4 && t->s[0] == B && t->s[1] == H && t->s[2] >= rows && t->s[3] == D, "%s %s: expected (%lld, %lld, %lld or more, %lld)", nm, t->shape().c_str(),
+             (long long)B, (long long)H, (long long)rows, (long long)D);
+    }
+    unit4(k, "k");
+    if (bits8) {
+        NEED(e.block == 32 || e.block == 64 || e.block == 128, "block: expected 32, 64 or 128, got %d", e.block);
+        NEED(ks.given && kso.given && vs.given && vso.given, "8-bit caches need k_scale, v_scale, k_scale_out and v_scale_out");
+        scales_of(ks.v, "k_scale", B, H, (S + e.block - 1) / e.block, false, k); scales_of(vs.v, "v_scale", B, H, (S + e.block - 1) / e.block, false, k);
+        scales_of(kso.v, "k_scale_out", B, H, (rows + e.block - 1) / e.block, true, k); scales_of(vso.v, "v_scale_out", B, H, (rows + e.block - 1) / e.block, true, k);
+        for (int i = 0; i < 2; ++i) {
+            e.k_scale_stride[i] = ks.v.st[i]; e.v_scale_stride[i] = vs.v.st[i];
+            e.k_scale_out_stride[i] = kso.v.st[i]; e.v_scale_out_stride[i] = vso.v.st[i];
+        }
+    }
+    on(w, "weights", k);
+    NEED((w.f32() || w.half()) && w.dim == 3 && w.s[0] == B && H > 0 && w.s[1] > 0 && w.s[1] % H == 0 && w.s[2] == S && w.contiguous(),
+         "weights %s: expected contiguous float32 or float16 (%lld, a multiple of %lld, %lld)", w.shape().c_str(), (long long)B, (long long)H, (long long)S);
+    if (wo.given) {
+        on(wo.v, "weights_out", k);
+        NEED(wo.v.dt == w.dt && wo.v.dim == 3 && wo.v.s[0] == B && wo.v.s[1] == w.s[1] && (wo.v.p == w.p ? wo.v.s[2] == S : wo.v.s[2] == e.keep) && wo.v.contiguous(),
+             "weights_out %s: expected weights itself, or a contiguous tensor of its type (%lld, %lld, %d)", wo.v.shape().c_str(), (long long)B, (long long)w.s[1], e.keep);
+    }
+    on(kept, "kept", k);
+    NEED(kept.dt == c10::ScalarType::Int && kept.dim == 3 && kept.s[0] == B && kept.s[1] == H && kept.s[2] == e.keep && kept.contiguous(),
+         "kept %s: expected contiguous int32 (%lld, %lld, %d)", kept.shape().c_str(), (long long)B, (long long)H, e.keep);
+    const int32_t* const len = batch_ints(lengths, "lengths", B, k);
+    int32_t* const nlen = const_cast<int32_t*>(batch_ints(fresh, "new_lengths", B, k));
+    e.batch = (int32_t)B; e.n_kv_heads = (int32_t)H; e.n_weight_rows = (int32_t)w.s[1]; e.keys = (int32_t)S; e.head_dim = (int32_t)D;
+    e.code_bytes = bits8 ? 1 : 2; e.weights_half = w.half();
+    for (int i = 0; i < 3; ++i) { e.k_stride[i] = k.st[i]; e.v_stride[i] = v.st[i]; e.k_out_stride[i] = ko.st[i]; e.v_out_stride[i] = vo.st[i]; }
+    at::Tensor hold;
+    void* ws = nullptr;
+    int64_t bytes = 0;
+    if (Py_TYPE(a[0]) == workspaces_type()) {
+        if (const int64_t need = trn_cache_evict_workspace_bytes(&e)) {
+            hold = workspace(ws_arg(a[0]), "evict", {kept_bytes(need)}, c10::ScalarType::Byte, k.dev);
+            ws = hold.data_ptr(); bytes = kept_bytes(need);
+        }
+    } else {
+        const View given = arg(a[0], "workspace");
+        on(given, "workspace", k);
+        NEED(given.contiguous() && given.dt == c10::ScalarType::Byte, "workspace: expected a contiguous uint8 GPU tensor");
+        ws = given.p; bytes = given.numel();
+    }
+    const OnDevice here(k.dev);
+    CALL(trn_cache_evict, &e, k.p, v.p, ko.p, vo.p, (const float*)ks.p(), (const float*)vs.p(), (float*)kso.p(), (float*)vso.p(), w.p, wo.p(), len,
+         (int32_t*)kept.p, nlen, ws, bytes, stream_of(k));
+    return true;
+}
+
 // ---------------------------------------------------------------------------------------------- Python glue
 PyObject* raise_trn(const char* fn, int status) {
     if (!g_trn_error) { PyErr_Format(PyExc_RuntimeError, "%s failed: %s (%d)", fn, trn_status_name(status), status); return nullptr; }
@@ -548,6 +736,7 @@ Py_ssize_t ws_len(PyObject* o) { return (Py_ssize_t)reinterpret_cast<Workspaces*
 PyMethodDef ws_methods[] = {{"clear", ws_clear, METH_NOARGS, "forget every tensor"}, {nullptr, nullptr, 0, nullptr}};
 PySequenceMethods ws_seq = {ws_len};
 PyTypeObject ws_type = {PyVarObject_HEAD_INIT(nullptr, 0)};
+PyTypeObject* workspaces_type() { return &ws_type; }
 Workspaces* ws_arg(PyObject* o) {
     if (Py_TYPE(o) != &ws_type) { PyErr_SetString(PyExc_TypeError, "expected Workspaces"); throw PyErrSet{}; }
     return reinterpret_cast<Workspaces*>(o);
@@ -564,6 +753,7 @@ PyObject* set_error_class(PyObject*, PyObject* cls) {
 #define OPERATOR(name) {#name, (PyCFunction)(void (*)(void))entry<f_##name, true>, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {OPERATOR(rmsnorm), OPERATOR(attention), OPERATOR(prenorm_qkv), FN(rmsnorm_forward), FN(attention_forward),
                          FN(qknorm_forward), FN(key_scores_forward), FN(prenorm_forward), FN(decode_forward), FN(lora_forward), FN(gmlp_forward),
+                         OPERATOR(cache8_append), OPERATOR(cache8_attention), OPERATOR(cache_evict),
                          {"set_error_class", set_error_class, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "host side of the modules' forward", -1, methods};
 

@@ -541,6 +541,71 @@ class GatedMLP(FusedModule):
         ops.gate(O, c2, O, self.gate)
 
 
+# ============================================================================ 8-bit caches, eviction
+class Cache8Append(FusedModule):
+    """New keys and values into an 8-bit cache (`ops.cache8_append`): K, V [B,Hkv,M,D] fp16; K8, V8 [B,Hkv,S,D] e4m3 codes; K_scale, V_scale float32
+    [B,Hkv,ceil(S/block)]; lengths, counts int32 [B] or None.  One launch."""
+    TENSOR_PARAMS = ["K", "K8", "K_scale", "V", "V8", "V_scale", "counts", "lengths"]
+
+    def __init__(self, block: int = 64):
+        super().__init__()
+        self.block = block
+
+    def _native(self, host, ws, K, K8, K_scale, V, V8, V_scale, counts, lengths):
+        return host.cache8_append(self.block, K, K8, K_scale, V, V8, V_scale, counts, lengths)
+
+
+class Cache8Attention(FusedModule):
+    """Attention over an 8-bit cache (`ops.cache8_attention`): Q, O [B,Hq,M,D] fp16, the M new tokens' queries, the last of each sequence."""
+    TENSOR_PARAMS = ["K8", "K_scale", "O", "Q", "V8", "V_scale", "counts", "lengths"]
+
+    def __init__(self, scale: Optional[float] = None, causal: bool = True, block: int = 64):
+        super().__init__()
+        self.scale, self.causal, self.block = scale, causal, block
+
+    def _native(self, host, ws, K8, K_scale, O, Q, V8, V_scale, counts, lengths):
+        return host.cache8_attention(ws, self.scale, self.causal, self.block, K8, K_scale, O, Q, V8, V_scale, counts, lengths, None, None, None)
+
+
+class Cache8KeyWeights(Cache8Attention):
+    """Cache8Attention, and the attention weight that each key gets added to what it has: weights_out = weights + sums, float32 [B,Hkv,S];
+    weights may be None (zeros) or weights_out."""
+    TENSOR_PARAMS = ["K8", "K_scale", "O", "Q", "V8", "V_scale", "counts", "lengths", "weights", "weights_out"]
+
+    def _native(self, host, ws, K8, K_scale, O, Q, V8, V_scale, counts, lengths, weights, weights_out):
+        return host.cache8_attention(ws, self.scale, self.causal, self.block, K8, K_scale, O, Q, V8, V_scale, counts, lengths, None, weights, weights_out)
+
+
+class CacheEvict(FusedModule):
+    """Eviction from an fp16 cache by accumulated weight (`ops.cache_evict`): the scores of KeyFormerAttention and RoCoAttention (C_out, C_out1), a
+    row for each query head, or those of Cache8KeyWeights.  K_out, V_out may be K, V; weights_out weights or None; new_lengths lengths or None."""
+    TENSOR_PARAMS = ["K", "K_out", "V", "V_out", "kept", "lengths", "new_lengths", "weights", "weights_out"]
+
+    def __init__(self, keep: int, recent: int = 0):
+        super().__init__()
+        if not 0 <= recent <= keep or keep < 1:
+            raise ValueError("keep, recent: expected 0 <= recent <= keep, keep >= 1")
+        self.keep, self.recent = keep, recent
+
+    def _native(self, host, ws, K, K_out, V, V_out, kept, lengths, new_lengths, weights, weights_out):
+        return host.cache_evict(ws, self.keep, self.recent, 0, K, K_out, None, None, V, V_out, None, None, kept, lengths, new_lengths, weights, weights_out)
+
+
+class Cache8Evict(CacheEvict):
+    """CacheEvict for an 8-bit cache and its scales."""
+    TENSOR_PARAMS = ["K", "K_out", "K_scale", "K_scale_out", "V", "V_out", "V_scale", "V_scale_out", "kept", "lengths", "new_lengths", "weights", "weights_out"]
+
+    def __init__(self, keep: int, recent: int = 0, block: int = 64):
+        super().__init__(keep, recent)
+        self.block = block
+
+    def _native(self, host, ws, K, K_out, K_scale, K_scale_out, V, V_out, V_scale, V_scale_out, kept, lengths, new_lengths, weights, weights_out):
+        return host.cache_evict(ws, self.keep, self.recent, self.block, K, K_out, K_scale, K_scale_out, V, V_out, V_scale, V_scale_out, kept, lengths,
+                                new_lengths, weights, weights_out)
+
+
+CACHE = {"append8": Cache8Append, "attn8": Cache8Attention, "weights8": Cache8KeyWeights, "evict": CacheEvict, "evict8": Cache8Evict}
+
 PREFILL = {"rms": RMSNorm, "vanilla": Attention, "prenorm": PreNormBlock, "qknorm": QKNormAttention,
            "keyformer": KeyFormerAttention, "roco": RoCoAttention}
 DECODE = {"vanilla": DecodeVanilla, "prenorm": lambda **kw: DecodeVanilla(prenorm=True, **kw),
@@ -555,8 +620,9 @@ def get(variant: str, form: str = "prefill", **consts) -> FusedModule:
     {'lora','gmlp'} (form='linear').
     form='prefill': Q/K/V (or X and weights) given, causal, 1/sqrt(D) scale by default.
     form='decode' : the reference's decode-append problem (needs head_dim=...).
-    form='linear' : the reference's LoRA and gated-MLP workloads."""
-    table = {"prefill": PREFILL, "decode": DECODE, "linear": LINEAR}.get(form)
+    form='linear' : the reference's LoRA and gated-MLP workloads.
+    form='cache'  : an 8-bit cache's append, attention and key weights, and eviction, {'append8','attn8','weights8','evict','evict8'}."""
+    table = {"prefill": PREFILL, "decode": DECODE, "linear": LINEAR, "cache": CACHE}.get(form)
     if table is None or variant not in table:
         raise KeyError(f"no module for variant={variant!r} form={form!r}")
     return table[variant](**consts)

@@ -380,6 +380,53 @@ def gate(c1: torch.Tensor, c2: torch.Tensor, out: torch.Tensor, kind: str = "sig
     _lib.check("trn_gate_f16", st)
 
 
+def cache8_append(k, v, k8, v8, k_scale, v_scale, lengths: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None,
+                  block: int = 64) -> None:
+    """Quantise new keys and values k, v [B,Hkv,M,D] fp16 into an 8-bit cache: e4m3 codes k8, v8 [B,Hkv,S,D] (float8_e4m3fn or uint8) and
+    float32 scales [B,Hkv,ceil(S/block)], powers of two.  lengths int32 [B]: the keys of each sequence with the new ones (None: S);
+    counts int32 [B]: its new tokens (None: M).  Token i goes to position lengths[b] - counts[b] + i; k, v rows from counts[b] on are padding."""
+    _lib.host().cache8_append(block, k, k8, k_scale, v, v8, v_scale, counts, lengths)
+
+
+def cache8_attention(q, k8, v8, k_scale, v_scale, o, scale: Optional[float] = None, causal: bool = True, lengths: Optional[torch.Tensor] = None,
+                     counts: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None, weights: Optional[torch.Tensor] = None,
+                     weights_out: Optional[torch.Tensor] = None, block: int = 64, workspace: Optional[torch.Tensor] = None) -> None:
+    """`attention` of q, o [B,Hq,Sq,D] over an 8-bit cache (see cache8_append); query i of sequence b is its token lengths[b] - counts[b] + i, and
+    outputs from counts[b] on are not written.  A query that sees no key gets zeros.  scale: None for 1/sqrt(D).  weights_out float32 [B,Hkv,S]
+    receives weights (None: zeros; may be weights_out itself) plus the attention weight of each key, summed over the queries and the query
+    heads of its KV head.  workspace: uint8, cache8_attention_workspace_bytes(...) bytes of any contents; required with weights_out,
+    without it a head's keys are not shared out over workgroups."""
+    _lib.host().cache8_attention(workspace, scale, causal, block, k8, k_scale, o, q, v8, v_scale, counts, lengths, lse, weights, weights_out)
+
+
+def cache8_attention_workspace_bytes(q, k8, with_weights: bool = False) -> int:
+    """Bytes of workspace that `cache8_attention` takes for these tensors' shapes."""
+    c = _lib.Cache8()
+    c.batch, c.n_kv_heads, c.capacity, c.head_dim = (int(x) for x in k8.shape)
+    c.block = 64
+    return int(_lib.load().trn_cache8_attn_workspace_bytes(C.byref(c), int(q.shape[1]), int(q.shape[2]), int(with_weights)))
+
+
+def cache_evict(k, v, weights, k_out, v_out, kept, keep: int, recent: int, workspace: torch.Tensor, lengths: Optional[torch.Tensor] = None,
+                new_lengths: Optional[torch.Tensor] = None, weights_out: Optional[torch.Tensor] = None, k_scale: Optional[torch.Tensor] = None,
+                v_scale: Optional[torch.Tensor] = None, k_scale_out: Optional[torch.Tensor] = None, v_scale_out: Optional[torch.Tensor] = None,
+                block: int = 64) -> None:
+    """Shorten caches k, v [B,Hkv,S,D] (fp16, or e4m3 codes with their scales) to `keep` keys a head: the `recent` last ones of each sequence and
+    of the others those with the largest weights (float32 or float16 [B,Hw,S], Hw a multiple of Hkv whose rows are summed; ties to the earlier
+    key), in their order at the front of k_out, v_out, which may be k, v.  kept int32 [B,Hkv,keep] receives their old positions, then -1;
+    weights_out [B,Hw,keep], or weights itself, their weights; new_lengths int32 [B], or lengths itself, min(lengths, keep)."""
+    _lib.host().cache_evict(workspace, keep, recent, block, k, k_out, k_scale, k_scale_out, v, v_out, v_scale, v_scale_out, kept, lengths, new_lengths,
+                            weights, weights_out)
+
+
+def cache_evict_workspace_bytes(k, keep: int) -> int:
+    """Bytes of workspace that `cache_evict` takes for a cache of k's shape and type."""
+    e = _lib.CacheEvictDesc()
+    e.batch, e.n_kv_heads, e.keys, e.head_dim = (int(x) for x in k.shape)
+    e.keep, e.code_bytes = int(keep), k.element_size()
+    return int(_lib.load().trn_cache_evict_workspace_bytes(C.byref(e)))
+
+
 def calibration_copy(src: torch.Tensor, dst: torch.Tensor) -> None:
     """dst <- src with the library's plain streaming copy kernel (measurement yardstick)."""
     _need(src.is_cuda and dst.is_cuda and src.is_contiguous() and dst.is_contiguous(), "expected contiguous GPU tensors")
