@@ -126,6 +126,8 @@ ATTNS = [
     (1, 8, 8, 128, 1, 2500, 64, [2431], [1], True),              # split over workgroups
     (2, 16, 4, 64, 2, 3000, 128, [3000, 1777], [2, 2], False),
     (1, 4, 2, 128, 1, 1100, 32, [1100], [1], True),
+    (2, 8, 2, 128, 150, 400, 64, [400, 260], [150, 101], True),  # many rows: the weights in chunks of row tiles
+    (1, 71, 1, 64, 9, 700, 32, [611], [9], False),
 ]
 
 

@@ -41,8 +41,27 @@ __device__ __forceinline__ uint32_t recoded(uint32_t w, float ratio) {
     return codes_of((float)h[0] * ratio, (float)h[1] * ratio, (float)h[2] * ratio, (float)h[3] * ratio);
 }
 
+// One attention over an 8-bit cache: the arguments of its launches.
+struct Attn8Args {
+    const uint8_t *k, *v; const float *ks, *vs;
+    const int32_t *lengths, *counts;
+    const half_t* q; half_t* o; float* lse;
+    int B, Hq, Hkv, Sq, cap, G, R, n_rt, ns, bshift, causal;       // R = G * Sq rows in n_rt tiles; ns shares
+    Div by_units, by_g, by_hkv, by_ns, by_w;
+    int64_t kb, kh, kst, vb, vh, vst, ksb, ksh, vsb, vsh, qb, qh, qs, ob, oh, os;
+    float c;               // scale * log2(e)
+    float *part, *ml;      // shares: [B Hkv][n_rt][ns][32][D] and [..][32][2] (m, l)
+    float* lse2;           // [B Hkv][R]: log2 of the row sums, for the key weights (or null)
+    const float* w_in; float* w_out;
+    float* scores; int sp; // few rows: [B Hkv][R][sp] s = q k scale log2(e), what a row does not see -inf (or null)
+    float* w_part; int n_chunks, chunk_tiles;      // many rows: [n_chunks][B Hkv][cap] sums over a chunk's row tiles
+};
+
 inline bool block_ok(int block) { return block == 32 || block == 64 || block == 128; }
 // The checks of a cache that every entry point makes; base pointers, and strides of axes with more than one element.
 int cache8_check(const trn_cache8* c);
+// The second launch of an attention: shares joined, and the key weights of few rows out of their scores; the key weights of many rows.
+hipError_t launch_cache8_finish(const Attn8Args& a, int head_dim, hipStream_t s);
+hipError_t launch_cache8_weights(const Attn8Args& a, int head_dim, hipStream_t s);
 
 }  // namespace trn

@@ -16,19 +16,6 @@
 
 namespace trn {
 
-struct Attn8Args {
-    const uint8_t *k, *v; const float *ks, *vs;
-    const int32_t *lengths, *counts;
-    const half_t* q; half_t* o; float* lse;
-    int B, Hq, Hkv, Sq, cap, G, R, n_rt, ns, bshift, causal;       // R = G * Sq rows in n_rt tiles; ns shares
-    Div by_units, by_g, by_hkv, by_ns, by_w;
-    int64_t kb, kh, kst, vb, vh, vst, ksb, ksh, vsb, vsh, qb, qh, qs, ob, oh, os;
-    float c;               // scale * log2(e)
-    float *part, *ml;      // shares: [B Hkv][n_rt][ns][32][D] and [..][32][2] (m, l)
-    float* lse2;           // [B Hkv][R]: log2 of the row sums, for the key weights (or null)
-    const float* w_in; float* w_out;
-};
-
 // 32 keys of K and V a wave and stage
 template <int D> constexpr int kTile = 32 * D;
 
@@ -149,6 +136,16 @@ __global__ __launch_bounds__(NW * 64, 2) void cache8_attn_kernel(const Attn8Args
             const int lim = last - key0 - 4 * h;
 #pragma unroll
             for (int e = 0; e < 16; ++e) s[e] = 8 * (e >> 2) + (e & 3) <= lim ? s[e] : -INFINITY;
+        }
+        if (a.scores && there) {
+            float* const to = a.scores + ((int64_t)bh * a.R + row) * a.sp + key0 + 4 * h;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float4_t x;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[r] = s[4 * e + r] == -INFINITY ? -INFINITY : s[4 * e + r] * c;
+                *reinterpret_cast<float4_t*>(to + 8 * e) = x;
+            }
         }
         // (the largest score times a factor that is not negative; a score of -inf stays one beside a factor of zero)
         const float top = half_max(max16(s));
@@ -314,98 +311,8 @@ __global__ __launch_bounds__(NW * 64, 2) void cache8_attn_kernel(const Attn8Args
 #endif
 }
 
-// The shares of a row, D / 4 threads of it.
-template <int D>
-__global__ __launch_bounds__(256) void cache8_merge_kernel(const Attn8Args a) {
-    constexpr int TPR = D / 4, RPB = 256 / TPR;
-    const int per = (a.R + RPB - 1) / RPB;       // workgroups of a KV head
-    const int bh = blockIdx.x / per, r = (blockIdx.x - bh * per) * RPB + threadIdx.x / TPR, piece = threadIdx.x % TPR;
-    const int b = a.by_hkv.of(bh), kvh = bh - b * a.Hkv;
-    const int i0 = a.by_g.of(r), g0 = r - i0 * a.G;
-    if (r >= a.R || i0 >= tokens_of(a.counts, b, a.Sq)) return;
-    const int64_t at = ((int64_t)bh * a.n_rt + (r >> 5)) * a.ns;
-    const float* ml = a.ml + (at * 32 + (r & 31)) * 2;
-    const float* part = a.part + (at * 32 + (r & 31)) * D + 4 * piece;
-    float top = -INFINITY;
-    for (int i = 0; i < a.ns; ++i) top = fmaxf(top, ml[i * 64]);
-    float l = 0.f;
-    float4_t x = {0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < a.ns; ++i) {
-        const float m = ml[i * 64], f = m == -INFINITY ? 0.f : fast_exp2(m - top);
-        const float4_t y = *reinterpret_cast<const float4_t*>(part + (int64_t)i * 32 * D);
-        l = __builtin_fmaf(ml[i * 64 + 1], f, l);
-        x = x + y * f;
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    half4_t y;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = (half_t)(x[e] * inv);
-    *reinterpret_cast<half4_t*>(a.o + b * a.ob + (int64_t)(kvh * a.G + g0) * a.oh + (int64_t)i0 * a.os + 4 * piece) = y;
-    if (piece == 0) {
-        const float z = top + fast_log2(l);
-        if (a.lse) a.lse[((int64_t)b * a.Hq + kvh * a.G + g0) * a.Sq + i0] = z * kLn2;
-        if (a.lse2) a.lse2[(int64_t)bh * a.R + r] = z;
-    }
-}
-
-// What the keys have gathered: w_out[j] = w_in[j] + sum over the rows that see key j of 2^(s - lse2).  A wave has 32 keys, whose
-// codes it holds as operands, and walks over the row tiles.
-template <int D>
-__global__ __launch_bounds__(256) void cache8_weights_kernel(const Attn8Args a) {
-#if defined(__HIP_DEVICE_COMPILE__)
-    constexpr int NJ = D / 32;
-    const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int n_kt = (a.cap + 127) / 128;
-    const int bh = blockIdx.x / n_kt, key0 = (blockIdx.x - bh * n_kt) * 128 + wave * 32;
-    const int b = a.by_hkv.of(bh), kvh = bh - b * a.Hkv;
-    const int L = keys_of(a.lengths, b, a.cap), C = tokens_of(a.counts, b, a.Sq), off = L - C;
-    if (key0 >= L) return;
-    const uint8_t* kp = a.k + b * a.kb + kvh * a.kh + (int64_t)min(key0 + n, L - 1) * a.kst + h * 16;
-    half8_t kA[2 * NJ];
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-        const uint4_t w = *reinterpret_cast<const uint4_t*>(kp + 32 * j);
-        kA[2 * j] = half_of_codes(w.x, w.y); kA[2 * j + 1] = half_of_codes(w.z, w.w);
-    }
-    const float c = a.c * a.ks[b * a.ksb + kvh * a.ksh + (key0 >> a.bshift)];
-    float sum[16];
-#pragma unroll
-    for (int e = 0; e < 16; ++e) sum[e] = 0.f;
-    const int rows = min(a.R, C * a.G);
-    const int r_first = a.causal ? max(0, key0 - off) * a.G : 0;      // rows before it see none of these keys
-    for (int rt = r_first >> 5; rt * 32 < rows; ++rt) {
-        const int row = rt * 32 + n, qi = a.by_g.of(row), qg = row - qi * a.G;
-        const bool there = row < rows;
-        const half_t* qp = a.q + b * a.qb + (int64_t)(kvh * a.G + qg) * a.qh + (int64_t)qi * a.qs;
-        float16_t s;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = 0.f;
-#pragma unroll
-        for (int i = 0; i < 2 * NJ; ++i) {
-            half8_t z = {};
-            s = mfma32(kA[i], there ? *reinterpret_cast<const half8_t*>(qp + 16 * (2 * (i >> 1) + h) + 8 * (i & 1)) : z, s);
-        }
-        const float l2 = there ? a.lse2[(int64_t)bh * a.R + row] : 0.f;
-        const int lim = (there ? (a.causal ? min(L - 1, qi + off) : L - 1) : -1) - key0 - 4 * h;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) sum[e] += 8 * (e >> 2) + (e & 3) <= lim ? fast_exp2(__builtin_fmaf(s[e], c, -l2)) : 0.f;
-    }
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-#pragma unroll
-        for (int x = 16; x >= 1; x >>= 1) sum[e] += __shfl_xor(sum[e], x, 64);
-        const int key = key0 + 8 * (e >> 2) + 4 * h + (e & 3);
-        if (n == e && key < L) {
-            const int64_t at = (int64_t)bh * a.cap + key;
-            a.w_out[at] = (a.w_in ? a.w_in[at] : 0.f) + sum[e];
-        }
-    }
-#endif
-}
-
 // ------------------------------------------------------------------------------------------------ host
-struct Plan8 { int G, R, n_rt, ns; int64_t part, ml, lse2, bytes; };
+struct Plan8 { int G, R, n_rt, ns, n_chunks, chunk_tiles, sp; int64_t ml, lse2, more, bytes; };
 
 // How many workgroups share the keys of a row tile: two a compute unit over the launch, as long as a wave has two tiles.
 static Plan8 plan8(const trn_cache8* c, int Hq, int Sq, bool weights) {
@@ -413,15 +320,30 @@ static Plan8 plan8(const trn_cache8* c, int Hq, int Sq, bool weights) {
     p.G = Hq / c->n_kv_heads;
     p.R = p.G * Sq;
     p.n_rt = (p.R + 31) / 32;
-    const int64_t units = (int64_t)c->batch * c->n_kv_heads * p.n_rt, tiles = (c->capacity + 31) / 32;
+    const int64_t heads = (int64_t)c->batch * c->n_kv_heads, units = heads * p.n_rt, tiles = (c->capacity + 31) / 32;
     int64_t ns = units ? 512 / units : 1;
     if (ns > tiles / 8) ns = tiles / 8;
     p.ns = (int)(ns < 1 ? 1 : ns > 64 ? 64 : ns);
     auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
-    p.part = 0;
     p.ml = p.ns > 1 ? up(units * p.ns * 32 * c->head_dim * 4) : 0;
     p.lse2 = p.ml + (p.ns > 1 ? up(units * p.ns * 64 * 4) : 0);
-    p.bytes = p.lse2 + (weights ? up((int64_t)c->batch * c->n_kv_heads * p.R * 4) : 0);
+    p.more = p.lse2 + (weights ? up(heads * p.R * 4) : 0);
+    p.bytes = p.more;
+    // Key weights: a score of 4 bytes goes out and comes back for each row and key, or K is read again.
+    p.sp = weights && 8 * p.R <= c->head_dim ? (int)tiles * 32 : 0;
+    p.n_chunks = 1; p.chunk_tiles = p.n_rt;
+    if (p.sp) p.bytes += up(heads * p.R * p.sp * 4);
+    else if (weights) {
+        // (four workgroups a compute unit, a chunk of four row tiles at least)
+        const int64_t blocks = heads * ((c->capacity + 255) / 256);
+        int64_t chunks = blocks ? 1024 / blocks : 1;
+        if (chunks > p.n_rt / 4) chunks = p.n_rt / 4;
+        if (chunks > 1) {
+            p.chunk_tiles = (int)((p.n_rt + chunks - 1) / chunks);
+            p.n_chunks = (p.n_rt + p.chunk_tiles - 1) / p.chunk_tiles;
+            if (p.n_chunks > 1) p.bytes += up(p.n_chunks * heads * c->capacity * 4);
+        }
+    }
     return p;
 }
 
@@ -469,7 +391,7 @@ extern "C" int trn_cache8_attn_f16(const trn_cache8* c, const void* q, void* o, 
     a.G = p.G; a.R = p.R; a.n_rt = p.n_rt; a.ns = p.ns; a.causal = causal != 0;
     a.bshift = c->block == 32 ? 5 : c->block == 64 ? 6 : 7;
     const int64_t heads = (int64_t)c->batch * c->n_kv_heads, units = heads * p.ns;
-    if (units * p.n_rt > 0x7fffffffLL) return TRN_E_SHAPE;
+    if (units * p.n_rt > 0x7fffffffLL || heads * ((int64_t)p.R + 1) > 0x7fffffffLL || heads * ((c->capacity + 255) / 256) * p.n_chunks > 0x3fffffffLL) return TRN_E_SHAPE;
     a.by_units = Div(units); a.by_g = Div(p.G); a.by_hkv = Div(c->n_kv_heads); a.by_ns = Div(p.ns); a.by_w = Div(4 * p.ns);
     a.kb = c->k_stride_b; a.kh = c->k_stride_h; a.kst = c->k_stride_s;
     a.vb = c->v_stride_b; a.vh = c->v_stride_h; a.vst = c->v_stride_s;
@@ -479,21 +401,14 @@ extern "C" int trn_cache8_attn_f16(const trn_cache8* c, const void* q, void* o, 
     a.part = (float*)workspace; a.ml = (float*)((char*)workspace + p.ml);
     a.lse2 = weights_out ? (float*)((char*)workspace + p.lse2) : nullptr;
     a.w_in = weights_in; a.w_out = weights_out;
+    a.sp = p.sp; a.scores = p.sp ? (float*)((char*)workspace + p.more) : nullptr;
+    a.n_chunks = p.n_chunks; a.chunk_tiles = p.chunk_tiles; a.w_part = p.n_chunks > 1 ? (float*)((char*)workspace + p.more) : nullptr;
     const hipStream_t s = (hipStream_t)stream;
     const bool d128 = c->head_dim == 128;
     if (d128) hipLaunchKernelGGL((cache8_attn_kernel<128, 4>), dim3((unsigned)(units * p.n_rt)), dim3(256), 0, s, a);
     else hipLaunchKernelGGL((cache8_attn_kernel<64, 4>), dim3((unsigned)(units * p.n_rt)), dim3(256), 0, s, a);
-    if (p.ns > 1) {
-        const int64_t grid = heads * (((int64_t)p.R + (d128 ? 7 : 15)) / (d128 ? 8 : 16));
-        if (grid > 0x7fffffffLL) return TRN_E_SHAPE;
-        if (d128) hipLaunchKernelGGL((cache8_merge_kernel<128>), dim3((unsigned)grid), dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((cache8_merge_kernel<64>), dim3((unsigned)grid), dim3(256), 0, s, a);
-    }
-    if (weights_out && c->capacity > 0) {
-        const int64_t grid = heads * ((c->capacity + 127) / 128);
-        if (grid > 0x7fffffffLL) return TRN_E_SHAPE;
-        if (d128) hipLaunchKernelGGL((cache8_weights_kernel<128>), dim3((unsigned)grid), dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((cache8_weights_kernel<64>), dim3((unsigned)grid), dim3(256), 0, s, a);
-    }
-    return hipGetLastError() == hipSuccess ? TRN_OK : TRN_E_LAUNCH;
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess && (p.ns > 1 || p.sp)) e = launch_cache8_finish(a, c->head_dim, s);
+    if (e == hipSuccess && weights_out && !p.sp && c->capacity > 0) e = launch_cache8_weights(a, c->head_dim, s);
+    return e == hipSuccess ? TRN_OK : TRN_E_LAUNCH;
 }
