@@ -114,8 +114,11 @@ def test_other_blocks_and_token_major_caches(block, place):
     _run(CASES[1], "spread", True, 16, place, layout="token")
 
 
-def test_long_rows_of_equal_weights():
-    _run((1, 1, 1, 64, 40000, 20000, 100, [39999]), "ties", False, 16, "within")
+@pytest.mark.parametrize("kind", ["spread", "ties"])
+@pytest.mark.parametrize("S", [4096, 4097, 8193, 16385, 32768, 32769, 40000])
+def test_long_rows(S, kind):
+    _run((1, 1, 2, 64, S, S // 2 + 1, 100, [S - 1]), kind, False, 16, "within")
+    _run((1, 2, 1, 64, S, S // 3, 0, [S]), kind, True, 8, "apart")
 
 
 def test_keyformer_scores_cut_a_prompt():
@@ -224,7 +227,7 @@ def test_refusals():
     bad(keep=0); bad(recent=17); bad(recent=-1); bad(kept=kept[:, :1]); bad(kept=kept.long()); bad(weights=w[:, :3].contiguous()); bad(weights=w.double())
     bad(weights=w[:, :, ::2]); bad(v=v[:, :, :32]); bad(k_out=out[:, :, :8]); bad(k_out=out.float()); bad(weights_out=torch.zeros(1, 4, 64, device=DEV))
     bad(k=k.float()); bad(lengths=torch.zeros(1, device=DEV)); bad(workspace=ws.float()); bad(k=k.cpu())
-    bad(_lib.TrnError, workspace=ws[:256]); bad(_lib.TrnError, k_out=k[:, :, 8:24]); bad(_lib.TrnError, k_out=v[:, :, :16]); bad(_lib.TrnError, v_out=out)
+    bad(_lib.TrnError, workspace=ws[:128]); bad(_lib.TrnError, k_out=k[:, :, 8:24]); bad(_lib.TrnError, k_out=v[:, :, :16]); bad(_lib.TrnError, v_out=out)
     bad(_lib.TrnError, k_out=out[:, :1].expand(1, 2, 16, 64))
     codes = torch.zeros(1, 2, 64, 64, dtype=torch.uint8, device=DEV)
     bad(k=codes, v=codes, k_out=codes, v_out=codes)

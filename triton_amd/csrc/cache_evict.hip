@@ -3,10 +3,11 @@
 //
 // Two launches.  Selection: a workgroup has one head of a sequence.  The weights of its query heads are added up in 64 bits and rounded
 // once to fp32, turned into integers that order as they do, and the smallest one kept is found by digits of 11, 11 and 10 bits, counted in
-// LDS; ties are filled up from the front.  A last pass numbers the kept keys in order.  Move: rows of K and V, 16 bytes a lane.  Into
-// another cache, workgroups share the rows; within the same one, a workgroup has a 64-byte column of all of a head's rows and
-// moves them front to back: a row goes to its own place or one before it, so what a step overwrites has been read by this step or an
-// earlier one, and columns never meet.
+// LDS; ties are filled up from the front.  Up to 32768 keys stay in registers, a thread with consecutive ones, so that one scan over the
+// threads numbers what is kept.  Move: rows of K and V, 16 bytes a lane, past the caches (each byte once).  Into another cache, workgroups
+// share the rows; within the same one, a workgroup has a 64-byte column of all of a head's rows and moves them front to back: a row
+// goes to its own place or one before it, so what a step overwrites has been read by this step or an earlier one, and columns
+// never meet.
 //
 // 8-bit caches: a block of the shortened cache takes the largest of the scales that its rows come with; codes of rows with a smaller
 // one are multiplied by the ratio, which between powers of two only rounds what leaves e4m3's normal numbers.
@@ -23,7 +24,8 @@ struct EvictArgs {
     int64_t st[2][3], ot[2][3];        // strides of K and V in bytes, given and kept
     int64_t sst[2][2], sot[2][2];      // ... of their scales
     uint32_t* order;                   // [B Hkv][S]
-    float* ratio;                      // [2][B Hkv][keep]
+    float* scales;                     // 8 bits: [2][B Hkv][n_blocks], the scales as they were
+    int n_blocks;
     int32_t* now;                      // [2][B]: keys that stay, and that there were
     int chunks, cols;                  // move: workgroups of a head's rows and columns
     Div by_hkv, by_chunks, by_cols;
@@ -36,187 +38,242 @@ __device__ __forceinline__ uint32_t order_of(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;       // (0xff800000's complement, of -inf, is 0x7fffff: above NaN's)
 }
 
+// The sum of a key's weights over its KV head's rows.
+__device__ __forceinline__ uint32_t order_at(const EvictArgs& a, int64_t at, int per) {
+    double s = 0.0;
+    for (int g = 0; g < per; ++g)
+        s += a.w_half ? (double)(float)static_cast<const half_t*>(a.w)[at + (int64_t)g * a.S] : (double)static_cast<const float*>(a.w)[at + (int64_t)g * a.S];
+    return order_of((float)s);
+}
+// (x, y) summed over the threads before this one; `all`: over all of them.  16 waves.
+__device__ __forceinline__ int2 scan_before(int x, int y, int2* waves, int2& all) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int sx = x, sy = y;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        const int px = __shfl_up(sx, m, 64), py = __shfl_up(sy, m, 64);
+        if (lane >= m) { sx += px; sy += py; }
+    }
+    if (lane == 63) waves[wave] = int2{sx, sy};
+    __syncthreads();
+    int2 r = {sx - x, sy - y};
+    all = int2{0, 0};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int2 w = waves[i];
+        if (i < wave) { r.x += w.x; r.y += w.y; }
+        all.x += w.x; all.y += w.y;
+    }
+    __syncthreads();
+    return r;
+}
+
+// NV: a thread has as many consecutive keys, in registers (0: any number, whose order lies in the workspace and is walked over 1024 keys at a
+// time).
+template <int NV>
 __global__ __launch_bounds__(1024) void cache_evict_select_kernel(const EvictArgs a) {
     __shared__ int bins[2048];
-    __shared__ int waves[16], s_digit, s_above, s_base, s_ties;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __shared__ int2 waves[16];
+    __shared__ int s_digit, s_above;
+    const int tid = threadIdx.x;
     const int bh = blockIdx.x, b = a.by_hkv.of(bh), h = bh - b * a.Hkv;
     const int n = keys_of(a.lengths, b, a.S), stay = min(n, a.keep);
     const int late = min(a.recent, stay), early = n - late;              // the last `late` keys stay in any case
-    int want = stay - late;                                              // ... and so many of the first `early`
+    const int want = stay - late;                                        // ... and so many of the first `early`
     int32_t* kept = a.kept + (int64_t)bh * a.keep;
     uint32_t* order = a.order + (int64_t)bh * a.S;
     const int per = a.Hw / a.Hkv;
+    const int64_t w0 = ((int64_t)b * a.Hw + h * per) * a.S;
 
-    uint32_t least = 0; int ties = 0;         // kept: order > least, and the first `ties` of those equal to it
-    if (want < early && want > 0) {
-        for (int j = tid; j < early; j += 1024) {
-            double s = 0.0;
-            const int64_t at = ((int64_t)b * a.Hw + h * per) * a.S + j;
-            for (int g = 0; g < per; ++g)
-                s += a.w_half ? (double)(float)static_cast<const half_t*>(a.w)[at + (int64_t)g * a.S] : (double)static_cast<const float*>(a.w)[at + (int64_t)g * a.S];
-            order[j] = order_of((float)s);
-        }
-        int rest = want;
-        for (int pass = 0; pass < 3; ++pass) {
-            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-            for (int i = tid; i < 2048; i += 1024) bins[i] = 0;
-            __syncthreads();
-            for (int j = tid; j < early; j += 1024) {
-                const uint32_t u = order[j];
-                if (pass == 0 || (u >> (shift + bits)) == (least >> (shift + bits))) atomicAdd(&bins[(u >> shift) & ((1 << bits) - 1)], 1);
-            }
-            __syncthreads();
-            // from the top: thread i has the bins 2047 - 2 i and one below
-            const int hi = bins[2047 - 2 * tid], lo = bins[2046 - 2 * tid];
-            int sum = hi + lo;
-#pragma unroll
-            for (int m = 1; m < 64; m <<= 1) { const int x = __shfl_up(sum, m, 64); if (lane >= m) sum += x; }
-            if (lane == 63) waves[wave] = sum;
-            __syncthreads();
-            int before = sum - hi - lo;
-            for (int i = 0; i < wave; ++i) before += waves[i];
-            if (before < rest && before + hi + lo >= rest) {
-                const bool first = before + hi >= rest;
-                s_digit = first ? 2047 - 2 * tid : 2046 - 2 * tid;
-                s_above = first ? before : before + hi;
-            }
-            __syncthreads();
-            least |= (uint32_t)s_digit << shift;
-            rest -= s_above;
-            __syncthreads();
-        }
-        ties = rest;
-    }
-    const bool all = want >= early;
-    // in order, 1024 keys at a time
-    if (tid == 0) { s_base = 0; s_ties = 0; }
-    __syncthreads();
-    if (want > 0) {
-        for (int j0 = 0; j0 < early; j0 += 1024) {
-            const int j = j0 + tid;
-            const uint32_t u = j < early && !all ? order[j] : 0;
-            const bool tie = j < early && !all && u == least;
-            const uint64_t tb = __ballot(tie);
-            if (lane == 0) waves[wave] = __popcll(tb);
-            __syncthreads();
-            int t_before = s_ties + __popcll(tb & ((1ull << lane) - 1)), t_all = 0;
-            for (int i = 0; i < 16; ++i) { if (i < wave) t_before += waves[i]; t_all += waves[i]; }
-            const bool take = j < early && (all || u > least || (tie && t_before < ties));
-            const uint64_t kb = __ballot(take);
-            __syncthreads();
-            if (lane == 0) waves[wave] = __popcll(kb);
-            __syncthreads();
-            int at = s_base + __popcll(kb & ((1ull << lane) - 1)), k_all = 0;
-            for (int i = 0; i < 16; ++i) { if (i < wave) at += waves[i]; k_all += waves[i]; }
-            if (take) kept[at] = j;
-            __syncthreads();
-            if (tid == 0) { s_base += k_all; s_ties += t_all; }
-            __syncthreads();
+    // (the scales as they were: the move writes where they lie)
+    if (a.scales) {
+        const int blocks = (n + (1 << a.bshift) - 1) >> a.bshift;
+        for (int kv = 0; kv < 2; ++kv) {
+            const float* s = (kv ? a.vs : a.ks) + b * a.sst[kv][0] + h * a.sst[kv][1];
+            float* to = a.scales + ((int64_t)kv * a.B * a.Hkv + bh) * a.n_blocks;
+            for (int i = tid; i < blocks; i += 1024) to[i] = s[i];
         }
     }
+    if (h == 0 && tid == 0) { a.now[b] = stay; a.now[a.B + b] = n; }
     for (int i = tid; i < late; i += 1024) kept[want + i] = early + i;
     for (int i = stay + tid; i < a.keep; i += 1024) kept[i] = -1;
-    if (h == 0 && tid == 0) { a.now[b] = stay; a.now[a.B + b] = n; }
-    if (!a.ratio) return;
-    // 8 bits: new scales, and what each kept row's codes are to be multiplied by
-    __syncthreads();
-    for (int kv = 0; kv < 2; ++kv) {
-        const float* s = (kv ? a.vs : a.ks) + b * a.sst[kv][0] + h * a.sst[kv][1];
-        float* so = (kv ? a.vs_out : a.ks_out) + b * a.sot[kv][0] + h * a.sot[kv][1];
-        float* ratio = a.ratio + ((int64_t)kv * a.B * a.Hkv + bh) * a.keep;
-        for (int i = tid; i < stay; i += 1024) ratio[i] = s[kept[i] >> a.bshift];
-        __syncthreads();      // (the scales may be written where they were read)
-        const int block = 1 << a.bshift;
-        for (int i0 = wave * block; i0 < stay; i0 += 16 * block) {
-            float top = 0.f;
-            for (int i = i0 + lane; i < min(i0 + block, stay); i += 64) top = fmaxf(top, ratio[i]);
+    if (want == 0) return;
+    if (want == early) {
+        for (int i = tid; i < early; i += 1024) kept[i] = i;
+        return;
+    }
+
+    uint32_t u[NV ? NV : 1];
+    if constexpr (NV > 0) {
 #pragma unroll
-            for (int m = 32; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
-            for (int i = i0 + lane; i < min(i0 + block, stay); i += 64) ratio[i] = top > 0.f ? ratio[i] / top : 1.f;
-            if (lane == 0) so[i0 >> a.bshift] = top;
+        for (int i = 0; i < NV; ++i) { const int j = tid * NV + i; u[i] = j < early ? order_at(a, w0 + j, per) : 0; }
+    } else {
+        for (int j = tid; j < early; j += 1024) order[j] = order_at(a, w0 + j, per);
+    }
+    // The smallest order kept: kept are those above it, and the first `rest` of its equals.
+    uint32_t least = 0;
+    int rest = want;
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+        for (int i = tid; i < 2048; i += 1024) bins[i] = 0;
+        __syncthreads();
+        auto count = [&](uint32_t x) {
+            if (pass == 0 || (x >> (shift + bits)) == (least >> (shift + bits))) atomicAdd(&bins[(x >> shift) & ((1 << bits) - 1)], 1);
+        };
+        if constexpr (NV > 0) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) if (tid * NV + i < early) count(u[i]);
+        } else for (int j = tid; j < early; j += 1024) count(order[j]);
+        __syncthreads();
+        // from the top: thread i has the bins 2047 - 2 i and one below
+        const int hi = bins[2047 - 2 * tid], lo = bins[2046 - 2 * tid];
+        int2 all;
+        const int before = scan_before(hi + lo, 0, waves, all).x;
+        if (before < rest && before + hi + lo >= rest) {
+            const bool first = before + hi >= rest;
+            s_digit = first ? 2047 - 2 * tid : 2046 - 2 * tid;
+            s_above = first ? before : before + hi;
         }
         __syncthreads();
+        least |= (uint32_t)s_digit << shift;
+        rest -= s_above;
+    }
+    // Their places: by what is kept, and by how many equals of the least there are, before them.
+    int2 all;
+    if constexpr (NV > 0) {
+        int above = 0, ties = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const bool real = tid * NV + i < early;
+            above += real && u[i] > least; ties += real && u[i] == least;
+        }
+        const int2 before = scan_before(above, ties, waves, all);
+        int tie = before.y, at = before.x + min(before.y, rest);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const bool real = tid * NV + i < early, eq = real && u[i] == least;
+            if (real && (u[i] > least || (eq && tie < rest))) kept[at++] = tid * NV + i;
+            tie += eq;
+        }
+    } else {
+        int2 base = {0, 0};
+        for (int j0 = 0; j0 < early; j0 += 1024) {
+            const int j = j0 + tid;
+            const uint32_t x = j < early ? order[j] : 0;
+            const bool up = j < early && x > least, eq = j < early && x == least;
+            const int2 before = scan_before(up, eq, waves, all);
+            const int tie = base.y + before.y;
+            if (up || (eq && tie < rest)) kept[base.x + before.x + min(tie, rest)] = j;
+            base.x += all.x; base.y += all.y;
+        }
     }
 }
 
-// blockIdx.y: 0 K, 1 V; blockIdx.x: (head of a sequence, chunk of rows, column).  W: 16-byte pieces of a row; in place a workgroup has 4 of
-// them, as a column, and all rows.
+// Workgroups from n_rows on: (head of a sequence, K or V, chunk of rows, column).  The first: the weights of the kept keys, one for each row of
+// them, and the new lengths.
 template <bool BITS8>
-__global__ __launch_bounds__(256) void cache_evict_move_kernel(const EvictArgs a, int row_pieces, int piece_shift, int rows_per_chunk) {
-    const int kv = blockIdx.y;
-    const int u = a.by_cols.of(blockIdx.x), col = blockIdx.x - u * a.cols;
-    const int bh = a.by_chunks.of(u), chunk = u - bh * a.chunks;
+__global__ __launch_bounds__(256) void cache_evict_move_kernel(const EvictArgs a, int row_pieces, int piece_shift, int rows_per_chunk, int n_rows) {
+    const int tid = threadIdx.x;
+    if ((int)blockIdx.x < n_rows) {
+        const int row = blockIdx.x, b = row / a.Hw, hw = row - b * a.Hw;
+        const int stay = a.now[b];
+        if (hw == 0 && tid == 0 && a.new_lengths) a.new_lengths[b] = stay;
+        if (!a.w_out) return;
+        const int32_t* kept = a.kept + ((int64_t)b * a.Hkv + hw / (a.Hw / a.Hkv)) * a.keep;
+        const int64_t from = (int64_t)row * a.S;
+        // (w_out may be w, whose rows are S apart, or a tensor of its own with rows of `keep`)
+        const int64_t to = a.w_out == a.w ? from : (int64_t)row * a.keep;
+        constexpr int NW = 4;
+        for (int i0 = 0; i0 < stay; i0 += NW * 256) {
+            float x[NW];
+#pragma unroll
+            for (int e = 0; e < NW; ++e) {
+                const int i = i0 + e * 256 + tid;
+                if (i < stay) x[e] = a.w_half ? (float)static_cast<const half_t*>(a.w)[from + kept[i]] : static_cast<const float*>(a.w)[from + kept[i]];
+            }
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < NW; ++e) {
+                const int i = i0 + e * 256 + tid;
+                if (i < stay) {
+                    if (a.w_half) static_cast<half_t*>(a.w_out)[to + i] = (half_t)x[e];
+                    else static_cast<float*>(a.w_out)[to + i] = x[e];
+                }
+            }
+        }
+        // (the places that new keys will take have gathered nothing)
+        if (a.w_out == a.w) {
+            const int n = a.now[a.B + b];
+            for (int i = stay + tid; i < n; i += 256) {
+                if (a.w_half) static_cast<half_t*>(a.w_out)[to + i] = (half_t)0.f;
+                else static_cast<float*>(a.w_out)[to + i] = 0.f;
+            }
+        }
+        return;
+    }
+    int u = blockIdx.x - n_rows;
+    const int v2 = a.by_cols.of(u), col = u - v2 * a.cols;
+    u = a.by_chunks.of(v2);
+    const int chunk = v2 - u * a.chunks, kv = u & 1, bh = u >> 1;
     const int b = a.by_hkv.of(bh), h = bh - b * a.Hkv;
     const int stay = a.now[b];
+    const int from = chunk * rows_per_chunk, to = min(stay, from + rows_per_chunk);
+    if (from >= to) return;
     const int32_t* kept = a.kept + (int64_t)bh * a.keep;
     const char* src = (const char*)(kv ? a.v : a.k) + b * a.st[kv][0] + h * a.st[kv][1];
     char* dst = (char*)(kv ? a.v_out : a.k_out) + b * a.ot[kv][0] + h * a.ot[kv][1];
-    const float* ratio = BITS8 ? a.ratio + ((int64_t)kv * a.B * a.Hkv + bh) * a.keep : nullptr;
-    const int sub = threadIdx.x & (row_pieces - 1), r0 = threadIdx.x >> piece_shift, step = 256 >> piece_shift;
+    const int sub = tid & (row_pieces - 1), r0 = tid >> piece_shift, step = 256 >> piece_shift;
     const int off = (col * row_pieces + sub) * 16;
-    const int from = chunk * rows_per_chunk, to = min(stay, from + rows_per_chunk);
     constexpr int NB = 4;      // rows of a lane on their way at once
+    __shared__ float ratio[256], top[8];
     for (int i0 = from; i0 < to; i0 += NB * step) {
-        uint4_t x[NB]; float f[NB];
+        uint4_t x[NB];
+#pragma unroll
+        for (int e = 0; e < NB; ++e) {
+            const int i = i0 + e * step + r0;
+            if (i < to) x[e] = __builtin_nontemporal_load(reinterpret_cast<const uint4_t*>(src + (int64_t)kept[i] * a.st[kv][2] + off));
+        }
+        // 8 bits: the blocks of these rows (128 or 256: whole blocks) and what their codes are to be multiplied by
+        if constexpr (BITS8) {
+            const float* was = a.scales + ((int64_t)kv * a.B * a.Hkv + bh) * a.n_blocks;
+            const float s = tid < NB * step && i0 + tid < to ? was[kept[i0 + tid] >> a.bshift] : 0.f;
+            float t = s;
+#pragma unroll
+            for (int m = 16; m >= 1; m >>= 1) t = fmaxf(t, __shfl_xor(t, m, 64));
+            if ((tid & 31) == 0) top[tid >> 5] = t;
+            __syncthreads();
+            const int groups = 1 << (a.bshift - 5), g0 = (tid >> 5) & ~(groups - 1);
+            for (int i = 0; i < groups; ++i) t = fmaxf(t, top[g0 + i]);
+            ratio[tid] = t > 0.f ? s / t : 1.f;
+            if (col == 0 && (tid & ((1 << a.bshift) - 1)) == 0 && tid < NB * step && i0 + tid < to)
+                ((kv ? a.vs_out : a.ks_out) + b * a.sot[kv][0] + h * a.sot[kv][1])[(i0 + tid) >> a.bshift] = t;
+        }
+        if (BITS8 || a.in_place[kv]) __syncthreads();      // (waits for the loads as well: what this step overwrites has been read)
 #pragma unroll
         for (int e = 0; e < NB; ++e) {
             const int i = i0 + e * step + r0;
             if (i < to) {
-                x[e] = *reinterpret_cast<const uint4_t*>(src + (int64_t)kept[i] * a.st[kv][2] + off);
-                if (BITS8) f[e] = ratio[i];
+                if constexpr (BITS8) {
+                    const float f = ratio[e * step + r0];
+                    if (f != 1.f) x[e] = uint4_t{recoded(x[e].x, f), recoded(x[e].y, f), recoded(x[e].z, f), recoded(x[e].w, f)};
+                }
+                __builtin_nontemporal_store(x[e], reinterpret_cast<uint4_t*>(dst + (int64_t)i * a.ot[kv][2] + off));
             }
         }
-        if (a.in_place[kv]) __syncthreads();      // (waits for the loads as well: what this step overwrites has been read)
-#pragma unroll
-        for (int e = 0; e < NB; ++e) {
-            const int i = i0 + e * step + r0;
-            if (i < to) {
-                if (BITS8 && f[e] != 1.f) x[e] = uint4_t{recoded(x[e].x, f[e]), recoded(x[e].y, f[e]), recoded(x[e].z, f[e]), recoded(x[e].w, f[e])};
-                *reinterpret_cast<uint4_t*>(dst + (int64_t)i * a.ot[kv][2] + off) = x[e];
-            }
-        }
+        if (BITS8 && i0 + NB * step < to) __syncthreads();      // (`ratio` and `top` are written again)
     }
 }
 
-// The weights of the kept keys, a workgroup for each row of them; and the new lengths.
-__global__ __launch_bounds__(1024) void cache_evict_weights_kernel(const EvictArgs a) {
-    const int row = blockIdx.x, b = row / a.Hw, hw = row - b * a.Hw;
-    const int stay = a.now[b];
-    if (hw == 0 && threadIdx.x == 0 && a.new_lengths) a.new_lengths[b] = stay;
-    if (!a.w_out) return;
-    const int32_t* kept = a.kept + ((int64_t)b * a.Hkv + hw / (a.Hw / a.Hkv)) * a.keep;
-    const int64_t from = (int64_t)row * a.S;
-    // (w_out may be w, whose rows are S apart, or a tensor of its own with rows of `keep`)
-    const int64_t to = a.w_out == a.w ? from : (int64_t)row * a.keep;
-    for (int i0 = 0; i0 < stay; i0 += 1024) {
-        const int i = i0 + threadIdx.x;
-        float x = 0.f;
-        if (i < stay) x = a.w_half ? (float)static_cast<const half_t*>(a.w)[from + kept[i]] : static_cast<const float*>(a.w)[from + kept[i]];
-        __syncthreads();
-        if (i < stay) {
-            if (a.w_half) static_cast<half_t*>(a.w_out)[to + i] = (half_t)x;
-            else static_cast<float*>(a.w_out)[to + i] = x;
-        }
-    }
-    // (the places that new keys will take have gathered nothing)
-    if (a.w_out == a.w) {
-        const int n = a.now[a.B + b];
-        for (int i = stay + threadIdx.x; i < n; i += 1024) {
-            if (a.w_half) static_cast<half_t*>(a.w_out)[to + i] = (half_t)0.f;
-            else static_cast<float*>(a.w_out)[to + i] = 0.f;
-        }
-    }
-}
+// Keys of which a thread of the selection has its own in registers.
+constexpr int kMostKept = 32768;
 
-struct EvictSizes { int64_t order, ratio, now, bytes; };
+struct EvictSizes { int64_t scales, now, bytes; };
 static EvictSizes evict_sizes(const trn_cache_evict_desc* e) {
     auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
     EvictSizes s;
     const int64_t heads = (int64_t)e->batch * e->n_kv_heads;
-    s.order = 0;
-    s.ratio = up(heads * e->keys * 4);
-    s.now = s.ratio + (e->code_bytes == 1 ? up(2 * heads * e->keep * 4) : 0);
+    s.scales = e->keys > kMostKept ? up(heads * e->keys * 4) : 0;
+    s.now = s.scales + (e->code_bytes == 1 ? up(2 * heads * ((e->keys + 31) / 32) * 4) : 0);
     s.bytes = s.now + up((int64_t)e->batch * 8);
     return s;
 }
@@ -291,13 +348,19 @@ extern "C" int trn_cache_evict(const trn_cache_evict_desc* e, const void* k, con
     a.sst[0][0] = e->k_scale_stride[0]; a.sst[0][1] = e->k_scale_stride[1]; a.sst[1][0] = e->v_scale_stride[0]; a.sst[1][1] = e->v_scale_stride[1];
     a.sot[0][0] = e->k_scale_out_stride[0]; a.sot[0][1] = e->k_scale_out_stride[1]; a.sot[1][0] = e->v_scale_out_stride[0]; a.sot[1][1] = e->v_scale_out_stride[1];
     a.order = (uint32_t*)workspace;
-    a.ratio = bits8 ? (float*)((char*)workspace + sz.ratio) : nullptr;
+    a.scales = bits8 ? (float*)((char*)workspace + sz.scales) : nullptr;
+    a.n_blocks = bits8 ? (e->keys + e->block - 1) / e->block : 0;
     a.now = (int32_t*)((char*)workspace + sz.now);
     const int64_t heads = (int64_t)e->batch * e->n_kv_heads;
     if (heads > 0x7fffffff || (int64_t)e->batch * e->n_weight_rows > 0x7fffffff) return TRN_E_SHAPE;
     a.by_hkv = Div(e->n_kv_heads);
     const hipStream_t s = (hipStream_t)stream;
-    hipLaunchKernelGGL(cache_evict_select_kernel, dim3((unsigned)heads), dim3(1024), 0, s, a);
+    const dim3 sel((unsigned)heads);
+    if (e->keys <= 4096) hipLaunchKernelGGL(cache_evict_select_kernel<4>, sel, dim3(1024), 0, s, a);
+    else if (e->keys <= 8192) hipLaunchKernelGGL(cache_evict_select_kernel<8>, sel, dim3(1024), 0, s, a);
+    else if (e->keys <= 16384) hipLaunchKernelGGL(cache_evict_select_kernel<16>, sel, dim3(1024), 0, s, a);
+    else if (e->keys <= kMostKept) hipLaunchKernelGGL(cache_evict_select_kernel<32>, sel, dim3(1024), 0, s, a);
+    else hipLaunchKernelGGL(cache_evict_select_kernel<0>, sel, dim3(1024), 0, s, a);
     // rows shared out, or in columns of 64 bytes
     const bool columns = a.in_place[0] || a.in_place[1];
     const int pieces = width / 16, row_pieces = columns ? 4 : pieces;
@@ -306,12 +369,10 @@ extern "C" int trn_cache_evict(const trn_cache_evict_desc* e, const void* k, con
     const int rows_per_chunk = columns ? rows_out : 4 * (256 / row_pieces);
     a.cols = pieces / row_pieces;
     a.chunks = (rows_out + rows_per_chunk - 1) / rows_per_chunk;
-    if (heads * a.chunks * a.cols > 0x7fffffffLL) return TRN_E_SHAPE;
+    const int64_t n_rows = weights_out || new_lengths ? (int64_t)e->batch * e->n_weight_rows : 0, grid = n_rows + 2 * heads * a.chunks * a.cols;
+    if (grid > 0x7fffffffLL) return TRN_E_SHAPE;
     a.by_cols = Div(a.cols); a.by_chunks = Div(a.chunks);
-    const dim3 grid((unsigned)(heads * a.chunks * a.cols), 2);
-    if (bits8) hipLaunchKernelGGL((cache_evict_move_kernel<true>), grid, dim3(256), 0, s, a, row_pieces, shift, rows_per_chunk);
-    else hipLaunchKernelGGL((cache_evict_move_kernel<false>), grid, dim3(256), 0, s, a, row_pieces, shift, rows_per_chunk);
-    if (weights_out || new_lengths)
-        hipLaunchKernelGGL(cache_evict_weights_kernel, dim3((unsigned)(e->batch * e->n_weight_rows)), dim3(1024), 0, s, a);
+    if (bits8) hipLaunchKernelGGL((cache_evict_move_kernel<true>), dim3((unsigned)grid), dim3(256), 0, s, a, row_pieces, shift, rows_per_chunk, (int)n_rows);
+    else hipLaunchKernelGGL((cache_evict_move_kernel<false>), dim3((unsigned)grid), dim3(256), 0, s, a, row_pieces, shift, rows_per_chunk, (int)n_rows);
     return hipGetLastError() == hipSuccess ? TRN_OK : TRN_E_LAUNCH;
 }
