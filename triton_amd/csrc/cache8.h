@@ -46,11 +46,11 @@ struct Attn8Args {
     const uint8_t *k, *v; const float *ks, *vs;
     const int32_t *lengths, *counts;
     const half_t* q; half_t* o; float* lse;
-    int B, Hq, Hkv, Sq, cap, G, R, n_rt, ns, bshift, causal;       // R = G * Sq rows in n_rt tiles; ns shares
+    int B, Hq, Hkv, Sq, cap, G, R, rshift, n_rt, ns, bshift, causal;       // R = G * Sq rows in n_rt tiles of 2^rshift; ns shares
     Div by_units, by_g, by_hkv, by_ns, by_w;
     int64_t kb, kh, kst, vb, vh, vst, ksb, ksh, vsb, vsh, qb, qh, qs, ob, oh, os;
     float c;               // scale * log2(e)
-    float *part, *ml;      // shares: [B Hkv][n_rt][ns][32][D] and [..][32][2] (m, l)
+    float *part, *ml;      // shares: [B Hkv][n_rt][ns][rows of a tile][D] and [..][rows][2] (m, l)
     float* lse2;           // [B Hkv][R]: log2 of the row sums, for the key weights (or null)
     const float* w_in; float* w_out;
     float* scores; int sp; // few rows: [B Hkv][R][sp] s = q k scale log2(e), what a row does not see -inf (or null)

@@ -1,17 +1,21 @@
 // Attention over an 8-bit key/value cache: o = softmax(scale * q (K8 ks)^T) (V8 vs), GQA / MQA, each sequence of a length of its own.
 //
-// The rows of a KV head are its query heads' queries, row r = (query r / G, head r % G): a tile of 32 of them reads the head's keys
+// The rows of a KV head are its query heads' queries, row r = (query r / G, head r % G): a tile of 16 NQ of them reads the head's keys
 // once.  A wave has such a tile and keys of its own, 32 at a time: codes come from memory straight into LDS, 16 bytes a lane and whole
-// rows, one tile ahead, and become fp16 on the way into the matrix pipe (every e4m3 number is one of fp16; queries enter as given):
-//     S^T[key][row] = K8 . Q^T              contraction 16 ks + 8 e + ..: 16-byte reads, two steps each
-//     O^T[d][row]  += V8^T[d][key] P^T      transposing 8-byte reads; the keys of a lane's scores are those of its operand
+// rows, one tile ahead, and become fp16 on the way into the matrix pipe (every e4m3 number is one of fp16; queries enter as given).
+// On the 16x16x32 MFMA, lane 16 g + n with the rows 16 qb + n:
+//     S^T(kb, qb)[key][row] = K8[16 kb + key] . Q[16 qb + row]          16-byte reads, two contraction steps each; the lane receives the
+//                                                                      keys 16 kb + 4 g ..+3
+//     O^T(db, qb)[d][row]  += V8^T[16 db + d][slot] P^T[slot][row]      transposing 8-byte reads; slot 8 g + j is key 4 g + j, or
+//                                                                      16 + 4 g + j - 4: the lane's own scores
 // The scales cost no work by the element.  ks is part of the factor that the scores are multiplied by for the exponential anyway, and vs
 // is added to the exponent: with t = s + log2 vs, p = 2^(t - m) is the weight of the CODES of V, and the sum of probabilities is
-// that of p / vs, one division a tile.  The reference m is a maximum of t: what counts for the output is near one in fp16, however
+// that of p / vs, one multiplication a tile.  The reference m is a maximum of t: what counts for the output is near one in fp16, however
 // much the blocks differ.  (A block whose vs is below 2^-64 adds nothing that fp16 could hold; it counts in the sum alone.)
 //
 // Waves of a workgroup, and workgroups (shares) of a row tile, have consecutive runs of the keys that its rows see; their results
 // are joined by (m, l, O) in LDS, and by a second launch.
+#include <type_traits>
 #include "cache8.h"
 
 namespace trn {
@@ -19,279 +23,320 @@ namespace trn {
 // 32 keys of K and V a wave and stage
 template <int D> constexpr int kTile = 32 * D;
 
-// Where a 16-byte chunk of a stage row lies.  A K read has 32 rows at one chunk, served 16 lanes at a time ({0-3, 12-15, 20-27} and the
-// others); a V read has the rows {0-3, 8-11} (or 4 further on) at two neighbouring chunks, served in halves of the wave.
-template <int D> __device__ __forceinline__ int k_swz(int row) { return D == 128 ? (row >> 1) & 7 : (row >> 2) & 3; }
-template <int D> __device__ __forceinline__ int v_swz(int row) { return D == 128 ? ((row & 2) | ((row >> 1) & 4)) : (row >> 2) & 2; }
+// Where a 16-byte chunk of a stage row lies.  A K read is served 16 lanes at a time ({0-3, 12-15, 20-27} and the others): the rows {0-3, 12-15} at
+// one chunk and {4-11} at its neighbour.  A V read is served in halves of the wave: the rows {0-7, 16-23} (or 8 further on) at one chunk.
+template <int D> __device__ __forceinline__ int k_swz(int row) { return D == 128 ? (row >> 1) & 7 : -(row >> 2) & 3; }
+template <int D> __device__ __forceinline__ int v_swz(int row) { return D == 128 ? ((row >> 1) & 3) | ((row >> 2) & 4) : ((row >> 2) & 1) | ((row >> 3) & 2); }
 
 #if defined(__HIP_DEVICE_COMPILE__)
-// One wave's 32 keys of K or V from key0 on: rows past the sequence's end arrive as zeros.  vo: the lane's offset in an even and in
-// an odd one of the 1 KB loads (whose rows swizzle differently).
-template <int D>
-__device__ __forceinline__ void fetch32(const uint8_t* head, int64_t pitch, int key0, int L, uint8_t* dst, int vo_even, int vo_odd) {
-    constexpr int RPI = 1024 / D;
-    const int rows = min(L - key0, 32);       // (none: nothing is read, zeros arrive)
-    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)(head + key0 * pitch), 0, rows > 0 ? (int)((rows - 1) * pitch) + D : 0, 0x00020000);
+// One wave's 32 keys of K or V at `rows`: `bytes` of them, what lies past arrives as zeros.  lo, hi: the lane's offset in the first and the other
+// half (V) or the even and odd ones (K) of the 1 KB loads, whose rows swizzle differently.
+template <int D, bool V>
+__device__ __forceinline__ void fetch32(const uint8_t* rows, int pitch, int bytes, uint8_t* dst, int lo, int hi) {
+    constexpr int RPI = 1024 / D, N = 32 / RPI;
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)rows, 0, bytes, 0x00020000);
 #pragma unroll
-    for (int n = 0; n < 32 / RPI; ++n)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(dst + n * 1024), 16, n & 1 ? vo_odd : vo_even,
-                                                 (int)(n * RPI * pitch), 0, 0);
+    for (int n = 0; n < N; ++n)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(dst + n * 1024), 16, (V ? n >= N / 2 : n & 1) ? hi : lo, n * RPI * pitch, 0, 0);
 }
 __device__ __forceinline__ uint2_t lds_read_tr8(const uint8_t* p) {
     typedef int int2_t __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr8_b64_v2i32((int2_t __attribute__((address_space(3)))*)(p)));
 }
-// Whether a byte of these is a NaN code (0x7f or 0xff).
+// Which bytes of these are a NaN code (0x7f or 0xff), by their top bits.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+__device__ __forceinline__ float4_t mfma16(half8_t a, half8_t b, float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+// Over the four lanes n, n + 16, n + 32, n + 48 of a row.
+__device__ __forceinline__ void swap_rows16(float& a, float& b) { asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b)); }
+__device__ __forceinline__ float quad_max(float x) { float a = x, b = x; swap_rows16(a, b); return half_max(fmaxf(a, b)); }
+__device__ __forceinline__ float quad_sum(float x) { float a = x, b = x; swap_rows16(a, b); return half_sum(a + b); }
 #endif
 
-template <int D, int NW>
+template <int D, int NW, int NQ>
 __global__ __launch_bounds__(NW * 64, 2) void cache8_attn_kernel(const Attn8Args a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    constexpr int NJ = D / 32;       // 16-byte K reads a lane, two contraction steps each; tiles of 32 output columns
+    constexpr int NJ = D / 64, NDB = D / 16, RT = 16 * NQ;      // 16-byte K reads a lane and key half, of two contraction steps each; output blocks
     __shared__ __attribute__((aligned(1024))) uint8_t Ks0[NW * kTile<D>];
     __shared__ __attribute__((aligned(1024))) uint8_t Ks1[NW * kTile<D>];
     __shared__ __attribute__((aligned(1024))) uint8_t Vs0[NW * kTile<D>];
     __shared__ __attribute__((aligned(1024))) uint8_t Vs1[NW * kTile<D>];
-    __shared__ float ms[NW][32], ls[NW][32], m_all[32], l_all[32];
+    __shared__ float ms[NW][RT], ls[NW][RT], m_all[RT], l_all[RT];
 
-    const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
+    const int lane = threadIdx.x & 63, n = lane & 15, g4 = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // (workgroups of one share of a head, the row tiles apart, follow each other at the distance of all shares: one XCD where that is a
-    // multiple of eight)
-    const int rt = a.by_units.of(blockIdx.x), unit = blockIdx.x - rt * a.by_units.d;
+    // multiple of eight; the last rows, which see the most keys, first)
+    const int nth = a.by_units.of(blockIdx.x), unit = blockIdx.x - nth * a.by_units.d, rt = a.n_rt - 1 - nth;
     const int bh = a.by_ns.of(unit), share = unit - bh * a.ns;
     const int b = a.by_hkv.of(bh), kvh = bh - b * a.Hkv;
 
     const int L = keys_of(a.lengths, b, a.cap), C = tokens_of(a.counts, b, a.Sq);
-    const int row = rt * 32 + n, qi = a.by_g.of(row), qg = row - qi * a.G;
-    if (a.by_g.of(rt * 32) >= C) return;                       // no row of this tile is there
-    const bool there = row < a.R && qi < C;
+    const int rows = min(a.R, C * a.G);
+    if (rt * RT >= rows) return;                               // no row of this tile is there
     const int off = L - C;                                     // causal: query i sees keys <= i + off
-    const int last = there ? (a.causal ? min(L - 1, qi + off) : L - 1) : -1;
-    const int last_q = min(a.by_g.of(min(rt * 32 + 31, a.R - 1)), C - 1);
-    const int seen = a.causal ? min(L, max(0, last_q + off + 1)) : L;       // keys that some row sees
-    const int all_see = a.causal ? min(L, a.by_g.of(rt * 32) + off + 1) : L;      // ... and that all rows there do
+    auto sees = [&](int row) { return a.causal ? min(L, max(0, a.by_g.of(row) + off + 1)) : L; };      // keys that a row sees: the first so many
+    const int seen = sees(min(rt * RT + RT - 1, rows - 1)), all_see = sees(rt * RT);      // that some row sees, and all of them
+    int last[NQ];                                              // the last key that the lane's rows see
+    bool there[NQ];
+    half8_t qB[NQ][2 * NJ];
+#pragma unroll
+    for (int qb = 0; qb < NQ; ++qb) {
+        const int row = rt * RT + 16 * qb + n, qi = a.by_g.of(row), qg = row - qi * a.G;
+        there[qb] = row < rows;
+        last[qb] = there[qb] ? sees(row) - 1 : -1;
+        const half_t* qp = a.q + (there[qb] ? b * a.qb + (int64_t)(kvh * a.G + qg) * a.qh + (int64_t)qi * a.qs : 0);
+#pragma unroll
+        for (int i = 0; i < 2 * NJ; ++i) qB[qb][i] = *reinterpret_cast<const half8_t*>(qp + 64 * (i >> 1) + 16 * g4 + 8 * (i & 1));
+    }
 
-    // This wave's tiles.
+    // This wave's tiles, and the first of them that not all rows see whole.
     const int T = (seen + 31) >> 5, w = share * NW + wave;
     const int t0 = a.by_w.of(T * w), t1 = a.by_w.of(T * (w + 1));       // (2^21 tiles and 512 waves at most)
-
-    const half_t* qp = a.q + (there ? b * a.qb + (int64_t)(kvh * a.G + qg) * a.qh + (int64_t)qi * a.qs : 0);
-    half8_t qB[2 * NJ];
-#pragma unroll
-    for (int i = 0; i < 2 * NJ; ++i) qB[i] = *reinterpret_cast<const half8_t*>(qp + 16 * (2 * (i >> 1) + h) + 8 * (i & 1));
-
-    const uint8_t* kp = a.k + b * a.kb + kvh * a.kh;
-    const uint8_t* vp = a.v + b * a.vb + kvh * a.vh;
+    const int t_mask = min(t1, max(t0, all_see >> 5)), t_part = L >> 5;
+    const int kpitch = (int)a.kst, vpitch = (int)a.vst, rest = L & 31;
+    const int k_full = 31 * kpitch + D, v_full = 31 * vpitch + D, k_part = rest ? (rest - 1) * kpitch + D : 0, v_part = rest ? (rest - 1) * vpitch + D : 0;
+    const uint8_t* kp = a.k + b * a.kb + kvh * a.kh + (int64_t)t0 * 32 * kpitch;      // of the tile that is requested next
+    const uint8_t* vp = a.v + b * a.vb + kvh * a.vh + (int64_t)t0 * 32 * vpitch;
     const float* ksp = a.ks + b * a.ksb + kvh * a.ksh;
     const float* vsp = a.vs + b * a.vsb + kvh * a.vsh;
 
     // staging: load i of a wave covers rows RPI i + lane / CPR
     constexpr int CPR = D / 16, RPI = 64 / CPR;
     const int sr = lane / CPR, sc = lane % CPR;
-    const int ko_e = (int)(sr * a.kst) + ((sc ^ k_swz<D>(sr)) << 4), ko_o = (int)(sr * a.kst) + ((sc ^ k_swz<D>(sr + RPI)) << 4);
-    const int vo_e = (int)(sr * a.vst) + ((sc ^ v_swz<D>(sr)) << 4), vo_o = (int)(sr * a.vst) + ((sc ^ v_swz<D>(sr + RPI)) << 4);
+    const int k_lo = sr * kpitch + ((sc ^ k_swz<D>(sr)) << 4), k_hi = sr * kpitch + ((sc ^ k_swz<D>(sr + RPI)) << 4);
+    const int v_lo = sr * vpitch + ((sc ^ v_swz<D>(sr)) << 4), v_hi = sr * vpitch + ((sc ^ v_swz<D>(sr + 16)) << 4);
     uint8_t* const K0 = Ks0 + wave * kTile<D>;
     uint8_t* const K1 = Ks1 + wave * kTile<D>;
     uint8_t* const V0 = Vs0 + wave * kTile<D>;
     uint8_t* const V1 = Vs1 + wave * kTile<D>;
-    // reads
-    const int kr = n * D + ((h ^ k_swz<D>(n)) << 4);
-    const int g16 = lane >> 4, ar = (lane & 15) >> 1;
-    const int vkey = 4 * h + (ar & 3) + 8 * (ar >> 2);
-    const int vr = vkey * D + (((g16 & 1) ^ v_swz<D>(vkey)) << 4) + 8 * (lane & 1);
+    // reads (the swizzles of rows 16 apart are the same for K)
+    const int kr = n * D + ((g4 ^ k_swz<D>(n)) << 4);
+    const int ar = n >> 1, vkey = 4 * g4 + (ar & 3) + 16 * (ar >> 2);
+    const int vr = vkey * D + (v_swz<D>(vkey) << 4) + 8 * (n & 1);
 
-    float16_t o[NJ];
+    const float4_t zero = {0.f, 0.f, 0.f, 0.f};
+    float4_t o[NDB][NQ];
+    float m[NQ], l[NQ];
 #pragma unroll
-    for (int i = 0; i < NJ; ++i)
+    for (int qb = 0; qb < NQ; ++qb) {
+        m[qb] = -INFINITY; l[qb] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
-    float m = -INFINITY, l = 0.f;
+        for (int i = 0; i < NDB; ++i) o[i][qb] = zero;
+    }
 
-    float sk = 0.f, sv = 0.f;        // lane i: the scales of the i-th tile of the 64 around this one
+    float c8 = 0.f, lv8 = 0.f, inv8 = 0.f;        // lane i: factor of the scores, log2 vs and 1 / vs of the i-th tile of the 64 around this one
+    float sk = 0.f, sv = 0.f;
     auto scales = [&](int t) {
         const int blk = min(t + lane, t1 - 1) >> (a.bshift - 5);
         sk = ksp[blk]; sv = vsp[blk];
     };
-    auto settle = [&] { asm volatile("" : "+v"(sk), "+v"(sv)); };       // (waited for here, not in every step)
+    auto settle = [&] {
+        const float v = fmaxf(sv, 0x1p-64f);
+        c8 = fmaxf(a.c * sk, 0x1p-100f);          // (a scale of zero: -inf stays -inf)
+        lv8 = fast_log2(v); inv8 = __builtin_amdgcn_rcpf(v);
+        asm volatile("" : "+v"(c8), "+v"(lv8), "+v"(inv8));       // (waited for here, not in every step)
+    };
+    auto of_lane = [](float x, int i) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), i)); };
 
-    auto step = [&](int t, const uint8_t* Kt, const uint8_t* Vt) __attribute__((always_inline)) {
-        const int i64 = (t - t0) & 63;
-        const float ksc = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sk), i64));
-        const float vsc = fmaxf(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sv), i64)), 0x1p-64f);
-        const float lv = fast_log2(vsc), c = a.c * ksc;
-        float16_t s;
+    auto step = [&](auto mask_tag, int t, const uint8_t* Kt, const uint8_t* Vt) __attribute__((always_inline)) {
+        constexpr bool MASK = decltype(mask_tag)::value;
+        const int i64 = (t - t0) & 63, key0 = t * 32;
+        const float c = of_lane(c8, i64), lv = of_lane(lv8, i64), inv = of_lane(inv8, i64);
+        float4_t s[2][NQ];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = 0.f;
+        for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            const uint4_t w4 = *reinterpret_cast<const uint4_t*>(Kt + (kr ^ (j << 5)));
-            s = mfma32(half_of_codes(w4.x, w4.y), qB[2 * j], s);
-            s = mfma32(half_of_codes(w4.z, w4.w), qB[2 * j + 1], s);
-        }
-        const int key0 = t * 32;
-        const bool masked = key0 + 32 > all_see;
-        if (masked) {
-            const int lim = last - key0 - 4 * h;
+            for (int j = 0; j < NJ; ++j) {
+                const uint4_t w4 = *reinterpret_cast<const uint4_t*>(Kt + kb * 16 * D + (kr ^ (j << 6)));
+                const half8_t k0 = half_of_codes(w4.x, w4.y), k1 = half_of_codes(w4.z, w4.w);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[e] = 8 * (e >> 2) + (e & 3) <= lim ? s[e] : -INFINITY;
-        }
-        if (a.scores && there) {
-            float* const to = a.scores + ((int64_t)bh * a.R + row) * a.sp + key0 + 4 * h;
+                for (int qb = 0; qb < NQ; ++qb) {
+                    s[kb][qb] = mfma16(k0, qB[qb][2 * j], j == 0 ? zero : s[kb][qb]);
+                    s[kb][qb] = mfma16(k1, qB[qb][2 * j + 1], s[kb][qb]);
+                }
+            }
+        if constexpr (MASK) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                float4_t x;
+            for (int qb = 0; qb < NQ; ++qb) {
+                const int lim = last[qb] - key0 - 4 * g4;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) x[r] = s[4 * e + r] == -INFINITY ? -INFINITY : s[4 * e + r] * c;
-                *reinterpret_cast<float4_t*>(to + 8 * e) = x;
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[kb][qb][e] = 16 * kb + e <= lim ? s[kb][qb][e] : -INFINITY;
             }
         }
-        // (the largest score times a factor that is not negative; a score of -inf stays one beside a factor of zero)
-        const float top = half_max(max16(s));
-        const float tm = top == -INFINITY ? top : __builtin_fmaf(top, c, lv);
-        if (__builtin_amdgcn_ballot_w64(tm > m + 8.f) != 0) {       // lazily: p stays below 2^8
-            const float up = fmaxf(m, tm), alpha = up == -INFINITY ? 1.f : fast_exp2(m - up);
-            m = up;
-            l *= alpha;
+        if (__builtin_expect(a.scores != nullptr, 0)) {
 #pragma unroll
-            for (int i = 0; i < NJ; ++i) o[i] = o[i] * alpha;
+            for (int qb = 0; qb < NQ; ++qb)
+                if (there[qb]) {
+                    float* const to = a.scores + ((int64_t)bh * a.R + rt * RT + 16 * qb + n) * a.sp + key0 + 4 * g4;
+#pragma unroll
+                    for (int kb = 0; kb < 2; ++kb) *reinterpret_cast<float4_t*>(to + 16 * kb) = s[kb][qb] * c;
+                }
         }
-        const float d = (m == -INFINITY ? 0.f : -m) + lv;
-        float p[16], sum = 0.f;
+        float tm[NQ];
+        bool due = false;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            p[e] = fast_exp2(__builtin_fmaf(s[e], c, d));
-            if (masked) p[e] = s[e] == -INFINITY ? 0.f : p[e];          // (-inf times a scale of zero)
+        for (int qb = 0; qb < NQ; ++qb) {
+            const float4_t &u = s[0][qb], &v = s[1][qb];
+            tm[qb] = __builtin_fmaf(max3(max3(u[0], u[1], u[2]), max3(u[3], v[0], v[1]), fmaxf(v[2], v[3])), c, lv);
+            due = due || tm[qb] > m[qb] + 8.f;
         }
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(due) != 0, 0)) {       // lazily: p stays below 2^8
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) sum += (p[e] + p[e + 1]) + (p[e + 2] + p[e + 3]);
-        l = __builtin_fmaf(sum, __builtin_amdgcn_rcpf(vsc), l);
-        half8_t pB[2];
+            for (int qb = 0; qb < NQ; ++qb) {
+                const float up = fmaxf(m[qb], quad_max(tm[qb])), alpha = up == -INFINITY ? 1.f : fast_exp2(m[qb] - up);
+                m[qb] = up;
+                l[qb] *= alpha;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) pB[e >> 3][e & 7] = (half_t)p[e];
-        // A NaN code of a key that not all rows see: a product would hand it to the rows that do not (0 * NaN).  It is taken out,
-        // and the rows that see it get it in its columns.
-        uint2_t vw[NJ][2];
+                for (int i = 0; i < NDB; ++i) o[i][qb] = o[i][qb] * alpha;
+            }
+        }
+        half8_t p[NQ];
+#pragma unroll
+        for (int qb = 0; qb < NQ; ++qb) {
+            const float d = (m[qb] == -INFINITY ? 0.f : -m[qb]) + lv;
+            float sum[2];
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { x[e] = fast_exp2(__builtin_fmaf(s[kb][qb][e], c, d)); p[qb][4 * kb + e] = (half_t)x[e]; }
+                sum[kb] = (x[0] + x[1]) + (x[2] + x[3]);
+            }
+            l[qb] = __builtin_fmaf(sum[0] + sum[1], inv, l[qb]);
+        }
+        uint2_t vw[NDB];
         uint32_t bad = 0;
 #pragma unroll
-        for (int i = 0; i < NJ; ++i)
+        for (int i = 0; i < NDB; ++i) {
+            vw[i] = lds_read_tr8(Vt + (vr ^ (i << 4)));
+            if constexpr (MASK) bad |= nan_bytes(vw[i].x) | nan_bytes(vw[i].y);
+        }
+        // A NaN code of a key that not all rows see: a product would hand it to the rows that do not (0 * NaN).  It is taken out,
+        // and the rows that see it get it in its columns.
+        if constexpr (MASK) {
+            if (__builtin_expect(__builtin_amdgcn_ballot_w64(bad != 0) != 0, 0)) {
+                const half_t one = (half_t)1.f, nil = (half_t)0.f;
 #pragma unroll
-            for (int k2 = 0; k2 < 2; ++k2) {
-                vw[i][k2] = lds_read_tr8(Vt + (vr ^ (i << 5)) + k2 * 16 * D);
-                if (masked) bad |= nan_bytes(vw[i][k2].x) | nan_bytes(vw[i][k2].y);
-            }
-        if (masked && __builtin_amdgcn_ballot_w64(bad != 0) != 0) {
-            const half_t one = (half_t)1.f, nil = (half_t)0.f;
-            const int lim = last - key0 - 4 * h;
+                for (int i = 0; i < NDB; ++i) {
+                    const uint32_t nx = nan_bytes(vw[i].x), ny = nan_bytes(vw[i].y);
+                    half8_t is;
 #pragma unroll
-            for (int i = 0; i < NJ; ++i) {
-                float16_t hit;
+                    for (int e = 0; e < 8; ++e) is[e] = ((e < 4 ? nx : ny) >> (8 * (e & 3)) & 0x80u) ? one : nil;
+                    vw[i].x &= ~((nx >> 7) * 0xffu); vw[i].y &= ~((ny >> 7) * 0xffu);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) hit[e] = 0.f;
+                    for (int qb = 0; qb < NQ; ++qb) {
+                        const int lim = last[qb] - key0 - 4 * g4;
+                        half8_t see;
 #pragma unroll
-                for (int k2 = 0; k2 < 2; ++k2) {
-                    const uint32_t nx = nan_bytes(vw[i][k2].x), ny = nan_bytes(vw[i][k2].y);
-                    half8_t is, sees;
+                        for (int e = 0; e < 8; ++e) see[e] = 16 * (e >> 2) + (e & 3) <= lim ? one : nil;
+                        const float4_t hit = mfma16(is, see, zero);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        is[e] = ((e < 4 ? nx : ny) >> (8 * (e & 3)) & 0x80u) ? one : nil;
-                        const int key = 16 * k2 + 8 * (e >> 2) + (e & 3);
-                        sees[e] = key <= lim ? one : nil;
+                        for (int e = 0; e < 4; ++e) o[i][qb][e] = hit[e] > 0.f ? NAN : o[i][qb][e];
                     }
-                    hit = mfma32(is, sees, hit);
-                    vw[i][k2].x &= ~((nx >> 7) * 0xffu); vw[i][k2].y &= ~((ny >> 7) * 0xffu);
                 }
-#pragma unroll
-                for (int e = 0; e < 16; ++e) o[i][e] = hit[e] > 0.f ? NAN : o[i][e];
             }
         }
 #pragma unroll
-        for (int i = 0; i < NJ; ++i)
+        for (int i = 0; i < NDB; ++i) {
+            const half8_t v = half_of_codes(vw[i].x, vw[i].y);
 #pragma unroll
-            for (int k2 = 0; k2 < 2; ++k2) o[i] = mfma32(half_of_codes(vw[i][k2].x, vw[i][k2].y), pB[k2], o[i]);
+            for (int qb = 0; qb < NQ; ++qb) o[i][qb] = mfma16(v, p[qb], o[i][qb]);
+        }
     };
     // Everything of the stage that the next load overwrites has been read: its values are in registers before the load goes out.
     auto ahead = [&](int t, uint8_t* Kt, uint8_t* Vt) __attribute__((always_inline)) {
         __builtin_amdgcn_sched_barrier(0);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        const int end = t < t1 ? L : 0;
-        fetch32<D>(kp, a.kst, t * 32, end, Kt, ko_e, ko_o);
-        fetch32<D>(vp, a.vst, t * 32, end, Vt, vo_e, vo_o);
+        const bool full = t < t_part, any = t < t1;
+        fetch32<D, false>(kp, kpitch, any ? (full ? k_full : k_part) : 0, Kt, k_lo, k_hi);      // (none: nothing is read, zeros arrive)
+        fetch32<D, true>(vp, vpitch, any ? (full ? v_full : v_part) : 0, Vt, v_lo, v_hi);
+        kp += 32 * (int64_t)kpitch; vp += 32 * (int64_t)vpitch;
         __builtin_amdgcn_sched_barrier(0);
     };
     auto arrived = [&] {       // the tile before the one that was requested last
         if constexpr (D == 128) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
         else asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
     };
+    const std::false_type whole{};
+    const std::true_type partly{};
     if (t0 < t1) {
         scales(t0);
         ahead(t0, K0, V0);
         settle();
 #pragma unroll
-        for (int i = 0; i < 2 * NJ; ++i) {
-            half8_t z = {};
-            qB[i] = there ? qB[i] : z;
+        for (int qb = 0; qb < NQ; ++qb)
+#pragma unroll
+            for (int i = 0; i < 2 * NJ; ++i) {
+                const half8_t z = {};
+                qB[qb][i] = there[qb] ? qB[qb][i] : z;
+            }
+        int t = t0;
+        for (; t + 2 <= t_mask; t += 2) {
+            if (__builtin_expect(t > t0 && ((t - t0) & 63) == 0, 0)) { scales(t); settle(); }
+            ahead(t + 1, K1, V1);
+            arrived();
+            step(whole, t, K0, V0);
+            ahead(t + 2, K0, V0);
+            arrived();
+            step(whole, t + 1, K1, V1);
         }
-        for (int t = t0; t < t1; t += 2) {
+        for (; t < t1; t += 2) {
             if (t > t0 && ((t - t0) & 63) == 0) { scales(t); settle(); }
             ahead(t + 1, K1, V1);
             arrived();
-            step(t, K0, V0);
+            step(partly, t, K0, V0);
             ahead(t + 2, K0, V0);
             arrived();
-            if (t + 1 < t1) step(t + 1, K1, V1);
+            if (t + 1 < t1) step(partly, t + 1, K1, V1);
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
-    l = half_sum(l);
 
     // ---- the waves' results
-    if (h == 0) { ms[wave][n] = m; ls[wave][n] = l; }
+#pragma unroll
+    for (int qb = 0; qb < NQ; ++qb) {
+        l[qb] = quad_sum(l[qb]);
+        if (g4 == 0) { ms[wave][16 * qb + n] = m[qb]; ls[wave][16 * qb + n] = l[qb]; }
+    }
     __syncthreads();
-    float top = -INFINITY, sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < NW; ++i) top = fmaxf(top, ms[i][n]);
-#pragma unroll
-    for (int i = 0; i < NW; ++i) sum = __builtin_fmaf(ls[i][n], ms[i][n] == -INFINITY ? 0.f : fast_exp2(ms[i][n] - top), sum);      // (a sum of NaN stays)
-    const float mine = m == -INFINITY ? 0.f : fast_exp2(m - top);
-    // (a stage array holds 32 rows of D floats of one wave in four; the 16-byte pieces of a row are swizzled by the row)
+    // (a stage array holds RT rows of D floats of one wave in four; the 16-byte pieces of a row are swizzled by the row)
     auto area = [&](int i) __attribute__((always_inline)) {
         uint8_t* const base = i % 4 == 0 ? Ks0 : i % 4 == 1 ? Ks1 : i % 4 == 2 ? Vs0 : Vs1;
-        return reinterpret_cast<float4_t*>(base + (i / 4) * 32 * D * 4);
+        return reinterpret_cast<float4_t*>(base + (i / 4) * RT * D * 4);
     };
-    {
-        float4_t* const mem = area(wave);
+    float4_t* const mem = area(wave);
 #pragma unroll
-        for (int i = 0; i < NJ; ++i)
+    for (int qb = 0; qb < NQ; ++qb) {
+        const int r = 16 * qb + n;
+        float top = -INFINITY, sum = 0.f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int piece = 8 * i + 2 * e + h;               // columns 32 i + 8 e + 4 h ..
-                float4_t x;
+        for (int i = 0; i < NW; ++i) top = fmaxf(top, ms[i][r]);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) x[r] = o[i][4 * e + r] * mine;
-                mem[n * (D / 4) + (piece ^ (n & 15))] = x;
-            }
+        for (int i = 0; i < NW; ++i) sum = __builtin_fmaf(ls[i][r], ms[i][r] == -INFINITY ? 0.f : fast_exp2(ms[i][r] - top), sum);      // (a sum of NaN stays)
+        const float mine = m[qb] == -INFINITY ? 0.f : fast_exp2(m[qb] - top);
+#pragma unroll
+        for (int i = 0; i < NDB; ++i) mem[r * (D / 4) + ((4 * i + g4) ^ n)] = o[i][qb] * mine;
+        if (wave == 0 && g4 == 0) { m_all[r] = top; l_all[r] = sum; }
     }
-    if (wave == 0 && h == 0) { m_all[n] = top; l_all[n] = sum; }
     __syncthreads();
-    constexpr int TPR = NW * 64 / 32, NP = D / 4 / TPR;                // threads a row, 16-byte pieces a thread
-    static_assert(NP >= 1, "a row's pieces for its threads");
+    constexpr int TPR = NW * 64 / RT, NP = D / 4 / TPR;                // threads a row, 16-byte pieces a thread
+    static_assert(NP >= 1 && D / 4 >= 16, "a row's pieces for its threads, and for the swizzle");
     const int orow = threadIdx.x / TPR, sub = threadIdx.x % TPR;
-    const int r = rt * 32 + orow, i0 = a.by_g.of(r), g0 = r - i0 * a.G;
-    if (r >= a.R || i0 >= C) return;
+    const int r = rt * RT + orow, i0 = a.by_g.of(r), g0 = r - i0 * a.G;
+    if (r >= rows) return;
     const float rm = m_all[orow], rl = l_all[orow];
     const float inv = rl == 0.f ? 0.f : 1.f / rl;
+    const int64_t at = (((int64_t)bh * a.n_rt + rt) * a.ns + share) * RT + orow;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
         const int piece = sub + i * TPR;
-        float4_t x = {0.f, 0.f, 0.f, 0.f};
+        float4_t x = zero;
 #pragma unroll
         for (int k2 = 0; k2 < NW; ++k2) x = x + area(k2)[orow * (D / 4) + (piece ^ (orow & 15))];
-        if (a.ns > 1) {
-            const int64_t at = ((int64_t)bh * a.n_rt + rt) * a.ns + share;
-            *reinterpret_cast<float4_t*>(a.part + (at * 32 + orow) * D + 4 * piece) = x;
-        } else {
+        if (a.ns > 1) *reinterpret_cast<float4_t*>(a.part + at * D + 4 * piece) = x;
+        else {
             half4_t y;
 #pragma unroll
             for (int e = 0; e < 4; ++e) y[e] = (half_t)(x[e] * inv);
@@ -299,10 +344,8 @@ __global__ __launch_bounds__(NW * 64, 2) void cache8_attn_kernel(const Attn8Args
         }
     }
     if (sub == 0) {
-        if (a.ns > 1) {
-            float* const to = a.ml + ((((int64_t)bh * a.n_rt + rt) * a.ns + share) * 32 + orow) * 2;
-            to[0] = rm; to[1] = rl;
-        } else {
+        if (a.ns > 1) { a.ml[at * 2] = rm; a.ml[at * 2 + 1] = rl; }
+        else {
             const float x = rm + fast_log2(rl);            // (-inf for a row that sees nothing)
             if (a.lse) a.lse[((int64_t)b * a.Hq + kvh * a.G + g0) * a.Sq + i0] = x * kLn2;
             if (a.lse2) a.lse2[(int64_t)bh * a.R + r] = x;
@@ -312,35 +355,41 @@ __global__ __launch_bounds__(NW * 64, 2) void cache8_attn_kernel(const Attn8Args
 }
 
 // ------------------------------------------------------------------------------------------------ host
-struct Plan8 { int G, R, n_rt, ns, n_chunks, chunk_tiles, sp; int64_t ml, lse2, more, bytes; };
+struct Plan8 { int G, R, nq, nw, n_rt, ns, n_chunks, chunk_tiles, sp; int64_t ml, lse2, more, bytes; };
 
-// How many workgroups share the keys of a row tile: two a compute unit over the launch, as long as a wave has two tiles.
+// Rows of a tile, waves of a workgroup, and how many workgroups share the keys of a row tile: two a compute unit over the launch, as long as a wave
+// has two tiles.
 static Plan8 plan8(const trn_cache8* c, int Hq, int Sq, bool weights) {
     Plan8 p;
     p.G = Hq / c->n_kv_heads;
     p.R = p.G * Sq;
-    p.n_rt = (p.R + 31) / 32;
+    p.nq = p.R <= 16 ? 1 : 2;
+    p.nw = 4;
+    // PLAN1
+    p.n_rt = (p.R + 16 * p.nq - 1) / (16 * p.nq);
     const int64_t heads = (int64_t)c->batch * c->n_kv_heads, units = heads * p.n_rt, tiles = (c->capacity + 31) / 32;
     int64_t ns = units ? 512 / units : 1;
     if (ns > tiles / 8) ns = tiles / 8;
     p.ns = (int)(ns < 1 ? 1 : ns > 64 ? 64 : ns);
+    // PLAN
     auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
-    p.ml = p.ns > 1 ? up(units * p.ns * 32 * c->head_dim * 4) : 0;
-    p.lse2 = p.ml + (p.ns > 1 ? up(units * p.ns * 64 * 4) : 0);
+    p.ml = p.ns > 1 ? up(units * p.ns * 16 * p.nq * c->head_dim * 4) : 0;
+    p.lse2 = p.ml + (p.ns > 1 ? up(units * p.ns * 32 * p.nq * 4) : 0);
     p.more = p.lse2 + (weights ? up(heads * p.R * 4) : 0);
     p.bytes = p.more;
     // Key weights: a score of 4 bytes goes out and comes back for each row and key, or K is read again.
     p.sp = weights && 8 * p.R <= c->head_dim ? (int)tiles * 32 : 0;
-    p.n_chunks = 1; p.chunk_tiles = p.n_rt;
+    const int tiles32 = (p.R + 31) / 32;
+    p.n_chunks = 1; p.chunk_tiles = tiles32;
     if (p.sp) p.bytes += up(heads * p.R * p.sp * 4);
     else if (weights) {
         // (four workgroups a compute unit, a chunk of four row tiles at least)
         const int64_t blocks = heads * ((c->capacity + 255) / 256);
         int64_t chunks = blocks ? 1024 / blocks : 1;
-        if (chunks > p.n_rt / 4) chunks = p.n_rt / 4;
+        if (chunks > tiles32 / 4) chunks = tiles32 / 4;
         if (chunks > 1) {
-            p.chunk_tiles = (int)((p.n_rt + chunks - 1) / chunks);
-            p.n_chunks = (p.n_rt + p.chunk_tiles - 1) / p.chunk_tiles;
+            p.chunk_tiles = (int)((tiles32 + chunks - 1) / chunks);
+            p.n_chunks = (tiles32 + p.chunk_tiles - 1) / p.chunk_tiles;
             if (p.n_chunks > 1) p.bytes += up(p.n_chunks * heads * c->capacity * 4);
         }
     }
@@ -388,11 +437,11 @@ extern "C" int trn_cache8_attn_f16(const trn_cache8* c, const void* q, void* o, 
     a.lengths = c->lengths; a.counts = c->counts;
     a.q = (const half_t*)q; a.o = (half_t*)o; a.lse = lse;
     a.B = c->batch; a.Hq = n_q_heads; a.Hkv = c->n_kv_heads; a.Sq = seq_q; a.cap = c->capacity;
-    a.G = p.G; a.R = p.R; a.n_rt = p.n_rt; a.ns = p.ns; a.causal = causal != 0;
+    a.G = p.G; a.R = p.R; a.n_rt = p.n_rt; a.rshift = p.nq == 1 ? 4 : 5; a.ns = p.ns; a.causal = causal != 0;
     a.bshift = c->block == 32 ? 5 : c->block == 64 ? 6 : 7;
     const int64_t heads = (int64_t)c->batch * c->n_kv_heads, units = heads * p.ns;
     if (units * p.n_rt > 0x7fffffffLL || heads * ((int64_t)p.R + 1) > 0x7fffffffLL || heads * ((c->capacity + 255) / 256) * p.n_chunks > 0x3fffffffLL) return TRN_E_SHAPE;
-    a.by_units = Div(units); a.by_g = Div(p.G); a.by_hkv = Div(c->n_kv_heads); a.by_ns = Div(p.ns); a.by_w = Div(4 * p.ns);
+    a.by_units = Div(units); a.by_g = Div(p.G); a.by_hkv = Div(c->n_kv_heads); a.by_ns = Div(p.ns); a.by_w = Div(p.nw * p.ns);
     a.kb = c->k_stride_b; a.kh = c->k_stride_h; a.kst = c->k_stride_s;
     a.vb = c->v_stride_b; a.vh = c->v_stride_h; a.vst = c->v_stride_s;
     a.ksb = c->ks_stride_b; a.ksh = c->ks_stride_h; a.vsb = c->vs_stride_b; a.vsh = c->vs_stride_h;
@@ -405,8 +454,13 @@ extern "C" int trn_cache8_attn_f16(const trn_cache8* c, const void* q, void* o, 
     a.n_chunks = p.n_chunks; a.chunk_tiles = p.chunk_tiles; a.w_part = p.n_chunks > 1 ? (float*)((char*)workspace + p.more) : nullptr;
     const hipStream_t s = (hipStream_t)stream;
     const bool d128 = c->head_dim == 128;
-    if (d128) hipLaunchKernelGGL((cache8_attn_kernel<128, 4>), dim3((unsigned)(units * p.n_rt)), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((cache8_attn_kernel<64, 4>), dim3((unsigned)(units * p.n_rt)), dim3(256), 0, s, a);
+    const dim3 grid((unsigned)(units * p.n_rt)), block(p.nw * 64);
+#define TRN_ATTN8(D, NW, NQ) hipLaunchKernelGGL((cache8_attn_kernel<D, NW, NQ>), grid, block, 0, s, a)
+    if (d128 && p.nq == 1) TRN_ATTN8(128, 4, 1);
+    else if (d128) TRN_ATTN8(128, 4, 2);
+    else if (p.nq == 1) TRN_ATTN8(64, 4, 1);
+    else TRN_ATTN8(64, 4, 2);
+#undef TRN_ATTN8
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && (p.ns > 1 || p.sp)) e = launch_cache8_finish(a, c->head_dim, s);
     if (e == hipSuccess && weights_out && !p.sp && c->capacity > 0) e = launch_cache8_weights(a, c->head_dim, s);

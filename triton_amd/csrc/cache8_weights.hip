@@ -7,8 +7,8 @@
 namespace trn {
 
 // (m, l) of a row's shares, a lane each: the factors by which they count, the row's sum, and log2 of it.
-__device__ __forceinline__ void join_row(const Attn8Args& a, int64_t at, int r32, int lane, float& f, float& l, float& l2) {
-    const float2_t x = lane < a.ns ? *reinterpret_cast<const float2_t*>(a.ml + ((at + lane) * 32 + r32) * 2) : float2_t{-INFINITY, 0.f};
+__device__ __forceinline__ void join_row(const Attn8Args& a, int bh, int r, int lane, float& f, float& l, float& l2) {
+    const float2_t x = lane < a.ns ? *reinterpret_cast<const float2_t*>(a.ml + (((((int64_t)bh * a.n_rt + (r >> a.rshift)) * a.ns + lane) << a.rshift) + (r & ((1 << a.rshift) - 1))) * 2) : float2_t{-INFINITY, 0.f};
     float top = x.x;
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
@@ -36,7 +36,7 @@ __global__ __launch_bounds__(256) void cache8_finish_kernel(const Attn8Args a, i
             const int r = r0 + i;
             if (r >= there) break;
             float f, l, l2;
-            join_row(a, ((int64_t)bh * a.n_rt + (r >> 5)) * a.ns, r & 31, lane, f, l, l2);
+            join_row(a, bh, r, lane, f, l, l2);
             fs[i][lane] = f;
             if (lane == 0) {
                 inv[i] = l == 0.f ? 0.f : 1.f / l;
@@ -50,9 +50,9 @@ __global__ __launch_bounds__(256) void cache8_finish_kernel(const Attn8Args a, i
         const bool mine = r < there;
         float4_t x = {0.f, 0.f, 0.f, 0.f};
         if (mine) {
-            const float* part = a.part + ((((int64_t)bh * a.n_rt + (r >> 5)) * a.ns) * 32 + (r & 31)) * D + 4 * piece;
+            const float* part = a.part + (((((int64_t)bh * a.n_rt + (r >> a.rshift)) * a.ns) << a.rshift) + (r & ((1 << a.rshift) - 1))) * D + 4 * piece;
 #pragma unroll 4
-            for (int k = nth; k < a.ns; k += sg) x = x + *reinterpret_cast<const float4_t*>(part + (int64_t)k * 32 * D) * fs[i][k];
+            for (int k = nth; k < a.ns; k += sg) x = x + *reinterpret_cast<const float4_t*>(part + ((int64_t)k << a.rshift) * D) * fs[i][k];
         }
         if (sg > 1) {
             red[tid] = x;
@@ -73,7 +73,7 @@ __global__ __launch_bounds__(256) void cache8_finish_kernel(const Attn8Args a, i
     if (key0 >= L) return;
     for (int r = wave; r < rows; r += 4) {
         float f, l, l2;
-        if (a.ns > 1) join_row(a, (int64_t)bh * a.n_rt * a.ns, r, lane, f, l, l2);
+        if (a.ns > 1) join_row(a, bh, r, lane, f, l, l2);
         else l2 = a.lse2[(int64_t)bh * a.R + r];
         if (lane == 0) inv[r] = l2;
     }
