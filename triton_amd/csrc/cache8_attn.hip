@@ -30,14 +30,14 @@ template <int D> __device__ __forceinline__ int v_swz(int row) { return D == 128
 
 #if defined(__HIP_DEVICE_COMPILE__)
 // One wave's 32 keys of K or V at `rows`: `bytes` of them, what lies past arrives as zeros.  lo, hi: the lane's offset in the first and the other
-// half (V) or the even and odd ones (K) of the 1 KB loads, whose rows swizzle differently.
-template <int D, bool V>
+// half (V) or the even and odd ones (K) of the 1 KB loads, whose rows swizzle differently.  PAST: past the caches.
+template <int D, bool V, bool PAST>
 __device__ __forceinline__ void fetch32(const uint8_t* rows, int pitch, int bytes, uint8_t* dst, int lo, int hi) {
     constexpr int RPI = 1024 / D, N = 32 / RPI;
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)rows, 0, bytes, 0x00020000);
 #pragma unroll
     for (int n = 0; n < N; ++n)
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(dst + n * 1024), 16, (V ? n >= N / 2 : n & 1) ? hi : lo, n * RPI * pitch, 0, 0);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)(dst + n * 1024), 16, (V ? n >= N / 2 : n & 1) ? hi : lo, n * RPI * pitch, 0, PAST ? 2 : 0);
 }
 __device__ __forceinline__ uint2_t lds_read_tr8(const uint8_t* p) {
     typedef int int2_t __attribute__((ext_vector_type(2)));
@@ -52,7 +52,8 @@ __device__ __forceinline__ float quad_max(float x) { float a = x, b = x; swap_ro
 __device__ __forceinline__ float quad_sum(float x) { float a = x, b = x; swap_rows16(a, b); return half_sum(a + b); }
 #endif
 
-template <int D, int NW, int NQ>
+// PAST: a single row tile reads the cache, each byte once (see plan8).
+template <int D, int NW, int NQ, bool PAST>
 __global__ __launch_bounds__(NW * 64, 2) void cache8_attn_kernel(const Attn8Args a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr int NJ = D / 64, NDB = D / 16, RT = 16 * NQ;      // 16-byte K reads a lane and key half, of two contraction steps each; output blocks
@@ -250,8 +251,8 @@ __global__ __launch_bounds__(NW * 64, 2) void cache8_attn_kernel(const Attn8Args
         __builtin_amdgcn_sched_barrier(0);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         const bool full = t < t_part, any = t < t1;
-        fetch32<D, false>(kp, kpitch, any ? (full ? k_full : k_part) : 0, Kt, k_lo, k_hi);      // (none: nothing is read, zeros arrive)
-        fetch32<D, true>(vp, vpitch, any ? (full ? v_full : v_part) : 0, Vt, v_lo, v_hi);
+        fetch32<D, false, PAST>(kp, kpitch, any ? (full ? k_full : k_part) : 0, Kt, k_lo, k_hi);      // (none: nothing is read, zeros arrive)
+        fetch32<D, true, PAST>(vp, vpitch, any ? (full ? v_full : v_part) : 0, Vt, v_lo, v_hi);
         kp += 32 * (int64_t)kpitch; vp += 32 * (int64_t)vpitch;
         __builtin_amdgcn_sched_barrier(0);
     };
@@ -357,19 +358,33 @@ __global__ __launch_bounds__(NW * 64, 2) void cache8_attn_kernel(const Attn8Args
 // ------------------------------------------------------------------------------------------------ host
 struct Plan8 { int G, R, nq, nw, n_rt, ns, n_chunks, chunk_tiles, sp; int64_t ml, lse2, more, bytes; };
 
-// Rows of a tile, waves of a workgroup, and how many workgroups share the keys of a row tile: two a compute unit over the launch, as long as a wave
-// has two tiles.
+// Rows of a tile: 32 where they make workgroups enough, otherwise 16, whose waves have half the work a key and need half the registers.  us, tiles of
+// 16 / 32 rows, each with its best number of shares: 16 heads of 64, batch 4, 2000 keys, 64 queries (128 tiles of 32) 10.2 / 13.0, 300 (640) 23.6 / 21.6; 71
+// heads on one, batch 8, 16 queries (288) 23.0 / 22.7; 32 heads of 128 on 8: batch 4, 8 queries, 2000 keys (32) 12.8 / 13.5, batch 16, 4000 keys (128) 31.7 / 28.9;
+// one prompt of 1501 (1504) 49 / 37.
+// Shares of a row tile's keys: one workgroup a compute unit over the launch -- one share from some 160 row tiles on --, no more shares than tiles of 32 keys.  32 heads
+// of 128 on 8, one query, us with 1 / 2 / 4 / 8 / 16 / 32 shares: 1025 keys 9.6 / 10.9 / 9.5 / 9.3 / 9.0 / 8.9; batch 8, 1500 keys 12.0 / 12.4 / 11.9 / 12.5 / 16.6; batch 12, 3000
+// 23.7 / 19.5 / 20.8; batch 16, 4097 31.3 / 28.6 / 28.4; batch 24, 4000 33.9 / 41.6 / 39.9; batch 32, 8192 88.7 / 91.4 / 93.8; of two to one lengths 70.5 / 72.2 / 70.8.  A
+// second launch is some 3 us: without weights, which need it anyway, short caches have one share (512 keys 6.4, against 8.5; batch 8: 1025 keys 10.1 / 11.0; 16
+// heads of 64: 1025 keys 7.6 / 8.1, 2000 10.7 / 8.3).  Tiles of more than one read no more from memory than one does, and their waves rather
+// have a second workgroup beside them than walk long: 16 heads of 64, batch 4, 8000 keys, 20 queries 26.3 with two shares, 23.3 with four.
+// A cache that is read by one row tile goes past the caches (each byte once), us through / past: batch 32, 8192 keys 99.5 / 89.4, one sequence of 131072 56.7 /
+// 51.2, of 4000 11.2 / 10.6; with two row tiles and more the others find it there: 64 rows, 16000 keys 18.7 / 20.6.
 static Plan8 plan8(const trn_cache8* c, int Hq, int Sq, bool weights) {
     Plan8 p;
+    const bool d128 = c->head_dim == 128;
     p.G = Hq / c->n_kv_heads;
     p.R = p.G * Sq;
-    p.nq = p.R <= 16 ? 1 : 2;
+    const int64_t heads = (int64_t)c->batch * c->n_kv_heads, tiles = (c->capacity + 31) / 32;
+    p.nq = p.R > 16 && heads * ((p.R + 31) / 32) >= (d128 ? 128 : 256) ? 2 : 1;
     p.nw = 4;
     // PLAN1
     p.n_rt = (p.R + 16 * p.nq - 1) / (16 * p.nq);
-    const int64_t heads = (int64_t)c->batch * c->n_kv_heads, units = heads * p.n_rt, tiles = (c->capacity + 31) / 32;
-    int64_t ns = units ? 512 / units : 1;
-    if (ns > tiles / 8) ns = tiles / 8;
+    const int64_t units = heads * p.n_rt;
+    int64_t ns = units ? 256 / units : 1;
+    if (p.n_rt > 1 && ns >= 1 && tiles > 24 * p.nw * ns) ns *= 2;
+    if (!weights && tiles <= (d128 ? 26 : 34) + units / 4) ns = 1;
+    if (ns > tiles) ns = tiles;
     p.ns = (int)(ns < 1 ? 1 : ns > 64 ? 64 : ns);
     // PLAN
     auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
@@ -455,7 +470,8 @@ extern "C" int trn_cache8_attn_f16(const trn_cache8* c, const void* q, void* o, 
     const hipStream_t s = (hipStream_t)stream;
     const bool d128 = c->head_dim == 128;
     const dim3 grid((unsigned)(units * p.n_rt)), block(p.nw * 64);
-#define TRN_ATTN8(D, NW, NQ) hipLaunchKernelGGL((cache8_attn_kernel<D, NW, NQ>), grid, block, 0, s, a)
+#define TRN_ATTN8(D, NW, NQ) do { if (p.n_rt == 1) hipLaunchKernelGGL((cache8_attn_kernel<D, NW, NQ, true>), grid, block, 0, s, a); \
+                                  else hipLaunchKernelGGL((cache8_attn_kernel<D, NW, NQ, false>), grid, block, 0, s, a); } while (0)
     if (d128 && p.nq == 1) TRN_ATTN8(128, 4, 1);
     else if (d128) TRN_ATTN8(128, 4, 2);
     else if (p.nq == 1) TRN_ATTN8(64, 4, 1);
