@@ -143,12 +143,22 @@ __global__ __launch_bounds__(NW * 64, 2) void cache8_attn_kernel(const Attn8Args
         constexpr bool MASK = decltype(mask_tag)::value;
         const int i64 = (t - t0) & 63, key0 = t * 32;
         const float c = of_lane(c8, i64), lv = of_lane(lv8, i64), inv = of_lane(inv8, i64);
+        // (all codes of the tile are requested at once: left to the compiler each of V's reads came right before its products, and was waited for)
+        uint4_t kw[2][NJ];
+        uint2_t vw[NDB];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) kw[kb][j] = *reinterpret_cast<const uint4_t*>(Kt + kb * 16 * D + (kr ^ (j << 6)));
+#pragma unroll
+        for (int i = 0; i < NDB; ++i) vw[i] = lds_read_tr8(Vt + (vr ^ (i << 4)));
+        __builtin_amdgcn_sched_barrier(0);
         float4_t s[2][NQ];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
-                const uint4_t w4 = *reinterpret_cast<const uint4_t*>(Kt + kb * 16 * D + (kr ^ (j << 6)));
+                const uint4_t w4 = kw[kb][j];
                 const half8_t k0 = half_of_codes(w4.x, w4.y), k1 = half_of_codes(w4.z, w4.w);
 #pragma unroll
                 for (int qb = 0; qb < NQ; ++qb) {
@@ -207,12 +217,10 @@ __global__ __launch_bounds__(NW * 64, 2) void cache8_attn_kernel(const Attn8Args
             }
             l[qb] = __builtin_fmaf(sum[0] + sum[1], inv, l[qb]);
         }
-        uint2_t vw[NDB];
         uint32_t bad = 0;
+        if constexpr (MASK) {
 #pragma unroll
-        for (int i = 0; i < NDB; ++i) {
-            vw[i] = lds_read_tr8(Vt + (vr ^ (i << 4)));
-            if constexpr (MASK) bad |= nan_bytes(vw[i].x) | nan_bytes(vw[i].y);
+            for (int i = 0; i < NDB; ++i) bad |= nan_bytes(vw[i].x) | nan_bytes(vw[i].y);
         }
         // A NaN code of a key that not all rows see: a product would hand it to the rows that do not (0 * NaN).  It is taken out,
         // and the rows that see it get it in its columns.
