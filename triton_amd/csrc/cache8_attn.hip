@@ -368,7 +368,7 @@ struct Plan8 { int G, R, nq, nw, n_rt, ns, n_chunks, chunk_tiles, sp; int64_t ml
 
 // Rows of a tile: 32 where they make workgroups enough, otherwise 16, whose waves have half the work a key and need half the registers.  us, tiles of
 // 16 / 32 rows, each with its best number of shares: 16 heads of 64, batch 4, 2000 keys, 64 queries (128 tiles of 32) 10.2 / 13.0, 300 (640) 23.6 / 21.6; 71
-// heads on one, batch 8, 16 queries (288) 23.0 / 22.7; 32 heads of 128 on 8: batch 4, 8 queries, 2000 keys (32) 12.8 / 13.5, batch 16, 4000 keys (128) 31.7 / 28.9;
+// heads on one, batch 8, 16 queries (288) 21.9 / 23.4, one sequence, 200 (444) 27.6 / 22.8; 32 heads of 128 on 8: batch 4, 8 queries, 2000 keys (32) 12.8 / 13.5, batch 16, 4000 keys (128) 31.7 / 28.9;
 // one prompt of 1501 (1504) 49 / 37.
 // Shares of a row tile's keys: one workgroup a compute unit over the launch -- one share from some 160 row tiles on --, no more shares than tiles of 32 keys.  32 heads
 // of 128 on 8, one query, us with 1 / 2 / 4 / 8 / 16 / 32 shares: 1025 keys 9.6 / 10.9 / 9.5 / 9.3 / 9.0 / 8.9; batch 8, 1500 keys 12.0 / 12.4 / 11.9 / 12.5 / 16.6; batch 12, 3000
@@ -384,7 +384,7 @@ static Plan8 plan8(const trn_cache8* c, int Hq, int Sq, bool weights) {
     p.G = Hq / c->n_kv_heads;
     p.R = p.G * Sq;
     const int64_t heads = (int64_t)c->batch * c->n_kv_heads, tiles = (c->capacity + 31) / 32;
-    p.nq = p.R > 16 && heads * ((p.R + 31) / 32) >= (d128 ? 128 : 256) ? 2 : 1;
+    p.nq = p.R > 16 && heads * ((p.R + 31) / 32) >= (d128 ? 128 : 320) ? 2 : 1;
     p.nw = 4;
     // PLAN1
     p.n_rt = (p.R + 16 * p.nq - 1) / (16 * p.nq);
@@ -406,9 +406,10 @@ static Plan8 plan8(const trn_cache8* c, int Hq, int Sq, bool weights) {
     p.n_chunks = 1; p.chunk_tiles = tiles32;
     if (p.sp) p.bytes += up(heads * p.R * p.sp * 4);
     else if (weights) {
-        // (four workgroups a compute unit, a chunk of four row tiles at least)
+        // (three workgroups a compute unit, a chunk of four row tiles at least: a prompt of 1501, 32 heads of 128 on 8, us a call with one / two / three / four /
+        // six 86 / 75 / 72 / 77 / 81)
         const int64_t blocks = heads * ((c->capacity + 255) / 256);
-        int64_t chunks = blocks ? 1024 / blocks : 1;
+        int64_t chunks = blocks ? 768 / blocks : 1;
         if (chunks > tiles32 / 4) chunks = tiles32 / 4;
         if (chunks > 1) {
             p.chunk_tiles = (int)((tiles32 + chunks - 1) / chunks);

@@ -107,6 +107,20 @@ hipError_t launch_cache8_finish(const Attn8Args& a, int head_dim, hipStream_t s)
     return hipGetLastError();
 }
 
+#if defined(__HIP_DEVICE_COMPILE__)
+// The sum over the 32 lanes of a half, in all of them: rotations within 16 lanes, and the exchange of neighbouring sixteens.  (Through LDS, by __shfl_xor,
+// a workgroup's 32 of them were 5 us of a prompt's 38.)
+__device__ __forceinline__ float sum32(float x) {
+    x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x121, 0xf, 0xf, true));      // row_ror:1, 2, 4, 8
+    x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x122, 0xf, 0xf, true));
+    x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x124, 0xf, 0xf, true));
+    x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x128, 0xf, 0xf, true));
+    float a = x, b = x;
+    asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
+    return a + b;
+}
+#endif
+
 // The weights that 256 keys get from a chunk of row tiles.  A wave has 64 keys, whose codes it holds as operands (A, two blocks of 32); the
 // tile's queries (B) come through LDS, for all four waves, one tile ahead.  Per row and key: one exponential, one multiply-add and one addition.
 template <int D>
@@ -126,12 +140,19 @@ __global__ __launch_bounds__(256, 2) void cache8_weights_kernel(const Attn8Args 
     // (rows before the first that sees the block's first key add nothing)
     const int first = a.causal ? max(0, block0 - off) * a.G >> 5 : 0;
     const int t0 = max(first, chunk * a.chunk_tiles), t1 = min((rows + 31) >> 5, (chunk + 1) * a.chunk_tiles);
+    float* const to = a.n_chunks > 1 ? a.w_part + ((int64_t)chunk * a.B * a.Hkv + bh) * a.cap : a.w_out + (int64_t)bh * a.cap;
+    const float* from = a.n_chunks > 1 || !a.w_in ? nullptr : a.w_in + (int64_t)bh * a.cap;
+    if (t0 >= t1) {
+        const int key = block0 + threadIdx.x;
+        if (key < L) to[key] = from ? from[key] : 0.f;
+        return;
+    }
     float sum[2][16];
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
         for (int e = 0; e < 16; ++e) sum[k][e] = 0.f;
-    if (t0 < t1) {
+    {
         half8_t kA[2][NS];
         float c[2];
 #pragma unroll
@@ -173,7 +194,7 @@ __global__ __launch_bounds__(256, 2) void cache8_weights_kernel(const Attn8Args 
                 s[1] = mfma32(kA[1][i], qB, s[1]);
             }
             const int seen = a.causal ? min(L, a.by_g.of(t * 32) + off + 1) : L;         // by the tile's first row
-            if (key0 + 64 > seen) {
+            if (__builtin_expect(key0 + 64 > seen, 0)) {
                 const int lim = (row < rows ? (a.causal ? min(L - 1, qi + off) : L - 1) : -1) - key0 - 4 * h;
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
@@ -204,15 +225,11 @@ __global__ __launch_bounds__(256, 2) void cache8_weights_kernel(const Attn8Args 
             l2 = l2_next;
         }
     }
-    float* const to = a.n_chunks > 1 ? a.w_part + ((int64_t)chunk * a.B * a.Hkv + bh) * a.cap : a.w_out + (int64_t)bh * a.cap;
-    const float* from = a.n_chunks > 1 || !a.w_in ? nullptr : a.w_in + (int64_t)bh * a.cap;
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            float x = sum[k][e];
-#pragma unroll
-            for (int m = 16; m >= 1; m >>= 1) x += __shfl_xor(x, m, 64);
+            const float x = sum32(sum[k][e]);
             const int key = key0 + 32 * k + 8 * (e >> 2) + 4 * h + (e & 3);
             if (n == e && key < L) to[key] = (from ? from[key] : 0.f) + x;
         }
