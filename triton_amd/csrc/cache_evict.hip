@@ -3,8 +3,8 @@
 //
 // Two launches.  Selection: a workgroup has one head of a sequence.  The weights of its query heads are added up in 64 bits and rounded
 // once to fp32, turned into integers that order as they do, and the smallest one kept is found by digits of 11, 11 and 10 bits, counted in
-// LDS; ties are filled up from the front.  Up to 32768 keys stay in registers, a thread with consecutive ones, so that one scan over the
-// threads numbers what is kept.  Move: rows of K and V, 16 bytes a lane, past the caches (each byte once).  Into another cache, workgroups
+// LDS; ties are filled up from the front.  Up to 32768 keys stay in registers, and one scan over the counts of each 64 numbers what is
+// kept.  Move: rows of K and V, 16 bytes a lane, past the caches (each byte once).  Into another cache, workgroups
 // share the rows; within the same one, a workgroup has a 64-byte column of all of a head's rows and moves them front to back: a row
 // goes to its own place or one before it, so what a step overwrites has been read by this step or an earlier one, and columns
 // never meet.
@@ -38,12 +38,40 @@ __device__ __forceinline__ uint32_t order_of(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;       // (0xff800000's complement, of -inf, is 0x7fffff: above NaN's)
 }
 
-// The sum of a key's weights over its KV head's rows.
-__device__ __forceinline__ uint32_t order_at(const EvictArgs& a, int64_t at, int per) {
-    double s = 0.0;
-    for (int g = 0; g < per; ++g)
-        s += a.w_half ? (double)(float)static_cast<const half_t*>(a.w)[at + (int64_t)g * a.S] : (double)static_cast<const float*>(a.w)[at + (int64_t)g * a.S];
-    return order_of((float)s);
+// The order of the NK keys first, first + 1024, .. (below `end`): their weights summed over the rows of their KV head, all keys of a row, and of four rows,
+// on their way at once.  (A key after the other, each sum waited for its loads alone: 8 keys a thread took 8 us of a selection's 14.)
+template <class T, int NK>
+__device__ __forceinline__ void orders_of(const T* w, int64_t pitch, int rows, int first, int end, uint32_t (&u)[NK]) {
+    constexpr int UR = NK <= 8 ? 4 : 1;
+    double s[NK];
+#pragma unroll
+    for (int i = 0; i < NK; ++i) s[i] = 0.0;
+    int g = 0;
+    for (; g + UR <= rows; g += UR) {
+        T x[UR][NK];
+#pragma unroll
+        for (int k = 0; k < UR; ++k)
+#pragma unroll
+            for (int i = 0; i < NK; ++i) x[k][i] = w[(g + k) * pitch + min(first + i * 1024, end - 1)];
+#pragma unroll
+        for (int k = 0; k < UR; ++k)
+#pragma unroll
+            for (int i = 0; i < NK; ++i) s[i] += (double)(float)x[k][i];
+    }
+    for (; g < rows; ++g) {
+        T x[NK];
+#pragma unroll
+        for (int i = 0; i < NK; ++i) x[i] = w[g * pitch + min(first + i * 1024, end - 1)];
+#pragma unroll
+        for (int i = 0; i < NK; ++i) s[i] += (double)(float)x[i];
+    }
+#pragma unroll
+    for (int i = 0; i < NK; ++i) u[i] = order_of((float)s[i]);
+}
+template <int NK>
+__device__ __forceinline__ void orders_of(const EvictArgs& a, int64_t at, int rows, int first, int end, uint32_t (&u)[NK]) {
+    if (a.w_half) orders_of(static_cast<const half_t*>(a.w) + at, a.S, rows, first, end, u);
+    else orders_of(static_cast<const float*>(a.w) + at, a.S, rows, first, end, u);
 }
 // (x, y) summed over the threads before this one; `all`: over all of them.  16 waves.
 __device__ __forceinline__ int2 scan_before(int x, int y, int2* waves, int2& all) {
@@ -68,8 +96,7 @@ __device__ __forceinline__ int2 scan_before(int x, int y, int2* waves, int2& all
     return r;
 }
 
-// NV: a thread has as many consecutive keys, in registers (0: any number, whose order lies in the workspace and is walked over 1024 keys at a
-// time).
+// NV: a thread has as many keys, 1024 apart, in registers (0: any number, whose order lies in the workspace and is walked over 1024 at a time).
 template <int NV>
 __global__ __launch_bounds__(1024) void cache_evict_select_kernel(const EvictArgs a) {
     __shared__ int bins[2048];
@@ -103,12 +130,20 @@ __global__ __launch_bounds__(1024) void cache_evict_select_kernel(const EvictArg
         return;
     }
 
-    uint32_t u[NV ? NV : 1];
-    if constexpr (NV > 0) {
+    uint32_t u[NV ? NV : 4];
+    if constexpr (NV == 32) {
+        uint32_t half[16];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) { const int j = tid * NV + i; u[i] = j < early ? order_at(a, w0 + j, per) : 0; }
-    } else {
-        for (int j = tid; j < early; j += 1024) order[j] = order_at(a, w0 + j, per);
+        for (int k = 0; k < 2; ++k) {
+            orders_of(a, w0, per, tid + k * 16384, early, half);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) u[16 * k + i] = half[i];
+        }
+    } else if constexpr (NV > 0) orders_of(a, w0, per, tid, early, u);
+    else for (int j0 = tid; j0 < early; j0 += 4096) {
+        orders_of(a, w0, per, j0, early, u);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) if (j0 + i * 1024 < early) order[j0 + i * 1024] = u[i];
     }
     // The smallest order kept: kept are those above it, and the first `rest` of its equals.
     uint32_t least = 0;
@@ -122,7 +157,7 @@ __global__ __launch_bounds__(1024) void cache_evict_select_kernel(const EvictArg
         };
         if constexpr (NV > 0) {
 #pragma unroll
-            for (int i = 0; i < NV; ++i) if (tid * NV + i < early) count(u[i]);
+            for (int i = 0; i < NV; ++i) if (tid + i * 1024 < early) count(u[i]);
         } else for (int j = tid; j < early; j += 1024) count(order[j]);
         __syncthreads();
         // from the top: thread i has the bins 2047 - 2 i and one below
@@ -139,24 +174,47 @@ __global__ __launch_bounds__(1024) void cache_evict_select_kernel(const EvictArg
         rest -= s_above;
     }
     // Their places: by what is kept, and by how many equals of the least there are, before them.
-    int2 all;
     if constexpr (NV > 0) {
-        int above = 0, ties = 0;
+        // ... counted for each wave's 64 consecutive keys, in whose order the first wave adds them up
+        int2* const runs = reinterpret_cast<int2*>(bins);
+        static_assert(sizeof(int2) * NV * 16 <= sizeof(bins), "room for the runs");
+        const int lane = tid & 63, wave = tid >> 6;
+        __syncthreads();
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const bool real = tid * NV + i < early;
-            above += real && u[i] > least; ties += real && u[i] == least;
+            const bool real = tid + i * 1024 < early;
+            const uint64_t up = __ballot(real && u[i] > least), eq = __ballot(real && u[i] == least);
+            if (lane == 0) runs[i * 16 + wave] = int2{__popcll(up), __popcll(eq)};
         }
-        const int2 before = scan_before(above, ties, waves, all);
-        int tie = before.y, at = before.x + min(before.y, rest);
+        __syncthreads();
+        if (wave == 0) {
+            constexpr int PER = NV / 4;
+            int2 mine[PER], sum = {0, 0};
+#pragma unroll
+            for (int i = 0; i < PER; ++i) { mine[i] = runs[lane * PER + i]; sum.x += mine[i].x; sum.y += mine[i].y; }
+            int2 at = sum;
+#pragma unroll
+            for (int m = 1; m < 64; m <<= 1) {
+                const int px = __shfl_up(at.x, m, 64), py = __shfl_up(at.y, m, 64);
+                if (lane >= m) { at.x += px; at.y += py; }
+            }
+            at.x -= sum.x; at.y -= sum.y;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) { runs[lane * PER + i] = at; at.x += mine[i].x; at.y += mine[i].y; }
+        }
+        __syncthreads();
+        const uint64_t below = ((uint64_t)1 << lane) - 1;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const bool real = tid * NV + i < early, eq = real && u[i] == least;
-            if (real && (u[i] > least || (eq && tie < rest))) kept[at++] = tid * NV + i;
-            tie += eq;
+            const int j = tid + i * 1024;
+            const bool up = j < early && u[i] > least, eq = j < early && u[i] == least;
+            const uint64_t ub = __ballot(up), eb = __ballot(eq);
+            const int2 run = runs[i * 16 + wave];
+            const int tie = run.y + __popcll(eb & below);
+            if (up || (eq && tie < rest)) kept[run.x + __popcll(ub & below) + min(tie, rest)] = j;
         }
     } else {
-        int2 base = {0, 0};
+        int2 all, base = {0, 0};
         for (int j0 = 0; j0 < early; j0 += 1024) {
             const int j = j0 + tid;
             const uint32_t x = j < early ? order[j] : 0;
@@ -185,11 +243,15 @@ __global__ __launch_bounds__(256) void cache_evict_move_kernel(const EvictArgs a
         const int64_t to = a.w_out == a.w ? from : (int64_t)row * a.keep;
         constexpr int NW = 4;
         for (int i0 = 0; i0 < stay; i0 += NW * 256) {
-            float x[NW];
+            float x[NW]; int j[NW];
 #pragma unroll
-            for (int e = 0; e < NW; ++e) {
-                const int i = i0 + e * 256 + tid;
-                if (i < stay) x[e] = a.w_half ? (float)static_cast<const half_t*>(a.w)[from + kept[i]] : static_cast<const float*>(a.w)[from + kept[i]];
+            for (int e = 0; e < NW; ++e) j[e] = kept[min(i0 + e * 256 + tid, stay - 1)];
+            if (a.w_half) {
+#pragma unroll
+                for (int e = 0; e < NW; ++e) x[e] = (float)static_cast<const half_t*>(a.w)[from + j[e]];
+            } else {
+#pragma unroll
+                for (int e = 0; e < NW; ++e) x[e] = static_cast<const float*>(a.w)[from + j[e]];
             }
             __syncthreads();
 #pragma unroll
@@ -227,12 +289,11 @@ __global__ __launch_bounds__(256) void cache_evict_move_kernel(const EvictArgs a
     constexpr int NB = 4;      // rows of a lane on their way at once
     __shared__ float ratio[256], top[8];
     for (int i0 = from; i0 < to; i0 += NB * step) {
-        uint4_t x[NB];
+        uint4_t x[NB]; int j[NB];
 #pragma unroll
-        for (int e = 0; e < NB; ++e) {
-            const int i = i0 + e * step + r0;
-            if (i < to) x[e] = __builtin_nontemporal_load(reinterpret_cast<const uint4_t*>(src + (int64_t)kept[i] * a.st[kv][2] + off));
-        }
+        for (int e = 0; e < NB; ++e) j[e] = kept[min(i0 + e * step + r0, to - 1)];
+#pragma unroll
+        for (int e = 0; e < NB; ++e) x[e] = __builtin_nontemporal_load(reinterpret_cast<const uint4_t*>(src + (int64_t)j[e] * a.st[kv][2] + off));
         // 8 bits: the blocks of these rows (128 or 256: whole blocks) and what their codes are to be multiplied by
         if constexpr (BITS8) {
             const float* was = a.scales + ((int64_t)kv * a.B * a.Hkv + bh) * a.n_blocks;
