@@ -68,7 +68,7 @@ def _run(case, kind, half, bits, place, block=64, seed=3, layout="head"):
     kept = torch.full((B, H, keep), 77, dtype=torch.int32, device=DEV)
     n = torch.tensor(lengths, dtype=torch.int32, device=DEV)
     new = n if place == "within" else torch.full_like(n, 77)
-    ws = torch.full((ops.cache_evict_workspace_bytes(dk, keep),), 0xff, dtype=torch.uint8, device=DEV)
+    ws = torch.full((ops.cache_evict_workspace_bytes(dk, dw, keep),), 0xff, dtype=torch.uint8, device=DEV)
     ops.cache_evict(dk, dv, dw, ko, vo, kept, keep, recent, ws, n, new, wo, dks, dvs, kso, vso, block)
     want = ref.evict(k, v, w, keep, recent, lengths, ks, vs, block)
     assert new.tolist() == [min(x, keep) for x in lengths]
@@ -119,6 +119,7 @@ def test_other_blocks_and_token_major_caches(block, place):
 def test_long_rows(S, kind):
     _run((1, 1, 2, 64, S, S // 2 + 1, 100, [S - 1]), kind, False, 16, "within")
     _run((1, 2, 1, 64, S, S // 3, 0, [S]), kind, True, 8, "apart")
+    _run((1, 1, 9, 64, S, S // 2, 3, [S - 5]), kind, True, 16, "apart")
 
 
 def test_keyformer_scores_cut_a_prompt():
@@ -217,7 +218,7 @@ def test_refusals():
     k = torch.zeros(1, 2, 64, 64, dtype=torch.float16, device=DEV)
     v, out, vout = k.clone(), torch.zeros(1, 2, 16, 64, dtype=torch.float16, device=DEV), torch.zeros(1, 2, 16, 64, dtype=torch.float16, device=DEV)
     w, kept = torch.zeros(1, 4, 64, device=DEV), torch.zeros(1, 2, 16, dtype=torch.int32, device=DEV)
-    ws = torch.zeros(ops.cache_evict_workspace_bytes(k, 16), dtype=torch.uint8, device=DEV)
+    ws = torch.zeros(ops.cache_evict_workspace_bytes(k, w, 16), dtype=torch.uint8, device=DEV)
     good = dict(k=k, v=v, weights=w, k_out=out, v_out=vout, kept=kept, keep=16, recent=4, workspace=ws)
     ops.cache_evict(**good)
 

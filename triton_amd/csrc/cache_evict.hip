@@ -1,7 +1,7 @@
 // Eviction from a key/value cache by accumulated attention weight: of each sequence and KV head the `recent` last keys and those of the
 // largest weight among the others, `keep` in all, gathered to the front in their order.
 //
-// Two launches.  Selection: a workgroup has one head of a sequence.  The weights of its query heads are added up in 64 bits and rounded
+// Two launches, or three.  Selection: a workgroup has one head of a sequence.  The weights of its query heads are added up in 64 bits and rounded
 // once to fp32, turned into integers that order as they do, and the smallest one kept is found by digits of 11, 11 and 10 bits, counted in
 // LDS; ties are filled up from the front.  Up to 32768 keys stay in registers, and one scan over the counts of each 64 numbers what is
 // kept.  Move: rows of K and V, 16 bytes a lane, past the caches (each byte once).  Into another cache, workgroups
@@ -23,7 +23,7 @@ struct EvictArgs {
     int B, Hkv, Hw, S, keep, recent, bshift, w_half, in_place[2];
     int64_t st[2][3], ot[2][3];        // strides of K and V in bytes, given and kept
     int64_t sst[2][2], sot[2][2];      // ... of their scales
-    uint32_t* order;                   // [B Hkv][S]
+    uint32_t* order; int summed;       // [B Hkv][S] if summed by a launch of its own, or too many keys for registers
     float* scales;                     // 8 bits: [2][B Hkv][n_blocks], the scales as they were
     int n_blocks;
     int32_t* now;                      // [2][B]: keys that stay, and that there were
@@ -42,7 +42,7 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 // on their way at once.  (A key after the other, each sum waited for its loads alone: 8 keys a thread took 8 us of a selection's 14.)
 template <class T, int NK>
 __device__ __forceinline__ void orders_of(const T* w, int64_t pitch, int rows, int first, int end, uint32_t (&u)[NK]) {
-    constexpr int UR = NK <= 8 ? 4 : 1;
+    constexpr int UR = NK == 1 ? 8 : NK <= 8 ? 4 : 1;
     double s[NK];
 #pragma unroll
     for (int i = 0; i < NK; ++i) s[i] = 0.0;
@@ -73,34 +73,36 @@ __device__ __forceinline__ void orders_of(const EvictArgs& a, int64_t at, int ro
     if (a.w_half) orders_of(static_cast<const half_t*>(a.w) + at, a.S, rows, first, end, u);
     else orders_of(static_cast<const float*>(a.w) + at, a.S, rows, first, end, u);
 }
-// (x, y) summed over the threads before this one; `all`: over all of them.  16 waves.
-__device__ __forceinline__ int2 scan_before(int x, int y, int2* waves, int2& all) {
+// x summed over the threads before this one of 1024.
+__device__ __forceinline__ int scan_before(int x, int* waves) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int sx = x, sy = y;
+    int s = x;
 #pragma unroll
-    for (int m = 1; m < 64; m <<= 1) {
-        const int px = __shfl_up(sx, m, 64), py = __shfl_up(sy, m, 64);
-        if (lane >= m) { sx += px; sy += py; }
-    }
-    if (lane == 63) waves[wave] = int2{sx, sy};
+    for (int m = 1; m < 64; m <<= 1) { const int p = __shfl_up(s, m, 64); if (lane >= m) s += p; }
+    if (lane == 63) waves[wave] = s;
     __syncthreads();
-    int2 r = {sx - x, sy - y};
-    all = int2{0, 0};
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const int2 w = waves[i];
-        if (i < wave) { r.x += w.x; r.y += w.y; }
-        all.x += w.x; all.y += w.y;
-    }
+    s -= x;
+    for (int i = 0; i < wave; ++i) s += waves[i];
     __syncthreads();
-    return r;
+    return s;
 }
 
-// NV: a thread has as many keys, 1024 apart, in registers (0: any number, whose order lies in the workspace and is walked over 1024 at a time).
+// The orders by a launch of their own, 256 keys a workgroup.
+__global__ __launch_bounds__(256) void cache_evict_sums_kernel(const EvictArgs a) {
+    const int n_kb = (a.S + 255) >> 8, bh = blockIdx.x / n_kb, j = (blockIdx.x - bh * n_kb) * 256 + threadIdx.x;
+    const int b = a.by_hkv.of(bh), h = bh - b * a.Hkv, per = a.Hw / a.Hkv, n = keys_of(a.lengths, b, a.S);
+    if (j >= n) return;
+    uint32_t u[1];
+    orders_of(a, ((int64_t)b * a.Hw + h * per) * a.S, per, j, n, u);
+    a.order[(int64_t)bh * a.S + j] = u[0];
+}
+
+// NV: a thread has as many keys, 1024 apart, in registers (0: any number, whose orders lie in the workspace and are walked
+// over 16384 at a time).
 template <int NV>
 __global__ __launch_bounds__(1024) void cache_evict_select_kernel(const EvictArgs a) {
-    __shared__ int bins[2048];
-    __shared__ int2 waves[16];
+    __shared__ __attribute__((aligned(16))) int bins[2048];
+    __shared__ int waves[16];
     __shared__ int s_digit, s_above;
     const int tid = threadIdx.x;
     const int bh = blockIdx.x, b = a.by_hkv.of(bh), h = bh - b * a.Hkv;
@@ -130,8 +132,14 @@ __global__ __launch_bounds__(1024) void cache_evict_select_kernel(const EvictArg
         return;
     }
 
-    uint32_t u[NV ? NV : 4];
-    if constexpr (NV == 32) {
+    constexpr int NU = NV ? NV : 16;
+    uint32_t u[NU];
+    auto stored = [&](int first) {
+#pragma unroll
+        for (int i = 0; i < NU; ++i) u[i] = order[min(first + i * 1024, early - 1)];
+    };
+    if (NV > 0 && a.summed) stored(tid);
+    else if constexpr (NV == 32) {
         uint32_t half[16];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -140,11 +148,6 @@ __global__ __launch_bounds__(1024) void cache_evict_select_kernel(const EvictArg
             for (int i = 0; i < 16; ++i) u[16 * k + i] = half[i];
         }
     } else if constexpr (NV > 0) orders_of(a, w0, per, tid, early, u);
-    else for (int j0 = tid; j0 < early; j0 += 4096) {
-        orders_of(a, w0, per, j0, early, u);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) if (j0 + i * 1024 < early) order[j0 + i * 1024] = u[i];
-    }
     // The smallest order kept: kept are those above it, and the first `rest` of its equals.
     uint32_t least = 0;
     int rest = want;
@@ -155,15 +158,15 @@ __global__ __launch_bounds__(1024) void cache_evict_select_kernel(const EvictArg
         auto count = [&](uint32_t x) {
             if (pass == 0 || (x >> (shift + bits)) == (least >> (shift + bits))) atomicAdd(&bins[(x >> shift) & ((1 << bits) - 1)], 1);
         };
-        if constexpr (NV > 0) {
+        for (int j0 = tid; NV ? j0 == tid : j0 < early; j0 += NU * 1024) {
+            if constexpr (NV == 0) stored(j0);
 #pragma unroll
-            for (int i = 0; i < NV; ++i) if (tid + i * 1024 < early) count(u[i]);
-        } else for (int j = tid; j < early; j += 1024) count(order[j]);
+            for (int i = 0; i < NU; ++i) if (j0 + i * 1024 < early) count(u[i]);
+        }
         __syncthreads();
         // from the top: thread i has the bins 2047 - 2 i and one below
         const int hi = bins[2047 - 2 * tid], lo = bins[2046 - 2 * tid];
-        int2 all;
-        const int before = scan_before(hi + lo, 0, waves, all).x;
+        const int before = scan_before(hi + lo, waves);
         if (before < rest && before + hi + lo >= rest) {
             const bool first = before + hi >= rest;
             s_digit = first ? 2047 - 2 * tid : 2046 - 2 * tid;
@@ -173,22 +176,25 @@ __global__ __launch_bounds__(1024) void cache_evict_select_kernel(const EvictArg
         least |= (uint32_t)s_digit << shift;
         rest -= s_above;
     }
-    // Their places: by what is kept, and by how many equals of the least there are, before them.
-    if constexpr (NV > 0) {
-        // ... counted for each wave's 64 consecutive keys, in whose order the first wave adds them up
-        int2* const runs = reinterpret_cast<int2*>(bins);
-        static_assert(sizeof(int2) * NV * 16 <= sizeof(bins), "room for the runs");
-        const int lane = tid & 63, wave = tid >> 6;
+    // Their places: by what is kept, and by how many equals of the least there are, before them -- counted for each wave's 64 consecutive keys, in
+    // whose order the first wave adds them up.
+    int2* const runs = reinterpret_cast<int2*>(bins);
+    static_assert(sizeof(int2) * (NU * 16 + 1) <= sizeof(bins), "room for the runs and their sum");
+    const int lane = tid & 63, wave = tid >> 6;
+    const uint64_t below = ((uint64_t)1 << lane) - 1;
+    int2 base = {0, 0};
+    for (int j0 = tid; NV ? j0 == tid : j0 - tid < early; j0 += NU * 1024) {
+        if constexpr (NV == 0) stored(j0);
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const bool real = tid + i * 1024 < early;
+        for (int i = 0; i < NU; ++i) {
+            const bool real = j0 + i * 1024 < early;
             const uint64_t up = __ballot(real && u[i] > least), eq = __ballot(real && u[i] == least);
             if (lane == 0) runs[i * 16 + wave] = int2{__popcll(up), __popcll(eq)};
         }
         __syncthreads();
         if (wave == 0) {
-            constexpr int PER = NV / 4;
+            constexpr int PER = NU / 4;
             int2 mine[PER], sum = {0, 0};
 #pragma unroll
             for (int i = 0; i < PER; ++i) { mine[i] = runs[lane * PER + i]; sum.x += mine[i].x; sum.y += mine[i].y; }
@@ -198,32 +204,22 @@ __global__ __launch_bounds__(1024) void cache_evict_select_kernel(const EvictArg
                 const int px = __shfl_up(at.x, m, 64), py = __shfl_up(at.y, m, 64);
                 if (lane >= m) { at.x += px; at.y += py; }
             }
+            if (lane == 63) runs[NU * 16] = at;
             at.x -= sum.x; at.y -= sum.y;
 #pragma unroll
             for (int i = 0; i < PER; ++i) { runs[lane * PER + i] = at; at.x += mine[i].x; at.y += mine[i].y; }
         }
         __syncthreads();
-        const uint64_t below = ((uint64_t)1 << lane) - 1;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int j = tid + i * 1024;
+        for (int i = 0; i < NU; ++i) {
+            const int j = j0 + i * 1024;
             const bool up = j < early && u[i] > least, eq = j < early && u[i] == least;
             const uint64_t ub = __ballot(up), eb = __ballot(eq);
             const int2 run = runs[i * 16 + wave];
-            const int tie = run.y + __popcll(eb & below);
-            if (up || (eq && tie < rest)) kept[run.x + __popcll(ub & below) + min(tie, rest)] = j;
+            const int tie = base.y + run.y + __popcll(eb & below);
+            if (up || (eq && tie < rest)) kept[base.x + run.x + __popcll(ub & below) + min(tie, rest)] = j;
         }
-    } else {
-        int2 all, base = {0, 0};
-        for (int j0 = 0; j0 < early; j0 += 1024) {
-            const int j = j0 + tid;
-            const uint32_t x = j < early ? order[j] : 0;
-            const bool up = j < early && x > least, eq = j < early && x == least;
-            const int2 before = scan_before(up, eq, waves, all);
-            const int tie = base.y + before.y;
-            if (up || (eq && tie < rest)) kept[base.x + before.x + min(tie, rest)] = j;
-            base.x += all.x; base.y += all.y;
-        }
+        base.x += runs[NU * 16].x; base.y += runs[NU * 16].y;
     }
 }
 
@@ -325,15 +321,17 @@ __global__ __launch_bounds__(256) void cache_evict_move_kernel(const EvictArgs a
     }
 }
 
-// Keys of which a thread of the selection has its own in registers.
-constexpr int kMostKept = 32768;
+// Keys of which a thread of the selection has its own in registers; and from how many rows of weights a head on they are added up by a launch of their own
+// (one KV head of 71 query heads, 4096 keys: 21 us by the selection's one workgroup).
+constexpr int kMostKept = 32768, kManyRows = 9;
+static bool orders_stored(const trn_cache_evict_desc* e) { return e->keys > kMostKept || e->n_weight_rows >= kManyRows * e->n_kv_heads; }
 
 struct EvictSizes { int64_t scales, now, bytes; };
 static EvictSizes evict_sizes(const trn_cache_evict_desc* e) {
     auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
     EvictSizes s;
     const int64_t heads = (int64_t)e->batch * e->n_kv_heads;
-    s.scales = e->keys > kMostKept ? up(heads * e->keys * 4) : 0;
+    s.scales = orders_stored(e) ? up(heads * e->keys * 4) : 0;
     s.now = s.scales + (e->code_bytes == 1 ? up(2 * heads * ((e->keys + 31) / 32) * 4) : 0);
     s.bytes = s.now + up((int64_t)e->batch * 8);
     return s;
@@ -349,7 +347,7 @@ static bool apart(const void* x, int64_t nx, const void* y, int64_t ny) {
 }  // namespace trn
 
 extern "C" int64_t trn_cache_evict_workspace_bytes(const trn_cache_evict_desc* e) {
-    if (!e || e->batch <= 0 || e->n_kv_heads <= 0 || e->keys <= 0 || e->keep <= 0) return 0;
+    if (!e || e->batch <= 0 || e->n_kv_heads <= 0 || e->n_weight_rows <= 0 || e->keys <= 0 || e->keep <= 0) return 0;
     return trn::evict_sizes(e).bytes;
 }
 
@@ -416,6 +414,12 @@ extern "C" int trn_cache_evict(const trn_cache_evict_desc* e, const void* k, con
     if (heads > 0x7fffffff || (int64_t)e->batch * e->n_weight_rows > 0x7fffffff) return TRN_E_SHAPE;
     a.by_hkv = Div(e->n_kv_heads);
     const hipStream_t s = (hipStream_t)stream;
+    a.summed = orders_stored(e);
+    if (a.summed) {
+        const int64_t blocks = heads * ((e->keys + 255) / 256);
+        if (blocks > 0x7fffffffLL) return TRN_E_SHAPE;
+        hipLaunchKernelGGL(cache_evict_sums_kernel, dim3((unsigned)blocks), dim3(256), 0, s, a);
+    }
     const dim3 sel((unsigned)heads);
     if (e->keys <= 4096) hipLaunchKernelGGL(cache_evict_select_kernel<4>, sel, dim3(1024), 0, s, a);
     else if (e->keys <= 8192) hipLaunchKernelGGL(cache_evict_select_kernel<8>, sel, dim3(1024), 0, s, a);

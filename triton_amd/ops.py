@@ -419,11 +419,11 @@ def cache_evict(k, v, weights, k_out, v_out, kept, keep: int, recent: int, works
                             weights, weights_out)
 
 
-def cache_evict_workspace_bytes(k, keep: int) -> int:
-    """Bytes of workspace that `cache_evict` takes for a cache of k's shape and type."""
+def cache_evict_workspace_bytes(k, weights, keep: int) -> int:
+    """Bytes of workspace that `cache_evict` takes for a cache of k's shape and type and so many rows of weights."""
     e = _lib.CacheEvictDesc()
     e.batch, e.n_kv_heads, e.keys, e.head_dim = (int(x) for x in k.shape)
-    e.keep, e.code_bytes = int(keep), k.element_size()
+    e.keep, e.code_bytes, e.n_weight_rows = int(keep), k.element_size(), int(weights.shape[1])
     return int(_lib.load().trn_cache_evict_workspace_bytes(C.byref(e)))
 
 
