@@ -374,7 +374,7 @@ struct Plan8 { int G, R, nq, nw, n_rt, ns, n_chunks, chunk_tiles, sp; int64_t ml
 // of 128 on 8, one query, us with 1 / 2 / 4 / 8 / 16 / 32 shares: 1025 keys 9.6 / 10.9 / 9.5 / 9.3 / 9.0 / 8.9; batch 8, 1500 keys 12.0 / 12.4 / 11.9 / 12.5 / 16.6; batch 12, 3000
 // 23.7 / 19.5 / 20.8; batch 16, 4097 31.3 / 28.6 / 28.4; batch 24, 4000 33.9 / 41.6 / 39.9; batch 32, 8192 88.7 / 91.4 / 93.8; of two to one lengths 70.5 / 72.2 / 70.8.  A
 // second launch is some 3 us: without weights, which need it anyway, short caches have one share (512 keys 6.4, against 8.5; batch 8: 1025 keys 10.1 / 11.0; 16
-// heads of 64: 1025 keys 7.6 / 8.1, 2000 10.7 / 8.3).  Tiles of more than one read no more from memory than one does, and their waves rather
+// heads of 64: 1025 keys 7.6 / 8.1, 2000 10.7 / 8.3; batch 16, 32 heads of 128, 2000 17.5 / 18.6).  Tiles of more than one read no more from memory than one does, and their waves rather
 // have a second workgroup beside them than walk long: 16 heads of 64, batch 4, 8000 keys, 20 queries 26.3 with two shares, 23.3 with four.
 // A cache that is read by one row tile goes past the caches (each byte once), us through / past: batch 32, 8192 keys 99.5 / 89.4, one sequence of 131072 56.7 /
 // 51.2, of 4000 11.2 / 10.6; with two row tiles and more the others find it there: 64 rows, 16000 keys 18.7 / 20.6.
@@ -391,7 +391,7 @@ static Plan8 plan8(const trn_cache8* c, int Hq, int Sq, bool weights) {
     const int64_t units = heads * p.n_rt;
     int64_t ns = units ? 256 / units : 1;
     if (p.n_rt > 1 && ns >= 1 && tiles > 24 * p.nw * ns) ns *= 2;
-    if (!weights && tiles <= (d128 ? 26 : 34) + units / 4) ns = 1;
+    if (!weights && tiles <= (d128 ? 26 : 34) + units / 2) ns = 1;
     if (ns > tiles) ns = tiles;
     p.ns = (int)(ns < 1 ? 1 : ns > 64 ? 64 : ns);
     // PLAN
