@@ -413,12 +413,12 @@ int trn_cache8_append_f16(const trn_cache8* cache, const void* k, const void* v,
                           int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_s, void* stream);
 
 /*
- * o = softmax(scale * q k^T) v over an 8-bit cache: trn_attn_fwd_f16 for q, o [batch, n_q_heads, seq_q, head_dim] fp16 (o on 8 bytes), GQA / MQA.
+ * o = softmax(scale * q k^T) v over an 8-bit cache: trn_attn_fwd_f16 for q, o [batch, n_q_heads, seq_q, head_dim] fp16 (o on 8 bytes, apart from q), GQA / MQA.
  * causal: query i sees the keys j <= lengths[b] - counts[b] + i.  A query that sees no key gets zeros (lse -inf).
  *   lse           nullable float [batch, n_q_heads, seq_q] contiguous, natural log.
  *   weights_out   nullable float [batch, n_kv_heads, capacity] contiguous: weights_in (nullable: zeros) plus the attention weight that each key gets,
  *                 summed over the queries and the query heads of its KV head; keys from lengths[b] on are left as they are.  weights_in may be
- *                 weights_out: a running sum, as eviction by accumulated weight takes it.  Deterministic: no atomics.
+ *                 weights_out (but not overlap it otherwise): a running sum, as eviction by accumulated weight takes it.  Deterministic: no atomics.
  *   workspace     trn_cache8_attn_workspace_bytes(...) bytes, 256-byte aligned, no initial contents: the keys of a head are then shared out over
  *                 workgroups.  May be NULL or smaller without weights_out: a workgroup then walks over all of a row tile's keys; with weights_out
  *                 it is TRN_E_SCRATCH.  One call at a time may use it.

@@ -61,7 +61,7 @@ def test_attention_statuses(lib):
     assert _attend(lib, ws=P + 64, nbytes=1 << 30) == "TRN_E_ALIGN"
     assert _attend(lib, os=(256, 0, 64)) == "TRN_E_STRIDE"
     assert _attend(lib, w_out=P) == "TRN_E_SCRATCH" and _attend(lib, w_out=P, ws=P, nbytes=16) == "TRN_E_SCRATCH"
-    assert _attend(lib, Sq=1 << 26) == "TRN_E_UNSUPPORTED"
+    assert _attend(lib, Sq=1 << 26) == "TRN_E_UNSUPPORTED" and _attend(lib, w_in=P, w_out=P + 64, ws=P, nbytes=1 << 30) == "TRN_E_UNSUPPORTED"
 
 
 def test_attention_workspace_is_bounded(lib):
@@ -128,6 +128,8 @@ def test_wrappers_refuse_cpu_tensors_and_bad_constants():
         modules.get("attn8", "cache").forward(c, s)
     with pytest.raises(KeyError):
         modules.get("attn4", "cache")
+    with pytest.raises(KeyError):
+        modules.get("roco", "cache8", head_dim=64)
 
 
 def test_oracle_codes_against_the_type():

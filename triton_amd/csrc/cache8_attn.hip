@@ -433,6 +433,7 @@ static int attn8_check(const trn_cache8* c, int32_t n_q_heads, int32_t seq_q) {
 extern "C" int64_t trn_cache8_attn_workspace_bytes(const trn_cache8* c, int32_t n_q_heads, int32_t seq_q, int32_t weights) {
     using namespace trn;
     if (!c || c->n_kv_heads <= 0 || n_q_heads <= 0 || n_q_heads % c->n_kv_heads || seq_q <= 0 || c->batch <= 0 || c->capacity <= 0) return 0;
+    if ((int64_t)n_q_heads / c->n_kv_heads * seq_q > (1 << 26)) return 0;       // (refused by the call)
     return plan8(c, n_q_heads, seq_q, weights != 0).bytes;
 }
 
@@ -446,6 +447,10 @@ extern "C" int trn_cache8_attn_f16(const trn_cache8* c, const void* q, void* o, 
     if (c->batch == 0 || seq_q == 0) return TRN_OK;
     if (!q || !o || (weights_in && !weights_out)) return TRN_E_NULL;
     if (!(scale > 0.f)) return TRN_E_SHAPE;
+    if (weights_in && weights_in != weights_out) {
+        const int64_t size = (int64_t)c->batch * c->n_kv_heads * c->capacity * 4;
+        if (!apart(weights_in, size, weights_out, size)) return TRN_E_UNSUPPORTED;
+    }
     if ((c->batch > 1 && !o_stride_b) || (n_q_heads > 1 && !o_stride_h) || (seq_q > 1 && !o_stride_s)) return TRN_E_STRIDE;
     if (!aligned16(q) || (reinterpret_cast<uintptr_t>(o) & 7)) return TRN_E_ALIGN;
     for (int64_t s : {q_stride_b, q_stride_h, q_stride_s}) if (!pitch16(s, 2)) return TRN_E_ALIGN;

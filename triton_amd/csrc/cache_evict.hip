@@ -339,10 +339,6 @@ static EvictSizes evict_sizes(const trn_cache_evict_desc* e) {
 
 // The bytes that a tensor [batch, heads, rows, width] spans from its base (strides in bytes, not negative).
 static int64_t span(const int64_t* st, int64_t b, int64_t h, int64_t rows, int64_t width) { return (b - 1) * st[0] + (h - 1) * st[1] + (rows - 1) * st[2] + width; }
-static bool apart(const void* x, int64_t nx, const void* y, int64_t ny) {
-    const uintptr_t p = (uintptr_t)x, q = (uintptr_t)y;
-    return p + (uint64_t)nx <= q || q + (uint64_t)ny <= p;
-}
 
 }  // namespace trn
 
