@@ -323,6 +323,71 @@ def test_captured_and_replayed_on_a_cache_that_grows():
         assert torch.equal(_cpu(dk8)[0, :, :lengths[0]], k8[0, :, :lengths[0]])
 
 
+def test_two_instances_on_two_streams():
+    case = ATTNS[8]
+    B, Hq, Hkv, D, M, S, block, lengths, counts, causal = case
+    rs = [_attend(case, seed=s) for s in (41, 51)]
+    outs = [torch.zeros_like(r["q"]) for r in rs]
+    ws = [torch.zeros(B, Hkv, S, device=DEV) for _ in rs]
+    n = _ints(lengths)
+    torch.cuda.synchronize()
+    mods, streams = [modules.get("weights8", "cache", block=block) for _ in rs], [torch.cuda.Stream() for _ in rs]
+    for _ in range(20):
+        for r, o, w, mod, st in zip(rs, outs, ws, mods, streams):
+            with torch.cuda.stream(st):
+                mod.forward(r["k8"], r["ks"], o, r["q"], r["v8"], r["vs"], None, n, None, w)
+    torch.cuda.synchronize()
+    for r, o, w in zip(rs, outs, ws):
+        _check(_cpu(o), r["want"], r["tol"], "o")
+        _check(_cpu(w)[0, :, :lengths[0]], r["ww"][0, :, :lengths[0]], r["wtol"][0, :, :lengths[0]], "weights")
+
+
+def test_caches_and_batches_of_nothing():
+    z = lambda *s, dt=torch.uint8: torch.zeros(*s, dtype=dt, device=DEV)
+    q, o, lse = z(1, 4, 2, 64, dt=torch.float16), torch.full((1, 4, 2, 64), 7.0, dtype=torch.float16, device=DEV), z(1, 4, 2, dt=torch.float32)
+    k8, s = z(1, 2, 0, 64), z(1, 2, 0, dt=torch.float32)
+    ops.cache8_append(q[:, :2], q[:, :2], k8, k8, s, s)
+    ops.cache8_attention(q, k8, k8, s, s, o, lse=lse)
+    assert (o == 0).all() and (lse == -math.inf).all()
+    k8, s = z(0, 2, 64, 64), z(0, 2, 1, dt=torch.float32)
+    ops.cache8_append(q[:0, :2], q[:0, :2], k8, k8, s, s)
+    ops.cache8_attention(q[:0], k8, k8, s, s, o[:0])
+
+
+@pytest.mark.parametrize("variant", ["vanilla", "prenorm", "weights"])
+def test_the_step_of_projection_append_and_attention(variant):
+    """modules.get(.., "cache8"): three steps of a ragged, padded batch, with what its projections leave held to the definitions."""
+    B, Hq, Hkv, D, N, S, block, M = 2, 4, 2, 64, 256, 120, 32, 5
+    g = torch.Generator().manual_seed(61)
+    wq, wk, wv = ((torch.randn(N, h * D, generator=g) * N ** -0.5).half().to(DEV) for h in (Hq, Hkv, Hkv))
+    mod = modules.get(variant, "cache8", head_dim=D, block=block)
+    k8, v8 = (torch.zeros(B, Hkv, S, D, dtype=torch.uint8) for _ in range(2))
+    ks, vs = (torch.zeros(B, Hkv, -(-S // block)) for _ in range(2))
+    dk8, dv8, dks, dvs = (t.to(DEV) for t in (k8, v8, ks, vs))
+    w, ww, slack = torch.zeros(B, Hkv, S, device=DEV), torch.zeros(B, Hkv, S, dtype=torch.float64), torch.zeros(B, Hkv, S, dtype=torch.float64)
+    lengths = [0, 0]
+    for counts in ([5, 3], [1, 5], [5, 5]):
+        x = torch.randn(B, M, N, generator=g).half().to(DEV)
+        o = torch.full((B, M, Hq * D), 7.0, dtype=torch.float16, device=DEV)
+        lengths = [n + c for n, c in zip(lengths, counts)]
+        extra = (w,) if variant == "weights" else ()
+        mod.forward(dk8, dks, o, dv8, dvs, wk, wq, wv, x, _ints(counts), _ints(lengths), *extra)
+        q, k, v = (torch.empty(B * M, h * D, dtype=torch.float16, device=DEV) for h in (Hq, Hkv, Hkv))
+        ops.prenorm_qkv(x.view(B * M, N), None, wq, wk, wv, *(t.view(B * M, -1, D).permute(1, 0, 2) for t in (q, k, v)), 0.0, variant == "prenorm")
+        q, k, v = (_cpu(t).view(B, M, -1, D).permute(0, 2, 1, 3) for t in (q, k, v))
+        k8, ks = ref.append(k, k8, ks, lengths, counts, block)
+        v8, vs = ref.append(v, v8, vs, lengths, counts, block)
+        assert torch.equal(_cpu(dk8), k8) and torch.equal(_cpu(dvs), vs)
+        want, _, got, tol, wtol, _ = ref.attention(q, k8, v8, ks, vs, D ** -0.5, True, lengths, counts, block)
+        for b, c in enumerate(counts):
+            _check(_cpu(o)[b, :c].view(c, Hq, D).permute(1, 0, 2), want[b, :, :c], tol[b, :, :c], "O2")
+            assert (_cpu(o)[b, c:] == 7.0).all()
+        ww += got
+        slack += wtol + 2.0 ** -23 * ww
+    if variant == "weights":
+        _check(_cpu(w), ww, slack + 1e-30, "weights")
+
+
 def test_first_call_inside_a_capture_is_refused():
     k8, ks, dk8, dks, v8, vs, dv8, dvs = _cache(1, 2, 64, 64, 64, 31, [64])
     q = torch.zeros(1, 2, 1, 64, dtype=torch.float16, device=DEV)

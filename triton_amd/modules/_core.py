@@ -604,6 +604,43 @@ class Cache8Evict(CacheEvict):
                                 new_lengths, weights, weights_out)
 
 
+class Cache8Step(FusedModule):
+    """The decode-append step (ref_rms.py:45-83, 101-127) on an 8-bit cache of a batch whose sequences have lengths of their own: X [B,M,N] is
+    projected (norm=True: RMS-normalised first, no weight), keys and values are quantised into the cache, the queries attend over it, O2 [B,M,Hq*D].
+    WQ [N,Hq*D], WK, WV [N,Hkv*D]; lengths and counts as in `ops.cache8_append`, with this step's tokens.  Three launches, or four with a
+    cache's shares."""
+    TENSOR_PARAMS = ["K8", "K_scale", "O2", "V8", "V_scale", "WK", "WQ", "WV", "X", "counts", "lengths"]
+
+    def __init__(self, head_dim: int, scale: Optional[float] = None, causal: bool = True, block: int = 64, norm: bool = False, eps: float = 0.0):
+        super().__init__()
+        self.head_dim, self.scale, self.causal, self.block, self.norm, self.eps = head_dim, scale, causal, block, norm, eps
+
+    def _run(self, K8, K_scale, O2, V8, V_scale, WK, WQ, WV, X, counts, lengths, weights=None):
+        D = self.head_dim
+        if X.dim() != 3 or O2.dim() != 3 or WQ.dim() != 2 or WK.dim() != 2 or WQ.shape[1] % D or WK.shape[1] % D:
+            raise ValueError(f"inconsistent shapes: X {tuple(X.shape)}, O2 {tuple(O2.shape)}, WQ {tuple(WQ.shape)}, WK {tuple(WK.shape)}, head_dim {D}")
+        if not X.is_contiguous() or not O2.is_contiguous():
+            raise ValueError("X, O2: expected contiguous tensors")
+        B, M, N = X.shape
+        nq, nkv = WQ.shape[1], WK.shape[1]
+        if O2.shape != (B, M, nq):
+            raise ValueError(f"O2 {tuple(O2.shape)}: expected {(B, M, nq)}")
+        qkv = self._workspace("qkv", (B * M, nq + 2 * nkv), X.dtype, X.device)
+        parts = (qkv[:, :nq], qkv[:, nq:nq + nkv], qkv[:, nq + nkv:])
+        hm = [t.view(B * M, -1, D).permute(1, 0, 2) for t in parts]               # [head, token, D]
+        ops.prenorm_qkv(X.view(B * M, N), None, WQ, WK, WV, *hm, self.eps, self.norm)
+        q, k, v = (t.view(B, M, -1, D).permute(0, 2, 1, 3) for t in parts)        # [B, H, M, D]
+        ops.cache8_append(k, v, K8, V8, K_scale, V_scale, lengths, counts, self.block)
+        self._host.cache8_attention(self._hws, self.scale, self.causal, self.block, K8, K_scale, O2.view(B, M, -1, D).permute(0, 2, 1, 3), q, V8, V_scale,
+                                    counts, lengths, None, weights, weights)
+
+
+class Cache8StepWeights(Cache8Step):
+    """Cache8Step that adds the attention weight of each key to weights, float32 [B,Hkv,S], as Cache8Evict takes it."""
+    TENSOR_PARAMS = Cache8Step.TENSOR_PARAMS + ["weights"]
+
+
+CACHE8 = {"vanilla": Cache8Step, "prenorm": lambda **kw: Cache8Step(norm=True, **kw), "weights": Cache8StepWeights}
 CACHE = {"append8": Cache8Append, "attn8": Cache8Attention, "weights8": Cache8KeyWeights, "evict": CacheEvict, "evict8": Cache8Evict}
 
 PREFILL = {"rms": RMSNorm, "vanilla": Attention, "prenorm": PreNormBlock, "qknorm": QKNormAttention,
@@ -621,8 +658,9 @@ def get(variant: str, form: str = "prefill", **consts) -> FusedModule:
     form='prefill': Q/K/V (or X and weights) given, causal, 1/sqrt(D) scale by default.
     form='decode' : the reference's decode-append problem (needs head_dim=...).
     form='linear' : the reference's LoRA and gated-MLP workloads.
+    form='cache8' : the decode-append step on an 8-bit cache, {'vanilla','prenorm','weights'} (needs head_dim=...).
     form='cache'  : an 8-bit cache's append, attention and key weights, and eviction, {'append8','attn8','weights8','evict','evict8'}."""
-    table = {"prefill": PREFILL, "decode": DECODE, "linear": LINEAR, "cache": CACHE}.get(form)
+    table = {"prefill": PREFILL, "decode": DECODE, "linear": LINEAR, "cache": CACHE, "cache8": CACHE8}.get(form)
     if table is None or variant not in table:
         raise KeyError(f"no module for variant={variant!r} form={form!r}")
     return table[variant](**consts)
