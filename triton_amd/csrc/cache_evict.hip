@@ -223,6 +223,9 @@ __global__ __launch_bounds__(1024) void cache_evict_select_kernel(const EvictArg
     }
 }
 
+// All that this wave has requested from memory is there: a barrier alone does not say so of loads whose values are used behind it.
+__device__ __forceinline__ void loaded() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 // Workgroups from n_rows on: (head of a sequence, K or V, chunk of rows, column).  The first: the weights of the kept keys, one for each row of
 // them, and the new lengths.
 template <bool BITS8>
@@ -249,6 +252,7 @@ __global__ __launch_bounds__(256) void cache_evict_move_kernel(const EvictArgs a
 #pragma unroll
                 for (int e = 0; e < NW; ++e) x[e] = static_cast<const float*>(a.w)[from + j[e]];
             }
+            loaded();
             __syncthreads();
 #pragma unroll
             for (int e = 0; e < NW; ++e) {
@@ -305,7 +309,9 @@ __global__ __launch_bounds__(256) void cache_evict_move_kernel(const EvictArgs a
             if (col == 0 && (tid & ((1 << a.bshift) - 1)) == 0 && tid < NB * step && i0 + tid < to)
                 ((kv ? a.vs_out : a.ks_out) + b * a.sot[kv][0] + h * a.sot[kv][1])[(i0 + tid) >> a.bshift] = t;
         }
-        if (BITS8 || a.in_place[kv]) __syncthreads();      // (waits for the loads as well: what this step overwrites has been read)
+        // (what this step overwrites has been read)
+        if (a.in_place[kv]) loaded();
+        if (BITS8 || a.in_place[kv]) __syncthreads();
 #pragma unroll
         for (int e = 0; e < NB; ++e) {
             const int i = i0 + e * step + r0;
