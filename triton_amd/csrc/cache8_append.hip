@@ -34,7 +34,7 @@ __global__ __launch_bounds__(256) void cache8_append_kernel(const AppendArgs a) 
     uint8_t* code = a.code[kv] + b * a.cb[kv] + h * a.ch[kv];
     float* scale = a.scale[kv] + b * a.sb[kv] + h * a.sh[kv] + blk;
     const int sub = threadIdx.x % LPR, r0 = threadIdx.x / LPR;
-    const float was = base < first ? *scale : kScaleFloor;      // (a block that begins with a new token takes over nothing)
+    float was = base < first ? *scale : kScaleFloor;      // (a block that begins with a new token takes over nothing)
 
     half8_t v[NP];
     uint32_t top = 0;
@@ -43,6 +43,9 @@ __global__ __launch_bounds__(256) void cache8_append_kernel(const AppendArgs a) 
         const int row = p * RPP + r0, pos = base + row;
         if (row < a.block && pos >= first && pos < L) v[p] = *reinterpret_cast<const half8_t*>(x + (int64_t)(pos - first + skip) * a.xs[kv] + sub * 8);
     }
+    // (all are waited for here: where a row is there or not, the compiler waits at each use, for the stores before it as well)
+#pragma unroll
+    for (int p = 0; p < NP; ++p) asm volatile("" : "+v"(v[p]));
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
         const int row = p * RPP + r0, pos = base + row;
@@ -58,6 +61,7 @@ __global__ __launch_bounds__(256) void cache8_append_kernel(const AppendArgs a) 
     for (int m = 32; m >= 1; m >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, m, 64));
     __shared__ uint32_t part[4];
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
+    asm volatile("" : "+v"(was));       // (read by every wave before the first thread writes it, behind the barrier)
     __syncthreads();
     top = max(max(part[0], part[1]), max(part[2], part[3]));
     const float s = fmaxf(was, scale_for(__uint_as_float(top))), inv = 1.f / s;
@@ -65,16 +69,19 @@ __global__ __launch_bounds__(256) void cache8_append_kernel(const AppendArgs a) 
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
         const int row = p * RPP + r0, pos = base + row;
-        if (row >= a.block || pos >= L) continue;
-        uint2_t* to = reinterpret_cast<uint2_t*>(code + (int64_t)pos * a.cs[kv] + sub * 8);
-        if (pos >= first) {
+        if (row < a.block && pos >= first && pos < L) {
             float f[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[e] = (float)v[p][e] * inv;
-            *to = uint2_t{codes_of(f[0], f[1], f[2], f[3]), codes_of(f[4], f[5], f[6], f[7])};
-        } else if (s != was) {
+            *reinterpret_cast<uint2_t*>(code + (int64_t)pos * a.cs[kv] + sub * 8) = uint2_t{codes_of(f[0], f[1], f[2], f[3]), codes_of(f[4], f[5], f[6], f[7])};
+        }
+    }
+    if (base < first && s != was) {
+        const float ratio = was / s;
+        for (int pos = base + r0; pos < first; pos += RPP) {
+            uint2_t* to = reinterpret_cast<uint2_t*>(code + (int64_t)pos * a.cs[kv] + sub * 8);
             const uint2_t w = *to;
-            *to = uint2_t{recoded(w.x, was / s), recoded(w.y, was / s)};
+            *to = uint2_t{recoded(w.x, ratio), recoded(w.y, ratio)};
         }
     }
     if (threadIdx.x == 0 && s != was) *scale = s;
