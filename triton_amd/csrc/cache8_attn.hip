@@ -386,7 +386,6 @@ static Plan8 plan8(const trn_cache8* c, int Hq, int Sq, bool weights) {
     const int64_t heads = (int64_t)c->batch * c->n_kv_heads, tiles = (c->capacity + 31) / 32;
     p.nq = p.R > 16 && heads * ((p.R + 31) / 32) >= (d128 ? 128 : 320) ? 2 : 1;
     p.nw = 4;
-    // PLAN1
     p.n_rt = (p.R + 16 * p.nq - 1) / (16 * p.nq);
     const int64_t units = heads * p.n_rt;
     int64_t ns = units ? 256 / units : 1;
@@ -394,7 +393,6 @@ static Plan8 plan8(const trn_cache8* c, int Hq, int Sq, bool weights) {
     if (!weights && tiles <= (d128 ? 26 : 34) + units / 2) ns = 1;
     if (ns > tiles) ns = tiles;
     p.ns = (int)(ns < 1 ? 1 : ns > 64 ? 64 : ns);
-    // PLAN
     auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
     p.ml = p.ns > 1 ? up(units * p.ns * 16 * p.nq * c->head_dim * 4) : 0;
     p.lse2 = p.ml + (p.ns > 1 ? up(units * p.ns * 32 * p.nq * 4) : 0);

@@ -180,7 +180,12 @@ __global__ __launch_bounds__(256, 2) void cache8_weights_kernel(const Attn8Args 
             }
         };
         int qi = 0; float l2 = 0.f, l2_next;
-        auto row_sum = [&](int t) { const int r = t * 32 + n; return r < rows ? a.lse2[(int64_t)bh * a.R + r] : INFINITY; };      // (a row that is not there adds zeros)
+        // (a row that is not there, or has no weight to give, adds zeros)
+        auto row_sum = [&](int t) {
+            const int r = t * 32 + n;
+            const float x = r < rows ? a.lse2[(int64_t)bh * a.R + r] : INFINITY;
+            return x == -INFINITY ? INFINITY : x;
+        };
         auto tile = [&](int t, const half_t* Q) __attribute__((always_inline)) {
             const int row = t * 32 + n;
             qi = a.by_g.of(row);

@@ -415,19 +415,6 @@ extern "C" int trn_cache_evict(const trn_cache_evict_desc* e, const void* k, con
     const int64_t heads = (int64_t)e->batch * e->n_kv_heads;
     if (heads > 0x7fffffff || (int64_t)e->batch * e->n_weight_rows > 0x7fffffff) return TRN_E_SHAPE;
     a.by_hkv = Div(e->n_kv_heads);
-    const hipStream_t s = (hipStream_t)stream;
-    a.summed = orders_stored(e);
-    if (a.summed) {
-        const int64_t blocks = heads * ((e->keys + 255) / 256);
-        if (blocks > 0x7fffffffLL) return TRN_E_SHAPE;
-        hipLaunchKernelGGL(cache_evict_sums_kernel, dim3((unsigned)blocks), dim3(256), 0, s, a);
-    }
-    const dim3 sel((unsigned)heads);
-    if (e->keys <= 4096) hipLaunchKernelGGL(cache_evict_select_kernel<4>, sel, dim3(1024), 0, s, a);
-    else if (e->keys <= 8192) hipLaunchKernelGGL(cache_evict_select_kernel<8>, sel, dim3(1024), 0, s, a);
-    else if (e->keys <= 16384) hipLaunchKernelGGL(cache_evict_select_kernel<16>, sel, dim3(1024), 0, s, a);
-    else if (e->keys <= kMostKept) hipLaunchKernelGGL(cache_evict_select_kernel<32>, sel, dim3(1024), 0, s, a);
-    else hipLaunchKernelGGL(cache_evict_select_kernel<0>, sel, dim3(1024), 0, s, a);
     // rows shared out, or in columns of 64 bytes
     const bool columns = a.in_place[0] || a.in_place[1];
     const int pieces = width / 16, row_pieces = columns ? 4 : pieces;
@@ -437,8 +424,18 @@ extern "C" int trn_cache_evict(const trn_cache_evict_desc* e, const void* k, con
     a.cols = pieces / row_pieces;
     a.chunks = (rows_out + rows_per_chunk - 1) / rows_per_chunk;
     const int64_t n_rows = weights_out || new_lengths ? (int64_t)e->batch * e->n_weight_rows : 0, grid = n_rows + 2 * heads * a.chunks * a.cols;
-    if (grid > 0x7fffffffLL) return TRN_E_SHAPE;
+    a.summed = orders_stored(e);
+    const int64_t sums = heads * ((e->keys + 255) / 256);
+    if (grid > 0x7fffffffLL || sums > 0x7fffffffLL) return TRN_E_SHAPE;
     a.by_cols = Div(a.cols); a.by_chunks = Div(a.chunks);
+    const hipStream_t s = (hipStream_t)stream;
+    if (a.summed) hipLaunchKernelGGL(cache_evict_sums_kernel, dim3((unsigned)sums), dim3(256), 0, s, a);
+    const dim3 sel((unsigned)heads);
+    if (e->keys <= 4096) hipLaunchKernelGGL(cache_evict_select_kernel<4>, sel, dim3(1024), 0, s, a);
+    else if (e->keys <= 8192) hipLaunchKernelGGL(cache_evict_select_kernel<8>, sel, dim3(1024), 0, s, a);
+    else if (e->keys <= 16384) hipLaunchKernelGGL(cache_evict_select_kernel<16>, sel, dim3(1024), 0, s, a);
+    else if (e->keys <= kMostKept) hipLaunchKernelGGL(cache_evict_select_kernel<32>, sel, dim3(1024), 0, s, a);
+    else hipLaunchKernelGGL(cache_evict_select_kernel<0>, sel, dim3(1024), 0, s, a);
     if (bits8) hipLaunchKernelGGL((cache_evict_move_kernel<true>), dim3((unsigned)grid), dim3(256), 0, s, a, row_pieces, shift, rows_per_chunk, (int)n_rows);
     else hipLaunchKernelGGL((cache_evict_move_kernel<false>), dim3((unsigned)grid), dim3(256), 0, s, a, row_pieces, shift, rows_per_chunk, (int)n_rows);
     return hipGetLastError() == hipSuccess ? TRN_OK : TRN_E_LAUNCH;
