@@ -6,23 +6,47 @@
 
 namespace trn {
 
-// (m, l) of a row's shares, a lane each: the factors by which they count, the row's sum, and log2 of it.
-__device__ __forceinline__ void join_row(const Attn8Args& a, int bh, int r, int lane, float& f, float& l, float& l2) {
-    const float2_t x = lane < a.ns ? *reinterpret_cast<const float2_t*>(a.ml + (((((int64_t)bh * a.n_rt + (r >> a.rshift)) * a.ns + lane) << a.rshift) + (r & ((1 << a.rshift) - 1))) * 2) : float2_t{-INFINITY, 0.f};
-    float top = x.x;
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) top = fmaxf(top, __shfl_xor(top, m, 64));
-    f = x.x == -INFINITY ? 0.f : fast_exp2(x.x - top);
-    l = x.y * f;                                  // (a sum of NaN stays)
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) l += __shfl_xor(l, m, 64);
+#if defined(__HIP_DEVICE_COMPILE__)
+// Over the 16 lanes of a row by rotations within it, over rows by exchanges.  (By __shfl_xor through LDS the sums of 32 rows a lane were 5 us of a prompt's 38.)
+template <int CTRL> __device__ __forceinline__ float rotated(float x) { return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true)); }
+__device__ __forceinline__ void swap_rows16(float& a, float& b) { asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b)); }
+__device__ __forceinline__ float sum32(float x) {
+    x += rotated<0x121>(x);       // row_ror:1, 2, 4, 8
+    x += rotated<0x122>(x);
+    x += rotated<0x124>(x);
+    x += rotated<0x128>(x);
+    float a = x, b = x;
+    swap_rows16(a, b);
+    return a + b;
+}
+__device__ __forceinline__ float max32(float x) {
+    x = fmaxf(x, rotated<0x121>(x));
+    x = fmaxf(x, rotated<0x122>(x));
+    x = fmaxf(x, rotated<0x124>(x));
+    x = fmaxf(x, rotated<0x128>(x));
+    float a = x, b = x;
+    swap_rows16(a, b);
+    return fmaxf(a, b);
+}
+
+// (m, l) of a row's shares, a lane each; and out of them the factors by which they count, the row's sum, and log2 of it.
+__device__ __forceinline__ float2_t shares_of(const Attn8Args& a, int bh, int r, int lane) {
+    const int row = min(r, a.R - 1);
+    return *reinterpret_cast<const float2_t*>(a.ml + (((((int64_t)bh * a.n_rt + (row >> a.rshift)) * a.ns + min(lane, a.ns - 1)) << a.rshift) + (row & ((1 << a.rshift) - 1))) * 2);
+}
+__device__ __forceinline__ void join_row(const Attn8Args& a, float2_t x, int lane, float& f, float& l, float& l2) {
+    const float m = lane < a.ns ? x.x : -INFINITY, top = half_max(max32(m));
+    f = m == -INFINITY ? 0.f : fast_exp2(m - top);
+    l = half_sum(sum32(lane < a.ns ? x.y * f : 0.f));      // (a sum of NaN stays)
     l2 = top + fast_log2(l);
 }
+#endif
 
 // Workgroups below n_merge: rows' shares, D / 4 threads a row and `sg` groups of them that have every sg-th share.  The others: 1024 keys'
 // weights out of their scores.
 template <int D>
 __global__ __launch_bounds__(256) void cache8_finish_kernel(const Attn8Args a, int n_merge, int per_head, int sg) {
+#if defined(__HIP_DEVICE_COMPILE__)
     constexpr int TPR = D / 4, GROUPS = 256 / TPR;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     __shared__ float fs[GROUPS][64], inv[32];
@@ -30,29 +54,36 @@ __global__ __launch_bounds__(256) void cache8_finish_kernel(const Attn8Args a, i
         __shared__ float4_t red[256];
         const int rows = GROUPS / sg, bh = blockIdx.x / per_head, r0 = (blockIdx.x - bh * per_head) * rows;
         const int b = a.by_hkv.of(bh), kvh = bh - b * a.Hkv;
+        const int grp = tid / TPR, piece = tid % TPR, i = grp / sg, nth = grp - i * sg, r = r0 + i;
+        // (a thread's first four shares are requested at once with what their factors come from)
+        const float2_t first = shares_of(a, bh, r0 + min(wave, rows - 1), lane);
+        constexpr int PRE = 4;
+        float4_t got[PRE];
+        const int row = min(r, a.R - 1);
+        const float* part = a.part + (((((int64_t)bh * a.n_rt + (row >> a.rshift)) * a.ns) << a.rshift) + (row & ((1 << a.rshift) - 1))) * D + 4 * piece;
+#pragma unroll
+        for (int e = 0; e < PRE; ++e) got[e] = *reinterpret_cast<const float4_t*>(part + ((int64_t)min(nth + e * sg, a.ns - 1) << a.rshift) * D);
         const int there = min(a.R, tokens_of(a.counts, b, a.Sq) * a.G);
         if (r0 >= there) return;
-        for (int i = wave; i < rows; i += 4) {
-            const int r = r0 + i;
-            if (r >= there) break;
+        for (int j = wave; j < rows; j += 4) {
+            if (r0 + j >= there) break;
             float f, l, l2;
-            join_row(a, bh, r, lane, f, l, l2);
-            fs[i][lane] = f;
+            join_row(a, j == wave ? first : shares_of(a, bh, r0 + j, lane), lane, f, l, l2);
+            fs[j][lane] = f;
             if (lane == 0) {
-                inv[i] = l == 0.f ? 0.f : 1.f / l;
-                const int i0 = a.by_g.of(r), g0 = r - i0 * a.G;
+                inv[j] = l == 0.f ? 0.f : 1.f / l;
+                const int i0 = a.by_g.of(r0 + j), g0 = r0 + j - i0 * a.G;
                 if (a.lse) a.lse[((int64_t)b * a.Hq + kvh * a.G + g0) * a.Sq + i0] = l2 * kLn2;
-                if (a.lse2) a.lse2[(int64_t)bh * a.R + r] = l2;
+                if (a.lse2) a.lse2[(int64_t)bh * a.R + r0 + j] = l2;
             }
         }
         __syncthreads();
-        const int grp = tid / TPR, piece = tid % TPR, i = grp / sg, nth = grp - i * sg, r = r0 + i;
         const bool mine = r < there;
         float4_t x = {0.f, 0.f, 0.f, 0.f};
         if (mine) {
-            const float* part = a.part + (((((int64_t)bh * a.n_rt + (r >> a.rshift)) * a.ns) << a.rshift) + (r & ((1 << a.rshift) - 1))) * D + 4 * piece;
-#pragma unroll 4
-            for (int k = nth; k < a.ns; k += sg) x = x + *reinterpret_cast<const float4_t*>(part + ((int64_t)k << a.rshift) * D) * fs[i][k];
+#pragma unroll
+            for (int e = 0; e < PRE; ++e) x = x + (nth + e * sg < a.ns ? got[e] * fs[i][nth + e * sg] : float4_t{0.f, 0.f, 0.f, 0.f});
+            for (int k = nth + PRE * sg; k < a.ns; k += sg) x = x + *reinterpret_cast<const float4_t*>(part + ((int64_t)k << a.rshift) * D) * fs[i][k];
         }
         if (sg > 1) {
             red[tid] = x;
@@ -69,32 +100,49 @@ __global__ __launch_bounds__(256) void cache8_finish_kernel(const Attn8Args a, i
         return;
     }
     const int n_kb = (a.cap + 1023) >> 10, u = blockIdx.x - n_merge, bh = u / n_kb, key0 = (u - bh * n_kb) << 10;
-    const int b = a.by_hkv.of(bh), L = keys_of(a.lengths, b, a.cap), rows = min(a.R, tokens_of(a.counts, b, a.Sq) * a.G);
+    const int b = a.by_hkv.of(bh);
+    // (the scores of the first rows and the old weights are requested at once with what the rows' sums come from; what is past the sequence's keys counts nowhere)
+    const bool shared = a.ns > 1;
+    const float2_t first = shared ? shares_of(a, bh, wave, lane) : float2_t{0.f, a.lse2[(int64_t)bh * a.R + min(wave, a.R - 1)]};
+    constexpr int PRE = 4;
+    const float* s = a.scores + (int64_t)bh * a.R * a.sp;
+    float got[PRE][4], old[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int key = key0 + 256 * i + tid;
+#pragma unroll
+        for (int r = 0; r < PRE; ++r) got[r][i] = s[(int64_t)min(r, a.R - 1) * a.sp + min(key, a.sp - 1)];
+        old[i] = *((a.w_in ? a.w_in : a.w_out) + (int64_t)bh * a.cap + min(key, a.cap - 1));
+    }
+    const int L = keys_of(a.lengths, b, a.cap), rows = min(a.R, tokens_of(a.counts, b, a.Sq) * a.G);
     if (key0 >= L) return;
     for (int r = wave; r < rows; r += 4) {
         float f, l, l2;
-        if (a.ns > 1) join_row(a, bh, r, lane, f, l, l2);
-        else l2 = a.lse2[(int64_t)bh * a.R + r];
+        if (shared) join_row(a, r == wave ? first : shares_of(a, bh, r, lane), lane, f, l, l2);
+        else l2 = r == wave ? first.y : a.lse2[(int64_t)bh * a.R + r];
         if (lane == 0) inv[r] = l2;
     }
     __syncthreads();
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
-    const float* s = a.scores + (int64_t)bh * a.R * a.sp + key0 + tid;
-#pragma unroll 4
-    for (int r = 0; r < rows; ++r) {
-        const float l2 = inv[r];
+    auto add = [&](int i, float x, float l2) { sum[i] += x == -INFINITY ? 0.f : fast_exp2(x - l2); };
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float x = key0 + 256 * i + tid < L ? s[(int64_t)r * a.sp + 256 * i] : -INFINITY;
-            sum[i] += x == -INFINITY ? 0.f : fast_exp2(x - l2);
+    for (int r = 0; r < PRE; ++r)
+        if (r < rows) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) add(i, got[r][i], inv[r]);
         }
+#pragma unroll 4
+    for (int r = PRE; r < rows; ++r) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) add(i, s[(int64_t)r * a.sp + min(key0 + 256 * i + tid, a.sp - 1)], inv[r]);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int key = key0 + 256 * i + tid;
         const int64_t at = (int64_t)bh * a.cap + key;
-        if (key < L) a.w_out[at] = (a.w_in ? a.w_in[at] : 0.f) + sum[i];
+        if (key < L) a.w_out[at] = (a.w_in ? old[i] : 0.f) + sum[i];
     }
+#endif
 }
 
 hipError_t launch_cache8_finish(const Attn8Args& a, int head_dim, hipStream_t s) {
@@ -106,20 +154,6 @@ hipError_t launch_cache8_finish(const Attn8Args& a, int head_dim, hipStream_t s)
     else hipLaunchKernelGGL((cache8_finish_kernel<64>), dim3(grid), dim3(256), 0, s, a, n_merge, per_head, sg);
     return hipGetLastError();
 }
-
-#if defined(__HIP_DEVICE_COMPILE__)
-// The sum over the 32 lanes of a half, in all of them: rotations within 16 lanes, and the exchange of neighbouring sixteens.  (Through LDS, by __shfl_xor,
-// a workgroup's 32 of them were 5 us of a prompt's 38.)
-__device__ __forceinline__ float sum32(float x) {
-    x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x121, 0xf, 0xf, true));      // row_ror:1, 2, 4, 8
-    x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x122, 0xf, 0xf, true));
-    x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x124, 0xf, 0xf, true));
-    x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x128, 0xf, 0xf, true));
-    float a = x, b = x;
-    asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
-    return a + b;
-}
-#endif
 
 // The weights that 256 keys get from a chunk of row tiles.  A wave has 64 keys, whose codes it holds as operands (A, two blocks of 32); the
 // tile's queries (B) come through LDS, for all four waves, one tile ahead.  Per row and key: one exponential, one multiply-add and one addition.
