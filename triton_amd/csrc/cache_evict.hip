@@ -73,19 +73,18 @@ __device__ __forceinline__ void orders_of(const EvictArgs& a, int64_t at, int ro
     if (a.w_half) orders_of(static_cast<const half_t*>(a.w) + at, a.S, rows, first, end, u);
     else orders_of(static_cast<const float*>(a.w) + at, a.S, rows, first, end, u);
 }
-// x summed over the threads before this one of 1024.
-__device__ __forceinline__ int scan_before(int x, int* waves) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int s = x;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) { const int p = __shfl_up(s, m, 64); if (lane >= m) s += p; }
-    if (lane == 63) waves[wave] = s;
-    __syncthreads();
-    s -= x;
-    for (int i = 0; i < wave; ++i) s += waves[i];
-    __syncthreads();
-    return s;
+#if defined(__HIP_DEVICE_COMPILE__)
+// x summed over the lanes up to this one: within rows of 16 by shifts, over rows by handing on their last lanes.
+template <int CTRL, int ROWS> __device__ __forceinline__ int moved(int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false); }
+__device__ __forceinline__ int scan64(int x) {
+    x += moved<0x111, 0xf>(x);       // row_shr:1, 2, 4, 8
+    x += moved<0x112, 0xf>(x);
+    x += moved<0x114, 0xf>(x);
+    x += moved<0x118, 0xf>(x);
+    x += moved<0x142, 0xa>(x);       // row_bcast:15, 31
+    return x + moved<0x143, 0xc>(x);
 }
+#endif
 
 // The orders by a launch of their own, 256 keys a workgroup.
 __global__ __launch_bounds__(256) void cache_evict_sums_kernel(const EvictArgs a) {
@@ -101,10 +100,11 @@ __global__ __launch_bounds__(256) void cache_evict_sums_kernel(const EvictArgs a
 // over 16384 at a time).
 template <int NV>
 __global__ __launch_bounds__(1024) void cache_evict_select_kernel(const EvictArgs a) {
-    __shared__ __attribute__((aligned(16))) int bins[2048];
-    __shared__ int waves[16];
+#if defined(__HIP_DEVICE_COMPILE__)
+    __shared__ __attribute__((aligned(16))) int bins[3 * 2048];
+    __shared__ __attribute__((aligned(16))) int waves[3][16];
     __shared__ int s_digit, s_above;
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int bh = blockIdx.x, b = a.by_hkv.of(bh), h = bh - b * a.Hkv;
     const int n = keys_of(a.lengths, b, a.S), stay = min(n, a.keep);
     const int late = min(a.recent, stay), early = n - late;              // the last `late` keys stay in any case
@@ -132,6 +132,7 @@ __global__ __launch_bounds__(1024) void cache_evict_select_kernel(const EvictArg
         return;
     }
 
+    for (int i = tid; i < 3 * 2048; i += 1024) bins[i] = 0;
     constexpr int NU = NV ? NV : 16;
     uint32_t u[NU];
     auto stored = [&](int first) {
@@ -151,12 +152,12 @@ __global__ __launch_bounds__(1024) void cache_evict_select_kernel(const EvictArg
     // The smallest order kept: kept are those above it, and the first `rest` of its equals.
     uint32_t least = 0;
     int rest = want;
+    __syncthreads();
     for (int pass = 0; pass < 3; ++pass) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
-        for (int i = tid; i < 2048; i += 1024) bins[i] = 0;
-        __syncthreads();
+        int* const bin = bins + pass * 2048;
         auto count = [&](uint32_t x) {
-            if (pass == 0 || (x >> (shift + bits)) == (least >> (shift + bits))) atomicAdd(&bins[(x >> shift) & ((1 << bits) - 1)], 1);
+            if (pass == 0 || (x >> (shift + bits)) == (least >> (shift + bits))) atomicAdd(&bin[(x >> shift) & ((1 << bits) - 1)], 1);
         };
         for (int j0 = tid; NV ? j0 == tid : j0 < early; j0 += NU * 1024) {
             if constexpr (NV == 0) stored(j0);
@@ -165,8 +166,12 @@ __global__ __launch_bounds__(1024) void cache_evict_select_kernel(const EvictArg
         }
         __syncthreads();
         // from the top: thread i has the bins 2047 - 2 i and one below
-        const int hi = bins[2047 - 2 * tid], lo = bins[2046 - 2 * tid];
-        const int before = scan_before(hi + lo, waves);
+        const int hi = bin[2047 - 2 * tid], lo = bin[2046 - 2 * tid], upto = scan64(hi + lo);
+        if (lane == 63) waves[pass][wave] = upto;
+        __syncthreads();
+        int before = upto - hi - lo;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) before += i < wave ? waves[pass][i] : 0;
         if (before < rest && before + hi + lo >= rest) {
             const bool first = before + hi >= rest;
             s_digit = first ? 2047 - 2 * tid : 2046 - 2 * tid;
@@ -180,12 +185,10 @@ __global__ __launch_bounds__(1024) void cache_evict_select_kernel(const EvictArg
     // whose order the first wave adds them up.
     int2* const runs = reinterpret_cast<int2*>(bins);
     static_assert(sizeof(int2) * (NU * 16 + 1) <= sizeof(bins), "room for the runs and their sum");
-    const int lane = tid & 63, wave = tid >> 6;
     const uint64_t below = ((uint64_t)1 << lane) - 1;
     int2 base = {0, 0};
     for (int j0 = tid; NV ? j0 == tid : j0 - tid < early; j0 += NU * 1024) {
-        if constexpr (NV == 0) stored(j0);
-        __syncthreads();
+        if constexpr (NV == 0) { stored(j0); __syncthreads(); }
 #pragma unroll
         for (int i = 0; i < NU; ++i) {
             const bool real = j0 + i * 1024 < early;
@@ -198,12 +201,7 @@ __global__ __launch_bounds__(1024) void cache_evict_select_kernel(const EvictArg
             int2 mine[PER], sum = {0, 0};
 #pragma unroll
             for (int i = 0; i < PER; ++i) { mine[i] = runs[lane * PER + i]; sum.x += mine[i].x; sum.y += mine[i].y; }
-            int2 at = sum;
-#pragma unroll
-            for (int m = 1; m < 64; m <<= 1) {
-                const int px = __shfl_up(at.x, m, 64), py = __shfl_up(at.y, m, 64);
-                if (lane >= m) { at.x += px; at.y += py; }
-            }
+            int2 at = {scan64(sum.x), scan64(sum.y)};
             if (lane == 63) runs[NU * 16] = at;
             at.x -= sum.x; at.y -= sum.y;
 #pragma unroll
@@ -221,6 +219,7 @@ __global__ __launch_bounds__(1024) void cache_evict_select_kernel(const EvictArg
         }
         base.x += runs[NU * 16].x; base.y += runs[NU * 16].y;
     }
+#endif
 }
 
 // All that this wave has requested from memory is there: a barrier alone does not say so of loads whose values are used behind it.
