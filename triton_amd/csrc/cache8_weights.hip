@@ -29,6 +29,15 @@ __device__ __forceinline__ float max32(float x) {
     return fmaxf(a, b);
 }
 
+// The first 2 N of x as N: of number i and i + N a lane keeps the second if its index has bit N, and gets the same from the lane that DPP names.
+template <int CTRL, int N> __device__ __forceinline__ void keep_half(float (&x)[16], int lane) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float keep = lane & N ? x[i + N] : x[i], give = lane & N ? x[i] : x[i + N];
+        x[i] = keep + rotated<CTRL>(give);
+    }
+}
+
 // (m, l) of a row's shares, a lane each; and out of them the factors by which they count, the row's sum, and log2 of it.
 __device__ __forceinline__ float2_t shares_of(const Attn8Args& a, int bh, int r, int lane) {
     const int row = min(r, a.R - 1);
@@ -165,8 +174,9 @@ __global__ __launch_bounds__(256, 2) void cache8_weights_kernel(const Attn8Args 
     __shared__ __attribute__((aligned(1024))) half_t Q1[32 * D];
     const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int n_kb = (a.cap + 255) >> 8;
-    const int chunk = blockIdx.y, bh = blockIdx.x / n_kb, block0 = (blockIdx.x - bh * n_kb) * 256, key0 = block0 + wave * 64;
+    // (a head's workgroups are as far apart as there are heads: where those are a multiple of eight, its queries are read by one XCD)
+    const int heads = a.B * a.Hkv, kb = blockIdx.x / heads;
+    const int chunk = blockIdx.y, bh = blockIdx.x - kb * heads, block0 = kb * 256, key0 = block0 + wave * 64;
     const int b = a.by_hkv.of(bh), kvh = bh - b * a.Hkv;
     const int L = keys_of(a.lengths, b, a.cap), C = tokens_of(a.counts, b, a.Sq), off = L - C;
     if (block0 >= L) return;
@@ -187,18 +197,6 @@ __global__ __launch_bounds__(256, 2) void cache8_weights_kernel(const Attn8Args 
 #pragma unroll
         for (int e = 0; e < 16; ++e) sum[k][e] = 0.f;
     {
-        half8_t kA[2][NS];
-        float c[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const uint8_t* kp = a.k + b * a.kb + kvh * a.kh + (int64_t)min(key0 + 32 * k + n, L - 1) * a.kst + h * 16;
-#pragma unroll
-            for (int j = 0; j < NS / 2; ++j) {
-                const uint4_t w = *reinterpret_cast<const uint4_t*>(kp + 32 * j);
-                kA[k][2 * j] = half_of_codes(w.x, w.y); kA[k][2 * j + 1] = half_of_codes(w.z, w.w);
-            }
-            c[k] = a.c * a.ks[b * a.ksb + kvh * a.ksh + (min(key0 + 32 * k, L - 1) >> a.bshift)];
-        }
         const half_t* qh = a.q + b * a.qb + (int64_t)kvh * a.G * a.qh;
         // staging: a wave-wide load has 64 / CPR rows, a wave every fourth of them
         constexpr int RPI = 64 / CPR, NL = 32 / RPI / 4;
@@ -220,6 +218,20 @@ __global__ __launch_bounds__(256, 2) void cache8_weights_kernel(const Attn8Args 
             const float x = r < rows ? a.lse2[(int64_t)bh * a.R + r] : INFINITY;
             return x == -INFINITY ? INFINITY : x;
         };
+        fetch(t0, Q0);
+        l2 = row_sum(t0);
+        half8_t kA[2][NS];
+        float c[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const uint8_t* kp = a.k + b * a.kb + kvh * a.kh + (int64_t)min(key0 + 32 * k + n, L - 1) * a.kst + h * 16;
+#pragma unroll
+            for (int j = 0; j < NS / 2; ++j) {
+                const uint4_t w = *reinterpret_cast<const uint4_t*>(kp + 32 * j);
+                kA[k][2 * j] = half_of_codes(w.x, w.y); kA[k][2 * j + 1] = half_of_codes(w.z, w.w);
+            }
+            c[k] = a.c * a.ks[b * a.ksb + kvh * a.ksh + (min(key0 + 32 * k, L - 1) >> a.bshift)];
+        }
         auto tile = [&](int t, const half_t* Q) __attribute__((always_inline)) {
             const int row = t * 32 + n;
             qi = a.by_g.of(row);
@@ -246,8 +258,6 @@ __global__ __launch_bounds__(256, 2) void cache8_weights_kernel(const Attn8Args 
                     for (int e = 0; e < 16; ++e) sum[k][e] += fast_exp2(__builtin_fmaf(s[k][e], c[k], -l2));
             }
         };
-        fetch(t0, Q0);
-        l2 = row_sum(t0);
         for (int t = t0; t < t1; t += 2) {
             __builtin_amdgcn_s_waitcnt(0);
             __syncthreads();                       // this tile is there, and the one before it has been read
@@ -264,14 +274,15 @@ __global__ __launch_bounds__(256, 2) void cache8_weights_kernel(const Attn8Args 
             l2 = l2_next;
         }
     }
+    // Sums over the 32 lanes of a half, each lane left with one key's: a lane hands the half of its numbers that it does not keep to the one that does.
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const float x = sum32(sum[k][e]);
-            const int key = key0 + 32 * k + 8 * (e >> 2) + 4 * h + (e & 3);
-            if (n == e && key < L) to[key] = (from ? from[key] : 0.f) + x;
-        }
+    for (int e = 0; e < 16; ++e) { swap_rows16(sum[0][e], sum[1][e]); sum[0][e] += sum[1][e]; }
+    keep_half<0x128, 8>(sum[0], n);       // row_ror:8
+    keep_half<0x141, 4>(sum[0], n);       // row_half_mirror: another four lanes, in reverse
+    keep_half<0x4e, 2>(sum[0], n);        // quad_perm: the other two
+    keep_half<0xb1, 1>(sum[0], n);        // ... and the other one
+    const int key = key0 + 32 * (n >> 4) + 8 * ((n & 15) >> 2) + 4 * h + (n & 3);
+    if (key < L) to[key] = (from ? from[key] : 0.f) + sum[0][0];
 #endif
 }
 
