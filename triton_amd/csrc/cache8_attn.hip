@@ -404,10 +404,11 @@ static Plan8 plan8(const trn_cache8* c, int Hq, int Sq, bool weights) {
     p.n_chunks = 1; p.chunk_tiles = tiles32;
     if (p.sp) p.bytes += up(heads * p.R * p.sp * 4);
     else if (weights) {
-        // (three workgroups a compute unit, a chunk of four row tiles at least: a prompt of 1501, 32 heads of 128 on 8, us a call with one / two / three / four /
-        // six 86 / 75 / 72 / 77 / 81)
+        // (Two workgroups a compute unit, all that it holds; three for a prompt, half of whose queries and keys do not see each other; chunks of four row tiles
+        // at least.  32 heads of 128 on 8, us a call with one / two / three / four / six: prompts of 1501 82 / 65 / 61 / 66 / 63, of 4096 374 / 293 / 266 / 296 /
+        // 269; 512 queries, 4096 keys 80 / 70 / 77 / 73 / 75.)
         const int64_t blocks = heads * ((c->capacity + 255) / 256);
-        int64_t chunks = blocks ? 768 / blocks : 1;
+        int64_t chunks = blocks ? (2 * Sq > c->capacity ? 768 : 512) / blocks : 1;
         if (chunks > tiles32 / 4) chunks = tiles32 / 4;
         if (chunks > 1) {
             p.chunk_tiles = (int)((tiles32 + chunks - 1) / chunks);
