@@ -185,6 +185,22 @@ def test_attention_and_weights(case, layout):
     _hold(_attend(case, layout), case[7])
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("heads, causal", [((7, 8, 40), True), ((20, 16, 16), True), ((20, 16, 16), False)], ids=["two waves", "one wave", "one wave, all keys"])
+def test_row_tiles_of_fewer_waves(heads, causal, D):
+    """So many rows that two waves share a row tile's keys, or that one has them: most of the batch is padding, for the oracle's sake."""
+    B, Hkv, Hq = heads
+    M, S, block = (73, 90, 64) if Hq > Hkv else (150, 170, 32)
+    lengths = [S, 33, 0, 1, 64, 65, 32] + [40 + b for b in range(B - 7)]
+    counts = [M, 33, 2, 1, 5, 0, 70] + [1 + b % 3 for b in range(B - 7)]
+    case = (B, Hq, Hkv, D, M, S, block, lengths, counts, causal)
+    _hold(_attend(case, "token"), lengths)
+
+    def edit(k8, ks, v8, vs):
+        v8[:, :, 20] = 0x7f
+    _hold(_attend(case, edit=edit, spoil=False), lengths)
+
+
 @pytest.mark.parametrize("spread", [0.0, 4.0])
 @pytest.mark.parametrize("case", [ATTNS[3], ATTNS[8], ATTNS[6]], ids=["tiles", "split", "prompt"])
 def test_scales_that_differ_by_powers_and_by_nothing(case, spread):

@@ -13,7 +13,7 @@
 // that of p / vs, one multiplication a tile.  The reference m is a maximum of t: what counts for the output is near one in fp16, however
 // much the blocks differ.  (A block whose vs is below 2^-64 adds nothing that fp16 could hold; it counts in the sum alone.)
 //
-// Waves of a workgroup, and workgroups (shares) of a row tile, have consecutive runs of the keys that its rows see; their results
+// A row tile's waves (four, two or one of a workgroup), and workgroups (shares), have consecutive runs of the keys that its rows see; their results
 // are joined by (m, l, O) in LDS, and by a second launch.
 #include <type_traits>
 #include "cache8.h"
@@ -52,28 +52,30 @@ __device__ __forceinline__ float quad_max(float x) { float a = x, b = x; swap_ro
 __device__ __forceinline__ float quad_sum(float x) { float a = x, b = x; swap_rows16(a, b); return half_sum(a + b); }
 #endif
 
-// PAST: a single row tile reads the cache, each byte once (see plan8).
-template <int D, int NW, int NQ, bool PAST>
-__global__ __launch_bounds__(NW * 64, 2) void cache8_attn_kernel(const Attn8Args a) {
+// KS waves of the four have a row tile's keys, one after the other; 4 / KS row tiles a workgroup.  PAST: a single row tile reads the cache, each byte
+// once (see plan8).
+template <int D, int NQ, int KS, bool PAST>
+__global__ __launch_bounds__(256, 2) void cache8_attn_kernel(const Attn8Args a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    constexpr int NJ = D / 64, NDB = D / 16, RT = 16 * NQ;      // 16-byte K reads a lane and key half, of two contraction steps each; output blocks
+    constexpr int NW = 4, NG = NW / KS, NJ = D / 64, NDB = D / 16, RT = 16 * NQ;      // 16-byte K reads a lane and key half, of two contraction steps each; output blocks
     __shared__ __attribute__((aligned(1024))) uint8_t Ks0[NW * kTile<D>];
     __shared__ __attribute__((aligned(1024))) uint8_t Ks1[NW * kTile<D>];
     __shared__ __attribute__((aligned(1024))) uint8_t Vs0[NW * kTile<D>];
     __shared__ __attribute__((aligned(1024))) uint8_t Vs1[NW * kTile<D>];
-    __shared__ float ms[NW][RT], ls[NW][RT], m_all[RT], l_all[RT];
+    __shared__ float ms[NW][RT], ls[NW][RT], m_all[NG][RT], l_all[NG][RT];
 
     const int lane = threadIdx.x & 63, n = lane & 15, g4 = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // (workgroups of one share of a head, the row tiles apart, follow each other at the distance of all shares: one XCD where that is a
     // multiple of eight; the last rows, which see the most keys, first)
-    const int nth = a.by_units.of(blockIdx.x), unit = blockIdx.x - nth * a.by_units.d, rt = a.n_rt - 1 - nth;
+    const int nth = a.by_units.of(blockIdx.x), unit = blockIdx.x - nth * a.by_units.d, grp = wave / KS;
+    const int rt0 = ((a.n_rt - 1) / NG - nth) * NG, rt = rt0 + grp;
     const int bh = a.by_ns.of(unit), share = unit - bh * a.ns;
     const int b = a.by_hkv.of(bh), kvh = bh - b * a.Hkv;
 
     const int L = keys_of(a.lengths, b, a.cap), C = tokens_of(a.counts, b, a.Sq);
     const int rows = min(a.R, C * a.G);
-    if (rt * RT >= rows) return;                               // no row of this tile is there
+    if ((KS == 1 ? rt : rt0) * RT >= rows) return;             // no row of this tile, or of these, is there
     const int off = L - C;                                     // causal: query i sees keys <= i + off
     auto sees = [&](int row) { return a.causal ? min(L, max(0, a.by_g.of(row) + off + 1)) : L; };      // keys that a row sees: the first so many
     const int seen = sees(min(rt * RT + RT - 1, rows - 1)), all_see = sees(rt * RT);      // that some row sees, and all of them
@@ -91,7 +93,7 @@ __global__ __launch_bounds__(NW * 64, 2) void cache8_attn_kernel(const Attn8Args
     }
 
     // This wave's tiles, and the first of them that not all rows see whole.
-    const int T = (seen + 31) >> 5, w = share * NW + wave;
+    const int T = rt * RT < rows ? (seen + 31) >> 5 : 0, w = share * KS + wave % KS;
     const int t0 = a.by_w.of(T * w), t1 = a.by_w.of(T * (w + 1));       // (2^21 tiles and 512 waves at most)
     const int t_mask = min(t1, max(t0, all_see >> 5)), t_part = L >> 5;
     const int kpitch = (int)a.kst, vpitch = (int)a.vst, rest = L & 31;
@@ -303,17 +305,39 @@ __global__ __launch_bounds__(NW * 64, 2) void cache8_attn_kernel(const Attn8Args
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
 
-    // ---- the waves' results
+    // ---- a wave with rows of its own (never shared): out of its registers
+    if constexpr (KS == 1) {
+#pragma unroll
+        for (int qb = 0; qb < NQ; ++qb) {
+            const int r = rt * RT + 16 * qb + n, i0 = a.by_g.of(r), g0 = r - i0 * a.G;
+            const float sum = quad_sum(l[qb]), inv = sum == 0.f ? 0.f : 1.f / sum;
+            if (!there[qb]) continue;
+            half_t* const to = a.o + b * a.ob + (int64_t)(kvh * a.G + g0) * a.oh + (int64_t)i0 * a.os + 4 * g4;
+#pragma unroll
+            for (int i = 0; i < NDB; ++i) {
+                half4_t y;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = (half_t)(o[i][qb][e] * inv);
+                *reinterpret_cast<half4_t*>(to + 16 * i) = y;
+            }
+            if (g4 == 0) {
+                const float x = m[qb] + fast_log2(sum);            // (-inf for a row that sees nothing)
+                if (a.lse) a.lse[((int64_t)b * a.Hq + kvh * a.G + g0) * a.Sq + i0] = x * kLn2;
+                if (a.lse2) a.lse2[(int64_t)bh * a.R + r] = x;
+            }
+        }
+        return;
+    }
+    // ---- the results of a row tile's waves
 #pragma unroll
     for (int qb = 0; qb < NQ; ++qb) {
         l[qb] = quad_sum(l[qb]);
         if (g4 == 0) { ms[wave][16 * qb + n] = m[qb]; ls[wave][16 * qb + n] = l[qb]; }
     }
     __syncthreads();
-    // (a stage array holds RT rows of D floats of one wave in four; the 16-byte pieces of a row are swizzled by the row)
+    // (a stage array holds RT rows of D floats of one wave; the 16-byte pieces of a row are swizzled by the row)
     auto area = [&](int i) __attribute__((always_inline)) {
-        uint8_t* const base = i % 4 == 0 ? Ks0 : i % 4 == 1 ? Ks1 : i % 4 == 2 ? Vs0 : Vs1;
-        return reinterpret_cast<float4_t*>(base + (i / 4) * RT * D * 4);
+        return reinterpret_cast<float4_t*>(i == 0 ? Ks0 : i == 1 ? Ks1 : i == 2 ? Vs0 : Vs1);
     };
     float4_t* const mem = area(wave);
 #pragma unroll
@@ -321,21 +345,21 @@ __global__ __launch_bounds__(NW * 64, 2) void cache8_attn_kernel(const Attn8Args
         const int r = 16 * qb + n;
         float top = -INFINITY, sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < NW; ++i) top = fmaxf(top, ms[i][r]);
+        for (int i = grp * KS; i < grp * KS + KS; ++i) top = fmaxf(top, ms[i][r]);
 #pragma unroll
-        for (int i = 0; i < NW; ++i) sum = __builtin_fmaf(ls[i][r], ms[i][r] == -INFINITY ? 0.f : fast_exp2(ms[i][r] - top), sum);      // (a sum of NaN stays)
+        for (int i = grp * KS; i < grp * KS + KS; ++i) sum = __builtin_fmaf(ls[i][r], ms[i][r] == -INFINITY ? 0.f : fast_exp2(ms[i][r] - top), sum);      // (a sum of NaN stays)
         const float mine = m[qb] == -INFINITY ? 0.f : fast_exp2(m[qb] - top);
 #pragma unroll
         for (int i = 0; i < NDB; ++i) mem[r * (D / 4) + ((4 * i + g4) ^ n)] = o[i][qb] * mine;
-        if (wave == 0 && g4 == 0) { m_all[r] = top; l_all[r] = sum; }
+        if (wave % KS == 0 && g4 == 0) { m_all[grp][r] = top; l_all[grp][r] = sum; }
     }
     __syncthreads();
-    constexpr int TPR = NW * 64 / RT, NP = D / 4 / TPR;                // threads a row, 16-byte pieces a thread
+    constexpr int TPR = KS * 64 / RT, NP = D / 4 / TPR;                // threads a row, 16-byte pieces a thread
     static_assert(NP >= 1 && D / 4 >= 16, "a row's pieces for its threads, and for the swizzle");
-    const int orow = threadIdx.x / TPR, sub = threadIdx.x % TPR;
+    const int orow = threadIdx.x % (KS * 64) / TPR, sub = threadIdx.x % TPR;
     const int r = rt * RT + orow, i0 = a.by_g.of(r), g0 = r - i0 * a.G;
     if (r >= rows) return;
-    const float rm = m_all[orow], rl = l_all[orow];
+    const float rm = m_all[grp][orow], rl = l_all[grp][orow];
     const float inv = rl == 0.f ? 0.f : 1.f / rl;
     const int64_t at = (((int64_t)bh * a.n_rt + rt) * a.ns + share) * RT + orow;
 #pragma unroll
@@ -343,7 +367,7 @@ __global__ __launch_bounds__(NW * 64, 2) void cache8_attn_kernel(const Attn8Args
         const int piece = sub + i * TPR;
         float4_t x = zero;
 #pragma unroll
-        for (int k2 = 0; k2 < NW; ++k2) x = x + area(k2)[orow * (D / 4) + (piece ^ (orow & 15))];
+        for (int k2 = grp * KS; k2 < grp * KS + KS; ++k2) x = x + area(k2)[orow * (D / 4) + (piece ^ (orow & 15))];
         if (a.ns > 1) *reinterpret_cast<float4_t*>(a.part + at * D + 4 * piece) = x;
         else {
             half4_t y;
@@ -364,7 +388,7 @@ __global__ __launch_bounds__(NW * 64, 2) void cache8_attn_kernel(const Attn8Args
 }
 
 // ------------------------------------------------------------------------------------------------ host
-struct Plan8 { int G, R, nq, nw, n_rt, ns, n_chunks, chunk_tiles, sp; int64_t ml, lse2, more, bytes; };
+struct Plan8 { int G, R, nq, ks, n_rt, ns, n_chunks, chunk_tiles, sp; int64_t ml, lse2, more, bytes; };
 
 // Rows of a tile: 32 where they make workgroups enough, otherwise 16, whose waves have half the work a key and need half the registers.  us, tiles of
 // 16 / 32 rows, each with its best number of shares: 16 heads of 64, batch 4, 2000 keys, 64 queries (128 tiles of 32) 10.2 / 13.0, 300 (640) 23.6 / 21.6; 71
@@ -376,6 +400,11 @@ struct Plan8 { int G, R, nq, nw, n_rt, ns, n_chunks, chunk_tiles, sp; int64_t ml
 // second launch is some 3 us: without weights, which need it anyway, short caches have one share (512 keys 6.4, against 8.5; batch 8: 1025 keys 10.1 / 11.0; 16
 // heads of 64: 1025 keys 7.6 / 8.1, 2000 10.7 / 8.3; batch 16, 32 heads of 128, 2000 17.5 / 18.6).  Tiles of more than one read no more from memory than one does, and their waves rather
 // have a second workgroup beside them than walk long: 16 heads of 64, batch 4, 8000 keys, 20 queries 26.3 with two shares, 23.3 with four.
+// Waves that share a row tile's keys: four where no more row tiles are there than two workgroups a compute unit hold; with more the
+// frame of a workgroup (queries, first keys, joining: a fifth to a half of a short prompt's time) is spent less often by two waves, or one that has all
+// keys.  us with four / two / one, 32 heads of 128 on 8, row tiles of 32: one prompt of 512 (512 row tiles) 11.2 / 12.5 / 17.5, of 1501 (1504) 37.7 / 34.8 /
+// 40.6; 512 queries on 8448 keys (512) 82.8 / 94.1 / 177; two of 300 (608) 14.0 / 11.5 / 13.2; four of 512 (2048) 34.8 / 24.6 / 24.0, of 2047 (8192) 213 / 180 /
+// 161; 71 heads of 64 on one, 700 (1554) 17.8 / 15.3 / 16.4, four of them 57.7 / 42.8 / 36.1.
 // A cache that is read by one row tile goes past the caches (each byte once), us through / past: batch 32, 8192 keys 99.5 / 89.4, one sequence of 131072 56.7 /
 // 51.2, of 4000 11.2 / 10.6; with two row tiles and more the others find it there: 64 rows, 16000 keys 18.7 / 20.6.
 static Plan8 plan8(const trn_cache8* c, int Hq, int Sq, bool weights) {
@@ -385,14 +414,15 @@ static Plan8 plan8(const trn_cache8* c, int Hq, int Sq, bool weights) {
     p.R = p.G * Sq;
     const int64_t heads = (int64_t)c->batch * c->n_kv_heads, tiles = (c->capacity + 31) / 32;
     p.nq = p.R > 16 && heads * ((p.R + 31) / 32) >= (d128 ? 128 : 320) ? 2 : 1;
-    p.nw = 4;
     p.n_rt = (p.R + 16 * p.nq - 1) / (16 * p.nq);
     const int64_t units = heads * p.n_rt;
     int64_t ns = units ? 256 / units : 1;
-    if (p.n_rt > 1 && ns >= 1 && tiles > 24 * p.nw * ns) ns *= 2;
+    if (p.n_rt > 1 && ns >= 1 && tiles > 96 * ns) ns *= 2;
     if (!weights && tiles <= (d128 ? 26 : 34) + units / 2) ns = 1;
     if (ns > tiles) ns = tiles;
     p.ns = (int)(ns < 1 ? 1 : ns > 64 ? 64 : ns);
+    const int64_t row_tiles = heads * p.n_rt;
+    p.ks = p.nq == 1 || row_tiles <= 512 ? 4 : row_tiles < 1600 ? 2 : 1;      // (there is one share from 256 row tiles on)
     auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
     p.ml = p.ns > 1 ? up(units * p.ns * 16 * p.nq * c->head_dim * 4) : 0;
     p.lse2 = p.ml + (p.ns > 1 ? up(units * p.ns * 32 * p.nq * 4) : 0);
@@ -469,7 +499,7 @@ extern "C" int trn_cache8_attn_f16(const trn_cache8* c, const void* q, void* o, 
     a.bshift = c->block == 32 ? 5 : c->block == 64 ? 6 : 7;
     const int64_t heads = (int64_t)c->batch * c->n_kv_heads, units = heads * p.ns;
     if (units * p.n_rt > 0x7fffffffLL || heads * ((int64_t)p.R + 1) > 0x7fffffffLL || heads * ((c->capacity + 255) / 256) * p.n_chunks > 0x3fffffffLL) return TRN_E_SHAPE;
-    a.by_units = Div(units); a.by_g = Div(p.G); a.by_hkv = Div(c->n_kv_heads); a.by_ns = Div(p.ns); a.by_w = Div(p.nw * p.ns);
+    a.by_units = Div(units); a.by_g = Div(p.G); a.by_hkv = Div(c->n_kv_heads); a.by_ns = Div(p.ns); a.by_w = Div(p.ks * p.ns);
     a.kb = c->k_stride_b; a.kh = c->k_stride_h; a.kst = c->k_stride_s;
     a.vb = c->v_stride_b; a.vh = c->v_stride_h; a.vst = c->v_stride_s;
     a.ksb = c->ks_stride_b; a.ksh = c->ks_stride_h; a.vsb = c->vs_stride_b; a.vsh = c->vs_stride_h;
@@ -482,13 +512,15 @@ extern "C" int trn_cache8_attn_f16(const trn_cache8* c, const void* q, void* o, 
     a.n_chunks = p.n_chunks; a.chunk_tiles = p.chunk_tiles; a.w_part = p.n_chunks > 1 ? (float*)((char*)workspace + p.more) : nullptr;
     const hipStream_t s = (hipStream_t)stream;
     const bool d128 = c->head_dim == 128;
-    const dim3 grid((unsigned)(units * p.n_rt)), block(p.nw * 64);
-#define TRN_ATTN8(D, NW, NQ) do { if (p.n_rt == 1) hipLaunchKernelGGL((cache8_attn_kernel<D, NW, NQ, true>), grid, block, 0, s, a); \
-                                  else hipLaunchKernelGGL((cache8_attn_kernel<D, NW, NQ, false>), grid, block, 0, s, a); } while (0)
-    if (d128 && p.nq == 1) TRN_ATTN8(128, 4, 1);
-    else if (d128) TRN_ATTN8(128, 4, 2);
-    else if (p.nq == 1) TRN_ATTN8(64, 4, 1);
-    else TRN_ATTN8(64, 4, 2);
+    const int per = 4 / p.ks;
+    const dim3 grid((unsigned)(units * ((p.n_rt + per - 1) / per))), block(256);
+#define TRN_ATTN8(D, NQ, KS, PAST) hipLaunchKernelGGL((cache8_attn_kernel<D, NQ, KS, PAST>), grid, block, 0, s, a)
+#define TRN_ATTN8_OF(D) do { if (p.nq == 1 && p.n_rt == 1) TRN_ATTN8(D, 1, 4, true); else if (p.nq == 1) TRN_ATTN8(D, 1, 4, false); \
+                             else if (p.n_rt == 1) TRN_ATTN8(D, 2, 4, true); else if (p.ks == 4) TRN_ATTN8(D, 2, 4, false); \
+                             else if (p.ks == 2) TRN_ATTN8(D, 2, 2, false); else TRN_ATTN8(D, 2, 1, false); } while (0)
+    if (d128) TRN_ATTN8_OF(128);
+    else TRN_ATTN8_OF(64);
+#undef TRN_ATTN8_OF
 #undef TRN_ATTN8
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && (p.ns > 1 || p.sp)) e = launch_cache8_finish(a, c->head_dim, s);
