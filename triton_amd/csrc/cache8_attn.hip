@@ -68,7 +68,7 @@ __global__ __launch_bounds__(256, 2) void cache8_attn_kernel(const Attn8Args a) 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // (workgroups of one share of a head, the row tiles apart, follow each other at the distance of all shares: one XCD where that is a
     // multiple of eight; the last rows, which see the most keys, first)
-    const int nth = a.by_units.of(blockIdx.x), unit = blockIdx.x - nth * a.by_units.d, grp = wave / KS;
+    const int nth = a.by_units.of(blockIdx.x), unit = blockIdx.x - nth * a.by_units.d, grp = KS == NW ? 0 : wave / KS;
     const int rt0 = ((a.n_rt - 1) / NG - nth) * NG, rt = rt0 + grp;
     const int bh = a.by_ns.of(unit), share = unit - bh * a.ns;
     const int b = a.by_hkv.of(bh), kvh = bh - b * a.Hkv;
@@ -93,7 +93,7 @@ __global__ __launch_bounds__(256, 2) void cache8_attn_kernel(const Attn8Args a) 
     }
 
     // This wave's tiles, and the first of them that not all rows see whole.
-    const int T = rt * RT < rows ? (seen + 31) >> 5 : 0, w = share * KS + wave % KS;
+    const int T = rt * RT < rows ? (seen + 31) >> 5 : 0, w = share * KS + (KS == NW ? wave : wave % KS);
     const int t0 = a.by_w.of(T * w), t1 = a.by_w.of(T * (w + 1));       // (2^21 tiles and 512 waves at most)
     const int t_mask = min(t1, max(t0, all_see >> 5)), t_part = L >> 5;
     const int kpitch = (int)a.kst, vpitch = (int)a.vst, rest = L & 31;
@@ -351,7 +351,7 @@ __global__ __launch_bounds__(256, 2) void cache8_attn_kernel(const Attn8Args a) 
         const float mine = m[qb] == -INFINITY ? 0.f : fast_exp2(m[qb] - top);
 #pragma unroll
         for (int i = 0; i < NDB; ++i) mem[r * (D / 4) + ((4 * i + g4) ^ n)] = o[i][qb] * mine;
-        if (wave % KS == 0 && g4 == 0) { m_all[grp][r] = top; l_all[grp][r] = sum; }
+        if (wave == grp * KS && g4 == 0) { m_all[grp][r] = top; l_all[grp][r] = sum; }
     }
     __syncthreads();
     constexpr int TPR = KS * 64 / RT, NP = D / 4 / TPR;                // threads a row, 16-byte pieces a thread
