@@ -164,6 +164,8 @@ hipError_t launch_cache8_finish(const Attn8Args& a, int head_dim, hipStream_t s)
     return hipGetLastError();
 }
 
+// A prompt of 1501, 32 heads of 128 on 8: 23.4 us -- launch and the end of the chunks that see nothing 4.8, the first queries and keys and one tile 5, the
+// sums over lanes 1, eleven tiles 12, near what their exponentials and products take.
 // The weights that 256 keys get from a chunk of row tiles.  A wave has 64 keys, whose codes it holds as operands (A, two blocks of 32); the
 // tile's queries (B) come through LDS, for all four waves, one tile ahead.  Per row and key: one exponential, one multiply-add and one addition.
 template <int D>
