@@ -128,6 +128,8 @@ ATTNS = [
     (1, 4, 2, 128, 1, 1100, 32, [1100], [1], True),
     (2, 8, 2, 128, 150, 400, 64, [400, 260], [150, 101], True),  # many rows: the weights in chunks of row tiles
     (1, 71, 1, 64, 9, 700, 32, [611], [9], False),
+    (1, 32, 2, 64, 3, 2600, 64, [2555], [3], True),              # shares, and the weights of many rows behind them
+    (2, 12, 2, 128, 4, 1500, 32, [1500, 901], [4, 2], True),
 ]
 
 

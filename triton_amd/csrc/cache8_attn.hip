@@ -402,9 +402,10 @@ struct Plan8 { int G, R, nq, ks, n_rt, ns, n_chunks, chunk_tiles, sp; int64_t ml
 // Shares of a row tile's keys: one workgroup a compute unit over the launch -- one share from some 160 row tiles on --, no more shares than tiles of 32 keys.  32 heads
 // of 128 on 8, one query, us with 1 / 2 / 4 / 8 / 16 / 32 shares: 1025 keys 9.6 / 10.9 / 9.5 / 9.3 / 9.0 / 8.9; batch 8, 1500 keys 12.0 / 12.4 / 11.9 / 12.5 / 16.6; batch 12, 3000
 // 23.7 / 19.5 / 20.8; batch 16, 4097 31.3 / 28.6 / 28.4; batch 24, 4000 33.9 / 41.6 / 39.9; batch 32, 8192 88.7 / 91.4 / 93.8; of two to one lengths 70.5 / 72.2 / 70.8.  A
-// second launch is some 3 us: without weights, which need it anyway, short caches have one share (512 keys 6.4, against 8.5; batch 8: 1025 keys 10.1 / 11.0; 16
+// second launch is some 3 us: short caches have one share, but where few rows' weights need that launch anyway (512 keys 6.4, against 8.5; batch 8: 1025 keys 10.1 / 11.0; 16
 // heads of 64: 1025 keys 7.6 / 8.1, 2000 10.7 / 8.3; batch 16, 32 heads of 128, 2000 17.5 / 18.6).  Tiles of more than one read no more from memory than one does, and their waves rather
-// have a second workgroup beside them than walk long: 16 heads of 64, batch 4, 8000 keys, 20 queries 26.3 with two shares, 23.3 with four.
+// have a second workgroup beside them than walk long, of 64 a third and fourth: 16 heads of 64, batch 4, 8000 keys, 20 queries 26.3 with two shares, 23.3 with four;
+// 71 on one, batch 28, 11316 keys, one query, with 1 / 2 / 4 / 8 40.8 / 32.0 / 26.4 / 28.5.
 // Waves that share a row tile's keys: four where no more row tiles are there than two workgroups a compute unit hold; with more the
 // frame of a workgroup (queries, first keys, joining: a fifth to a half of a short prompt's time) is spent less often by two waves, or one that has all
 // keys.  us with four / two / one, 32 heads of 128 on 8, row tiles of 32: one prompt of 512 (512 row tiles) 11.2 / 12.5 / 17.5, of 1501 (1504) 37.7 / 34.8 /
@@ -422,8 +423,10 @@ static Plan8 plan8(const trn_cache8* c, int Hq, int Sq, bool weights) {
     p.n_rt = (p.R + 16 * p.nq - 1) / (16 * p.nq);
     const int64_t units = heads * p.n_rt;
     int64_t ns = units ? 256 / units : 1;
-    if (p.n_rt > 1 && ns >= 1 && tiles > 96 * ns) ns *= 2;
-    if (!weights && tiles <= (d128 ? 26 : 34) + units / 2) ns = 1;
+    while (p.n_rt > 1 && ns >= 1 && tiles > 96 * ns && units * ns <= (d128 ? 256 : 512)) ns *= 2;
+    // (key weights: a score of 4 bytes goes out and comes back for each row and key, or K is read again)
+    p.sp = weights && 8 * p.R <= c->head_dim ? (int)tiles * 32 : 0;
+    if (!p.sp && tiles <= (d128 ? 26 : 34) + units / 2) ns = 1;
     if (ns > tiles) ns = tiles;
     p.ns = (int)(ns < 1 ? 1 : ns > 64 ? 64 : ns);
     const int64_t row_tiles = heads * p.n_rt;
@@ -433,18 +436,16 @@ static Plan8 plan8(const trn_cache8* c, int Hq, int Sq, bool weights) {
     p.lse2 = p.ml + (p.ns > 1 ? up(units * p.ns * 32 * p.nq * 4) : 0);
     p.more = p.lse2 + (weights ? up(heads * p.R * 4) : 0);
     p.bytes = p.more;
-    // Key weights: a score of 4 bytes goes out and comes back for each row and key, or K is read again.
-    p.sp = weights && 8 * p.R <= c->head_dim ? (int)tiles * 32 : 0;
     const int tiles32 = (p.R + 31) / 32;
     p.n_chunks = 1; p.chunk_tiles = tiles32;
     if (p.sp) p.bytes += up(heads * p.R * p.sp * 4);
     else if (weights) {
-        // (Two workgroups a compute unit, all that it holds; three for a prompt, half of whose queries and keys do not see each other; chunks of four row tiles
-        // at least.  32 heads of 128 on 8, us a call with one / two / three / four / six: prompts of 1501 82 / 65 / 61 / 66 / 63, of 4096 374 / 293 / 266 / 296 /
+        // (Two workgroups a compute unit, all that it holds; three for a prompt, half of whose queries and keys do not see each other; chunks of two row tiles
+        // at least (a prompt of 128 with chunks of one / two / four / six 12.5 / 13.2 / 15.6 / 19.0, of 300 23.3 / 19.3 / 20.5 / 23.2).  32 heads of 128 on 8, us a call with one / two / three / four / six: prompts of 1501 82 / 65 / 61 / 66 / 63, of 4096 374 / 293 / 266 / 296 /
         // 269; 512 queries, 4096 keys 80 / 70 / 77 / 73 / 75.)
         const int64_t blocks = heads * ((c->capacity + 255) / 256);
         int64_t chunks = blocks ? (2 * Sq > c->capacity ? 768 : 512) / blocks : 1;
-        if (chunks > tiles32 / 4) chunks = tiles32 / 4;
+        if (chunks > tiles32 / 2) chunks = tiles32 / 2;
         if (chunks > 1) {
             p.chunk_tiles = (int)((tiles32 + chunks - 1) / chunks);
             p.n_chunks = (tiles32 + p.chunk_tiles - 1) / p.chunk_tiles;
