@@ -31,8 +31,8 @@ struct EvictArgs {
     float* scales;                     // 8 bits: [2][B Hkv][n_blocks], the scales as they were
     int n_blocks;
     int32_t* now;                      // [2][B]: keys that stay, and that there were
-    int chunks, cols;                  // move: workgroups of a head's rows and columns
-    Div by_hkv, by_chunks, by_cols;
+    int chunks;                        // move: workgroups of a head's rows
+    Div by_hkv, by_chunks, by_heads2;
 };
 
 // Larger numbers first, NaN last of all.
@@ -226,107 +226,161 @@ __global__ __launch_bounds__(1024) void cache_evict_select_kernel(const EvictArg
 #endif
 }
 
-// All that this wave has requested from memory is there: a barrier alone does not say so of loads whose values are used behind it.
-__device__ __forceinline__ void loaded() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-
-// Workgroups from n_rows on: (head of a sequence, K or V, chunk of rows, column).  The first: the weights of the kept keys, one for each row of
-// them, and the new lengths.
-template <bool BITS8>
-__global__ __launch_bounds__(256) void cache_evict_move_kernel(const EvictArgs a, int row_pieces, int piece_shift, int rows_per_chunk, int n_rows) {
-    const int tid = threadIdx.x;
-    if ((int)blockIdx.x < n_rows) {
-        const int row = blockIdx.x, b = row / a.Hw, hw = row - b * a.Hw;
-        const int stay = a.now[b];
-        if (hw == 0 && tid == 0 && a.new_lengths) a.new_lengths[b] = stay;
-        if (!a.w_out) return;
-        const int32_t* kept = a.kept + ((int64_t)b * a.Hkv + hw / (a.Hw / a.Hkv)) * a.keep;
-        const int64_t from = (int64_t)row * a.S;
-        // (w_out may be w, whose rows are S apart, or a tensor of its own with rows of `keep`)
-        const int64_t to = a.w_out == a.w ? from : (int64_t)row * a.keep;
-        constexpr int NW = 4;
-        for (int i0 = 0; i0 < stay; i0 += NW * 256) {
-            float x[NW]; int j[NW];
-#pragma unroll
-            for (int e = 0; e < NW; ++e) j[e] = kept[min(i0 + e * 256 + tid, stay - 1)];
-            if (a.w_half) {
-#pragma unroll
-                for (int e = 0; e < NW; ++e) x[e] = (float)static_cast<const half_t*>(a.w)[from + j[e]];
-            } else {
-#pragma unroll
-                for (int e = 0; e < NW; ++e) x[e] = static_cast<const float*>(a.w)[from + j[e]];
-            }
-            loaded();
-            __syncthreads();
-#pragma unroll
-            for (int e = 0; e < NW; ++e) {
-                const int i = i0 + e * 256 + tid;
-                if (i < stay) {
-                    if (a.w_half) static_cast<half_t*>(a.w_out)[to + i] = (half_t)x[e];
-                    else static_cast<float*>(a.w_out)[to + i] = x[e];
-                }
-            }
-        }
-        // (the places that new keys will take have gathered nothing)
-        if (a.w_out == a.w) {
-            const int n = a.now[a.B + b];
-            for (int i = stay + tid; i < n; i += 256) {
-                if (a.w_half) static_cast<half_t*>(a.w_out)[to + i] = (half_t)0.f;
-                else static_cast<float*>(a.w_out)[to + i] = 0.f;
-            }
-        }
-        return;
-    }
-    int u = blockIdx.x - n_rows;
-    const int v2 = a.by_cols.of(u), col = u - v2 * a.cols;
-    u = a.by_chunks.of(v2);
-    const int chunk = v2 - u * a.chunks, kv = u & 1, bh = u >> 1;
-    const int b = a.by_hkv.of(bh), h = bh - b * a.Hkv;
+// Of a row of weights: those of the kept keys, to the front; and the new lengths.
+template <int THREADS>
+__device__ __forceinline__ void move_weights(const EvictArgs& a, int row) {
+    const int tid = threadIdx.x, b = row / a.Hw, hw = row - b * a.Hw;
     const int stay = a.now[b];
-    const int from = chunk * rows_per_chunk, to = min(stay, from + rows_per_chunk);
+    if (hw == 0 && tid == 0 && a.new_lengths) a.new_lengths[b] = stay;
+    if (!a.w_out) return;
+    const int32_t* kept = a.kept + ((int64_t)b * a.Hkv + hw / (a.Hw / a.Hkv)) * a.keep;
+    const int64_t from = (int64_t)row * a.S;
+    // (w_out may be w, whose rows are S apart, or a tensor of its own with rows of `keep`)
+    const int64_t to = a.w_out == a.w ? from : (int64_t)row * a.keep;
+    constexpr int NW = 4;
+    for (int i0 = 0; i0 < stay; i0 += NW * THREADS) {
+        float x[NW]; int j[NW];
+#pragma unroll
+        for (int e = 0; e < NW; ++e) j[e] = kept[min(i0 + e * THREADS + tid, stay - 1)];
+        if (a.w_half) {
+#pragma unroll
+            for (int e = 0; e < NW; ++e) x[e] = (float)static_cast<const half_t*>(a.w)[from + j[e]];
+        } else {
+#pragma unroll
+            for (int e = 0; e < NW; ++e) x[e] = static_cast<const float*>(a.w)[from + j[e]];
+        }
+        // (in place: what this step overwrites has been read; a barrier alone does not wait for loads whose values are used behind it)
+#pragma unroll
+        for (int e = 0; e < NW; ++e) asm volatile("" : "+v"(x[e]));
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < NW; ++e) {
+            const int i = i0 + e * THREADS + tid;
+            if (i < stay) {
+                if (a.w_half) static_cast<half_t*>(a.w_out)[to + i] = (half_t)x[e];
+                else static_cast<float*>(a.w_out)[to + i] = x[e];
+            }
+        }
+    }
+    // (the places that new keys will take have gathered nothing)
+    if (a.w_out == a.w) {
+        const int n = a.now[a.B + b];
+        for (int i = stay + tid; i < n; i += THREADS) {
+            if (a.w_half) static_cast<half_t*>(a.w_out)[to + i] = (half_t)0.f;
+            else static_cast<float*>(a.w_out)[to + i] = 0.f;
+        }
+    }
+}
+
+// 8 bits: by what the codes of the rows of this step, one a thread, are multiplied, and the scales of their blocks (whole ones) -- the largest of
+// those that the rows come with.  Holds two barriers.
+__device__ __forceinline__ void block_scales(const EvictArgs& a, float s, float* top, float* ratio, bool writes, float* scales_out, int row) {
+    const int tid = threadIdx.x;
+    float t = s;
+#pragma unroll
+    for (int m = 16; m >= 1; m >>= 1) t = fmaxf(t, __shfl_xor(t, m, 64));
+    if ((tid & 31) == 0) top[tid >> 5] = t;
+    __syncthreads();
+    const int groups = 1 << (a.bshift - 5), g0 = (tid >> 5) & ~(groups - 1);
+    for (int i = 0; i < groups; ++i) t = fmaxf(t, top[g0 + i]);
+    ratio[tid] = t > 0.f ? s / t : 1.f;
+    if (writes && (tid & ((1 << a.bshift) - 1)) == 0) scales_out[row >> a.bshift] = t;
+    __syncthreads();
+}
+__device__ __forceinline__ uint4_t recoded(uint4_t x, float f) {
+    return f != 1.f ? uint4_t{recoded(x.x, f), recoded(x.y, f), recoded(x.z, f), recoded(x.w, f)} : x;
+}
+
+// Into another cache.  Workgroups from n_rows on: (head of a sequence, K or V, chunk of rows).  The first: a row of weights each.
+template <bool BITS8>
+__global__ __launch_bounds__(256) void cache_evict_move_kernel(const EvictArgs a, int piece_shift, int n_rows) {
+    const int tid = threadIdx.x;
+    if ((int)blockIdx.x < n_rows) { move_weights<256>(a, blockIdx.x); return; }
+    constexpr int NB = 4;      // rows of a lane on their way at once
+    const int u = a.by_chunks.of(blockIdx.x - n_rows), chunk = blockIdx.x - n_rows - u * a.chunks, kv = u & 1, bh = u >> 1;
+    const int b = a.by_hkv.of(bh), h = bh - b * a.Hkv;
+    const int stay = a.now[b], step = 256 >> piece_shift;
+    const int from = chunk * NB * step, to = min(stay, from + NB * step);
     if (from >= to) return;
     const int32_t* kept = a.kept + (int64_t)bh * a.keep;
     const char* src = (const char*)(kv ? a.v : a.k) + b * a.st[kv][0] + h * a.st[kv][1];
     char* dst = (char*)(kv ? a.v_out : a.k_out) + b * a.ot[kv][0] + h * a.ot[kv][1];
-    const int sub = tid & (row_pieces - 1), r0 = tid >> piece_shift, step = 256 >> piece_shift;
-    const int off = (col * row_pieces + sub) * 16;
-    constexpr int NB = 4;      // rows of a lane on their way at once
-    __shared__ float ratio[256], top[8];
-    for (int i0 = from; i0 < to; i0 += NB * step) {
-        uint4_t x[NB]; int j[NB];
+    const int r0 = tid >> piece_shift, off = (tid & ((1 << piece_shift) - 1)) * 16;
+    uint4_t x[NB]; int j[NB];
 #pragma unroll
-        for (int e = 0; e < NB; ++e) j[e] = kept[min(i0 + e * step + r0, to - 1)];
+    for (int e = 0; e < NB; ++e) j[e] = kept[min(from + e * step + r0, to - 1)];
+#pragma unroll
+    for (int e = 0; e < NB; ++e) x[e] = __builtin_nontemporal_load(reinterpret_cast<const uint4_t*>(src + (int64_t)j[e] * a.st[kv][2] + off));
+    __shared__ float ratio[256], top[8];
+    if constexpr (BITS8) {
+        const float* was = a.scales + ((int64_t)kv * a.B * a.Hkv + bh) * a.n_blocks;
+        const bool mine = tid < NB * step && from + tid < to;
+        block_scales(a, mine ? was[kept[from + tid] >> a.bshift] : 0.f, top, ratio, mine, (kv ? a.vs_out : a.ks_out) + b * a.sot[kv][0] + h * a.sot[kv][1], from + tid);
+    }
+#pragma unroll
+    for (int e = 0; e < NB; ++e) {
+        const int i = from + e * step + r0;
+        if (i < to) {
+            if constexpr (BITS8) x[e] = recoded(x[e], ratio[e * step + r0]);
+            __builtin_nontemporal_store(x[e], reinterpret_cast<uint4_t*>(dst + (int64_t)i * a.ot[kv][2] + off));
+        }
+    }
+}
+
+// Within the same cache.  Workgroups from n_rows on: (column, head of a sequence, K or V); the columns of a head as far apart as there are heads, on one XCD
+// where those are a multiple of four.  A step's rows are requested before the last one's are stored: they lie behind all that those overwrite.
+template <bool BITS8>
+__global__ __launch_bounds__(1024) void cache_evict_shift_kernel(const EvictArgs a, int piece_shift, int n_rows) {
+    const int tid = threadIdx.x;
+    if ((int)blockIdx.x < n_rows) { move_weights<1024>(a, blockIdx.x); return; }
+    constexpr int NB = 4;
+    const int col = a.by_heads2.of(blockIdx.x - n_rows), u = blockIdx.x - n_rows - col * a.by_heads2.d, kv = u & 1, bh = u >> 1;
+    const int b = a.by_hkv.of(bh), h = bh - b * a.Hkv;
+    const int stay = a.now[b], rows = 1024 >> piece_shift, step = NB * rows;
+    if (stay == 0) return;
+    const int32_t* kept = a.kept + (int64_t)bh * a.keep;
+    const char* src = (const char*)(kv ? a.v : a.k) + b * a.st[kv][0] + h * a.st[kv][1];
+    char* dst = (char*)(kv ? a.v_out : a.k_out) + b * a.ot[kv][0] + h * a.ot[kv][1];
+    const int r0 = tid >> piece_shift, off = ((col << piece_shift) + (tid & ((1 << piece_shift) - 1))) * 16;
+    const float* was = BITS8 ? a.scales + ((int64_t)kv * a.B * a.Hkv + bh) * a.n_blocks : nullptr;
+    float* const scales_out = BITS8 ? (kv ? a.vs_out : a.ks_out) + b * a.sot[kv][0] + h * a.sot[kv][1] : nullptr;
+    __shared__ float ratio[1024], top[32];
+    // (past the last row that one again: a row that is there, and goes nowhere)
+    auto places = [&](int i0, int (&j)[NB], int& own) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < NB; ++e) j[e] = kept[min(i0 + e * rows + r0, stay - 1)];
+        if constexpr (BITS8) own = kept[min(i0 + tid, stay - 1)];
+    };
+    auto request = [&](const int (&j)[NB], int own, uint4_t (&x)[NB], float& s) __attribute__((always_inline)) {
 #pragma unroll
         for (int e = 0; e < NB; ++e) x[e] = __builtin_nontemporal_load(reinterpret_cast<const uint4_t*>(src + (int64_t)j[e] * a.st[kv][2] + off));
-        // 8 bits: the blocks of these rows (128 or 256: whole blocks) and what their codes are to be multiplied by
-        if constexpr (BITS8) {
-            const float* was = a.scales + ((int64_t)kv * a.B * a.Hkv + bh) * a.n_blocks;
-            const float s = tid < NB * step && i0 + tid < to ? was[kept[i0 + tid] >> a.bshift] : 0.f;
-            float t = s;
+        if constexpr (BITS8) s = was[own >> a.bshift];
+    };
+    uint4_t x[NB], x_next[NB]; int j[NB], own = 0; float s = 0.f, s_next = 0.f;
+    places(0, j, own);
+    request(j, own, x, s);
+    places(step, j, own);
+    for (int i0 = 0; i0 < stay; i0 += step) {
+        request(j, own, x_next, s_next);
+        places(i0 + 2 * step, j, own);
+        // (what this step overwrites has been read by all waves: a barrier alone does not wait for loads whose values are used behind it)
 #pragma unroll
-            for (int m = 16; m >= 1; m >>= 1) t = fmaxf(t, __shfl_xor(t, m, 64));
-            if ((tid & 31) == 0) top[tid >> 5] = t;
-            __syncthreads();
-            const int groups = 1 << (a.bshift - 5), g0 = (tid >> 5) & ~(groups - 1);
-            for (int i = 0; i < groups; ++i) t = fmaxf(t, top[g0 + i]);
-            ratio[tid] = t > 0.f ? s / t : 1.f;
-            if (col == 0 && (tid & ((1 << a.bshift) - 1)) == 0 && tid < NB * step && i0 + tid < to)
-                ((kv ? a.vs_out : a.ks_out) + b * a.sot[kv][0] + h * a.sot[kv][1])[(i0 + tid) >> a.bshift] = t;
-        }
-        // (what this step overwrites has been read)
-        if (a.in_place[kv]) loaded();
-        if (BITS8 || a.in_place[kv]) __syncthreads();
+        for (int e = 0; e < NB; ++e) asm volatile("" : "+v"(x[e]));
+        if constexpr (BITS8) {
+            const bool mine = tid < step && i0 + tid < stay;
+            block_scales(a, mine ? s : 0.f, top, ratio, mine && col == 0, scales_out, i0 + tid);
+        } else __syncthreads();
 #pragma unroll
         for (int e = 0; e < NB; ++e) {
-            const int i = i0 + e * step + r0;
-            if (i < to) {
-                if constexpr (BITS8) {
-                    const float f = ratio[e * step + r0];
-                    if (f != 1.f) x[e] = uint4_t{recoded(x[e].x, f), recoded(x[e].y, f), recoded(x[e].z, f), recoded(x[e].w, f)};
-                }
+            const int i = i0 + e * rows + r0;
+            if (i < stay) {
+                if constexpr (BITS8) x[e] = recoded(x[e], ratio[e * rows + r0]);
                 __builtin_nontemporal_store(x[e], reinterpret_cast<uint4_t*>(dst + (int64_t)i * a.ot[kv][2] + off));
             }
+            x[e] = x_next[e];
         }
-        if (BITS8 && i0 + NB * step < to) __syncthreads();      // (`ratio` and `top` are written again)
+        s = s_next;
+        if constexpr (BITS8) __syncthreads();      // (`ratio` and `top` are written again)
     }
 }
 
@@ -416,21 +470,20 @@ extern "C" int trn_cache_evict(const trn_cache_evict_desc* e, const void* k, con
     a.n_blocks = bits8 ? (e->keys + e->block - 1) / e->block : 0;
     a.now = (int32_t*)((char*)workspace + sz.now);
     const int64_t heads = (int64_t)e->batch * e->n_kv_heads;
-    if (heads > 0x7fffffff || (int64_t)e->batch * e->n_weight_rows > 0x7fffffff) return TRN_E_SHAPE;
+    if (heads > 0x3fffffff || (int64_t)e->batch * e->n_weight_rows > 0x7fffffff) return TRN_E_SHAPE;
     a.by_hkv = Div(e->n_kv_heads);
-    // rows shared out, or in columns of 64 bytes
-    const bool columns = a.in_place[0] || a.in_place[1];
-    const int pieces = width / 16, row_pieces = columns ? 4 : pieces;
-    int shift = 0;
-    while ((1 << shift) < row_pieces) ++shift;
-    const int rows_per_chunk = columns ? rows_out : 4 * (256 / row_pieces);
-    a.cols = pieces / row_pieces;
+    // Rows are shared out; or within the same cache, columns: as wide as leaves a workgroup for each compute unit, 64 bytes at least.
+    const bool within = a.in_place[0] || a.in_place[1];
+    const int pieces = width / 16;
+    int shift = 2;
+    while ((1 << shift) < pieces && (!within || 2 * heads * (pieces >> (shift + 1)) >= 256)) ++shift;
+    const int rows_per_chunk = 4 * (256 >> shift);
     a.chunks = (rows_out + rows_per_chunk - 1) / rows_per_chunk;
-    const int64_t n_rows = weights_out || new_lengths ? (int64_t)e->batch * e->n_weight_rows : 0, grid = n_rows + 2 * heads * a.chunks * a.cols;
+    const int64_t n_rows = weights_out || new_lengths ? (int64_t)e->batch * e->n_weight_rows : 0, grid = n_rows + 2 * heads * (within ? pieces >> shift : a.chunks);
     a.summed = orders_stored(e);
     const int64_t sums = heads * ((e->keys + 255) / 256);
     if (grid > 0x7fffffffLL || sums > 0x7fffffffLL) return TRN_E_SHAPE;
-    a.by_cols = Div(a.cols); a.by_chunks = Div(a.chunks);
+    a.by_chunks = Div(a.chunks); a.by_heads2 = Div(2 * heads);
     const hipStream_t s = (hipStream_t)stream;
     if (a.summed) hipLaunchKernelGGL(cache_evict_sums_kernel, dim3((unsigned)sums), dim3(256), 0, s, a);
     const dim3 sel((unsigned)heads);
@@ -439,7 +492,10 @@ extern "C" int trn_cache_evict(const trn_cache_evict_desc* e, const void* k, con
     else if (e->keys <= 16384) hipLaunchKernelGGL(cache_evict_select_kernel<16>, sel, dim3(1024), 0, s, a);
     else if (e->keys <= kMostKept) hipLaunchKernelGGL(cache_evict_select_kernel<32>, sel, dim3(1024), 0, s, a);
     else hipLaunchKernelGGL(cache_evict_select_kernel<0>, sel, dim3(1024), 0, s, a);
-    if (bits8) hipLaunchKernelGGL((cache_evict_move_kernel<true>), dim3((unsigned)grid), dim3(256), 0, s, a, row_pieces, shift, rows_per_chunk, (int)n_rows);
-    else hipLaunchKernelGGL((cache_evict_move_kernel<false>), dim3((unsigned)grid), dim3(256), 0, s, a, row_pieces, shift, rows_per_chunk, (int)n_rows);
+    const dim3 all((unsigned)grid);
+    if (within && bits8) hipLaunchKernelGGL((cache_evict_shift_kernel<true>), all, dim3(1024), 0, s, a, shift, (int)n_rows);
+    else if (within) hipLaunchKernelGGL((cache_evict_shift_kernel<false>), all, dim3(1024), 0, s, a, shift, (int)n_rows);
+    else if (bits8) hipLaunchKernelGGL((cache_evict_move_kernel<true>), all, dim3(256), 0, s, a, shift, (int)n_rows);
+    else hipLaunchKernelGGL((cache_evict_move_kernel<false>), all, dim3(256), 0, s, a, shift, (int)n_rows);
     return hipGetLastError() == hipSuccess ? TRN_OK : TRN_E_LAUNCH;
 }
