@@ -114,6 +114,13 @@ def test_other_blocks_and_token_major_caches(block, place):
     _run(CASES[1], "spread", True, 16, place, layout="token")
 
 
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("B, D", [(20, 128), (20, 64), (10, 128)])
+def test_many_heads_in_place(B, D, bits):
+    """Heads enough for columns of 128 bytes and of whole rows; several steps of each."""
+    _run((B, 7, 1, D, 1300, 1100, 9, [1300 - 137 * (b % 10) for b in range(B)]), "spread", False, bits, "within")
+
+
 @pytest.mark.parametrize("kind", ["spread", "ties"])
 @pytest.mark.parametrize("S", [4096, 4097, 8193, 16385, 32768, 32769, 40000])
 def test_long_rows(S, kind):

@@ -4,14 +4,13 @@
 // Two launches, or three.  Selection: a workgroup has one head of a sequence.  The weights of its query heads are added up in 64 bits and rounded
 // once to fp32, turned into integers that order as they do, and the smallest one kept is found by digits of 11, 11 and 10 bits, counted in
 // LDS; ties are filled up from the front.  Up to 32768 keys stay in registers, and one scan over the counts of each 64 numbers what is
-// kept.  Move: rows of K and V, 16 bytes a lane, past the caches (each byte once).  Into another cache, workgroups
-// share the rows; within the same one, a workgroup has a 64-byte column of all of a head's rows and moves them front to back: a row
-// goes to its own place or one before it, so what a step overwrites has been read by this step or an earlier one, and columns
-// never meet.
+// kept.  Move: rows of K and V, 16 bytes a lane.  Into another cache, workgroups share the rows; within the same one, a workgroup has a column of
+// all of a head's rows and moves them front to back: a row goes to its own place or one before it, so what a step overwrites has been read by
+// this step or an earlier one, and columns never meet.
 //
 // Selection, 4 sequences of 4096 keys, 8 heads of 4 rows of weights: 7.4 us, of them launch and lengths 2.3, weights 1.8, the first digit 1.2, the others 0.3 and
 // 0.7, places 1.0: latency of one workgroup, whose barriers are what is left.  Move, 1024 of each kept, 35 MB: 8.4 us; 8-bit, 16 sequences of 8193
-// to 4096, 279 MB: 47.5 us, 5.9 TB/s.
+// to 4096, 279 MB: 47.5 us, 5.9 TB/s; fp16 in place, 16 of 8192 to 4096, 537 MB: 92 us, 5.8 TB/s.
 //
 // 8-bit caches: a block of the shortened cache takes the largest of the scales that its rows come with; codes of rows with a smaller
 // one are multiplied by the ratio, which between powers of two only rounds what leaves e4m3's normal numbers.
@@ -272,9 +271,9 @@ __device__ __forceinline__ void move_weights(const EvictArgs& a, int row) {
     }
 }
 
-// 8 bits: by what the codes of the rows of this step, one a thread, are multiplied, and the scales of their blocks (whole ones) -- the largest of
-// those that the rows come with.  Holds two barriers.
-__device__ __forceinline__ void block_scales(const EvictArgs& a, float s, float* top, float* ratio, bool writes, float* scales_out, int row) {
+// 8 bits: by what the codes of a step's rows, one a thread, are multiplied, and the scales of their blocks (whole ones) -- the largest of those that the rows
+// come with.  s: the scale a row comes with, zero where there is none.  Holds two barriers.
+__device__ __forceinline__ void block_scales(const EvictArgs& a, float s, float* top, float* ratio, float* scales_out, int row, int end) {
     const int tid = threadIdx.x;
     float t = s;
 #pragma unroll
@@ -284,7 +283,7 @@ __device__ __forceinline__ void block_scales(const EvictArgs& a, float s, float*
     const int groups = 1 << (a.bshift - 5), g0 = (tid >> 5) & ~(groups - 1);
     for (int i = 0; i < groups; ++i) t = fmaxf(t, top[g0 + i]);
     ratio[tid] = t > 0.f ? s / t : 1.f;
-    if (writes && (tid & ((1 << a.bshift) - 1)) == 0) scales_out[row >> a.bshift] = t;
+    if (scales_out && row < end && (tid & ((1 << a.bshift) - 1)) == 0) scales_out[row >> a.bshift] = t;
     __syncthreads();
 }
 __device__ __forceinline__ uint4_t recoded(uint4_t x, float f) {
@@ -314,8 +313,7 @@ __global__ __launch_bounds__(256) void cache_evict_move_kernel(const EvictArgs a
     __shared__ float ratio[256], top[8];
     if constexpr (BITS8) {
         const float* was = a.scales + ((int64_t)kv * a.B * a.Hkv + bh) * a.n_blocks;
-        const bool mine = tid < NB * step && from + tid < to;
-        block_scales(a, mine ? was[kept[from + tid] >> a.bshift] : 0.f, top, ratio, mine, (kv ? a.vs_out : a.ks_out) + b * a.sot[kv][0] + h * a.sot[kv][1], from + tid);
+        block_scales(a, from + tid < to ? was[kept[from + tid] >> a.bshift] : 0.f, top, ratio, (kv ? a.vs_out : a.ks_out) + b * a.sot[kv][0] + h * a.sot[kv][1], from + tid, to);
     }
 #pragma unroll
     for (int e = 0; e < NB; ++e) {
@@ -327,55 +325,63 @@ __global__ __launch_bounds__(256) void cache_evict_move_kernel(const EvictArgs a
     }
 }
 
-// Within the same cache.  Workgroups from n_rows on: (column, head of a sequence, K or V); the columns of a head as far apart as there are heads, on one XCD
-// where those are a multiple of four.  A step's rows are requested before the last one's are stored: they lie behind all that those overwrite.
-template <bool BITS8>
-__global__ __launch_bounds__(1024) void cache_evict_shift_kernel(const EvictArgs a, int piece_shift, int n_rows) {
+// Within the same cache.  Workgroups from n_rows on: (column of 16 << SHIFT bytes, head of a sequence, K or V); the columns of a head as far apart as there are
+// heads, on one XCD where those are a multiple of four.  A step's rows are requested before the last one's are stored: they lie behind all that
+// those overwrite.  Columns of less than a line of 128 bytes go through the caches, where they meet: past them, 4 sequences of 8192 rows of 8 heads of 128
+// to 4096 took 34 us, not 19; one of 65536 to 32768 145, not 114 (a compute unit's rate, of 64: with columns of 16 bytes 91, but 16384 rows
+// of 16 heads of 64 to 4096 14 instead of 12).
+template <bool BITS8, int SHIFT>
+__global__ __launch_bounds__(1024) void cache_evict_shift_kernel(const EvictArgs a, int n_rows) {
     const int tid = threadIdx.x;
     if ((int)blockIdx.x < n_rows) { move_weights<1024>(a, blockIdx.x); return; }
-    constexpr int NB = 4;
+    constexpr int NB = 4, ROWS = 1024 >> SHIFT, STEP = NB * ROWS;
+    constexpr bool WHOLE = SHIFT >= 3;
     const int col = a.by_heads2.of(blockIdx.x - n_rows), u = blockIdx.x - n_rows - col * a.by_heads2.d, kv = u & 1, bh = u >> 1;
     const int b = a.by_hkv.of(bh), h = bh - b * a.Hkv;
-    const int stay = a.now[b], rows = 1024 >> piece_shift, step = NB * rows;
+    const int stay = a.now[b];
     if (stay == 0) return;
     const int32_t* kept = a.kept + (int64_t)bh * a.keep;
     const char* src = (const char*)(kv ? a.v : a.k) + b * a.st[kv][0] + h * a.st[kv][1];
     char* dst = (char*)(kv ? a.v_out : a.k_out) + b * a.ot[kv][0] + h * a.ot[kv][1];
-    const int r0 = tid >> piece_shift, off = ((col << piece_shift) + (tid & ((1 << piece_shift) - 1))) * 16;
+    const int r0 = tid >> SHIFT, off = ((col << SHIFT) + (tid & ((1 << SHIFT) - 1))) * 16;
     const float* was = BITS8 ? a.scales + ((int64_t)kv * a.B * a.Hkv + bh) * a.n_blocks : nullptr;
-    float* const scales_out = BITS8 ? (kv ? a.vs_out : a.ks_out) + b * a.sot[kv][0] + h * a.sot[kv][1] : nullptr;
-    __shared__ float ratio[1024], top[32];
+    float* const scales_out = BITS8 && col == 0 ? (kv ? a.vs_out : a.ks_out) + b * a.sot[kv][0] + h * a.sot[kv][1] : nullptr;
+    __shared__ float ratio[BITS8 ? 1024 : 1], top[BITS8 ? 32 : 1];
     // (past the last row that one again: a row that is there, and goes nowhere)
     auto places = [&](int i0, int (&j)[NB], int& own) __attribute__((always_inline)) {
 #pragma unroll
-        for (int e = 0; e < NB; ++e) j[e] = kept[min(i0 + e * rows + r0, stay - 1)];
+        for (int e = 0; e < NB; ++e) j[e] = kept[min(i0 + e * ROWS + r0, stay - 1)];
         if constexpr (BITS8) own = kept[min(i0 + tid, stay - 1)];
     };
     auto request = [&](const int (&j)[NB], int own, uint4_t (&x)[NB], float& s) __attribute__((always_inline)) {
 #pragma unroll
-        for (int e = 0; e < NB; ++e) x[e] = __builtin_nontemporal_load(reinterpret_cast<const uint4_t*>(src + (int64_t)j[e] * a.st[kv][2] + off));
+        for (int e = 0; e < NB; ++e) {
+            const uint4_t* const from = reinterpret_cast<const uint4_t*>(src + (int64_t)j[e] * a.st[kv][2] + off);
+            x[e] = WHOLE ? __builtin_nontemporal_load(from) : *from;
+        }
         if constexpr (BITS8) s = was[own >> a.bshift];
     };
     uint4_t x[NB], x_next[NB]; int j[NB], own = 0; float s = 0.f, s_next = 0.f;
     places(0, j, own);
     request(j, own, x, s);
-    places(step, j, own);
-    for (int i0 = 0; i0 < stay; i0 += step) {
+    places(STEP, j, own);
+    for (int i0 = 0; i0 < stay; i0 += STEP) {
         request(j, own, x_next, s_next);
-        places(i0 + 2 * step, j, own);
+        places(i0 + 2 * STEP, j, own);
         // (what this step overwrites has been read by all waves: a barrier alone does not wait for loads whose values are used behind it)
 #pragma unroll
         for (int e = 0; e < NB; ++e) asm volatile("" : "+v"(x[e]));
-        if constexpr (BITS8) {
-            const bool mine = tid < step && i0 + tid < stay;
-            block_scales(a, mine ? s : 0.f, top, ratio, mine && col == 0, scales_out, i0 + tid);
-        } else __syncthreads();
+        const int end = min(stay, i0 + STEP);
+        if constexpr (BITS8) block_scales(a, i0 + tid < end ? s : 0.f, top, ratio, scales_out, i0 + tid, end);
+        else __syncthreads();
 #pragma unroll
         for (int e = 0; e < NB; ++e) {
-            const int i = i0 + e * rows + r0;
+            const int i = i0 + e * ROWS + r0;
             if (i < stay) {
-                if constexpr (BITS8) x[e] = recoded(x[e], ratio[e * rows + r0]);
-                __builtin_nontemporal_store(x[e], reinterpret_cast<uint4_t*>(dst + (int64_t)i * a.ot[kv][2] + off));
+                if constexpr (BITS8) x[e] = recoded(x[e], ratio[e * ROWS + r0]);
+                uint4_t* const to = reinterpret_cast<uint4_t*>(dst + (int64_t)i * a.ot[kv][2] + off);
+                if constexpr (WHOLE) __builtin_nontemporal_store(x[e], to);
+                else *to = x[e];
             }
             x[e] = x_next[e];
         }
@@ -493,8 +499,12 @@ extern "C" int trn_cache_evict(const trn_cache_evict_desc* e, const void* k, con
     else if (e->keys <= kMostKept) hipLaunchKernelGGL(cache_evict_select_kernel<32>, sel, dim3(1024), 0, s, a);
     else hipLaunchKernelGGL(cache_evict_select_kernel<0>, sel, dim3(1024), 0, s, a);
     const dim3 all((unsigned)grid);
-    if (within && bits8) hipLaunchKernelGGL((cache_evict_shift_kernel<true>), all, dim3(1024), 0, s, a, shift, (int)n_rows);
-    else if (within) hipLaunchKernelGGL((cache_evict_shift_kernel<false>), all, dim3(1024), 0, s, a, shift, (int)n_rows);
+#define TRN_SHIFT(S) do { if (bits8) hipLaunchKernelGGL((cache_evict_shift_kernel<true, S>), all, dim3(1024), 0, s, a, (int)n_rows); \
+                          else hipLaunchKernelGGL((cache_evict_shift_kernel<false, S>), all, dim3(1024), 0, s, a, (int)n_rows); } while (0)
+    if (within && shift == 2) TRN_SHIFT(2);
+    else if (within && shift == 3) TRN_SHIFT(3);
+    else if (within) hipLaunchKernelGGL((cache_evict_shift_kernel<false, 4>), all, dim3(1024), 0, s, a, (int)n_rows);      // (8-bit rows are 128 bytes at most)
+#undef TRN_SHIFT
     else if (bits8) hipLaunchKernelGGL((cache_evict_move_kernel<true>), all, dim3(256), 0, s, a, shift, (int)n_rows);
     else hipLaunchKernelGGL((cache_evict_move_kernel<false>), all, dim3(256), 0, s, a, shift, (int)n_rows);
     return hipGetLastError() == hipSuccess ? TRN_OK : TRN_E_LAUNCH;
