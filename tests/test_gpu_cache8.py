@@ -188,7 +188,7 @@ def test_attention_and_weights(case, layout):
 
 
 @pytest.mark.parametrize("D", [64, 128])
-@pytest.mark.parametrize("heads, causal", [((7, 8, 40), True), ((20, 16, 16), True), ((20, 16, 16), False)], ids=["two waves", "one wave", "one wave, all keys"])
+@pytest.mark.parametrize("heads, causal", [((8, 8, 40), True), ((20, 16, 16), True), ((33, 16, 16), True), ((33, 16, 16), False)], ids=["two waves", "two, fewer rows", "one wave", "one wave, all keys"])
 def test_row_tiles_of_fewer_waves(heads, causal, D):
     """So many rows that two waves share a row tile's keys, or that one has them: most of the batch is padding, for the oracle's sake."""
     B, Hkv, Hq = heads

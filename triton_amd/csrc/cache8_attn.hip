@@ -406,15 +406,15 @@ struct Plan8 { int G, R, nq, ks, n_rt, ns, n_chunks, chunk_tiles, sp; int64_t ml
 // 23.7 / 19.5 / 20.8; batch 16, 4097 31.3 / 28.6 / 28.4; batch 24, 4000 33.9 / 41.6 / 39.9; batch 32, 8192 88.7 / 91.4 / 93.8; of two to one lengths 70.5 / 72.2 / 70.8.  A
 // second launch is some 3 us: short caches have one share, but where few rows' weights need that launch anyway (512 keys 6.4, against 8.5; batch 8: 1025 keys 10.1 / 11.0; 16
 // heads of 64: 1025 keys 7.6 / 8.1, 2000 10.7 / 8.3; batch 16, 32 heads of 128, 2000 17.5 / 18.6).
-// Several row tiles are bound by their vector work rather than by memory: they rather fill two workgroups a compute unit (2.5 of head_dim 64 and 16 rows) with shares of
+// Several row tiles are bound by their vector work rather than by memory: they rather fill two workgroups a compute unit (2.25 of head_dim 64 and 16 rows) with shares of
 // 48 tiles of keys and more, if that is more than one and a half.  16 heads of 64, batch 4, 8000 keys, 20 queries 26.3 with two shares, 23.3 with four; 71 on
 // one, batch 28, 11316 keys, one query, with 1 / 2 / 4 / 8 40.8 / 32.0 / 26.4 / 28.5; 32 on 8 of 128, 100 queries, 16000 keys (104 row tiles of 32), with 1 / 2 / 3 / 4 / 6
 // 88.9 / 53.5 / 55.2 / 46.3 / 50.7; 4 x 40 queries, 8000 keys (160) 48.6 / 46.7 / 41.1 / 46.0; 8 on 2, 4 x 64 queries, 4000 keys (128 of 16) 19.6 / 17.1 / 18.8 / 17.1.
-// Waves that share a row tile's keys: four where no more row tiles are there than two workgroups a compute unit hold; with more the
+// Waves that share a row tile's keys: four where there are about as many row tiles of 32 as two workgroups a compute unit hold; with more the
 // frame of a workgroup (queries, first keys, joining: a fifth to a half of a short prompt's time) is spent less often by two waves, or one that has all
-// keys.  us with four / two / one, 32 heads of 128 on 8, row tiles of 32: one prompt of 512 (512 row tiles) 11.2 / 12.5 / 17.5, of 1501 (1504) 37.7 / 34.8 /
-// 40.6; 512 queries on 8448 keys (512) 82.8 / 94.1 / 177; two of 300 (608) 14.0 / 11.5 / 13.2; four of 512 (2048) 34.8 / 24.6 / 24.0, of 2047 (8192) 213 / 180 /
-// 161; 71 heads of 64 on one, 700 (1554) 17.8 / 15.3 / 16.4, four of them 57.7 / 42.8 / 36.1.
+// keys.  us with four / two / one, 32 heads of 128 on 8: 512 queries on 8448 keys (512 row tiles) 82.8 / 94.1 / 177; one prompt of 602 behind 64 keys (602) 17.6 / 16.1 /
+// 20.4, behind 2500 47.4 / 52.9 / 69.7; 799 behind 64 (799) 20.8 / 18.6 / 24.8, behind 2500 59.4 / 56.6 / 73.7; 1600 behind 700 (1600) 62.0 / 55.3 / 62.7, 2400 (2400) 103 / 93.8 / 99.3; two of 1500
+// (3008) 72.1 / 57.5 / 55.1; four of 512 (2048) 34.8 / 24.6 / 24.0, of 2047 (8192) 213 / 180 / 161; 71 heads of 64 on one, four of 700 (6216) 57.7 / 42.8 / 36.1.
 // A cache that is read by one row tile goes past the caches (each byte once), us through / past: batch 32, 8192 keys 99.5 / 89.4, one sequence of 131072 56.7 /
 // 51.2, of 4000 11.2 / 10.6; with two row tiles and more the others find it there: 64 rows, 16000 keys 18.7 / 20.6.
 static Plan8 plan8(const trn_cache8* c, int Hq, int Sq, bool weights) {
@@ -429,7 +429,7 @@ static Plan8 plan8(const trn_cache8* c, int Hq, int Sq, bool weights) {
     const int64_t units = heads * p.n_rt;
     int64_t ns = units ? 256 / units : 1;
     if (p.n_rt > 1) {
-        const int64_t most = (d128 || p.nq == 2 ? 512 : 640) / units, worth = (tiles + 47) / 48, more = most < worth ? most : worth;
+        const int64_t most = (d128 || p.nq == 2 ? 512 : 576) / units, worth = (tiles + 47) / 48, more = most < worth ? most : worth;
         if (units * more > 384) ns = more;
     }
     // (key weights: a score of 4 bytes goes out and comes back for each row and key, or K is read again)
@@ -438,7 +438,7 @@ static Plan8 plan8(const trn_cache8* c, int Hq, int Sq, bool weights) {
     if (ns > tiles) ns = tiles;
     p.ns = (int)(ns < 1 ? 1 : ns > 64 ? 64 : ns);
     const int64_t row_tiles = heads * p.n_rt;
-    p.ks = p.nq == 1 || row_tiles <= 512 ? 4 : row_tiles < 1600 ? 2 : 1;      // (there is one share from 256 row tiles on)
+    p.ks = p.nq == 1 || row_tiles <= 700 ? 4 : row_tiles < 2560 ? 2 : 1;      // (there is one share from 256 row tiles on)
     auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
     p.ml = p.ns > 1 ? up(units * p.ns * 16 * p.nq * c->head_dim * 4) : 0;
     p.lse2 = p.ml + (p.ns > 1 ? up(units * p.ns * 32 * p.nq * 4) : 0);

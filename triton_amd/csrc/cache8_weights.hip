@@ -288,23 +288,26 @@ __global__ __launch_bounds__(256, 2) void cache8_weights_kernel(const Attn8Args 
 #endif
 }
 
-// The chunks' sums, in their order.
+// The chunks' sums: 64 keys a workgroup, every fourth chunk a wave, in their order.  (One thread a key: 813 keys of one head in 192 chunks 10 us.)
 __global__ __launch_bounds__(256) void cache8_weights_join_kernel(const Attn8Args a) {
-    const int n_kb = (a.cap + 255) >> 8, bh = blockIdx.x / n_kb, key = (blockIdx.x - bh * n_kb) * 256 + threadIdx.x;
+    __shared__ float part[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int n_kb = (a.cap + 63) >> 6, bh = blockIdx.x / n_kb, key = (blockIdx.x - bh * n_kb) * 64 + lane;
     const int b = a.by_hkv.of(bh);
-    if (key >= keys_of(a.lengths, b, a.cap)) return;
-    const int64_t at = (int64_t)bh * a.cap + key, step = (int64_t)a.B * a.Hkv * a.cap;
+    const int64_t at = (int64_t)bh * a.cap + min(key, a.cap - 1), step = (int64_t)a.B * a.Hkv * a.cap;
     float x = 0.f;
 #pragma unroll 8
-    for (int i = 0; i < a.n_chunks; ++i) x += a.w_part[i * step + at];
-    a.w_out[at] = (a.w_in ? a.w_in[at] : 0.f) + x;
+    for (int i = wave; i < a.n_chunks; i += 4) x += a.w_part[i * step + at];
+    part[wave][lane] = x;
+    __syncthreads();
+    if (wave == 0 && key < keys_of(a.lengths, b, a.cap)) a.w_out[at] = (a.w_in ? a.w_in[at] : 0.f) + ((part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]));
 }
 
 hipError_t launch_cache8_weights(const Attn8Args& a, int head_dim, hipStream_t s) {
     const unsigned blocks = (unsigned)(a.B * a.Hkv * ((a.cap + 255) / 256));
     if (head_dim == 128) hipLaunchKernelGGL((cache8_weights_kernel<128>), dim3(blocks, (unsigned)a.n_chunks), dim3(256), 0, s, a);
     else hipLaunchKernelGGL((cache8_weights_kernel<64>), dim3(blocks, (unsigned)a.n_chunks), dim3(256), 0, s, a);
-    if (a.n_chunks > 1) hipLaunchKernelGGL(cache8_weights_join_kernel, dim3(blocks), dim3(256), 0, s, a);
+    if (a.n_chunks > 1) hipLaunchKernelGGL(cache8_weights_join_kernel, dim3((unsigned)(a.B * a.Hkv * ((a.cap + 63) / 64))), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 
