@@ -45,6 +45,7 @@ def test_append_statuses(lib):
     assert _append(lib, k_stride_s=48) == "TRN_E_STRIDE" and _append(lib, v_stride_h=0) == "TRN_E_STRIDE" and _append(lib, ks_stride_b=0) == "TRN_E_STRIDE"
     assert _append(lib, k=P + 8) == "TRN_E_ALIGN" and _append(lib, k_stride_h=128 * 64 + 8) == "TRN_E_ALIGN" and _append(lib, strides=(128, 64, 68, 128, 64, 64)) == "TRN_E_ALIGN"
     assert _append(lib, v_scale=P + 2) == "TRN_E_ALIGN"
+    assert _append(lib, tokens=1 << 26, capacity=1 << 26, batch=16) == "TRN_E_SHAPE"
 
 
 def _attend(lib, q=P, o=P, Hq=4, Sq=1, scale=1.0, w_in=None, w_out=None, ws=None, nbytes=0, qs=(256, 64, 64), os=(256, 64, 64), **kw):
@@ -103,6 +104,7 @@ def test_evict_statuses(lib):
     for kw in (dict(code_bytes=4), dict(head_dim=80), dict(code_bytes=1, block=48), dict(keys=1 << 27)):
         assert _evict(lib, **kw) == "TRN_E_UNSUPPORTED"
     assert _evict(lib, nbytes=100) == "TRN_E_SCRATCH"
+    assert _evict(lib, batch=1 << 22) == "TRN_E_SHAPE" and _evict(lib, batch=1 << 20, n_weight_rows=8) == "TRN_E_SHAPE"      # more threads than 32 bits number
     assert _evict(lib, {"k": P + 8}) == "TRN_E_ALIGN" and _evict(lib, ws=P + 16) == "TRN_E_ALIGN" and _evict(lib, k_stride=(8192, 4096, 68)) == "TRN_E_ALIGN"
     assert _evict(lib, {"k_out": P}) == "TRN_E_STRIDE"                      # the same cache with other strides
     assert _evict(lib, {"k_out": P + 1024}) == "TRN_E_UNSUPPORTED"          # a part of it

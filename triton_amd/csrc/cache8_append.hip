@@ -133,7 +133,7 @@ extern "C" int trn_cache8_append_f16(const trn_cache8* c, const void* k, const v
     const int most = tokens < c->capacity ? tokens : c->capacity;
     a.n_blocks = (most + 2 * c->block - 2) / c->block;                  // (the first of them may be the last of its block)
     const int64_t units = (int64_t)c->batch * c->n_kv_heads;
-    if (units * a.n_blocks > 0x7fffffffLL) return TRN_E_SHAPE;
+    if (units * a.n_blocks > 0xffffff) return TRN_E_SHAPE;            // (threads in 32 bits)
     a.by_blocks = Div(a.n_blocks); a.by_heads = Div(c->n_kv_heads);
     a.xb[0] = k_stride_b; a.xh[0] = k_stride_h; a.xs[0] = k_stride_s;
     a.xb[1] = v_stride_b; a.xh[1] = v_stride_h; a.xs[1] = v_stride_s;

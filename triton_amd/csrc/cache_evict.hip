@@ -423,6 +423,8 @@ extern "C" int trn_cache_evict(const trn_cache_evict_desc* e, const void* k, con
     using namespace trn;
     if (!e) return TRN_E_NULL;
     if (e->batch < 0 || e->n_kv_heads <= 0 || e->n_weight_rows <= 0 || e->n_weight_rows % e->n_kv_heads || e->keys <= 0 || e->keep <= 0 || e->recent < 0 || e->recent > e->keep) return TRN_E_SHAPE;
+    // (a workgroup of 1024 threads a head, and as many threads in all as 32 bits number)
+    if ((int64_t)e->batch * e->n_kv_heads > 0x3fffff || (int64_t)e->batch * e->n_weight_rows > 0x3fffff) return TRN_E_SHAPE;
     if (e->code_bytes != 1 && e->code_bytes != 2) return TRN_E_UNSUPPORTED;
     if (e->head_dim != 64 && e->head_dim != 128) return TRN_E_UNSUPPORTED;
     const bool bits8 = e->code_bytes == 1;
@@ -476,7 +478,6 @@ extern "C" int trn_cache_evict(const trn_cache_evict_desc* e, const void* k, con
     a.n_blocks = bits8 ? (e->keys + e->block - 1) / e->block : 0;
     a.now = (int32_t*)((char*)workspace + sz.now);
     const int64_t heads = (int64_t)e->batch * e->n_kv_heads;
-    if (heads > 0x3fffffff || (int64_t)e->batch * e->n_weight_rows > 0x7fffffff) return TRN_E_SHAPE;
     a.by_hkv = Div(e->n_kv_heads);
     // Rows are shared out; or within the same cache, columns: as wide as leaves a workgroup for each compute unit, 64 bytes at least.
     const bool within = a.in_place[0] || a.in_place[1];
@@ -488,7 +489,7 @@ extern "C" int trn_cache_evict(const trn_cache_evict_desc* e, const void* k, con
     const int64_t n_rows = weights_out || new_lengths ? (int64_t)e->batch * e->n_weight_rows : 0, grid = n_rows + 2 * heads * (within ? pieces >> shift : a.chunks);
     a.summed = orders_stored(e);
     const int64_t sums = heads * ((e->keys + 255) / 256);
-    if (grid > 0x7fffffffLL || sums > 0x7fffffffLL) return TRN_E_SHAPE;
+    if (grid > (within ? 0x3fffff : 0xffffff) || (a.summed && sums > 0xffffff)) return TRN_E_SHAPE;
     a.by_chunks = Div(a.chunks); a.by_heads2 = Div(2 * heads);
     const hipStream_t s = (hipStream_t)stream;
     if (a.summed) hipLaunchKernelGGL(cache_evict_sums_kernel, dim3((unsigned)sums), dim3(256), 0, s, a);
@@ -498,6 +499,7 @@ extern "C" int trn_cache_evict(const trn_cache_evict_desc* e, const void* k, con
     else if (e->keys <= 16384) hipLaunchKernelGGL(cache_evict_select_kernel<16>, sel, dim3(1024), 0, s, a);
     else if (e->keys <= kMostKept) hipLaunchKernelGGL(cache_evict_select_kernel<32>, sel, dim3(1024), 0, s, a);
     else hipLaunchKernelGGL(cache_evict_select_kernel<0>, sel, dim3(1024), 0, s, a);
+    if (hipGetLastError() != hipSuccess) return TRN_E_LAUNCH;       // (the move would go by places that nothing has set)
     const dim3 all((unsigned)grid);
 #define TRN_SHIFT(S) do { if (bits8) hipLaunchKernelGGL((cache_evict_shift_kernel<true, S>), all, dim3(1024), 0, s, a, (int)n_rows); \
                           else hipLaunchKernelGGL((cache_evict_shift_kernel<false, S>), all, dim3(1024), 0, s, a, (int)n_rows); } while (0)
