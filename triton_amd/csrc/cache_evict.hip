@@ -291,6 +291,7 @@ __device__ __forceinline__ uint4_t recoded(uint4_t x, float f) {
 }
 
 // Into another cache.  Workgroups from n_rows on: (head of a sequence, K or V, chunk of rows).  The first: a row of weights each.
+// Past the caches, each byte once: 8-bit, 16 sequences of 8193 to 4096 47.6 us, through them 55.8; 4 of 4096 to 1024 in fp16 8.8 / 8.3.
 template <bool BITS8>
 __global__ __launch_bounds__(256) void cache_evict_move_kernel(const EvictArgs a, int piece_shift, int n_rows) {
     const int tid = threadIdx.x;
