@@ -203,6 +203,16 @@ def test_row_tiles_of_fewer_waves(heads, causal, D):
     _hold(_attend(case, edit=edit, spoil=False), lengths)
 
 
+@pytest.mark.parametrize("B, Hq, Hkv, D, M", [(96, 32, 8, 128, 8), (320, 32, 8, 128, 8), (48, 16, 16, 64, 20)], ids=["768 heads", "2560", "768 of 64"])
+def test_one_row_tile_of_very_many_heads(B, Hq, Hkv, D, M):
+    """Heads enough for row tiles of fewer waves, each of which has a single tile of 17 to 32 rows: its four waves have its keys, and none behind them."""
+    S, block = 75, 32
+    lengths = [1 + 37 * b % S for b in range(B)]
+    lengths[1], lengths[-1] = 0, S
+    counts = [M if b in (0, 5, B - 1) else int(b % 4 < 2) for b in range(B)]
+    _hold(_attend((B, Hq, Hkv, D, M, S, block, lengths, counts, True), "padded"), lengths)
+
+
 @pytest.mark.parametrize("spread", [0.0, 4.0])
 @pytest.mark.parametrize("case", [ATTNS[3], ATTNS[8], ATTNS[6]], ids=["tiles", "split", "prompt"])
 def test_scales_that_differ_by_powers_and_by_nothing(case, spread):
