@@ -65,6 +65,17 @@ def test_attention_statuses(lib):
     assert _attend(lib, Sq=1 << 26) == "TRN_E_UNSUPPORTED" and _attend(lib, w_in=P, w_out=P + 64, ws=P, nbytes=1 << 30) == "TRN_E_UNSUPPORTED"
 
 
+def test_weights_of_no_queries_and_of_no_keys(lib):
+    """They are launches like others (which fail here): nothing else would bring the old weights, or zeros, into weights_out.  A cache without keys has no weights
+    and needs no workspace for them."""
+    W = P + (1 << 20)
+    assert _attend(lib, Sq=0, w_out=W) == "TRN_E_LAUNCH" and _attend(lib, Sq=0, w_in=P, w_out=W) == "TRN_E_LAUNCH"
+    assert _attend(lib, Sq=0, w_in=W, w_out=W) == "TRN_OK" and _attend(lib, Sq=0, w_out=W, capacity=0) == "TRN_OK"
+    assert _attend(lib, Sq=0, w_in=P) == "TRN_E_NULL" and _attend(lib, Sq=0, w_in=P, w_out=P + 64) == "TRN_E_UNSUPPORTED"
+    assert _attend(lib, w_out=W, capacity=0) == "TRN_E_LAUNCH"
+    assert lib.trn_cache8_attn_workspace_bytes(C.byref(_cache(capacity=0)), 4, 1, 1) == 0
+
+
 def test_attention_workspace_is_bounded(lib):
     """By what the shares, the rows' sums and either the scores of few rows or the chunks' sums of many take, whatever the sizes."""
     for B in (1, 3, 32):

@@ -382,6 +382,45 @@ def test_caches_and_batches_of_nothing():
     ops.cache8_attention(q[:0], k8, k8, s, s, o[:0])
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_weights_of_no_queries(D):
+    """weights_out is weights, or zeros, up to each sequence's length; a cache without keys has none and takes no workspace."""
+    B, Hq, Hkv, S, block, lengths = 3, 4, 2, 700, 64, [700, 0, 301]
+    k8, ks, dk8, dks, v8, vs, dv8, dvs = _cache(B, Hkv, S, D, block, 71, lengths)
+    q = torch.zeros(B, Hq, 0, D, dtype=torch.float16, device=DEV)
+    w = torch.rand(B, Hkv, S, generator=torch.Generator().manual_seed(72))
+    mod = modules.get("weights8", "cache", block=block)
+    for w_in in (None, w):
+        for via in ("ops", "module", "counts"):
+            out = torch.full((B, Hkv, S), 7.0, device=DEV)
+            given = None if w_in is None else w_in.to(DEV)
+            if via == "ops":
+                ops.cache8_attention(q, dk8, dv8, dks, dvs, q.clone(), lengths=_ints(lengths), lse=torch.zeros(B, Hq, 0, device=DEV), weights=given, weights_out=out, block=block)
+            elif via == "module":
+                mod.forward(dk8, dks, q.clone(), q, dv8, dvs, None, _ints(lengths), given, out)
+            else:
+                some = torch.zeros(B, Hq, 3, D, dtype=torch.float16, device=DEV)
+                mod.forward(dk8, dks, some.clone(), some, dv8, dvs, _ints([0] * B), _ints(lengths), given, out)
+            for b, n in enumerate(lengths):
+                assert torch.equal(_cpu(out)[b, :, :n], torch.zeros(Hkv, n) if w_in is None else w[b, :, :n]) and (out[b, :, n:] == 7.0).all()
+    same = w.to(DEV)
+    mod.forward(dk8, dks, q.clone(), q, dv8, dvs, None, _ints(lengths), same, same)
+    assert torch.equal(_cpu(same), w)
+    none = lambda *s, dt=torch.uint8: torch.zeros(*s, dtype=dt, device=DEV)
+    some, o = torch.ones(B, Hq, 2, D, dtype=torch.float16, device=DEV), torch.full((B, Hq, 2, D), 7.0, dtype=torch.float16, device=DEV)
+    k8, s, w0 = none(B, Hkv, 0, D), none(B, Hkv, 0, dt=torch.float32), none(B, Hkv, 0, dt=torch.float32)
+    mod.forward(k8, s, o, some, k8, s, None, None, w0, w0)
+    assert (o == 0).all()
+    # (the C ABI may be given an address for weights of nothing)
+    c = _lib.Cache8()
+    c.batch, c.n_kv_heads, c.capacity, c.head_dim, c.block = B, Hkv, 0, D, block
+    o.fill_(7.0)
+    strides = (Hq * 2 * D, 2 * D, D)
+    st = _lib.load().trn_cache8_attn_f16(_lib.C.byref(c), some.data_ptr(), o.data_ptr(), Hq, 2, *strides, *strides, 0.125, 1, None, None, same.data_ptr(), None, 0,
+                                         torch.cuda.current_stream().cuda_stream)
+    assert st == 0 and (o == 0).all() and torch.equal(_cpu(same), w)
+
+
 @pytest.mark.parametrize("variant", ["vanilla", "prenorm", "weights"])
 def test_the_step_of_projection_append_and_attention(variant):
     """modules.get(.., "cache8"): three steps of a ragged, padded batch, with what its projections leave held to the definitions."""

@@ -403,6 +403,15 @@ static int attn8_check(const trn_cache8* c, int32_t n_q_heads, int32_t seq_q) {
     return TRN_OK;
 }
 
+// No queries: the keys' weights are what they were, and to be in weights_out all the same.
+static int weights_of_nothing(const trn_cache8* c, const float* weights_in, float* weights_out, hipStream_t s) {
+    if ((int64_t)c->batch * c->n_kv_heads * ((c->capacity + 255) / 256) > 0xffffff) return TRN_E_SHAPE;       // (threads in 32 bits)
+    Attn8Args a{};
+    a.lengths = c->lengths; a.B = c->batch; a.Hkv = c->n_kv_heads; a.cap = c->capacity; a.by_hkv = Div(c->n_kv_heads);
+    a.w_in = weights_in; a.w_out = weights_out; a.n_chunks = 1;
+    return launch_cache8_weights(a, c->head_dim, s) == hipSuccess ? TRN_OK : TRN_E_LAUNCH;
+}
+
 }  // namespace trn
 
 extern "C" int64_t trn_cache8_attn_workspace_bytes(const trn_cache8* c, int32_t n_q_heads, int32_t seq_q, int32_t weights) {
@@ -419,13 +428,16 @@ extern "C" int trn_cache8_attn_f16(const trn_cache8* c, const void* q, void* o, 
     using namespace trn;
     const int st = attn8_check(c, n_q_heads, seq_q);
     if (st != TRN_OK) return st;
-    if (c->batch == 0 || seq_q == 0) return TRN_OK;
-    if (!q || !o || (weights_in && !weights_out)) return TRN_E_NULL;
-    if (!(scale > 0.f)) return TRN_E_SHAPE;
+    if (c->batch == 0) return TRN_OK;
+    if (weights_in && !weights_out) return TRN_E_NULL;
     if (weights_in && weights_in != weights_out) {
         const int64_t size = (int64_t)c->batch * c->n_kv_heads * c->capacity * 4;
         if (!apart(weights_in, size, weights_out, size)) return TRN_E_UNSUPPORTED;
     }
+    if (c->capacity == 0) weights_in = weights_out = nullptr;       // (no key has a weight)
+    if (seq_q == 0) return weights_out && weights_in != weights_out ? weights_of_nothing(c, weights_in, weights_out, (hipStream_t)stream) : TRN_OK;
+    if (!q || !o) return TRN_E_NULL;
+    if (!(scale > 0.f)) return TRN_E_SHAPE;
     if ((c->batch > 1 && !o_stride_b) || (n_q_heads > 1 && !o_stride_h) || (seq_q > 1 && !o_stride_s)) return TRN_E_STRIDE;
     if (!aligned16(q) || (reinterpret_cast<uintptr_t>(o) & 7)) return TRN_E_ALIGN;
     for (int64_t s : {q_stride_b, q_stride_h, q_stride_s}) if (!pitch16(s, 2)) return TRN_E_ALIGN;
@@ -468,6 +480,6 @@ extern "C" int trn_cache8_attn_f16(const trn_cache8* c, const void* q, void* o, 
     });
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && (p.ns > 1 || p.sp)) e = launch_cache8_finish(a, c->head_dim, s);
-    if (e == hipSuccess && weights_out && !p.sp && c->capacity > 0) e = launch_cache8_weights(a, c->head_dim, s);
+    if (e == hipSuccess && weights_out && !p.sp) e = launch_cache8_weights(a, c->head_dim, s);
     return e == hipSuccess ? TRN_OK : TRN_E_LAUNCH;
 }

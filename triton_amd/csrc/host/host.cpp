@@ -513,6 +513,7 @@ void dims4(const View& t, const char* n, int64_t b, int64_t h, int64_t s, int64_
          (long long)b, (long long)h, (long long)s, (long long)d);
 }
 void unit4(const View& t, const char* n) { NEED(t.s[t.dim - 1] == 1 || t.unit(), "%s: innermost stride must be 1", n); }
+bool packed(const View& t) { return t.contiguous() || t.numel() == 0; }      // (of nothing, strides may be anything)
 const int32_t* batch_ints(const OptView& t, const char* n, int64_t b, const View& first) {
     if (!t.given) return nullptr;
     on(t.v, n, first);
@@ -584,7 +585,7 @@ bool f_cache8_attention(Args a, Py_ssize_t n) {
     const OptView lse = opt(a[12], "lse"), w = opt(a[13], "weights"), wo = opt(a[14], "weights_out");
     if (lse.given) {
         dev_float(lse.v, "lse"); on(lse.v, "lse", k8);
-        NEED(lse.v.dim == 3 && lse.v.s[0] == q.s[0] && lse.v.s[1] == q.s[1] && lse.v.s[2] == q.s[2] && lse.v.contiguous(), "lse: expected contiguous float32 (%lld, %lld, %lld)",
+        NEED(lse.v.dim == 3 && lse.v.s[0] == q.s[0] && lse.v.s[1] == q.s[1] && lse.v.s[2] == q.s[2] && packed(lse.v), "lse: expected contiguous float32 (%lld, %lld, %lld)",
              (long long)q.s[0], (long long)q.s[1], (long long)q.s[2]);
     }
     NEED(!w.given || wo.given, "weights given without weights_out");
@@ -592,7 +593,7 @@ bool f_cache8_attention(Args a, Py_ssize_t n) {
         if (!t->given) continue;
         const char* nm = t == &w ? "weights" : "weights_out";
         on(t->v, nm, k8);
-        NEED(t->v.f32() && t->v.dim == 3 && t->v.s[0] == k8.s[0] && t->v.s[1] == k8.s[1] && t->v.s[2] == k8.s[2] && t->v.contiguous(),
+        NEED(t->v.f32() && t->v.dim == 3 && t->v.s[0] == k8.s[0] && t->v.s[1] == k8.s[1] && t->v.s[2] == k8.s[2] && packed(t->v),
              "%s: expected contiguous float32 (%lld, %lld, %lld)", nm, (long long)k8.s[0], (long long)k8.s[1], (long long)k8.s[2]);
     }
     at::Tensor kept;
