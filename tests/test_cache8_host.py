@@ -76,6 +76,17 @@ def test_weights_of_no_queries_and_of_no_keys(lib):
     assert lib.trn_cache8_attn_workspace_bytes(C.byref(_cache(capacity=0)), 4, 1, 1) == 0
 
 
+def test_attention_of_more_threads_than_32_bits_number(lib):
+    """Refused before the first launch, whichever of the launches it is; one workgroup fewer is a launch (which fails here)."""
+    big = dict(ws=P, nbytes=1 << 60)
+    assert _attend(lib, batch=1 << 23) == "TRN_E_SHAPE" and _attend(lib, batch=(1 << 23) - 1) == "TRN_E_LAUNCH"                       # the attention's: heads
+    assert _attend(lib, batch=1 << 13, Hq=2, Sq=1 << 15) == "TRN_E_LAUNCH" and _attend(lib, batch=1 << 16, Hq=2, Sq=1 << 15) == "TRN_E_SHAPE"      # ... rows
+    many = dict(Hq=2, Sq=16, w_out=P + (1 << 20), **big)
+    assert _attend(lib, batch=1 << 15, capacity=(1 << 16) + 1, **many) == "TRN_E_SHAPE" and _attend(lib, batch=1 << 15, capacity=1 << 15, **many) == "TRN_E_LAUNCH"      # key weights of many rows
+    few = dict(w_out=P + (1 << 20), **big)
+    assert _attend(lib, batch=1 << 15, capacity=1 << 18, **few) == "TRN_E_SHAPE" and _attend(lib, batch=1 << 15, capacity=1 << 17, **few) == "TRN_E_LAUNCH"      # ... of few
+
+
 def test_attention_workspace_is_bounded(lib):
     """By what the shares, the rows' sums and either the scores of few rows or the chunks' sums of many take, whatever the sizes."""
     for B in (1, 3, 32):

@@ -456,7 +456,12 @@ extern "C" int trn_cache8_attn_f16(const trn_cache8* c, const void* q, void* o, 
     a.G = p.G; a.R = p.R; a.n_rt = p.n_rt; a.rshift = p.nq == 1 ? 4 : 5; a.ns = p.ns; a.causal = causal != 0;
     a.bshift = c->block == 32 ? 5 : c->block == 64 ? 6 : 7;
     const int64_t heads = (int64_t)c->batch * c->n_kv_heads, units = heads * p.ns;
-    if (units * p.n_rt > 0x7fffffffLL || heads * ((int64_t)p.R + 1) > 0x7fffffffLL || heads * ((c->capacity + 255) / 256) * p.n_chunks > 0x3fffffffLL) return TRN_E_SHAPE;
+    if (heads * ((int64_t)p.R + 1) > 0x7fffffffLL) return TRN_E_SHAPE;
+    // (workgroups of 256, and as many threads in all as 32 bits number: of every launch, before the first one)
+    const int per = 4 / p.ks;
+    const int64_t groups = units * ((p.n_rt + per - 1) / per), n_scores = p.sp ? heads * ((c->capacity + 1023) / 1024) : 0;
+    const int64_t n_sums = weights_out && !p.sp ? heads * ((c->capacity + (p.n_chunks > 1 ? 63 : 255)) / (p.n_chunks > 1 ? 64 : 256)) : 0;
+    if (groups > 0xffffff || (p.ns > 1 ? heads * p.R : 0) + n_scores > 0xffffff || n_sums > 0xffffff) return TRN_E_SHAPE;
     a.by_units = Div(units); a.by_g = Div(p.G); a.by_hkv = Div(c->n_kv_heads); a.by_ns = Div(p.ns);
     a.kb = c->k_stride_b; a.kh = c->k_stride_h; a.kst = c->k_stride_s;
     a.vb = c->v_stride_b; a.vh = c->v_stride_h; a.vst = c->v_stride_s;
@@ -471,10 +476,10 @@ extern "C" int trn_cache8_attn_f16(const trn_cache8* c, const void* q, void* o, 
     const hipStream_t s = (hipStream_t)stream;
     const bool d128 = c->head_dim == 128;
     with_kernel8(p, [&](auto nq, auto ks, auto past) {
-        constexpr int NQ = decltype(nq)::value, KS = decltype(ks)::value, per = 4 / KS;
+        constexpr int NQ = decltype(nq)::value, KS = decltype(ks)::value;
         constexpr bool PAST = decltype(past)::value;
         a.by_w = Div(KS * p.ns);
-        const dim3 grid((unsigned)(units * ((p.n_rt + per - 1) / per))), block(256);
+        const dim3 grid((unsigned)groups), block(256);
         if (d128) hipLaunchKernelGGL((cache8_attn_kernel<128, NQ, KS, PAST>), grid, block, 0, s, a);
         else hipLaunchKernelGGL((cache8_attn_kernel<64, NQ, KS, PAST>), grid, block, 0, s, a);
     });
