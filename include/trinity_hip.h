@@ -437,7 +437,8 @@ int trn_cache8_attn_f16(const trn_cache8* cache, const void* q, void* o, int32_t
  *   weights     float, or fp16 with weights_half, [batch, n_weight_rows, keys] contiguous; n_weight_rows a multiple of n_kv_heads: a KV head's are its
  *               rows' sum, added in 64 bits and rounded once to float (KeyFormer's C_out has a row for each query head).
  *   k, v        fp16 (code_bytes 2) or e4m3 codes (1) [batch, n_kv_heads, keys, head_dim]; k_out, v_out [.., keep (or more), head_dim].  An output may be its
- *               input, with the same strides; otherwise no output may overlap K or V.  Rows from the new length on are left as they are.
+ *               input, with the same strides; otherwise no output may overlap K or V, or the other one (keys and values packed into one tensor by
+ *               sequence, head or token do not).  Rows from the new length on are left as they are.
  *   *_scale     8 bits only: float [batch, n_kv_heads, ceil(keys / block)], the outputs over ceil(keep / block) blocks; an output may be its input.  A block
  *               of the result has the largest of the scales that its rows come with; codes of rows with a smaller one are multiplied by the
  *               ratio and rounded again.

@@ -135,6 +135,23 @@ def test_evict_statuses(lib):
     assert _evict(lib, k_stride=(-8192, 4096, 64)) == "TRN_E_STRIDE" and _evict(lib, k_out_stride=(2048, 0, 64)) == "TRN_E_STRIDE"
 
 
+def test_evict_of_caches_packed_into_one_tensor(lib):
+    """Keys and values of one tensor that share no element, in place and into such a tensor: by sequence, by head, and by token, are launches (which fail here); a row
+    of one that lies in the other is refused, wherever it is."""
+    B, H, S, D = 2, 2, 64, 64
+    row = 2 * D      # bytes
+    for strides, off in (((2 * H * S * D, S * D, D), H * S * row), ((2 * H * S * D, 2 * S * D, D), S * row), ((2 * H * S * D, D, 2 * H * D), H * row), ((2 * H * S * D, 2 * D, 2 * H * D), row)):
+        kw = dict(batch=B, k_stride=strides, v_stride=strides)
+        same = dict(k_out_stride=strides, v_out_stride=strides)
+        assert _evict(lib, dict(k=P, v=P + off, k_out=P, v_out=P + off), **kw, **same) == "TRN_E_LAUNCH", strides
+        Q = P + (1 << 21)
+        assert _evict(lib, dict(k=P, v=P + off, k_out=Q, v_out=Q + off), **kw, **same) == "TRN_E_LAUNCH"
+        assert _evict(lib, dict(k=P, v=P + off, k_out=Q, v_out=Q), **kw, **same) == "TRN_E_UNSUPPORTED"
+        assert _evict(lib, dict(k=P, v=P + off, k_out=P, v_out=P + off - 16), **kw, **same) == "TRN_E_UNSUPPORTED"
+        assert _evict(lib, dict(k=P, v=P + off, k_out=P + off, v_out=Q), **kw, **same) == "TRN_E_UNSUPPORTED"          # K's rows to where V's are
+        assert _evict(lib, dict(k=P, v=P + off, k_out=P + 32 * strides[2] * 2, v_out=Q), **kw, **same) == "TRN_E_UNSUPPORTED"
+
+
 def test_wrappers_refuse_cpu_tensors_and_bad_constants():
     t = torch.zeros(1, 2, 64, 64, dtype=torch.float16)
     c = torch.zeros(1, 2, 64, 64, dtype=torch.uint8)

@@ -129,6 +129,63 @@ def test_long_rows(S, kind):
     _run((1, 1, 9, 64, S, S // 2, 3, [S - 5]), kind, True, 16, "apart")
 
 
+def _sides(place, bits, make):
+    """An eviction whose caches, and results, `make` lays out on the device as (k, v, k_out, v_out), held to the definition; rows that are not written stay."""
+    B, H, D, S, keep, recent, block, lengths = 2, 3, 64, 300, 130, 20, 32, [300, 207]
+    g = torch.Generator().manual_seed(14)
+    w = torch.exp(2 * torch.randn(B, H, S, generator=g))
+    if bits == 8:
+        k, v = (ref.encode((torch.randn(B, H, S, D, generator=g) * 100).clamp(-448, 448)) for _ in range(2))
+        ks, vs = (torch.exp2(torch.randint(-4, 5, (B, H, -(-S // block)), generator=g).float()) for _ in range(2))
+    else:
+        k, v = (torch.randn(B, H, S, D, generator=g).half() for _ in range(2))
+        ks = vs = None
+    dk, dv, ko, vo = make(k.to(DEV), v.to(DEV))
+    scales = [None] * 4 if bits == 16 else [t.to(DEV) for t in (ks, vs, ks, vs)]
+    before = [t.cpu() for t in (ko, vo)]
+    kept, n = torch.zeros(B, H, keep, dtype=torch.int32, device=DEV), torch.tensor(lengths, dtype=torch.int32, device=DEV)
+    dw = w.to(DEV)
+    ws = torch.full((ops.cache_evict_workspace_bytes(dk, dw, keep),), 0xff, dtype=torch.uint8, device=DEV)
+    ops.cache_evict(dk, dv, dw, ko, vo, kept, keep, recent, ws, n, n, None, *scales, block)
+    want = ref.evict(k, v, w, keep, recent, lengths, ks, vs, block)
+    for b in range(B):
+        for h in range(H):
+            assert torch.equal(kept[b, h].cpu(), want["kept"][b][h].int())
+            for name, out, old in (("k", ko, before[0]), ("v", vo, before[1])):
+                o = out[b, h].cpu().contiguous()
+                assert torch.equal(o[:keep].view(torch.uint8), want[name][b][h].view(torch.uint8)), (name, b, h)
+                assert torch.equal(o[keep:].view(torch.uint8), old[b, h, keep:].contiguous().view(torch.uint8))
+            if bits == 8:
+                for name, out in (("ks", scales[2]), ("vs", scales[3])):
+                    assert torch.equal(out[b, h, :len(want[name][b][h])].cpu(), want[name][b][h])
+
+
+@pytest.mark.parametrize("axis", [1, 2, 3], ids=["by sequence", "by head", "by token"])
+@pytest.mark.parametrize("place", ["apart", "within"])
+@pytest.mark.parametrize("bits", [16, 8])
+def test_keys_and_values_of_one_tensor(bits, place, axis):
+    def make(k, v):
+        def pack(a, b):
+            a, b = (a.transpose(1, 2), b.transpose(1, 2)) if axis == 3 else (a, b)
+            both = torch.stack((a, b), 2 if axis == 3 else axis)
+            return [t.transpose(1, 2) if axis == 3 else t for t in both.unbind(2 if axis == 3 else axis)]
+        k, v = pack(k, v)
+        if place == "within":
+            return k, v, k, v
+        return k, v, *pack(torch.full((2, 3, 140, 64), 9, dtype=k.dtype, device=DEV), torch.full((2, 3, 140, 64), 8, dtype=k.dtype, device=DEV))
+    _sides(place, bits, make)
+
+
+@pytest.mark.parametrize("stays", ["k", "v"])
+@pytest.mark.parametrize("bits", [16, 8])
+def test_one_of_keys_and_values_in_place(bits, stays):
+    """The other goes into a cache of its own."""
+    def make(k, v):
+        out = torch.full((2, 3, 140, 64), 9, dtype=k.dtype, device=DEV)
+        return (k, v, k, out) if stays == "k" else (k, v, out, v)
+    _sides("mixed", bits, make)
+
+
 def test_keyformer_scores_cut_a_prompt():
     """KeyFormer's prompt module and eviction by its scores, one after the other, as a user has them."""
     B, Hq, Hkv, S, D, keep, recent = 2, 8, 2, 300, 128, 100, 20

@@ -2,6 +2,7 @@
 // head and block of 32, 64 or 128 tokens.
 #pragma once
 #include "common.h"
+#include "extent.h"
 
 namespace trn {
 
@@ -57,11 +58,6 @@ struct Attn8Args {
     float* w_part; int n_chunks, chunk_tiles;      // many rows: [n_chunks][B Hkv][cap] sums over a chunk's row tiles
 };
 
-// Whether two ranges of memory share nothing.
-inline bool apart(const void* x, int64_t nx, const void* y, int64_t ny) {
-    const uintptr_t p = (uintptr_t)x, q = (uintptr_t)y;
-    return p + (uint64_t)nx <= q || q + (uint64_t)ny <= p;
-}
 inline bool block_ok(int block) { return block == 32 || block == 64 || block == 128; }
 // The checks of a cache that every entry point makes; base pointers, and strides of axes with more than one element.
 int cache8_check(const trn_cache8* c);

@@ -407,9 +407,6 @@ static EvictSizes evict_sizes(const trn_cache_evict_desc* e) {
     return s;
 }
 
-// The bytes that a tensor [batch, heads, rows, width] spans from its base (strides in bytes, not negative).
-static int64_t span(const int64_t* st, int64_t b, int64_t h, int64_t rows, int64_t width) { return (b - 1) * st[0] + (h - 1) * st[1] + (rows - 1) * st[2] + width; }
-
 }  // namespace trn
 
 extern "C" int64_t trn_cache_evict_workspace_bytes(const trn_cache_evict_desc* e) {
@@ -448,6 +445,7 @@ extern "C" int trn_cache_evict(const trn_cache_evict_desc* e, const void* k, con
     const int64_t* in[2] = {e->k_stride, e->v_stride};
     const int64_t* out[2] = {e->k_out_stride, e->v_out_stride};
     const int rows_out = e->keep < e->keys ? e->keep : e->keys;
+    Extent in_at[2], out_at[2];
     for (int i = 0; i < 2; ++i) {
         for (int j = 0; j < 3; ++j) {
             a.st[i][j] = in[i][j] * e->code_bytes; a.ot[i][j] = out[i][j] * e->code_bytes;
@@ -456,18 +454,15 @@ extern "C" int trn_cache_evict(const trn_cache_evict_desc* e, const void* k, con
         }
         if ((in[i][2] < e->head_dim && e->keys > 1) || (out[i][2] < e->head_dim && rows_out > 1)) return TRN_E_STRIDE;
         if ((e->batch > 1 && !out[i][0]) || (e->n_kv_heads > 1 && !out[i][1])) return TRN_E_STRIDE;
-        const void* x = i ? v : k;
-        const void* y = i ? v_out : k_out;
-        const int64_t nx = span(a.st[i], e->batch, e->n_kv_heads, e->keys, width), ny = span(a.ot[i], e->batch, e->n_kv_heads, rows_out, width);
-        a.in_place[i] = x == y;
-        if (x == y) {       // the same cache, shortened
+        in_at[i] = Extent{i ? v : k, {e->batch, e->n_kv_heads, e->keys}, {a.st[i][0], a.st[i][1], a.st[i][2]}, width};
+        out_at[i] = Extent{i ? v_out : k_out, {e->batch, e->n_kv_heads, rows_out}, {a.ot[i][0], a.ot[i][1], a.ot[i][2]}, width};
+        a.in_place[i] = in_at[i].p == out_at[i].p;
+        if (a.in_place[i]) {       // the same cache, shortened
             for (int j = 0; j < 3; ++j)
                 if (a.st[i][j] != a.ot[i][j]) return TRN_E_STRIDE;
-        } else if (!apart(x, nx, y, ny)) return TRN_E_UNSUPPORTED;
-        const void* other = i ? k : v;
-        if (!apart(other, span(a.st[1 - i], e->batch, e->n_kv_heads, e->keys, width), y, ny)) return TRN_E_UNSUPPORTED;
+        } else if (meet(in_at[i], out_at[i])) return TRN_E_UNSUPPORTED;
     }
-    if (!apart(k_out, span(a.ot[0], e->batch, e->n_kv_heads, rows_out, width), v_out, span(a.ot[1], e->batch, e->n_kv_heads, rows_out, width))) return TRN_E_UNSUPPORTED;
+    if (meet(in_at[0], out_at[1]) || meet(in_at[1], out_at[0]) || meet(out_at[0], out_at[1])) return TRN_E_UNSUPPORTED;
     if (weights_out && weights_out != weights) {
         const int64_t rows = (int64_t)e->batch * e->n_weight_rows, size = e->weights_half ? 2 : 4;
         if (!apart(weights, rows * e->keys * size, weights_out, rows * e->keep * size)) return TRN_E_UNSUPPORTED;
