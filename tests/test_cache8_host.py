@@ -152,6 +152,27 @@ def test_evict_of_caches_packed_into_one_tensor(lib):
         assert _evict(lib, dict(k=P, v=P + off, k_out=P + 32 * strides[2] * 2, v_out=Q), **kw, **same) == "TRN_E_UNSUPPORTED"
 
 
+def test_evict_of_scales_that_share_memory(lib):
+    """Scale outputs of two heads, or of keys and values, in one place are refused; apart, over their inputs and packed into one tensor they are launches (which
+    fail here)."""
+    M = 1 << 20
+
+    def call(ks=P + 6 * M, vs=P + 7 * M, kso=P + 8 * M, vso=P + 9 * M, k=(4, 2), v=(4, 2), ko=(2, 1), vo=(2, 1)):
+        e = _lib.CacheEvictDesc(batch=2, n_kv_heads=2, n_weight_rows=4, keys=64, head_dim=64, code_bytes=1, block=32, keep=16, recent=4)
+        e.k_stride = e.v_stride = (8192, 4096, 64)
+        e.k_out_stride = e.v_out_stride = (2048, 1024, 64)
+        e.k_scale_stride, e.v_scale_stride, e.k_scale_out_stride, e.v_scale_out_stride = k, v, ko, vo
+        return _name(lib, lib.trn_cache_evict(C.byref(e), P, P + M, P + 2 * M, P + 3 * M, ks, vs, kso, vso, P + 4 * M, None, None, P + 5 * M, None, P, 1 << 40, None))
+    assert call() == "TRN_E_LAUNCH" and call(kso=P + 6 * M, vso=P + 7 * M, ko=(4, 2), vo=(4, 2)) == "TRN_E_LAUNCH"
+    for kw in (dict(ko=(0, 1)), dict(ko=(2, 0)), dict(vo=(0, 1)), dict(vo=(2, 0)), dict(k=(-4, 2)), dict(vo=(2, -1))):
+        assert call(**kw) == "TRN_E_STRIDE", kw
+    for kw in (dict(ks=P + 6 * M + 2), dict(vs=P + 1), dict(kso=P + 8 * M + 2), dict(vso=P + 9 * M + 3)):
+        assert call(**kw) == "TRN_E_ALIGN", kw
+    for kw in (dict(vso=P + 8 * M), dict(vso=P + 8 * M + 4), dict(vso=P + 8 * M + 4, ko=(4, 1), vo=(4, 1))):
+        assert call(**kw) == "TRN_E_UNSUPPORTED", kw
+    assert call(vso=P + 8 * M + 8, ko=(4, 1), vo=(4, 1)) == "TRN_E_LAUNCH" and call(vso=P + 8 * M + 4, ko=(4, 2), vo=(4, 2)) == "TRN_E_LAUNCH"      # by sequence, by head
+
+
 def test_wrappers_refuse_cpu_tensors_and_bad_constants():
     t = torch.zeros(1, 2, 64, 64, dtype=torch.float16)
     c = torch.zeros(1, 2, 64, 64, dtype=torch.uint8)

@@ -467,6 +467,15 @@ extern "C" int trn_cache_evict(const trn_cache_evict_desc* e, const void* k, con
         const int64_t rows = (int64_t)e->batch * e->n_weight_rows, size = e->weights_half ? 2 : 4;
         if (!apart(weights, rows * e->keys * size, weights_out, rows * e->keep * size)) return TRN_E_UNSUPPORTED;
     }
+    if (bits8) {
+        for (const void* p : {k_scale, v_scale, (const float*)k_scale_out, (const float*)v_scale_out}) if ((uintptr_t)p & 3) return TRN_E_ALIGN;
+        const int64_t *ks = e->k_scale_out_stride, *vs = e->v_scale_out_stride, blocks = (rows_out + e->block - 1) / e->block;
+        for (const int64_t* st : {e->k_scale_stride, e->v_scale_stride, ks, vs}) if (st[0] < 0 || st[1] < 0) return TRN_E_STRIDE;
+        // (a workgroup writes the scales of one head, of its keys or its values, and nothing else does)
+        if ((e->batch > 1 && (!ks[0] || !vs[0])) || (e->n_kv_heads > 1 && (!ks[1] || !vs[1]))) return TRN_E_STRIDE;
+        if (meet(Extent{k_scale_out, {e->batch, e->n_kv_heads, 1}, {4 * ks[0], 4 * ks[1], 0}, 4 * blocks},
+                 Extent{v_scale_out, {e->batch, e->n_kv_heads, 1}, {4 * vs[0], 4 * vs[1], 0}, 4 * blocks})) return TRN_E_UNSUPPORTED;
+    }
     a.sst[0][0] = e->k_scale_stride[0]; a.sst[0][1] = e->k_scale_stride[1]; a.sst[1][0] = e->v_scale_stride[0]; a.sst[1][1] = e->v_scale_stride[1];
     a.sot[0][0] = e->k_scale_out_stride[0]; a.sot[0][1] = e->k_scale_out_stride[1]; a.sot[1][0] = e->v_scale_out_stride[0]; a.sot[1][1] = e->v_scale_out_stride[1];
     a.order = (uint32_t*)workspace;
