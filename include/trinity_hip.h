@@ -406,7 +406,8 @@ typedef struct trn_cache8 {
  * of ref_rms.py:72-73.  A block's scale is the least power of two s with |x| <= 448 s for its finite values, 2^-32 at least; a code is x * (1 / s) rounded to
  * nearest even, infinities and NaN become NaN.  A block that holds earlier tokens keeps its scale unless the new ones need a larger one:
  * the codes that are there are then multiplied by old / new and rounded again (between powers of two: exactly, but for those that
- * become subnormal).  Nothing else of the cache is written.  k and v must not overlap the cache.
+ * become subnormal).  Nothing else of the cache is written.  k and v must not overlap the cache; its keys and values, and their scales, share no
+ * memory (they may be packed into one tensor).
  */
 int trn_cache8_append_f16(const trn_cache8* cache, const void* k, const void* v, int32_t tokens,
                           int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_s,

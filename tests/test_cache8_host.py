@@ -48,6 +48,24 @@ def test_append_statuses(lib):
     assert _append(lib, tokens=1 << 26, capacity=1 << 26, batch=16) == "TRN_E_SHAPE"
 
 
+def test_append_to_keys_and_values_of_one_place(lib):
+    """One tensor for both, or for both their scales, is refused; packed into one tensor, by sequence, head or token, they are a launch (which fails here)."""
+    M = 1 << 20
+    apart = dict(v=P + M, cache_v=P + 2 * M, k_scale=P + 3 * M, v_scale=P + 4 * M)
+
+    def call(cache_v, v, **kw):
+        st = lib.trn_cache8_append_f16(C.byref(_cache(v=cache_v, **kw)), P + 5 * M, v, 1, 128, 64, 64, 128, 64, 64, None)
+        return _name(lib, st)
+    assert call(**apart) == "TRN_E_LAUNCH"
+    for kw in (dict(cache_v=P), dict(cache_v=P + 64 * 127), dict(v_scale=P + 3 * M), dict(v_scale=P + 3 * M + 4)):
+        assert call(**{**apart, **kw}) == "TRN_E_UNSUPPORTED", kw
+    S, D = 128, 64
+    for b, h, s, off in ((4 * S * D, S * D, D, 2 * S * D), (4 * S * D, 2 * S * D, D, S * D), (4 * S * D, D, 4 * D, 2 * D)):
+        kw = dict(k_stride_b=b, k_stride_h=h, k_stride_s=s, v_stride_b=b, v_stride_h=h, v_stride_s=s)
+        assert call(**{**apart, "cache_v": P + off}, **kw) == "TRN_E_LAUNCH" and call(**{**apart, "cache_v": P + off - 16}, **kw) == "TRN_E_UNSUPPORTED"
+    assert call(**{**apart, "v_scale": P + 3 * M + 8}, ks_stride_b=8, ks_stride_h=4, vs_stride_b=8, vs_stride_h=4) == "TRN_E_LAUNCH"
+
+
 def _attend(lib, q=P, o=P, Hq=4, Sq=1, scale=1.0, w_in=None, w_out=None, ws=None, nbytes=0, qs=(256, 64, 64), os=(256, 64, 64), **kw):
     return _name(lib, lib.trn_cache8_attn_f16(C.byref(_cache(**kw)), q, o, Hq, Sq, *qs, *os, scale, 1, None, w_in, w_out, ws, nbytes, None))
 

@@ -421,6 +421,32 @@ def test_weights_of_no_queries(D):
     assert st == 0 and (o == 0).all() and torch.equal(_cpu(same), w)
 
 
+@pytest.mark.parametrize("axis", [1, 2, 3], ids=["by sequence", "by head", "by token"])
+def test_keys_and_values_of_one_tensor(axis):
+    """Append and attention on caches packed into one tensor, scales too: the bits that tensors of their own give.  One tensor for both is refused."""
+    B, Hq, Hkv, D, S, block, lengths, counts = 2, 4, 2, 64, 200, 32, [200, 131], [3, 2]
+    g = torch.Generator().manual_seed(81)
+    k, v = (torch.randn(B, Hkv, 3, D, generator=g).half().to(DEV) for _ in range(2))
+    q = torch.randn(B, Hq, 3, D, generator=g).half().to(DEV)
+    codes = [ref.encode((torch.randn(B, Hkv, S, D, generator=g) * 100).clamp(-448, 448)).to(DEV) for _ in range(2)]
+    scale = [torch.exp2(torch.randint(-3, 4, (B, Hkv, -(-S // block)), generator=g).float()).to(DEV) for _ in range(2)]
+    pack = lambda x, a: torch.stack(x, a).unbind(a)
+    packed = [t.transpose(1, 2) for t in pack([c.transpose(1, 2) for c in codes], 2)] if axis == 3 else pack(codes, axis)
+    packed_scale = pack(scale, min(axis, 2))
+    outs = []
+    for (k8, v8), (ks, vs) in ((codes, scale), (packed, packed_scale)):
+        ops.cache8_append(k, v, k8, v8, ks, vs, _ints(lengths), _ints(counts), block)
+        o = torch.zeros_like(q)
+        ops.cache8_attention(q, k8, v8, ks, vs, o, lengths=_ints(lengths), counts=_ints(counts), block=block)
+        outs.append(o)
+    assert torch.equal(outs[0], outs[1])
+    for a, b in zip((*codes, *scale), (*packed, *packed_scale)):
+        assert torch.equal(a, b)
+    for kw in (dict(v8=codes[0]), dict(v_scale=scale[0])):
+        with pytest.raises(_lib.TrnError):
+            ops.cache8_append(**{**dict(k=k, v=v, k8=codes[0], v8=codes[1], k_scale=scale[0], v_scale=scale[1], block=block), **kw})
+
+
 @pytest.mark.parametrize("variant", ["vanilla", "prenorm", "weights"])
 def test_the_step_of_projection_append_and_attention(variant):
     """modules.get(.., "cache8"): three steps of a ragged, padded batch, with what its projections leave held to the definitions."""

@@ -134,6 +134,14 @@ extern "C" int trn_cache8_append_f16(const trn_cache8* c, const void* k, const v
     a.n_blocks = (most + 2 * c->block - 2) / c->block;                  // (the first of them may be the last of its block)
     const int64_t units = (int64_t)c->batch * c->n_kv_heads;
     if (units * a.n_blocks > 0xffffff) return TRN_E_SHAPE;            // (threads in 32 bits)
+    // (nor as keys by one workgroup and as values by another)
+    auto same = [&](const void* x, const void* y, int64_t xb, int64_t xh, int64_t xs, int64_t yb, int64_t yh, int64_t ys, int64_t rows, int64_t width) {
+        if (xb < 0 || xh < 0 || yb < 0 || yh < 0) return x == y;
+        return meet(Extent{x, {c->batch, c->n_kv_heads, rows}, {xb, xh, xs}, width}, Extent{y, {c->batch, c->n_kv_heads, rows}, {yb, yh, ys}, width});
+    };
+    if (same(c->k, c->v, c->k_stride_b, c->k_stride_h, c->k_stride_s, c->v_stride_b, c->v_stride_h, c->v_stride_s, c->capacity, c->head_dim) ||
+        same(c->k_scale, c->v_scale, 4 * c->ks_stride_b, 4 * c->ks_stride_h, 0, 4 * c->vs_stride_b, 4 * c->vs_stride_h, 0, 1, 4 * ((c->capacity + c->block - 1) / c->block)))
+        return TRN_E_UNSUPPORTED;
     a.by_blocks = Div(a.n_blocks); a.by_heads = Div(c->n_kv_heads);
     a.xb[0] = k_stride_b; a.xh[0] = k_stride_h; a.xs[0] = k_stride_s;
     a.xb[1] = v_stride_b; a.xh[1] = v_stride_h; a.xs[1] = v_stride_s;
