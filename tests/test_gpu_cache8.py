@@ -481,6 +481,23 @@ def test_the_step_of_projection_append_and_attention(variant):
         _check(_cpu(w), ww, slack + 1e-30, "weights")
 
 
+@pytest.mark.parametrize("variant", ["vanilla", "prenorm", "weights"])
+@pytest.mark.parametrize("B, M", [(2, 0), (0, 3), (0, 0)])
+def test_a_step_of_nothing(B, M, variant):
+    """No token, or no sequence: cache, scales and weights stay as they are."""
+    Hq, Hkv, D, N, S = 4, 2, 64, 256, 120
+    mod = modules.get(variant, "cache8", head_dim=D)
+    half = lambda *s: torch.ones(*s, dtype=torch.float16, device=DEV)
+    codes = [torch.full((B, Hkv, S, D), 5, dtype=torch.uint8, device=DEV) for _ in range(2)]
+    scale = [torch.full((B, Hkv, 2), 0.5, device=DEV) for _ in range(2)]
+    w = torch.full((B, Hkv, S), 3.0, device=DEV)
+    n = _ints([S] * B)
+    for lengths, counts in ((None, None), (n, _ints([0] * B))):
+        mod.forward(codes[0], scale[0], half(B, M, Hq * D), codes[1], scale[1], half(N, Hkv * D), half(N, Hq * D), half(N, Hkv * D), half(B, M, N), counts, lengths,
+                    *((w,) if variant == "weights" else ()))
+    assert all((t == 5).all() for t in codes) and all((t == 0.5).all() for t in scale) and (w == 3.0).all()
+
+
 def test_first_call_inside_a_capture_is_refused():
     k8, ks, dk8, dks, v8, vs, dv8, dvs = _cache(1, 2, 64, 64, 64, 31, [64])
     q = torch.zeros(1, 2, 1, 64, dtype=torch.float16, device=DEV)

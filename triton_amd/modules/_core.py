@@ -626,12 +626,12 @@ class Cache8Step(FusedModule):
         if O2.shape != (B, M, nq):
             raise ValueError(f"O2 {tuple(O2.shape)}: expected {(B, M, nq)}")
         qkv = self._workspace("qkv", (B * M, nq + 2 * nkv), X.dtype, X.device)
-        parts = (qkv[:, :nq], qkv[:, nq:nq + nkv], qkv[:, nq + nkv:])
-        hm = [t.view(B * M, -1, D).permute(1, 0, 2) for t in parts]               # [head, token, D]
-        ops.prenorm_qkv(X.view(B * M, N), None, WQ, WK, WV, *hm, self.eps, self.norm)
-        q, k, v = (t.view(B, M, -1, D).permute(0, 2, 1, 3) for t in parts)        # [B, H, M, D]
+        parts = [(t, t.shape[1] // D) for t in (qkv[:, :nq], qkv[:, nq:nq + nkv], qkv[:, nq + nkv:])]
+        if B * M:
+            ops.prenorm_qkv(X.view(B * M, N), None, WQ, WK, WV, *(t.view(B * M, h, D).permute(1, 0, 2) for t, h in parts), self.eps, self.norm)      # [head, token, D]
+        q, k, v = (t.view(B, M, h, D).permute(0, 2, 1, 3) for t, h in parts)      # [B, H, M, D]
         ops.cache8_append(k, v, K8, V8, K_scale, V_scale, lengths, counts, self.block)
-        self._host.cache8_attention(self._hws, self.scale, self.causal, self.block, K8, K_scale, O2.view(B, M, -1, D).permute(0, 2, 1, 3), q, V8, V_scale,
+        self._host.cache8_attention(self._hws, self.scale, self.causal, self.block, K8, K_scale, O2.view(B, M, nq // D, D).permute(0, 2, 1, 3), q, V8, V_scale,
                                     counts, lengths, None, weights, weights)
 
 
