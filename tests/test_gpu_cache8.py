@@ -498,6 +498,27 @@ def test_a_step_of_nothing(B, M, variant):
     assert all((t == 5).all() for t in codes) and all((t == 0.5).all() for t in scale) and (w == 3.0).all()
 
 
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_a_step_on_another_device_than_the_current_one():
+    B, Hq, Hkv, D, N, S, M = 2, 4, 2, 64, 256, 120, 3
+    g = torch.Generator().manual_seed(91)
+    half = lambda *s: torch.randn(*s, generator=g).half().to("cuda:1")
+    wk, wq, wv, x = half(N, Hkv * D), half(N, Hq * D), half(N, Hkv * D), half(B, M, N)
+    outs = []
+    for current in (0, 1):
+        with torch.cuda.device(current):
+            codes = [torch.zeros(B, Hkv, S, D, dtype=torch.uint8, device="cuda:1") for _ in range(2)]
+            scale = [torch.zeros(B, Hkv, 2, device="cuda:1") for _ in range(2)]
+            o, n = torch.zeros(B, M, Hq * D, dtype=torch.float16, device="cuda:1"), torch.full((B,), M, dtype=torch.int32, device="cuda:1")
+            modules.get("vanilla", "cache8", head_dim=D).forward(codes[0], scale[0], o, codes[1], scale[1], wk, wq, wv, x, None, n)
+            torch.cuda.synchronize("cuda:1")
+            assert torch.cuda.current_device() == current
+            outs.append((o, *codes, *scale))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    with pytest.raises(ValueError, match="device of x"):
+        modules.get("vanilla", "cache8", head_dim=D).forward(codes[0], scale[0], o, codes[1], scale[1], wk.to("cuda:0"), wq, wv, x, None, n)
+
+
 def test_first_call_inside_a_capture_is_refused():
     k8, ks, dk8, dks, v8, vs, dv8, dvs = _cache(1, 2, 64, 64, 64, 31, [64])
     q = torch.zeros(1, 2, 1, 64, dtype=torch.float16, device=DEV)

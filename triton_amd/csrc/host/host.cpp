@@ -383,10 +383,21 @@ bool f_key_scores_forward(Args a, Py_ssize_t n) {         // workspaces, scale |
     return true;
 }
 
+// Launches go to the device of the tensors, which need not be the current one.
+struct OnDevice {
+    int was;
+    explicit OnDevice(int dev) : was((int)c10::hip::current_device()) { if (dev != was) c10::hip::set_device((c10::DeviceIndex)dev); else was = -1; }
+    ~OnDevice() { if (was >= 0) c10::hip::set_device((c10::DeviceIndex)was); }
+};
 bool f_prenorm_qkv(Args a, Py_ssize_t n) {                // x, gamma | None, wq, wk, wv, q_out, k_out, v_out, eps, norm
     count(n, 10, "prenorm_qkv");
-    const View w[3] = {arg(a[2], "wq"), arg(a[3], "wk"), arg(a[4], "wv")}, o[3] = {arg(a[5], "q_out"), arg(a[6], "k_out"), arg(a[7], "v_out")};
-    prenorm_qkv_call(arg(a[0], "x"), opt(a[1], "gamma"), w, o, num(a[8]), flag(a[9]));
+    const View x = arg(a[0], "x"), w[3] = {arg(a[2], "wq"), arg(a[3], "wk"), arg(a[4], "wv")}, o[3] = {arg(a[5], "q_out"), arg(a[6], "k_out"), arg(a[7], "v_out")};
+    const OptView gamma = opt(a[1], "gamma");
+    NEED(x.cuda, "x: expected a GPU tensor");
+    for (const View* t : {&w[0], &w[1], &w[2], &o[0], &o[1], &o[2], &gamma.v})
+        NEED(!t->cuda || t->dev == x.dev, "weights, gamma, outputs: expected tensors on the device of x");
+    const OnDevice here(x.dev);
+    prenorm_qkv_call(x, gamma, w, o, num(a[8]), flag(a[9]));
     return true;
 }
 
@@ -501,12 +512,6 @@ bool f_gmlp_forward(Args a, Py_ssize_t n) {               // workspaces, silu, O
 }
 
 // ---------------------------------------------------------------------------------------------- 8-bit caches, eviction
-// Launches go to the device of the tensors, which need not be the current one.
-struct OnDevice {
-    int was;
-    explicit OnDevice(int dev) : was((int)c10::hip::current_device()) { if (dev != was) c10::hip::set_device((c10::DeviceIndex)dev); else was = -1; }
-    ~OnDevice() { if (was >= 0) c10::hip::set_device((c10::DeviceIndex)was); }
-};
 void on(const View& t, const char* n, const View& first) { NEED(t.cuda && t.dev == first.dev, "%s: expected a tensor on the device of the others", n); }
 void dims4(const View& t, const char* n, int64_t b, int64_t h, int64_t s, int64_t d) {
     NEED(t.dim == 4 && t.s[0] == b && t.s[1] == h && t.s[2] == s && t.s[3] == d, "%s %s: expected (%lld, %lld, %lld, %lld)", n, t.shape().c_str(),
