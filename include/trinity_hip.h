@@ -416,6 +416,8 @@ int trn_cache8_append_f16(const trn_cache8* cache, const void* k, const void* v,
 /*
  * o = softmax(scale * q k^T) v over an 8-bit cache: trn_attn_fwd_f16 for q, o [batch, n_q_heads, seq_q, head_dim] fp16 (o on 8 bytes, apart from q), GQA / MQA.
  * causal: query i sees the keys j <= lengths[b] - counts[b] + i.  A query that sees no key gets zeros (lse -inf).
+ * Scores, sums and key weights are in fp32.  The weights enter the product with V in fp16: as two numbers each (what the first leaves over is the second) where
+ * all sequences' heads together have up to 512 rows of queries, or a KV head one tile of them (16 rows, 32 with many heads), as one otherwise.
  *   lse           nullable float [batch, n_q_heads, seq_q] contiguous, natural log.
  *   weights_out   nullable float [batch, n_kv_heads, capacity] contiguous: weights_in (nullable: zeros) plus the attention weight that each key gets,
  *                 summed over the queries and the query heads of its KV head; keys from lengths[b] on are left as they are.  weights_in may be

@@ -12,11 +12,11 @@ using namespace trn;
 static long bad = 0, plans = 0, fewer = 0;
 static void look(int batch, int kv, int cap, int d, int hq, int sq, bool weights) {
     const Plan8 p = plan8(batch, kv, cap, d, hq, sq, weights);
-    int nq = 0, ks = 0; bool past = false;
-    with_kernel8(p, [&](auto a, auto b, auto c) { nq = a; ks = b; past = c; });
+    int nq = 0, ks = 0; bool past = false, fine = false;
+    with_kernel8(p, [&](auto a, auto b, auto c, auto d) { nq = a; ks = b; past = c; fine = d; });
     ++plans;
     fewer += ks < 4;
-    bool ok = nq == p.nq && ks == p.ks && past == (p.n_rt == 1) && (int64_t)p.n_rt * 16 * nq >= p.R && p.ns >= 1 && p.ns <= 64 && (p.n_rt - 1) * 16 * nq < p.R;
+    bool ok = nq == p.nq && ks == p.ks && past == (p.n_rt == 1) && fine == p.fine && (int64_t)p.n_rt * 16 * nq >= p.R && p.ns >= 1 && p.ns <= 64 && (p.n_rt - 1) * 16 * nq < p.R;
     ok = ok && (ks == 4 || nq == 2) && (ks > 1 || p.ns == 1) && (p.sp == 0 || (p.n_rt == 1 && p.R <= 16));
     // the tiles of 32 keys that a wave takes (those of all waves one after the other), of caches from none to all
     const int most = (cap + 31) / 32, waves = ks * p.ns;

@@ -235,6 +235,26 @@ def test_large_scores_and_a_single_key_that_takes_all():
     _hold(r, case[7])
 
 
+FEW = [ATTNS[0], ATTNS[1], ATTNS[4], ATTNS[8], ATTNS[9], ATTNS[10], ATTNS[14], (1, 8, 2, 128, 1, 900, 64, [900], [1], True), (96, 8, 2, 128, 8, 75, 32, [1 + b % 75 for b in range(96)], [int(b % 8 == 0) * 8 for b in range(96)], True)]
+
+
+@pytest.mark.parametrize("size", [0.05, 1.0, 8.0, 40.0])
+@pytest.mark.parametrize("case", FEW, ids=lambda c: f"B{c[0]}q{c[1]}kv{c[2]}D{c[3]}M{c[4]}S{c[5]}")
+def test_weights_of_few_rows_are_not_rounded(case, size):
+    """Where all heads have up to 512 rows, or each one row tile, the weight of a key is two numbers of fp16: what the first leaves over, at most 2^-11 of it, is rounded to 2^-11 of
+    that, or to 2^-25 of the largest weight.  So of the oracle's bound 2^-22 is left of the term for a weight's rounding, where it has 2^-11; of the output's own
+    rounding half a step, 2^-11 of it, or 2^-25."""
+    r = _attend(case, size=size)
+    there = r["there"][..., None].expand_as(r["want"])
+    B, Hq, Hkv, D, M, S, block, lengths, counts, causal = case
+    q, k8, v8, ks, vs = (_cpu(r[n]) for n in ("q", "k8", "v8", "ks", "vs"))
+    _, _, _, tol, _, _ = ref.attention(q, k8, v8, ks, vs, D ** -0.5, causal, lengths, counts, block)
+    mass = ref.attention(q, k8, v8 & 0x7f, ks, vs, D ** -0.5, causal, lengths, counts, block)[0]       # sum of p |v|
+    fine = tol - (2.0 ** -11 - 2.0 ** -22) * mass
+    assert (fine[there] >= 0).all()       # (zero for a query that sees no key: exactly zeros)
+    _check(r["o"][there], r["want"][there], fine[there], "o")
+
+
 @pytest.mark.parametrize("case", [ATTNS[6], ATTNS[7], ATTNS[3]], ids=["prompt", "tile", "chunk"])
 def test_nan_of_a_key_reaches_only_the_queries_that_see_it(case):
     def edit(k8, ks, v8, vs):

@@ -12,6 +12,9 @@
 // is added to the exponent: with t = s + log2 vs, p = 2^(t - m) is the weight of the CODES of V, and the sum of probabilities is
 // that of p / vs, one multiplication a tile.  The reference m is a maximum of t: what counts for the output is near one in fp16, however
 // much the blocks differ.  (A block whose vs is below 2^-64 adds nothing that fp16 could hold; it counts in the sum alone.)
+// The product with V takes p as fp16.  Rounded once, it brings an error of 2^-12 of each key's part, about as much as the output's own rounding: the
+// distance from 64 bits is then 1.0 to 1.45 times that of a computation in fp32 with more than 512 rows (480 drawn shapes), but up to 1.65 times with few, of which
+// one may be off by 2^-11 throughout.  There p is two numbers of fp16 (1.00 times), at the price of the second product.
 //
 // A row tile's waves (four, two or one of a workgroup), and workgroups (shares), have consecutive runs of the keys that its rows see; their results
 // are joined by (m, l, O) in LDS, and by a second launch.
@@ -58,8 +61,8 @@ __device__ __forceinline__ float quad_sum(float x) { float a = x, b = x; swap_ro
 #endif
 
 // KS waves of the four have a row tile's keys, one after the other; 4 / KS row tiles a workgroup.  PAST: a single row tile reads the cache, each byte
-// once (see plan8).
-template <int D, int NQ, int KS, bool PAST>
+// once.  FINE: the weight enters the product with V as two fp16 numbers, what the first leaves over being the second, not rounded to one (see plan8).
+template <int D, int NQ, int KS, bool PAST, bool FINE>
 __global__ __launch_bounds__(256, 2) void cache8_attn_kernel(const Attn8Args a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr int NW = 4, NG = NW / KS, NJ = D / 64, NDB = D / 16, RT = 16 * NQ;      // 16-byte K reads a lane and key half, of two contraction steps each; output blocks
@@ -210,7 +213,7 @@ __global__ __launch_bounds__(256, 2) void cache8_attn_kernel(const Attn8Args a) 
                 for (int i = 0; i < NDB; ++i) o[i][qb] = o[i][qb] * alpha;
             }
         }
-        half8_t p[NQ];
+        half8_t p[NQ], p_rest[NQ];
 #pragma unroll
         for (int qb = 0; qb < NQ; ++qb) {
             const float d = (m[qb] == -INFINITY ? 0.f : -m[qb]) + lv;
@@ -219,7 +222,11 @@ __global__ __launch_bounds__(256, 2) void cache8_attn_kernel(const Attn8Args a) 
             for (int kb = 0; kb < 2; ++kb) {
                 float x[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) { x[e] = fast_exp2(__builtin_fmaf(s[kb][qb][e], c, d)); p[qb][4 * kb + e] = (half_t)x[e]; }
+                for (int e = 0; e < 4; ++e) {
+                    x[e] = fast_exp2(__builtin_fmaf(s[kb][qb][e], c, d));
+                    p[qb][4 * kb + e] = (half_t)x[e];
+                    if constexpr (FINE) p_rest[qb][4 * kb + e] = (half_t)(x[e] - (float)p[qb][4 * kb + e]);
+                }
                 sum[kb] = (x[0] + x[1]) + (x[2] + x[3]);
             }
             l[qb] = __builtin_fmaf(sum[0] + sum[1], inv, l[qb]);
@@ -258,7 +265,10 @@ __global__ __launch_bounds__(256, 2) void cache8_attn_kernel(const Attn8Args a) 
         for (int i = 0; i < NDB; ++i) {
             const half8_t v = half_of_codes(vw[i].x, vw[i].y);
 #pragma unroll
-            for (int qb = 0; qb < NQ; ++qb) o[i][qb] = mfma16(v, p[qb], o[i][qb]);
+            for (int qb = 0; qb < NQ; ++qb) {
+                o[i][qb] = mfma16(v, p[qb], o[i][qb]);
+                if constexpr (FINE) o[i][qb] = mfma16(v, p_rest[qb], o[i][qb]);
+            }
         }
     };
     // Everything of the stage that the next load overwrites has been read: its values are in registers before the load goes out.
@@ -475,13 +485,13 @@ extern "C" int trn_cache8_attn_f16(const trn_cache8* c, const void* q, void* o, 
     a.n_chunks = p.n_chunks; a.chunk_tiles = p.chunk_tiles; a.w_part = p.n_chunks > 1 ? (float*)((char*)workspace + p.more) : nullptr;
     const hipStream_t s = (hipStream_t)stream;
     const bool d128 = c->head_dim == 128;
-    with_kernel8(p, [&](auto nq, auto ks, auto past) {
+    with_kernel8(p, [&](auto nq, auto ks, auto past, auto fine) {
         constexpr int NQ = decltype(nq)::value, KS = decltype(ks)::value;
-        constexpr bool PAST = decltype(past)::value;
+        constexpr bool PAST = decltype(past)::value, FINE = decltype(fine)::value;
         a.by_w = Div(KS * p.ns);
         const dim3 grid((unsigned)groups), block(256);
-        if (d128) hipLaunchKernelGGL((cache8_attn_kernel<128, NQ, KS, PAST>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((cache8_attn_kernel<64, NQ, KS, PAST>), grid, block, 0, s, a);
+        if (d128) hipLaunchKernelGGL((cache8_attn_kernel<128, NQ, KS, PAST, FINE>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((cache8_attn_kernel<64, NQ, KS, PAST, FINE>), grid, block, 0, s, a);
     });
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && (p.ns > 1 || p.sp)) e = launch_cache8_finish(a, c->head_dim, s);

@@ -7,8 +7,9 @@
 namespace trn {
 
 // G query heads a KV head, R rows; n_rt tiles of 16 nq rows; ks waves and ns workgroups (shares) have a tile's keys; the key weights of many rows in n_chunks of chunk_tiles
-// row tiles, of few rows from sp scores a row; offsets of the workspace's parts behind the shares' outputs, and its size.
-struct Plan8 { int G, R, nq, ks, n_rt, ns, n_chunks, chunk_tiles, sp; int64_t ml, lse2, more, bytes; };
+// row tiles, of few rows from sp scores a row; weights as two fp16 numbers or one (fine);
+// offsets of the workspace's parts behind the shares' outputs, and its size.
+struct Plan8 { int G, R, nq, ks, n_rt, ns, n_chunks, chunk_tiles, sp; bool fine; int64_t ml, lse2, more, bytes; };
 
 // Rows of a tile: 32 where they make workgroups enough, otherwise 16, whose waves have half the work a key and need half the registers.  us, tiles of
 // 16 / 32 rows, each with its best number of shares: 16 heads of 64, batch 4, 2000 keys, 64 queries (128 tiles of 32) 10.2 / 13.0, 300 (640) 23.6 / 21.6; 71
@@ -54,6 +55,10 @@ inline Plan8 plan8(int batch, int n_kv_heads, int capacity, int head_dim, int Hq
     p.ns = (int)(ns < 1 ? 1 : ns > 64 ? 64 : ns);
     // (there is one share above 288 row tiles, the most of which two fit; a wave that has all keys of its rows writes no share)
     p.ks = p.nq == 1 || p.n_rt == 1 || units <= 700 ? 4 : units < 2560 || p.ns > 1 ? 2 : 1;
+    // (The errors of few rows' weights do not average out, and there the second product costs little.  us with one number / two: one row tile, 32 x 1 on 8193 81.8 / 82.5, 16 x 8
+    // queries of 32 heads on 8 on 4000 29.4 / 30.5, 96 x 8 on 300 19.6 / 20.9; several of 512 rows at most, 32 on 8 of 128, 16 queries on 16000 keys 16.9 / 18.8, on 60000 47.6 /
+    // 50.1, 71 on one of 64, 5 on 16000 12.4 / 13.5, on 60000 22.8 / 26.5; of more, 100 queries on 16000 46.2 / 57.2, the 512 on 8448 85 / 110, four prompts of 2047 169 / 209.)
+    p.fine = p.n_rt == 1 || heads * p.R <= 512;
     auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
     p.ml = p.ns > 1 ? up(units * p.ns * 16 * p.nq * head_dim * 4) : 0;
     p.lse2 = p.ml + (p.ns > 1 ? up(units * p.ns * 32 * p.nq * 4) : 0);
@@ -77,17 +82,19 @@ inline Plan8 plan8(int batch, int n_kv_heads, int capacity, int head_dim, int Hq
     return p;
 }
 
-// The kernel that such a plan is for: f(nq, ks, past) of constants, past where a single row tile reads a cache.  What is launched, and by how much its waves
-// divide a row tile's keys, are one choice: with ks of the plan and another one of the kernel, waves would walk behind the last key.
+// The kernel that such a plan is for: f(nq, ks, past, fine) of constants, past where a single row tile reads a cache.  What is launched, and by how much its
+// waves divide a row tile's keys, are one choice: with ks of the plan and another one of the kernel, waves would walk behind the last key.
 template <class F> inline void with_kernel8(const Plan8& p, F&& f) {
     const std::integral_constant<int, 1> one{};
     const std::integral_constant<int, 2> two{};
     const std::integral_constant<int, 4> four{};
-    if (p.n_rt == 1) p.nq == 1 ? f(one, four, std::true_type{}) : f(two, four, std::true_type{});
-    else if (p.nq == 1) f(one, four, std::false_type{});
-    else if (p.ks == 4) f(two, four, std::false_type{});
-    else if (p.ks == 2) f(two, two, std::false_type{});
-    else f(two, one, std::false_type{});
+    const std::true_type yes{};
+    const std::false_type no{};
+    if (p.n_rt == 1) p.nq == 1 ? f(one, four, yes, yes) : f(two, four, yes, yes);
+    else if (p.nq == 1) p.fine ? f(one, four, no, yes) : f(one, four, no, no);
+    else if (p.ks == 4) p.fine ? f(two, four, no, yes) : f(two, four, no, no);
+    else if (p.ks == 2) f(two, two, no, no);
+    else f(two, one, no, no);
 }
 
 }  // namespace trn
