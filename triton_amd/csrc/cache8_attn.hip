@@ -13,16 +13,18 @@
 // that of p / vs, one multiplication a tile.  The reference m is a maximum of t: what counts for the output is near one in fp16, however
 // much the blocks differ.  (A block whose vs is below 2^-64 adds nothing that fp16 could hold; it counts in the sum alone.)
 // The product with V takes p as fp16.  Rounded once, it brings an error of 2^-12 of each key's part, about as much as the output's own rounding: the
-// distance from 64 bits is then 1.0 to 1.45 times that of a computation in fp32 with more than 512 rows (480 drawn shapes), but up to 1.65 times with few, of which
+// distance from 64 bits is then 1.0 to 1.45 times that of a computation in fp32 with more than 512 rows (400 drawn shapes), but up to 1.65 times with few, of which
 // one may be off by 2^-11 throughout.  There p is two numbers of fp16 (1.00 times), at the price of the second product.
 //
 // A row tile's waves (four, two or one of a workgroup), and workgroups (shares), have consecutive runs of the keys that its rows see; their results
 // are joined by (m, l, O) in LDS, and by a second launch.
 //
-// One query on a long cache is bound by memory: 32 sequences of up to 8193 keys, 8 heads of 128, 408 MB in 67 us, 6.1 TB/s; one of 131072, 269 MB, 47 us + 4
-// for the joining of shares.  Chunks and prompts are bound by the board's power (1.8 to 2.0 GHz): 512 queries of 32 heads on 8448 keys 81 to 86 us, 800 to 850
-// TFLOP/s, four prompts of 2047 161 us, 850.  A few hundred rows a head (71 heads of 64 on one, 16 queries, 3001 keys: 19.5 us) are bound by vector work: K's and V's
-// conversion, and 2.2 workgroups a compute unit.
+// One query on a long cache is bound by memory: 32 sequences of up to 8193 keys, 8 heads of 128, 408 MB in 68 us, 6.0 TB/s; one of 131072, 269 MB, 47 us + 4
+// for the joining of shares.  Chunks and prompts are bound by the conversion of K and V beside the products, which every row tile repeats: 512 queries of 32 heads on
+// 8448 keys 80 us, 860 TFLOP/s (the attention on fp16 caches 93), four prompts of 2047 166 us, 830 (134), one of 4096 157, 870 (118).  So are a few hundred rows a head (71 heads of
+// 64 on one, up to 16 queries on up to 3001 keys 19.2 us; all as long 22.3), with two or three workgroups a compute unit as they come.
+// Sequences of very different lengths are not shared out evenly, as the host does not know them: one of 131072 keys among 31 of 1000, one query 600 us, as many keys
+// in equal lengths 53.
 #include "cache8.h"
 #include "cache8_rules.h"
 

@@ -17,7 +17,7 @@ struct Plan8 { int G, R, nq, ks, n_rt, ns, n_chunks, chunk_tiles, sp; bool fine;
 // one prompt of 1501 (1504) 49 / 37.  And where the keys are so many that shares make them (row tiles x tiles of 32 keys): 16 heads of 64, 311 queries on 8869 keys
 // (160 x 278) 31.5 / 29.4; 32 of 128 on 8, 100 on 16000 (104 x 500) 56.8 / 46.3; 8 on 2, 2 x 102 on 36907 (52 x 1153) 64.6 / 52.5; but 71 of 64 on one, 8 x 16 on 3017 (288 x
 // 95) 19.7 / 21.8.
-// Shares of a row tile's keys: one workgroup a compute unit over the launch -- one share from some 160 row tiles on --, no more shares than tiles of 32 keys.  32 heads
+// Shares of a row tile's keys: one workgroup a compute unit over the launch -- one share from 129 row tiles on where each head has one --, no more shares than tiles of 32 keys.  32 heads
 // of 128 on 8, one query, us with 1 / 2 / 4 / 8 / 16 / 32 shares: 1025 keys 9.6 / 10.9 / 9.5 / 9.3 / 9.0 / 8.9; batch 8, 1500 keys 12.0 / 12.4 / 11.9 / 12.5 / 16.6; batch 12, 3000
 // 23.7 / 19.5 / 20.8; batch 16, 4097 31.3 / 28.6 / 28.4; batch 24, 4000 33.9 / 41.6 / 39.9; batch 32, 8192 88.7 / 91.4 / 93.8; of two to one lengths 70.5 / 72.2 / 70.8.  A
 // second launch is some 3 us: short caches have one share, but where few rows' weights need that launch anyway (512 keys 6.4, against 8.5; batch 8: 1025 keys 10.1 / 11.0; 16
@@ -70,6 +70,7 @@ inline Plan8 plan8(int batch, int n_kv_heads, int capacity, int head_dim, int Hq
         // (Two workgroups a compute unit, all that it holds; three for a prompt, half of whose queries and keys do not see each other; chunks of two row tiles
         // at least (a prompt of 128 with chunks of one / two / four / six 12.5 / 13.2 / 15.6 / 19.0, of 300 23.3 / 19.3 / 20.5 / 23.2).  32 heads of 128 on 8, us a call with one / two / three / four / six: prompts of 1501 82 / 65 / 61 / 66 / 63, of 4096 374 / 293 / 266 / 296 /
         // 269; 512 queries, 4096 keys 80 / 70 / 77 / 73 / 75.)
+        // (By the capacity, as the host does not know the lengths: a prompt of 1501 on a cache of 1501 / 4096 / 8192 / 32768 keys 61 / 86 / 125 / 185 us.)
         const int64_t blocks = heads * ((capacity + 255) / 256);
         int64_t chunks = blocks ? (2 * Sq > capacity ? 768 : 512) / blocks : 1;
         if (chunks > tiles32 / 2) chunks = tiles32 / 2;

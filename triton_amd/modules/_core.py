@@ -608,7 +608,7 @@ class Cache8Step(FusedModule):
     """The decode-append step (ref_rms.py:45-83, 101-127) on an 8-bit cache of a batch whose sequences have lengths of their own: X [B,M,N] is
     projected (norm=True: RMS-normalised first, no weight), keys and values are quantised into the cache, the queries attend over it, O2 [B,M,Hq*D].
     WQ [N,Hq*D], WK, WV [N,Hkv*D]; lengths and counts as in `ops.cache8_append`, with this step's tokens.  Three launches, or four with a
-    cache's shares."""
+    cache's shares; with the weights of few rows four, of many up to six."""
     TENSOR_PARAMS = ["K8", "K_scale", "O2", "V8", "V_scale", "WK", "WQ", "WV", "X", "counts", "lengths"]
 
     def __init__(self, head_dim: int, scale: Optional[float] = None, causal: bool = True, block: int = 64, norm: bool = False, eps: float = 0.0):
