@@ -462,6 +462,80 @@ int trn_cache_evict(const trn_cache_evict_desc* desc, const void* k, const void*
                     float* k_scale_out, float* v_scale_out, const void* weights, void* weights_out, const int32_t* lengths,
                     int32_t* kept, int32_t* new_lengths, void* workspace, int64_t workspace_bytes, void* stream);
 
+/*
+ * An fp16 key/value cache [batch, n_kv_heads, capacity, head_dim] whose sequences have lengths of their own, as in trn_cache8: lengths and counts
+ * (nullable int32 [batch], on the device) are the keys of each sequence, this step's new ones among them, and its new tokens.
+ * Strides {batch, head, token} are in elements, not negative, multiples of 8, that of a token at most 2^23; head_dim 64 or 128; capacity at most 2^26.
+ */
+typedef struct trn_cache16 {
+    void* k; void* v;
+    const int32_t* lengths; const int32_t* counts;
+    int32_t batch, n_kv_heads, capacity, head_dim;
+    int64_t k_stride[3], v_stride[3];
+} trn_cache16;
+
+/*
+ * New tokens into an fp16 cache, normalised by head and rotated by their positions: the QKNorm of ref_rms.py:197-231 and the append of
+ * ref_rms.py:72-73 with the positions that the reference leaves out, in one pass.  For the row i < counts[b] of q [batch, n_q_heads, tokens, head_dim] and k, v
+ * [batch, n_kv_heads, tokens, head_dim]:
+ *   norm         x <- x / sqrt(mean(x^2) + eps) * gamma for queries and keys, gamma_q, gamma_k nullable fp16 [head_dim].
+ *   rotation     pair p < pairs of queries and keys, (x[p], x[p + pairs]) or, interleaved, (x[2 p], x[2 p + 1]), is turned by the angle position * inv_freq[p],
+ *                formed in 64 bits; the other dimensions stay.  pairs: a multiple of 4, 2 * pairs <= head_dim, 0 for none.
+ *   position     lengths[b] - counts[b] + i, or positions[axis][b][i] (int32, contiguous [axes, batch, tokens]); of several axes (time, height, width)
+ *                the pairs lie section by section, sections[axis] of them: their sum is pairs.  Up to four axes; more than one needs positions.
+ *   outputs      q_out[b, :, i] (q itself, with its strides, or apart from it); k_cache, v_cache at lengths[b] - counts[b] + i.  Of more new tokens than
+ *                keys the last ones are the cache's.  Computed in 32 bits, rounded once.  Nothing else is read or written.
+ * The cache shares no memory with q, k, v, q_out, nor its keys with its values (they may be packed into one tensor).
+ */
+typedef struct trn_rope {
+    const double* inv_freq; const int32_t* positions;
+    const void* gamma_q; const void* gamma_k;
+    int32_t pairs, interleaved, axes, norm;
+    int32_t sections[4];
+    float eps;
+} trn_rope;
+int trn_cache_rope_append_f16(const trn_cache16* cache, const trn_rope* rope, const void* q, void* q_out, const void* k, const void* v,
+                              int32_t n_q_heads, int32_t tokens, const int64_t* q_stride, const int64_t* q_out_stride,
+                              const int64_t* k_stride, const int64_t* v_stride, void* stream);
+
+/*
+ * o = softmax(scale * q [K_prefix ; K]^T) [V_prefix ; V]: attention of a batch whose sequences begin alike.  k_prefix, v_prefix [n_kv_heads, prefix, head_dim]
+ * (strides {head, token}, as the cache's) are seen by every query and read once for all; of its own sequence a query sees, causal, the
+ * keys j <= lengths[b] - counts[b] + i, otherwise all.  q, o [batch, n_q_heads, seq_q, head_dim] fp16, GQA / MQA, o on 8 bytes and apart from q; rows from counts[b] on are
+ * neither read nor written.  prefix 0: attention over the cache alone.  A query that sees no key gets zeros.  Scores, sums and the joining of shares are in fp32.
+ *   workspace  trn_cache_prefix_attn_workspace_bytes(...) bytes, 256-byte aligned, no initial contents; TRN_E_SCRATCH if smaller.  One call at a time may use it.
+ */
+typedef struct trn_prefix {
+    const void* k; const void* v;
+    int32_t keys;
+    int64_t k_stride[2], v_stride[2];
+} trn_prefix;
+int64_t trn_cache_prefix_attn_workspace_bytes(const trn_cache16* cache, int32_t prefix_keys, int32_t n_q_heads, int32_t seq_q);
+int trn_cache_prefix_attn_f16(const trn_cache16* cache, const trn_prefix* prefix, const void* q, void* o, int32_t n_q_heads, int32_t seq_q,
+                              const int64_t* q_stride, const int64_t* o_stride, float scale, int32_t causal,
+                              void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * The bounds of a cache's blocks of 32, 64 or 128 keys, by channel: bounds fp16 [batch, n_kv_heads, ceil(capacity / block), 2, head_dim] contiguous, the least and the
+ * largest of a block's keys.  Brought up to date for the blocks that the new tokens lie in, out of all keys that these hold; the others stay.  NaN does not count
+ * (a channel of nothing else: +inf, -inf).  The cache's v is not looked at and may be NULL.
+ */
+int trn_cache_bounds_f16(const trn_cache16* cache, int32_t block, int32_t tokens, void* bounds, void* stream);
+
+/*
+ * Causal attention of each query over `top` blocks of its sequence.  A block's score is the most that a key within its bounds could have,
+ * max over the KV head's query heads of sum_d max(q[d] lo[d], q[d] hi[d]), summed in 64 bits and rounded to 32; NaN counts as the least.  Selected are, of the blocks that hold a
+ * key which the query sees, the first `sink` ones, the last `recent` ones (its own is the last of them), and of the others those with the largest scores, ties to the
+ * earlier block: min(top, their number) in all.  sink + recent <= top, recent >= 1, top <= 2^16.
+ *   selected   int32 [batch, n_kv_heads, seq_q, top] contiguous: the blocks, ascending, then -1; rows from counts[b] on stay.
+ *   q, o, workspace and a query that sees no key as in trn_cache_prefix_attn_f16.
+ */
+int64_t trn_cache_sparse_attn_workspace_bytes(const trn_cache16* cache, int32_t block, int32_t top, int32_t n_q_heads, int32_t seq_q);
+int trn_cache_sparse_attn_f16(const trn_cache16* cache, const void* bounds, int32_t block, int32_t top, int32_t sink, int32_t recent,
+                              const void* q, void* o, int32_t* selected, int32_t n_q_heads, int32_t seq_q,
+                              const int64_t* q_stride, const int64_t* o_stride, float scale,
+                              void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -68,6 +68,23 @@ class CacheEvictDesc(C.Structure):
         [(n, C.c_int64 * 2) for n in ("k_scale_stride", "v_scale_stride", "k_scale_out_stride", "v_scale_out_stride")]
 
 
+class Cache16(C.Structure):
+    """Mirror of `trn_cache16`."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("lengths", C.c_void_p), ("counts", C.c_void_p)] + \
+        [(n, C.c_int32) for n in ("batch", "n_kv_heads", "capacity", "head_dim")] + [("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3)]
+
+
+class Rope(C.Structure):
+    """Mirror of `trn_rope`."""
+    _fields_ = [("inv_freq", C.c_void_p), ("positions", C.c_void_p), ("gamma_q", C.c_void_p), ("gamma_k", C.c_void_p)] + \
+        [(n, C.c_int32) for n in ("pairs", "interleaved", "axes", "norm")] + [("sections", C.c_int32 * 4), ("eps", C.c_float)]
+
+
+class Prefix(C.Structure):
+    """Mirror of `trn_prefix`."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("keys", C.c_int32), ("k_stride", C.c_int64 * 2), ("v_stride", C.c_int64 * 2)]
+
+
 _lib: Optional[C.CDLL] = None
 
 
@@ -145,6 +162,19 @@ def load() -> C.CDLL:
     lib.trn_cache_evict_workspace_bytes.argtypes = [C.POINTER(CacheEvictDesc)]
     lib.trn_cache_evict.restype = C.c_int
     lib.trn_cache_evict.argtypes = [C.POINTER(CacheEvictDesc)] + [vp] * 14 + [i64, vp]
+    st = C.POINTER(i64)
+    lib.trn_cache_rope_append_f16.restype = C.c_int
+    lib.trn_cache_rope_append_f16.argtypes = [C.POINTER(Cache16), C.POINTER(Rope), vp, vp, vp, vp, i32, i32, st, st, st, st, vp]
+    lib.trn_cache_prefix_attn_workspace_bytes.restype = C.c_int64
+    lib.trn_cache_prefix_attn_workspace_bytes.argtypes = [C.POINTER(Cache16), i32, i32, i32]
+    lib.trn_cache_prefix_attn_f16.restype = C.c_int
+    lib.trn_cache_prefix_attn_f16.argtypes = [C.POINTER(Cache16), C.POINTER(Prefix), vp, vp, i32, i32, st, st, f32, i32, vp, i64, vp]
+    lib.trn_cache_bounds_f16.restype = C.c_int
+    lib.trn_cache_bounds_f16.argtypes = [C.POINTER(Cache16), i32, i32, vp, vp]
+    lib.trn_cache_sparse_attn_workspace_bytes.restype = C.c_int64
+    lib.trn_cache_sparse_attn_workspace_bytes.argtypes = [C.POINTER(Cache16), i32, i32, i32, i32]
+    lib.trn_cache_sparse_attn_f16.restype = C.c_int
+    lib.trn_cache_sparse_attn_f16.argtypes = [C.POINTER(Cache16), vp, i32, i32, i32, i32, vp, vp, vp, i32, i32, st, st, f32, vp, i64, vp]
     lib.trn_calibration_copy.restype = C.c_int
     lib.trn_calibration_copy.argtypes = [vp, vp, i64, vp]
     lib.trn_calibration_mfma.restype = C.c_int

@@ -1,0 +1,390 @@
+// Attention over fp16 caches by tiles of rows: what the shared-prefix and the selected-blocks form have in common.
+//
+// The rows of a KV head are its query heads' queries, row r = (query r / G, head r % G): a tile of them reads a key once.  Two forms of a tile:
+//   narrow   16 or 32 rows; each of a workgroup's four waves has 32 keys of its own at a time, so that four times as many bytes are on their way; the waves' results are
+//            joined in LDS.  For few rows, which memory bounds.
+//   wide     128 rows, 32 a wave; the waves share 64 keys in LDS.  For many rows, which the matrix pipe bounds.
+// In both K and V come from memory straight into LDS, one stage ahead, scores are formed transposed, S^T = K Q^T, so that a lane's scores are the
+// operand P^T of O^T += V^T P^T as they are, and V is read transposing.  One pass with a running maximum m, taken anew only where a score exceeds it by 2^8, and sum l.
+// A workgroup may have a share of a tile's keys: (m, l, O) of the shares of a row are joined by a second launch (cache16_join).
+#pragma once
+#include "cache16.h"
+
+namespace trn {
+
+// What became of a row's keys in one share: O unnormalised, and (m, l) with m in units of log2.  Row `row` of B Hkv M G has `slots` of them.
+struct Parts { float* o; float* ml; int slots; };
+
+constexpr int kNarrowLds(int D) { return 4 * 4 * 32 * D * 2; }
+constexpr int kWideLds(int D) { return 4 * 64 * D * 2; }
+
+#if defined(__HIP_DEVICE_COMPILE__)
+__device__ __forceinline__ float4_t mfma16(half8_t a, half8_t b, float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+// Over the four lanes n, n + 16, n + 32, n + 48 of a row.
+__device__ __forceinline__ void swap_rows16(float& a, float& b) { asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b)); }
+__device__ __forceinline__ float quad_max(float x) { float a = x, b = x; swap_rows16(a, b); return half_max(fmaxf(a, b)); }
+__device__ __forceinline__ float quad_sum(float x) { float a = x, b = x; swap_rows16(a, b); return half_sum(a + b); }
+
+// Where a 16-byte chunk of a narrow stage's row lies.  A K read is served 16 lanes at a time ({0-3, 12-15, 20-27} and the others): the rows {0-3, 12-15} at one
+// chunk and {4-11} at its neighbour.  A transposing V read is served in halves of the wave: eight rows at two neighbouring chunks.
+template <int D> __device__ __forceinline__ int kn_swz(int r) { return D == 128 ? ((r & 3) << 2) | ((r >> 3 & 1) * 3) : ((r >> 1 & 1) << 2) | ((r >> 3 & 1) * 3); }
+template <int D> __device__ __forceinline__ int vn_swz(int r) { return D == 128 ? (r & 7) << 1 : (r >> 1 & 3) << 1; }
+
+// Which of eight fp16 values are not finite.
+__device__ __forceinline__ bool odd_values(half8_t v) {
+    const uint4_t w = __builtin_bit_cast(uint4_t, v);
+    uint32_t bad = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bad |= ((w[i] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+    return bad != 0;
+}
+// ... as numbers: one where a value is +inf (kind 0), -inf (1), NaN (2), zero elsewhere.
+__device__ __forceinline__ half8_t odd_kind(half8_t v, int kind) {
+    half8_t r;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const half_t x = v[e];
+        const bool is = kind == 0 ? x == (half_t)INFINITY : kind == 1 ? x == (half_t)-INFINITY : x != x;
+        r[e] = is ? (half_t)1.f : (half_t)0.f;
+    }
+    return r;
+}
+__device__ __forceinline__ half8_t finite_only(half8_t v) {
+    half8_t r;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = fabsf((float)v[e]) < INFINITY ? v[e] : (half_t)0.f;
+    return r;
+}
+
+// ------------------------------------------------------------------------------------------------ narrow
+// One wave's tiles t0 <= t < t1 of 32 keys for 16 NQ rows (queries in qB), into o, m, l.  `keys`: where the tile t begins and how many of its keys there are (0..32, wave-uniform; those
+// from there on arrive as zeros and count for no row), as .k(t), .v(t), .n(t), requested in order.  Keys from `last` on (relative to the tile, through .at(t)) are hidden from a row.
+template <int D, int NQ, class Keys>
+__device__ __forceinline__ void narrow_walk(Keys& keys, int t0, int t1, int t_mask, int kpitch, int vpitch, float c, const half8_t (&qB)[NQ][D / 32], const int (&last)[NQ], char* lds,
+                                            float4_t (&o)[D / 16][NQ], float (&m)[NQ], float (&l)[NQ]) {
+    constexpr int NI = D / 32, NDB = D / 16, TILE = 32 * D, RPI = 512 / D, NL = 32 / RPI, CPR = D / 8;
+    const int lane = threadIdx.x & 63, n = lane & 15, g4 = lane >> 4;
+    half_t* const K0 = reinterpret_cast<half_t*>(lds);
+    half_t* const K1 = K0 + TILE;
+    half_t* const V0 = K1 + TILE;
+    half_t* const V1 = V0 + TILE;
+    // staging: load i covers the rows RPI i + lane / CPR; swizzles repeat every other (or second other) load
+    const int sr = lane / CPR, sc = lane % CPR;
+    int k_off[2], v_off[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        k_off[i] = sr * kpitch * 2 + ((sc ^ kn_swz<D>(sr + 8 * i)) << 4);
+        v_off[i] = sr * vpitch * 2 + ((sc ^ vn_swz<D>(sr + RPI * i)) << 4);
+    }
+    int kr[NI], vr[2];
+#pragma unroll
+    for (int i = 0; i < NI; ++i) kr[i] = n * D + (((4 * i + g4) ^ kn_swz<D>(n)) << 3);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int key = 16 * i + 4 * g4 + (n >> 2);
+        vr[i] = key * D + ((vn_swz<D>(key) ^ ((n & 3) >> 1)) << 3) + 4 * (n & 1);
+    }
+    const float4_t zero = {0.f, 0.f, 0.f, 0.f};
+
+    auto ahead = [&](int t, half_t* Kt, half_t* Vt) __attribute__((always_inline)) {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // everything of the stage that is overwritten has been read
+        const int there = t < t1 ? keys.n(t) : 0;
+        const half_t* const kp = t < t1 ? keys.k(t) : keys.kp;
+        const half_t* const vp = t < t1 ? keys.v(t) : keys.vp;
+        const __amdgpu_buffer_rsrc_t ks = __builtin_amdgcn_make_buffer_rsrc((void*)kp, 0, there ? ((there - 1) * kpitch + D) * 2 : 0, 0x00020000);
+        const __amdgpu_buffer_rsrc_t vs = __builtin_amdgcn_make_buffer_rsrc((void*)vp, 0, there ? ((there - 1) * vpitch + D) * 2 : 0, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < NL; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ks, (__attribute__((address_space(3))) void*)(Kt + i * 512), 16, k_off[(i * RPI >> 3) & 1], i * RPI * kpitch * 2, 0, 0);
+#pragma unroll
+        for (int i = 0; i < NL; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(vs, (__attribute__((address_space(3))) void*)(Vt + i * 512), 16, v_off[D == 128 ? i & 1 : 0], i * RPI * vpitch * 2, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto arrived = [&] {       // the tile before the one that was requested last
+        if constexpr (D == 128) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+    };
+    auto step = [&](auto mask_tag, int t, const half_t* Kt, const half_t* Vt) __attribute__((always_inline)) {
+        constexpr bool MASK = decltype(mask_tag)::value;
+        half8_t kw[2][NI], vw[NDB];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int i = 0; i < NI; ++i) kw[kb][i] = *reinterpret_cast<const half8_t*>(Kt + kb * 16 * D + kr[i]);
+#pragma unroll
+        for (int i = 0; i < NDB; ++i) {
+            const half4_t x = lds_read_tr16(Vt + (vr[0] ^ (i << 4))), y = lds_read_tr16(Vt + (vr[1] ^ (i << 4)));
+            vw[i] = half8_t{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        float4_t s[2][NQ];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int i = 0; i < NI; ++i)
+#pragma unroll
+                for (int qb = 0; qb < NQ; ++qb) s[kb][qb] = mfma16(kw[kb][i], qB[qb][i], i == 0 ? zero : s[kb][qb]);
+        if constexpr (MASK) {
+            const int key0 = keys.at(t);
+#pragma unroll
+            for (int qb = 0; qb < NQ; ++qb) {
+                const int lim = last[qb] - key0 - 4 * g4;
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[kb][qb][e] = 16 * kb + e <= lim ? s[kb][qb][e] : -INFINITY;
+            }
+        }
+        float tm[NQ];
+        bool due = false;
+#pragma unroll
+        for (int qb = 0; qb < NQ; ++qb) {
+            const float4_t &u = s[0][qb], &v = s[1][qb];
+            tm[qb] = max3(max3(u[0], u[1], u[2]), max3(u[3], v[0], v[1]), fmaxf(v[2], v[3])) * c;
+            due = due || tm[qb] > m[qb] + 8.f;
+        }
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(due) != 0, 0)) {       // lazily: p stays below 2^8
+#pragma unroll
+            for (int qb = 0; qb < NQ; ++qb) {
+                const float up = fmaxf(m[qb], quad_max(tm[qb])), alpha = up == -INFINITY ? 1.f : fast_exp2(m[qb] - up);
+                m[qb] = up;
+                l[qb] *= alpha;
+#pragma unroll
+                for (int i = 0; i < NDB; ++i) o[i][qb] = o[i][qb] * alpha;
+            }
+        }
+        // (p enters the product with V as two fp16 numbers, what the first leaves over being the second: rounded once its error is 2^-12 of each key's part, as much as the output's own rounding)
+        half8_t p[NQ], rest[NQ];
+#pragma unroll
+        for (int qb = 0; qb < NQ; ++qb) {
+            const float d = m[qb] == -INFINITY ? 0.f : -m[qb];
+            float sum[2];
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[e] = fast_exp2(__builtin_fmaf(s[kb][qb][e], c, d));
+                    p[qb][4 * kb + e] = (half_t)x[e];
+                    rest[qb][4 * kb + e] = (half_t)(x[e] - (float)p[qb][4 * kb + e]);
+                }
+                sum[kb] = (x[0] + x[1]) + (x[2] + x[3]);
+            }
+            l[qb] += sum[0] + sum[1];
+        }
+        // An infinity or NaN of a key that not all rows see: a product would hand it to the rows that do not (0 * inf).  It is taken out, and the rows that see it get it by itself.
+        if constexpr (MASK) {
+            bool bad = false;
+#pragma unroll
+            for (int i = 0; i < NDB; ++i) bad = bad || odd_values(vw[i]);
+            if (__builtin_expect(__builtin_amdgcn_ballot_w64(bad) != 0, 0)) {
+                const int key0 = keys.at(t);
+#pragma unroll 1
+                for (int kind = 0; kind < 3; ++kind)
+#pragma unroll
+                    for (int qb = 0; qb < NQ; ++qb) {
+                        const int lim = last[qb] - key0 - 4 * g4;
+                        half8_t see;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) see[e] = 16 * (e >> 2) + (e & 3) <= lim ? (half_t)1.f : (half_t)0.f;
+#pragma unroll
+                        for (int i = 0; i < NDB; ++i) {
+                            const float4_t hit = mfma16(odd_kind(vw[i], kind), see, zero);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[i][qb][e] += hit[e] > 0.f ? (kind == 0 ? INFINITY : kind == 1 ? -INFINITY : NAN) : 0.f;
+                        }
+                    }
+#pragma unroll
+                for (int i = 0; i < NDB; ++i) vw[i] = finite_only(vw[i]);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NDB; ++i)
+#pragma unroll
+            for (int qb = 0; qb < NQ; ++qb) {
+                o[i][qb] = mfma16(vw[i], p[qb], o[i][qb]);
+                o[i][qb] = mfma16(vw[i], rest[qb], o[i][qb]);
+            }
+    };
+    const std::false_type whole{};
+    const std::true_type partly{};
+    if (t0 >= t1) return;
+    ahead(t0, K0, V0);
+    int t = t0;
+    for (; t + 2 <= t_mask; t += 2) {
+        ahead(t + 1, K1, V1);
+        arrived();
+        step(whole, t, K0, V0);
+        ahead(t + 2, K0, V0);
+        arrived();
+        step(whole, t + 1, K1, V1);
+    }
+    for (; t < t1; t += 2) {
+        ahead(t + 1, K1, V1);
+        arrived();
+        step(partly, t, K0, V0);
+        ahead(t + 2, K0, V0);
+        arrived();
+        if (t + 1 < t1) step(partly, t + 1, K1, V1);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+// The results of a row tile's four waves, joined and delivered: row i of the tile by put(i, first dimension, O, m, l, whether this is the row's first piece).
+struct NarrowStats { float m[4][32], l[4][32], m_all[32], l_all[32]; };
+template <int D, int NQ, class Put>
+__device__ __forceinline__ void narrow_join(char* lds, NarrowStats& st, float4_t (&o)[D / 16][NQ], float (&m)[NQ], float (&l)[NQ], Put put) {
+    constexpr int NDB = D / 16, RT = 16 * NQ;
+    const int lane = threadIdx.x & 63, n = lane & 15, g4 = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+    for (int qb = 0; qb < NQ; ++qb) {
+        l[qb] = quad_sum(l[qb]);
+        if (g4 == 0) { st.m[wave][16 * qb + n] = m[qb]; st.l[wave][16 * qb + n] = l[qb]; }
+    }
+    __syncthreads();
+    // (a wave's stage holds its RT rows of D floats; the 16-byte pieces of a row are swizzled by the row)
+    constexpr int AREA = 4 * 32 * D * 2;
+    float4_t* const mem = reinterpret_cast<float4_t*>(lds + wave * AREA);
+#pragma unroll
+    for (int qb = 0; qb < NQ; ++qb) {
+        const int r = 16 * qb + n;
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, st.m[i][r]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum = __builtin_fmaf(st.l[i][r], st.m[i][r] == -INFINITY ? 0.f : fast_exp2(st.m[i][r] - top), sum);      // (a sum of NaN stays)
+        const float mine = m[qb] == -INFINITY ? 0.f : fast_exp2(m[qb] - top);
+#pragma unroll
+        for (int i = 0; i < NDB; ++i) mem[r * (D / 4) + ((4 * i + g4) ^ n)] = o[i][qb] * mine;
+        if (wave == 0 && g4 == 0) { st.m_all[r] = top; st.l_all[r] = sum; }
+    }
+    __syncthreads();
+    constexpr int TPR = 256 / RT, NP = D / 4 / TPR;                // threads a row, 16-byte pieces a thread
+    const int row = threadIdx.x / TPR, sub = threadIdx.x % TPR;
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+        const int piece = sub + i * TPR;
+        float4_t x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x = x + reinterpret_cast<const float4_t*>(lds + k * AREA)[row * (D / 4) + (piece ^ (row & 15))];
+        put(row, 4 * piece, x, st.m_all[row], st.l_all[row], piece == 0);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ wide
+// A workgroup's tiles t0 <= t < t1 of 64 keys for 128 rows, of which this wave has 32 (none: idle).  keys as above; .lim(t, last): up to which key of the tile a row sees.
+template <int D, class Keys>
+__device__ __forceinline__ void wide_walk(const Keys& keys, int t0, int t1, int t_mask, bool idle, float c, const half8_t (&qB)[D / 16], int last, char* lds, float16_t (&o)[D / 32], float& m, float& l) {
+    constexpr int NS = D / 16, NDB = D / 32, CPR = D / 8, RPI = 64 / CPR, NL = 64 / (4 * RPI), STAGE = 64 * D;
+    const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    half_t* const base = reinterpret_cast<half_t*>(lds);      // K of both stages, then V
+    const int sr = wave * RPI + lane / CPR, sc = ((lane % CPR) ^ swz<D>(sr)) << 4;
+    int kr[NS], vr[2];
+#pragma unroll
+    for (int i = 0; i < NS; ++i) kr[i] = n * D + (((2 * i + h) ^ swz<D>(n)) << 3);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int e = lane & 15, key = 8 * i + 4 * h + (e >> 2);
+        vr[i] = key * D + (((2 * (lane >> 4 & 1) + ((e & 3) >> 1)) ^ swz<D>(key)) << 3) + 4 * (e & 1);
+    }
+    float16_t zero;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) zero[e] = 0.f;
+
+    auto ahead = [&](int t, int stage) __attribute__((always_inline)) {
+        const int there = keys.n(t), kpitch = keys.kpitch(t), vpitch = keys.vpitch(t);
+        const __amdgpu_buffer_rsrc_t ks = __builtin_amdgcn_make_buffer_rsrc((void*)keys.k(t), 0, there ? ((there - 1) * kpitch + D) * 2 : 0, 0x00020000);
+        const __amdgpu_buffer_rsrc_t vs = __builtin_amdgcn_make_buffer_rsrc((void*)keys.v(t), 0, there ? ((there - 1) * vpitch + D) * 2 : 0, 0x00020000);
+        fetch_tile<NL, D, 4>(ks, base + stage * STAGE + wave * RPI * D, sr * kpitch * 2 + sc, 0, RPI * kpitch * 2);
+        fetch_tile<NL, D, 4>(vs, base + (2 + stage) * STAGE + wave * RPI * D, sr * vpitch * 2 + sc, 0, RPI * vpitch * 2);
+    };
+    auto step = [&](auto mask_tag, int t, int stage) __attribute__((always_inline)) {
+        constexpr bool MASK = decltype(mask_tag)::value;
+        const half_t* const Kt = base + stage * STAGE;
+        const half_t* const Vt = base + (2 + stage) * STAGE;
+        float16_t s[2];
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) s[kb] = mfma32(*reinterpret_cast<const half8_t*>(Kt + kb * 32 * D + kr[i]), qB[i], i == 0 ? zero : s[kb]);
+        if constexpr (MASK) {
+            const int lim = keys.lim(t, last) - 4 * h;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[kb][e] = 32 * kb + 8 * (e >> 2) + (e & 3) <= lim ? s[kb][e] : -INFINITY;
+        }
+        const float tm = fmaxf(max16(s[0]), max16(s[1])) * c;
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(tm > m + 8.f) != 0, 0)) {
+            const float up = fmaxf(m, half_max(tm)), alpha = up == -INFINITY ? 1.f : fast_exp2(m - up);
+            m = up;
+            l *= alpha;
+#pragma unroll
+            for (int i = 0; i < NDB; ++i) o[i] = o[i] * alpha;
+        }
+        const float d = m == -INFINITY ? 0.f : -m;
+        half8_t p[4];
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float x = fast_exp2(__builtin_fmaf(s[kb][e], c, d));
+                sum[e & 3] += x;
+                p[2 * kb + (e >> 3)][e & 7] = (half_t)x;
+            }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {           // 16 keys each
+            half8_t vw[NDB];
+#pragma unroll
+            for (int i = 0; i < NDB; ++i) {
+                const half4_t x = lds_read_tr16(Vt + u * 16 * D + (vr[0] ^ (i << 5))), y = lds_read_tr16(Vt + u * 16 * D + (vr[1] ^ (i << 5)));
+                vw[i] = half8_t{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+            }
+            if constexpr (MASK) {               // (as in the narrow form)
+                bool bad = false;
+#pragma unroll
+                for (int i = 0; i < NDB; ++i) bad = bad || odd_values(vw[i]);
+                if (__builtin_expect(__builtin_amdgcn_ballot_w64(bad) != 0, 0)) {
+                    const int lim = keys.lim(t, last) - 16 * u - 4 * h;
+                    half8_t see;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) see[e] = 8 * (e >> 2) + (e & 3) <= lim ? (half_t)1.f : (half_t)0.f;
+#pragma unroll 1
+                    for (int kind = 0; kind < 3; ++kind)
+#pragma unroll
+                        for (int i = 0; i < NDB; ++i) {
+                            const float16_t hit = mfma32(odd_kind(vw[i], kind), see, zero);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[i][e] += hit[e] > 0.f ? (kind == 0 ? INFINITY : kind == 1 ? -INFINITY : NAN) : 0.f;
+                        }
+#pragma unroll
+                    for (int i = 0; i < NDB; ++i) vw[i] = finite_only(vw[i]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < NDB; ++i) o[i] = mfma32(vw[i], p[u], o[i]);
+        }
+    };
+    if (t0 >= t1) return;
+    ahead(t0, 0);
+    for (int t = t0; t < t1; ++t) {
+        // (the wave's pieces of tile t are there; behind the barrier everyone's are, and everyone is done with tile t - 1)
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        const int stage = (t - t0) & 1;
+        if (t + 1 < t1) ahead(t + 1, stage ^ 1);
+        if (idle) continue;
+        if (t < t_mask && keys.n(t) == 64) step(std::false_type{}, t, stage);
+        else step(std::true_type{}, t, stage);
+    }
+}
+#endif
+
+// ------------------------------------------------------------------------------------------------ joining
+struct JoinArgs { Parts parts; half_t* o; const int32_t* counts; int B, Hkv, M, G, rows; int64_t os[3]; Div by_g, by_m, by_hkv; };
+hipError_t launch_cache16_join(const JoinArgs& a, int head_dim, hipStream_t s);
+
+}  // namespace trn

@@ -1,0 +1,77 @@
+// How the work of an attention over fp16 caches is laid out (cache_prefix.hip, cache_sparse.hip): plain host arithmetic.
+#pragma once
+#include <cstdint>
+
+namespace trn {
+
+inline int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
+
+// one: wide tiles of each sequence's rows walk over prefix and own keys.  Otherwise rows of all sequences walk over the prefix, in wide tiles or narrow ones, and those of each
+// sequence, in narrow ones of 16 nq rows, over its own keys.  n_rt row tiles and ns shares of their keys (_p, _o; one: _p); slots: results of a row to be joined (one: none);
+// first, second: workgroups of both parts; ml: offset of the statistics in the workspace, bytes: its size.
+struct PlanPrefix { bool one, wide; int G, R, nq, n_rt_p, ns_p, n_rt_o, ns_o, slots; int64_t first, second, ml, bytes; };
+
+inline PlanPrefix plan_prefix(int batch, int n_kv_heads, int capacity, int head_dim, int prefix, int Hq, int Sq) {
+    PlanPrefix p{};
+    p.G = Hq / n_kv_heads;
+    p.R = p.G * Sq;
+    const int64_t heads = (int64_t)batch * n_kv_heads, rows_p = (int64_t)batch * p.R;
+    p.one = p.R > 64;
+    if (p.one) {
+        p.wide = true; p.nq = 2;
+        p.n_rt_p = (p.R + 127) / 128;
+        const int64_t units = heads * p.n_rt_p, tiles = ((int64_t)prefix + 63) / 64 + (capacity + 63) / 64;
+        int64_t ns = 512 / units;
+        if (ns > tiles / 4) ns = tiles / 4;
+        p.ns_p = (int)(ns < 1 ? 1 : ns > 32 ? 32 : ns);
+        p.slots = p.ns_p;
+        p.first = units * p.ns_p;
+    } else {
+        p.wide = rows_p > 32;
+        p.nq = p.R > 16 || (!p.wide && rows_p > 16) ? 2 : 1;
+        p.n_rt_p = (int)(p.wide ? (rows_p + 127) / 128 : (rows_p + 16 * p.nq - 1) / (16 * p.nq));
+        p.n_rt_o = (p.R + 16 * p.nq - 1) / (16 * p.nq);
+        const int64_t units_p = (int64_t)n_kv_heads * p.n_rt_p, units_o = heads * p.n_rt_o;
+        // (as many keys a workgroup as make one workgroup a compute unit, two of head_dim 64; 256 at least)
+        const int64_t groups = head_dim == 128 ? 256 : 512, all = units_p * prefix + units_o * capacity;
+        int64_t each = (all + groups - 1) / groups;
+        if (each < 256) each = 256;
+        auto shares = [&](int64_t n) { const int64_t s = (n + each - 1) / each; return (int)(s > 64 ? 64 : s); };
+        p.ns_p = shares(prefix);
+        p.ns_o = shares(capacity);
+        if (p.ns_p + p.ns_o == 0) p.ns_o = 1;      // (nothing to see: zeros)
+        p.slots = p.ns_p + p.ns_o;
+        p.first = units_p * p.ns_p; p.second = units_o * p.ns_o;
+    }
+    if (p.slots > 1) {
+        p.ml = up256(heads * p.R * p.slots * head_dim * 4);
+        p.bytes = p.ml + up256(heads * p.R * p.slots * 8);
+    }
+    return p;
+}
+
+// Selected blocks: a query's scores in rows of nbp floats, `step` queries of each head at a time; row tiles of 16 nq of a KV head's query heads, ns shares of a query's keys; offsets of
+// the shares' parts behind the scores.
+struct PlanSparse { int G, nb, nq, n_rt, ns, step; int64_t nbp, o, ml, bytes; };
+
+inline PlanSparse plan_sparse(int batch, int n_kv_heads, int capacity, int head_dim, int block, int top, int Hq, int Sq) {
+    PlanSparse p{};
+    p.G = Hq / n_kv_heads;
+    p.nb = (capacity + block - 1) / block;
+    p.nbp = (p.nb + 63) / 64 * 64;
+    const int64_t heads = (int64_t)batch * n_kv_heads, row = heads * p.nbp * 4;
+    int64_t step = row ? (64 << 20) / row : Sq;
+    p.step = (int)(step < 1 ? 1 : step > Sq ? Sq : step);
+    p.nq = p.G > 16 ? 2 : 1;
+    p.n_rt = (p.G + 16 * p.nq - 1) / (16 * p.nq);
+    const int64_t units = heads * Sq * p.n_rt, groups = head_dim == 128 ? 256 : 512, tiles = (int64_t)(top < p.nb ? top : p.nb) * (block / 32);
+    int64_t ns = units ? groups / units : 1;
+    if (ns > tiles / 8) ns = tiles / 8;
+    p.ns = (int)(ns < 1 ? 1 : ns > 32 ? 32 : ns);
+    p.o = up256(row * p.step);
+    p.ml = p.o + (p.ns > 1 ? up256(heads * Sq * p.G * p.ns * head_dim * 4) : 0);
+    p.bytes = p.ml + (p.ns > 1 ? up256(heads * Sq * p.G * p.ns * 8) : 0);
+    return p;
+}
+
+}  // namespace trn

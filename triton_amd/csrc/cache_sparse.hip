@@ -1,0 +1,374 @@
+// Attention over those blocks of a long cache that a cheap score selects for each query: bounds of the blocks' keys by channel, a score from them, the selection,
+// and the attention over what is selected.
+//
+// A key k within lo <= k <= hi scores q . k <= sum_d max(q_d lo_d, q_d hi_d): of a block of 64 keys that reads 2 rows in the place of 64.  The sum is over products of two fp16 numbers, exact in 32
+// bits, added in 64, so that the order of additions does not show in the 32 bits that are compared (but where a sum lies on the border of two of them) and the selection is the definition's.
+#include "cache16_attn.h"
+#include "cache16_rules.h"
+
+namespace trn {
+
+// ------------------------------------------------------------------------------------------------ bounds
+struct BoundsArgs { const half_t* k; half_t* bounds; const int32_t *lengths, *counts; int B, Hkv, M, cap, block, nb, per; int64_t ks[3]; Div by_per, by_hkv; };
+
+// A workgroup has every per-th touched block of a head: all keys that it holds are read once.
+template <int D>
+__global__ __launch_bounds__(256) void cache_bounds_kernel(const BoundsArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr int LPR = D / 8, RPP = 256 / LPR, NP = 128 / RPP;
+    __shared__ float lo_all[4][D], hi_all[4][D];
+    const int bh = a.by_per.of(blockIdx.x), nth = blockIdx.x - bh * a.per, b = a.by_hkv.of(bh), h = bh - b * a.Hkv;
+    const int L = length_of(a.lengths, b, a.cap), C = min(count_of(a.counts, b, a.M), L);
+    if (C == 0) return;
+    const int sub = threadIdx.x % LPR, r0 = threadIdx.x / LPR, wave = threadIdx.x >> 6, t = threadIdx.x;
+    const half_t* const kh = a.k + b * a.ks[0] + h * a.ks[1] + sub * 8;
+    for (int blk = (L - C) / a.block + nth; blk * a.block < L; blk += a.per) {
+        const int base = blk * a.block, rows = min(a.block, L - base);
+        half8_t x[NP];
+#pragma unroll
+        for (int p = 0; p < NP; ++p) x[p] = *reinterpret_cast<const half8_t*>(kh + (int64_t)(base + min(p * RPP + r0, rows - 1)) * a.ks[2]);      // (a row twice changes nothing)
+        float lo[8], hi[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { lo[e] = INFINITY; hi[e] = -INFINITY; }
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { lo[e] = fminf(lo[e], (float)x[p][e]); hi[e] = fmaxf(hi[e], (float)x[p][e]); }
+#pragma unroll
+        for (int d = LPR; d < 64; d *= 2)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { lo[e] = fminf(lo[e], __shfl_xor(lo[e], d, 64)); hi[e] = fmaxf(hi[e], __shfl_xor(hi[e], d, 64)); }
+        if ((t & 63) < LPR) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { lo_all[wave][sub * 8 + e] = lo[e]; hi_all[wave][sub * 8 + e] = hi[e]; }
+        }
+        __syncthreads();
+        if (t < 2 * D) {
+            const float (*all)[D] = t < D ? lo_all : hi_all;
+            const int d = t < D ? t : t - D;
+            const float w = all[0][d], x1 = all[1][d], y = all[2][d], z = all[3][d];
+            a.bounds[((int64_t)bh * a.nb + blk) * 2 * D + t] = (half_t)(t < D ? fminf(fminf(w, x1), fminf(y, z)) : fmaxf(fmaxf(w, x1), fmaxf(y, z)));
+        }
+        __syncthreads();
+    }
+#endif
+}
+
+// ------------------------------------------------------------------------------------------------ scores
+struct SelectArgs {
+    const half_t *q, *bounds; const int32_t *lengths, *counts;
+    float* scores; int32_t* selected;
+    int B, Hkv, M, cap, G, block_shift, nb, top, sink, recent, i0, n, steps;      // queries i0 .. i0 + n
+    int64_t nbp, qs[3];
+    Div by_hkv, by_n;
+};
+
+#if defined(__HIP_DEVICE_COMPILE__)
+template <int CTRL> __device__ __forceinline__ double moved64(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xf, 0xf, true), hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xf, 0xf, true);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// Scores as whole numbers of the same order; NaN is zero, the least.
+__device__ __forceinline__ uint32_t ordered(float x) {
+    const uint32_t u = __float_as_uint(x);
+    return x != x ? 0u : u ^ (u >> 31 ? 0xffffffffu : 0x80000000u);
+}
+#endif
+
+// D / 8 lanes have a block, eight channels each; a wave 512 / D blocks at a time.
+template <int D>
+__global__ __launch_bounds__(256) void cache_scores_kernel(const SelectArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr int LPR = D / 8, PER = 64 / LPR;
+    const int lane = threadIdx.x & 63, sub = lane % LPR, wave = threadIdx.x >> 6;
+    const int bh = blockIdx.z, b = a.by_hkv.of(bh), kvh = bh - b * a.Hkv, i = a.i0 + blockIdx.y;
+    const int L = length_of(a.lengths, b, a.cap), C = count_of(a.counts, b, a.M), last = L - C + i, n = last < 0 ? 0 : (last >> a.block_shift) + 1;
+    // (no row of bounds is needed where all blocks are taken, or for those that are taken anyway)
+    if (i >= C || n <= a.top) return;
+    const half_t* const qp = a.q + b * a.qs[0] + (int64_t)kvh * a.G * a.qs[1] + i * a.qs[2] + sub * 8;
+    float* const to = a.scores + ((int64_t)bh * a.n + blockIdx.y) * a.nbp;
+    for (int s = 0; s < a.steps; ++s) {
+        const int blk = ((blockIdx.x * a.steps + s) * 4 + wave) * PER + lane / LPR;
+        if (((blockIdx.x * a.steps + s) * 4 + wave) * PER >= n) return;
+        const half_t* const bp = a.bounds + ((int64_t)bh * a.nb + min(blk, n - 1)) * 2 * D + sub * 8;
+        const half8_t lo8 = *reinterpret_cast<const half8_t*>(bp), hi8 = *reinterpret_cast<const half8_t*>(bp + D);
+        float lo[8], hi[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { lo[e] = (float)lo8[e]; hi[e] = (float)hi8[e]; }
+        double best = -INFINITY;
+        for (int g = 0; g < a.G; ++g) {
+            const half8_t q8 = *reinterpret_cast<const half8_t*>(qp + g * a.qs[1]);
+            double x = 0., y = 0.;
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                const float q0 = (float)q8[e], q1 = (float)q8[e + 1];
+                x += (double)fmaxf(q0 * lo[e], q0 * hi[e]);
+                y += (double)fmaxf(q1 * lo[e + 1], q1 * hi[e + 1]);
+            }
+            x += y;
+            x += moved64<0xb1>(x);
+            x += moved64<0x4e>(x);
+            x += moved64<0x141>(x);
+            if constexpr (D == 128) x += moved64<0x140>(x);
+            best = fmax(best, x);
+        }
+        if (sub == 0 && blk < n) to[blk] = (float)best;
+    }
+#endif
+}
+
+// ------------------------------------------------------------------------------------------------ selection
+// A workgroup has one query of one KV head.  The score of the last one that is taken is found digit by digit (eight bits of the ordered scores, a count of each of their 256
+// values), then one walk over the blocks takes what is larger, and of its equals the first ones, in order.
+__global__ __launch_bounds__(256) void cache_select_kernel(const SelectArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __shared__ int count[256], waves[4], waves2[4], digit, left;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int bh = a.by_n.of(blockIdx.x), j = blockIdx.x - bh * a.n, i = a.i0 + j, b = a.by_hkv.of(bh);
+    const int L = length_of(a.lengths, b, a.cap), C = count_of(a.counts, b, a.M), last = L - C + i, n = last < 0 ? 0 : (last >> a.block_shift) + 1;
+    if (i >= C) return;
+    int32_t* const to = a.selected + ((int64_t)bh * a.M + i) * a.top;
+    if (n <= a.top) {
+        for (int x = tid; x < a.top; x += 256) to[x] = x < n ? x : -1;
+        return;
+    }
+    const float* const from = a.scores + ((int64_t)bh * a.n + j) * a.nbp;
+    const int lo = a.sink, hi = n - a.recent;                     // what is chosen from (top > their number: not empty)
+    int want = a.top - a.sink - a.recent;
+    uint32_t known = 0;
+    if (want > 0) {
+        for (int shift = 24; shift >= 0; shift -= 8) {
+            count[tid] = 0;
+            __syncthreads();
+            for (int x = lo + tid; x < hi; x += 256) {
+                const uint32_t u = ordered(from[x]);
+                if (shift == 24 || (u ^ known) >> (shift + 8) == 0) atomicAdd(&count[u >> shift & 255], 1);
+            }
+            __syncthreads();
+            // from the largest digit down
+            const int mine = count[255 - tid];
+            int sum = mine;
+#pragma unroll
+            for (int d = 1; d < 64; d *= 2) { const int y = __shfl_up(sum, d, 64); if (lane >= d) sum += y; }
+            if (lane == 63) waves[wave] = sum;
+            __syncthreads();
+            for (int w = 0; w < wave; ++w) sum += waves[w];
+            if (sum >= want && sum - mine < want) { digit = 255 - tid; left = want - (sum - mine); }
+            __syncthreads();
+            known |= (uint32_t)digit << shift;
+            want = left;
+        }
+    }
+    // taken so far, and of the equals of `known`
+    int done = 0, equals = 0;
+    for (int x0 = 0; x0 < n; x0 += 256) {
+        const int x = x0 + tid;
+        const bool forced = x < n && (x < lo || x >= hi), open = x >= lo && x < hi && want > 0;
+        const uint32_t u = open ? ordered(from[x]) : 0;
+        const bool equal = open && u == known;
+        const uint64_t eq = __builtin_amdgcn_ballot_w64(equal), below = (1ull << lane) - 1;
+        if (lane == 0) waves[wave] = __popcll(eq);
+        __syncthreads();
+        int rank = equals + __popcll(eq & below);
+        for (int w = 0; w < wave; ++w) rank += waves[w];
+        const bool take = forced || (open && (u > known || (equal && rank < want)));
+        const uint64_t tk = __builtin_amdgcn_ballot_w64(take);
+        if (lane == 0) waves2[wave] = __popcll(tk);
+        __syncthreads();
+        int at = done + __popcll(tk & below);
+        for (int w = 0; w < wave; ++w) at += waves2[w];
+        if (take) to[at] = x;
+        for (int w = 0; w < 4; ++w) { equals += waves[w]; done += waves2[w]; }
+        __syncthreads();
+    }
+#endif
+}
+
+// ------------------------------------------------------------------------------------------------ attention
+struct SparseArgs {
+    const half_t *k, *v, *q; half_t* o; const int32_t *lengths, *counts, *selected;
+    int B, Hkv, M, cap, G, block_shift, top, n_rt, ns;
+    int64_t ks[3], vs[3], qs[3], os[3];
+    float c;
+    Parts parts;
+    Div by_hkv, by_b, by_ns, by_rt, by_w;
+};
+
+#if defined(__HIP_DEVICE_COMPILE__)
+// The keys of the selected blocks, tiles of 32 of each block one after the other.  A lane holds the block of its place from `from` on.
+struct Chosen {
+    const half_t *kp, *vp; const int32_t* list; int kpitch, vpitch, seen, shift, most, from, held;
+    __device__ __forceinline__ void hold(int place) { from = place; held = list[min(place + (int)(threadIdx.x & 63), most - 1)]; }
+    __device__ __forceinline__ int at(int t) {
+        const int place = t >> (shift - 5);
+        if (place < from || place - from > 63) hold(place);
+        return (__builtin_amdgcn_readlane(held, place - from) << shift) + ((t & ((1 << (shift - 5)) - 1)) << 5);
+    }
+    __device__ __forceinline__ const half_t* k(int t) { return kp + (int64_t)at(t) * kpitch; }
+    __device__ __forceinline__ const half_t* v(int t) { return vp + (int64_t)at(t) * vpitch; }
+    __device__ __forceinline__ int n(int t) { return max(0, min(32, seen - at(t))); }
+};
+#endif
+
+template <int D, int NQ>
+__global__ __launch_bounds__(256, D == 128 ? 1 : 2) void cache_sparse_attn_kernel(const SparseArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __shared__ __attribute__((aligned(1024))) char lds[kNarrowLds(D)];
+    __shared__ NarrowStats stats;
+    constexpr int RT = 16 * NQ;
+    const int lane = threadIdx.x & 63, n = lane & 15, g4 = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int x = a.by_hkv.of(blockIdx.x), kvh = blockIdx.x - x * a.Hkv, y = a.by_b.of(x), b = x - y * a.B, z = a.by_ns.of(y), share = y - z * a.ns, i = a.by_rt.of(z), rt = z - i * a.n_rt;
+    const int L = length_of(a.lengths, b, a.cap), C = count_of(a.counts, b, a.M), seen = L - C + i + 1;       // the keys that the query sees
+    if (i >= C) return;
+    const int ends = seen > 0 ? (seen - 1) >> a.block_shift : -1, most = min(a.top, ends + 1), per = 1 << (a.block_shift - 5);
+    // (the last block is the query's own: the others are there as a whole)
+    const int T = most > 0 ? (most - 1) * per + ((seen - (ends << a.block_shift) + 31) >> 5) : 0, whole = most > 0 ? (most - 1) * per + ((seen - (ends << a.block_shift)) >> 5) : 0;
+    const int w = share * 4 + wave, t0 = a.by_w.of(T * w), t1 = a.by_w.of(T * (w + 1));
+    half8_t qB[NQ][D / 32];
+    int last[NQ];
+#pragma unroll
+    for (int qb = 0; qb < NQ; ++qb) {
+        const int g = rt * RT + 16 * qb + n;
+        const bool there = g < a.G;
+        last[qb] = there ? seen - 1 : -1;
+        const half_t* const qp = a.q + b * a.qs[0] + (int64_t)(kvh * a.G + (there ? g : 0)) * a.qs[1] + i * a.qs[2];
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) {
+            const half8_t zero = {}, v = *reinterpret_cast<const half8_t*>(qp + 32 * e + 8 * g4);
+            qB[qb][e] = there ? v : zero;
+        }
+    }
+    Chosen keys{a.k + b * a.ks[0] + kvh * a.ks[1], a.v + b * a.vs[0] + kvh * a.vs[1], a.selected + (((int64_t)b * a.Hkv + kvh) * a.M + i) * a.top,
+                (int)a.ks[2], (int)a.vs[2], seen, a.block_shift, max(most, 1), 0, 0};
+    if (t0 < t1) keys.hold(t0 >> (a.block_shift - 5));
+    float4_t o[D / 16][NQ];
+    float m[NQ], l[NQ];
+#pragma unroll
+    for (int qb = 0; qb < NQ; ++qb) {
+        m[qb] = -INFINITY; l[qb] = 0.f;
+#pragma unroll
+        for (int e = 0; e < D / 16; ++e) o[e][qb] = float4_t{0.f, 0.f, 0.f, 0.f};
+    }
+    narrow_walk<D, NQ>(keys, t0, t1, min(t1, max(t0, whole)), keys.kpitch, keys.vpitch, a.c, qB, last, lds + wave * 4 * 32 * D * 2, o, m, l);
+    narrow_join<D, NQ>(lds, stats, o, m, l, [&](int r, int d0, float4_t v, float mm, float ll, bool once) __attribute__((always_inline)) {
+        const int g = rt * RT + r;
+        if (g >= a.G) return;
+        if (a.ns > 1) {
+            const int64_t at = ((((int64_t)b * a.Hkv + kvh) * a.M + i) * a.G + g) * a.ns + share;
+            *reinterpret_cast<float4_t*>(a.parts.o + at * D + d0) = v;
+            if (once) *reinterpret_cast<float2_t*>(a.parts.ml + 2 * at) = float2_t{mm, ll};
+            return;
+        }
+        const float inv = ll == 0.f ? 0.f : 1.f / ll;
+        half4_t out;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[e] = (half_t)(v[e] * inv);
+        *reinterpret_cast<half4_t*>(a.o + b * a.os[0] + (int64_t)(kvh * a.G + g) * a.os[1] + i * a.os[2] + d0) = out;
+    });
+#endif
+}
+
+inline bool block16_ok(int block) { return block == 32 || block == 64 || block == 128; }
+inline int shift_of(int block) { return block == 32 ? 5 : block == 64 ? 6 : 7; }
+
+}  // namespace trn
+
+extern "C" int trn_cache_bounds_f16(const trn_cache16* c, int32_t block, int32_t tokens, void* bounds, void* stream) {
+    using namespace trn;
+    const int st = cache16_check(c, false);
+    if (st != TRN_OK) return st;
+    if (!block16_ok(block)) return TRN_E_UNSUPPORTED;
+    if (tokens < 0) return TRN_E_SHAPE;
+    if (c->batch == 0 || c->capacity == 0 || tokens == 0) return TRN_OK;
+    if (!bounds) return TRN_E_NULL;
+    if (!aligned16(bounds)) return TRN_E_ALIGN;
+    BoundsArgs a{};
+    a.k = (const half_t*)c->k; a.bounds = (half_t*)bounds; a.lengths = c->lengths; a.counts = c->counts;
+    a.B = c->batch; a.Hkv = c->n_kv_heads; a.M = tokens; a.cap = c->capacity; a.block = block; a.nb = (c->capacity + block - 1) / block;
+    for (int i = 0; i < 3; ++i) a.ks[i] = c->k_stride[i];
+    const int64_t heads = (int64_t)c->batch * c->n_kv_heads, size = heads * a.nb * 4 * c->head_dim;
+    if (!apart(bounds, size, c->k, rows_extent(c->k, c->k_stride, c->batch, c->n_kv_heads, c->capacity, c->head_dim).span())) return TRN_E_UNSUPPORTED;
+    const int most = tokens < c->capacity ? tokens : c->capacity;
+    // (the blocks that the new tokens can touch -- the first of them may be the last of its block --, but no more workgroups than the card holds at once: the most new tokens
+    // that a call allows are rarely there)
+    const int64_t blocks = ((int64_t)most + 2 * block - 2) / block, at_once = (2048 + heads - 1) / heads;
+    a.per = (int)(blocks < at_once ? blocks : at_once);
+    if (heads * a.per > 0xffffff) return TRN_E_SHAPE;                 // (threads in 32 bits)
+    a.by_per = Div(a.per); a.by_hkv = Div(c->n_kv_heads);
+    const dim3 grid((unsigned)(heads * a.per));
+    if (c->head_dim == 128) hipLaunchKernelGGL((cache_bounds_kernel<128>), grid, dim3(256), 0, (hipStream_t)stream, a);
+    else hipLaunchKernelGGL((cache_bounds_kernel<64>), grid, dim3(256), 0, (hipStream_t)stream, a);
+    return hipGetLastError() == hipSuccess ? TRN_OK : TRN_E_LAUNCH;
+}
+
+extern "C" int64_t trn_cache_sparse_attn_workspace_bytes(const trn_cache16* c, int32_t block, int32_t top, int32_t n_q_heads, int32_t seq_q) {
+    using namespace trn;
+    if (!c || attn16_rows(c->batch, c->n_kv_heads, n_q_heads, seq_q) != TRN_OK || c->batch == 0 || seq_q == 0 || !block16_ok(block) || top < 1 || top > (1 << 16)) return 0;
+    if (c->capacity < 0 || c->capacity > (1 << 26) || (c->head_dim != 64 && c->head_dim != 128)) return 0;
+    return plan_sparse(c->batch, c->n_kv_heads, c->capacity, c->head_dim, block, top, n_q_heads, seq_q).bytes;
+}
+
+extern "C" int trn_cache_sparse_attn_f16(const trn_cache16* c, const void* bounds, int32_t block, int32_t top, int32_t sink, int32_t recent, const void* q, void* o,
+                                         int32_t* selected, int32_t n_q_heads, int32_t seq_q, const int64_t* q_stride, const int64_t* o_stride, float scale,
+                                         void* workspace, int64_t workspace_bytes, void* stream) {
+    using namespace trn;
+    int st = cache16_check(c);
+    if (st != TRN_OK) return st;
+    if (!block16_ok(block) || top > (1 << 16)) return TRN_E_UNSUPPORTED;
+    if (sink < 0 || recent < 1 || top < 1 || (int64_t)sink + recent > top) return TRN_E_SHAPE;
+    if ((st = attn16_rows(c->batch, c->n_kv_heads, n_q_heads, seq_q)) != TRN_OK) return st;
+    if (c->batch == 0 || seq_q == 0) return TRN_OK;
+    if ((st = attn16_check(c, q, o, n_q_heads, seq_q, q_stride, o_stride, scale, workspace)) != TRN_OK) return st;
+    if (!selected || (c->capacity && !bounds)) return TRN_E_NULL;
+    if ((reinterpret_cast<uintptr_t>(selected) & 3) || !aligned16(bounds)) return TRN_E_ALIGN;
+    const int64_t heads = (int64_t)c->batch * c->n_kv_heads;
+    const PlanSparse p = plan_sparse(c->batch, c->n_kv_heads, c->capacity, c->head_dim, block, top, n_q_heads, seq_q);
+    if (p.bytes && (!workspace || workspace_bytes < p.bytes)) return TRN_E_SCRATCH;
+    const int64_t groups = heads * seq_q * p.n_rt * p.ns;
+    // (workgroups of 256, and as many threads in all as 32 bits number: of every launch, before the first one)
+    const int per = 4 * 512 / c->head_dim, steps = (int64_t)p.nb * p.step * heads > (1 << 17) ? 4 : 1;
+    const int64_t chunks = (p.nb + (int64_t)per * steps - 1) / (per * steps);
+    if (groups > 0xffffff || heads * p.step > 0xffffff || heads > 65535 || heads * p.step * chunks > 0xffffff) return TRN_E_SHAPE;
+    const hipStream_t s = (hipStream_t)stream;
+    const bool d128 = c->head_dim == 128;
+    hipError_t e = hipSuccess;
+    for (int64_t i0 = 0; i0 < seq_q && e == hipSuccess; i0 += p.step) {
+        SelectArgs a{};
+        a.q = (const half_t*)q; a.bounds = (const half_t*)bounds; a.lengths = c->lengths; a.counts = c->counts; a.scores = (float*)workspace; a.selected = selected;
+        a.B = c->batch; a.Hkv = c->n_kv_heads; a.M = seq_q; a.cap = c->capacity; a.G = p.G; a.block_shift = shift_of(block); a.nb = p.nb;
+        a.top = top; a.sink = sink; a.recent = recent; a.i0 = (int)i0; a.n = (int)(seq_q - i0 < p.step ? seq_q - i0 : p.step); a.steps = steps; a.nbp = p.nbp;
+        for (int i = 0; i < 3; ++i) a.qs[i] = q_stride[i];
+        a.by_hkv = Div(c->n_kv_heads); a.by_n = Div(a.n);
+        if (p.nb > top) {      // (a.n is at most 65535: 64 MB of at least 64 floats a query)
+            const dim3 grid((unsigned)chunks, (unsigned)a.n, (unsigned)heads);
+            if (d128) hipLaunchKernelGGL((cache_scores_kernel<128>), grid, dim3(256), 0, s, a);
+            else hipLaunchKernelGGL((cache_scores_kernel<64>), grid, dim3(256), 0, s, a);
+            if ((e = hipGetLastError()) != hipSuccess) break;
+        }
+        hipLaunchKernelGGL(cache_select_kernel, dim3((unsigned)(heads * a.n)), dim3(256), 0, s, a);
+        e = hipGetLastError();
+    }
+    if (e != hipSuccess) return TRN_E_LAUNCH;
+    SparseArgs a{};
+    a.k = (const half_t*)c->k; a.v = (const half_t*)c->v; a.q = (const half_t*)q; a.o = (half_t*)o; a.lengths = c->lengths; a.counts = c->counts; a.selected = selected;
+    a.B = c->batch; a.Hkv = c->n_kv_heads; a.M = seq_q; a.cap = c->capacity; a.G = p.G; a.block_shift = shift_of(block); a.top = top; a.n_rt = p.n_rt; a.ns = p.ns;
+    for (int i = 0; i < 3; ++i) { a.ks[i] = c->k_stride[i]; a.vs[i] = c->v_stride[i]; a.qs[i] = q_stride[i]; a.os[i] = o_stride[i]; }
+    a.c = scale * kLog2e;
+    a.parts = Parts{(float*)((char*)workspace + p.o), (float*)((char*)workspace + p.ml), p.ns};
+    a.by_hkv = Div(c->n_kv_heads); a.by_b = Div(c->batch); a.by_ns = Div(p.ns); a.by_rt = Div(p.n_rt); a.by_w = Div(4 * p.ns);
+    const dim3 grid((unsigned)groups), block3(256);
+    if (p.nq == 1) {
+        if (d128) hipLaunchKernelGGL((cache_sparse_attn_kernel<128, 1>), grid, block3, 0, s, a);
+        else hipLaunchKernelGGL((cache_sparse_attn_kernel<64, 1>), grid, block3, 0, s, a);
+    } else {
+        if (d128) hipLaunchKernelGGL((cache_sparse_attn_kernel<128, 2>), grid, block3, 0, s, a);
+        else hipLaunchKernelGGL((cache_sparse_attn_kernel<64, 2>), grid, block3, 0, s, a);
+    }
+    e = hipGetLastError();
+    if (e == hipSuccess && p.ns > 1) {
+        JoinArgs j{a.parts, a.o, a.counts, a.B, a.Hkv, a.M, a.G, (int)(heads * seq_q * p.G), {a.os[0], a.os[1], a.os[2]}, Div(p.G), Div(a.M), a.by_hkv};
+        e = launch_cache16_join(j, c->head_dim, s);
+    }
+    return e == hipSuccess ? TRN_OK : TRN_E_LAUNCH;
+}

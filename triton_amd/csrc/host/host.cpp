@@ -692,6 +692,170 @@ bool f_cache_evict(Args a, Py_ssize_t n) {
     return true;
 }
 
+// ---------------------------------------------------------------------------------------------- fp16 caches of sequences of their own lengths
+// (values: K and V; otherwise K alone)
+trn_cache16 cache16_of(const View& k, const char* kn, const View* v, const char* vn, const OptView& lengths, const OptView& counts) {
+    dev_half(k, kn);
+    NEED(k.dim == 4, "%s: expected [batch, heads, capacity, head_dim], got %s", kn, k.shape().c_str());
+    NEED(k.s[0] <= INT32_MAX && k.s[1] <= INT32_MAX && k.s[2] <= INT32_MAX && k.s[3] <= INT32_MAX, "%s %s: too large", kn, k.shape().c_str());
+    trn_cache16 c{};
+    c.k = k.p;
+    c.lengths = batch_ints(lengths, "lengths", k.s[0], k); c.counts = batch_ints(counts, "counts", k.s[0], k);
+    c.batch = (int32_t)k.s[0]; c.n_kv_heads = (int32_t)k.s[1]; c.capacity = (int32_t)k.s[2]; c.head_dim = (int32_t)k.s[3];
+    for (int i = 0; i < 3; ++i) c.k_stride[i] = k.st[i];
+    if (v) {
+        dev_half(*v, vn); on(*v, vn, k);
+        dims4(*v, vn, k.s[0], k.s[1], k.s[2], k.s[3]);
+        c.v = v->p;
+        for (int i = 0; i < 3; ++i) c.v_stride[i] = v->st[i];
+    }
+    return c;
+}
+
+bool f_cache_rope_append(Args a, Py_ssize_t n) {
+    // norm, eps, interleaved, sections | None, K, K_cache, Q, Q_out, V, V_cache, counts | None, gamma_k | None, gamma_q | None, inv_freq | None, lengths | None, positions | None
+    count(n, 16, "cache_rope_append");
+    const View k = arg(a[4], "k"), kc = arg(a[5], "k_cache"), q = arg(a[6], "q"), qo = arg(a[7], "q_out"), v = arg(a[8], "v"), vc = arg(a[9], "v_cache");
+    const trn_cache16 c = cache16_of(kc, "k_cache", &vc, "v_cache", opt(a[14], "lengths"), opt(a[10], "counts"));
+    for (const View* t : {&k, &q, &qo, &v}) { const char* nm = t == &k ? "k" : t == &q ? "q" : t == &qo ? "q_out" : "v"; dev_half(*t, nm); on(*t, nm, kc); }
+    NEED(q.dim == 4 && q.s[0] == kc.s[0] && q.s[3] == kc.s[3] && q.s[1] > 0 && q.s[1] <= INT32_MAX && q.s[2] <= INT32_MAX, "q %s does not match k_cache %s", q.shape().c_str(), kc.shape().c_str());
+    NEED(same_shape(qo, q), "q_out %s must equal q %s", qo.shape().c_str(), q.shape().c_str());
+    dims4(k, "k", kc.s[0], kc.s[1], q.s[2], kc.s[3]);
+    dims4(v, "v", kc.s[0], kc.s[1], q.s[2], kc.s[3]);
+    trn_rope r{};
+    r.norm = flag(a[0]); r.eps = (float)num(a[1]); r.interleaved = flag(a[2]);
+    const OptView gk = opt(a[11], "gamma_k"), gq = opt(a[12], "gamma_q"), inv = opt(a[13], "inv_freq"), pos = opt(a[15], "positions");
+    NEED(r.norm || (!gk.given && !gq.given), "gamma_q, gamma_k given without norm");
+    for (const OptView* t : {&gk, &gq}) {
+        if (!t->given) continue;
+        const char* nm = t == &gk ? "gamma_k" : "gamma_q";
+        dev_half(t->v, nm); on(t->v, nm, kc);
+        NEED(t->v.dim == 1 && t->v.s[0] == kc.s[3], "%s %s: expected (%lld,)", nm, t->v.shape().c_str(), (long long)kc.s[3]);
+    }
+    r.gamma_k = gk.p(); r.gamma_q = gq.p();
+    if (inv.given) {
+        on(inv.v, "inv_freq", kc);
+        NEED(inv.v.dt == c10::ScalarType::Double && inv.v.dim == 1 && inv.v.contiguous(), "inv_freq: expected contiguous float64 (pairs,)");
+        NEED(inv.v.s[0] % 4 == 0 && 2 * inv.v.s[0] <= kc.s[3], "inv_freq %s: expected a multiple of 4 pairs, at most head_dim / 2", inv.v.shape().c_str());
+        r.inv_freq = (const double*)inv.v.p; r.pairs = (int32_t)inv.v.s[0];
+    }
+    r.axes = 1; r.sections[0] = r.pairs;
+    if (a[3] != Py_None) {
+        PyObject* const seq = PySequence_Fast(a[3], "sections: expected a sequence of whole numbers");
+        if (!seq) throw PyErrSet{};
+        const struct Hold { PyObject* o; ~Hold() { Py_DECREF(o); } } hold{seq};
+        const Py_ssize_t axes = PySequence_Fast_GET_SIZE(seq);
+        NEED(axes >= 1 && axes <= 4, "sections: expected one to four axes, got %zd", axes);
+        int64_t all = 0;
+        for (Py_ssize_t i = 0; i < axes; ++i) {
+            r.sections[i] = whole(PySequence_Fast_GET_ITEM(seq, i), "sections");
+            NEED(r.sections[i] >= 0, "sections: expected no negative number");
+            all += r.sections[i];
+        }
+        NEED(all == r.pairs, "sections: expected %d pairs in all, got %lld", r.pairs, (long long)all);
+        r.axes = (int32_t)axes;
+    }
+    NEED(r.axes == 1 || pos.given, "several sections need positions");
+    if (pos.given) {
+        on(pos.v, "positions", kc);
+        NEED(pos.v.dt == c10::ScalarType::Int && pos.v.dim == 3 && pos.v.s[0] == r.axes && pos.v.s[1] == q.s[0] && pos.v.s[2] == q.s[2] && packed(pos.v),
+             "positions %s: expected contiguous int32 (%d, %lld, %lld)", pos.v.shape().c_str(), r.axes, (long long)q.s[0], (long long)q.s[2]);
+        r.positions = (const int32_t*)pos.v.p;
+    }
+    const OnDevice here(kc.dev);
+    CALL(trn_cache_rope_append_f16, &c, &r, q.p, qo.p, k.p, v.p, (int32_t)q.s[1], (int32_t)q.s[2], q.st, qo.st, k.st, v.st, stream_of(kc));
+    return true;
+}
+
+// The queries and outputs of an attention over the cache k.
+void queries_of(const View& q, const View& o, const View& k) {
+    dev_half(q, "q"); dev_half(o, "o");
+    on(q, "q", k); on(o, "o", k);
+    NEED(q.dim == 4 && q.s[0] == k.s[0] && q.s[3] == k.s[3] && q.s[1] > 0 && k.s[1] > 0 && q.s[1] % k.s[1] == 0 && q.s[1] <= INT32_MAX && q.s[2] <= INT32_MAX,
+         "q %s does not match k %s", q.shape().c_str(), k.shape().c_str());
+    NEED(same_shape(o, q), "o %s must equal q %s", o.shape().c_str(), q.shape().c_str());
+}
+// A workspace of the module's (under `name`), or the caller's.
+struct Scratch { at::Tensor kept; void* p = nullptr; int64_t bytes = 0; };
+Scratch scratch_of(PyObject* o, const char* name, int64_t need, const View& first) {
+    Scratch s;
+    if (Py_TYPE(o) == workspaces_type()) {
+        if (need) {
+            s.kept = workspace(ws_arg(o), name, {kept_bytes(need)}, c10::ScalarType::Byte, first.dev);
+            s.p = s.kept.data_ptr(); s.bytes = kept_bytes(need);
+        }
+    } else if (const OptView given = opt(o, "workspace"); given.given) {
+        on(given.v, "workspace", first);
+        NEED(given.v.contiguous() && given.v.dt == c10::ScalarType::Byte, "workspace: expected a contiguous uint8 GPU tensor");
+        s.p = given.v.p; s.bytes = given.v.numel();
+    }
+    return s;
+}
+
+bool f_cache_prefix_attention(Args a, Py_ssize_t n) {
+    // workspaces | workspace | None, scale | None, causal, K, K_prefix, O, Q, V, V_prefix, counts | None, lengths | None
+    count(n, 11, "cache_prefix_attention");
+    const View k = arg(a[3], "k"), kp = arg(a[4], "k_prefix"), o = arg(a[5], "o"), q = arg(a[6], "q"), v = arg(a[7], "v"), vp = arg(a[8], "v_prefix");
+    const trn_cache16 c = cache16_of(k, "k", &v, "v", opt(a[10], "lengths"), opt(a[9], "counts"));
+    queries_of(q, o, k);
+    trn_prefix p{};
+    for (const View* t : {&kp, &vp}) {
+        const char* nm = t == &kp ? "k_prefix" : "v_prefix";
+        dev_half(*t, nm); on(*t, nm, k);
+        NEED(t->dim == 3 && t->s[0] == k.s[1] && t->s[1] == kp.s[1] && t->s[1] <= INT32_MAX && t->s[2] == k.s[3], "%s %s: expected (%lld, %lld, %lld)", nm, t->shape().c_str(),
+             (long long)k.s[1], (long long)kp.s[1], (long long)k.s[3]);
+    }
+    p.k = kp.p; p.v = vp.p; p.keys = (int32_t)kp.s[1];
+    for (int i = 0; i < 2; ++i) { p.k_stride[i] = kp.st[i]; p.v_stride[i] = vp.st[i]; }
+    const Scratch s = scratch_of(a[0], "prefix", trn_cache_prefix_attn_workspace_bytes(&c, p.keys, (int32_t)q.s[1], (int32_t)q.s[2]), k);
+    const OnDevice here(k.dev);
+    CALL(trn_cache_prefix_attn_f16, &c, &p, q.p, o.p, (int32_t)q.s[1], (int32_t)q.s[2], q.st, o.st, (float)scale_of(a[1], q.s[3]), flag(a[2]) ? 1 : 0, s.p, s.bytes, stream_of(k));
+    return true;
+}
+
+// Bounds [batch, heads, blocks, 2, head_dim] of the cache k.
+void* bounds_of(PyObject* x, const View& k, int block) {
+    NEED(block == 32 || block == 64 || block == 128, "block: expected 32, 64 or 128, got %d", block);
+    NEED(THPVariable_Check(x), "bounds: expected a tensor");
+    const at::Tensor& t = THPVariable_Unpack(x);
+    NEED(t.is_cuda() && t.get_device() == k.dev, "bounds: expected a tensor on the device of the others");
+    NEED(t.scalar_type() == c10::ScalarType::Half && t.dim() == 5 && t.size(0) == k.s[0] && t.size(1) == k.s[1] && t.size(2) == (k.s[2] + block - 1) / block && t.size(3) == 2 &&
+             t.size(4) == k.s[3] && t.is_contiguous(),
+         "bounds: expected contiguous float16 (%lld, %lld, %lld, 2, %lld)", (long long)k.s[0], (long long)k.s[1], (long long)((k.s[2] + block - 1) / block), (long long)k.s[3]);
+    return t.data_ptr();
+}
+bool f_cache_bounds(Args a, Py_ssize_t n) {               // block, tokens, K, bounds, counts | None, lengths | None
+    count(n, 6, "cache_bounds");
+    const View k = arg(a[2], "k");
+    const int block = whole(a[0], "block"), tokens = a[1] == Py_None ? (int)std::min<int64_t>(k.dim == 4 ? k.s[2] : 0, INT32_MAX) : whole(a[1], "tokens");
+    NEED(tokens >= 0, "tokens: expected no negative number");
+    const trn_cache16 c = cache16_of(k, "k", nullptr, "", opt(a[5], "lengths"), opt(a[4], "counts"));
+    void* const bounds = bounds_of(a[3], k, block);
+    const OnDevice here(k.dev);
+    CALL(trn_cache_bounds_f16, &c, block, tokens, bounds, stream_of(k));
+    return true;
+}
+
+bool f_cache_sparse_attention(Args a, Py_ssize_t n) {
+    // workspaces | workspace | None, scale | None, block, top, sink, recent, K, O, Q, V, bounds, counts | None, lengths | None, selected
+    count(n, 14, "cache_sparse_attention");
+    const View k = arg(a[6], "k"), o = arg(a[7], "o"), q = arg(a[8], "q"), v = arg(a[9], "v"), sel = arg(a[13], "selected");
+    const int block = whole(a[2], "block"), top = whole(a[3], "top"), sink = whole(a[4], "sink"), recent = whole(a[5], "recent");
+    NEED(top >= 1 && top <= 65536 && sink >= 0 && recent >= 1 && (int64_t)sink + recent <= top, "top %d, sink %d, recent %d: expected sink >= 0, recent >= 1, sink + recent <= top <= 65536",
+         top, sink, recent);
+    const trn_cache16 c = cache16_of(k, "k", &v, "v", opt(a[12], "lengths"), opt(a[11], "counts"));
+    queries_of(q, o, k);
+    const void* const bounds = bounds_of(a[10], k, block);
+    on(sel, "selected", k);
+    NEED(sel.dt == c10::ScalarType::Int && sel.dim == 4 && sel.s[0] == q.s[0] && sel.s[1] == k.s[1] && sel.s[2] == q.s[2] && sel.s[3] == top && packed(sel),
+         "selected %s: expected contiguous int32 (%lld, %lld, %lld, %d)", sel.shape().c_str(), (long long)q.s[0], (long long)k.s[1], (long long)q.s[2], top);
+    const Scratch s = scratch_of(a[0], "sparse", trn_cache_sparse_attn_workspace_bytes(&c, block, top, (int32_t)q.s[1], (int32_t)q.s[2]), k);
+    const OnDevice here(k.dev);
+    CALL(trn_cache_sparse_attn_f16, &c, bounds, block, top, sink, recent, q.p, o.p, (int32_t*)sel.p, (int32_t)q.s[1], (int32_t)q.s[2], q.st, o.st, (float)scale_of(a[1], q.s[3]),
+         s.p, s.bytes, stream_of(k));
+    return true;
+}
+
 // ---------------------------------------------------------------------------------------------- Python glue
 PyObject* raise_trn(const char* fn, int status) {
     if (!g_trn_error) { PyErr_Format(PyExc_RuntimeError, "%s failed: %s (%d)", fn, trn_status_name(status), status); return nullptr; }
@@ -759,7 +923,8 @@ PyObject* set_error_class(PyObject*, PyObject* cls) {
 #define OPERATOR(name) {#name, (PyCFunction)(void (*)(void))entry<f_##name, true>, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {OPERATOR(rmsnorm), OPERATOR(attention), OPERATOR(prenorm_qkv), FN(rmsnorm_forward), FN(attention_forward),
                          FN(qknorm_forward), FN(key_scores_forward), FN(prenorm_forward), FN(decode_forward), FN(lora_forward), FN(gmlp_forward),
-                         OPERATOR(cache8_append), OPERATOR(cache8_attention), OPERATOR(cache_evict),
+                         OPERATOR(cache8_append), OPERATOR(cache8_attention), OPERATOR(cache_evict), OPERATOR(cache_rope_append), OPERATOR(cache_prefix_attention),
+                         OPERATOR(cache_bounds), OPERATOR(cache_sparse_attention),
                          {"set_error_class", set_error_class, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "host side of the modules' forward", -1, methods};
 

@@ -640,8 +640,63 @@ class Cache8StepWeights(Cache8Step):
     TENSOR_PARAMS = Cache8Step.TENSOR_PARAMS + ["weights"]
 
 
+# ============================================================================ fp16 caches of sequences of their own lengths
+class CacheRope(FusedModule):
+    """New tokens into an fp16 cache, rotated by their positions and, norm=True, RMS-normalised by head first (`ops.cache_rope_append`).  Q_out may be Q; gammas, inv_freq,
+    positions, lengths and counts may be None.  sections: pairs of each axis (None: one axis).  One launch."""
+    TENSOR_PARAMS = ["K", "K_cache", "Q", "Q_out", "V", "V_cache", "counts", "gamma_k", "gamma_q", "inv_freq", "lengths", "positions"]
+
+    def __init__(self, norm: bool = False, eps: float = 1e-6, interleaved: bool = False, sections=None):
+        super().__init__()
+        self.norm, self.eps, self.interleaved, self.sections = norm, eps, interleaved, None if sections is None else list(sections)
+
+    def _native(self, host, ws, K, K_cache, Q, Q_out, V, V_cache, counts, gamma_k, gamma_q, inv_freq, lengths, positions):
+        return host.cache_rope_append(self.norm, self.eps, self.interleaved, self.sections, K, K_cache, Q, Q_out, V, V_cache, counts, gamma_k, gamma_q, inv_freq,
+                                      lengths, positions)
+
+
+class CachePrefixAttention(FusedModule):
+    """Attention over a prefix that all sequences of a batch share and each one's own keys (`ops.cache_prefix_attention`).  One launch, or two with shares of the keys."""
+    TENSOR_PARAMS = ["K", "K_prefix", "O", "Q", "V", "V_prefix", "counts", "lengths"]
+
+    def __init__(self, scale: Optional[float] = None, causal: bool = True):
+        super().__init__()
+        self.scale, self.causal = scale, causal
+
+    def _native(self, host, ws, K, K_prefix, O, Q, V, V_prefix, counts, lengths):
+        return host.cache_prefix_attention(ws, self.scale, self.causal, K, K_prefix, O, Q, V, V_prefix, counts, lengths)
+
+
+class CacheBounds(FusedModule):
+    """Bounds of a cache's blocks by channel, of those that the new tokens lie in (`ops.cache_bounds`).  tokens: the most of them that a call has (None: any number).  One
+    launch."""
+    TENSOR_PARAMS = ["K", "bounds", "counts", "lengths"]
+
+    def __init__(self, block: int = 64, tokens: Optional[int] = None):
+        super().__init__()
+        self.block, self.tokens = block, tokens
+
+    def _native(self, host, ws, K, bounds, counts, lengths):
+        return host.cache_bounds(self.block, self.tokens, K, bounds, counts, lengths)
+
+
+class CacheSparseAttention(FusedModule):
+    """Attention over the blocks that each query selects by their bounds (`ops.cache_sparse_attention`)."""
+    TENSOR_PARAMS = ["K", "O", "Q", "V", "bounds", "counts", "lengths", "selected"]
+
+    def __init__(self, top: int, sink: int = 0, recent: int = 1, block: int = 64, scale: Optional[float] = None):
+        super().__init__()
+        if top < 1 or sink < 0 or recent < 1 or sink + recent > top:
+            raise ValueError("top, sink, recent: expected sink >= 0, recent >= 1, sink + recent <= top")
+        self.top, self.sink, self.recent, self.block, self.scale = top, sink, recent, block, scale
+
+    def _native(self, host, ws, K, O, Q, V, bounds, counts, lengths, selected):
+        return host.cache_sparse_attention(ws, self.scale, self.block, self.top, self.sink, self.recent, K, O, Q, V, bounds, counts, lengths, selected)
+
+
 CACHE8 = {"vanilla": Cache8Step, "prenorm": lambda **kw: Cache8Step(norm=True, **kw), "weights": Cache8StepWeights}
-CACHE = {"append8": Cache8Append, "attn8": Cache8Attention, "weights8": Cache8KeyWeights, "evict": CacheEvict, "evict8": Cache8Evict}
+CACHE = {"append8": Cache8Append, "attn8": Cache8Attention, "weights8": Cache8KeyWeights, "evict": CacheEvict, "evict8": Cache8Evict,
+         "rope": CacheRope, "prefix": CachePrefixAttention, "bounds": CacheBounds, "sparse": CacheSparseAttention}
 
 PREFILL = {"rms": RMSNorm, "vanilla": Attention, "prenorm": PreNormBlock, "qknorm": QKNormAttention,
            "keyformer": KeyFormerAttention, "roco": RoCoAttention}
@@ -659,7 +714,8 @@ def get(variant: str, form: str = "prefill", **consts) -> FusedModule:
     form='decode' : the reference's decode-append problem (needs head_dim=...).
     form='linear' : the reference's LoRA and gated-MLP workloads.
     form='cache8' : the decode-append step on an 8-bit cache, {'vanilla','prenorm','weights'} (needs head_dim=...).
-    form='cache'  : an 8-bit cache's append, attention and key weights, and eviction, {'append8','attn8','weights8','evict','evict8'}."""
+    form='cache'  : an 8-bit cache's append, attention and key weights, and eviction, {'append8','attn8','weights8','evict','evict8'};
+                    an fp16 cache's rotated append, attention behind a shared prefix and over selected blocks, {'rope','prefix','bounds','sparse'}."""
     table = {"prefill": PREFILL, "decode": DECODE, "linear": LINEAR, "cache": CACHE, "cache8": CACHE8}.get(form)
     if table is None or variant not in table:
         raise KeyError(f"no module for variant={variant!r} form={form!r}")

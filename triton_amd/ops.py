@@ -427,6 +427,55 @@ def cache_evict_workspace_bytes(k, weights, keep: int) -> int:
     return int(_lib.load().trn_cache_evict_workspace_bytes(C.byref(e)))
 
 
+def cache_rope_append(q, k, v, q_out, k_cache, v_cache, inv_freq: Optional[torch.Tensor], lengths: Optional[torch.Tensor] = None,
+                      counts: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None, gamma_q: Optional[torch.Tensor] = None,
+                      gamma_k: Optional[torch.Tensor] = None, norm: bool = False, eps: float = 1e-6, interleaved: bool = False, sections=None) -> None:
+    """New tokens q [B,Hq,M,D], k, v [B,Hkv,M,D] fp16 into q_out (or q itself) and caches [B,Hkv,S,D]: queries and keys RMS-normalised by head (norm=True;
+    gamma_q, gamma_k fp16 [D] or None) and rotated by their positions, values as they are.  inv_freq float64 [pairs] (None: no rotation): pair p, elements p and
+    p + pairs or, interleaved, 2p and 2p + 1, is turned by position * inv_freq[p].  lengths int32 [B]: the keys of each sequence with the new ones (None: S); counts int32
+    [B]: its new tokens (None: M).  Token i goes to position lengths[b] - counts[b] + i, which is what it is rotated by, unless positions int32 [axes,B,M] are
+    given: of several axes, sections[axis] pairs each, one after the other.  Rows from counts[b] on are padding: neither read nor written."""
+    _lib.host().cache_rope_append(norm, eps, interleaved, sections, k, k_cache, q, q_out, v, v_cache, counts, gamma_k, gamma_q, inv_freq, lengths, positions)
+
+
+def _cache16_sizes(k) -> "_lib.Cache16":
+    c = _lib.Cache16()
+    c.batch, c.n_kv_heads, c.capacity, c.head_dim = (int(x) for x in k.shape)
+    return c
+
+
+def cache_prefix_attention(q, k, v, k_prefix, v_prefix, o, scale: Optional[float] = None, causal: bool = True, lengths: Optional[torch.Tensor] = None,
+                           counts: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> None:
+    """`attention` of q, o [B,Hq,M,D] over a prefix k_prefix, v_prefix [Hkv,P,D] that all sequences share and over each one's own keys k, v [B,Hkv,S,D];
+    lengths and counts (of own keys) as in `cache_rope_append`.  A query sees the whole prefix and, causal, own keys up to its own position.  Outputs from
+    counts[b] on are not written; a query that sees no key gets zeros.  workspace: uint8, cache_prefix_attention_workspace_bytes(...) bytes of any contents."""
+    _lib.host().cache_prefix_attention(workspace, scale, causal, k, k_prefix, o, q, v, v_prefix, counts, lengths)
+
+
+def cache_prefix_attention_workspace_bytes(q, k, k_prefix) -> int:
+    """Bytes of workspace that `cache_prefix_attention` takes for these tensors' shapes."""
+    return int(_lib.load().trn_cache_prefix_attn_workspace_bytes(C.byref(_cache16_sizes(k)), int(k_prefix.shape[1]), int(q.shape[1]), int(q.shape[2])))
+
+
+def cache_bounds(k, bounds, block: int = 64, lengths: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None, tokens: Optional[int] = None) -> None:
+    """Least and largest of the keys k [B,Hkv,S,D] fp16 by channel and block of 32, 64 or 128: bounds fp16 [B,Hkv,ceil(S/block),2,D], brought up to date for the blocks
+    that the last counts[b] of lengths[b] keys lie in; tokens: the most that counts can be (None: S).  A block's keys from lengths[b] on do not count, nor does NaN."""
+    _lib.host().cache_bounds(block, tokens, k, bounds, counts, lengths)
+
+
+def cache_sparse_attention(q, k, v, bounds, o, selected, top: int, sink: int = 0, recent: int = 1, block: int = 64, scale: Optional[float] = None,
+                           lengths: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> None:
+    """Causal attention of q, o [B,Hq,M,D] over `top` blocks of the cache k, v [B,Hkv,S,D] for each query and KV head: the first `sink`, the last `recent` (the query's
+    own is the last) and of the others those whose bounds (see cache_bounds) allow the largest q . k of any query head, ties to the earlier one.  selected int32
+    [B,Hkv,M,top] receives them, ascending, then -1.  lengths, counts and workspace (cache_sparse_attention_workspace_bytes) as in `cache_prefix_attention`."""
+    _lib.host().cache_sparse_attention(workspace, scale, block, top, sink, recent, k, o, q, v, bounds, counts, lengths, selected)
+
+
+def cache_sparse_attention_workspace_bytes(q, k, top: int, block: int = 64) -> int:
+    """Bytes of workspace that `cache_sparse_attention` takes for these tensors' shapes."""
+    return int(_lib.load().trn_cache_sparse_attn_workspace_bytes(C.byref(_cache16_sizes(k)), int(block), int(top), int(q.shape[1]), int(q.shape[2])))
+
+
 def calibration_copy(src: torch.Tensor, dst: torch.Tensor) -> None:
     """dst <- src with the library's plain streaming copy kernel (measurement yardstick)."""
     _need(src.is_cuda and dst.is_cuda and src.is_contiguous() and dst.is_contiguous(), "expected contiguous GPU tensors")
