@@ -249,3 +249,34 @@ def test_selection_of_equals_and_of_what_is_no_number():
         score = torch.maximum(*(torch.nan_to_num((s * x[0, 0, :, :, c].double()).amax(-1), nan=-math.inf, posinf=math.inf) for c, s in ((0, 1.0), (1, -1.0)))).tolist()
         rest = sorted(range(1, 598), key=lambda b: (-score[b], b))[:6]
         assert got == sorted([0, 598, 599] + rest)
+
+
+MANY = [
+    # as SPARSES: blocks of more than 2048, and of more than a workgroup holds
+    (1, 4, 1, 64, 2, 32 * 3001, [32 * 3000 + 5], [2], 32, 33, 1, 2),
+    (2, 8, 1, 128, 1, 32 * 2100, [32 * 2100, 32 * 1500 + 7], [1, 1], 32, 20, 0, 1),
+    (1, 2, 2, 64, 1, 32 * 8300, [32 * 8300 - 1], [1], 32, 40, 2, 3),
+    (1, 2, 1, 128, 300, 1500, [1500], [300], 32, 6, 1, 1),
+    (5, 8, 8, 64, 30, 900, [900, 30, 500, 31, 0], [30, 30, 17, 1, 30], 64, 4, 1, 1),      # a wave a query
+]
+
+
+@pytest.mark.parametrize("case", MANY, ids=lambda c: f"B{c[0]}H{c[1]}_{c[2]}D{c[3]}M{c[4]}S{c[5]}b{c[8]}t{c[9]}")
+@pytest.mark.parametrize("size", [1.0, 2e-4, 300.0])
+def test_selection_of_many_blocks(case, size):
+    """Scores of ordinary size, of numbers near fp16's least (which a matrix pipe may take for zero), and of large ones; keys alike in all blocks but the last bits."""
+    B, Hq, Hkv, D, M, S, lengths, counts, block, top, sink, recent = case
+    g = _gen(9)
+    q = (torch.randn(B, Hq, M, D, generator=g) * size).half()
+    base = torch.randn(B, Hkv, 1, 2, D, generator=g)
+    blocks = -(-S // block)
+    bnd = ((base + torch.randn(B, Hkv, blocks, 2, D, generator=g) * 0.002).sort(3).values * min(size, 100.0)).half()
+    sel = torch.full((B, Hkv, M, top), 5, dtype=torch.int32)
+    want = ref.select(q, bnd, sel, block, top, sink, recent, Hq // Hkv, lengths, counts, S)
+    k, v = (torch.randn(B, Hkv, S, D, generator=g).half() for _ in range(2))
+    dsel, do = sel.to(DEV), torch.zeros_like(q, device=DEV)
+    modules.get("sparse", "cache", block=block, top=top, sink=sink, recent=recent).forward(k.to(DEV), do, q.to(DEV), v.to(DEV), bnd.to(DEV), _ints(counts), _ints(lengths), dsel)
+    assert torch.equal(dsel.cpu(), want)
+    if size == 1.0:
+        out, tol = ref.sparse_attention(q, k, v, torch.zeros_like(q), want, block, D ** -0.5, lengths, counts)
+        _within(do, out, tol)

@@ -21,6 +21,8 @@ EXPORTS = (
     "trn_attn_fwd_stats_half_f16", "trn_attn_fwd_stats_ws_f16", "trn_attn_stats_workspace_bytes",
     "trn_attn_key_scores_f16", "trn_attn_key_scores_workspace_bytes", "trn_attn_qknorm_f16", "trn_attn_qknorm_workspace_bytes",
     "trn_cache8_append_f16", "trn_cache8_attn_workspace_bytes", "trn_cache8_attn_f16", "trn_cache_evict_workspace_bytes", "trn_cache_evict",
+    "trn_cache_rope_append_f16", "trn_cache_prefix_attn_workspace_bytes", "trn_cache_prefix_attn_f16", "trn_cache_bounds_f16",
+    "trn_cache_sparse_attn_workspace_bytes", "trn_cache_sparse_attn_f16",
 )
 
 

@@ -15,7 +15,7 @@ namespace trn {
 // What became of a row's keys in one share: O unnormalised, and (m, l) with m in units of log2.  Row `row` of B Hkv M G has `slots` of them.
 struct Parts { float* o; float* ml; int slots; };
 
-constexpr int kNarrowLds(int D) { return 4 * 4 * 32 * D * 2; }
+constexpr int kNarrowLds(int D) { return 4 * 2 * 32 * D * 2; }
 constexpr int kWideLds(int D) { return 4 * 64 * D * 2; }
 
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -57,17 +57,15 @@ __device__ __forceinline__ half8_t finite_only(half8_t v) {
 }
 
 // ------------------------------------------------------------------------------------------------ narrow
-// One wave's tiles t0 <= t < t1 of 32 keys for 16 NQ rows (queries in qB), into o, m, l.  `keys`: where the tile t begins and how many of its keys there are (0..32, wave-uniform; those
+// One wave's tiles t0 <= t < t1, every STEP-th, of 32 keys for 16 NQ rows (queries in qB), into o, m, l.  `keys`: where the tile t begins and how many of its keys there are (0..32, wave-uniform; those
 // from there on arrive as zeros and count for no row), as .k(t), .v(t), .n(t), requested in order.  Keys from `last` on (relative to the tile, through .at(t)) are hidden from a row.
-template <int D, int NQ, class Keys>
+template <int D, int NQ, int STEP, class Keys>
 __device__ __forceinline__ void narrow_walk(Keys& keys, int t0, int t1, int t_mask, int kpitch, int vpitch, float c, const half8_t (&qB)[NQ][D / 32], const int (&last)[NQ], char* lds,
                                             float4_t (&o)[D / 16][NQ], float (&m)[NQ], float (&l)[NQ]) {
     constexpr int NI = D / 32, NDB = D / 16, TILE = 32 * D, RPI = 512 / D, NL = 32 / RPI, CPR = D / 8;
     const int lane = threadIdx.x & 63, n = lane & 15, g4 = lane >> 4;
-    half_t* const K0 = reinterpret_cast<half_t*>(lds);
-    half_t* const K1 = K0 + TILE;
-    half_t* const V0 = K1 + TILE;
-    half_t* const V1 = V0 + TILE;
+    half_t* const Kt = reinterpret_cast<half_t*>(lds);
+    half_t* const Vt = Kt + TILE;
     // staging: load i covers the rows RPI i + lane / CPR; swizzles repeat every other (or second other) load
     const int sr = lane / CPR, sc = lane % CPR;
     int k_off[2], v_off[2];
@@ -86,14 +84,10 @@ __device__ __forceinline__ void narrow_walk(Keys& keys, int t0, int t1, int t_ma
     }
     const float4_t zero = {0.f, 0.f, 0.f, 0.f};
 
-    auto ahead = [&](int t, half_t* Kt, half_t* Vt) __attribute__((always_inline)) {
-        __builtin_amdgcn_sched_barrier(0);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // everything of the stage that is overwritten has been read
-        const int there = t < t1 ? keys.n(t) : 0;
-        const half_t* const kp = t < t1 ? keys.k(t) : keys.kp;
-        const half_t* const vp = t < t1 ? keys.v(t) : keys.vp;
-        const __amdgpu_buffer_rsrc_t ks = __builtin_amdgcn_make_buffer_rsrc((void*)kp, 0, there ? ((there - 1) * kpitch + D) * 2 : 0, 0x00020000);
-        const __amdgpu_buffer_rsrc_t vs = __builtin_amdgcn_make_buffer_rsrc((void*)vp, 0, there ? ((there - 1) * vpitch + D) * 2 : 0, 0x00020000);
+    auto ahead = [&](int t) __attribute__((always_inline)) {
+        const int there = keys.n(t);
+        const __amdgpu_buffer_rsrc_t ks = __builtin_amdgcn_make_buffer_rsrc((void*)keys.k(t), 0, there ? ((there - 1) * kpitch + D) * 2 : 0, 0x00020000);
+        const __amdgpu_buffer_rsrc_t vs = __builtin_amdgcn_make_buffer_rsrc((void*)keys.v(t), 0, there ? ((there - 1) * vpitch + D) * 2 : 0, 0x00020000);
 #pragma unroll
         for (int i = 0; i < NL; ++i)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(ks, (__attribute__((address_space(3))) void*)(Kt + i * 512), 16, k_off[(i * RPI >> 3) & 1], i * RPI * kpitch * 2, 0, 0);
@@ -102,12 +96,11 @@ __device__ __forceinline__ void narrow_walk(Keys& keys, int t0, int t1, int t_ma
             __builtin_amdgcn_raw_ptr_buffer_load_lds(vs, (__attribute__((address_space(3))) void*)(Vt + i * 512), 16, v_off[D == 128 ? i & 1 : 0], i * RPI * vpitch * 2, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
     };
-    auto arrived = [&] {       // the tile before the one that was requested last
-        if constexpr (D == 128) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
-        else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-    };
-    auto step = [&](auto mask_tag, int t, const half_t* Kt, const half_t* Vt) __attribute__((always_inline)) {
+    // A tile passes from LDS into registers whole, and the next one is requested into the same place before it is worked on: one stage a wave, so that two workgroups share a
+    // compute unit, has as many bytes on their way as two stages of one.
+    auto step = [&](auto mask_tag, int t) __attribute__((always_inline)) {
         constexpr bool MASK = decltype(mask_tag)::value;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         half8_t kw[2][NI], vw[NDB];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
@@ -118,6 +111,9 @@ __device__ __forceinline__ void narrow_walk(Keys& keys, int t0, int t1, int t_ma
             const half4_t x = lds_read_tr16(Vt + (vr[0] ^ (i << 4))), y = lds_read_tr16(Vt + (vr[1] ^ (i << 4)));
             vw[i] = half8_t{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
         }
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (t + STEP < t1) ahead(t + STEP);
         __builtin_amdgcn_sched_barrier(0);
         float4_t s[2][NQ];
 #pragma unroll
@@ -181,21 +177,21 @@ __device__ __forceinline__ void narrow_walk(Keys& keys, int t0, int t1, int t_ma
             for (int i = 0; i < NDB; ++i) bad = bad || odd_values(vw[i]);
             if (__builtin_expect(__builtin_amdgcn_ballot_w64(bad) != 0, 0)) {
                 const int key0 = keys.at(t);
+#pragma unroll
+                for (int qb = 0; qb < NQ; ++qb) {
+                    const int lim = last[qb] - key0 - 4 * g4;
+                    half8_t see;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) see[e] = 16 * (e >> 2) + (e & 3) <= lim ? (half_t)1.f : (half_t)0.f;
+#pragma unroll
+                    for (int i = 0; i < NDB; ++i)
 #pragma unroll 1
-                for (int kind = 0; kind < 3; ++kind)
-#pragma unroll
-                    for (int qb = 0; qb < NQ; ++qb) {
-                        const int lim = last[qb] - key0 - 4 * g4;
-                        half8_t see;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) see[e] = 16 * (e >> 2) + (e & 3) <= lim ? (half_t)1.f : (half_t)0.f;
-#pragma unroll
-                        for (int i = 0; i < NDB; ++i) {
+                        for (int kind = 0; kind < 3; ++kind) {
                             const float4_t hit = mfma16(odd_kind(vw[i], kind), see, zero);
 #pragma unroll
                             for (int e = 0; e < 4; ++e) o[i][qb][e] += hit[e] > 0.f ? (kind == 0 ? INFINITY : kind == 1 ? -INFINITY : NAN) : 0.f;
                         }
-                    }
+                }
 #pragma unroll
                 for (int i = 0; i < NDB; ++i) vw[i] = finite_only(vw[i]);
             }
@@ -208,28 +204,11 @@ __device__ __forceinline__ void narrow_walk(Keys& keys, int t0, int t1, int t_ma
                 o[i][qb] = mfma16(vw[i], rest[qb], o[i][qb]);
             }
     };
-    const std::false_type whole{};
-    const std::true_type partly{};
     if (t0 >= t1) return;
-    ahead(t0, K0, V0);
+    ahead(t0);
     int t = t0;
-    for (; t + 2 <= t_mask; t += 2) {
-        ahead(t + 1, K1, V1);
-        arrived();
-        step(whole, t, K0, V0);
-        ahead(t + 2, K0, V0);
-        arrived();
-        step(whole, t + 1, K1, V1);
-    }
-    for (; t < t1; t += 2) {
-        ahead(t + 1, K1, V1);
-        arrived();
-        step(partly, t, K0, V0);
-        ahead(t + 2, K0, V0);
-        arrived();
-        if (t + 1 < t1) step(partly, t + 1, K1, V1);
-    }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    for (; t < t_mask; t += STEP) step(std::false_type{}, t);
+    for (; t < t1; t += STEP) step(std::true_type{}, t);
 }
 
 // The results of a row tile's four waves, joined and delivered: row i of the tile by put(i, first dimension, O, m, l, whether this is the row's first piece).
@@ -245,7 +224,7 @@ __device__ __forceinline__ void narrow_join(char* lds, NarrowStats& st, float4_t
     }
     __syncthreads();
     // (a wave's stage holds its RT rows of D floats; the 16-byte pieces of a row are swizzled by the row)
-    constexpr int AREA = 4 * 32 * D * 2;
+    constexpr int AREA = 2 * 32 * D * 2;
     float4_t* const mem = reinterpret_cast<float4_t*>(lds + wave * AREA);
 #pragma unroll
     for (int qb = 0; qb < NQ; ++qb) {
@@ -316,6 +295,7 @@ __device__ __forceinline__ void wide_walk(const Keys& keys, int t0, int t1, int 
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[kb][e] = 32 * kb + 8 * (e >> 2) + (e & 3) <= lim ? s[kb][e] : -INFINITY;
         }
+        __builtin_amdgcn_sched_barrier(0);
         const float tm = fmaxf(max16(s[0]), max16(s[1])) * c;
         if (__builtin_expect(__builtin_amdgcn_ballot_w64(tm > m + 8.f) != 0, 0)) {
             const float up = fmaxf(m, half_max(tm)), alpha = up == -INFINITY ? 1.f : fast_exp2(m - up);
@@ -336,38 +316,44 @@ __device__ __forceinline__ void wide_walk(const Keys& keys, int t0, int t1, int 
                 p[2 * kb + (e >> 3)][e & 7] = (half_t)x;
             }
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        auto value = [&](int u, int i) __attribute__((always_inline)) {       // of the keys 16 u + (0..3, 8..11) + 4 h, for one dimension
+            const half4_t x = lds_read_tr16(Vt + u * 16 * D + (vr[0] ^ (i << 5))), y = lds_read_tr16(Vt + u * 16 * D + (vr[1] ^ (i << 5)));
+            return half8_t{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+        };
+        bool odd = false;
+        if constexpr (MASK) {               // (as in the narrow form)
+            bool bad = false;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {           // 16 keys each
-            half8_t vw[NDB];
+            for (int u = 0; u < 4; ++u)
 #pragma unroll
-            for (int i = 0; i < NDB; ++i) {
-                const half4_t x = lds_read_tr16(Vt + u * 16 * D + (vr[0] ^ (i << 5))), y = lds_read_tr16(Vt + u * 16 * D + (vr[1] ^ (i << 5)));
-                vw[i] = half8_t{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-            }
-            if constexpr (MASK) {               // (as in the narrow form)
-                bool bad = false;
+                for (int i = 0; i < NDB; ++i) { bad = bad || odd_values(value(u, i)); __builtin_amdgcn_sched_barrier(0); }
+            odd = __builtin_amdgcn_ballot_w64(bad) != 0;
+            if (__builtin_expect(odd, 0)) {
 #pragma unroll
-                for (int i = 0; i < NDB; ++i) bad = bad || odd_values(vw[i]);
-                if (__builtin_expect(__builtin_amdgcn_ballot_w64(bad) != 0, 0)) {
+                for (int u = 0; u < 4; ++u) {
                     const int lim = keys.lim(t, last) - 16 * u - 4 * h;
                     half8_t see;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) see[e] = 8 * (e >> 2) + (e & 3) <= lim ? (half_t)1.f : (half_t)0.f;
-#pragma unroll 1
-                    for (int kind = 0; kind < 3; ++kind)
 #pragma unroll
-                        for (int i = 0; i < NDB; ++i) {
-                            const float16_t hit = mfma32(odd_kind(vw[i], kind), see, zero);
+                    for (int i = 0; i < NDB; ++i)
+#pragma unroll 1
+                        for (int kind = 0; kind < 3; ++kind) {
+                            const float16_t hit = mfma32(odd_kind(value(u, i), kind), see, zero);
 #pragma unroll
                             for (int e = 0; e < 16; ++e) o[i][e] += hit[e] > 0.f ? (kind == 0 ? INFINITY : kind == 1 ? -INFINITY : NAN) : 0.f;
                         }
-#pragma unroll
-                    for (int i = 0; i < NDB; ++i) vw[i] = finite_only(vw[i]);
                 }
             }
-#pragma unroll
-            for (int i = 0; i < NDB; ++i) o[i] = mfma32(vw[i], p[u], o[i]);
         }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int i = 0; i < NDB; ++i) {
+                half8_t v = value(u, i);
+                if (MASK && __builtin_expect(odd, 0)) v = finite_only(v);
+                o[i] = mfma32(v, p[u], o[i]);
+            }
     };
     if (t0 >= t1) return;
     ahead(t0, 0);

@@ -32,8 +32,8 @@ inline PlanPrefix plan_prefix(int batch, int n_kv_heads, int capacity, int head_
         p.n_rt_p = (int)(p.wide ? (rows_p + 127) / 128 : (rows_p + 16 * p.nq - 1) / (16 * p.nq));
         p.n_rt_o = (p.R + 16 * p.nq - 1) / (16 * p.nq);
         const int64_t units_p = (int64_t)n_kv_heads * p.n_rt_p, units_o = heads * p.n_rt_o;
-        // (as many keys a workgroup as make one workgroup a compute unit, two of head_dim 64; 256 at least)
-        const int64_t groups = head_dim == 128 ? 256 : 512, all = units_p * prefix + units_o * capacity;
+        // (as many keys a workgroup as make two workgroups a compute unit; 256 at least)
+        const int64_t groups = 512, all = units_p * prefix + units_o * capacity;
         int64_t each = (all + groups - 1) / groups;
         if (each < 256) each = 256;
         auto shares = [&](int64_t n) { const int64_t s = (n + each - 1) / each; return (int)(s > 64 ? 64 : s); };
@@ -50,9 +50,12 @@ inline PlanPrefix plan_prefix(int batch, int n_kv_heads, int capacity, int head_
     return p;
 }
 
+// Up to so many blocks a workgroup holds a query's scores in registers.
+constexpr int kMostBlocks = 8192;
+
 // Selected blocks: a query's scores in rows of nbp floats, `step` queries of each head at a time; row tiles of 16 nq of a KV head's query heads, ns shares of a query's keys; offsets of
-// the shares' parts behind the scores.
-struct PlanSparse { int G, nb, nq, n_rt, ns, step; int64_t nbp, o, ml, bytes; };
+// the shares' parts behind the scores and the norms; rows: a wave a row tile rather than a workgroup.
+struct PlanSparse { int G, nb, nq, n_rt, ns, step; bool rows; int64_t nbp, norms, o, ml, bytes; };
 
 inline PlanSparse plan_sparse(int batch, int n_kv_heads, int capacity, int head_dim, int block, int top, int Hq, int Sq) {
     PlanSparse p{};
@@ -64,11 +67,13 @@ inline PlanSparse plan_sparse(int batch, int n_kv_heads, int capacity, int head_
     p.step = (int)(step < 1 ? 1 : step > Sq ? Sq : step);
     p.nq = p.G > 16 ? 2 : 1;
     p.n_rt = (p.G + 16 * p.nq - 1) / (16 * p.nq);
-    const int64_t units = heads * Sq * p.n_rt, groups = head_dim == 128 ? 256 : 512, tiles = (int64_t)(top < p.nb ? top : p.nb) * (block / 32);
+    const int64_t units = heads * Sq * p.n_rt, groups = 512, tiles = (int64_t)(top < p.nb ? top : p.nb) * (block / 32);
     int64_t ns = units ? groups / units : 1;
     if (ns > tiles / 8) ns = tiles / 8;
     p.ns = (int)(ns < 1 ? 1 : ns > 32 ? 32 : ns);
-    p.o = up256(row * p.step);
+    p.rows = units >= 1024;
+    p.norms = up256(row * p.step);
+    p.o = p.norms + up256(row / 16);
     p.ml = p.o + (p.ns > 1 ? up256(heads * Sq * p.G * p.ns * head_dim * 4) : 0);
     p.bytes = p.ml + (p.ns > 1 ? up256(heads * Sq * p.G * p.ns * 8) : 0);
     return p;

@@ -98,7 +98,7 @@ __global__ __launch_bounds__(256, 2) void cache_prefix_rows_kernel(const PrefixA
 
 // The rows of all sequences over shares of the prefix (the first workgroups), each sequence's rows over shares of its own keys (the others).
 template <int D, int NQ, bool WIDE>
-__global__ __launch_bounds__(256, D == 128 ? 1 : 2) void cache_prefix_parts_kernel(const PrefixArgs a) {
+__global__ __launch_bounds__(256, 2) void cache_prefix_parts_kernel(const PrefixArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     __shared__ __attribute__((aligned(1024))) char lds[kNarrowLds(D)];
     __shared__ NarrowStats stats;
@@ -178,7 +178,7 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void cache_prefix_parts_kern
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) o[i][qb] = float4_t{0.f, 0.f, 0.f, 0.f};
     }
-    narrow_walk<D, NQ>(keys, t0, t1, min(t1, max(t0, sees(rt * RT) >> 5)), keys.kpitch, keys.vpitch, a.c, qB, last, lds + wave * 4 * 32 * D * 2, o, m, l);
+    narrow_walk<D, NQ, 1>(keys, t0, t1, min(t1, max(t0, sees(rt * RT) >> 5)), keys.kpitch, keys.vpitch, a.c, qB, last, lds + wave * 2 * 32 * D * 2, o, m, l);
     narrow_join<D, NQ>(lds, stats, o, m, l, [&](int i, int d0, float4_t v, float mm, float ll, bool once) __attribute__((always_inline)) {
         const int row = rt * RT + i;
         if (row >= all) return;

@@ -1,8 +1,9 @@
 // Attention over those blocks of a long cache that a cheap score selects for each query: bounds of the blocks' keys by channel, a score from them, the selection,
 // and the attention over what is selected.
 //
-// A key k within lo <= k <= hi scores q . k <= sum_d max(q_d lo_d, q_d hi_d): of a block of 64 keys that reads 2 rows in the place of 64.  The sum is over products of two fp16 numbers, exact in 32
-// bits, added in 64, so that the order of additions does not show in the 32 bits that are compared (but where a sum lies on the border of two of them) and the selection is the definition's.
+// A key k within lo <= k <= hi scores q . k <= sum_d max(q_d lo_d, q_d hi_d) = sum_d (max(q_d, 0) hi_d + min(q_d, 0) lo_d): of a block of 64 keys that reads 2 rows in the place of
+// 64, and is a product of matrices.  Selected is by that sum rounded from 64 bits, so that the order of additions does not show.  Up to 8192 blocks the matrix pipe computes it in 32 bits,
+// with a bound of how far that is off, and 64 bits are spent where it matters: on blocks within twice the bound of the last score that is taken, if not all of them are.
 #include "cache16_attn.h"
 #include "cache16_rules.h"
 
@@ -57,7 +58,7 @@ __global__ __launch_bounds__(256) void cache_bounds_kernel(const BoundsArgs a) {
 // ------------------------------------------------------------------------------------------------ scores
 struct SelectArgs {
     const half_t *q, *bounds; const int32_t *lengths, *counts;
-    float* scores; int32_t* selected;
+    float *scores, *norms; int32_t* selected;
     int B, Hkv, M, cap, G, block_shift, nb, top, sink, recent, i0, n, steps;      // queries i0 .. i0 + n
     int64_t nbp, qs[3];
     Div by_hkv, by_n;
@@ -76,9 +77,62 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 }
 #endif
 
-// D / 8 lanes have a block, eight channels each; a wave 512 / D blocks at a time.
+// Scores by the matrix pipe.  A wave has 16 blocks, whose bounds it holds as operands (lane 16 g + n: block n, channels 8 g..+7 of each 32), and goes through its queries, 16 at a
+// time and their heads one after the other, so that the largest over the heads stays in a lane.  norms: the largest |bound| vector (of each channel's larger end) of every 16 blocks, squared;
+// infinite where a bound is not finite.
 template <int D>
 __global__ __launch_bounds__(256) void cache_scores_kernel(const SelectArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    constexpr int NI = D / 32;
+    const int lane = threadIdx.x & 63, n = lane & 15, g4 = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int bh = blockIdx.z, b = a.by_hkv.of(bh), kvh = bh - b * a.Hkv, set = blockIdx.x * 4 + wave;
+    const int L = length_of(a.lengths, b, a.cap), C = min(count_of(a.counts, b, a.M), a.i0 + a.n), blocks = L > 0 ? ((L - 1) >> a.block_shift) + 1 : 0;
+    if (set * 16 >= blocks || blocks <= a.top) return;      // (where all blocks are taken no score is needed)
+    const int blk = set * 16 + n;
+    const half_t* const bp = a.bounds + ((int64_t)bh * a.nb + min(blk, blocks - 1)) * 2 * D + 8 * g4;
+    half8_t lo[NI], hi[NI];
+#pragma unroll
+    for (int i = 0; i < NI; ++i) { lo[i] = *reinterpret_cast<const half8_t*>(bp + 32 * i); hi[i] = *reinterpret_cast<const half8_t*>(bp + D + 32 * i); }
+    if (blockIdx.y == 0) {
+        float sum = 0.f;
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            bad = bad || odd_values(lo[i]) || odd_values(hi[i]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) { const float x = fmaxf(fabsf((float)lo[i][e]), fabsf((float)hi[i][e])); sum = __builtin_fmaf(x, x, sum); }
+        }
+        sum = quad_sum(bad ? INFINITY : sum);
+#pragma unroll
+        for (int d = 1; d < 16; d *= 2) sum = fmaxf(sum, __shfl_xor(sum, d, 64));
+        if (lane == 0) a.norms[(int64_t)bh * (a.nbp >> 4) + set] = sum;
+    }
+    const float4_t zero = {0.f, 0.f, 0.f, 0.f};
+    half8_t nil = {};
+    for (int s = 0; s < a.steps; ++s) {
+        const int j0 = (blockIdx.y * a.steps + s) * 16, i = a.i0 + j0 + n;
+        if (a.i0 + j0 >= C) return;
+        const half_t* const qp = a.q + b * a.qs[0] + (int64_t)kvh * a.G * a.qs[1] + (int64_t)min(i, C - 1) * a.qs[2] + 8 * g4;
+        float4_t best = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        for (int g = 0; g < a.G; ++g) {
+            float4_t x = zero;
+#pragma unroll
+            for (int e = 0; e < NI; ++e) {
+                const half8_t q = *reinterpret_cast<const half8_t*>(qp + g * a.qs[1] + 32 * e);
+                x = mfma16(hi[e], __builtin_elementwise_max(q, nil), x);
+                x = mfma16(lo[e], __builtin_elementwise_min(q, nil), x);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) best[e] = fmaxf(best[e], x[e]);
+        }
+        if (i < C) *reinterpret_cast<float4_t*>(a.scores + ((int64_t)bh * a.n + j0 + n) * a.nbp + set * 16 + 4 * g4) = best;
+    }
+#endif
+}
+
+// D / 8 lanes have a block, eight channels each; a wave 512 / D blocks at a time.
+template <int D>
+__global__ __launch_bounds__(256) void cache_scores64_kernel(const SelectArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr int LPR = D / 8, PER = 64 / LPR;
     const int lane = threadIdx.x & 63, sub = lane % LPR, wave = threadIdx.x >> 6;
@@ -119,9 +173,215 @@ __global__ __launch_bounds__(256) void cache_scores_kernel(const SelectArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------ selection
-// A workgroup has one query of one KV head.  The score of the last one that is taken is found digit by digit (eight bits of the ordered scores, a count of each of their 256
+#if defined(__HIP_DEVICE_COMPILE__)
+// The want-th largest of a workgroup's open keys (bit r: key[r]), digit by digit of eight bits from the first bit on that they differ in: `known`, and how many of its equals
+// belong to the first `want` (`want` then).  Where all of a digit's keys do, the rest of the digits need not be known: `known` is then one less than the least of them.
+template <int T> struct KthShared { uint32_t any[T / 64], all[T / 64]; int count[256], sums[4], digit, left, done; };
+template <int T, int REGS>
+__device__ __forceinline__ void kth(const uint32_t (&key)[REGS], uint32_t open, int& want, uint32_t& known, KthShared<T>& sh) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    uint32_t any = 0, all = ~0u;
+#pragma unroll
+    for (int r = 0; r < REGS; ++r)
+        if (open >> r & 1) { any |= key[r]; all &= key[r]; }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) { any |= __shfl_xor((int)any, d, 64); all &= __shfl_xor((int)all, d, 64); }
+    if (lane == 0) { sh.any[wave] = any; sh.all[wave] = all; }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < T / 64; ++w) { any |= sh.any[w]; all &= sh.all[w]; }
+    const uint32_t differ = any & ~all;
+    known = all;
+    if (differ == 0) { __syncthreads(); return; }
+    int above = 32 - __builtin_clz(differ);
+    known = above == 32 ? 0u : all >> above << above;
+    while (above > 0) {
+        const int shift = max(above - 8, 0);
+        const uint32_t width = (1u << (above - shift)) - 1;
+        if (tid < 256) sh.count[tid] = 0;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < REGS; ++r)
+            if ((open >> r & 1) && (above == 32 || (key[r] ^ known) >> above == 0)) atomicAdd(&sh.count[key[r] >> shift & width], 1);
+        __syncthreads();
+        int mine = 0, sum = 0;
+        if (wave < 4) {                          // from the largest digit down
+            sum = mine = sh.count[255 - tid];
+#pragma unroll
+            for (int d = 1; d < 64; d *= 2) { const int y = __shfl_up(sum, d, 64); if (lane >= d) sum += y; }
+            if (lane == 63) sh.sums[wave] = sum;
+        }
+        __syncthreads();
+        if (wave < 4) {
+            for (int w = 0; w < wave; ++w) sum += sh.sums[w];
+            if (sum >= want && sum - mine < want) { sh.digit = 255 - tid; sh.left = want - (sum - mine); sh.done = sum == want; }
+        }
+        __syncthreads();
+        known |= (uint32_t)sh.digit << shift;
+        want = sh.left;
+        if (sh.done && known) { known -= 1; want = 0; break; }
+        above = shift;
+    }
+    __syncthreads();
+}
+// The score of one block in 64 bits, by a wave: D / 8 lanes have eight channels each, and the others as many query heads at a time.
+template <int D>
+__device__ __forceinline__ float score64(const SelectArgs& a, const half_t* q, int bh, int blk) {
+    constexpr int LPR = D / 8, PER = 64 / LPR;
+    const int lane = threadIdx.x & 63, sub = lane % LPR;
+    const half_t* const bp = a.bounds + ((int64_t)bh * a.nb + blk) * 2 * D + sub * 8;
+    const half8_t lo = *reinterpret_cast<const half8_t*>(bp), hi = *reinterpret_cast<const half8_t*>(bp + D);
+    double best = -INFINITY;
+    for (int g0 = 0; g0 < a.G; g0 += PER) {
+        const half8_t q8 = *reinterpret_cast<const half8_t*>(q + (int64_t)min(g0 + lane / LPR, a.G - 1) * a.qs[1] + sub * 8);
+        double x = 0.;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x += (double)fmaxf((float)q8[e] * (float)lo[e], (float)q8[e] * (float)hi[e]);
+#pragma unroll
+        for (int d = 1; d < LPR; d *= 2) x += __shfl_xor(x, d, 64);
+        best = fmax(best, x);
+    }
+#pragma unroll
+    for (int d = LPR; d < 64; d *= 2) best = fmax(best, __shfl_xor(best, d, 64));
+    return (float)best;
+}
+#endif
+
+// A workgroup has one query of one KV head, and of its blocks' scores REGS a thread.  Scores s come with a bound e of how far they are off the definition's, r.  If t is the last of s that would be
+// taken, the last of r is within e of t: s > t + 2 e belongs to what is taken, s < t - 2 e does not, and between them the definition decides, if that is needed.  e: the sum of 128 products
+// in 32 bits, 2 x 128 additions that may each cut off 2^-23 of the sum of their magnitudes, which is |q| |b| at most, is off by 2^-15 of that; the rounding of r by 2^-24; numbers that the matrix
+// pipe takes for zero, below 2^-14, by 2^-14 sqrt(128) of the other factor: e = 2^-14 (|q| + 12) (|b| + 12) covers all of it.
+template <int D, int T, int REGS>
+__global__ __launch_bounds__(T) void cache_select_kernel(const SelectArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __shared__ KthShared<T> sh;
+    __shared__ int waves[T / 64], waves2[T / 64];
+    __shared__ float norm_q[T / 64], norm_b[T / 64], least[T / 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int bh = a.by_n.of(blockIdx.x), j = blockIdx.x - bh * a.n, i = a.i0 + j, b = a.by_hkv.of(bh), kvh = bh - b * a.Hkv;
+    const float* const from = a.scores + ((int64_t)bh * a.n + j) * a.nbp;
+    float s[REGS];
+#pragma unroll
+    for (int r = 0; r < REGS; ++r) s[r] = r * T + tid < a.nbp ? from[r * T + tid] : 0.f;      // (requested before it is known how many count)
+    const half_t* const q = a.q + b * a.qs[0] + (int64_t)kvh * a.G * a.qs[1] + (int64_t)i * a.qs[2];
+    const int L = length_of(a.lengths, b, a.cap), C = count_of(a.counts, b, a.M), last = L - C + i, n = last < 0 ? 0 : (last >> a.block_shift) + 1;
+    if (i >= C) return;
+    int32_t* const to = a.selected + ((int64_t)bh * a.M + i) * a.top;
+    if (n <= a.top) {
+        for (int x = tid; x < a.top; x += T) to[x] = x < n ? x : -1;
+        return;
+    }
+    const int lo = a.sink, hi = n - a.recent;                     // what is chosen from (top > their number: not empty)
+    int want = a.top - a.sink - a.recent;
+    uint32_t sure = 0, maybe = 0, known = 0;
+    uint32_t key[REGS];
+    if (want > 0) {
+        float bb = 0.f, qq = 0.f;
+        for (int x = tid; x < (n + 15) >> 4; x += T) bb = fmaxf(bb, a.norms[(int64_t)bh * (a.nbp >> 4) + x]);
+        for (int g = wave; g < a.G; g += T / 64) {
+            float sum = 0.f;
+            bool bad = false;
+            if (lane < D / 8) {
+                const half8_t x = *reinterpret_cast<const half8_t*>(q + (int64_t)g * a.qs[1] + lane * 8);
+                bad = odd_values(x);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum = __builtin_fmaf((float)x[e], (float)x[e], sum);
+            }
+            if (bad) sum = INFINITY;
+#pragma unroll
+            for (int d = 1; d < D / 8; d *= 2) sum += __shfl_xor(sum, d, 64);
+            qq = fmaxf(qq, sum);
+        }
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) { bb = fmaxf(bb, __shfl_xor(bb, d, 64)); qq = fmaxf(qq, __shfl_xor(qq, d, 64)); }
+        if (lane == 0) { norm_q[wave] = qq; norm_b[wave] = bb; }
+        uint32_t open = 0;
+#pragma unroll
+        for (int r = 0; r < REGS; ++r) {
+            const int x = r * T + tid;
+            if (x >= lo && x < hi) open |= 1u << r;
+            key[r] = ordered(s[r]);
+        }
+        int left = want;
+        kth<T, REGS>(key, open, left, known, sh);
+        if (left == 0) known += 1;                                // the least digit string of what is taken: not above the last of them
+#pragma unroll
+        for (int w = 0; w < T / 64; ++w) { qq = fmaxf(qq, norm_q[w]); bb = fmaxf(bb, norm_b[w]); }
+        float e2 = 2.f * 1.01f * 0x1p-14f * (sqrtf(qq) + 12.f) * (sqrtf(bb) + 12.f);
+        // (known may be less than the last that is taken, by a part of its last digit: the least of those above it is the last)
+        float t = INFINITY;
+#pragma unroll
+        for (int r = 0; r < REGS; ++r)
+            if ((open >> r & 1) && key[r] >= known) t = fminf(t, s[r]);
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) t = fminf(t, __shfl_xor(t, d, 64));
+        if (lane == 0) least[wave] = t;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < T / 64; ++w) t = fminf(t, least[w]);
+        if (!(e2 < INFINITY)) e2 = INFINITY;
+        const float above = e2 < INFINITY ? t + e2 : INFINITY, below = e2 < INFINITY ? t - e2 : -INFINITY;
+        int n_sure = 0, n_maybe = 0;
+#pragma unroll
+        for (int r = 0; r < REGS; ++r)
+            if (open >> r & 1) {
+                if (s[r] > above) sure |= 1u << r;
+                else if (!(s[r] < below)) maybe |= 1u << r;
+            }
+        n_sure = __popc(sure); n_maybe = __popc(maybe);
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) { n_sure += __shfl_xor(n_sure, d, 64); n_maybe += __shfl_xor(n_maybe, d, 64); }
+        if (lane == 0) { waves[wave] = n_sure; waves2[wave] = n_maybe; }
+        __syncthreads();
+        n_sure = n_maybe = 0;
+#pragma unroll
+        for (int w = 0; w < T / 64; ++w) { n_sure += waves[w]; n_maybe += waves2[w]; }
+        want -= n_sure;
+        __syncthreads();
+        if (n_maybe == want) { sure |= maybe; maybe = 0; }
+        else {
+#pragma unroll
+            for (int r = 0; r < REGS; ++r) {
+                uint64_t todo = __builtin_amdgcn_ballot_w64(maybe >> r & 1);
+                while (todo) {
+                    const int bit = __builtin_ctzll(todo);
+                    todo &= todo - 1;
+                    const float x = score64<D>(a, q, bh, r * T + wave * 64 + bit);
+                    if (lane == bit) key[r] = ordered(x);
+                }
+            }
+            kth<T, REGS>(key, maybe, want, known, sh);
+        }
+    }
+    // what is taken, in order; of the equals of `known` the first `want`
+    int done = 0, equals = 0;
+#pragma unroll
+    for (int r = 0; r < REGS; ++r) {
+        if (r * T >= n) break;
+        const int x = r * T + tid;
+        const bool mb = maybe >> r & 1, equal = mb && key[r] == known;
+        const uint64_t eq = __builtin_amdgcn_ballot_w64(equal), under = (1ull << lane) - 1;
+        if (lane == 0) waves[wave] = __popcll(eq);
+        __syncthreads();
+        int rank = equals + __popcll(eq & under);
+        for (int w = 0; w < wave; ++w) rank += waves[w];
+        const bool take = x < n && (x < lo || x >= hi || (sure >> r & 1) || (mb && (key[r] > known || (equal && rank < want))));
+        const uint64_t tk = __builtin_amdgcn_ballot_w64(take);
+        if (lane == 0) waves2[wave] = __popcll(tk);
+        __syncthreads();
+        int at = done + __popcll(tk & under);
+        for (int w = 0; w < wave; ++w) at += waves2[w];
+        if (take) to[at] = x;
+#pragma unroll
+        for (int w = 0; w < T / 64; ++w) { equals += waves[w]; done += waves2[w]; }
+        __syncthreads();
+    }
+#endif
+}
+
+// The same of any number of blocks, whose scores are the definition's.  The score of the last one that is taken is found digit by digit (eight bits of the ordered scores, a count of each of their 256
 // values), then one walk over the blocks takes what is larger, and of its equals the first ones, in order.
-__global__ __launch_bounds__(256) void cache_select_kernel(const SelectArgs a) {
+__global__ __launch_bounds__(256) void cache_select_many_kernel(const SelectArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     __shared__ int count[256], waves[4], waves2[4], digit, left;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -212,7 +472,7 @@ struct Chosen {
 #endif
 
 template <int D, int NQ>
-__global__ __launch_bounds__(256, D == 128 ? 1 : 2) void cache_sparse_attn_kernel(const SparseArgs a) {
+__global__ __launch_bounds__(256, 2) void cache_sparse_attn_kernel(const SparseArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     __shared__ __attribute__((aligned(1024))) char lds[kNarrowLds(D)];
     __shared__ NarrowStats stats;
@@ -250,7 +510,7 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void cache_sparse_attn_kerne
 #pragma unroll
         for (int e = 0; e < D / 16; ++e) o[e][qb] = float4_t{0.f, 0.f, 0.f, 0.f};
     }
-    narrow_walk<D, NQ>(keys, t0, t1, min(t1, max(t0, whole)), keys.kpitch, keys.vpitch, a.c, qB, last, lds + wave * 4 * 32 * D * 2, o, m, l);
+    narrow_walk<D, NQ, 1>(keys, t0, t1, min(t1, max(t0, whole)), keys.kpitch, keys.vpitch, a.c, qB, last, lds + wave * 2 * 32 * D * 2, o, m, l);
     narrow_join<D, NQ>(lds, stats, o, m, l, [&](int r, int d0, float4_t v, float mm, float ll, bool once) __attribute__((always_inline)) {
         const int g = rt * RT + r;
         if (g >= a.G) return;
@@ -266,6 +526,63 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void cache_sparse_attn_kerne
         for (int e = 0; e < 4; ++e) out[e] = (half_t)(v[e] * inv);
         *reinterpret_cast<half4_t*>(a.o + b * a.os[0] + (int64_t)(kvh * a.G + g) * a.os[1] + i * a.os[2] + d0) = out;
     });
+#endif
+}
+
+// Many queries: a wave has one query's row tile, all its keys, and nothing is joined.  All walk up the cache at the same pace, so that blocks which several of them selected are found in
+// the L2 of their XCD.
+template <int D, int NQ>
+__global__ __launch_bounds__(256, 2) void cache_sparse_rows_kernel(const SparseArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __shared__ __attribute__((aligned(1024))) char lds[kNarrowLds(D)];
+    constexpr int RT = 16 * NQ;
+    const int lane = threadIdx.x & 63, n = lane & 15, g4 = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int x = a.by_hkv.of(blockIdx.x), kvh = blockIdx.x - x * a.Hkv, y = a.by_b.of(x), b = x - y * a.B, z = y * 4 + wave, i = a.by_rt.of(z), rt = z - i * a.n_rt;
+    const int L = length_of(a.lengths, b, a.cap), C = count_of(a.counts, b, a.M), seen = L - C + i + 1;
+    if (i >= C) return;
+    const int ends = seen > 0 ? (seen - 1) >> a.block_shift : -1, most = min(a.top, ends + 1), per = 1 << (a.block_shift - 5);
+    const int T = most > 0 ? (most - 1) * per + ((seen - (ends << a.block_shift) + 31) >> 5) : 0, whole = most > 0 ? (most - 1) * per + ((seen - (ends << a.block_shift)) >> 5) : 0;
+    half8_t qB[NQ][D / 32];
+    int last[NQ];
+    const half_t* const q0 = a.q + b * a.qs[0] + (int64_t)kvh * a.G * a.qs[1] + i * a.qs[2];
+    half_t* const o0 = a.o + b * a.os[0] + (int64_t)kvh * a.G * a.os[1] + i * a.os[2];
+#pragma unroll
+    for (int qb = 0; qb < NQ; ++qb) {
+        const int g = rt * RT + 16 * qb + n;
+        const bool there = g < a.G;
+        last[qb] = there ? seen - 1 : -1;
+        const half_t* const qp = q0 + (there ? g : 0) * a.qs[1];
+#pragma unroll
+        for (int e = 0; e < D / 32; ++e) {
+            const half8_t zero = {}, v = *reinterpret_cast<const half8_t*>(qp + 32 * e + 8 * g4);
+            qB[qb][e] = there ? v : zero;
+        }
+    }
+    Chosen keys{a.k + b * a.ks[0] + kvh * a.ks[1], a.v + b * a.vs[0] + kvh * a.vs[1], a.selected + (((int64_t)b * a.Hkv + kvh) * a.M + i) * a.top,
+                (int)a.ks[2], (int)a.vs[2], seen, a.block_shift, max(most, 1), 0, 0};
+    if (T > 0) keys.hold(0);
+    float4_t o[D / 16][NQ];
+    float m[NQ], l[NQ];
+#pragma unroll
+    for (int qb = 0; qb < NQ; ++qb) {
+        m[qb] = -INFINITY; l[qb] = 0.f;
+#pragma unroll
+        for (int e = 0; e < D / 16; ++e) o[e][qb] = float4_t{0.f, 0.f, 0.f, 0.f};
+    }
+    narrow_walk<D, NQ, 1>(keys, 0, T, whole, keys.kpitch, keys.vpitch, a.c, qB, last, lds + wave * 2 * 32 * D * 2, o, m, l);
+#pragma unroll
+    for (int qb = 0; qb < NQ; ++qb) {
+        const int g = rt * RT + 16 * qb + n;
+        const float sum = quad_sum(l[qb]), inv = sum == 0.f ? 0.f : 1.f / sum;
+        if (g >= a.G) continue;
+#pragma unroll
+        for (int e = 0; e < D / 16; ++e) {
+            half4_t out;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) out[c] = (half_t)(o[e][qb][c] * inv);
+            *reinterpret_cast<half4_t*>(o0 + g * a.os[1] + 16 * e + 4 * g4) = out;
+        }
+    }
 #endif
 }
 
@@ -325,11 +642,15 @@ extern "C" int trn_cache_sparse_attn_f16(const trn_cache16* c, const void* bound
     const int64_t heads = (int64_t)c->batch * c->n_kv_heads;
     const PlanSparse p = plan_sparse(c->batch, c->n_kv_heads, c->capacity, c->head_dim, block, top, n_q_heads, seq_q);
     if (p.bytes && (!workspace || workspace_bytes < p.bytes)) return TRN_E_SCRATCH;
-    const int64_t groups = heads * seq_q * p.n_rt * p.ns;
+    const int64_t groups = p.rows ? heads * (((int64_t)seq_q * p.n_rt + 3) / 4) : heads * seq_q * p.n_rt * p.ns;
     // (workgroups of 256, and as many threads in all as 32 bits number: of every launch, before the first one)
-    const int per = 4 * 512 / c->head_dim, steps = (int64_t)p.nb * p.step * heads > (1 << 17) ? 4 : 1;
-    const int64_t chunks = (p.nb + (int64_t)per * steps - 1) / (per * steps);
-    if (groups > 0xffffff || heads * p.step > 0xffffff || heads > 65535 || heads * p.step * chunks > 0xffffff) return TRN_E_SHAPE;
+    const bool many = p.nb > kMostBlocks;
+    const int64_t q_tiles = (p.step + 15) / 16, waves = heads * (p.nbp / 16) * q_tiles;
+    const int steps = many ? (waves > 4096 ? 4 : 1) : (int)(waves <= 2048 ? 1 : waves / 2048 < 8 ? waves / 2048 : 8);
+    const int per64 = 4 * 512 / c->head_dim * steps;
+    const dim3 score_grid((unsigned)(many ? (p.nb + (int64_t)per64 - 1) / per64 : p.nbp / 64), (unsigned)(many ? p.step : (q_tiles + steps - 1) / steps), (unsigned)heads);
+    const int threads = p.nb > 2048 && !many ? 1024 : 256;
+    if (groups > 0xffffff || heads > 65535 || heads * p.step * (threads / 256) > 0xffffff || (int64_t)score_grid.x * score_grid.y * score_grid.z > 0xffffff) return TRN_E_SHAPE;
     const hipStream_t s = (hipStream_t)stream;
     const bool d128 = c->head_dim == 128;
     hipError_t e = hipSuccess;
@@ -338,15 +659,30 @@ extern "C" int trn_cache_sparse_attn_f16(const trn_cache16* c, const void* bound
         a.q = (const half_t*)q; a.bounds = (const half_t*)bounds; a.lengths = c->lengths; a.counts = c->counts; a.scores = (float*)workspace; a.selected = selected;
         a.B = c->batch; a.Hkv = c->n_kv_heads; a.M = seq_q; a.cap = c->capacity; a.G = p.G; a.block_shift = shift_of(block); a.nb = p.nb;
         a.top = top; a.sink = sink; a.recent = recent; a.i0 = (int)i0; a.n = (int)(seq_q - i0 < p.step ? seq_q - i0 : p.step); a.steps = steps; a.nbp = p.nbp;
+        a.norms = (float*)((char*)workspace + p.norms);
         for (int i = 0; i < 3; ++i) a.qs[i] = q_stride[i];
         a.by_hkv = Div(c->n_kv_heads); a.by_n = Div(a.n);
         if (p.nb > top) {      // (a.n is at most 65535: 64 MB of at least 64 floats a query)
-            const dim3 grid((unsigned)chunks, (unsigned)a.n, (unsigned)heads);
-            if (d128) hipLaunchKernelGGL((cache_scores_kernel<128>), grid, dim3(256), 0, s, a);
-            else hipLaunchKernelGGL((cache_scores_kernel<64>), grid, dim3(256), 0, s, a);
+            dim3 grid = score_grid;
+            grid.y = (unsigned)(many ? a.n : ((a.n + 15) / 16 + steps - 1) / steps);
+            if (many) {
+                if (d128) hipLaunchKernelGGL((cache_scores64_kernel<128>), grid, dim3(256), 0, s, a);
+                else hipLaunchKernelGGL((cache_scores64_kernel<64>), grid, dim3(256), 0, s, a);
+            } else {
+                if (d128) hipLaunchKernelGGL((cache_scores_kernel<128>), grid, dim3(256), 0, s, a);
+                else hipLaunchKernelGGL((cache_scores_kernel<64>), grid, dim3(256), 0, s, a);
+            }
             if ((e = hipGetLastError()) != hipSuccess) break;
         }
-        hipLaunchKernelGGL(cache_select_kernel, dim3((unsigned)(heads * a.n)), dim3(256), 0, s, a);
+        const dim3 grid((unsigned)(heads * a.n));
+        if (many) hipLaunchKernelGGL(cache_select_many_kernel, grid, dim3(256), 0, s, a);
+        else if (d128) {
+            if (threads == 256) hipLaunchKernelGGL((cache_select_kernel<128, 256, 8>), grid, dim3(256), 0, s, a);
+            else hipLaunchKernelGGL((cache_select_kernel<128, 1024, 8>), grid, dim3(1024), 0, s, a);
+        } else {
+            if (threads == 256) hipLaunchKernelGGL((cache_select_kernel<64, 256, 8>), grid, dim3(256), 0, s, a);
+            else hipLaunchKernelGGL((cache_select_kernel<64, 1024, 8>), grid, dim3(1024), 0, s, a);
+        }
         e = hipGetLastError();
     }
     if (e != hipSuccess) return TRN_E_LAUNCH;
@@ -358,7 +694,15 @@ extern "C" int trn_cache_sparse_attn_f16(const trn_cache16* c, const void* bound
     a.parts = Parts{(float*)((char*)workspace + p.o), (float*)((char*)workspace + p.ml), p.ns};
     a.by_hkv = Div(c->n_kv_heads); a.by_b = Div(c->batch); a.by_ns = Div(p.ns); a.by_rt = Div(p.n_rt); a.by_w = Div(4 * p.ns);
     const dim3 grid((unsigned)groups), block3(256);
-    if (p.nq == 1) {
+    if (p.rows) {
+        if (p.nq == 1) {
+            if (d128) hipLaunchKernelGGL((cache_sparse_rows_kernel<128, 1>), grid, block3, 0, s, a);
+            else hipLaunchKernelGGL((cache_sparse_rows_kernel<64, 1>), grid, block3, 0, s, a);
+        } else {
+            if (d128) hipLaunchKernelGGL((cache_sparse_rows_kernel<128, 2>), grid, block3, 0, s, a);
+            else hipLaunchKernelGGL((cache_sparse_rows_kernel<64, 2>), grid, block3, 0, s, a);
+        }
+    } else if (p.nq == 1) {
         if (d128) hipLaunchKernelGGL((cache_sparse_attn_kernel<128, 1>), grid, block3, 0, s, a);
         else hipLaunchKernelGGL((cache_sparse_attn_kernel<64, 1>), grid, block3, 0, s, a);
     } else {
