@@ -3,8 +3,8 @@
 // The rows of a KV head are its query heads' queries, row r = (query r / G, head r % G): a tile of them reads a key once.  Two forms of a tile:
 //   narrow   16 or 32 rows; each of a workgroup's four waves has 32 keys of its own at a time, so that four times as many bytes are on their way; the waves' results are
 //            joined in LDS.  For few rows, which memory bounds.
-//   wide     128 rows, 32 a wave; the waves share 64 keys in LDS.  For many rows, which the matrix pipe bounds.
-// In both K and V come from memory straight into LDS, one stage ahead, scores are formed transposed, S^T = K Q^T, so that a lane's scores are the
+//   wide     128 rows, 32 a wave; the waves share the keys in LDS, 32 at a time.  For many rows, which the matrix pipe bounds.
+// In both K and V come from memory straight into LDS, ahead of their use, scores are formed transposed, S^T = K Q^T, so that a lane's scores are the
 // operand P^T of O^T += V^T P^T as they are, and V is read transposing.  One pass with a running maximum m, taken anew only where a score exceeds it by 2^8, and sum l.
 // A workgroup may have a share of a tile's keys: (m, l, O) of the shares of a row are joined by a second launch (cache16_join).
 #pragma once
@@ -15,8 +15,17 @@ namespace trn {
 // What became of a row's keys in one share: O unnormalised, and (m, l) with m in units of log2.  Row `row` of B Hkv M G has `slots` of them.
 struct Parts { float* o; float* ml; int slots; };
 
-constexpr int kNarrowLds(int D) { return 4 * 2 * 32 * D * 2; }
-constexpr int kWideLds(int D) { return 4 * 64 * D * 2; }
+// LDS of a workgroup: 32 keys of K and of V four times, a stage of a wide tile or of a wave's narrow one each.  They are arrays of their own: of one array the compiler takes each read to be of
+// what the loads on their way write, and waits for all of them.
+template <int D> struct Lds {
+    half_t *k0, *k1, *k2, *k3, *v0, *v1, *v2, *v3;
+    __device__ __forceinline__ half_t* k(int i) const { return i == 0 ? k0 : i == 1 ? k1 : i == 2 ? k2 : k3; }
+    __device__ __forceinline__ half_t* v(int i) const { return i == 0 ? v0 : i == 1 ? v1 : i == 2 ? v2 : v3; }
+};
+#define TRN_LDS(D, name)                                                                                                                        \
+    __shared__ __attribute__((aligned(1024))) half_t name##_k0[32 * D], name##_k1[32 * D], name##_k2[32 * D], name##_k3[32 * D], name##_v0[32 * D], \
+        name##_v1[32 * D], name##_v2[32 * D], name##_v3[32 * D];                                                                              \
+    const Lds<D> name{name##_k0, name##_k1, name##_k2, name##_k3, name##_v0, name##_v1, name##_v2, name##_v3}
 
 #if defined(__HIP_DEVICE_COMPILE__)
 __device__ __forceinline__ float4_t mfma16(half8_t a, half8_t b, float4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
@@ -60,12 +69,10 @@ __device__ __forceinline__ half8_t finite_only(half8_t v) {
 // One wave's tiles t0 <= t < t1, every STEP-th, of 32 keys for 16 NQ rows (queries in qB), into o, m, l.  `keys`: where the tile t begins and how many of its keys there are (0..32, wave-uniform; those
 // from there on arrive as zeros and count for no row), as .k(t), .v(t), .n(t), requested in order.  Keys from `last` on (relative to the tile, through .at(t)) are hidden from a row.
 template <int D, int NQ, int STEP, class Keys>
-__device__ __forceinline__ void narrow_walk(Keys& keys, int t0, int t1, int t_mask, int kpitch, int vpitch, float c, const half8_t (&qB)[NQ][D / 32], const int (&last)[NQ], char* lds,
+__device__ __forceinline__ void narrow_walk(Keys& keys, int t0, int t1, int t_mask, int kpitch, int vpitch, float c, const half8_t (&qB)[NQ][D / 32], const int (&last)[NQ], half_t* Kt, half_t* Vt,
                                             float4_t (&o)[D / 16][NQ], float (&m)[NQ], float (&l)[NQ]) {
-    constexpr int NI = D / 32, NDB = D / 16, TILE = 32 * D, RPI = 512 / D, NL = 32 / RPI, CPR = D / 8;
+    constexpr int NI = D / 32, NDB = D / 16, RPI = 512 / D, NL = 32 / RPI, CPR = D / 8;
     const int lane = threadIdx.x & 63, n = lane & 15, g4 = lane >> 4;
-    half_t* const Kt = reinterpret_cast<half_t*>(lds);
-    half_t* const Vt = Kt + TILE;
     // staging: load i covers the rows RPI i + lane / CPR; swizzles repeat every other (or second other) load
     const int sr = lane / CPR, sc = lane % CPR;
     int k_off[2], v_off[2];
@@ -214,7 +221,7 @@ __device__ __forceinline__ void narrow_walk(Keys& keys, int t0, int t1, int t_ma
 // The results of a row tile's four waves, joined and delivered: row i of the tile by put(i, first dimension, O, m, l, whether this is the row's first piece).
 struct NarrowStats { float m[4][32], l[4][32], m_all[32], l_all[32]; };
 template <int D, int NQ, class Put>
-__device__ __forceinline__ void narrow_join(char* lds, NarrowStats& st, float4_t (&o)[D / 16][NQ], float (&m)[NQ], float (&l)[NQ], Put put) {
+__device__ __forceinline__ void narrow_join(const Lds<D>& lds, NarrowStats& st, float4_t (&o)[D / 16][NQ], float (&m)[NQ], float (&l)[NQ], Put put) {
     constexpr int NDB = D / 16, RT = 16 * NQ;
     const int lane = threadIdx.x & 63, n = lane & 15, g4 = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
@@ -223,9 +230,7 @@ __device__ __forceinline__ void narrow_join(char* lds, NarrowStats& st, float4_t
         if (g4 == 0) { st.m[wave][16 * qb + n] = m[qb]; st.l[wave][16 * qb + n] = l[qb]; }
     }
     __syncthreads();
-    // (a wave's stage holds its RT rows of D floats; the 16-byte pieces of a row are swizzled by the row)
-    constexpr int AREA = 2 * 32 * D * 2;
-    float4_t* const mem = reinterpret_cast<float4_t*>(lds + wave * AREA);
+    // (a wave's stage of K, and of V, holds 16 rows of D floats; the 16-byte pieces of a row are swizzled by the row)
 #pragma unroll
     for (int qb = 0; qb < NQ; ++qb) {
         const int r = 16 * qb + n;
@@ -236,7 +241,7 @@ __device__ __forceinline__ void narrow_join(char* lds, NarrowStats& st, float4_t
         for (int i = 0; i < 4; ++i) sum = __builtin_fmaf(st.l[i][r], st.m[i][r] == -INFINITY ? 0.f : fast_exp2(st.m[i][r] - top), sum);      // (a sum of NaN stays)
         const float mine = m[qb] == -INFINITY ? 0.f : fast_exp2(m[qb] - top);
 #pragma unroll
-        for (int i = 0; i < NDB; ++i) mem[r * (D / 4) + ((4 * i + g4) ^ n)] = o[i][qb] * mine;
+        for (int i = 0; i < NDB; ++i) reinterpret_cast<float4_t*>(qb ? lds.v(wave) : lds.k(wave))[n * (D / 4) + ((4 * i + g4) ^ n)] = o[i][qb] * mine;
         if (wave == 0 && g4 == 0) { st.m_all[r] = top; st.l_all[r] = sum; }
     }
     __syncthreads();
@@ -247,56 +252,87 @@ __device__ __forceinline__ void narrow_join(char* lds, NarrowStats& st, float4_t
         const int piece = sub + i * TPR;
         float4_t x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x = x + reinterpret_cast<const float4_t*>(lds + k * AREA)[row * (D / 4) + (piece ^ (row & 15))];
+        for (int k = 0; k < 4; ++k) x = x + reinterpret_cast<const float4_t*>(row >= 16 ? lds.v(k) : lds.k(k))[(row & 15) * (D / 4) + (piece ^ (row & 15))];
         put(row, 4 * piece, x, st.m_all[row], st.l_all[row], piece == 0);
     }
 }
 
 // ------------------------------------------------------------------------------------------------ wide
-// A workgroup's tiles t0 <= t < t1 of 64 keys for 128 rows, of which this wave has 32 (none: idle).  keys as above; .lim(t, last): up to which key of the tile a row sees.
+// A workgroup's tiles t0 <= t < t1 of 32 keys for 128 rows, of which this wave has 32 (none: idle).  keys: where a tile begins (.k, .v),
+// the pitches there, how many keys lie from there on at these (.left), whether tiles are there as a whole (.whole), and up to which key of a tile a row sees (.lim).
+// Four stages: a tile is requested three tiles ahead, so that a workgroup alone on its compute unit has 48 KB on their way.
 template <int D, class Keys>
-__device__ __forceinline__ void wide_walk(const Keys& keys, int t0, int t1, int t_mask, bool idle, float c, const half8_t (&qB)[D / 16], int last, char* lds, float16_t (&o)[D / 32], float& m, float& l) {
-    constexpr int NS = D / 16, NDB = D / 32, CPR = D / 8, RPI = 64 / CPR, NL = 64 / (4 * RPI), STAGE = 64 * D;
+__device__ __forceinline__ void wide_walk(const Keys& keys, int t0, int t1, int t_mask, bool idle, float c, const half8_t (&qB)[D / 16], int last, const Lds<D>& lds, float16_t (&o)[D / 32], float& m, float& l) {
+    constexpr int NS = D / 16, NDB = D / 32, CPR = D / 8, RPI = 64 / CPR, NL = 32 / (4 * RPI);
     const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    half_t* const base = reinterpret_cast<half_t*>(lds);      // K of both stages, then V
+    if (t0 >= t1) return;
     const int sr = wave * RPI + lane / CPR, sc = ((lane % CPR) ^ swz<D>(sr)) << 4;
     int kr[NS], vr[2];
 #pragma unroll
-    for (int i = 0; i < NS; ++i) kr[i] = n * D + (((2 * i + h) ^ swz<D>(n)) << 3);
+    for (int i = 0; i < NS; ++i) kr[i] = 2 * n * D + (((2 * i + h) ^ swz<D>(n)) << 4);       // (in bytes)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int e = lane & 15, key = 8 * i + 4 * h + (e >> 2);
-        vr[i] = key * D + (((2 * (lane >> 4 & 1) + ((e & 3) >> 1)) ^ swz<D>(key)) << 3) + 4 * (e & 1);
+        vr[i] = 2 * key * D + (((2 * (lane >> 4 & 1) + ((e & 3) >> 1)) ^ swz<D>(key)) << 4) + 8 * (e & 1);
     }
+    auto in = [](const half_t* p, int bytes) __attribute__((always_inline)) { return reinterpret_cast<const half_t*>(reinterpret_cast<const char*>(p) + bytes); };
     float16_t zero;
 #pragma unroll
     for (int e = 0; e < 16; ++e) zero[e] = 0.f;
 
-    auto ahead = [&](int t, int stage) __attribute__((always_inline)) {
-        const int there = keys.n(t), kpitch = keys.kpitch(t), vpitch = keys.vpitch(t);
-        const __amdgpu_buffer_rsrc_t ks = __builtin_amdgcn_make_buffer_rsrc((void*)keys.k(t), 0, there ? ((there - 1) * kpitch + D) * 2 : 0, 0x00020000);
-        const __amdgpu_buffer_rsrc_t vs = __builtin_amdgcn_make_buffer_rsrc((void*)keys.v(t), 0, there ? ((there - 1) * vpitch + D) * 2 : 0, 0x00020000);
-        fetch_tile<NL, D, 4>(ks, base + stage * STAGE + wave * RPI * D, sr * kpitch * 2 + sc, 0, RPI * kpitch * 2);
-        fetch_tile<NL, D, 4>(vs, base + (2 + stage) * STAGE + wave * RPI * D, sr * vpitch * 2 + sc, 0, RPI * vpitch * 2);
+    // Tiles are requested one after the other: pointers, pitches and how many keys there are move along (formed anew for each tile they were 30 scalar instructions a step).
+    const half_t *kp = keys.k(t0), *vp = keys.v(t0);
+    int kpitch = keys.kpitch(t0), vpitch = keys.vpitch(t0), keys_left = keys.left(t0), tiles_left = t1 - t0;
+    int k_off = sr * kpitch * 2 + sc, v_off = sr * vpitch * 2 + sc;
+    auto ahead = [&](half_t* Kt, half_t* Vt) __attribute__((always_inline)) {
+        // (none: nothing is read, zeros arrive, and the loads on their way are as many as ever)
+        const int last_row = min(32, keys_left) - 1;
+        const __amdgpu_buffer_rsrc_t ks = __builtin_amdgcn_make_buffer_rsrc((void*)kp, 0, tiles_left > 0 ? (last_row * kpitch + D) * 2 : 0, 0x00020000);
+        const __amdgpu_buffer_rsrc_t vs = __builtin_amdgcn_make_buffer_rsrc((void*)vp, 0, tiles_left > 0 ? (last_row * vpitch + D) * 2 : 0, 0x00020000);
+        fetch_tile<NL, D, 4>(ks, Kt + wave * RPI * D, k_off, 0, RPI * kpitch * 2);
+        fetch_tile<NL, D, 4>(vs, Vt + wave * RPI * D, v_off, 0, RPI * vpitch * 2);
+        kp += (int64_t)32 * kpitch; vp += (int64_t)32 * vpitch;
+        keys_left -= 32; --tiles_left;
+        if (__builtin_expect(keys_left <= 0 && tiles_left > 0, 0)) {
+            const int t = t1 - tiles_left;
+            kp = keys.k(t); vp = keys.v(t); kpitch = keys.kpitch(t); vpitch = keys.vpitch(t); keys_left = keys.left(t);
+            k_off = sr * kpitch * 2 + sc; v_off = sr * vpitch * 2 + sc;
+        }
     };
-    auto step = [&](auto mask_tag, int t, int stage) __attribute__((always_inline)) {
+    auto step = [&](auto mask_tag, int t, const half_t* Kt, const half_t* Vt) __attribute__((always_inline)) {
         constexpr bool MASK = decltype(mask_tag)::value;
-        const half_t* const Kt = base + stage * STAGE;
-        const half_t* const Vt = base + (2 + stage) * STAGE;
-        float16_t s[2];
+        // (addresses are formed here, of these and a stage's constant: hoisted out of the loop those of all stages would take 64 registers)
 #pragma unroll
-        for (int i = 0; i < NS; ++i)
+        for (int i = 0; i < NS; ++i) asm volatile("" : "+v"(kr[i]));
+        asm volatile("" : "+v"(vr[0]), "+v"(vr[1]));
+        // (what is read is requested at once: left to the compiler each read came right before its product, and was waited for)
+        half8_t kw[NS], vw[2][NDB];
+        auto value = [&](int u, int i) __attribute__((always_inline)) {       // of the keys 16 u + (0..3, 8..11) + 4 h, for one dimension
+            const half4_t x = lds_read_tr16(in(Vt + u * 16 * D, vr[0] ^ (i << 6))), y = lds_read_tr16(in(Vt + u * 16 * D, vr[1] ^ (i << 6)));
+            return half8_t{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+        };
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb) s[kb] = mfma32(*reinterpret_cast<const half8_t*>(Kt + kb * 32 * D + kr[i]), qB[i], i == 0 ? zero : s[kb]);
+        for (int i = 0; i < NS; ++i) kw[i] = *reinterpret_cast<const half8_t*>(in(Kt, kr[i]));
+        if constexpr (!MASK) {
+#pragma unroll
+            for (int i = 0; i < NDB; ++i) vw[0][i] = value(0, i);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        float16_t s;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) s = mfma32(kw[i], qB[i], i == 0 ? zero : s);
+        if constexpr (!MASK) {
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < NDB; ++i) vw[1][i] = value(1, i);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         if constexpr (MASK) {
             const int lim = keys.lim(t, last) - 4 * h;
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) s[kb][e] = 32 * kb + 8 * (e >> 2) + (e & 3) <= lim ? s[kb][e] : -INFINITY;
+            for (int e = 0; e < 16; ++e) s[e] = 8 * (e >> 2) + (e & 3) <= lim ? s[e] : -INFINITY;
         }
-        __builtin_amdgcn_sched_barrier(0);
-        const float tm = fmaxf(max16(s[0]), max16(s[1])) * c;
+        const float tm = max16(s) * c;
         if (__builtin_expect(__builtin_amdgcn_ballot_w64(tm > m + 8.f) != 0, 0)) {
             const float up = fmaxf(m, half_max(tm)), alpha = up == -INFINITY ? 1.f : fast_exp2(m - up);
             m = up;
@@ -305,32 +341,26 @@ __device__ __forceinline__ void wide_walk(const Keys& keys, int t0, int t1, int 
             for (int i = 0; i < NDB; ++i) o[i] = o[i] * alpha;
         }
         const float d = m == -INFINITY ? 0.f : -m;
-        half8_t p[4];
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        half8_t p[2];
+        float sum[4];
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const float x = fast_exp2(__builtin_fmaf(s[kb][e], c, d));
-                sum[e & 3] += x;
-                p[2 * kb + (e >> 3)][e & 7] = (half_t)x;
-            }
+        for (int e = 0; e < 16; ++e) {
+            const float x = fast_exp2(__builtin_fmaf(s[e], c, d));
+            sum[e & 3] = e < 4 ? x : sum[e & 3] + x;
+            p[e >> 3][e & 7] = (half_t)x;
+        }
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        auto value = [&](int u, int i) __attribute__((always_inline)) {       // of the keys 16 u + (0..3, 8..11) + 4 h, for one dimension
-            const half4_t x = lds_read_tr16(Vt + u * 16 * D + (vr[0] ^ (i << 5))), y = lds_read_tr16(Vt + u * 16 * D + (vr[1] ^ (i << 5)));
-            return half8_t{x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-        };
         bool odd = false;
         if constexpr (MASK) {               // (as in the narrow form)
             bool bad = false;
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
+            for (int u = 0; u < 2; ++u)
 #pragma unroll
                 for (int i = 0; i < NDB; ++i) { bad = bad || odd_values(value(u, i)); __builtin_amdgcn_sched_barrier(0); }
             odd = __builtin_amdgcn_ballot_w64(bad) != 0;
             if (__builtin_expect(odd, 0)) {
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
+                for (int u = 0; u < 2; ++u) {
                     const int lim = keys.lim(t, last) - 16 * u - 4 * h;
                     half8_t see;
 #pragma unroll
@@ -347,25 +377,36 @@ __device__ __forceinline__ void wide_walk(const Keys& keys, int t0, int t1, int 
             }
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int i = 0; i < NDB; ++i) {
-                half8_t v = value(u, i);
-                if (MASK && __builtin_expect(odd, 0)) v = finite_only(v);
+                half8_t v;
+                if constexpr (MASK) { v = value(u, i); if (__builtin_expect(odd, 0)) v = finite_only(v); }
+                else v = vw[u][i];
                 o[i] = mfma32(v, p[u], o[i]);
             }
     };
-    if (t0 >= t1) return;
-    ahead(t0, 0);
-    for (int t = t0; t < t1; ++t) {
-        // (the wave's pieces of tile t are there; behind the barrier everyone's are, and everyone is done with tile t - 1)
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        const int stage = (t - t0) & 1;
-        if (t + 1 < t1) ahead(t + 1, stage ^ 1);
-        if (idle) continue;
-        if (t < t_mask && keys.n(t) == 64) step(std::false_type{}, t, stage);
-        else step(std::true_type{}, t, stage);
+    ahead(lds.k0, lds.v0); ahead(lds.k1, lds.v1); ahead(lds.k2, lds.v2);
+    // (the wave's pieces of tile t are there; behind the barrier everyone's are, and everyone is done with tile t - 1, whose stage is the next one's)
+    auto arrived = [&] {
+        if constexpr (D == 128) asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(4) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    };
+    for (int t = t0; t < t1; t += 4) {
+        for (; t + 4 <= min(t1, t_mask) && keys.whole(t, t + 4); t += 4) {
+            arrived(); ahead(lds.k3, lds.v3); if (!idle) step(std::false_type{}, t, lds.k0, lds.v0);
+            arrived(); ahead(lds.k0, lds.v0); if (!idle) step(std::false_type{}, t + 1, lds.k1, lds.v1);
+            arrived(); ahead(lds.k1, lds.v1); if (!idle) step(std::false_type{}, t + 2, lds.k2, lds.v2);
+            arrived(); ahead(lds.k2, lds.v2); if (!idle) step(std::false_type{}, t + 3, lds.k3, lds.v3);
+        }
+#pragma unroll 1
+        for (int i = 0; i < 4 && t + i < t1; ++i) {
+            arrived();
+            ahead(lds.k((i + 3) & 3), lds.v((i + 3) & 3));
+            if (!idle) step(std::true_type{}, t + i, lds.k(i), lds.v(i));
+        }
     }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 #endif
 

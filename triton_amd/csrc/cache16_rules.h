@@ -21,7 +21,7 @@ inline PlanPrefix plan_prefix(int batch, int n_kv_heads, int capacity, int head_
         p.wide = true; p.nq = 2;
         p.n_rt_p = (p.R + 127) / 128;
         const int64_t units = heads * p.n_rt_p, tiles = ((int64_t)prefix + 63) / 64 + (capacity + 63) / 64;
-        int64_t ns = 512 / units;
+        int64_t ns = (head_dim == 128 ? 512 : 1024) / units;      // (two workgroups a compute unit, four of head_dim 64)
         if (ns > tiles / 4) ns = tiles / 4;
         p.ns_p = (int)(ns < 1 ? 1 : ns > 32 ? 32 : ns);
         p.slots = p.ns_p;
@@ -32,13 +32,16 @@ inline PlanPrefix plan_prefix(int batch, int n_kv_heads, int capacity, int head_
         p.n_rt_p = (int)(p.wide ? (rows_p + 127) / 128 : (rows_p + 16 * p.nq - 1) / (16 * p.nq));
         p.n_rt_o = (p.R + 16 * p.nq - 1) / (16 * p.nq);
         const int64_t units_p = (int64_t)n_kv_heads * p.n_rt_p, units_o = heads * p.n_rt_o;
-        // (as many keys a workgroup as make two workgroups a compute unit; 256 at least)
-        const int64_t groups = 512, all = units_p * prefix + units_o * capacity;
-        int64_t each = (all + groups - 1) / groups;
-        if (each < 256) each = 256;
-        auto shares = [&](int64_t n) { const int64_t s = (n + each - 1) / each; return (int)(s > 64 ? 64 : s); };
-        p.ns_p = shares(prefix);
-        p.ns_o = shares(capacity);
+        // Workgroups of both parts run at once, two a compute unit: these are shared out by the parts' work (a wide tile's key counts twice), in shares of 256 keys at least, 512 of a wide
+        // tile.  32 sequences of 700 keys behind 8192, 32 heads of 128 on 8, us with 8 / 16 / 32 shares of the prefix: 31.6 + 4.8 for the joining / 24.9 + 4.8 / 27.6 + 5.9.
+        const int64_t cost_p = units_p * prefix * (p.wide ? 2 : 1), cost_o = units_o * capacity, cost = cost_p + cost_o;
+        auto shares = [](int64_t groups, int64_t units, int64_t keys, int64_t least) {
+            int64_t s = groups / units;
+            if (s > keys / least) s = keys / least;
+            return (int)(keys == 0 ? 0 : s < 1 ? 1 : s > 64 ? 64 : s);
+        };
+        p.ns_p = shares(cost ? 512 * cost_p / cost : 0, units_p, prefix, p.wide ? 512 : 256);
+        p.ns_o = shares(cost ? 512 * cost_o / cost : 0, units_o, capacity, 256);
         if (p.ns_p + p.ns_o == 0) p.ns_o = 1;      // (nothing to see: zeros)
         p.slots = p.ns_p + p.ns_o;
         p.first = units_p * p.ns_p; p.second = units_o * p.ns_o;

@@ -31,12 +31,13 @@ struct Run {
 // ... of the prefix, `split` tiles, and of the sequence behind them.
 struct TwoRuns {
     const half_t *kp, *vp, *ko, *vo; int kpp, vpp, kpo, vpo, P, L, split;
-    __device__ __forceinline__ const half_t* k(int t) const { return t < split ? kp + (int64_t)t * 64 * kpp : ko + (int64_t)(t - split) * 64 * kpo; }
-    __device__ __forceinline__ const half_t* v(int t) const { return t < split ? vp + (int64_t)t * 64 * vpp : vo + (int64_t)(t - split) * 64 * vpo; }
+    __device__ __forceinline__ const half_t* k(int t) const { return t < split ? kp + (int32_t)t * 32 * kpp : ko + (int32_t)(t - split) * 32 * kpo; }
+    __device__ __forceinline__ const half_t* v(int t) const { return t < split ? vp + (int32_t)t * 32 * vpp : vo + (int32_t)(t - split) * 32 * vpo; }
     __device__ __forceinline__ int kpitch(int t) const { return t < split ? kpp : kpo; }
     __device__ __forceinline__ int vpitch(int t) const { return t < split ? vpp : vpo; }
-    __device__ __forceinline__ int n(int t) const { return t < split ? min(64, P - 64 * t) : min(64, L - 64 * (t - split)); }
-    __device__ __forceinline__ int lim(int t, int last) const { return t < split ? P - 1 - 64 * t : last - 64 * (t - split); }
+    __device__ __forceinline__ int left(int t) const { return t < split ? P - 32 * t : L - 32 * (t - split); }
+    __device__ __forceinline__ bool whole(int t, int to) const { return !(P & 31) || to < split || t >= split; }      // but for those that do not all see it
+    __device__ __forceinline__ int lim(int t, int last) const { return t < split ? P - 1 - 32 * t : last - 32 * (t - split); }
 };
 // A row's result, piece by piece: to the output, or to the row's slot.
 template <int D> __device__ __forceinline__ void put(const PrefixArgs& a, int slot, int b, int kvh, int r, int d0, float4_t x, float m, float l, bool once) {
@@ -61,17 +62,17 @@ __device__ __forceinline__ const half_t* query(const PrefixArgs& a, int b, int k
 
 // Tiles of 128 rows of one sequence, over the prefix and its own keys.
 template <int D>
-__global__ __launch_bounds__(256, 2) void cache_prefix_rows_kernel(const PrefixArgs a) {
+__global__ __launch_bounds__(256, D == 128 ? 2 : 4) void cache_prefix_rows_kernel(const PrefixArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    __shared__ __attribute__((aligned(1024))) char lds[kWideLds(D)];
+    TRN_LDS(D, lds);
     const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // (a KV head's workgroups follow each other at the distance of all KV heads: one XCD where those are a multiple of eight; the last rows, which see the most keys, first)
     const int x = a.by_hkv.of(blockIdx.x), kvh = blockIdx.x - x * a.Hkv, y = a.by_b.of(x), b = x - y * a.B, z = a.by_nsp.of(y), share = y - z * a.ns_p, rt = a.n_rt_p - 1 - z;
     const int L = length_of(a.lengths, b, a.cap), C = count_of(a.counts, b, a.M), rows = C * a.G, off = L - C;
     if (rt * 128 >= rows) return;
     auto sees = [&](int r) { return a.causal ? min(L, max(0, a.by_g.of(r) + off + 1)) : L; };      // own keys that a row sees
-    const int r0 = rt * 128 + wave * 32, row = r0 + n, split = (a.P + 63) >> 6;
-    const int T = split + ((sees(min(rt * 128 + 127, rows - 1)) + 63) >> 6);
+    const int r0 = rt * 128 + wave * 32, row = r0 + n, split = (a.P + 31) >> 5;
+    const int T = split + ((sees(min(rt * 128 + 127, rows - 1)) + 31) >> 5);
     const int t0 = a.by_wp.of(T * share), t1 = a.by_wp.of(T * (share + 1));
     half8_t qB[D / 16];
     const half_t* const qp = query(a, b, kvh, min(row, rows - 1));
@@ -85,7 +86,7 @@ __global__ __launch_bounds__(256, 2) void cache_prefix_rows_kernel(const PrefixA
     for (int i = 0; i < D / 32; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
-    wide_walk<D>(keys, t0, t1, split + (sees(min(r0, rows - 1)) >> 6), r0 >= rows, a.c, qB, sees(min(row, rows - 1)) - 1, lds, o, m, l);
+    wide_walk<D>(keys, t0, t1, split + (sees(min(r0, rows - 1)) >> 5), r0 >= rows, a.c, qB, sees(min(row, rows - 1)) - 1, lds, o, m, l);
     if (row >= rows) return;
     l = half_sum(l);
 #pragma unroll
@@ -100,7 +101,7 @@ __global__ __launch_bounds__(256, 2) void cache_prefix_rows_kernel(const PrefixA
 template <int D, int NQ, bool WIDE>
 __global__ __launch_bounds__(256, 2) void cache_prefix_parts_kernel(const PrefixArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    __shared__ __attribute__((aligned(1024))) char lds[kNarrowLds(D)];
+    TRN_LDS(D, lds);
     __shared__ NarrowStats stats;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const bool prefix = (int)blockIdx.x < a.first;
@@ -119,7 +120,7 @@ __global__ __launch_bounds__(256, 2) void cache_prefix_parts_kernel(const Prefix
             qB[i] = there ? y : z;
         }
         const half_t *const kp = a.kp + kvh * a.kps[0], *const vp = a.vp + kvh * a.vps[0];
-        const int T = (a.P + 63) >> 6;
+        const int T = (a.P + 31) >> 5;
         const TwoRuns keys{kp, vp, kp, vp, (int)a.kps[1], (int)a.vps[1], (int)a.kps[1], (int)a.vps[1], a.P, 0, T};
         float16_t o[D / 32];
         float m = -INFINITY, l = 0.f;
@@ -178,7 +179,7 @@ __global__ __launch_bounds__(256, 2) void cache_prefix_parts_kernel(const Prefix
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) o[i][qb] = float4_t{0.f, 0.f, 0.f, 0.f};
     }
-    narrow_walk<D, NQ, 1>(keys, t0, t1, min(t1, max(t0, sees(rt * RT) >> 5)), keys.kpitch, keys.vpitch, a.c, qB, last, lds + wave * 2 * 32 * D * 2, o, m, l);
+    narrow_walk<D, NQ, 1>(keys, t0, t1, min(t1, max(t0, sees(rt * RT) >> 5)), keys.kpitch, keys.vpitch, a.c, qB, last, lds.k(wave), lds.v(wave), o, m, l);
     narrow_join<D, NQ>(lds, stats, o, m, l, [&](int i, int d0, float4_t v, float mm, float ll, bool once) __attribute__((always_inline)) {
         const int row = rt * RT + i;
         if (row >= all) return;
@@ -190,26 +191,59 @@ __global__ __launch_bounds__(256, 2) void cache_prefix_parts_kernel(const Prefix
 }
 
 // ------------------------------------------------------------------------------------------------ joining
-// D / 4 threads a row.
+// D / 4 threads a row and `sg` groups of them, each with every sg-th slot.
 template <int D>
-__global__ __launch_bounds__(256) void cache16_join_kernel(const JoinArgs a) {
+__global__ __launch_bounds__(256) void cache16_join_kernel(const JoinArgs a, int sg) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    constexpr int TPR = D / 4;
-    const int at = blockIdx.x * (256 / TPR) + threadIdx.x / TPR, piece = threadIdx.x % TPR;
-    if (at >= a.rows) return;
-    const int bm = a.by_g.of(at), g = at - bm * a.G, bh = a.by_m.of(bm), i = bm - bh * a.M, b = a.by_hkv.of(bh), kvh = bh - b * a.Hkv;
-    if (i >= count_of(a.counts, b, a.M)) return;
-    const float2_t* const ml = reinterpret_cast<const float2_t*>(a.parts.ml) + (int64_t)at * a.parts.slots;
-    const float* const po = a.parts.o + (int64_t)at * a.parts.slots * D + 4 * piece;
+    constexpr int TPR = D / 4, GROUPS = 256 / TPR, AHEAD = 4;
+    __shared__ float4_t red[256];
+    __shared__ float2_t stat[GROUPS];
+    const int grp = threadIdx.x / TPR, piece = threadIdx.x % TPR, nth = grp & (sg - 1), at = blockIdx.x * (GROUPS / sg) + grp / sg, row = min(at, a.rows - 1), slots = a.parts.slots;
+    const float2_t* const ml = reinterpret_cast<const float2_t*>(a.parts.ml) + (int64_t)row * slots;
+    const float* const po = a.parts.o + (int64_t)row * slots * D + 4 * piece;
     float top = -INFINITY, sum = 0.f;
-    for (int s = 0; s < a.parts.slots; ++s) top = fmaxf(top, ml[s].x);
     float4_t x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int s = 0; s < a.parts.slots; ++s) {
-        const float f = ml[s].x == -INFINITY ? 0.f : fast_exp2(ml[s].x - top);
-        sum = __builtin_fmaf(ml[s].y, f, sum);                 // (a sum of NaN stays)
-        x = x + *reinterpret_cast<const float4_t*>(po + (int64_t)s * D) * f;
+    // (a thread's next four slots are requested at once, with their statistics, and joined to what there is so far)
+    for (int s0 = nth; s0 < slots; s0 += AHEAD * sg) {
+        float2_t st[AHEAD];
+        float4_t got[AHEAD];
+#pragma unroll
+        for (int e = 0; e < AHEAD; ++e) {
+            const int s = min(s0 + e * sg, slots - 1);
+            st[e] = ml[s];
+            got[e] = *reinterpret_cast<const float4_t*>(po + (int64_t)s * D);
+        }
+        float up = top;
+#pragma unroll
+        for (int e = 0; e < AHEAD; ++e) up = fmaxf(up, st[e].x);
+        const float alpha = top == -INFINITY ? 0.f : fast_exp2(top - up);
+        sum *= alpha; x = x * alpha; top = up;
+#pragma unroll
+        for (int e = 0; e < AHEAD; ++e) {
+            if (s0 + e * sg >= slots) break;
+            const float f = st[e].x == -INFINITY ? 0.f : fast_exp2(st[e].x - top);
+            sum = __builtin_fmaf(st[e].y, f, sum);                 // (a sum of NaN stays)
+            x = x + got[e] * f;
+        }
     }
+    const int bm = a.by_g.of(row), g = row - bm * a.G, bh = a.by_m.of(bm), i = bm - bh * a.M, b = a.by_hkv.of(bh), kvh = bh - b * a.Hkv;
+    const bool there = at < a.rows && i < count_of(a.counts, b, a.M);
+    if (sg > 1) {
+        red[threadIdx.x] = x;
+        if (piece == 0) stat[grp] = float2_t{top, sum};
+        __syncthreads();
+        if (nth != 0) return;
+        float up = top;
+        for (int k = 1; k < sg; ++k) up = fmaxf(up, stat[grp + k].x);
+        float f = top == -INFINITY ? 0.f : fast_exp2(top - up);
+        sum *= f; x = x * f;
+        for (int k = 1; k < sg; ++k) {
+            f = stat[grp + k].x == -INFINITY ? 0.f : fast_exp2(stat[grp + k].x - up);
+            sum = __builtin_fmaf(stat[grp + k].y, f, sum);
+            x = x + red[threadIdx.x + k * TPR] * f;
+        }
+    }
+    if (!there) return;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     half4_t y;
 #pragma unroll
@@ -219,9 +253,10 @@ __global__ __launch_bounds__(256) void cache16_join_kernel(const JoinArgs a) {
 }
 
 hipError_t launch_cache16_join(const JoinArgs& a, int head_dim, hipStream_t s) {
-    const unsigned per = 1024 / head_dim, grid = ((unsigned)a.rows + per - 1) / per;
-    if (head_dim == 128) hipLaunchKernelGGL((cache16_join_kernel<128>), dim3(grid), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((cache16_join_kernel<64>), dim3(grid), dim3(256), 0, s, a);
+    const int groups = 1024 / head_dim, sg = a.parts.slots > 4 ? groups < 8 ? groups : 8 : 1;
+    const unsigned per = groups / sg, grid = ((unsigned)a.rows + per - 1) / per;
+    if (head_dim == 128) hipLaunchKernelGGL((cache16_join_kernel<128>), dim3(grid), dim3(256), 0, s, a, sg);
+    else hipLaunchKernelGGL((cache16_join_kernel<64>), dim3(grid), dim3(256), 0, s, a, sg);
     return hipGetLastError();
 }
 

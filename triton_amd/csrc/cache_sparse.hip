@@ -70,29 +70,60 @@ template <int CTRL> __device__ __forceinline__ double moved64(double x) {
     const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xf, 0xf, true), hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xf, 0xf, true);
     return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
+template <int CTRL, int ROWS = 0xf> __device__ __forceinline__ uint32_t moved32(uint32_t x) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, true); }
+template <int CTRL> __device__ __forceinline__ float rotated(float x) { return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true)); }
+// Over 16 lanes, by rotations.
+__device__ __forceinline__ float row_max(float x) {
+    x = fmaxf(x, rotated<0x121>(x));
+    x = fmaxf(x, rotated<0x122>(x));
+    x = fmaxf(x, rotated<0x124>(x));
+    return fmaxf(x, rotated<0x128>(x));
+}
+// x of this lane and those below it, of an operation that zero leaves as it is; all of them in the last lane.
+template <class F> __device__ __forceinline__ uint32_t scan64(uint32_t x, F f) {
+    x = f(x, moved32<0x111>(x));       // row_shr:1, 2, 4, 8
+    x = f(x, moved32<0x112>(x));
+    x = f(x, moved32<0x114>(x));
+    x = f(x, moved32<0x118>(x));
+    x = f(x, moved32<0x142, 0xa>(x));  // the first and third row's last lane to the rows behind them
+    return f(x, moved32<0x143, 0xc>(x));
+}
+template <class F> __device__ __forceinline__ uint32_t all64(uint32_t x, F f) { return (uint32_t)__builtin_amdgcn_readlane((int)scan64(x, f), 63); }
+struct Or { __device__ __forceinline__ uint32_t operator()(uint32_t x, uint32_t y) const { return x | y; } };
+struct Add { __device__ __forceinline__ uint32_t operator()(uint32_t x, uint32_t y) const { return x + y; } };
+struct Max { __device__ __forceinline__ uint32_t operator()(uint32_t x, uint32_t y) const { return max(x, y); } };
 // Scores as whole numbers of the same order; NaN is zero, the least.
 __device__ __forceinline__ uint32_t ordered(float x) {
     const uint32_t u = __float_as_uint(x);
     return x != x ? 0u : u ^ (u >> 31 ? 0xffffffffu : 0x80000000u);
 }
+__device__ __forceinline__ float unordered(uint32_t u) { return __uint_as_float(u >> 31 ? u ^ 0x80000000u : ~u); }
 #endif
 
-// Scores by the matrix pipe.  A wave has 16 blocks, whose bounds it holds as operands (lane 16 g + n: block n, channels 8 g..+7 of each 32), and goes through its queries, 16 at a
-// time and their heads one after the other, so that the largest over the heads stays in a lane.  norms: the largest |bound| vector (of each channel's larger end) of every 16 blocks, squared;
-// infinite where a bound is not finite.
-template <int D>
+// Scores by the matrix pipe.  A wave has 16 blocks, whose bounds it holds as operands (lane 16 g + n: block n, channels 8 g..+7 of each 32).  HEADS: a query's heads are the other operand,
+// 16 at a time, and their largest is taken over lanes; otherwise 16 queries are, their heads one after the other, and the largest stays in a lane.  norms: the largest |bound| vector (of each
+// channel's larger end) of every 16 blocks, squared; infinite where a bound is not finite.
+template <int D, bool HEADS>
 __global__ __launch_bounds__(256) void cache_scores_kernel(const SelectArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr int NI = D / 32;
     const int lane = threadIdx.x & 63, n = lane & 15, g4 = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int bh = blockIdx.z, b = a.by_hkv.of(bh), kvh = bh - b * a.Hkv, set = blockIdx.x * 4 + wave;
-    const int L = length_of(a.lengths, b, a.cap), C = min(count_of(a.counts, b, a.M), a.i0 + a.n), blocks = L > 0 ? ((L - 1) >> a.block_shift) + 1 : 0;
-    if (set * 16 >= blocks || blocks <= a.top) return;      // (where all blocks are taken no score is needed)
-    const int blk = set * 16 + n;
-    const half_t* const bp = a.bounds + ((int64_t)bh * a.nb + min(blk, blocks - 1)) * 2 * D + 8 * g4;
-    half8_t lo[NI], hi[NI];
+    const int bh = blockIdx.z, b = a.by_hkv.of(bh), kvh = bh - b * a.Hkv, set = blockIdx.x * 4 + wave, blk = set * 16 + n;
+    // (bounds and queries are requested before it is known how many of them count)
+    const half_t* const bp = a.bounds + ((int64_t)bh * a.nb + min(blk, a.nb - 1)) * 2 * D + 8 * g4;
+    half8_t lo[NI], hi[NI], q[NI];
 #pragma unroll
     for (int i = 0; i < NI; ++i) { lo[i] = *reinterpret_cast<const half8_t*>(bp + 32 * i); hi[i] = *reinterpret_cast<const half8_t*>(bp + D + 32 * i); }
+    const half_t* const qh = a.q + b * a.qs[0] + (int64_t)kvh * a.G * a.qs[1] + 8 * g4;
+    const int j_first = blockIdx.y * a.steps * (HEADS ? 1 : 16);
+    auto load = [&](int i, int g) __attribute__((always_inline)) {
+        const half_t* const p = qh + (int64_t)g * a.qs[1] + (int64_t)i * a.qs[2];
+#pragma unroll
+        for (int e = 0; e < NI; ++e) q[e] = *reinterpret_cast<const half8_t*>(p + 32 * e);
+    };
+    if constexpr (HEADS) load(min(a.i0 + j_first, a.M - 1), min(n, a.G - 1));
+    const int L = length_of(a.lengths, b, a.cap), C = min(count_of(a.counts, b, a.M), a.i0 + a.n), blocks = L > 0 ? ((L - 1) >> a.block_shift) + 1 : 0;
+    if (set * 16 >= blocks || blocks <= a.top) return;      // (where all blocks are taken no score is needed)
     if (blockIdx.y == 0) {
         float sum = 0.f;
         bool bad = false;
@@ -103,29 +134,44 @@ __global__ __launch_bounds__(256) void cache_scores_kernel(const SelectArgs a) {
             for (int e = 0; e < 8; ++e) { const float x = fmaxf(fabsf((float)lo[i][e]), fabsf((float)hi[i][e])); sum = __builtin_fmaf(x, x, sum); }
         }
         sum = quad_sum(bad ? INFINITY : sum);
-#pragma unroll
-        for (int d = 1; d < 16; d *= 2) sum = fmaxf(sum, __shfl_xor(sum, d, 64));
+        sum = row_max(blk < blocks ? sum : 0.f);
         if (lane == 0) a.norms[(int64_t)bh * (a.nbp >> 4) + set] = sum;
     }
     const float4_t zero = {0.f, 0.f, 0.f, 0.f};
-    half8_t nil = {};
-    for (int s = 0; s < a.steps; ++s) {
-        const int j0 = (blockIdx.y * a.steps + s) * 16, i = a.i0 + j0 + n;
-        if (a.i0 + j0 >= C) return;
-        const half_t* const qp = a.q + b * a.qs[0] + (int64_t)kvh * a.G * a.qs[1] + (int64_t)min(i, C - 1) * a.qs[2] + 8 * g4;
-        float4_t best = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        for (int g = 0; g < a.G; ++g) {
-            float4_t x = zero;
+    const half8_t nil = {};
+    auto product = [&] {
+        float4_t x = zero;
 #pragma unroll
-            for (int e = 0; e < NI; ++e) {
-                const half8_t q = *reinterpret_cast<const half8_t*>(qp + g * a.qs[1] + 32 * e);
-                x = mfma16(hi[e], __builtin_elementwise_max(q, nil), x);
-                x = mfma16(lo[e], __builtin_elementwise_min(q, nil), x);
+        for (int e = 0; e < NI; ++e) {
+            x = mfma16(hi[e], __builtin_elementwise_max(q[e], nil), x);
+            x = mfma16(lo[e], __builtin_elementwise_min(q[e], nil), x);
+        }
+        return x;
+    };
+    float* const to = a.scores + (int64_t)bh * a.n * a.nbp + set * 16 + 4 * g4;
+    for (int s = 0; s < a.steps; ++s) {
+        const int j0 = j_first + s * (HEADS ? 1 : 16), i = a.i0 + j0 + (HEADS ? 0 : n);
+        if (a.i0 + j0 >= C) return;
+        float4_t best = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if constexpr (HEADS) {
+            for (int g0 = 0; g0 < a.G; g0 += 16) {
+                if (s > 0 || g0 > 0) load(i, min(g0 + n, a.G - 1));
+                const float4_t x = product();
+#pragma unroll
+                for (int e = 0; e < 4; ++e) best[e] = fmaxf(best[e], x[e]);
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) best[e] = fmaxf(best[e], x[e]);
+            for (int e = 0; e < 4; ++e) best[e] = row_max(best[e]);
+            if (n == 0) *reinterpret_cast<float4_t*>(to + j0 * a.nbp) = best;
+        } else {
+            for (int g = 0; g < a.G; ++g) {
+                load(min(i, C - 1), g);
+                const float4_t x = product();
+#pragma unroll
+                for (int e = 0; e < 4; ++e) best[e] = fmaxf(best[e], x[e]);
+            }
+            if (i < C) *reinterpret_cast<float4_t*>(to + (j0 + n) * a.nbp) = best;
         }
-        if (i < C) *reinterpret_cast<float4_t*>(a.scores + ((int64_t)bh * a.n + j0 + n) * a.nbp + set * 16 + 4 * g4) = best;
     }
 #endif
 }
@@ -174,55 +220,45 @@ __global__ __launch_bounds__(256) void cache_scores64_kernel(const SelectArgs a)
 
 // ------------------------------------------------------------------------------------------------ selection
 #if defined(__HIP_DEVICE_COMPILE__)
-// The want-th largest of a workgroup's open keys (bit r: key[r]), digit by digit of eight bits from the first bit on that they differ in: `known`, and how many of its equals
-// belong to the first `want` (`want` then).  Where all of a digit's keys do, the rest of the digits need not be known: `known` is then one less than the least of them.
-template <int T> struct KthShared { uint32_t any[T / 64], all[T / 64]; int count[256], sums[4], digit, left, done; };
+// What the waves of a selection tell each other.
+template <int T> struct SelectShared { int count[4][256]; uint32_t any[T / 64], none[T / 64], norm_q[T / 64], norm_b[T / 64], least[T / 64]; int sure[T / 64], maybe[T / 64], taken[T / 64]; };
+
+// The want-th largest of a workgroup's open keys (bit r: key[r]; any, none: the bits that are set, and not set, in some of them), digit by digit of eight bits from the first one on that they differ
+// in.  Returns the least number that the first `want` keys reach -- the want-th largest itself, or, where all keys of a digit are among them, that digit's first number --
+// and in `left` how many of those that equal it belong to them (0: all that reach it).  `count` is zero before.
 template <int T, int REGS>
-__device__ __forceinline__ void kth(const uint32_t (&key)[REGS], uint32_t open, int& want, uint32_t& known, KthShared<T>& sh) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    uint32_t any = 0, all = ~0u;
-#pragma unroll
-    for (int r = 0; r < REGS; ++r)
-        if (open >> r & 1) { any |= key[r]; all &= key[r]; }
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) { any |= __shfl_xor((int)any, d, 64); all &= __shfl_xor((int)all, d, 64); }
-    if (lane == 0) { sh.any[wave] = any; sh.all[wave] = all; }
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < T / 64; ++w) { any |= sh.any[w]; all &= sh.all[w]; }
-    const uint32_t differ = any & ~all;
-    known = all;
-    if (differ == 0) { __syncthreads(); return; }
-    int above = 32 - __builtin_clz(differ);
-    known = above == 32 ? 0u : all >> above << above;
+__device__ __forceinline__ uint32_t kth(const uint32_t (&key)[REGS], uint32_t open, uint32_t any, uint32_t none, int want, int& left, int (&count)[4][256]) {
+    const int lane = threadIdx.x & 63;
+    const uint32_t differ = any & none;
+    left = want;
+    if (differ == 0) return any;
+    int above = 32 - __builtin_clz(differ), pass = 0;
+    uint32_t known = above == 32 ? 0u : any >> above << above;
     while (above > 0) {
         const int shift = max(above - 8, 0);
         const uint32_t width = (1u << (above - shift)) - 1;
-        if (tid < 256) sh.count[tid] = 0;
-        __syncthreads();
+        int (&bins)[256] = count[pass++];
 #pragma unroll
         for (int r = 0; r < REGS; ++r)
-            if ((open >> r & 1) && (above == 32 || (key[r] ^ known) >> above == 0)) atomicAdd(&sh.count[key[r] >> shift & width], 1);
+            if ((open >> r & 1) && (above == 32 || (key[r] ^ known) >> above == 0)) atomicAdd(&bins[255 - (key[r] >> shift & width)], 1);      // (the largest first)
         __syncthreads();
-        int mine = 0, sum = 0;
-        if (wave < 4) {                          // from the largest digit down
-            sum = mine = sh.count[255 - tid];
+        // (every wave looks for itself: four digits a lane)
+        int c[4];
 #pragma unroll
-            for (int d = 1; d < 64; d *= 2) { const int y = __shfl_up(sum, d, 64); if (lane >= d) sum += y; }
-            if (lane == 63) sh.sums[wave] = sum;
-        }
-        __syncthreads();
-        if (wave < 4) {
-            for (int w = 0; w < wave; ++w) sum += sh.sums[w];
-            if (sum >= want && sum - mine < want) { sh.digit = 255 - tid; sh.left = want - (sum - mine); sh.done = sum == want; }
-        }
-        __syncthreads();
-        known |= (uint32_t)sh.digit << shift;
-        want = sh.left;
-        if (sh.done && known) { known -= 1; want = 0; break; }
+        for (int e = 0; e < 4; ++e) c[e] = bins[4 * lane + e];
+        const int mine = c[0] + c[1] + c[2] + c[3], upto = (int)scan64((uint32_t)mine, Add{});
+        const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto >= left));
+        int rest = left - (upto - mine), e = 0, in = c[0];
+#pragma unroll
+        for (int f = 1; f < 4; ++f)
+            if (e == f - 1 && rest > in) { rest -= in; e = f; in = c[f]; }
+        const int found = __builtin_amdgcn_readlane(4 * lane + e, at), done = __builtin_amdgcn_readlane(rest == in, at);
+        left = __builtin_amdgcn_readlane(rest, at);
+        known |= (uint32_t)(255 - found) << shift;
+        if (done) { left = 0; break; }
         above = shift;
     }
-    __syncthreads();
+    return known;
 }
 // The score of one block in 64 bits, by a wave: D / 8 lanes have eight channels each, and the others as many query heads at a time.
 template <int D>
@@ -245,137 +281,153 @@ __device__ __forceinline__ float score64(const SelectArgs& a, const half_t* q, i
     for (int d = LPR; d < 64; d *= 2) best = fmax(best, __shfl_xor(best, d, 64));
     return (float)best;
 }
-#endif
 
 // A workgroup has one query of one KV head, and of its blocks' scores REGS a thread.  Scores s come with a bound e of how far they are off the definition's, r.  If t is the last of s that would be
 // taken, the last of r is within e of t: s > t + 2 e belongs to what is taken, s < t - 2 e does not, and between them the definition decides, if that is needed.  e: the sum of 128 products
 // in 32 bits, 2 x 128 additions that may each cut off 2^-23 of the sum of their magnitudes, which is |q| |b| at most, is off by 2^-15 of that; the rounding of r by 2^-24; numbers that the matrix
 // pipe takes for zero, below 2^-14, by 2^-14 sqrt(128) of the other factor: e = 2^-14 (|q| + 12) (|b| + 12) covers all of it.
 template <int D, int T, int REGS>
-__global__ __launch_bounds__(T) void cache_select_kernel(const SelectArgs a) {
-#if defined(__HIP_DEVICE_COMPILE__)
-    __shared__ KthShared<T> sh;
-    __shared__ int waves[T / 64], waves2[T / 64];
-    __shared__ float norm_q[T / 64], norm_b[T / 64], least[T / 64];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int bh = a.by_n.of(blockIdx.x), j = blockIdx.x - bh * a.n, i = a.i0 + j, b = a.by_hkv.of(bh), kvh = bh - b * a.Hkv;
-    const float* const from = a.scores + ((int64_t)bh * a.n + j) * a.nbp;
+__device__ __forceinline__ void select_blocks(const SelectArgs& a, SelectShared<T>& sh, int bh, int b, int kvh, int i, int n, const float* from, int32_t* to) {
+    constexpr int W = T / 64, LPR = D / 8, PER = 64 / LPR;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), x0 = tid * REGS;
+    // all that is needed is requested at once: a thread's scores, neighbours; norms; queries
     float s[REGS];
 #pragma unroll
-    for (int r = 0; r < REGS; ++r) s[r] = r * T + tid < a.nbp ? from[r * T + tid] : 0.f;      // (requested before it is known how many count)
+    for (int r = 0; r < REGS; r += 4) {
+        const float4_t v = x0 + r < n ? *reinterpret_cast<const float4_t*>(from + x0 + r) : float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[r + e] = v[e];
+    }
     const half_t* const q = a.q + b * a.qs[0] + (int64_t)kvh * a.G * a.qs[1] + (int64_t)i * a.qs[2];
-    const int L = length_of(a.lengths, b, a.cap), C = count_of(a.counts, b, a.M), last = L - C + i, n = last < 0 ? 0 : (last >> a.block_shift) + 1;
-    if (i >= C) return;
-    int32_t* const to = a.selected + ((int64_t)bh * a.M + i) * a.top;
-    if (n <= a.top) {
-        for (int x = tid; x < a.top; x += T) to[x] = x < n ? x : -1;
-        return;
+    float bb = 0.f, qq = 0.f;
+    for (int x = tid; x < (n + 15) >> 4; x += T) bb = fmaxf(bb, a.norms[(int64_t)bh * (a.nbp >> 4) + x]);
+    for (int g0 = wave * PER; g0 < a.G; g0 += W * PER) {
+        const half8_t v = *reinterpret_cast<const half8_t*>(q + (int64_t)min(g0 + lane / LPR, a.G - 1) * a.qs[1] + lane % LPR * 8);
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = __builtin_fmaf((float)v[e], (float)v[e], sum);
+        if (odd_values(v)) sum = INFINITY;
+        sum += rotated<0xb1>(sum);
+        sum += rotated<0x4e>(sum);
+        sum += rotated<0x141>(sum);
+        if constexpr (D == 128) sum += rotated<0x140>(sum);
+        qq = fmaxf(qq, sum);
     }
     const int lo = a.sink, hi = n - a.recent;                     // what is chosen from (top > their number: not empty)
     int want = a.top - a.sink - a.recent;
-    uint32_t sure = 0, maybe = 0, known = 0;
-    uint32_t key[REGS];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) for (int c = tid; c < 256; c += T) sh.count[e][c] = 0;
+    uint32_t key[REGS], open = 0, any = 0, none = 0, sure = 0, maybe = 0, forced = 0;
+#pragma unroll
+    for (int r = 0; r < REGS; ++r) {
+        const int x = x0 + r;
+        key[r] = ordered(s[r]);
+        if (x >= lo && x < hi) { open |= 1u << r; any |= key[r]; none |= ~key[r]; }
+        else if (x < n) forced |= 1u << r;
+    }
     if (want > 0) {
-        float bb = 0.f, qq = 0.f;
-        for (int x = tid; x < (n + 15) >> 4; x += T) bb = fmaxf(bb, a.norms[(int64_t)bh * (a.nbp >> 4) + x]);
-        for (int g = wave; g < a.G; g += T / 64) {
-            float sum = 0.f;
-            bool bad = false;
-            if (lane < D / 8) {
-                const half8_t x = *reinterpret_cast<const half8_t*>(q + (int64_t)g * a.qs[1] + lane * 8);
-                bad = odd_values(x);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) sum = __builtin_fmaf((float)x[e], (float)x[e], sum);
-            }
-            if (bad) sum = INFINITY;
-#pragma unroll
-            for (int d = 1; d < D / 8; d *= 2) sum += __shfl_xor(sum, d, 64);
-            qq = fmaxf(qq, sum);
-        }
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) { bb = fmaxf(bb, __shfl_xor(bb, d, 64)); qq = fmaxf(qq, __shfl_xor(qq, d, 64)); }
-        if (lane == 0) { norm_q[wave] = qq; norm_b[wave] = bb; }
-        uint32_t open = 0;
-#pragma unroll
-        for (int r = 0; r < REGS; ++r) {
-            const int x = r * T + tid;
-            if (x >= lo && x < hi) open |= 1u << r;
-            key[r] = ordered(s[r]);
-        }
-        int left = want;
-        kth<T, REGS>(key, open, left, known, sh);
-        if (left == 0) known += 1;                                // the least digit string of what is taken: not above the last of them
-#pragma unroll
-        for (int w = 0; w < T / 64; ++w) { qq = fmaxf(qq, norm_q[w]); bb = fmaxf(bb, norm_b[w]); }
-        float e2 = 2.f * 1.01f * 0x1p-14f * (sqrtf(qq) + 12.f) * (sqrtf(bb) + 12.f);
-        // (known may be less than the last that is taken, by a part of its last digit: the least of those above it is the last)
-        float t = INFINITY;
-#pragma unroll
-        for (int r = 0; r < REGS; ++r)
-            if ((open >> r & 1) && key[r] >= known) t = fminf(t, s[r]);
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) t = fminf(t, __shfl_xor(t, d, 64));
-        if (lane == 0) least[wave] = t;
+        // (magnitudes are ordered as their bits)
+        any = all64(any, Or{}); none = all64(none, Or{});
+        uint32_t nq = all64(__float_as_uint(qq), Max{}), nb = all64(__float_as_uint(bb), Max{});
+        if (lane == 0) { sh.any[wave] = any; sh.none[wave] = none; sh.norm_q[wave] = nq; sh.norm_b[wave] = nb; }
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < T / 64; ++w) t = fminf(t, least[w]);
-        if (!(e2 < INFINITY)) e2 = INFINITY;
-        const float above = e2 < INFINITY ? t + e2 : INFINITY, below = e2 < INFINITY ? t - e2 : -INFINITY;
-        int n_sure = 0, n_maybe = 0;
+        for (int w = 0; w < W; ++w) { any |= sh.any[w]; none |= sh.none[w]; nq = max(nq, sh.norm_q[w]); nb = max(nb, sh.norm_b[w]); }
+        int left;
+        const uint32_t reach = kth<T, REGS>(key, open, any, none, want, left, sh.count);
+        // the last score that is taken: the least that reaches
+        uint32_t least = 0;
+#pragma unroll
+        for (int r = 0; r < REGS; ++r) if ((open >> r & 1) && key[r] >= reach) least = max(least, ~key[r]);
+        least = all64(least, Max{});
+        if (lane == 0) sh.least[wave] = least;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < W; ++w) least = max(least, sh.least[w]);
+        const float t = unordered(~least), e2 = 2.02f * 0x1p-14f * (sqrtf(__uint_as_float(nq)) + 12.f) * (sqrtf(__uint_as_float(nb)) + 12.f);
+        const bool bound = e2 < INFINITY;
+        const float above = bound ? t + e2 : INFINITY, below = bound ? t - e2 : -INFINITY;
 #pragma unroll
         for (int r = 0; r < REGS; ++r)
             if (open >> r & 1) {
                 if (s[r] > above) sure |= 1u << r;
                 else if (!(s[r] < below)) maybe |= 1u << r;
             }
-        n_sure = __popc(sure); n_maybe = __popc(maybe);
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) { n_sure += __shfl_xor(n_sure, d, 64); n_maybe += __shfl_xor(n_maybe, d, 64); }
-        if (lane == 0) { waves[wave] = n_sure; waves2[wave] = n_maybe; }
+        const uint32_t both = all64(__popc(sure) << 16 | __popc(maybe), Add{});
+        if (lane == 0) { sh.sure[wave] = both >> 16; sh.maybe[wave] = both & 0xffff; }
         __syncthreads();
-        n_sure = n_maybe = 0;
+        int n_maybe = 0;
 #pragma unroll
-        for (int w = 0; w < T / 64; ++w) { n_sure += waves[w]; n_maybe += waves2[w]; }
-        want -= n_sure;
-        __syncthreads();
-        if (n_maybe == want) { sure |= maybe; maybe = 0; }
+        for (int w = 0; w < W; ++w) { want -= sh.sure[w]; n_maybe += sh.maybe[w]; }
+        if (n_maybe == want) sure |= maybe;
         else {
+            any = none = 0;
 #pragma unroll
             for (int r = 0; r < REGS; ++r) {
                 uint64_t todo = __builtin_amdgcn_ballot_w64(maybe >> r & 1);
                 while (todo) {
                     const int bit = __builtin_ctzll(todo);
                     todo &= todo - 1;
-                    const float x = score64<D>(a, q, bh, r * T + wave * 64 + bit);
+                    const float x = score64<D>(a, q, bh, (wave * 64 + bit) * REGS + r);
                     if (lane == bit) key[r] = ordered(x);
                 }
+                if (maybe >> r & 1) { any |= key[r]; none |= ~key[r]; }
             }
-            kth<T, REGS>(key, maybe, want, known, sh);
+            any = all64(any, Or{}); none = all64(none, Or{});
+#pragma unroll
+            for (int e = 0; e < 4; ++e) for (int c = tid; c < 256; c += T) sh.count[e][c] = 0;
+            if (lane == 0) { sh.any[wave] = any; sh.none[wave] = none; }
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < W; ++w) { any |= sh.any[w]; none |= sh.none[w]; }
+            const uint32_t from_here = kth<T, REGS>(key, maybe, any, none, want, left, sh.count);
+            // those above; and of its equals the first `left` (none left: all of them)
+            uint32_t equal = 0;
+#pragma unroll
+            for (int r = 0; r < REGS; ++r)
+                if (maybe >> r & 1) {
+                    if (key[r] > from_here || (left == 0 && key[r] == from_here)) sure |= 1u << r;
+                    else if (key[r] == from_here) equal |= 1u << r;
+                }
+            if (left > 0) {
+                const int mine = __popc(equal), upto = (int)scan64(mine, Add{});
+                if (lane == 63) sh.taken[wave] = upto;
+                __syncthreads();
+                int rank = upto - mine;
+                for (int w = 0; w < wave; ++w) rank += sh.taken[w];
+#pragma unroll
+                for (int r = 0; r < REGS; ++r)
+                    if (equal >> r & 1) { if (rank < left) sure |= 1u << r; ++rank; }
+                __syncthreads();
+            }
         }
     }
-    // what is taken, in order; of the equals of `known` the first `want`
-    int done = 0, equals = 0;
+    // what is taken, in order
+    const uint32_t take = sure | forced;
+    const int mine = __popc(take), upto = (int)scan64(mine, Add{});
+    if (lane == 63) sh.taken[wave] = upto;
+    __syncthreads();
+    int at = upto - mine;
+    for (int w = 0; w < wave; ++w) at += sh.taken[w];
 #pragma unroll
-    for (int r = 0; r < REGS; ++r) {
-        if (r * T >= n) break;
-        const int x = r * T + tid;
-        const bool mb = maybe >> r & 1, equal = mb && key[r] == known;
-        const uint64_t eq = __builtin_amdgcn_ballot_w64(equal), under = (1ull << lane) - 1;
-        if (lane == 0) waves[wave] = __popcll(eq);
-        __syncthreads();
-        int rank = equals + __popcll(eq & under);
-        for (int w = 0; w < wave; ++w) rank += waves[w];
-        const bool take = x < n && (x < lo || x >= hi || (sure >> r & 1) || (mb && (key[r] > known || (equal && rank < want))));
-        const uint64_t tk = __builtin_amdgcn_ballot_w64(take);
-        if (lane == 0) waves2[wave] = __popcll(tk);
-        __syncthreads();
-        int at = done + __popcll(tk & under);
-        for (int w = 0; w < wave; ++w) at += waves2[w];
-        if (take) to[at] = x;
-#pragma unroll
-        for (int w = 0; w < T / 64; ++w) { equals += waves[w]; done += waves2[w]; }
-        __syncthreads();
+    for (int r = 0; r < REGS; ++r)
+        if (take >> r & 1) to[at++] = x0 + r;
+}
+#endif
+
+template <int D, int T, int REGS>
+__global__ __launch_bounds__(T) void cache_select_kernel(const SelectArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __shared__ __attribute__((aligned(16))) SelectShared<T> sh;
+    const int bh = a.by_n.of(blockIdx.x), j = blockIdx.x - bh * a.n, i = a.i0 + j, b = a.by_hkv.of(bh);
+    const int L = length_of(a.lengths, b, a.cap), C = count_of(a.counts, b, a.M), last = L - C + i, n = last < 0 ? 0 : (last >> a.block_shift) + 1;
+    if (i >= C) return;
+    int32_t* const to = a.selected + ((int64_t)bh * a.M + i) * a.top;
+    if (n <= a.top) {
+        for (int x = threadIdx.x; x < a.top; x += T) to[x] = x < n ? x : -1;
+        return;
     }
+    select_blocks<D, T, REGS>(a, sh, bh, b, bh - b * a.Hkv, i, n, a.scores + ((int64_t)bh * a.n + j) * a.nbp, to);
 #endif
 }
 
@@ -474,7 +526,7 @@ struct Chosen {
 template <int D, int NQ>
 __global__ __launch_bounds__(256, 2) void cache_sparse_attn_kernel(const SparseArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    __shared__ __attribute__((aligned(1024))) char lds[kNarrowLds(D)];
+    TRN_LDS(D, lds);
     __shared__ NarrowStats stats;
     constexpr int RT = 16 * NQ;
     const int lane = threadIdx.x & 63, n = lane & 15, g4 = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -510,7 +562,7 @@ __global__ __launch_bounds__(256, 2) void cache_sparse_attn_kernel(const SparseA
 #pragma unroll
         for (int e = 0; e < D / 16; ++e) o[e][qb] = float4_t{0.f, 0.f, 0.f, 0.f};
     }
-    narrow_walk<D, NQ, 1>(keys, t0, t1, min(t1, max(t0, whole)), keys.kpitch, keys.vpitch, a.c, qB, last, lds + wave * 2 * 32 * D * 2, o, m, l);
+    narrow_walk<D, NQ, 1>(keys, t0, t1, min(t1, max(t0, whole)), keys.kpitch, keys.vpitch, a.c, qB, last, lds.k(wave), lds.v(wave), o, m, l);
     narrow_join<D, NQ>(lds, stats, o, m, l, [&](int r, int d0, float4_t v, float mm, float ll, bool once) __attribute__((always_inline)) {
         const int g = rt * RT + r;
         if (g >= a.G) return;
@@ -534,7 +586,7 @@ __global__ __launch_bounds__(256, 2) void cache_sparse_attn_kernel(const SparseA
 template <int D, int NQ>
 __global__ __launch_bounds__(256, 2) void cache_sparse_rows_kernel(const SparseArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    __shared__ __attribute__((aligned(1024))) char lds[kNarrowLds(D)];
+    TRN_LDS(D, lds);
     constexpr int RT = 16 * NQ;
     const int lane = threadIdx.x & 63, n = lane & 15, g4 = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int x = a.by_hkv.of(blockIdx.x), kvh = blockIdx.x - x * a.Hkv, y = a.by_b.of(x), b = x - y * a.B, z = y * 4 + wave, i = a.by_rt.of(z), rt = z - i * a.n_rt;
@@ -569,7 +621,7 @@ __global__ __launch_bounds__(256, 2) void cache_sparse_rows_kernel(const SparseA
 #pragma unroll
         for (int e = 0; e < D / 16; ++e) o[e][qb] = float4_t{0.f, 0.f, 0.f, 0.f};
     }
-    narrow_walk<D, NQ, 1>(keys, 0, T, whole, keys.kpitch, keys.vpitch, a.c, qB, last, lds + wave * 2 * 32 * D * 2, o, m, l);
+    narrow_walk<D, NQ, 1>(keys, 0, T, whole, keys.kpitch, keys.vpitch, a.c, qB, last, lds.k(wave), lds.v(wave), o, m, l);
 #pragma unroll
     for (int qb = 0; qb < NQ; ++qb) {
         const int g = rt * RT + 16 * qb + n;
@@ -645,11 +697,12 @@ extern "C" int trn_cache_sparse_attn_f16(const trn_cache16* c, const void* bound
     const int64_t groups = p.rows ? heads * (((int64_t)seq_q * p.n_rt + 3) / 4) : heads * seq_q * p.n_rt * p.ns;
     // (workgroups of 256, and as many threads in all as 32 bits number: of every launch, before the first one)
     const bool many = p.nb > kMostBlocks;
-    const int64_t q_tiles = (p.step + 15) / 16, waves = heads * (p.nbp / 16) * q_tiles;
+    const bool by_heads = p.step < 12;
+    const int64_t q_tiles = by_heads ? p.step : (p.step + 15) / 16, waves = heads * (p.nbp / 16) * q_tiles;
     const int steps = many ? (waves > 4096 ? 4 : 1) : (int)(waves <= 2048 ? 1 : waves / 2048 < 8 ? waves / 2048 : 8);
     const int per64 = 4 * 512 / c->head_dim * steps;
     const dim3 score_grid((unsigned)(many ? (p.nb + (int64_t)per64 - 1) / per64 : p.nbp / 64), (unsigned)(many ? p.step : (q_tiles + steps - 1) / steps), (unsigned)heads);
-    const int threads = p.nb > 2048 && !many ? 1024 : 256;
+    const int threads = p.nb > 1024 && !many ? 1024 : 256;
     if (groups > 0xffffff || heads > 65535 || heads * p.step * (threads / 256) > 0xffffff || (int64_t)score_grid.x * score_grid.y * score_grid.z > 0xffffff) return TRN_E_SHAPE;
     const hipStream_t s = (hipStream_t)stream;
     const bool d128 = c->head_dim == 128;
@@ -664,23 +717,26 @@ extern "C" int trn_cache_sparse_attn_f16(const trn_cache16* c, const void* bound
         a.by_hkv = Div(c->n_kv_heads); a.by_n = Div(a.n);
         if (p.nb > top) {      // (a.n is at most 65535: 64 MB of at least 64 floats a query)
             dim3 grid = score_grid;
-            grid.y = (unsigned)(many ? a.n : ((a.n + 15) / 16 + steps - 1) / steps);
+            grid.y = (unsigned)(many ? a.n : ((by_heads ? a.n : (a.n + 15) / 16) + steps - 1) / steps);
             if (many) {
                 if (d128) hipLaunchKernelGGL((cache_scores64_kernel<128>), grid, dim3(256), 0, s, a);
                 else hipLaunchKernelGGL((cache_scores64_kernel<64>), grid, dim3(256), 0, s, a);
+            } else if (by_heads) {
+                if (d128) hipLaunchKernelGGL((cache_scores_kernel<128, true>), grid, dim3(256), 0, s, a);
+                else hipLaunchKernelGGL((cache_scores_kernel<64, true>), grid, dim3(256), 0, s, a);
             } else {
-                if (d128) hipLaunchKernelGGL((cache_scores_kernel<128>), grid, dim3(256), 0, s, a);
-                else hipLaunchKernelGGL((cache_scores_kernel<64>), grid, dim3(256), 0, s, a);
+                if (d128) hipLaunchKernelGGL((cache_scores_kernel<128, false>), grid, dim3(256), 0, s, a);
+                else hipLaunchKernelGGL((cache_scores_kernel<64, false>), grid, dim3(256), 0, s, a);
             }
             if ((e = hipGetLastError()) != hipSuccess) break;
         }
         const dim3 grid((unsigned)(heads * a.n));
         if (many) hipLaunchKernelGGL(cache_select_many_kernel, grid, dim3(256), 0, s, a);
         else if (d128) {
-            if (threads == 256) hipLaunchKernelGGL((cache_select_kernel<128, 256, 8>), grid, dim3(256), 0, s, a);
+            if (threads == 256) hipLaunchKernelGGL((cache_select_kernel<128, 256, 4>), grid, dim3(256), 0, s, a);
             else hipLaunchKernelGGL((cache_select_kernel<128, 1024, 8>), grid, dim3(1024), 0, s, a);
         } else {
-            if (threads == 256) hipLaunchKernelGGL((cache_select_kernel<64, 256, 8>), grid, dim3(256), 0, s, a);
+            if (threads == 256) hipLaunchKernelGGL((cache_select_kernel<64, 256, 4>), grid, dim3(256), 0, s, a);
             else hipLaunchKernelGGL((cache_select_kernel<64, 1024, 8>), grid, dim3(1024), 0, s, a);
         }
         e = hipGetLastError();
