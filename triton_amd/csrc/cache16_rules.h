@@ -37,7 +37,7 @@ inline PlanPrefix plan_prefix(int batch, int n_kv_heads, int capacity, int head_
         const int64_t cost_p = units_p * prefix * (p.wide ? 2 : 1), cost_o = units_o * capacity, cost = cost_p + cost_o;
         auto shares = [](int64_t groups, int64_t units, int64_t keys, int64_t least) {
             int64_t s = groups / units;
-            if (s > keys / least) s = keys / least;
+            if (s > (keys + least - 1) / least) s = (keys + least - 1) / least;
             return (int)(keys == 0 ? 0 : s < 1 ? 1 : s > 64 ? 64 : s);
         };
         p.ns_p = shares(cost ? 512 * cost_p / cost : 0, units_p, prefix, p.wide ? 512 : 256);

@@ -283,30 +283,39 @@ __device__ __forceinline__ float score64(const SelectArgs& a, const half_t* q, i
 }
 
 // A workgroup has one query of one KV head, and of its blocks' scores REGS a thread.  Scores s come with a bound e of how far they are off the definition's, r.  If t is the last of s that would be
-// taken, the last of r is within e of t: s > t + 2 e belongs to what is taken, s < t - 2 e does not, and between them the definition decides, if that is needed.  e: the sum of 128 products
-// in 32 bits, 2 x 128 additions that may each cut off 2^-23 of the sum of their magnitudes, which is |q| |b| at most, is off by 2^-15 of that; the rounding of r by 2^-24; numbers that the matrix
-// pipe takes for zero, below 2^-14, by 2^-14 sqrt(128) of the other factor: e = 2^-14 (|q| + 12) (|b| + 12) covers all of it.
+// taken, the last of r is within e of t: s > t + 2 e belongs to what is taken, s < t - 2 e does not, and between them the definition decides, if that is needed.  e: eight matrix instructions
+// add up to 17 numbers that are not zero each (of the two products of a channel one is zero), and may cut off 2^-23 of the largest at each: 2^-16 of the sum of the products' magnitudes, which is
+// |q| |b| at most; the rounding of r is 2^-24 of it: e = 2^-15 |q| |b| is enough.  (Products of fp16 numbers are normal in 32 bits; numbers below 2^-14 enter the pipe as they are.)
+template <int REGS> struct SelectInputs { float s[REGS], bb; };
+// All that a selection needs, requested before it is known how many blocks there are: a thread's scores, neighbours; norms; queries.
 template <int D, int T, int REGS>
-__device__ __forceinline__ void select_blocks(const SelectArgs& a, SelectShared<T>& sh, int bh, int b, int kvh, int i, int n, const float* from, int32_t* to) {
-    constexpr int W = T / 64, LPR = D / 8, PER = 64 / LPR;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), x0 = tid * REGS;
-    // all that is needed is requested at once: a thread's scores, neighbours; norms; queries
-    float s[REGS];
+__device__ __forceinline__ void select_inputs(const SelectArgs& a, SelectInputs<REGS>& in, half8_t& q8, int bh, int b, int kvh, int i, const float* from) {
+    constexpr int LPR = D / 8;
+    const int tid = threadIdx.x, lane = tid & 63, x0 = tid * REGS;
 #pragma unroll
     for (int r = 0; r < REGS; r += 4) {
-        const float4_t v = x0 + r < n ? *reinterpret_cast<const float4_t*>(from + x0 + r) : float4_t{0.f, 0.f, 0.f, 0.f};
+        const float4_t v = x0 + r < a.nbp ? *reinterpret_cast<const float4_t*>(from + x0 + r) : float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[r + e] = v[e];
+        for (int e = 0; e < 4; ++e) in.s[r + e] = v[e];
     }
+    static_assert(T * REGS <= 16 * T, "a norm a thread");
+    in.bb = tid < a.nbp >> 4 ? a.norms[(int64_t)bh * (a.nbp >> 4) + tid] : 0.f;
+    q8 = *reinterpret_cast<const half8_t*>(a.q + b * a.qs[0] + (int64_t)(kvh * a.G + min(tid / LPR, a.G - 1)) * a.qs[1] + (int64_t)i * a.qs[2] + lane % LPR * 8);
+}
+
+template <int D, int T, int REGS>
+__device__ __forceinline__ void select_blocks(const SelectArgs& a, SelectShared<T>& sh, const SelectInputs<REGS>& in, half8_t q8, int bh, int b, int kvh, int i, int n, int32_t* to) {
+    constexpr int W = T / 64, LPR = D / 8;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), x0 = tid * REGS;
+    const float (&s)[REGS] = in.s;
     const half_t* const q = a.q + b * a.qs[0] + (int64_t)kvh * a.G * a.qs[1] + (int64_t)i * a.qs[2];
-    float bb = 0.f, qq = 0.f;
-    for (int x = tid; x < (n + 15) >> 4; x += T) bb = fmaxf(bb, a.norms[(int64_t)bh * (a.nbp >> 4) + x]);
-    for (int g0 = wave * PER; g0 < a.G; g0 += W * PER) {
-        const half8_t v = *reinterpret_cast<const half8_t*>(q + (int64_t)min(g0 + lane / LPR, a.G - 1) * a.qs[1] + lane % LPR * 8);
+    float bb = tid < (n + 15) >> 4 ? in.bb : 0.f, qq = 0.f;
+    for (int g0 = 0; g0 < a.G; g0 += T / LPR) {
+        if (g0) q8 = *reinterpret_cast<const half8_t*>(q + (int64_t)min(g0 + tid / LPR, a.G - 1) * a.qs[1] + lane % LPR * 8);
         float sum = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum = __builtin_fmaf((float)v[e], (float)v[e], sum);
-        if (odd_values(v)) sum = INFINITY;
+        for (int e = 0; e < 8; ++e) sum = __builtin_fmaf((float)q8[e], (float)q8[e], sum);
+        if (odd_values(q8)) sum = INFINITY;
         sum += rotated<0xb1>(sum);
         sum += rotated<0x4e>(sum);
         sum += rotated<0x141>(sum);
@@ -344,7 +353,7 @@ __device__ __forceinline__ void select_blocks(const SelectArgs& a, SelectShared<
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < W; ++w) least = max(least, sh.least[w]);
-        const float t = unordered(~least), e2 = 2.02f * 0x1p-14f * (sqrtf(__uint_as_float(nq)) + 12.f) * (sqrtf(__uint_as_float(nb)) + 12.f);
+        const float t = unordered(~least), e2 = 2.02f * 0x1p-15f * sqrtf(__uint_as_float(nq)) * sqrtf(__uint_as_float(nb));
         const bool bound = e2 < INFINITY;
         const float above = bound ? t + e2 : INFINITY, below = bound ? t - e2 : -INFINITY;
 #pragma unroll
@@ -420,6 +429,9 @@ __global__ __launch_bounds__(T) void cache_select_kernel(const SelectArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     __shared__ __attribute__((aligned(16))) SelectShared<T> sh;
     const int bh = a.by_n.of(blockIdx.x), j = blockIdx.x - bh * a.n, i = a.i0 + j, b = a.by_hkv.of(bh);
+    SelectInputs<REGS> in;
+    half8_t q8;
+    select_inputs<D, T, REGS>(a, in, q8, bh, b, bh - b * a.Hkv, i, a.scores + ((int64_t)bh * a.n + j) * a.nbp);
     const int L = length_of(a.lengths, b, a.cap), C = count_of(a.counts, b, a.M), last = L - C + i, n = last < 0 ? 0 : (last >> a.block_shift) + 1;
     if (i >= C) return;
     int32_t* const to = a.selected + ((int64_t)bh * a.M + i) * a.top;
@@ -427,7 +439,7 @@ __global__ __launch_bounds__(T) void cache_select_kernel(const SelectArgs a) {
         for (int x = threadIdx.x; x < a.top; x += T) to[x] = x < n ? x : -1;
         return;
     }
-    select_blocks<D, T, REGS>(a, sh, bh, b, bh - b * a.Hkv, i, n, a.scores + ((int64_t)bh * a.n + j) * a.nbp, to);
+    select_blocks<D, T, REGS>(a, sh, in, q8, bh, b, bh - b * a.Hkv, i, n, to);
 #endif
 }
 
