@@ -31,7 +31,7 @@ template <int D> __device__ __forceinline__ float row_sum(float x) {
 }
 #endif
 
-template <int D>
+template <int D, bool INTER>
 __global__ __launch_bounds__(256) void cache_rope_kernel(const RopeArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     constexpr int LPR = D / 8, RPW = 64 / LPR, AHEAD = 4;
@@ -40,28 +40,49 @@ __global__ __launch_bounds__(256) void cache_rope_kernel(const RopeArgs a) {
     if (unit >= a.n_units) return;
     const int token = a.by_parts.of(unit), part = unit - token * a.n_parts;
     const int b = a.by_m.of(token), i = token - b * a.M;
-    const int L = length_of(a.lengths, b, a.cap), C = count_of(a.counts, b, a.M);
-    if (i >= C) return;
-    const int at = L - C + i;                        // (below zero: of more new tokens than keys)
 
     // a lane's pieces
     const bool turns = 4 * j < a.pairs;
-    const int c0 = a.inter || !turns ? 8 * j : 4 * j, c1 = a.inter || !turns ? 8 * j + 4 : 4 * j + a.pairs;
-
-    // the angle of pair 4 j + rg % 4
-    float cs = 1.f, sn = 0.f;
-    {
-        const int p = 4 * j + (rg & 3);
-        if (turns) {
-            int where = at;
-            if (a.pos) {
-                const int axis = (p >= a.end[0]) + (p >= a.end[1]) + (p >= a.end[2]);
-                where = a.pos[((int64_t)axis * a.B + b) * a.M + i];
+    const int c0 = INTER || !turns ? 8 * j : 4 * j, c1 = INTER || !turns ? 8 * j + 4 : 4 * j + a.pairs;
+    const half_t* const qp = a.q + b * a.qs[0] + i * a.qs[2];
+    const half_t* const kp = a.k + b * a.ks[0] + i * a.ks[2];
+    const half_t* const vp = a.v + b * a.vs[0] + i * a.vs[2];
+    const int all = a.Hq + 2 * a.Hkv, r0 = part * a.steps * RPW + rg;
+    half4_t x[AHEAD], y[AHEAD];
+    auto load = [&](int s0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < AHEAD; ++e) {
+            const int r = r0 + (s0 + e) * RPW;
+            const half_t* const src = r < a.Hq ? qp + r * a.qs[1] : r < a.Hq + a.Hkv ? kp + (r - a.Hq) * a.ks[1] : vp + (r - a.Hq - a.Hkv) * a.vs[1];
+            if (s0 + e < a.steps && r < all) {
+                if constexpr (INTER) {
+                    const half8_t w = __builtin_nontemporal_load(reinterpret_cast<const half8_t*>(src + c0));
+                    x[e] = half4_t{w[0], w[1], w[2], w[3]}; y[e] = half4_t{w[4], w[5], w[6], w[7]};
+                } else {
+                    x[e] = __builtin_nontemporal_load(reinterpret_cast<const half4_t*>(src + c0));
+                    y[e] = __builtin_nontemporal_load(reinterpret_cast<const half4_t*>(src + c1));
+                }
             }
-            const double turn = (double)where * a.inv[p] * 0.15915494309189535;
-            const float frac = (float)(turn - __builtin_rint(turn));
-            sincospif(2.f * frac, &sn, &cs);
         }
+    };
+    // (the pair 4 j + rg % 4 is this lane's to find the angle of; its frequency is requested before it is known whether and where the token is)
+    const int p = 4 * j + (rg & 3);
+    double freq = 0.;
+    if (turns) freq = a.inv[p];
+    const int L = length_of(a.lengths, b, a.cap), C = count_of(a.counts, b, a.M);
+    if (i >= C) return;
+    load(0);
+    const int at = L - C + i;                        // (below zero: of more new tokens than keys)
+    float cs = 1.f, sn = 0.f;
+    if (turns) {
+        int where = at;
+        if (a.pos) {
+            const int axis = (p >= a.end[0]) + (p >= a.end[1]) + (p >= a.end[2]);
+            where = a.pos[((int64_t)axis * a.B + b) * a.M + i];
+        }
+        const double turn = (double)where * freq * 0.15915494309189535;
+        const float frac = (float)(turn - __builtin_rint(turn));
+        sincospif(2.f * frac, &sn, &cs);
     }
     float co[4], si[4];
 #pragma unroll
@@ -73,35 +94,22 @@ __global__ __launch_bounds__(256) void cache_rope_kernel(const RopeArgs a) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) gq[e] = gk[e] = 1.f;
     if (a.gq) {
-        const half4_t x = *reinterpret_cast<const half4_t*>(a.gq + c0), y = *reinterpret_cast<const half4_t*>(a.gq + c1);
+        const half4_t u = *reinterpret_cast<const half4_t*>(a.gq + c0), w = *reinterpret_cast<const half4_t*>(a.gq + c1);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { gq[e] = (float)x[e]; gq[4 + e] = (float)y[e]; }
+        for (int e = 0; e < 4; ++e) { gq[e] = (float)u[e]; gq[4 + e] = (float)w[e]; }
     }
     if (a.gk) {
-        const half4_t x = *reinterpret_cast<const half4_t*>(a.gk + c0), y = *reinterpret_cast<const half4_t*>(a.gk + c1);
+        const half4_t u = *reinterpret_cast<const half4_t*>(a.gk + c0), w = *reinterpret_cast<const half4_t*>(a.gk + c1);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { gk[e] = (float)x[e]; gk[4 + e] = (float)y[e]; }
+        for (int e = 0; e < 4; ++e) { gk[e] = (float)u[e]; gk[4 + e] = (float)w[e]; }
     }
-
-    const half_t* const qp = a.q + b * a.qs[0] + i * a.qs[2];
-    const half_t* const kp = a.k + b * a.ks[0] + i * a.ks[2];
-    const half_t* const vp = a.v + b * a.vs[0] + i * a.vs[2];
     half_t* const qo = a.qo + b * a.qos[0] + i * a.qos[2];
     half_t* const kc = a.kc + b * a.kcs[0] + at * a.kcs[2];
     half_t* const vc = a.vc + b * a.vcs[0] + at * a.vcs[2];
-    const int rows = a.Hq + (at >= 0 ? 2 * a.Hkv : 0), r0 = part * a.steps * RPW + rg;
+    const int rows = at >= 0 ? all : a.Hq;
     const float inv_d = 1.f / D;
     for (int s0 = 0; s0 < a.steps; s0 += AHEAD) {
-        half4_t x[AHEAD], y[AHEAD];
-#pragma unroll
-        for (int e = 0; e < AHEAD; ++e) {
-            const int r = r0 + (s0 + e) * RPW;
-            const half_t* const src = r < a.Hq ? qp + r * a.qs[1] : r < a.Hq + a.Hkv ? kp + (r - a.Hq) * a.ks[1] : vp + (r - a.Hq - a.Hkv) * a.vs[1];
-            if (s0 + e < a.steps && r < rows) {
-                x[e] = *reinterpret_cast<const half4_t*>(src + c0);
-                y[e] = *reinterpret_cast<const half4_t*>(src + c1);
-            }
-        }
+        if (s0) load(s0);
 #pragma unroll
         for (int e = 0; e < AHEAD; ++e) {
             const int r = r0 + (s0 + e) * RPW;
@@ -118,29 +126,25 @@ __global__ __launch_bounds__(256) void cache_rope_kernel(const RopeArgs a) {
                 for (int c = 0; c < 8; ++c) f[c] = f[c] * n * (is_q ? gq[c] : gk[c]);
             }
             float t[8];
-            if (a.inter) {
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    t[2 * c] = f[2 * c] * co[c] - f[2 * c + 1] * si[c];
-                    t[2 * c + 1] = f[2 * c + 1] * co[c] + f[2 * c] * si[c];
-                }
-            } else {
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    t[c] = f[c] * co[c] - f[4 + c] * si[c];
-                    t[4 + c] = f[4 + c] * co[c] + f[c] * si[c];
-                }
-            }
-            half4_t p, w;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                p[c] = is_v ? x[e][c] : (half_t)(turns ? t[c] : f[c]);
+                const int u = INTER ? 2 * c : c, w = INTER ? 2 * c + 1 : 4 + c;
+                t[u] = f[u] * co[c] - f[w] * si[c];
+                t[w] = f[w] * co[c] + f[u] * si[c];
+            }
+            half4_t u, w;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                u[c] = is_v ? x[e][c] : (half_t)(turns ? t[c] : f[c]);
                 w[c] = is_v ? y[e][c] : (half_t)(turns ? t[4 + c] : f[4 + c]);
             }
             if (there) {
                 half_t* const to = is_q ? qo + r * a.qos[1] : is_v ? vc + (r - a.Hq - a.Hkv) * a.vcs[1] : kc + (r - a.Hq) * a.kcs[1];
-                *reinterpret_cast<half4_t*>(to + c0) = p;
-                *reinterpret_cast<half4_t*>(to + c1) = w;
+                if constexpr (INTER) __builtin_nontemporal_store(half8_t{u[0], u[1], u[2], u[3], w[0], w[1], w[2], w[3]}, reinterpret_cast<half8_t*>(to + c0));
+                else {
+                    __builtin_nontemporal_store(u, reinterpret_cast<half4_t*>(to + c0));
+                    __builtin_nontemporal_store(w, reinterpret_cast<half4_t*>(to + c1));
+                }
             }
         }
     }
@@ -199,10 +203,10 @@ extern "C" int trn_cache_rope_append_f16(const trn_cache16* c, const trn_rope* r
     if ((reinterpret_cast<uintptr_t>(rope->inv_freq) | reinterpret_cast<uintptr_t>(rope->gamma_q) | reinterpret_cast<uintptr_t>(rope->gamma_k)) & 7) return TRN_E_ALIGN;
     if (!rope->norm && (rope->gamma_q || rope->gamma_k)) return TRN_E_UNSUPPORTED;
     const int64_t B = c->batch, Hq = n_q_heads, Hkv = c->n_kv_heads, M = tokens, D = c->head_dim;
-    if ((st = rows16_check(q, q_stride, B, Hq, M, 8, false)) != TRN_OK) return st;
-    if ((st = rows16_check(q_out, q_out_stride, B, Hq, M, 8, true)) != TRN_OK) return st;
-    if ((st = rows16_check(k, k_stride, B, Hkv, M, 8, false)) != TRN_OK) return st;
-    if ((st = rows16_check(v, v_stride, B, Hkv, M, 8, false)) != TRN_OK) return st;
+    if ((st = rows16_check(q, q_stride, B, Hq, M, 16, false)) != TRN_OK) return st;
+    if ((st = rows16_check(q_out, q_out_stride, B, Hq, M, 16, true)) != TRN_OK) return st;
+    if ((st = rows16_check(k, k_stride, B, Hkv, M, 16, false)) != TRN_OK) return st;
+    if ((st = rows16_check(v, v_stride, B, Hkv, M, 16, false)) != TRN_OK) return st;
     // (nothing is written twice, or read after another lane has written it)
     const Extent eq = rows_extent(q, q_stride, B, Hq, M, D), eo = rows_extent(q_out, q_out_stride, B, Hq, M, D), ek = rows_extent(k, k_stride, B, Hkv, M, D),
                  ev = rows_extent(v, v_stride, B, Hkv, M, D);
@@ -235,7 +239,15 @@ extern "C" int trn_cache_rope_append_f16(const trn_cache16* c, const trn_rope* r
     if (groups > 0xffffff) return TRN_E_SHAPE;                       // (threads in 32 bits)
     a.n_units = (int)units;
     a.by_parts = Div(a.n_parts); a.by_m = Div(M);
-    if (D == 128) hipLaunchKernelGGL((cache_rope_kernel<128>), dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL((cache_rope_kernel<64>), dim3((unsigned)groups), dim3(256), 0, (hipStream_t)stream, a);
+    const dim3 grid((unsigned)groups), block(256);
+    const hipStream_t s = (hipStream_t)stream;
+    // (nothing to turn: pieces as the interleaved form has them, 16 bytes)
+    if (a.inter || a.pairs == 0) {
+        if (D == 128) hipLaunchKernelGGL((cache_rope_kernel<128, true>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((cache_rope_kernel<64, true>), grid, block, 0, s, a);
+    } else {
+        if (D == 128) hipLaunchKernelGGL((cache_rope_kernel<128, false>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((cache_rope_kernel<64, false>), grid, block, 0, s, a);
+    }
     return hipGetLastError() == hipSuccess ? TRN_OK : TRN_E_LAUNCH;
 }

@@ -139,7 +139,7 @@ __global__ __launch_bounds__(256) void cache_scores_kernel(const SelectArgs a) {
     }
     const float4_t zero = {0.f, 0.f, 0.f, 0.f};
     const half8_t nil = {};
-    auto product = [&] {
+    auto product = [&](const half8_t (&q)[NI]) {
         float4_t x = zero;
 #pragma unroll
         for (int e = 0; e < NI; ++e) {
@@ -156,7 +156,7 @@ __global__ __launch_bounds__(256) void cache_scores_kernel(const SelectArgs a) {
         if constexpr (HEADS) {
             for (int g0 = 0; g0 < a.G; g0 += 16) {
                 if (s > 0 || g0 > 0) load(i, min(g0 + n, a.G - 1));
-                const float4_t x = product();
+                const float4_t x = product(q);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) best[e] = fmaxf(best[e], x[e]);
             }
@@ -164,9 +164,13 @@ __global__ __launch_bounds__(256) void cache_scores_kernel(const SelectArgs a) {
             for (int e = 0; e < 4; ++e) best[e] = row_max(best[e]);
             if (n == 0) *reinterpret_cast<float4_t*>(to + j0 * a.nbp) = best;
         } else {
+            load(min(i, C - 1), 0);
             for (int g = 0; g < a.G; ++g) {
-                load(min(i, C - 1), g);
-                const float4_t x = product();
+                half8_t now[NI];
+#pragma unroll
+                for (int e = 0; e < NI; ++e) now[e] = q[e];
+                load(min(i, C - 1), min(g + 1, a.G - 1));
+                const float4_t x = product(now);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) best[e] = fmaxf(best[e], x[e]);
             }
@@ -535,14 +539,21 @@ struct Chosen {
 };
 #endif
 
-template <int D, int NQ>
-__global__ __launch_bounds__(256, 2) void cache_sparse_attn_kernel(const SparseArgs a) {
+// SELECT: up to 1024 blocks the workgroup selects by itself, each of a query's shares the same, which is less than a launch.
+constexpr int kOwnBlocks = 1024;
+template <int D, int NQ, bool SELECT>
+__global__ __launch_bounds__(256, 2) void cache_sparse_attn_kernel(const SparseArgs a, const SelectArgs sel) {
 #if defined(__HIP_DEVICE_COMPILE__)
     TRN_LDS(D, lds);
     __shared__ NarrowStats stats;
+    __shared__ __attribute__((aligned(16))) SelectShared<SELECT ? 256 : 64> sh;
+    __shared__ int32_t list[SELECT ? kOwnBlocks : 1];
     constexpr int RT = 16 * NQ;
     const int lane = threadIdx.x & 63, n = lane & 15, g4 = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int x = a.by_hkv.of(blockIdx.x), kvh = blockIdx.x - x * a.Hkv, y = a.by_b.of(x), b = x - y * a.B, z = a.by_ns.of(y), share = y - z * a.ns, i = a.by_rt.of(z), rt = z - i * a.n_rt;
+    [[maybe_unused]] SelectInputs<4> in;
+    [[maybe_unused]] half8_t q8;
+    if constexpr (SELECT) select_inputs<D, 256, 4>(sel, in, q8, b * a.Hkv + kvh, b, kvh, i, sel.scores + (((int64_t)b * a.Hkv + kvh) * sel.n + i) * sel.nbp);
     const int L = length_of(a.lengths, b, a.cap), C = count_of(a.counts, b, a.M), seen = L - C + i + 1;       // the keys that the query sees
     if (i >= C) return;
     const int ends = seen > 0 ? (seen - 1) >> a.block_shift : -1, most = min(a.top, ends + 1), per = 1 << (a.block_shift - 5);
@@ -563,7 +574,14 @@ __global__ __launch_bounds__(256, 2) void cache_sparse_attn_kernel(const SparseA
             qB[qb][e] = there ? v : zero;
         }
     }
-    Chosen keys{a.k + b * a.ks[0] + kvh * a.ks[1], a.v + b * a.vs[0] + kvh * a.vs[1], a.selected + (((int64_t)b * a.Hkv + kvh) * a.M + i) * a.top,
+    if constexpr (SELECT) {
+        if (ends + 1 > a.top) select_blocks<D, 256, 4>(sel, sh, in, q8, b * a.Hkv + kvh, b, kvh, i, ends + 1, list);
+        else for (int x = threadIdx.x; x <= ends; x += 256) list[x] = x;
+        __syncthreads();
+        if (share == 0 && rt == 0)
+            for (int x = threadIdx.x; x < a.top; x += 256) sel.selected[(((int64_t)b * a.Hkv + kvh) * a.M + i) * a.top + x] = x < most ? list[x] : -1;
+    }
+    Chosen keys{a.k + b * a.ks[0] + kvh * a.ks[1], a.v + b * a.vs[0] + kvh * a.vs[1], SELECT ? list : a.selected + (((int64_t)b * a.Hkv + kvh) * a.M + i) * a.top,
                 (int)a.ks[2], (int)a.vs[2], seen, a.block_shift, max(most, 1), 0, 0};
     if (t0 < t1) keys.hold(t0 >> (a.block_shift - 5));
     float4_t o[D / 16][NQ];
@@ -673,7 +691,7 @@ extern "C" int trn_cache_bounds_f16(const trn_cache16* c, int32_t block, int32_t
     const int most = tokens < c->capacity ? tokens : c->capacity;
     // (the blocks that the new tokens can touch -- the first of them may be the last of its block --, but no more workgroups than the card holds at once: the most new tokens
     // that a call allows are rarely there)
-    const int64_t blocks = ((int64_t)most + 2 * block - 2) / block, at_once = (2048 + heads - 1) / heads;
+    const int64_t blocks = ((int64_t)most + 2 * block - 2) / block, at_once = (1024 + heads - 1) / heads;
     a.per = (int)(blocks < at_once ? blocks : at_once);
     if (heads * a.per > 0xffffff) return TRN_E_SHAPE;                 // (threads in 32 bits)
     a.by_per = Div(a.per); a.by_hkv = Div(c->n_kv_heads);
@@ -714,11 +732,13 @@ extern "C" int trn_cache_sparse_attn_f16(const trn_cache16* c, const void* bound
     const int steps = many ? (waves > 4096 ? 4 : 1) : (int)(waves <= 2048 ? 1 : waves / 2048 < 8 ? waves / 2048 : 8);
     const int per64 = 4 * 512 / c->head_dim * steps;
     const dim3 score_grid((unsigned)(many ? (p.nb + (int64_t)per64 - 1) / per64 : p.nbp / 64), (unsigned)(many ? p.step : (q_tiles + steps - 1) / steps), (unsigned)heads);
-    const int threads = p.nb > 1024 && !many ? 1024 : 256;
-    if (groups > 0xffffff || heads > 65535 || heads * p.step * (threads / 256) > 0xffffff || (int64_t)score_grid.x * score_grid.y * score_grid.z > 0xffffff) return TRN_E_SHAPE;
+    const int threads = p.nb > 1024 && !many ? 1024 : p.nb <= 512 ? 128 : 256;
+    const bool own = !p.rows && p.nb > top && p.nb <= kOwnBlocks && p.step == seq_q;       // (the attention's workgroups select)
+    if (groups > 0xffffff || heads > 65535 || heads * p.step * ((threads + 255) / 256) > 0xffffff || (int64_t)score_grid.x * score_grid.y * score_grid.z > 0xffffff) return TRN_E_SHAPE;
     const hipStream_t s = (hipStream_t)stream;
     const bool d128 = c->head_dim == 128;
     hipError_t e = hipSuccess;
+    SelectArgs select{};
     for (int64_t i0 = 0; i0 < seq_q && e == hipSuccess; i0 += p.step) {
         SelectArgs a{};
         a.q = (const half_t*)q; a.bounds = (const half_t*)bounds; a.lengths = c->lengths; a.counts = c->counts; a.scores = (float*)workspace; a.selected = selected;
@@ -742,13 +762,17 @@ extern "C" int trn_cache_sparse_attn_f16(const trn_cache16* c, const void* bound
             }
             if ((e = hipGetLastError()) != hipSuccess) break;
         }
+        select = a;
+        if (own) break;
         const dim3 grid((unsigned)(heads * a.n));
         if (many) hipLaunchKernelGGL(cache_select_many_kernel, grid, dim3(256), 0, s, a);
         else if (d128) {
-            if (threads == 256) hipLaunchKernelGGL((cache_select_kernel<128, 256, 4>), grid, dim3(256), 0, s, a);
+            if (threads == 128) hipLaunchKernelGGL((cache_select_kernel<128, 128, 4>), grid, dim3(128), 0, s, a);
+            else if (threads == 256) hipLaunchKernelGGL((cache_select_kernel<128, 256, 4>), grid, dim3(256), 0, s, a);
             else hipLaunchKernelGGL((cache_select_kernel<128, 1024, 8>), grid, dim3(1024), 0, s, a);
         } else {
-            if (threads == 256) hipLaunchKernelGGL((cache_select_kernel<64, 256, 4>), grid, dim3(256), 0, s, a);
+            if (threads == 128) hipLaunchKernelGGL((cache_select_kernel<64, 128, 4>), grid, dim3(128), 0, s, a);
+            else if (threads == 256) hipLaunchKernelGGL((cache_select_kernel<64, 256, 4>), grid, dim3(256), 0, s, a);
             else hipLaunchKernelGGL((cache_select_kernel<64, 1024, 8>), grid, dim3(1024), 0, s, a);
         }
         e = hipGetLastError();
@@ -770,12 +794,17 @@ extern "C" int trn_cache_sparse_attn_f16(const trn_cache16* c, const void* bound
             if (d128) hipLaunchKernelGGL((cache_sparse_rows_kernel<128, 2>), grid, block3, 0, s, a);
             else hipLaunchKernelGGL((cache_sparse_rows_kernel<64, 2>), grid, block3, 0, s, a);
         }
-    } else if (p.nq == 1) {
-        if (d128) hipLaunchKernelGGL((cache_sparse_attn_kernel<128, 1>), grid, block3, 0, s, a);
-        else hipLaunchKernelGGL((cache_sparse_attn_kernel<64, 1>), grid, block3, 0, s, a);
     } else {
-        if (d128) hipLaunchKernelGGL((cache_sparse_attn_kernel<128, 2>), grid, block3, 0, s, a);
-        else hipLaunchKernelGGL((cache_sparse_attn_kernel<64, 2>), grid, block3, 0, s, a);
+        auto launch = [&](auto nq, auto selects) {
+            constexpr int NQ = decltype(nq)::value;
+            constexpr bool SELECT = decltype(selects)::value;
+            if (d128) hipLaunchKernelGGL((cache_sparse_attn_kernel<128, NQ, SELECT>), grid, block3, 0, s, a, select);
+            else hipLaunchKernelGGL((cache_sparse_attn_kernel<64, NQ, SELECT>), grid, block3, 0, s, a, select);
+        };
+        const std::integral_constant<int, 1> one{};
+        const std::integral_constant<int, 2> two{};
+        if (p.nq == 1) own ? launch(one, std::true_type{}) : launch(one, std::false_type{});
+        else own ? launch(two, std::true_type{}) : launch(two, std::false_type{});
     }
     e = hipGetLastError();
     if (e == hipSuccess && p.ns > 1) {
