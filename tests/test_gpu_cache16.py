@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import cache16 as ref
-from triton_amd import modules, ops
+from triton_amd import _lib, modules, ops
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -280,3 +280,237 @@ def test_selection_of_many_blocks(case, size):
     if size == 1.0:
         out, tol = ref.sparse_attention(q, k, v, torch.zeros_like(q), want, block, D ** -0.5, lengths, counts)
         _within(do, out, tol)
+
+
+# ------------------------------------------------------------------------------------------------ every path of the attention behind a prefix
+PATHS = [
+    # as PREFIXES: narrow shares of prefix and own keys; two row tiles; wide tiles of 36 and of 300 rows; wide prefix, two narrow blocks of rows; wide rows in shares; no own keys; nothing
+    (2, 8, 2, 128, 1, 3000, [3000, 1500], [1, 1], 2500, True),
+    (1, 8, 1, 64, 5, 2500, [2500], [5], 1700, True),
+    (9, 8, 2, 64, 1, 2700, [2700, 1, 0, 5, 64, 700, 33, 2699, 31], [1, 1, 1, 1, 1, 1, 1, 0, 1], 4001, True),
+    (25, 6, 2, 128, 4, 900, [900 - 30 * i for i in range(25)], [1 + i % 4 for i in range(25)], 1500, True),
+    (3, 10, 2, 128, 9, 1100, [1100, 9, 300], [9, 9, 4], 1300, True),
+    (1, 4, 1, 128, 40, 2600, [2570], [40], 3011, True),
+    (1, 5, 1, 64, 33, 3000, [3000], [33], 0, False),
+    (2, 4, 2, 64, 2, 0, [0, 0], [2, 1], 70, True),
+    (2, 4, 2, 128, 40, 0, [0, 0], [40, 3], 70, True),
+    (2, 4, 2, 64, 2, 0, [0, 0], [2, 1], 0, True),
+    (1, 8, 8, 128, 1, 700, [1], [1], 0, True),
+]
+
+
+@pytest.mark.parametrize("case", PATHS, ids=lambda c: f"B{c[0]}H{c[1]}_{c[2]}D{c[3]}M{c[4]}S{c[5]}P{c[8]}{'c' if c[9] else ''}")
+def test_prefix_attention_paths(case):
+    test_prefix_attention(case, "head")
+
+
+def test_prefix_of_another_layout_than_the_cache():
+    """Few keys whose pitches differ between prefix and cache; keys and values likewise."""
+    B, Hq, Hkv, D, M, S, P = 2, 4, 2, 64, 2, 60, 45
+    g = _gen(11)
+    q, k, v = (torch.randn(B, h, s, D, generator=g).half() for h, s in ((Hq, M), (Hkv, S), (Hkv, S)))
+    kp, vp = (torch.randn(1, Hkv, P, D, generator=g).half() for _ in range(2))
+    want, tol = ref.prefix_attention(q, k, v, kp[0], vp[0], torch.zeros_like(q), D ** -0.5, True, [60, 31], [2, 2])
+    for lk, lv, lkp, lvp in (("token", "head", "head", "padded"), ("head", "padded", "token", "head")):
+        o = torch.zeros_like(q, device=DEV)
+        args = (_laid(k, lk), _laid(kp, lkp)[0], o, q.to(DEV), _laid(v, lv), _laid(vp, lvp)[0], None, _ints([60, 31]))
+        modules.get("prefix", "cache").forward(*args)
+        _within(o, want, tol)
+
+
+def test_caches_past_32_bits():
+    """Sequences that lie more than 2^32 bytes apart."""
+    B, Hq, Hkv, D, M, S, far = 2, 4, 1, 64, 1, 200, (1 << 31) + 4096
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    g = _gen(12)
+    q, k, v = (torch.randn(B, h, s, D, generator=g).half() for h, s in ((Hq, M), (Hkv, S), (Hkv, S)))
+    new = [torch.randn(B, h, M, D, generator=g).half() for h in (Hq, Hkv, Hkv)]
+    room = [torch.empty(far + S * D, dtype=torch.float16, device=DEV) for _ in range(2)]
+    dk, dv = (r.as_strided((B, Hkv, S, D), (far, S * D, D, 1)) for r in room)
+    dk.copy_(k); dv.copy_(v)
+    inv = 100.0 ** (-torch.arange(32, dtype=torch.float64) / 32)
+    lengths, counts = [200, 150], [1, 1]
+    qo = torch.zeros_like(q, device=DEV)
+    modules.get("rope", "cache").forward(new[1].to(DEV), dk, new[0].to(DEV), qo, new[2].to(DEV), dv, _ints(counts), None, None, inv.to(DEV), _ints(lengths), None)
+    outs, tols = ref.rope(*new, torch.zeros_like(q), k, v, inv, lengths, counts)
+    for got, want, tol in zip((qo, dk, dv), outs, tols):
+        _within(got, want, tol)
+    k, v, q = dk.cpu(), dv.cpu(), qo.cpu()
+    o = torch.zeros_like(qo)
+    modules.get("prefix", "cache").forward(dk, dk[0, :, :10], o, qo, dv, dv[0, :, :10], _ints(counts), _ints(lengths))
+    _within(o, *ref.prefix_attention(q, k, v, k[0, :, :10], v[0, :, :10], torch.zeros_like(q), D ** -0.5, True, lengths, counts))
+    bnd, sel = torch.zeros(B, Hkv, 7, 2, D, dtype=torch.float16, device=DEV), torch.zeros(B, Hkv, M, 3, dtype=torch.int32, device=DEV)
+    modules.get("bounds", "cache", block=32).forward(dk, bnd, None, _ints(lengths))
+    assert torch.equal(bnd.cpu(), ref.bounds(k, torch.zeros(bnd.shape).half(), 32, lengths, [S] * B))
+    modules.get("sparse", "cache", block=32, top=3).forward(dk, o, qo, dv, bnd, _ints(counts), _ints(lengths), sel)
+    want = ref.select(q, bnd.cpu(), torch.zeros(sel.shape, dtype=torch.int32), 32, 3, 0, 1, 4, lengths, counts, S)
+    assert torch.equal(sel.cpu(), want)
+    _within(o, *ref.sparse_attention(q, k, v, torch.zeros_like(q), want, 32, D ** -0.5, lengths, counts))
+
+
+# ------------------------------------------------------------------------------------------------ together
+def _loop(kind, prenorm=False):
+    B, Hq, Hkv, D, N, S, P = 3, 8, 2, 64, 192, 500, 90 if kind == "prefix" else 0
+    g = _gen(13)
+    w = lambda *s: (torch.randn(*s, generator=g) * N ** -0.5).half().to(DEV)
+    t = dict(WK=w(N, Hkv * D), WQ=w(N, Hq * D), WV=w(N, Hkv * D), gamma_q=(1 + 0.1 * torch.randn(D, generator=g)).half().to(DEV),
+             gamma_k=(1 + 0.1 * torch.randn(D, generator=g)).half().to(DEV), inv_freq=(100.0 ** (-torch.arange(16, dtype=torch.float64) / 16)).to(DEV), positions=None,
+             K_cache=torch.zeros(B, Hkv, S, D, dtype=torch.float16, device=DEV), V_cache=torch.zeros(B, Hkv, S, D, dtype=torch.float16, device=DEV))
+    if kind == "prefix":
+        t.update(K_prefix=torch.randn(Hkv, P, D, generator=g).half().to(DEV), V_prefix=torch.randn(Hkv, P, D, generator=g).half().to(DEV))
+        step = modules.get("prenorm" if prenorm else "prefix", "cache16", head_dim=D, qk_norm=True)
+    else:
+        t.update(bounds=torch.zeros(B, Hkv, -(-S // 32), 2, D, dtype=torch.float16, device=DEV))
+        step = modules.get("sparse", "cache16", head_dim=D, qk_norm=True, block=32, top=5, sink=1, recent=2, norm=prenorm)
+    return step, t, g, (B, Hq, Hkv, D, N, S)
+
+
+def _feed(t, g, dims, lengths, counts, M, top=5):
+    B, Hq, Hkv, D, N, S = dims
+    t.update(X=torch.randn(B, M, N, generator=g).half().to(DEV), O2=torch.zeros(B, M, Hq * D, dtype=torch.float16, device=DEV), lengths=_ints(lengths), counts=_ints(counts),
+             selected=torch.full((B, Hkv, M, top), -7, dtype=torch.int32, device=DEV))
+
+
+@pytest.mark.parametrize("kind", ["prefix", "sparse"])
+@pytest.mark.parametrize("prenorm", [False, True])
+def test_a_serving_loop(kind, prenorm):
+    """Prompts, a chunk, single tokens: each step's caches are the last one's with its own tokens behind them, and its outputs are the definition's on them."""
+    step, t, g, dims = _loop(kind, prenorm)
+    B, Hq, Hkv, D, N, S = dims
+    lengths = [0] * B
+    for M, counts in ((140, [140, 33, 1]), (17, [17, 0, 17]), (1, [1, 1, 1]), (1, [1, 0, 1]), (4, [2, 4, 3])):
+        lengths = [n + c for n, c in zip(lengths, counts)]
+        _feed(t, g, dims, lengths, counts, M)
+        before = [t[n].cpu() for n in ("K_cache", "V_cache")] + [t["bounds"].cpu() if kind == "sparse" else None]
+        step.forward(*[t[n] for n in step.TENSOR_PARAMS])
+        # the projection, as the library makes it by itself
+        x, qkv = t["X"].view(B * M, N), [torch.zeros(B, M, h, D, dtype=torch.float16, device=DEV) for h in (Hq, Hkv, Hkv)]
+        ops.prenorm_qkv(x, None, t["WQ"], t["WK"], t["WV"], *(y.view(B * M, -1, D).permute(1, 0, 2) for y in qkv), 0.0, prenorm)
+        q, k, v = (y.permute(0, 2, 1, 3).cpu() for y in qkv)
+        outs, tols = ref.rope(q, k, v, q, before[0], before[1], t["inv_freq"].cpu(), lengths, counts, None, t["gamma_q"].cpu(), t["gamma_k"].cpu(), True)
+        for n, want, tol in zip(("K_cache", "V_cache"), outs[1:], tols[1:]):
+            _within(t[n], want, tol, n)
+        # (the queries that the step had: the operator's own)
+        qr = torch.zeros_like(qkv[0]).permute(0, 2, 1, 3)
+        scratch = [y.clone() for y in (t["K_cache"], t["V_cache"])]
+        ops.cache_rope_append(*(y.permute(0, 2, 1, 3) for y in qkv), qr, *scratch, t["inv_freq"], t["lengths"], t["counts"], None, t["gamma_q"], t["gamma_k"], True)
+        qr, kc, vc = qr.cpu(), t["K_cache"].cpu(), t["V_cache"].cpu()
+        o = t["O2"].view(B, M, Hq, D).permute(0, 2, 1, 3)
+        if kind == "prefix":
+            _within(o, *ref.prefix_attention(qr, kc, vc, t["K_prefix"].cpu(), t["V_prefix"].cpu(), torch.zeros_like(qr), D ** -0.5, True, lengths, counts))
+        else:
+            bnd = ref.bounds(kc, before[2], 32, lengths, counts)
+            assert torch.equal(t["bounds"].cpu(), bnd)
+            sel = ref.select(qr, bnd, torch.full((B, Hkv, M, 5), -7, dtype=torch.int32), 32, 5, 1, 2, Hq // Hkv, lengths, counts, S)
+            assert torch.equal(t["selected"].cpu(), sel)
+            _within(o, *ref.sparse_attention(qr, kc, vc, torch.zeros_like(qr), sel, 32, D ** -0.5, lengths, counts))
+
+
+@pytest.mark.parametrize("kind", ["prefix", "sparse"])
+def test_a_captured_step_on_caches_that_grow(kind):
+    """One token a sequence, captured once and replayed on longer and longer caches, with eager work in between: bit for bit what the eager step leaves."""
+    runs = []
+    for captured in (False, True):
+        step, t, g, dims = _loop(kind)
+        _feed(t, g, dims, [150, 40, 7], [150, 40, 7], 150)
+        step.forward(*[t[n] for n in step.TENSOR_PARAMS])
+        _feed(t, g, dims, [151, 41, 8], [1, 1, 1], 1)
+        side, got = torch.cuda.Stream(), []
+        step.forward(*[t[n] for n in step.TENSOR_PARAMS])
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        if captured:
+            with torch.cuda.graph(graph, stream=side):
+                step.forward(*[t[n] for n in step.TENSOR_PARAMS])
+        for i in range(5):
+            t["lengths"] += torch.tensor([1, 1, i % 2], dtype=torch.int32, device=DEV)
+            t["counts"].copy_(torch.tensor([1, 1, i % 2]))
+            t["X"].copy_(torch.randn(t["X"].shape, generator=g))
+            t["O2"].zero_()
+            graph.replay() if captured else step.forward(*[t[n] for n in step.TENSOR_PARAMS])
+            torch.cuda.synchronize()
+            got += [t[n].clone() for n in ("O2", "K_cache", "V_cache") + (("bounds", "selected") if kind == "sparse" else ())]
+        runs.append(got)
+    assert all(torch.equal(a, b) for a, b in zip(*runs))
+
+
+def test_on_a_stream_of_its_own():
+    case = PATHS[0]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        test_prefix_attention(case, "head")
+        test_sparse_attention(SPARSES[1], "token")
+    torch.cuda.current_stream().wait_stream(side)
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_on_another_device_than_the_current_one():
+    B, Hq, Hkv, D, M, S, P = 2, 4, 2, 64, 1, 60, 45
+    g = _gen(14)
+    q, k, v = (torch.randn(B, h, s, D, generator=g).half() for h, s in ((Hq, M), (Hkv, S), (Hkv, S)))
+    with torch.cuda.device(0):
+        args = [x.to("cuda:1") for x in (k, k[0], torch.zeros_like(q), q, v, v[0])]
+        modules.get("prefix", "cache").forward(*args, None, None)
+        torch.cuda.synchronize("cuda:1")
+    _within(args[2], *ref.prefix_attention(q, k, v, k[0], v[0], torch.zeros_like(q), D ** -0.5, True, [S] * B, [M] * B))
+
+
+def test_steps_and_calls_of_nothing():
+    for kind in ("prefix", "sparse"):
+        step, t, g, dims = _loop(kind)
+        B, Hq, Hkv, D, N, S = dims
+        _feed(t, g, dims, [5, 0, 1], [0, 0, 0], 0)
+        step.forward(*[t[n] for n in step.TENSOR_PARAMS])
+        _feed(t, g, dims, [5, 0, 1], [0, 0, 0], 2)
+        t["O2"].fill_(3.0)
+        step.forward(*[t[n] for n in step.TENSOR_PARAMS])
+        assert (t["O2"] == 3.0).all() and (t["selected"] == -7).all() and not t["K_cache"].any()
+
+
+def test_first_call_inside_a_capture_is_refused():
+    q = torch.zeros(1, 4, 1, 64, dtype=torch.float16, device=DEV)
+    k = torch.zeros(1, 2, 4000, 64, dtype=torch.float16, device=DEV)
+    att = modules.get("prefix", "cache")
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side), pytest.raises(RuntimeError, match="eagerly"):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            att.forward(k, k[0], q, q.clone(), k, k[0], None, None)
+
+
+def test_refusals():
+    half = lambda *s: torch.zeros(*s, dtype=torch.float16, device=DEV)
+    q, o, k, v = half(1, 4, 2, 64), half(1, 4, 2, 64), half(1, 2, 64, 64), half(1, 2, 64, 64)
+    n1 = torch.zeros(2, dtype=torch.int32, device=DEV)
+
+    def tried(fn, good):
+        fn(**good)
+
+        def bad(error=ValueError, **kw):
+            with pytest.raises(error):
+                fn(**{**good, **kw})
+        return bad
+    inv = torch.zeros(32, dtype=torch.float64, device=DEV)
+    new = half(1, 2, 2, 64)
+    bad = tried(ops.cache_rope_append, dict(q=q, k=new, v=new.clone(), q_out=o, k_cache=k, v_cache=v, inv_freq=inv))
+    bad(q=q.float()); bad(q_out=o[:, :2]); bad(k=new[:, :1]); bad(v=new[:, :, :1]); bad(k_cache=k[..., :32]); bad(inv_freq=inv.float()); bad(inv_freq=inv[:30]); bad(inv_freq=inv.cpu())
+    bad(lengths=n1); bad(counts=n1[:1].long()); bad(sections=[16, 15]); bad(sections=[]); bad(sections=[8] * 5); bad(sections=[16, 16]); bad(gamma_q=half(64)); bad(q=q.cpu())
+    bad(positions=torch.zeros(1, 1, 3, dtype=torch.int32, device=DEV)); bad(norm=True, gamma_k=half(32)); bad(TypeError, sections=3); bad(_lib.TrnError, norm=True, eps=-1.0)
+    bad(_lib.TrnError, v_cache=k); bad(_lib.TrnError, q=half(1, 4, 2, 72)[..., 4:68])
+    bad = tried(ops.cache_prefix_attention, dict(q=q, k=k, v=v, k_prefix=k[0], v_prefix=v[0], o=o))
+    bad(q=q.float()); bad(o=o[:, :2]); bad(q=q[:, :3], o=o[:, :3]); bad(k_prefix=k); bad(v_prefix=v[0, :, :3]); bad(k_prefix=k[0, :1]); bad(v=v[:, :, :3]); bad(lengths=n1); bad(q=q.cpu())
+    bad(_lib.TrnError, scale=0.0); bad(_lib.TrnError, o=q); bad(workspace=torch.zeros(4, device=DEV))
+    big = half(1, 2, 8000, 64)
+    bad(_lib.TrnError, k=big, v=big)                                           # shares without a workspace
+    bnd, sel = half(1, 2, 1, 2, 64), torch.zeros(1, 2, 2, 3, dtype=torch.int32, device=DEV)
+    bad = tried(ops.cache_bounds, dict(k=k, bounds=bnd))
+    bad(block=48); bad(block=32); bad(bounds=bnd.float()); bad(bounds=bnd[0]); bad(k=k[0]); bad(tokens=-1); bad(counts=n1)
+    ws = torch.zeros(1 << 20, dtype=torch.uint8, device=DEV)
+    bad = tried(ops.cache_sparse_attention, dict(q=q, k=k, v=v, bounds=bnd, o=o, selected=sel, top=3, workspace=ws))
+    bad(top=2); bad(top=3, recent=0); bad(sink=3); bad(selected=sel.long()); bad(selected=sel[..., :2]); bad(bounds=half(1, 2, 2, 2, 64)); bad(block=96); bad(_lib.TrnError, workspace=None)
+    bad(_lib.TrnError, scale=-1.0); bad(v=v.float()); bad(_lib.TrnError, q=half(1, 4, 2, 72)[..., 4:68])
+    step = modules.get("prefix", "cache16", head_dim=64)
+    with pytest.raises(ValueError):
+        step.forward(k, k[0], half(1, 2, 128), v, v[0], half(96, 128), half(96, 256), half(96, 128), half(1, 2, 96), None, None, None, None, None, None)

@@ -67,7 +67,7 @@ __device__ __forceinline__ half8_t finite_only(half8_t v) {
 
 // ------------------------------------------------------------------------------------------------ narrow
 // One wave's tiles t0 <= t < t1, every STEP-th, of 32 keys for 16 NQ rows (queries in qB), into o, m, l.  `keys`: where the tile t begins and how many of its keys there are (0..32, wave-uniform; those
-// from there on arrive as zeros and count for no row), as .k(t), .v(t), .n(t), requested in order.  Keys from `last` on (relative to the tile, through .at(t)) are hidden from a row.
+// from there on arrive as zeros and count for no row), as .k(t), .v(t), .n(t); and up to which key of a tile a row sees whose last one is `last`, .lim(t, last).
 template <int D, int NQ, int STEP, class Keys>
 __device__ __forceinline__ void narrow_walk(Keys& keys, int t0, int t1, int t_mask, int kpitch, int vpitch, float c, const half8_t (&qB)[NQ][D / 32], const int (&last)[NQ], half_t* Kt, half_t* Vt,
                                             float4_t (&o)[D / 16][NQ], float (&m)[NQ], float (&l)[NQ]) {
@@ -130,10 +130,9 @@ __device__ __forceinline__ void narrow_walk(Keys& keys, int t0, int t1, int t_ma
 #pragma unroll
                 for (int qb = 0; qb < NQ; ++qb) s[kb][qb] = mfma16(kw[kb][i], qB[qb][i], i == 0 ? zero : s[kb][qb]);
         if constexpr (MASK) {
-            const int key0 = keys.at(t);
 #pragma unroll
             for (int qb = 0; qb < NQ; ++qb) {
-                const int lim = last[qb] - key0 - 4 * g4;
+                const int lim = keys.lim(t, last[qb]) - 4 * g4;
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -183,10 +182,9 @@ __device__ __forceinline__ void narrow_walk(Keys& keys, int t0, int t1, int t_ma
 #pragma unroll
             for (int i = 0; i < NDB; ++i) bad = bad || odd_values(vw[i]);
             if (__builtin_expect(__builtin_amdgcn_ballot_w64(bad) != 0, 0)) {
-                const int key0 = keys.at(t);
 #pragma unroll
                 for (int qb = 0; qb < NQ; ++qb) {
-                    const int lim = last[qb] - key0 - 4 * g4;
+                    const int lim = keys.lim(t, last[qb]) - 4 * g4;
                     half8_t see;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) see[e] = 16 * (e >> 2) + (e & 3) <= lim ? (half_t)1.f : (half_t)0.f;
@@ -218,10 +216,11 @@ __device__ __forceinline__ void narrow_walk(Keys& keys, int t0, int t1, int t_ma
     for (; t < t1; t += STEP) step(std::true_type{}, t);
 }
 
-// The results of a row tile's four waves, joined and delivered: row i of the tile by put(i, first dimension, O, m, l, whether this is the row's first piece).
-struct NarrowStats { float m[4][32], l[4][32], m_all[32], l_all[32]; };
-template <int D, int NQ, class Put>
-__device__ __forceinline__ void narrow_join(const Lds<D>& lds, NarrowStats& st, float4_t (&o)[D / 16][NQ], float (&m)[NQ], float (&l)[NQ], Put put) {
+// The results of a row tile's NW waves, joined and delivered: row i of the tile by put(i, first dimension, O, m, l, whether this is the row's first piece).  area(i, 0), area(i, 1): a wave's stage of K
+// and of V, 16 rows of D floats each.
+template <int NW> struct NarrowStats { float m[NW][32], l[NW][32], m_all[32], l_all[32]; };
+template <int D, int NQ, int NW, class Area, class Put>
+__device__ __forceinline__ void narrow_join(Area area, NarrowStats<NW>& st, float4_t (&o)[D / 16][NQ], float (&m)[NQ], float (&l)[NQ], Put put) {
     constexpr int NDB = D / 16, RT = 16 * NQ;
     const int lane = threadIdx.x & 63, n = lane & 15, g4 = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
@@ -230,29 +229,30 @@ __device__ __forceinline__ void narrow_join(const Lds<D>& lds, NarrowStats& st, 
         if (g4 == 0) { st.m[wave][16 * qb + n] = m[qb]; st.l[wave][16 * qb + n] = l[qb]; }
     }
     __syncthreads();
-    // (a wave's stage of K, and of V, holds 16 rows of D floats; the 16-byte pieces of a row are swizzled by the row)
+    // (the 16-byte pieces of a row are swizzled by the row)
 #pragma unroll
     for (int qb = 0; qb < NQ; ++qb) {
         const int r = 16 * qb + n;
         float top = -INFINITY, sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, st.m[i][r]);
+        for (int i = 0; i < NW; ++i) top = fmaxf(top, st.m[i][r]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum = __builtin_fmaf(st.l[i][r], st.m[i][r] == -INFINITY ? 0.f : fast_exp2(st.m[i][r] - top), sum);      // (a sum of NaN stays)
+        for (int i = 0; i < NW; ++i) sum = __builtin_fmaf(st.l[i][r], st.m[i][r] == -INFINITY ? 0.f : fast_exp2(st.m[i][r] - top), sum);      // (a sum of NaN stays)
         const float mine = m[qb] == -INFINITY ? 0.f : fast_exp2(m[qb] - top);
 #pragma unroll
-        for (int i = 0; i < NDB; ++i) reinterpret_cast<float4_t*>(qb ? lds.v(wave) : lds.k(wave))[n * (D / 4) + ((4 * i + g4) ^ n)] = o[i][qb] * mine;
+        for (int i = 0; i < NDB; ++i) reinterpret_cast<float4_t*>(area(wave, qb))[n * (D / 4) + ((4 * i + g4) ^ n)] = o[i][qb] * mine;
         if (wave == 0 && g4 == 0) { st.m_all[r] = top; st.l_all[r] = sum; }
     }
     __syncthreads();
-    constexpr int TPR = 256 / RT, NP = D / 4 / TPR;                // threads a row, 16-byte pieces a thread
+    constexpr int TPR = NW * 64 / RT, NP = (D / 4 + TPR - 1) / TPR;                // threads a row, 16-byte pieces a thread
     const int row = threadIdx.x / TPR, sub = threadIdx.x % TPR;
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
         const int piece = sub + i * TPR;
+        if (D / 4 % TPR && piece >= D / 4) break;
         float4_t x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x = x + reinterpret_cast<const float4_t*>(row >= 16 ? lds.v(k) : lds.k(k))[(row & 15) * (D / 4) + (piece ^ (row & 15))];
+        for (int k = 0; k < NW; ++k) x = x + reinterpret_cast<const float4_t*>(area(k, row >> 4))[(row & 15) * (D / 4) + (piece ^ (row & 15))];
         put(row, 4 * piece, x, st.m_all[row], st.l_all[row], piece == 0);
     }
 }

@@ -9,7 +9,8 @@ inline int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 // one: wide tiles of each sequence's rows walk over prefix and own keys.  Otherwise rows of all sequences walk over the prefix, in wide tiles or narrow ones, and those of each
 // sequence, in narrow ones of 16 nq rows, over its own keys.  n_rt row tiles and ns shares of their keys (_p, _o; one: _p); slots: results of a row to be joined (one: none);
 // first, second: workgroups of both parts; ml: offset of the statistics in the workspace, bytes: its size.
-struct PlanPrefix { bool one, wide; int G, R, nq, n_rt_p, ns_p, n_rt_o, ns_o, slots; int64_t first, second, ml, bytes; };
+// short_rt: row tiles of eight waves each that have all keys, where pitches allow.
+struct PlanPrefix { bool one, wide; int short_rt; int G, R, nq, n_rt_p, ns_p, n_rt_o, ns_o, slots; int64_t first, second, ml, bytes; };
 
 inline PlanPrefix plan_prefix(int batch, int n_kv_heads, int capacity, int head_dim, int prefix, int Hq, int Sq) {
     PlanPrefix p{};
@@ -17,6 +18,13 @@ inline PlanPrefix plan_prefix(int batch, int n_kv_heads, int capacity, int head_
     p.R = p.G * Sq;
     const int64_t heads = (int64_t)batch * n_kv_heads, rows_p = (int64_t)batch * p.R;
     p.one = p.R > 64;
+    const int64_t tiles16 = (p.R + 15) / 16;
+    // (as long as a wave's tiles, one after the other, take less than a second launch.  One query of 32 heads of 128 on 8, us by shares / by eight waves: one sequence, 60 keys behind 200 9.2 / 6.4, behind
+    // 1000 9.7 / 10.4; 8 sequences 12.7 / 10.6, 500 behind 1000 13.3 / 13.5; 32 (wide tiles) 26.8 / 17.0, 60 behind 3000 24.4 / 20.9 before those had shares of 128 keys, 18.7 with them; 16 heads of
+    // 64, 4 sequences, 60 behind 1000 8.9 / 7.6, 500 behind 1000 9.1 / 9.0, 60 behind 3000 9.8 / 11.4.)
+    const bool shared = prefix > 0 && rows_p > 32;
+    const int64_t rounds = (heads * tiles16 + 255) / 256, most = head_dim == 128 ? (shared ? 1800 : 1000) : (shared ? 2500 : 1500);
+    if (p.R <= 64 && rounds <= 2 && rounds * ((int64_t)prefix + capacity) <= most) p.short_rt = (int)tiles16;
     if (p.one) {
         p.wide = true; p.nq = 2;
         p.n_rt_p = (p.R + 127) / 128;
@@ -40,7 +48,8 @@ inline PlanPrefix plan_prefix(int batch, int n_kv_heads, int capacity, int head_
             if (s > (keys + least - 1) / least) s = (keys + least - 1) / least;
             return (int)(keys == 0 ? 0 : s < 1 ? 1 : s > 64 ? 64 : s);
         };
-        p.ns_p = shares(cost ? 512 * cost_p / cost : 0, units_p, prefix, p.wide ? 512 : 256);
+        p.ns_p = shares(cost ? 512 * cost_p / cost : 0, units_p, prefix, p.wide ? 128 : 256);
+        if (p.wide && p.ns_p > 16) p.ns_p = 16;
         p.ns_o = shares(cost ? 512 * cost_o / cost : 0, units_o, capacity, 256);
         if (p.ns_p + p.ns_o == 0) p.ns_o = 1;      // (nothing to see: zeros)
         p.slots = p.ns_p + p.ns_o;

@@ -26,7 +26,7 @@ struct Run {
     __device__ __forceinline__ const half_t* k(int t) const { return kp + (int64_t)t * 32 * kpitch; }
     __device__ __forceinline__ const half_t* v(int t) const { return vp + (int64_t)t * 32 * vpitch; }
     __device__ __forceinline__ int n(int t) const { return min(32, L - 32 * t); }
-    __device__ __forceinline__ int at(int t) const { return 32 * t; }
+    __device__ __forceinline__ int lim(int t, int last) const { return last - 32 * t; }
 };
 // ... of the prefix, `split` tiles, and of the sequence behind them.
 struct TwoRuns {
@@ -35,6 +35,7 @@ struct TwoRuns {
     __device__ __forceinline__ const half_t* v(int t) const { return t < split ? vp + (int32_t)t * 32 * vpp : vo + (int32_t)(t - split) * 32 * vpo; }
     __device__ __forceinline__ int kpitch(int t) const { return t < split ? kpp : kpo; }
     __device__ __forceinline__ int vpitch(int t) const { return t < split ? vpp : vpo; }
+    __device__ __forceinline__ int n(int t) const { return min(32, left(t)); }
     __device__ __forceinline__ int left(int t) const { return t < split ? P - 32 * t : L - 32 * (t - split); }
     __device__ __forceinline__ bool whole(int t, int to) const { return !(P & 31) || to < split || t >= split; }      // but for those that do not all see it
     __device__ __forceinline__ int lim(int t, int last) const { return t < split ? P - 1 - 32 * t : last - 32 * (t - split); }
@@ -97,12 +98,44 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 4) void cache_prefix_rows_kerne
 #endif
 }
 
+// Few keys: eight waves have 16 rows of one sequence, over the prefix (whose pitches are the cache's) and its own keys, and nothing is joined by a second launch.
+template <int D>
+__global__ __launch_bounds__(512, 1) void cache_prefix_short_kernel(const PrefixArgs a) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    __shared__ __attribute__((aligned(1024))) half_t lds[16][32 * D];
+    __shared__ NarrowStats<8> stats;
+    auto area = [&](int w, int v) __attribute__((always_inline)) { return lds[2 * w + v]; };
+    const int lane = threadIdx.x & 63, n = lane & 15, g4 = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int x = a.by_hkv.of(blockIdx.x), kvh = blockIdx.x - x * a.Hkv, rt = a.by_b.of(x), b = x - rt * a.B;
+    const int L = length_of(a.lengths, b, a.cap), C = count_of(a.counts, b, a.M), rows = C * a.G, off = L - C, split = (a.P + 31) >> 5;
+    if (rt * 16 >= rows) return;
+    auto sees = [&](int r) { return a.causal ? min(L, max(0, a.by_g.of(r) + off + 1)) : L; };
+    const int row = rt * 16 + n, T = split + ((sees(min(rt * 16 + 15, rows - 1)) + 31) >> 5), t0 = T * wave >> 3, t1 = T * (wave + 1) >> 3;
+    half8_t qB[1][D / 32];
+    const half_t* const qp = query(a, b, kvh, min(row, rows - 1));
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) qB[0][i] = *reinterpret_cast<const half8_t*>(qp + 32 * i + 8 * g4);
+    const int last[1] = {sees(min(row, rows - 1)) - 1};
+    TwoRuns keys{a.kp + kvh * a.kps[0], a.vp + kvh * a.vps[0], a.k + b * a.ks[0] + kvh * a.ks[1], a.v + b * a.vs[0] + kvh * a.vs[1],
+                 (int)a.ks[2], (int)a.vs[2], (int)a.ks[2], (int)a.vs[2], a.P, L, split};
+    float4_t o[D / 16][1];
+    float m[1] = {-INFINITY}, l[1] = {0.f};
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) o[i][0] = float4_t{0.f, 0.f, 0.f, 0.f};
+    const int t_mask = a.P & 31 ? split - 1 : split + (sees(rt * 16) >> 5);
+    narrow_walk<D, 1, 1>(keys, t0, t1, min(t1, max(t0, t_mask)), (int)a.ks[2], (int)a.vs[2], a.c, qB, last, area(wave, 0), area(wave, 1), o, m, l);
+    narrow_join<D, 1, 8>(area, stats, o, m, l, [&](int i, int d0, float4_t v, float mm, float ll, bool once) __attribute__((always_inline)) {
+        if (rt * 16 + i < rows) put<D>(a, 0, b, kvh, rt * 16 + i, d0, v, mm, ll, once);
+    });
+#endif
+}
+
 // The rows of all sequences over shares of the prefix (the first workgroups), each sequence's rows over shares of its own keys (the others).
 template <int D, int NQ, bool WIDE>
 __global__ __launch_bounds__(256, 2) void cache_prefix_parts_kernel(const PrefixArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     TRN_LDS(D, lds);
-    __shared__ NarrowStats stats;
+    __shared__ NarrowStats<4> stats;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const bool prefix = (int)blockIdx.x < a.first;
     const int j = prefix ? blockIdx.x : blockIdx.x - a.first;
@@ -180,7 +213,7 @@ __global__ __launch_bounds__(256, 2) void cache_prefix_parts_kernel(const Prefix
         for (int i = 0; i < D / 16; ++i) o[i][qb] = float4_t{0.f, 0.f, 0.f, 0.f};
     }
     narrow_walk<D, NQ, 1>(keys, t0, t1, min(t1, max(t0, sees(rt * RT) >> 5)), keys.kpitch, keys.vpitch, a.c, qB, last, lds.k(wave), lds.v(wave), o, m, l);
-    narrow_join<D, NQ>(lds, stats, o, m, l, [&](int i, int d0, float4_t v, float mm, float ll, bool once) __attribute__((always_inline)) {
+    narrow_join<D, NQ, 4>([&](int w, int v) { return v ? lds.v(w) : lds.k(w); }, stats, o, m, l, [&](int i, int d0, float4_t v, float mm, float ll, bool once) __attribute__((always_inline)) {
         const int row = rt * RT + i;
         if (row >= all) return;
         const int b = prefix ? a.by_r.of(row) : b0, r = prefix ? row - b * a.R : row;
@@ -311,7 +344,9 @@ extern "C" int trn_cache_prefix_attn_f16(const trn_cache16* c, const trn_prefix*
         if (meet(rows_extent(o, o_stride, c->batch, n_q_heads, seq_q, c->head_dim), rows_extent(p, s3, 1, c->n_kv_heads, prefix->keys, c->head_dim))) return TRN_E_UNSUPPORTED;
         (i ? a.vps : a.kps)[0] = s2[0]; (i ? a.vps : a.kps)[1] = s2[1];
     }
-    const PlanPrefix p = plan_prefix(c->batch, c->n_kv_heads, c->capacity, c->head_dim, prefix->keys, n_q_heads, seq_q);
+    PlanPrefix p = plan_prefix(c->batch, c->n_kv_heads, c->capacity, c->head_dim, prefix->keys, n_q_heads, seq_q);
+    const bool shrt = p.short_rt > 0 && (prefix->keys == 0 || c->capacity == 0 || (prefix->k_stride[1] == c->k_stride[2] && prefix->v_stride[1] == c->v_stride[2]));
+    if (shrt) { p.slots = 1; p.bytes = 0; p.first = (int64_t)c->batch * c->n_kv_heads * p.short_rt; p.second = 0; }
     if (p.first + p.second > 0xffffff) return TRN_E_SHAPE;            // (threads in 32 bits)
     if (p.bytes && (!workspace || workspace_bytes < p.bytes)) return TRN_E_SCRATCH;
     a.k = (const half_t*)c->k; a.v = (const half_t*)c->v; a.kp = (const half_t*)prefix->k; a.vp = (const half_t*)prefix->v; a.q = (const half_t*)q; a.o = (half_t*)o;
@@ -327,7 +362,11 @@ extern "C" int trn_cache_prefix_attn_f16(const trn_cache16* c, const trn_prefix*
     const hipStream_t s = (hipStream_t)stream;
     const dim3 grid((unsigned)(p.first + p.second)), block(256);
     const bool d128 = c->head_dim == 128;
-    if (p.one) {
+    if (shrt) {
+        if (prefix->keys && !c->capacity) { a.ks[2] = prefix->k_stride[1]; a.vs[2] = prefix->v_stride[1]; }
+        if (d128) hipLaunchKernelGGL((cache_prefix_short_kernel<128>), grid, dim3(512), 0, s, a);
+        else hipLaunchKernelGGL((cache_prefix_short_kernel<64>), grid, dim3(512), 0, s, a);
+    } else if (p.one) {
         if (d128) hipLaunchKernelGGL((cache_prefix_rows_kernel<128>), grid, block, 0, s, a);
         else hipLaunchKernelGGL((cache_prefix_rows_kernel<64>), grid, block, 0, s, a);
     } else {

@@ -44,34 +44,17 @@ __global__ __launch_bounds__(256) void cache_rope_kernel(const RopeArgs a) {
     // a lane's pieces
     const bool turns = 4 * j < a.pairs;
     const int c0 = INTER || !turns ? 8 * j : 4 * j, c1 = INTER || !turns ? 8 * j + 4 : 4 * j + a.pairs;
+    // (strides by value: of a choice between members of `a` the compiler makes a load from the chosen place)
+    const int64_t q_h = a.qs[1], k_h = a.ks[1], v_h = a.vs[1], qo_h = a.qos[1], kc_h = a.kcs[1], vc_h = a.vcs[1];
     const half_t* const qp = a.q + b * a.qs[0] + i * a.qs[2];
     const half_t* const kp = a.k + b * a.ks[0] + i * a.ks[2];
     const half_t* const vp = a.v + b * a.vs[0] + i * a.vs[2];
-    const int all = a.Hq + 2 * a.Hkv, r0 = part * a.steps * RPW + rg;
-    half4_t x[AHEAD], y[AHEAD];
-    auto load = [&](int s0) __attribute__((always_inline)) {
-#pragma unroll
-        for (int e = 0; e < AHEAD; ++e) {
-            const int r = r0 + (s0 + e) * RPW;
-            const half_t* const src = r < a.Hq ? qp + r * a.qs[1] : r < a.Hq + a.Hkv ? kp + (r - a.Hq) * a.ks[1] : vp + (r - a.Hq - a.Hkv) * a.vs[1];
-            if (s0 + e < a.steps && r < all) {
-                if constexpr (INTER) {
-                    const half8_t w = __builtin_nontemporal_load(reinterpret_cast<const half8_t*>(src + c0));
-                    x[e] = half4_t{w[0], w[1], w[2], w[3]}; y[e] = half4_t{w[4], w[5], w[6], w[7]};
-                } else {
-                    x[e] = __builtin_nontemporal_load(reinterpret_cast<const half4_t*>(src + c0));
-                    y[e] = __builtin_nontemporal_load(reinterpret_cast<const half4_t*>(src + c1));
-                }
-            }
-        }
-    };
     // (the pair 4 j + rg % 4 is this lane's to find the angle of; its frequency is requested before it is known whether and where the token is)
     const int p = 4 * j + (rg & 3);
     double freq = 0.;
     if (turns) freq = a.inv[p];
     const int L = length_of(a.lengths, b, a.cap), C = count_of(a.counts, b, a.M);
     if (i >= C) return;
-    load(0);
     const int at = L - C + i;                        // (below zero: of more new tokens than keys)
     float cs = 1.f, sn = 0.f;
     if (turns) {
@@ -106,10 +89,26 @@ __global__ __launch_bounds__(256) void cache_rope_kernel(const RopeArgs a) {
     half_t* const qo = a.qo + b * a.qos[0] + i * a.qos[2];
     half_t* const kc = a.kc + b * a.kcs[0] + at * a.kcs[2];
     half_t* const vc = a.vc + b * a.vcs[0] + at * a.vcs[2];
-    const int rows = at >= 0 ? all : a.Hq;
+    const int rows = a.Hq + (at >= 0 ? 2 * a.Hkv : 0), r0 = part * a.steps * RPW + rg;
+    half4_t x[AHEAD], y[AHEAD];
+    auto load = [&](int s0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < AHEAD; ++e) {
+            const int r = r0 + (s0 + e) * RPW;
+            const half_t* const src = r < a.Hq ? qp + r * q_h : r < a.Hq + a.Hkv ? kp + (r - a.Hq) * k_h : vp + (r - a.Hq - a.Hkv) * v_h;
+            if (s0 + e >= a.steps || r >= rows) continue;
+            if constexpr (INTER) {
+                const half8_t w = __builtin_nontemporal_load(reinterpret_cast<const half8_t*>(src + c0));
+                x[e] = half4_t{w[0], w[1], w[2], w[3]}; y[e] = half4_t{w[4], w[5], w[6], w[7]};
+            } else {
+                x[e] = __builtin_nontemporal_load(reinterpret_cast<const half4_t*>(src + c0));
+                y[e] = __builtin_nontemporal_load(reinterpret_cast<const half4_t*>(src + c1));
+            }
+        }
+    };
     const float inv_d = 1.f / D;
     for (int s0 = 0; s0 < a.steps; s0 += AHEAD) {
-        if (s0) load(s0);
+        load(s0);
 #pragma unroll
         for (int e = 0; e < AHEAD; ++e) {
             const int r = r0 + (s0 + e) * RPW;
@@ -139,7 +138,7 @@ __global__ __launch_bounds__(256) void cache_rope_kernel(const RopeArgs a) {
                 w[c] = is_v ? y[e][c] : (half_t)(turns ? t[4 + c] : f[4 + c]);
             }
             if (there) {
-                half_t* const to = is_q ? qo + r * a.qos[1] : is_v ? vc + (r - a.Hq - a.Hkv) * a.vcs[1] : kc + (r - a.Hq) * a.kcs[1];
+                half_t* const to = is_q ? qo + r * qo_h : is_v ? vc + (r - a.Hq - a.Hkv) * vc_h : kc + (r - a.Hq) * kc_h;
                 if constexpr (INTER) __builtin_nontemporal_store(half8_t{u[0], u[1], u[2], u[3], w[0], w[1], w[2], w[3]}, reinterpret_cast<half8_t*>(to + c0));
                 else {
                     __builtin_nontemporal_store(u, reinterpret_cast<half4_t*>(to + c0));

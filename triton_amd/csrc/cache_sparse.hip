@@ -287,9 +287,9 @@ __device__ __forceinline__ float score64(const SelectArgs& a, const half_t* q, i
 }
 
 // A workgroup has one query of one KV head, and of its blocks' scores REGS a thread.  Scores s come with a bound e of how far they are off the definition's, r.  If t is the last of s that would be
-// taken, the last of r is within e of t: s > t + 2 e belongs to what is taken, s < t - 2 e does not, and between them the definition decides, if that is needed.  e: eight matrix instructions
-// add up to 17 numbers that are not zero each (of the two products of a channel one is zero), and may cut off 2^-23 of the largest at each: 2^-16 of the sum of the products' magnitudes, which is
-// |q| |b| at most; the rounding of r is 2^-24 of it: e = 2^-15 |q| |b| is enough.  (Products of fp16 numbers are normal in 32 bits; numbers below 2^-14 enter the pipe as they are.)
+// taken, the last of r is within e of t: s > t + 2 e belongs to what is taken, s < t - 2 e does not, and between them the definition decides, if that is needed.  e: matrix instructions add 128 products
+// (of the two of a channel one is zero) and eight earlier sums, and may cut off 2^-23 of the largest sum at each: 136 2^-23 < 1.07 2^-16 of the sum of the products' magnitudes, which is |q| |b| at
+// most; the rounding of r, and of t + 2 e, is 2^-24 each: e = 1.15 2^-16 |q| |b|.  (Products of fp16 numbers are normal in 32 bits; numbers below 2^-14 enter the pipe as they are.)
 template <int REGS> struct SelectInputs { float s[REGS], bb; };
 // All that a selection needs, requested before it is known how many blocks there are: a thread's scores, neighbours; norms; queries.
 template <int D, int T, int REGS>
@@ -357,7 +357,7 @@ __device__ __forceinline__ void select_blocks(const SelectArgs& a, SelectShared<
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < W; ++w) least = max(least, sh.least[w]);
-        const float t = unordered(~least), e2 = 2.02f * 0x1p-15f * sqrtf(__uint_as_float(nq)) * sqrtf(__uint_as_float(nb));
+        const float t = unordered(~least), e2 = 2.3f * 0x1p-16f * sqrtf(__uint_as_float(nq)) * sqrtf(__uint_as_float(nb));
         const bool bound = e2 < INFINITY;
         const float above = bound ? t + e2 : INFINITY, below = bound ? t - e2 : -INFINITY;
 #pragma unroll
@@ -536,6 +536,7 @@ struct Chosen {
     __device__ __forceinline__ const half_t* k(int t) { return kp + (int64_t)at(t) * kpitch; }
     __device__ __forceinline__ const half_t* v(int t) { return vp + (int64_t)at(t) * vpitch; }
     __device__ __forceinline__ int n(int t) { return max(0, min(32, seen - at(t))); }
+    __device__ __forceinline__ int lim(int t, int last) { return last - at(t); }
 };
 #endif
 
@@ -545,7 +546,7 @@ template <int D, int NQ, bool SELECT>
 __global__ __launch_bounds__(256, 2) void cache_sparse_attn_kernel(const SparseArgs a, const SelectArgs sel) {
 #if defined(__HIP_DEVICE_COMPILE__)
     TRN_LDS(D, lds);
-    __shared__ NarrowStats stats;
+    __shared__ NarrowStats<4> stats;
     __shared__ __attribute__((aligned(16))) SelectShared<SELECT ? 256 : 64> sh;
     __shared__ int32_t list[SELECT ? kOwnBlocks : 1];
     constexpr int RT = 16 * NQ;
@@ -593,7 +594,7 @@ __global__ __launch_bounds__(256, 2) void cache_sparse_attn_kernel(const SparseA
         for (int e = 0; e < D / 16; ++e) o[e][qb] = float4_t{0.f, 0.f, 0.f, 0.f};
     }
     narrow_walk<D, NQ, 1>(keys, t0, t1, min(t1, max(t0, whole)), keys.kpitch, keys.vpitch, a.c, qB, last, lds.k(wave), lds.v(wave), o, m, l);
-    narrow_join<D, NQ>(lds, stats, o, m, l, [&](int r, int d0, float4_t v, float mm, float ll, bool once) __attribute__((always_inline)) {
+    narrow_join<D, NQ, 4>([&](int w, int v) { return v ? lds.v(w) : lds.k(w); }, stats, o, m, l, [&](int r, int d0, float4_t v, float mm, float ll, bool once) __attribute__((always_inline)) {
         const int g = rt * RT + r;
         if (g >= a.G) return;
         if (a.ns > 1) {
@@ -732,7 +733,7 @@ extern "C" int trn_cache_sparse_attn_f16(const trn_cache16* c, const void* bound
     const int steps = many ? (waves > 4096 ? 4 : 1) : (int)(waves <= 2048 ? 1 : waves / 2048 < 8 ? waves / 2048 : 8);
     const int per64 = 4 * 512 / c->head_dim * steps;
     const dim3 score_grid((unsigned)(many ? (p.nb + (int64_t)per64 - 1) / per64 : p.nbp / 64), (unsigned)(many ? p.step : (q_tiles + steps - 1) / steps), (unsigned)heads);
-    const int threads = p.nb > 1024 && !many ? 1024 : p.nb <= 512 ? 128 : 256;
+    const int threads = many ? 256 : p.nb > 6144 ? 1024 : p.nb > 1024 ? 512 : p.nb > 512 ? 256 : 128;
     const bool own = !p.rows && p.nb > top && p.nb <= kOwnBlocks && p.step == seq_q;       // (the attention's workgroups select)
     if (groups > 0xffffff || heads > 65535 || heads * p.step * ((threads + 255) / 256) > 0xffffff || (int64_t)score_grid.x * score_grid.y * score_grid.z > 0xffffff) return TRN_E_SHAPE;
     const hipStream_t s = (hipStream_t)stream;
@@ -747,7 +748,7 @@ extern "C" int trn_cache_sparse_attn_f16(const trn_cache16* c, const void* bound
         a.norms = (float*)((char*)workspace + p.norms);
         for (int i = 0; i < 3; ++i) a.qs[i] = q_stride[i];
         a.by_hkv = Div(c->n_kv_heads); a.by_n = Div(a.n);
-        if (p.nb > top) {      // (a.n is at most 65535: 64 MB of at least 64 floats a query)
+        if (p.nb > top) {      // (grid.y: 64 MB of scores, 64 of them at least, are 262144 queries, 16 a workgroup; 2048 where there are many blocks)
             dim3 grid = score_grid;
             grid.y = (unsigned)(many ? a.n : ((by_heads ? a.n : (a.n + 15) / 16) + steps - 1) / steps);
             if (many) {
@@ -769,10 +770,12 @@ extern "C" int trn_cache_sparse_attn_f16(const trn_cache16* c, const void* bound
         else if (d128) {
             if (threads == 128) hipLaunchKernelGGL((cache_select_kernel<128, 128, 4>), grid, dim3(128), 0, s, a);
             else if (threads == 256) hipLaunchKernelGGL((cache_select_kernel<128, 256, 4>), grid, dim3(256), 0, s, a);
+            else if (threads == 512) hipLaunchKernelGGL((cache_select_kernel<128, 512, 12>), grid, dim3(512), 0, s, a);
             else hipLaunchKernelGGL((cache_select_kernel<128, 1024, 8>), grid, dim3(1024), 0, s, a);
         } else {
             if (threads == 128) hipLaunchKernelGGL((cache_select_kernel<64, 128, 4>), grid, dim3(128), 0, s, a);
             else if (threads == 256) hipLaunchKernelGGL((cache_select_kernel<64, 256, 4>), grid, dim3(256), 0, s, a);
+            else if (threads == 512) hipLaunchKernelGGL((cache_select_kernel<64, 512, 12>), grid, dim3(512), 0, s, a);
             else hipLaunchKernelGGL((cache_select_kernel<64, 1024, 8>), grid, dim3(1024), 0, s, a);
         }
         e = hipGetLastError();

@@ -694,6 +694,63 @@ class CacheSparseAttention(FusedModule):
         return host.cache_sparse_attention(ws, self.scale, self.block, self.top, self.sink, self.recent, K, O, Q, V, bounds, counts, lengths, selected)
 
 
+class _CacheStep(FusedModule):
+    """What the steps on an fp16 cache share: X [B,M,N] projected (norm=True: RMS-normalised first, no weight), queries and keys normalised by head (qk_norm=True) and rotated, keys and
+    values put into the cache (`ops.cache_rope_append`, whose arguments positions, gammas, inv_freq, lengths and counts are)."""
+
+    def __init__(self, head_dim: int, scale: Optional[float] = None, norm: bool = False, eps: float = 0.0, qk_norm: bool = False, qk_eps: float = 1e-6, interleaved: bool = False,
+                 sections=None):
+        super().__init__()
+        self.head_dim, self.scale, self.norm, self.eps = head_dim, scale, norm, eps
+        self.qk_norm, self.qk_eps, self.interleaved, self.sections = qk_norm, qk_eps, interleaved, None if sections is None else list(sections)
+
+    def _put(self, K_cache, O2, V_cache, WK, WQ, WV, X, counts, gamma_k, gamma_q, inv_freq, lengths, positions):
+        """The step's queries, and O2, as [B,Hq,M,D]."""
+        D = self.head_dim
+        if X.dim() != 3 or O2.dim() != 3 or WQ.dim() != 2 or WK.dim() != 2 or WQ.shape[1] % D or WK.shape[1] % D:
+            raise ValueError(f"inconsistent shapes: X {tuple(X.shape)}, O2 {tuple(O2.shape)}, WQ {tuple(WQ.shape)}, WK {tuple(WK.shape)}, head_dim {D}")
+        if not X.is_contiguous() or not O2.is_contiguous():
+            raise ValueError("X, O2: expected contiguous tensors")
+        B, M, N = X.shape
+        nq, nkv = WQ.shape[1], WK.shape[1]
+        if O2.shape != (B, M, nq):
+            raise ValueError(f"O2 {tuple(O2.shape)}: expected {(B, M, nq)}")
+        qkv = self._workspace("qkv", (B * M, nq + 2 * nkv), X.dtype, X.device)
+        parts = [(t, t.shape[1] // D) for t in (qkv[:, :nq], qkv[:, nq:nq + nkv], qkv[:, nq + nkv:])]
+        if B * M:
+            ops.prenorm_qkv(X.view(B * M, N), None, WQ, WK, WV, *(t.view(B * M, h, D).permute(1, 0, 2) for t, h in parts), self.eps, self.norm)      # [head, token, D]
+        q, k, v = (t.view(B, M, h, D).permute(0, 2, 1, 3) for t, h in parts)      # [B, H, M, D]
+        self._host.cache_rope_append(self.qk_norm, self.qk_eps, self.interleaved, self.sections, k, K_cache, q, q, v, V_cache, counts, gamma_k, gamma_q, inv_freq, lengths, positions)
+        return q, O2.view(B, M, nq // D, D).permute(0, 2, 1, 3)
+
+
+class CacheStep(_CacheStep):
+    """The decode-append step (ref_rms.py:45-83, 101-127, 197-231) on an fp16 cache of a batch whose sequences have lengths of their own, with positions, behind a prefix that they
+    share (K_prefix, V_prefix [Hkv,P,D]; P may be 0): X [B,M,N], O2 [B,M,Hq*D].  Three launches, or four with shares of the keys."""
+    TENSOR_PARAMS = ["K_cache", "K_prefix", "O2", "V_cache", "V_prefix", "WK", "WQ", "WV", "X", "counts", "gamma_k", "gamma_q", "inv_freq", "lengths", "positions"]
+
+    def _run(self, K_cache, K_prefix, O2, V_cache, V_prefix, WK, WQ, WV, X, counts, gamma_k, gamma_q, inv_freq, lengths, positions):
+        q, o = self._put(K_cache, O2, V_cache, WK, WQ, WV, X, counts, gamma_k, gamma_q, inv_freq, lengths, positions)
+        self._host.cache_prefix_attention(self._hws, self.scale, True, K_cache, K_prefix, o, q, V_cache, V_prefix, counts, lengths)
+
+
+class CacheSparseStep(_CacheStep):
+    """CacheStep without a prefix whose queries attend over the blocks that they select (`ops.cache_bounds`, `ops.cache_sparse_attention`)."""
+    TENSOR_PARAMS = ["K_cache", "O2", "V_cache", "WK", "WQ", "WV", "X", "bounds", "counts", "gamma_k", "gamma_q", "inv_freq", "lengths", "positions", "selected"]
+
+    def __init__(self, head_dim: int, top: int, sink: int = 0, recent: int = 1, block: int = 64, **kw):
+        super().__init__(head_dim, **kw)
+        if top < 1 or sink < 0 or recent < 1 or sink + recent > top:
+            raise ValueError("top, sink, recent: expected sink >= 0, recent >= 1, sink + recent <= top")
+        self.top, self.sink, self.recent, self.block = top, sink, recent, block
+
+    def _run(self, K_cache, O2, V_cache, WK, WQ, WV, X, bounds, counts, gamma_k, gamma_q, inv_freq, lengths, positions, selected):
+        q, o = self._put(K_cache, O2, V_cache, WK, WQ, WV, X, counts, gamma_k, gamma_q, inv_freq, lengths, positions)
+        self._host.cache_bounds(self.block, X.shape[1], K_cache, bounds, counts, lengths)
+        self._host.cache_sparse_attention(self._hws, self.scale, self.block, self.top, self.sink, self.recent, K_cache, o, q, V_cache, bounds, counts, lengths, selected)
+
+
+CACHE16 = {"prefix": CacheStep, "prenorm": lambda **kw: CacheStep(norm=True, **kw), "sparse": CacheSparseStep}
 CACHE8 = {"vanilla": Cache8Step, "prenorm": lambda **kw: Cache8Step(norm=True, **kw), "weights": Cache8StepWeights}
 CACHE = {"append8": Cache8Append, "attn8": Cache8Attention, "weights8": Cache8KeyWeights, "evict": CacheEvict, "evict8": Cache8Evict,
          "rope": CacheRope, "prefix": CachePrefixAttention, "bounds": CacheBounds, "sparse": CacheSparseAttention}
@@ -714,9 +771,10 @@ def get(variant: str, form: str = "prefill", **consts) -> FusedModule:
     form='decode' : the reference's decode-append problem (needs head_dim=...).
     form='linear' : the reference's LoRA and gated-MLP workloads.
     form='cache8' : the decode-append step on an 8-bit cache, {'vanilla','prenorm','weights'} (needs head_dim=...).
+    form='cache16': that step on an fp16 cache of sequences of their own lengths, with positions, {'prefix','prenorm','sparse'} (needs head_dim=...).
     form='cache'  : an 8-bit cache's append, attention and key weights, and eviction, {'append8','attn8','weights8','evict','evict8'};
                     an fp16 cache's rotated append, attention behind a shared prefix and over selected blocks, {'rope','prefix','bounds','sparse'}."""
-    table = {"prefill": PREFILL, "decode": DECODE, "linear": LINEAR, "cache": CACHE, "cache8": CACHE8}.get(form)
+    table = {"prefill": PREFILL, "decode": DECODE, "linear": LINEAR, "cache": CACHE, "cache8": CACHE8, "cache16": CACHE16}.get(form)
     if table is None or variant not in table:
         raise KeyError(f"no module for variant={variant!r} form={form!r}")
     return table[variant](**consts)
