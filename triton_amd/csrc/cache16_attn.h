@@ -260,9 +260,10 @@ __device__ __forceinline__ void narrow_join(Area area, NarrowStats<NW>& st, floa
 // ------------------------------------------------------------------------------------------------ wide
 // A workgroup's tiles t0 <= t < t1 of 32 keys for 128 rows, of which this wave has 32 (none: idle).  keys: where a tile begins (.k, .v),
 // the pitches there, how many keys lie from there on at these (.left), whether tiles are there as a whole (.whole), and up to which key of a tile a row sees (.lim).
+// FINE: p enters the product with V as two numbers, as in the narrow form; as one its error is about the output's own, and averages out over many rows.
 // Four stages: a tile is requested three tiles ahead, so that a workgroup alone on its compute unit has 48 KB on their way.
-template <int D, class Keys>
-__device__ __forceinline__ void wide_walk(const Keys& keys, int t0, int t1, int t_mask, bool idle, float c, const half8_t (&qB)[D / 16], int last, const Lds<D>& lds, float16_t (&o)[D / 32], float& m, float& l) {
+template <int D, bool FINE, class Keys>
+__device__ __forceinline__ void wide_walk(const Keys keys, int t0, int t1, int t_mask, bool idle, float c, const half8_t (&qB)[D / 16], int last, const Lds<D>& lds, float16_t (&o)[D / 32], float& m, float& l) {
     constexpr int NS = D / 16, NDB = D / 32, CPR = D / 8, RPI = 64 / CPR, NL = 32 / (4 * RPI);
     const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (t0 >= t1) return;
@@ -341,13 +342,14 @@ __device__ __forceinline__ void wide_walk(const Keys& keys, int t0, int t1, int 
             for (int i = 0; i < NDB; ++i) o[i] = o[i] * alpha;
         }
         const float d = m == -INFINITY ? 0.f : -m;
-        half8_t p[2];
+        half8_t p[2], rest[2];
         float sum[4];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             const float x = fast_exp2(__builtin_fmaf(s[e], c, d));
             sum[e & 3] = e < 4 ? x : sum[e & 3] + x;
             p[e >> 3][e & 7] = (half_t)x;
+            if constexpr (FINE) rest[e >> 3][e & 7] = (half_t)(x - (float)p[e >> 3][e & 7]);
         }
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         bool odd = false;
@@ -384,6 +386,7 @@ __device__ __forceinline__ void wide_walk(const Keys& keys, int t0, int t1, int 
                 if constexpr (MASK) { v = value(u, i); if (__builtin_expect(odd, 0)) v = finite_only(v); }
                 else v = vw[u][i];
                 o[i] = mfma32(v, p[u], o[i]);
+                if constexpr (FINE) o[i] = mfma32(v, rest[u], o[i]);
             }
     };
     ahead(lds.k0, lds.v0); ahead(lds.k1, lds.v1); ahead(lds.k2, lds.v2);

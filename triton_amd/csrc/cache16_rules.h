@@ -10,7 +10,8 @@ inline int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 // sequence, in narrow ones of 16 nq rows, over its own keys.  n_rt row tiles and ns shares of their keys (_p, _o; one: _p); slots: results of a row to be joined (one: none);
 // first, second: workgroups of both parts; ml: offset of the statistics in the workspace, bytes: its size.
 // short_rt: row tiles of eight waves each that have all keys, where pitches allow.
-struct PlanPrefix { bool one, wide; int short_rt; int G, R, nq, n_rt_p, ns_p, n_rt_o, ns_o, slots; int64_t first, second, ml, bytes; };
+// fine: weights as two fp16 numbers in the first of these, where all heads together have up to 512 rows (else everywhere).
+struct PlanPrefix { bool one, wide, fine; int short_rt; int G, R, nq, n_rt_p, ns_p, n_rt_o, ns_o, slots; int64_t first, second, ml, bytes; };
 
 inline PlanPrefix plan_prefix(int batch, int n_kv_heads, int capacity, int head_dim, int prefix, int Hq, int Sq) {
     PlanPrefix p{};
@@ -18,6 +19,7 @@ inline PlanPrefix plan_prefix(int batch, int n_kv_heads, int capacity, int head_
     p.R = p.G * Sq;
     const int64_t heads = (int64_t)batch * n_kv_heads, rows_p = (int64_t)batch * p.R;
     p.one = p.R > 64;
+    p.fine = heads * p.R <= 512;
     const int64_t tiles16 = (p.R + 15) / 16;
     // (as long as a wave's tiles, one after the other, take less than a second launch.  One query of 32 heads of 128 on 8, us by shares / by eight waves: one sequence, 60 keys behind 200 9.2 / 6.4, behind
     // 1000 9.7 / 10.4; 8 sequences 12.7 / 10.6, 500 behind 1000 13.3 / 13.5; 32 (wide tiles) 26.8 / 17.0, 60 behind 3000 24.4 / 20.9 before those had shares of 128 keys, 18.7 with them; 16 heads of

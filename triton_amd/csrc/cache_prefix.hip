@@ -62,8 +62,8 @@ __device__ __forceinline__ const half_t* query(const PrefixArgs& a, int b, int k
 #endif
 
 // Tiles of 128 rows of one sequence, over the prefix and its own keys.
-template <int D>
-__global__ __launch_bounds__(256, D == 128 ? 2 : 4) void cache_prefix_rows_kernel(const PrefixArgs a) {
+template <int D, bool FINE>
+__global__ __launch_bounds__(256, D == 128 ? 2 : FINE ? 3 : 4) void cache_prefix_rows_kernel(const PrefixArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
     TRN_LDS(D, lds);
     const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -87,7 +87,7 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : 4) void cache_prefix_rows_kerne
     for (int i = 0; i < D / 32; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
-    wide_walk<D>(keys, t0, t1, split + (sees(min(r0, rows - 1)) >> 5), r0 >= rows, a.c, qB, sees(min(row, rows - 1)) - 1, lds, o, m, l);
+    wide_walk<D, FINE>(keys, t0, t1, split + (sees(min(r0, rows - 1)) >> 5), r0 >= rows, a.c, qB, sees(min(row, rows - 1)) - 1, lds, o, m, l);
     if (row >= rows) return;
     l = half_sum(l);
 #pragma unroll
@@ -161,7 +161,7 @@ __global__ __launch_bounds__(256, 2) void cache_prefix_parts_kernel(const Prefix
         for (int i = 0; i < D / 32; ++i)
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
-        wide_walk<D>(keys, a.by_nsp.of(T * share), a.by_nsp.of(T * (share + 1)), T, __builtin_amdgcn_ballot_w64(there) == 0, a.c, qB, a.P - 1, lds, o, m, l);
+        wide_walk<D, true>(keys, a.by_nsp.of(T * share), a.by_nsp.of(T * (share + 1)), T, __builtin_amdgcn_ballot_w64(there) == 0, a.c, qB, a.P - 1, lds, o, m, l);
         if (!there) return;
         l = half_sum(l);
 #pragma unroll
@@ -367,8 +367,13 @@ extern "C" int trn_cache_prefix_attn_f16(const trn_cache16* c, const trn_prefix*
         if (d128) hipLaunchKernelGGL((cache_prefix_short_kernel<128>), grid, dim3(512), 0, s, a);
         else hipLaunchKernelGGL((cache_prefix_short_kernel<64>), grid, dim3(512), 0, s, a);
     } else if (p.one) {
-        if (d128) hipLaunchKernelGGL((cache_prefix_rows_kernel<128>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((cache_prefix_rows_kernel<64>), grid, block, 0, s, a);
+        if (p.fine) {
+            if (d128) hipLaunchKernelGGL((cache_prefix_rows_kernel<128, true>), grid, block, 0, s, a);
+            else hipLaunchKernelGGL((cache_prefix_rows_kernel<64, true>), grid, block, 0, s, a);
+        } else {
+            if (d128) hipLaunchKernelGGL((cache_prefix_rows_kernel<128, false>), grid, block, 0, s, a);
+            else hipLaunchKernelGGL((cache_prefix_rows_kernel<64, false>), grid, block, 0, s, a);
+        }
     } else {
         auto launch = [&](auto nq, auto wide) {
             constexpr int NQ = decltype(nq)::value;
