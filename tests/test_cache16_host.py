@@ -127,8 +127,9 @@ def test_sparse_and_bounds_statuses(lib):
     for kw in (dict(block=48), dict(block=256), dict(top=(1 << 16) + 1), dict(o=P + 64), dict(o=P + 2 * M + 128)):
         assert _sparse(lib, **kw) == "TRN_E_UNSUPPORTED", kw
     assert _sparse(lib, bounds=P + 6 * M + 8) == "TRN_E_ALIGN" and _sparse(lib, sel=P + 2) == "TRN_E_ALIGN"
-    need = lib.trn_cache_sparse_attn_workspace_bytes(C.byref(_cache()), 32, 4, 4, 3)
-    assert need > 0 and _sparse(lib, n=need) == "TRN_E_LAUNCH" and _sparse(lib, n=need - 1) == "TRN_E_SCRATCH" and _sparse(lib, ws=None) == "TRN_E_SCRATCH"
+    assert lib.trn_cache_sparse_attn_workspace_bytes(C.byref(_cache()), 32, 4, 4, 3) == 0 and _sparse(lib, ws=None) == "TRN_E_LAUNCH"      # four blocks, all selected
+    need = lib.trn_cache_sparse_attn_workspace_bytes(C.byref(_cache()), 32, 3, 4, 3)
+    assert need > 0 and _sparse(lib, top=3, n=need) == "TRN_E_LAUNCH" and _sparse(lib, top=3, n=need - 1) == "TRN_E_SCRATCH" and _sparse(lib, top=3, ws=None) == "TRN_E_SCRATCH"
     assert lib.trn_cache_sparse_attn_workspace_bytes(C.byref(_cache()), 48, 4, 4, 3) == 0
     bounds = lambda block=32, tokens=1, to=P + 6 * M, **kw: _name(lib, lib.trn_cache_bounds_f16(C.byref(_cache(v=None, **kw)), block, tokens, to, None))
     assert bounds() == "TRN_E_LAUNCH" and bounds(tokens=0) == "TRN_OK" and bounds(capacity=0) == "TRN_OK" and bounds(block=16) == "TRN_E_UNSUPPORTED"
@@ -180,13 +181,13 @@ int main() {
         ++plans;
         const int64_t heads = (int64_t)batch * kv;
         bool ok = p.R == g * sq && p.slots >= 1 && (p.slots == 1) == (p.bytes == 0) && (p.nq == 1 || p.nq == 2);
-        if (p.one) ok = ok && p.slots == p.ns_p && (int64_t)p.n_rt_p * 128 >= p.R && p.first == heads * p.n_rt_p * p.ns_p && p.second == 0 && p.short_rt == 0;
+        if (p.one) ok = ok && p.slots == p.ns_p && (int64_t)p.n_rt_p * 128 >= p.R && p.first == heads * p.n_rt_p * p.ns_p && p.second == 0;
         else {
             const int64_t rows_p = (int64_t)batch * p.R;
             ok = ok && p.slots == p.ns_p + p.ns_o && (p.ns_p > 0) == (pre > 0) && (p.ns_o > 0 || cap == 0) && (p.ns_o > 0 || pre > 0) && p.ns_p <= 64 && p.ns_o <= 64;
             ok = ok && (int64_t)p.n_rt_p * (p.wide ? 128 : 16 * p.nq) >= rows_p && (int64_t)p.n_rt_o * 16 * p.nq >= p.R && p.first == (int64_t)kv * p.n_rt_p * p.ns_p && p.second == heads * p.n_rt_o * p.ns_o;
-            if (p.short_rt) ok = ok && p.short_rt * 16 >= p.R;
         }
+        if (p.short_rt) ok = ok && p.short_rt * 16 >= p.R;
         if (p.slots > 1) ok = ok && p.ml >= heads * p.R * p.slots * d * 4 && p.bytes >= p.ml + heads * p.R * p.slots * 8;
         if (!ok) { if (bad < 5) printf("prefix %d %d %d %d %d %d %d\n", batch, kv, g, sq, d, cap, pre); ++bad; }
     }
@@ -196,6 +197,11 @@ int main() {
         const PlanSparse p = plan_sparse(batch, kv, cap, d, block, top, kv * g, sq);
         ++plans;
         const int64_t heads = (int64_t)batch * kv;
+        if (p.dense) {
+            const bool good = p.nb <= top && p.step >= 1 && p.step <= sq && heads * p.step <= 0xffffff && p.bytes == plan_prefix(batch, kv, cap, d, 0, kv * g, sq).bytes;
+            if (!good) { if (bad < 5) printf("dense %d %d %d %d %d %d %d %d\n", batch, kv, g, sq, d, block, cap, top); ++bad; }
+            continue;
+        }
         bool ok = p.nbp >= p.nb && p.nbp % 64 == 0 && p.step >= 1 && p.step <= sq && p.norms >= heads * p.nbp * 4 * p.step && p.o >= p.norms + heads * p.nbp / 16 * 4 && p.n_rt * 16 * p.nq >= g;
         ok = ok && p.ns >= 1 && (!p.rows || p.ns == 1) && (p.ns == 1 ? p.bytes == p.o : p.ml >= p.o + heads * sq * g * p.ns * d * 4 && p.bytes >= p.ml + heads * sq * g * p.ns * 8);
         if (!ok) { if (bad < 5) printf("sparse %d %d %d %d %d %d %d %d\n", batch, kv, g, sq, d, block, cap, top); ++bad; }

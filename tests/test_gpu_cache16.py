@@ -251,6 +251,12 @@ def test_selection_of_equals_and_of_what_is_no_number():
         assert got == sorted([0, 598, 599] + rest)
 
 
+def test_all_blocks_of_a_long_chunk():
+    """No more blocks than places: the attention over the whole cache, and the selection says so."""
+    for case in ((2, 8, 2, 128, 150, 260, [260, 150], [150, 97], 64, 5, 1, 1), (1, 71, 1, 64, 2, 3000, [2999], [2], 128, 24, 0, 1)):
+        test_sparse_attention(case, "token")
+
+
 MANY = [
     # as SPARSES: blocks of more than 2048, and of more than a workgroup holds
     (1, 4, 1, 64, 2, 32 * 3001, [32 * 3000 + 5], [2], 32, 33, 1, 2),
@@ -296,6 +302,8 @@ PATHS = [
     (2, 4, 2, 128, 40, 0, [0, 0], [40, 3], 70, True),
     (2, 4, 2, 64, 2, 0, [0, 0], [2, 1], 0, True),
     (1, 8, 8, 128, 1, 700, [1], [1], 0, True),
+    (3, 71, 1, 64, 1, 20, [20, 1, 7], [1, 1, 1], 5000, True),
+    (2, 71, 1, 64, 3, 100, [100, 50], [3, 2], 300, True),
 ]
 
 
@@ -509,7 +517,8 @@ def test_refusals():
     bad(block=48); bad(block=32); bad(bounds=bnd.float()); bad(bounds=bnd[0]); bad(k=k[0]); bad(tokens=-1); bad(counts=n1)
     ws = torch.zeros(1 << 20, dtype=torch.uint8, device=DEV)
     bad = tried(ops.cache_sparse_attention, dict(q=q, k=k, v=v, bounds=bnd, o=o, selected=sel, top=3, workspace=ws))
-    bad(top=2); bad(top=3, recent=0); bad(sink=3); bad(selected=sel.long()); bad(selected=sel[..., :2]); bad(bounds=half(1, 2, 2, 2, 64)); bad(block=96); bad(_lib.TrnError, workspace=None)
+    bad(top=2); bad(top=3, recent=0); bad(sink=3); bad(selected=sel.long()); bad(selected=sel[..., :2]); bad(bounds=half(1, 2, 2, 2, 64)); bad(block=96)
+    bad(_lib.TrnError, block=32, bounds=half(1, 2, 2, 2, 64), selected=sel[..., :1].contiguous(), top=1, workspace=None)
     bad(_lib.TrnError, scale=-1.0); bad(v=v.float()); bad(_lib.TrnError, q=half(1, 4, 2, 72)[..., 4:68])
     step = modules.get("prefix", "cache16", head_dim=64)
     with pytest.raises(ValueError):

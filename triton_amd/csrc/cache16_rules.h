@@ -1,5 +1,6 @@
 // How the work of an attention over fp16 caches is laid out (cache_prefix.hip, cache_sparse.hip): plain host arithmetic.
 #pragma once
+#include <cmath>
 #include <cstdint>
 
 namespace trn {
@@ -18,7 +19,8 @@ inline PlanPrefix plan_prefix(int batch, int n_kv_heads, int capacity, int head_
     p.G = Hq / n_kv_heads;
     p.R = p.G * Sq;
     const int64_t heads = (int64_t)batch * n_kv_heads, rows_p = (int64_t)batch * p.R;
-    p.one = p.R > 64;
+    // (rows of all sequences fill tiles better than those of each: up to one tile of these, where the prefix is what there is to read)
+    p.one = p.R > 64 && !(p.R <= 128 && prefix > 4 * (int64_t)capacity && batch > 1);
     p.fine = heads * p.R <= 512;
     const int64_t tiles16 = (p.R + 15) / 16;
     // (as long as a wave's tiles, one after the other, take less than a second launch.  One query of 32 heads of 128 on 8, us by shares / by eight waves: one sequence, 60 keys behind 200 9.2 / 6.4, behind
@@ -26,7 +28,7 @@ inline PlanPrefix plan_prefix(int batch, int n_kv_heads, int capacity, int head_
     // 64, 4 sequences, 60 behind 1000 8.9 / 7.6, 500 behind 1000 9.1 / 9.0, 60 behind 3000 9.8 / 11.4.)
     const bool shared = prefix > 0 && rows_p > 32;
     const int64_t rounds = (heads * tiles16 + 255) / 256, most = head_dim == 128 ? (shared ? 1800 : 1000) : (shared ? 2500 : 1500);
-    if (p.R <= 64 && rounds <= 2 && rounds * ((int64_t)prefix + capacity) <= most) p.short_rt = (int)tiles16;
+    if (rounds <= 2 && rounds * ((int64_t)prefix + capacity) <= most) p.short_rt = (int)tiles16;
     if (p.one) {
         p.wide = true; p.nq = 2;
         p.n_rt_p = (p.R + 127) / 128;
@@ -42,8 +44,9 @@ inline PlanPrefix plan_prefix(int batch, int n_kv_heads, int capacity, int head_
         p.n_rt_p = (int)(p.wide ? (rows_p + 127) / 128 : (rows_p + 16 * p.nq - 1) / (16 * p.nq));
         p.n_rt_o = (p.R + 16 * p.nq - 1) / (16 * p.nq);
         const int64_t units_p = (int64_t)n_kv_heads * p.n_rt_p, units_o = heads * p.n_rt_o;
-        // Workgroups of both parts run at once, two a compute unit: these are shared out by the parts' work (a wide tile's key counts twice), in shares of 256 keys at least, 512 of a wide
-        // tile.  32 sequences of 700 keys behind 8192, 32 heads of 128 on 8, us with 8 / 16 / 32 shares of the prefix: 31.6 + 4.8 for the joining / 24.9 + 4.8 / 27.6 + 5.9.
+        // Workgroups of both parts run at once, two a compute unit: these are shared out by the parts' work (a wide tile's key counts twice), in shares of 256 keys at least, 128 of a wide
+        // tile.  There a key takes some 0.016 us, and a share more is written and read again, 8 head_dim bytes a row at 4 TB/s: P / ns keys and ns shares take the least time at the root of the ratio.
+        // 32 heads of 128 on 8, 32 sequences of 700 keys behind 8192, us with 8 / 16 / 32 shares of the prefix: 31.6 + 4.8 for the joining / 24.9 + 4.8 / 27.6 + 5.9.
         const int64_t cost_p = units_p * prefix * (p.wide ? 2 : 1), cost_o = units_o * capacity, cost = cost_p + cost_o;
         auto shares = [](int64_t groups, int64_t units, int64_t keys, int64_t least) {
             int64_t s = groups / units;
@@ -51,7 +54,10 @@ inline PlanPrefix plan_prefix(int batch, int n_kv_heads, int capacity, int head_
             return (int)(keys == 0 ? 0 : s < 1 ? 1 : s > 64 ? 64 : s);
         };
         p.ns_p = shares(cost ? 512 * cost_p / cost : 0, units_p, prefix, p.wide ? 128 : 256);
-        if (p.wide && p.ns_p > 16) p.ns_p = 16;
+        if (p.wide && p.ns_p > 1) {
+            const int best = (int)std::sqrt(0.016 * prefix / (0.1 + (double)heads * p.R * head_dim * 2e-6));
+            if (p.ns_p > best) p.ns_p = best < 1 ? 1 : best;
+        }
         p.ns_o = shares(cost ? 512 * cost_o / cost : 0, units_o, capacity, 256);
         if (p.ns_p + p.ns_o == 0) p.ns_o = 1;      // (nothing to see: zeros)
         p.slots = p.ns_p + p.ns_o;
@@ -69,7 +75,8 @@ constexpr int kMostBlocks = 8192;
 
 // Selected blocks: a query's scores in rows of nbp floats, `step` queries of each head at a time; row tiles of 16 nq of a KV head's query heads, ns shares of a query's keys; offsets of
 // the shares' parts behind the scores and the norms; rows: a wave a row tile rather than a workgroup.
-struct PlanSparse { int G, nb, nq, n_rt, ns, step; bool rows; int64_t nbp, norms, o, ml, bytes; };
+// dense: all blocks are selected, and the attention is that over the cache, without a prefix.
+struct PlanSparse { int G, nb, nq, n_rt, ns, step; bool rows, dense; int64_t nbp, norms, o, ml, bytes; };
 
 inline PlanSparse plan_sparse(int batch, int n_kv_heads, int capacity, int head_dim, int block, int top, int Hq, int Sq) {
     PlanSparse p{};
@@ -77,6 +84,13 @@ inline PlanSparse plan_sparse(int batch, int n_kv_heads, int capacity, int head_
     p.nb = (capacity + block - 1) / block;
     p.nbp = (p.nb + 63) / 64 * 64;
     const int64_t heads = (int64_t)batch * n_kv_heads, row = heads * p.nbp * 4;
+    p.dense = p.nb <= top;
+    if (p.dense) {
+        p.step = (int)(0xffffff / heads < Sq ? 0xffffff / heads : Sq);
+        p.ns = 1;
+        p.bytes = plan_prefix(batch, n_kv_heads, capacity, head_dim, 0, Hq, Sq).bytes;
+        return p;
+    }
     int64_t step = row ? (64 << 20) / row : Sq;
     p.step = (int)(step < 1 ? 1 : step > Sq ? Sq : step);
     p.nq = p.G > 16 ? 2 : 1;

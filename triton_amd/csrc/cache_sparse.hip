@@ -725,6 +725,21 @@ extern "C" int trn_cache_sparse_attn_f16(const trn_cache16* c, const void* bound
     const int64_t heads = (int64_t)c->batch * c->n_kv_heads;
     const PlanSparse p = plan_sparse(c->batch, c->n_kv_heads, c->capacity, c->head_dim, block, top, n_q_heads, seq_q);
     if (p.bytes && (!workspace || workspace_bytes < p.bytes)) return TRN_E_SCRATCH;
+    if (p.dense) {
+        if (p.step < 1) return TRN_E_SHAPE;
+        SelectArgs a{};
+        a.lengths = c->lengths; a.counts = c->counts; a.selected = selected;
+        a.B = c->batch; a.Hkv = c->n_kv_heads; a.M = seq_q; a.cap = c->capacity; a.G = p.G; a.block_shift = shift_of(block); a.nb = p.nb; a.top = top; a.sink = sink; a.recent = recent;
+        a.by_hkv = Div(c->n_kv_heads);
+        for (int64_t i0 = 0; i0 < seq_q; i0 += p.step) {
+            a.i0 = (int)i0; a.n = (int)(seq_q - i0 < p.step ? seq_q - i0 : p.step);
+            a.by_n = Div(a.n);
+            hipLaunchKernelGGL(cache_select_many_kernel, dim3((unsigned)(heads * a.n)), dim3(256), 0, (hipStream_t)stream, a);
+            if (hipGetLastError() != hipSuccess) return TRN_E_LAUNCH;
+        }
+        const trn_prefix none{};
+        return trn_cache_prefix_attn_f16(c, &none, q, o, n_q_heads, seq_q, q_stride, o_stride, scale, 1, workspace, workspace_bytes, stream);
+    }
     const int64_t groups = p.rows ? heads * (((int64_t)seq_q * p.n_rt + 3) / 4) : heads * seq_q * p.n_rt * p.ns;
     // (workgroups of 256, and as many threads in all as 32 bits number: of every launch, before the first one)
     const bool many = p.nb > kMostBlocks;
@@ -734,7 +749,7 @@ extern "C" int trn_cache_sparse_attn_f16(const trn_cache16* c, const void* bound
     const int per64 = 4 * 512 / c->head_dim * steps;
     const dim3 score_grid((unsigned)(many ? (p.nb + (int64_t)per64 - 1) / per64 : p.nbp / 64), (unsigned)(many ? p.step : (q_tiles + steps - 1) / steps), (unsigned)heads);
     const int threads = many ? 256 : p.nb > 6144 ? 1024 : p.nb > 1024 ? 512 : p.nb > 512 ? 256 : 128;
-    const bool own = !p.rows && p.nb > top && p.nb <= kOwnBlocks && p.step == seq_q;       // (the attention's workgroups select)
+    const bool own = !p.rows && p.nb <= kOwnBlocks && p.step == seq_q;       // (the attention's workgroups select)
     if (groups > 0xffffff || heads > 65535 || heads * p.step * ((threads + 255) / 256) > 0xffffff || (int64_t)score_grid.x * score_grid.y * score_grid.z > 0xffffff) return TRN_E_SHAPE;
     const hipStream_t s = (hipStream_t)stream;
     const bool d128 = c->head_dim == 128;
@@ -748,7 +763,7 @@ extern "C" int trn_cache_sparse_attn_f16(const trn_cache16* c, const void* bound
         a.norms = (float*)((char*)workspace + p.norms);
         for (int i = 0; i < 3; ++i) a.qs[i] = q_stride[i];
         a.by_hkv = Div(c->n_kv_heads); a.by_n = Div(a.n);
-        if (p.nb > top) {      // (grid.y: 64 MB of scores, 64 of them at least, are 262144 queries, 16 a workgroup; 2048 where there are many blocks)
+        {      // (grid.y: 64 MB of scores, 64 of them at least, are 262144 queries, 16 a workgroup; 2048 where there are many blocks)
             dim3 grid = score_grid;
             grid.y = (unsigned)(many ? a.n : ((by_heads ? a.n : (a.n + 15) / 16) + steps - 1) / steps);
             if (many) {
