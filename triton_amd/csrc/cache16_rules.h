@@ -45,7 +45,7 @@ inline PlanPrefix plan_prefix(int batch, int n_kv_heads, int capacity, int head_
         p.n_rt_o = (p.R + 16 * p.nq - 1) / (16 * p.nq);
         const int64_t units_p = (int64_t)n_kv_heads * p.n_rt_p, units_o = heads * p.n_rt_o;
         // Workgroups of both parts run at once, two a compute unit: these are shared out by the parts' work (a wide tile's key counts twice), in shares of 256 keys at least, 128 of a wide
-        // tile.  There a key takes some 0.016 us, and a share more is written and read again, 8 head_dim bytes a row at 4 TB/s: P / ns keys and ns shares take the least time at the root of the ratio.
+        // tile.  There a key takes some 0.012 us beside the other workgroups, and a share more is written and read again, 8 head_dim bytes a row at 4 TB/s: P / ns keys and ns shares take the least time at the root of the ratio.
         // 32 heads of 128 on 8, 32 sequences of 700 keys behind 8192, us with 8 / 16 / 32 shares of the prefix: 31.6 + 4.8 for the joining / 24.9 + 4.8 / 27.6 + 5.9.
         const int64_t cost_p = units_p * prefix * (p.wide ? 2 : 1), cost_o = units_o * capacity, cost = cost_p + cost_o;
         auto shares = [](int64_t groups, int64_t units, int64_t keys, int64_t least) {
@@ -55,7 +55,7 @@ inline PlanPrefix plan_prefix(int batch, int n_kv_heads, int capacity, int head_
         };
         p.ns_p = shares(cost ? 512 * cost_p / cost : 0, units_p, prefix, p.wide ? 128 : 256);
         if (p.wide && p.ns_p > 1) {
-            const int best = (int)std::sqrt(0.016 * prefix / (0.1 + (double)heads * p.R * head_dim * 2e-6));
+            const int best = (int)std::sqrt(0.012 * prefix / (0.1 + (double)heads * p.R * head_dim * 2e-6));
             if (p.ns_p > best) p.ns_p = best < 1 ? 1 : best;
         }
         p.ns_o = shares(cost ? 512 * cost_o / cost : 0, units_o, capacity, 256);
