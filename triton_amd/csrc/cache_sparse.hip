@@ -9,6 +9,10 @@
 
 namespace trn {
 
+#if defined(__HIP_DEVICE_COMPILE__)
+template <int CTRL> __device__ __forceinline__ float rotated(float x) { return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true)); }
+#endif
+
 // ------------------------------------------------------------------------------------------------ bounds
 struct BoundsArgs { const half_t* k; half_t* bounds; const int32_t *lengths, *counts; int B, Hkv, M, cap, block, nb, per; int64_t ks[3]; Div by_per, by_hkv; };
 
@@ -35,10 +39,12 @@ __global__ __launch_bounds__(256) void cache_bounds_kernel(const BoundsArgs a) {
         for (int p = 0; p < NP; ++p)
 #pragma unroll
             for (int e = 0; e < 8; ++e) { lo[e] = fminf(lo[e], (float)x[p][e]); hi[e] = fmaxf(hi[e], (float)x[p][e]); }
+        // (over the lanes of one channel group, 8 and 16 apart and more, without LDS)
 #pragma unroll
-        for (int d = LPR; d < 64; d *= 2)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) { lo[e] = fminf(lo[e], __shfl_xor(lo[e], d, 64)); hi[e] = fmaxf(hi[e], __shfl_xor(hi[e], d, 64)); }
+        for (int e = 0; e < 8; ++e) {
+            if constexpr (D == 64) { lo[e] = fminf(lo[e], rotated<0x128>(lo[e])); hi[e] = fmaxf(hi[e], rotated<0x128>(hi[e])); }
+            lo[e] = -quad_max(-lo[e]); hi[e] = quad_max(hi[e]);
+        }
         if ((t & 63) < LPR) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) { lo_all[wave][sub * 8 + e] = lo[e]; hi_all[wave][sub * 8 + e] = hi[e]; }
@@ -71,7 +77,6 @@ template <int CTRL> __device__ __forceinline__ double moved64(double x) {
     return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 template <int CTRL, int ROWS = 0xf> __device__ __forceinline__ uint32_t moved32(uint32_t x) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, true); }
-template <int CTRL> __device__ __forceinline__ float rotated(float x) { return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true)); }
 // Over 16 lanes, by rotations.
 __device__ __forceinline__ float row_max(float x) {
     x = fmaxf(x, rotated<0x121>(x));
@@ -100,20 +105,24 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 __device__ __forceinline__ float unordered(uint32_t u) { return __uint_as_float(u >> 31 ? u ^ 0x80000000u : ~u); }
 #endif
 
-// Scores by the matrix pipe.  A wave has 16 blocks, whose bounds it holds as operands (lane 16 g + n: block n, channels 8 g..+7 of each 32).  HEADS: a query's heads are the other operand,
-// 16 at a time, and their largest is taken over lanes; otherwise 16 queries are, their heads one after the other, and the largest stays in a lane.  norms: the largest |bound| vector (of each
-// channel's larger end) of every 16 blocks, squared; infinite where a bound is not finite.
+// Scores by the matrix pipe.  A wave has 16 blocks or two times 16, whose bounds it holds as operands (lane 16 g + n: block n, channels 8 g..+7 of each 32).  HEADS: a query's heads are the other
+// operand, 16 at a time, and their largest is taken over lanes; otherwise 16 queries are, their heads one after the other, and the largest stays in a lane: twice 16 blocks then, as rows in this shape are
+// loaded at 16 bytes a clock and compute unit, which bounds it (256 queries on 512 blocks, 32 heads of 128 on 8: 11.4 us with 16 blocks, 10.0 with 32).
+// norms: the largest |bound| vector (of each channel's larger end) of every 16 blocks, squared; infinite where a bound is not finite.
 template <int D, bool HEADS>
 __global__ __launch_bounds__(256) void cache_scores_kernel(const SelectArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    constexpr int NI = D / 32;
+    constexpr int NI = D / 32, SETS = HEADS ? 1 : 2;
     const int lane = threadIdx.x & 63, n = lane & 15, g4 = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int bh = blockIdx.z, b = a.by_hkv.of(bh), kvh = bh - b * a.Hkv, set = blockIdx.x * 4 + wave, blk = set * 16 + n;
+    const int bh = blockIdx.z, b = a.by_hkv.of(bh), kvh = bh - b * a.Hkv, set = (blockIdx.x * 4 + wave) * SETS;
     // (bounds and queries are requested before it is known how many of them count)
-    const half_t* const bp = a.bounds + ((int64_t)bh * a.nb + min(blk, a.nb - 1)) * 2 * D + 8 * g4;
-    half8_t lo[NI], hi[NI], q[NI];
+    half8_t lo[SETS][NI], hi[SETS][NI], q[NI];
 #pragma unroll
-    for (int i = 0; i < NI; ++i) { lo[i] = *reinterpret_cast<const half8_t*>(bp + 32 * i); hi[i] = *reinterpret_cast<const half8_t*>(bp + D + 32 * i); }
+    for (int u = 0; u < SETS; ++u) {
+        const half_t* const bp = a.bounds + ((int64_t)bh * a.nb + min((set + u) * 16 + n, a.nb - 1)) * 2 * D + 8 * g4;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) { lo[u][i] = *reinterpret_cast<const half8_t*>(bp + 32 * i); hi[u][i] = *reinterpret_cast<const half8_t*>(bp + D + 32 * i); }
+    }
     const half_t* const qh = a.q + b * a.qs[0] + (int64_t)kvh * a.G * a.qs[1] + 8 * g4;
     const int j_first = blockIdx.y * a.steps * (HEADS ? 1 : 16);
     auto load = [&](int i, int g) __attribute__((always_inline)) {
@@ -125,44 +134,50 @@ __global__ __launch_bounds__(256) void cache_scores_kernel(const SelectArgs a) {
     const int L = length_of(a.lengths, b, a.cap), C = min(count_of(a.counts, b, a.M), a.i0 + a.n), blocks = L > 0 ? ((L - 1) >> a.block_shift) + 1 : 0;
     if (set * 16 >= blocks || blocks <= a.top) return;      // (where all blocks are taken no score is needed)
     if (blockIdx.y == 0) {
-        float sum = 0.f;
-        bool bad = false;
 #pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            bad = bad || odd_values(lo[i]) || odd_values(hi[i]);
+        for (int u = 0; u < SETS; ++u) {
+            float sum = 0.f;
+            bool bad = false;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) { const float x = fmaxf(fabsf((float)lo[i][e]), fabsf((float)hi[i][e])); sum = __builtin_fmaf(x, x, sum); }
+            for (int i = 0; i < NI; ++i) {
+                bad = bad || odd_values(lo[u][i]) || odd_values(hi[u][i]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) { const float x = fmaxf(fabsf((float)lo[u][i][e]), fabsf((float)hi[u][i][e])); sum = __builtin_fmaf(x, x, sum); }
+            }
+            sum = quad_sum(bad ? INFINITY : sum);
+            sum = row_max((set + u) * 16 + n < blocks ? sum : 0.f);
+            if (lane == 0) a.norms[(int64_t)bh * (a.nbp >> 4) + set + u] = sum;
         }
-        sum = quad_sum(bad ? INFINITY : sum);
-        sum = row_max(blk < blocks ? sum : 0.f);
-        if (lane == 0) a.norms[(int64_t)bh * (a.nbp >> 4) + set] = sum;
     }
-    const float4_t zero = {0.f, 0.f, 0.f, 0.f};
     const half8_t nil = {};
-    auto product = [&](const half8_t (&q)[NI]) {
-        float4_t x = zero;
+    float4_t best[SETS];
+    auto add = [&](const half8_t (&q)[NI]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int e = 0; e < NI; ++e) {
-            x = mfma16(hi[e], __builtin_elementwise_max(q[e], nil), x);
-            x = mfma16(lo[e], __builtin_elementwise_min(q[e], nil), x);
+        for (int u = 0; u < SETS; ++u) {
+            float4_t x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < NI; ++e) {
+                x = mfma16(hi[u][e], __builtin_elementwise_max(q[e], nil), x);
+                x = mfma16(lo[u][e], __builtin_elementwise_min(q[e], nil), x);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) best[u][e] = fmaxf(best[u][e], x[e]);
         }
-        return x;
     };
     float* const to = a.scores + (int64_t)bh * a.n * a.nbp + set * 16 + 4 * g4;
     for (int s = 0; s < a.steps; ++s) {
         const int j0 = j_first + s * (HEADS ? 1 : 16), i = a.i0 + j0 + (HEADS ? 0 : n);
         if (a.i0 + j0 >= C) return;
-        float4_t best = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int u = 0; u < SETS; ++u) best[u] = float4_t{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         if constexpr (HEADS) {
             for (int g0 = 0; g0 < a.G; g0 += 16) {
                 if (s > 0 || g0 > 0) load(i, min(g0 + n, a.G - 1));
-                const float4_t x = product(q);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) best[e] = fmaxf(best[e], x[e]);
+                add(q);
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) best[e] = row_max(best[e]);
-            if (n == 0) *reinterpret_cast<float4_t*>(to + j0 * a.nbp) = best;
+            for (int e = 0; e < 4; ++e) best[0][e] = row_max(best[0][e]);
+            if (n == 0) *reinterpret_cast<float4_t*>(to + j0 * a.nbp) = best[0];
         } else {
             load(min(i, C - 1), 0);
             for (int g = 0; g < a.G; ++g) {
@@ -170,11 +185,11 @@ __global__ __launch_bounds__(256) void cache_scores_kernel(const SelectArgs a) {
 #pragma unroll
                 for (int e = 0; e < NI; ++e) now[e] = q[e];
                 load(min(i, C - 1), min(g + 1, a.G - 1));
-                const float4_t x = product(now);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) best[e] = fmaxf(best[e], x[e]);
+                add(now);
             }
-            if (i < C) *reinterpret_cast<float4_t*>(to + (j0 + n) * a.nbp) = best;
+#pragma unroll
+            for (int u = 0; u < SETS; ++u)       // (a row has room for a multiple of 64 blocks)
+                if (i < C) *reinterpret_cast<float4_t*>(to + (j0 + n) * a.nbp + 16 * u) = best[u];
         }
     }
 #endif
@@ -692,7 +707,7 @@ extern "C" int trn_cache_bounds_f16(const trn_cache16* c, int32_t block, int32_t
     const int most = tokens < c->capacity ? tokens : c->capacity;
     // (the blocks that the new tokens can touch -- the first of them may be the last of its block --, but no more workgroups than the card holds at once: the most new tokens
     // that a call allows are rarely there)
-    const int64_t blocks = ((int64_t)most + 2 * block - 2) / block, at_once = (1024 + heads - 1) / heads;
+    const int64_t blocks = ((int64_t)most + 2 * block - 2) / block, at_once = (512 + heads - 1) / heads;
     a.per = (int)(blocks < at_once ? blocks : at_once);
     if (heads * a.per > 0xffffff) return TRN_E_SHAPE;                 // (threads in 32 bits)
     a.by_per = Div(a.per); a.by_hkv = Div(c->n_kv_heads);
@@ -744,10 +759,10 @@ extern "C" int trn_cache_sparse_attn_f16(const trn_cache16* c, const void* bound
     // (workgroups of 256, and as many threads in all as 32 bits number: of every launch, before the first one)
     const bool many = p.nb > kMostBlocks;
     const bool by_heads = p.step < 12;
-    const int64_t q_tiles = by_heads ? p.step : (p.step + 15) / 16, waves = heads * (p.nbp / 16) * q_tiles;
+    const int64_t q_tiles = by_heads ? p.step : (p.step + 15) / 16, waves = heads * (p.nbp / (by_heads || many ? 16 : 32)) * q_tiles;
     const int steps = many ? (waves > 4096 ? 4 : 1) : (int)(waves <= 2048 ? 1 : waves / 2048 < 8 ? waves / 2048 : 8);
     const int per64 = 4 * 512 / c->head_dim * steps;
-    const dim3 score_grid((unsigned)(many ? (p.nb + (int64_t)per64 - 1) / per64 : p.nbp / 64), (unsigned)(many ? p.step : (q_tiles + steps - 1) / steps), (unsigned)heads);
+    const dim3 score_grid((unsigned)(many ? (p.nb + (int64_t)per64 - 1) / per64 : by_heads ? p.nbp / 64 : (p.nbp + 127) / 128), (unsigned)(many ? p.step : (q_tiles + steps - 1) / steps), (unsigned)heads);
     const int threads = many ? 256 : p.nb > 6144 ? 1024 : p.nb > 1024 ? 512 : p.nb > 512 ? 256 : 128;
     const bool own = !p.rows && p.nb <= kOwnBlocks && p.step == seq_q;       // (the attention's workgroups select)
     if (groups > 0xffffff || heads > 65535 || heads * p.step * ((threads + 255) / 256) > 0xffffff || (int64_t)score_grid.x * score_grid.y * score_grid.z > 0xffffff) return TRN_E_SHAPE;
