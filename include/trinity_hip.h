@@ -527,7 +527,7 @@ int trn_cache_bounds_f16(const trn_cache16* cache, int32_t block, int32_t tokens
  * max over the KV head's query heads of sum_d max(q[d] lo[d], q[d] hi[d]), summed in 64 bits and rounded to 32; NaN counts as the least.  Selected are, of the blocks that hold a
  * key which the query sees, the first `sink` ones, the last `recent` ones (its own is the last of them), and of the others those with the largest scores, ties to the
  * earlier block: min(top, their number) in all.  sink + recent <= top, recent >= 1, top <= 2^16.
- *   selected   int32 [batch, n_kv_heads, seq_q, top] contiguous: the blocks, ascending, then -1; rows from counts[b] on stay.
+ *   selected   int32 [batch, n_kv_heads, seq_q, top] contiguous: the blocks, ascending, then -1; rows from counts[b] on stay.  It and o share no memory with each other, bounds or q.
  *   q, o, workspace and a query that sees no key as in trn_cache_prefix_attn_f16.
  */
 int64_t trn_cache_sparse_attn_workspace_bytes(const trn_cache16* cache, int32_t block, int32_t top, int32_t n_q_heads, int32_t seq_q);

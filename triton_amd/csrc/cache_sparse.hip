@@ -738,6 +738,11 @@ extern "C" int trn_cache_sparse_attn_f16(const trn_cache16* c, const void* bound
     if (!selected || (c->capacity && !bounds)) return TRN_E_NULL;
     if ((reinterpret_cast<uintptr_t>(selected) & 3) || !aligned16(bounds)) return TRN_E_ALIGN;
     const int64_t heads = (int64_t)c->batch * c->n_kv_heads;
+    // (what is written: apart from each other and from what the launches read)
+    const Extent eo = rows_extent(o, o_stride, c->batch, n_q_heads, seq_q, c->head_dim), eq = rows_extent(q, q_stride, c->batch, n_q_heads, seq_q, c->head_dim);
+    const int64_t n_bounds = c->capacity ? heads * ((c->capacity + block - 1) / block) * 4 * c->head_dim : 0, n_selected = heads * seq_q * top * 4;
+    if (!apart(o, eo.span(), bounds, n_bounds) || !apart(o, eo.span(), selected, n_selected) || !apart(q, eq.span(), selected, n_selected) || !apart(bounds, n_bounds, selected, n_selected))
+        return TRN_E_UNSUPPORTED;
     const PlanSparse p = plan_sparse(c->batch, c->n_kv_heads, c->capacity, c->head_dim, block, top, n_q_heads, seq_q);
     if (p.bytes && (!workspace || workspace_bytes < p.bytes)) return TRN_E_SCRATCH;
     if (p.dense) {
