@@ -357,6 +357,39 @@ def test_caches_past_32_bits():
     _within(o, *ref.sparse_attention(q, k, v, torch.zeros_like(q), want, 32, D ** -0.5, lengths, counts))
 
 
+@pytest.mark.parametrize("case", [(2, 64, 4, 300, 280), (1, 128, 4, 300, 280), (2, 64, 1, 1500, 280), (1, 128, 40, 290, 300), (2, 64, 40, 0, 290)], ids=lambda c: "B%dD%dM%dP%dS%d" % c)
+def test_rows_far_apart(case):
+    """The largest pitch of a token: the keys of one sequence, and those of a prefix, reach past 2^32 bytes."""
+    B, D, M, P, S = case
+    Hq, Hkv, far = 4, 1, 1 << 23
+    rows = P + B * S
+    if torch.cuda.mem_get_info()[0] < 2 * rows * far + (4 << 30):
+        pytest.skip("needs %d GB" % (2 * rows * far + (4 << 30) >> 30))
+    g = _gen(13)
+    q = torch.randn(B, Hq, M, D, generator=g).half()
+    kv = torch.randn(rows, 2 * D, generator=g).half()
+    room = torch.empty(rows * far, dtype=torch.float16, device=DEV).view(rows, far)
+    room[:, :2 * D] = kv.to(DEV)
+    lengths, counts = [S - 7 * b for b in range(B)], [M] * B
+
+    def parts(x):
+        own = x[P:, :].view(B, S, 1, x.shape[1]).permute(0, 2, 1, 3)
+        return own[..., :D], own[..., D:2 * D], x[None, :P, :D], x[None, :P, D:2 * D]
+    k, v, kp, vp = parts(kv)
+    dk, dv, dkp, dvp = parts(room)
+    o = torch.zeros(B, Hq, M, D, dtype=torch.float16, device=DEV)
+    modules.get("prefix", "cache").forward(dk, dkp, o, q.to(DEV), dv, dvp, _ints(counts), _ints(lengths))
+    _within(o, *ref.prefix_attention(q, k, v, kp, vp, torch.zeros_like(q), D ** -0.5, True, lengths, counts))
+    nb = (S + 31) // 32
+    bnd, sel = torch.zeros(B, Hkv, nb, 2, D, dtype=torch.float16, device=DEV), torch.zeros(B, Hkv, M, 3, dtype=torch.int32, device=DEV)
+    modules.get("bounds", "cache", block=32).forward(dk, bnd, None, _ints(lengths))
+    assert torch.equal(bnd.cpu(), ref.bounds(k, torch.zeros(bnd.shape).half(), 32, lengths, [S] * B))
+    modules.get("sparse", "cache", block=32, top=3).forward(dk, o, q.to(DEV), dv, bnd, _ints(counts), _ints(lengths), sel)
+    want = ref.select(q, bnd.cpu(), torch.zeros(sel.shape, dtype=torch.int32), 32, 3, 0, 1, 4, lengths, counts, S)
+    assert torch.equal(sel.cpu(), want)
+    _within(o, *ref.sparse_attention(q, k, v, torch.zeros_like(q), want, 32, D ** -0.5, lengths, counts))
+
+
 # ------------------------------------------------------------------------------------------------ together
 def _loop(kind, prenorm=False):
     B, Hq, Hkv, D, N, S, P = 3, 8, 2, 64, 192, 500, 90 if kind == "prefix" else 0

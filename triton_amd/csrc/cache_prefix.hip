@@ -31,8 +31,8 @@ struct Run {
 // ... of the prefix, `split` tiles, and of the sequence behind them.
 struct TwoRuns {
     const half_t *kp, *vp, *ko, *vo; int kpp, vpp, kpo, vpo, P, L, split;
-    __device__ __forceinline__ const half_t* k(int t) const { return t < split ? kp + (int32_t)t * 32 * kpp : ko + (int32_t)(t - split) * 32 * kpo; }
-    __device__ __forceinline__ const half_t* v(int t) const { return t < split ? vp + (int32_t)t * 32 * vpp : vo + (int32_t)(t - split) * 32 * vpo; }
+    __device__ __forceinline__ const half_t* k(int t) const { return t < split ? kp + (int64_t)t * 32 * kpp : ko + (int64_t)(t - split) * 32 * kpo; }
+    __device__ __forceinline__ const half_t* v(int t) const { return t < split ? vp + (int64_t)t * 32 * vpp : vo + (int64_t)(t - split) * 32 * vpo; }
     __device__ __forceinline__ int kpitch(int t) const { return t < split ? kpp : kpo; }
     __device__ __forceinline__ int vpitch(int t) const { return t < split ? vpp : vpo; }
     __device__ __forceinline__ int n(int t) const { return min(32, left(t)); }
