@@ -502,7 +502,8 @@ int trn_cache_rope_append_f16(const trn_cache16* cache, const trn_rope* rope, co
  * o = softmax(scale * q [K_prefix ; K]^T) [V_prefix ; V]: attention of a batch whose sequences begin alike.  k_prefix, v_prefix [n_kv_heads, prefix, head_dim]
  * (strides {head, token}, as the cache's) are seen by every query and read once for all; of its own sequence a query sees, causal, the
  * keys j <= lengths[b] - counts[b] + i, otherwise all.  q, o [batch, n_q_heads, seq_q, head_dim] fp16, GQA / MQA, o on 8 bytes and apart from q; rows from counts[b] on are
- * neither read nor written.  prefix 0: attention over the cache alone.  A query that sees no key gets zeros.  Scores, sums and the joining of shares are in fp32.
+ * neither read nor written.  prefix 0: attention over the cache alone.  A query that sees no key gets zeros; a channel in which it sees
+ * an infinite value is infinite or NaN, whatever tokens hold that it does not see stays out.  Scores, sums and the joining of shares are in fp32.
  *   workspace  trn_cache_prefix_attn_workspace_bytes(...) bytes, 256-byte aligned, no initial contents; TRN_E_SCRATCH if smaller.  One call at a time may use it.
  */
 typedef struct trn_prefix {
@@ -527,7 +528,7 @@ int trn_cache_bounds_f16(const trn_cache16* cache, int32_t block, int32_t tokens
  * max over the KV head's query heads of sum_d max(q[d] lo[d], q[d] hi[d]), summed in 64 bits and rounded to 32; NaN counts as the least.  Selected are, of the blocks that hold a
  * key which the query sees, the first `sink` ones, the last `recent` ones (its own is the last of them), and of the others those with the largest scores, ties to the
  * earlier block: min(top, their number) in all.  sink + recent <= top, recent >= 1, top <= 2^16.
- *   selected   int32 [batch, n_kv_heads, seq_q, top] contiguous: the blocks, ascending, then -1; rows from counts[b] on stay.  It and o share no memory with each other, bounds or q.
+ *   selected   int32 [batch, n_kv_heads, seq_q, top] contiguous: the blocks, ascending, then -1; rows from counts[b] on stay.  It and o share no memory with each other, bounds, q or the cache.
  *   q, o, workspace and a query that sees no key as in trn_cache_prefix_attn_f16.
  */
 int64_t trn_cache_sparse_attn_workspace_bytes(const trn_cache16* cache, int32_t block, int32_t top, int32_t n_q_heads, int32_t seq_q);

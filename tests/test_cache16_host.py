@@ -124,7 +124,7 @@ def test_sparse_and_bounds_statuses(lib):
         assert _sparse(lib, **kw) == "TRN_E_NULL", kw
     for kw in (dict(top=0), dict(sink=-1), dict(recent=0), dict(top=2, sink=1, recent=2), dict(heads=6 + 1), dict(scale=-1.0)):
         assert _sparse(lib, **kw) == "TRN_E_SHAPE", kw
-    for kw in (dict(block=48), dict(block=256), dict(top=(1 << 16) + 1), dict(o=P + 64), dict(o=P + 2 * M + 128), dict(sel=P + 3 * M), dict(sel=P + 2 * M + 64), dict(sel=P + 6 * M), dict(o=P + 6 * M)):
+    for kw in (dict(block=48), dict(block=256), dict(top=(1 << 16) + 1), dict(o=P + 64), dict(o=P + 2 * M + 128), dict(sel=P + 3 * M), dict(sel=P + 2 * M + 64), dict(sel=P + 6 * M), dict(o=P + 6 * M), dict(sel=P + 64), dict(sel=P + M)):
         assert _sparse(lib, **kw) == "TRN_E_UNSUPPORTED", kw
     assert _sparse(lib, bounds=P + 6 * M + 8) == "TRN_E_ALIGN" and _sparse(lib, sel=P + 2) == "TRN_E_ALIGN"
     assert lib.trn_cache_sparse_attn_workspace_bytes(C.byref(_cache()), 32, 4, 4, 3) == 0 and _sparse(lib, ws=None) == "TRN_E_LAUNCH"      # four blocks, all selected

@@ -164,6 +164,32 @@ def test_prefix_attention_of_what_is_not_finite(D, M):
     _within(got, want, torch.nan_to_num(tol, nan=0.0, posinf=0.0))
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B,M,P,S", [(2, 2, 170, 300), (2, 40, 170, 300), (1, 6, 1300, 700), (12, 1, 2000, 1100), (4, 70, 200, 500)])
+def test_infinite_values_that_a_query_sees(B, M, P, S, D):
+    """Infinities and NaN in values of the prefix and of the cache, wherever they lie: a channel that has one is no number, as in the formula, and the others keep their numbers."""
+    Hq, Hkv = 8, 2
+    g = _gen(14)
+    q, k, v = (torch.randn(B, h, s, D, generator=g).half() for h, s in ((Hq, M), (Hkv, S), (Hkv, S)))
+    kp, vp = (torch.randn(Hkv, P, D, generator=g).half() for _ in range(2))
+    vp[0, 40, 3], vp[0, P - 1, 4], vp[1, 70, 5] = math.inf, -math.inf, math.nan
+    for b in range(B):
+        v[b, 0, 45 + b, 9], v[b, 0, 130, 10], v[b, 1, 64, 11], v[b, 1, 140, 9] = -math.inf, math.nan, math.inf, math.inf
+        v[b, 1, 70, 9] = -math.inf if b % 2 else math.inf
+    lengths, counts = [S - 9 * b for b in range(B)], [M] * B
+    want, tol = ref.prefix_attention(q, k, v, kp, vp, torch.zeros_like(q), D ** -0.5, True, lengths, counts)
+    o = torch.zeros(B, Hq, M, D, dtype=torch.float16, device=DEV)
+    modules.get("prefix", "cache").forward(*(x.to(DEV) for x in (k, kp)), o, *(x.to(DEV) for x in (q, v, vp)), _ints(counts), _ints(lengths))
+    assert torch.equal(o.cpu().isfinite(), want.isfinite())
+    _within(o.cpu()[want.isfinite()], want[want.isfinite()], tol[want.isfinite()])
+    bnd, sel = torch.zeros(B, Hkv, (S + 63) // 64, 2, D, dtype=torch.float16, device=DEV), torch.zeros(B, Hkv, M, 4, dtype=torch.int32, device=DEV)
+    modules.get("bounds", "cache").forward(k.to(DEV), bnd, None, _ints(lengths))
+    modules.get("sparse", "cache", top=4).forward(k.to(DEV), o, q.to(DEV), v.to(DEV), bnd, _ints(counts), _ints(lengths), sel)
+    want, tol = ref.sparse_attention(q, k, v, torch.zeros_like(q), sel.cpu(), 64, D ** -0.5, lengths, counts)
+    assert torch.equal(o.cpu().isfinite(), want.isfinite())
+    _within(o.cpu()[want.isfinite()], want[want.isfinite()], tol[want.isfinite()])
+
+
 # ------------------------------------------------------------------------------------------------ bounds, selection
 SPARSES = [
     # B, Hq, Hkv, D, new, capacity, lengths, counts, block, top, sink, recent

@@ -743,6 +743,9 @@ extern "C" int trn_cache_sparse_attn_f16(const trn_cache16* c, const void* bound
     const int64_t n_bounds = c->capacity ? heads * ((c->capacity + block - 1) / block) * 4 * c->head_dim : 0, n_selected = heads * seq_q * top * 4;
     if (!apart(o, eo.span(), bounds, n_bounds) || !apart(o, eo.span(), selected, n_selected) || !apart(q, eq.span(), selected, n_selected) || !apart(bounds, n_bounds, selected, n_selected))
         return TRN_E_UNSUPPORTED;
+    for (int i = 0; i < 2 && c->capacity; ++i)
+        if (!apart(i ? c->v : c->k, rows_extent(i ? c->v : c->k, i ? c->v_stride : c->k_stride, c->batch, c->n_kv_heads, c->capacity, c->head_dim).span(), selected, n_selected))
+            return TRN_E_UNSUPPORTED;
     const PlanSparse p = plan_sparse(c->batch, c->n_kv_heads, c->capacity, c->head_dim, block, top, n_q_heads, seq_q);
     if (p.bytes && (!workspace || workspace_bytes < p.bytes)) return TRN_E_SCRATCH;
     if (p.dense) {
