@@ -61,7 +61,7 @@ __device__ __forceinline__ const half_t* query(const PrefixArgs& a, int b, int k
 }
 #endif
 
-// Tiles of 128 rows of one sequence, over the prefix and its own keys.  32 heads of 128 on 8, 4 chunks of up to 500 behind 4000 keys: 138 us, 810 TFLOP/s (a share of 1024
+// Tiles of 128 rows of one sequence, over the prefix and its own keys.  32 heads of 128 on 8, 4 chunks of up to 500 behind 4000 keys: 133 us, 840 TFLOP/s (a share of 1024
 // keys takes 53 us with one array for all stages, 32 so); 71 heads of 64 on 1, 16 of up to 5 behind 16001: 41 us, 490 TFLOP/s, where the exponentials bound it.
 template <int D, bool FINE>
 __global__ __launch_bounds__(256, D == 128 ? 2 : FINE ? 3 : 4) void cache_prefix_rows_kernel(const PrefixArgs a) {
