@@ -13,6 +13,11 @@
 
 namespace trn {
 
+// Weights enter their product with V in fp16, 2^(score - m), and m lies below the largest score: by 2^7 (narrow) or 2^5 (wide) in units of the weights when it is taken, so that they come to 2^15 at most.
+// A key that has nearly all of the weight (what all queries look at first, its value often next to nothing) leaves little to each of the others: of a weight w of the largest's 1 this keeps 2^-32 (two
+// numbers) or 2^-30 (one), where m at the largest score would keep 2^-25: keys of 2^-20 each are off by 0.03 % or 0.1 % at most, and would be by 3 %.
+constexpr float kBelowNarrow = 7.f, kBelowWide = 5.f;
+
 // What became of a row's keys in one share: O unnormalised, and (m, l) with m in units of log2.  Row `row` of B Hkv M G has `slots` of them.
 struct Parts { float* o; float* ml; int slots; };
 
@@ -146,19 +151,19 @@ __device__ __forceinline__ void narrow_walk(Keys& keys, int t0, int t1, int t_ma
         for (int qb = 0; qb < NQ; ++qb) {
             const float4_t &u = s[0][qb], &v = s[1][qb];
             tm[qb] = max3(max3(u[0], u[1], u[2]), max3(u[3], v[0], v[1]), fmaxf(v[2], v[3])) * c;
-            due = due || tm[qb] > m[qb] + 8.f;
+            due = due || tm[qb] > m[qb] + 15.f;
         }
-        if (__builtin_expect(__builtin_amdgcn_ballot_w64(due) != 0, 0)) {       // lazily: p stays below 2^8
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(due) != 0, 0)) {       // lazily: p stays below 2^15
 #pragma unroll
             for (int qb = 0; qb < NQ; ++qb) {
-                const float up = fmaxf(m[qb], quad_max(tm[qb])), alpha = up == -INFINITY ? 1.f : fast_exp2(m[qb] - up);
+                const float up = fmaxf(m[qb], quad_max(tm[qb]) - kBelowNarrow), alpha = up == -INFINITY ? 1.f : fast_exp2(m[qb] - up);
                 m[qb] = up;
                 l[qb] *= alpha;
 #pragma unroll
                 for (int i = 0; i < NDB; ++i) o[i][qb] = o[i][qb] * alpha;
             }
         }
-        // (p enters the product with V as two fp16 numbers, what the first leaves over being the second: rounded once its error is 2^-12 of each key's part, as much as the output's own rounding)
+        // (p enters the product with V as two fp16 numbers, what the first leaves over being the second: rounded once its error is up to 2^-11 of each key's part, as much as the output's own rounding)
         half8_t p[NQ], rest[NQ];
 #pragma unroll
         for (int qb = 0; qb < NQ; ++qb) {
@@ -356,10 +361,10 @@ __device__ __forceinline__ void wide_walk(const Keys keys, int t0, int t1, int t
 #pragma unroll
             for (int i = 0; i < NS; ++i) s = mfma32(*reinterpret_cast<const half8_t*>(in(Kt, kr[i])), qB[i], i == 0 ? zero : s);
             masked();
-            const float up = fmaxf(m, half_max(max16(s) * c)), alpha = up == -INFINITY ? 1.f : fast_exp2(m - up);
+            const float up = fmaxf(m, half_max(max16(s) * c) - kBelowWide), alpha = up == -INFINITY ? 1.f : fast_exp2(m - up);
             m = up;
             l *= alpha;
-            if (m != -INFINITY) { d = -m; most = 1024.f; }
+            if (m != -INFINITY) { d = -m; most = 32768.f; }
 #pragma unroll
             for (int i = 0; i < NDB; ++i) o[i] = o[i] * alpha;
             sum = weights();
