@@ -465,7 +465,7 @@ int trn_cache_evict(const trn_cache_evict_desc* desc, const void* k, const void*
 /*
  * An fp16 key/value cache [batch, n_kv_heads, capacity, head_dim] whose sequences have lengths of their own, as in trn_cache8: lengths and counts
  * (nullable int32 [batch], on the device) are the keys of each sequence, this step's new ones among them, and its new tokens.
- * Strides {batch, head, token} are in elements, not negative, multiples of 8, that of a token at most 2^23; head_dim 64 or 128; capacity at most 2^26.
+ * Strides {batch, head, token} are in elements, not negative, multiples of 8, that of a token at most 2^23 (of an axis of one entry: any); head_dim 64 or 128; capacity at most 2^26.
  */
 typedef struct trn_cache16 {
     void* k; void* v;

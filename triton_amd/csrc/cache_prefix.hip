@@ -342,12 +342,17 @@ extern "C" int trn_cache_prefix_attn_f16(const trn_cache16* c, const trn_prefix*
         const int64_t s3[3] = {0, s2[0], s2[1]};
         if ((st = rows16_check(p, s3, 1, c->n_kv_heads, prefix->keys, 16, false)) != TRN_OK) return st;
         if (s2[1] < c->head_dim && prefix->keys > 1) return TRN_E_STRIDE;
-        if (s2[1] > (1 << 23)) return TRN_E_UNSUPPORTED;
+        if (s2[1] > (1 << 23) && prefix->keys > 1) return TRN_E_UNSUPPORTED;
         if (meet(rows_extent(o, o_stride, c->batch, n_q_heads, seq_q, c->head_dim), rows_extent(p, s3, 1, c->n_kv_heads, prefix->keys, c->head_dim))) return TRN_E_UNSUPPORTED;
         (i ? a.vps : a.kps)[0] = s2[0]; (i ? a.vps : a.kps)[1] = s2[1];
     }
+    for (int i = 0; i < 3; ++i) { a.ks[i] = c->k_stride[i]; a.vs[i] = c->v_stride[i]; a.qs[i] = q_stride[i]; a.os[i] = o_stride[i]; }
+    // (a stride between tokens of which there is one may be anything, but a tile's rows are all addressed by it: the other part's then, or that of contiguous rows)
+    const bool many_p = prefix->keys > 1, many_o = c->capacity > 1;
+    if (!many_o) { a.ks[2] = many_p ? a.kps[1] : c->head_dim; a.vs[2] = many_p ? a.vps[1] : c->head_dim; }
+    if (!many_p) { a.kps[1] = a.ks[2]; a.vps[1] = a.vs[2]; }
     PlanPrefix p = plan_prefix(c->batch, c->n_kv_heads, c->capacity, c->head_dim, prefix->keys, n_q_heads, seq_q);
-    const bool shrt = p.short_rt > 0 && (prefix->keys == 0 || c->capacity == 0 || (prefix->k_stride[1] == c->k_stride[2] && prefix->v_stride[1] == c->v_stride[2]));
+    const bool shrt = p.short_rt > 0 && a.kps[1] == a.ks[2] && a.vps[1] == a.vs[2];
     if (shrt) { p.slots = 1; p.bytes = 0; p.first = (int64_t)c->batch * c->n_kv_heads * p.short_rt; p.second = 0; }
     if (p.first + p.second > 0xffffff) return TRN_E_SHAPE;            // (threads in 32 bits)
     if (p.bytes && (!workspace || workspace_bytes < p.bytes)) return TRN_E_SCRATCH;
@@ -355,7 +360,6 @@ extern "C" int trn_cache_prefix_attn_f16(const trn_cache16* c, const trn_prefix*
     a.lengths = c->lengths; a.counts = c->counts;
     a.B = c->batch; a.Hkv = c->n_kv_heads; a.M = seq_q; a.cap = c->capacity; a.P = prefix->keys; a.G = p.G; a.R = p.R; a.causal = causal != 0;
     a.n_rt_p = p.n_rt_p; a.ns_p = p.ns_p; a.n_rt_o = p.n_rt_o; a.ns_o = p.ns_o; a.first = (int)p.first;
-    for (int i = 0; i < 3; ++i) { a.ks[i] = c->k_stride[i]; a.vs[i] = c->v_stride[i]; a.qs[i] = q_stride[i]; a.os[i] = o_stride[i]; }
     a.c = scale * kLog2e;
     a.parts = Parts{(float*)workspace, (float*)((char*)workspace + p.ml), p.slots};
     auto div = [](int64_t n) { return Div(n > 0 ? n : 1); };
@@ -365,7 +369,6 @@ extern "C" int trn_cache_prefix_attn_f16(const trn_cache16* c, const trn_prefix*
     const dim3 grid((unsigned)(p.first + p.second)), block(256);
     const bool d128 = c->head_dim == 128;
     if (shrt) {
-        if (prefix->keys && !c->capacity) { a.ks[2] = prefix->k_stride[1]; a.vs[2] = prefix->v_stride[1]; }
         if (d128) hipLaunchKernelGGL((cache_prefix_short_kernel<128>), grid, dim3(512), 0, s, a);
         else hipLaunchKernelGGL((cache_prefix_short_kernel<64>), grid, dim3(512), 0, s, a);
     } else if (p.one) {

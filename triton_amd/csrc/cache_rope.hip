@@ -175,7 +175,7 @@ int cache16_check(const trn_cache16* c, bool values) {
         const int e = rows16_check(i ? c->v : c->k, st, c->batch, c->n_kv_heads, c->capacity, 16, false);
         if (e != TRN_OK) return e;
         if (st[2] < c->head_dim && c->capacity > 1) return TRN_E_STRIDE;
-        if (st[2] > (1 << 23)) return TRN_E_UNSUPPORTED;            // (64 rows in 32-bit offsets)
+        if (st[2] > (1 << 23) && c->capacity > 1) return TRN_E_UNSUPPORTED;            // (64 rows in 32-bit offsets)
     }
     return TRN_OK;
 }
