@@ -147,12 +147,11 @@ __global__ __launch_bounds__(256, 2) void cache_prefix_parts_kernel(const Prefix
         const int r0 = rt * 128 + wave * 32, row = min(r0 + n, a.B * a.R - 1), b = a.by_r.of(row), r = row - b * a.R;
         const bool there = r0 + n < a.B * a.R && r < count_of(a.counts, b, a.M) * a.G;
         if (!__syncthreads_or(there)) return;
-        half8_t qB[D / 16];
-        const half_t* const qp = there ? query(a, b, kvh, r) : a.q;
+        half8_t qB[D / 16] = {};
+        if (there) {
+            const half_t* const qp = query(a, b, kvh, r);
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-            const half8_t z = {}, y = *reinterpret_cast<const half8_t*>(qp + 16 * i + 8 * h);
-            qB[i] = there ? y : z;
+            for (int i = 0; i < D / 16; ++i) qB[i] = *reinterpret_cast<const half8_t*>(qp + 16 * i + 8 * h);
         }
         const half_t *const kp = a.kp + kvh * a.kps[0], *const vp = a.vp + kvh * a.vps[0];
         const int T = (a.P + 31) >> 5;
@@ -187,18 +186,17 @@ __global__ __launch_bounds__(256, 2) void cache_prefix_parts_kernel(const Prefix
         if (rt * RT >= all) return;
     }
     auto sees = [&](int r) { return !prefix && a.causal ? min(L, max(0, a.by_g.of(r) + off + 1)) : L; };
-    half8_t qB[NQ][D / 32];
+    half8_t qB[NQ][D / 32] = {};
     int last[NQ];
 #pragma unroll
     for (int qb = 0; qb < NQ; ++qb) {
         const int row = min(rt * RT + 16 * qb + n, all - 1), b = prefix ? a.by_r.of(row) : b0, r = prefix ? row - b * a.R : row;
         const bool there = rt * RT + 16 * qb + n < all && (!prefix || r < count_of(a.counts, b, a.M) * a.G);
         last[qb] = there ? sees(r) - 1 : -1;
-        const half_t* const qp = there ? query(a, b, kvh, r) : a.q;
+        if (there) {
+            const half_t* const qp = query(a, b, kvh, r);
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i) {
-            const half8_t z = {}, y = *reinterpret_cast<const half8_t*>(qp + 32 * i + 8 * g4);
-            qB[qb][i] = there ? y : z;
+            for (int i = 0; i < D / 32; ++i) qB[qb][i] = *reinterpret_cast<const half8_t*>(qp + 32 * i + 8 * g4);
         }
     }
     const int T = (sees(min(rt * RT + RT - 1, all - 1)) + 31) >> 5, w = share * 4 + wave;

@@ -115,7 +115,7 @@ __global__ __launch_bounds__(256) void cache_scores_kernel(const SelectArgs a) {
     constexpr int NI = D / 32, SETS = HEADS ? 1 : 2;
     const int lane = threadIdx.x & 63, n = lane & 15, g4 = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int bh = blockIdx.z, b = a.by_hkv.of(bh), kvh = bh - b * a.Hkv, set = (blockIdx.x * 4 + wave) * SETS;
-    // (bounds and queries are requested before it is known how many of them count)
+    // (bounds are requested before it is known how many of them count; queries are read only where they are there)
     half8_t lo[SETS][NI], hi[SETS][NI], q[NI];
 #pragma unroll
     for (int u = 0; u < SETS; ++u) {
@@ -130,8 +130,9 @@ __global__ __launch_bounds__(256) void cache_scores_kernel(const SelectArgs a) {
 #pragma unroll
         for (int e = 0; e < NI; ++e) q[e] = *reinterpret_cast<const half8_t*>(p + 32 * e);
     };
-    if constexpr (HEADS) load(min(a.i0 + j_first, a.M - 1), min(n, a.G - 1));
-    const int L = length_of(a.lengths, b, a.cap), C = min(count_of(a.counts, b, a.M), a.i0 + a.n), blocks = L > 0 ? ((L - 1) >> a.block_shift) + 1 : 0;
+    const int C = min(count_of(a.counts, b, a.M), a.i0 + a.n), L = length_of(a.lengths, b, a.cap), blocks = L > 0 ? ((L - 1) >> a.block_shift) + 1 : 0;
+    if (a.i0 + j_first >= C) return;
+    if constexpr (HEADS) load(a.i0 + j_first, min(n, a.G - 1));
     if (set * 16 >= blocks || blocks <= a.top) return;      // (where all blocks are taken no score is needed)
     if (blockIdx.y == 0) {
 #pragma unroll
@@ -306,11 +307,10 @@ __device__ __forceinline__ float score64(const SelectArgs& a, const half_t* q, i
 // (of the two of a channel one is zero) and eight earlier sums, and may cut off 2^-23 of the largest sum at each: 136 2^-23 < 1.07 2^-16 of the sum of the products' magnitudes, which is |q| |b| at
 // most; the rounding of r, and of t + 2 e, is 2^-24 each: e = 1.15 2^-16 |q| |b|.  (Products of fp16 numbers are normal in 32 bits; numbers below 2^-14 enter the pipe as they are.)
 template <int REGS> struct SelectInputs { float s[REGS], bb; };
-// All that a selection needs, requested before it is known how many blocks there are: a thread's scores, neighbours; norms; queries.
+// What a selection needs, requested before it is known how many blocks there are: a thread's scores, neighbours; norms.
 template <int D, int T, int REGS>
-__device__ __forceinline__ void select_inputs(const SelectArgs& a, SelectInputs<REGS>& in, half8_t& q8, int bh, int b, int kvh, int i, const float* from) {
-    constexpr int LPR = D / 8;
-    const int tid = threadIdx.x, lane = tid & 63, x0 = tid * REGS;
+__device__ __forceinline__ void select_inputs(const SelectArgs& a, SelectInputs<REGS>& in, int bh, const float* from) {
+    const int tid = threadIdx.x, x0 = tid * REGS;
 #pragma unroll
     for (int r = 0; r < REGS; r += 4) {
         const float4_t v = x0 + r < a.nbp ? *reinterpret_cast<const float4_t*>(from + x0 + r) : float4_t{0.f, 0.f, 0.f, 0.f};
@@ -319,7 +319,12 @@ __device__ __forceinline__ void select_inputs(const SelectArgs& a, SelectInputs<
     }
     static_assert(T * REGS <= 16 * T, "a norm a thread");
     in.bb = tid < a.nbp >> 4 ? a.norms[(int64_t)bh * (a.nbp >> 4) + tid] : 0.f;
-    q8 = *reinterpret_cast<const half8_t*>(a.q + b * a.qs[0] + (int64_t)(kvh * a.G + min(tid / LPR, a.G - 1)) * a.qs[1] + (int64_t)i * a.qs[2] + lane % LPR * 8);
+}
+// Eight channels of one head a thread, of the query i, which is there.
+template <int D>
+__device__ __forceinline__ half8_t select_query(const SelectArgs& a, int b, int kvh, int i) {
+    constexpr int LPR = D / 8;
+    return *reinterpret_cast<const half8_t*>(a.q + b * a.qs[0] + (int64_t)(kvh * a.G + min((int)threadIdx.x / LPR, a.G - 1)) * a.qs[1] + (int64_t)i * a.qs[2] + (threadIdx.x & 63) % LPR * 8);
 }
 
 template <int D, int T, int REGS>
@@ -449,10 +454,10 @@ __global__ __launch_bounds__(T) void cache_select_kernel(const SelectArgs a) {
     __shared__ __attribute__((aligned(16))) SelectShared<T> sh;
     const int bh = a.by_n.of(blockIdx.x), j = blockIdx.x - bh * a.n, i = a.i0 + j, b = a.by_hkv.of(bh);
     SelectInputs<REGS> in;
-    half8_t q8;
-    select_inputs<D, T, REGS>(a, in, q8, bh, b, bh - b * a.Hkv, i, a.scores + ((int64_t)bh * a.n + j) * a.nbp);
+    select_inputs<D, T, REGS>(a, in, bh, a.scores + ((int64_t)bh * a.n + j) * a.nbp);
     const int L = length_of(a.lengths, b, a.cap), C = count_of(a.counts, b, a.M), last = L - C + i, n = last < 0 ? 0 : (last >> a.block_shift) + 1;
     if (i >= C) return;
+    const half8_t q8 = select_query<D>(a, b, bh - b * a.Hkv, i);
     int32_t* const to = a.selected + ((int64_t)bh * a.M + i) * a.top;
     if (n <= a.top) {
         for (int x = threadIdx.x; x < a.top; x += T) to[x] = x < n ? x : -1;
@@ -570,9 +575,10 @@ __global__ __launch_bounds__(256, 2) void cache_sparse_attn_kernel(const SparseA
     const int x = a.by_hkv.of(blockIdx.x), kvh = blockIdx.x - x * a.Hkv, y = a.by_b.of(x), b = x - y * a.B, z = a.by_ns.of(y), share = y - z * a.ns, i = a.by_rt.of(z), rt = z - i * a.n_rt;
     [[maybe_unused]] SelectInputs<4> in;
     [[maybe_unused]] half8_t q8;
-    if constexpr (SELECT) select_inputs<D, 256, 4>(sel, in, q8, b * a.Hkv + kvh, b, kvh, i, sel.scores + (((int64_t)b * a.Hkv + kvh) * sel.n + i) * sel.nbp);
+    if constexpr (SELECT) select_inputs<D, 256, 4>(sel, in, b * a.Hkv + kvh, sel.scores + (((int64_t)b * a.Hkv + kvh) * sel.n + i) * sel.nbp);
     const int L = length_of(a.lengths, b, a.cap), C = count_of(a.counts, b, a.M), seen = L - C + i + 1;       // the keys that the query sees
     if (i >= C) return;
+    if constexpr (SELECT) q8 = select_query<D>(sel, b, kvh, i);
     const int ends = seen > 0 ? (seen - 1) >> a.block_shift : -1, most = min(a.top, ends + 1), per = 1 << (a.block_shift - 5);
     // (the last block is the query's own: the others are there as a whole)
     const int T = most > 0 ? (most - 1) * per + ((seen - (ends << a.block_shift) + 31) >> 5) : 0, whole = most > 0 ? (most - 1) * per + ((seen - (ends << a.block_shift)) >> 5) : 0;
