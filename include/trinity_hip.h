@@ -481,7 +481,7 @@ typedef struct trn_cache16 {
  *   norm         x <- x / sqrt(mean(x^2) + eps) * gamma for queries and keys, gamma_q, gamma_k nullable fp16 [head_dim].
  *   rotation     pair p < pairs of queries and keys, (x[p], x[p + pairs]) or, interleaved, (x[2 p], x[2 p + 1]), is turned by the angle position * inv_freq[p],
  *                formed in 64 bits; the other dimensions stay.  pairs: a multiple of 4, 2 * pairs <= head_dim, 0 for none.
- *   position     lengths[b] - counts[b] + i, or positions[axis][b][i] (int32, contiguous [axes, batch, tokens]); of several axes (time, height, width)
+ *   position     offset + lengths[b] - counts[b] + i, or positions[axis][b][i] (int32, contiguous [axes, batch, tokens]; offset 0); of several axes (time, height, width)
  *                the pairs lie section by section, sections[axis] of them: their sum is pairs.  Up to four axes; more than one needs positions.
  *   outputs      q_out[b, :, i] (q itself, with its strides, or apart from it); k_cache, v_cache at lengths[b] - counts[b] + i.  Of more new tokens than
  *                keys the last ones are the cache's.  Computed in 32 bits, rounded once.  Nothing else is read or written.
@@ -493,6 +493,7 @@ typedef struct trn_rope {
     int32_t pairs, interleaved, axes, norm;
     int32_t sections[4];
     float eps;
+    int32_t offset;
 } trn_rope;
 int trn_cache_rope_append_f16(const trn_cache16* cache, const trn_rope* rope, const void* q, void* q_out, const void* k, const void* v,
                               int32_t n_q_heads, int32_t tokens, const int64_t* q_stride, const int64_t* q_out_stride,

@@ -79,7 +79,7 @@ class Cache16(C.Structure):
 class Rope(C.Structure):
     """Mirror of `trn_rope`."""
     _fields_ = [("inv_freq", C.c_void_p), ("positions", C.c_void_p), ("gamma_q", C.c_void_p), ("gamma_k", C.c_void_p)] + \
-        [(n, C.c_int32) for n in ("pairs", "interleaved", "axes", "norm")] + [("sections", C.c_int32 * 4), ("eps", C.c_float)]
+        [(n, C.c_int32) for n in ("pairs", "interleaved", "axes", "norm")] + [("sections", C.c_int32 * 4), ("eps", C.c_float), ("offset", C.c_int32)]
 
 
 class Prefix(C.Structure):

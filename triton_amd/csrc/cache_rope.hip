@@ -14,7 +14,7 @@ namespace trn {
 struct RopeArgs {
     const half_t *q, *k, *v, *gq, *gk; half_t *qo, *kc, *vc;
     const double* inv; const int32_t *pos, *lengths, *counts;
-    int B, Hq, Hkv, M, cap, pairs, inter, axes, norm, end[3];      // end: of all sections but the last
+    int B, Hq, Hkv, M, cap, pairs, inter, axes, norm, offset, end[3];      // end: of all sections but the last
     int n_parts, steps, n_units;                                   // a token's rows in n_parts shares of `steps` steps
     float eps;
     Div by_parts, by_m;
@@ -60,12 +60,12 @@ __global__ __launch_bounds__(256) void cache_rope_kernel(const RopeArgs a) {
     const int at = L - C + i;                        // (below zero: of more new tokens than keys)
     float cs = 1.f, sn = 0.f;
     if (turns) {
-        int where = at;
+        double where = (double)at + (double)a.offset;
         if (a.pos) {
             const int axis = (p >= a.end[0]) + (p >= a.end[1]) + (p >= a.end[2]);
             where = a.pos[((int64_t)axis * a.B + b) * a.M + i];
         }
-        const double turn = (double)where * freq * 0.15915494309189535;
+        const double turn = where * freq * 0.15915494309189535;
         const float frac = (float)(turn - __builtin_rint(turn));
         sincospif(2.f * frac, &sn, &cs);
     }
@@ -199,6 +199,7 @@ extern "C" int trn_cache_rope_append_f16(const trn_cache16* c, const trn_rope* r
         all += rope->sections[i];
     }
     if (all != rope->pairs) return TRN_E_SHAPE;
+    if (rope->offset && rope->positions) return TRN_E_UNSUPPORTED;
     if (c->batch == 0 || tokens == 0) return TRN_OK;
     if ((rope->pairs && !rope->inv_freq) || (rope->axes > 1 && !rope->positions)) return TRN_E_NULL;
     if ((reinterpret_cast<uintptr_t>(rope->inv_freq) | reinterpret_cast<uintptr_t>(rope->gamma_q) | reinterpret_cast<uintptr_t>(rope->gamma_k)) & 7) return TRN_E_ALIGN;
@@ -226,7 +227,7 @@ extern "C" int trn_cache_rope_append_f16(const trn_cache16* c, const trn_rope* r
     a.gq = (const half_t*)rope->gamma_q; a.gk = (const half_t*)rope->gamma_k;
     a.inv = rope->inv_freq; a.pos = rope->positions; a.lengths = c->lengths; a.counts = c->counts;
     a.B = c->batch; a.Hq = n_q_heads; a.Hkv = c->n_kv_heads; a.M = tokens; a.cap = c->capacity;
-    a.pairs = rope->pairs; a.inter = rope->interleaved != 0; a.axes = rope->axes; a.norm = rope->norm != 0; a.eps = rope->eps;
+    a.pairs = rope->pairs; a.inter = rope->interleaved != 0; a.axes = rope->axes; a.norm = rope->norm != 0; a.eps = rope->eps; a.offset = rope->offset;
     for (int i = 0, sum = 0; i < 3; ++i) { sum += i < rope->axes ? rope->sections[i] : 0; a.end[i] = i + 1 < rope->axes ? sum : 0x7fffffff; }
     for (int i = 0; i < 3; ++i) {
         a.qs[i] = q_stride[i]; a.qos[i] = q_out_stride[i]; a.ks[i] = k_stride[i]; a.vs[i] = v_stride[i]; a.kcs[i] = c->k_stride[i]; a.vcs[i] = c->v_stride[i];

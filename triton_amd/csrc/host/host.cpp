@@ -713,8 +713,8 @@ trn_cache16 cache16_of(const View& k, const char* kn, const View* v, const char*
 }
 
 bool f_cache_rope_append(Args a, Py_ssize_t n) {
-    // norm, eps, interleaved, sections | None, K, K_cache, Q, Q_out, V, V_cache, counts | None, gamma_k | None, gamma_q | None, inv_freq | None, lengths | None, positions | None
-    count(n, 16, "cache_rope_append");
+    // norm, eps, interleaved, sections | None, K, K_cache, Q, Q_out, V, V_cache, counts | None, gamma_k | None, gamma_q | None, inv_freq | None, lengths | None, positions | None, offset
+    count(n, 17, "cache_rope_append");
     const View k = arg(a[4], "k"), kc = arg(a[5], "k_cache"), q = arg(a[6], "q"), qo = arg(a[7], "q_out"), v = arg(a[8], "v"), vc = arg(a[9], "v_cache");
     const trn_cache16 c = cache16_of(kc, "k_cache", &vc, "v_cache", opt(a[14], "lengths"), opt(a[10], "counts"));
     for (const View* t : {&k, &q, &qo, &v}) { const char* nm = t == &k ? "k" : t == &q ? "q" : t == &qo ? "q_out" : "v"; dev_half(*t, nm); on(*t, nm, kc); }
@@ -725,6 +725,8 @@ bool f_cache_rope_append(Args a, Py_ssize_t n) {
     trn_rope r{};
     r.norm = flag(a[0]); r.eps = (float)num(a[1]); r.interleaved = flag(a[2]);
     const OptView gk = opt(a[11], "gamma_k"), gq = opt(a[12], "gamma_q"), inv = opt(a[13], "inv_freq"), pos = opt(a[15], "positions");
+    r.offset = whole(a[16], "offset");
+    NEED(!r.offset || !pos.given, "offset given with positions");
     NEED(r.norm || (!gk.given && !gq.given), "gamma_q, gamma_k given without norm");
     for (const OptView* t : {&gk, &gq}) {
         if (!t->given) continue;

@@ -28,6 +28,7 @@ eager call -- the call the reference's drivers make before capturing a graph.
 from __future__ import annotations
 
 import functools
+import warnings
 from typing import Dict, List, Optional, Tuple
 
 import torch
@@ -643,16 +644,18 @@ class Cache8StepWeights(Cache8Step):
 # ============================================================================ fp16 caches of sequences of their own lengths
 class CacheRope(FusedModule):
     """New tokens into an fp16 cache, rotated by their positions and, norm=True, RMS-normalised by head first (`ops.cache_rope_append`).  Q_out may be Q; gammas, inv_freq,
-    positions, lengths and counts may be None.  sections: pairs of each axis (None: one axis).  One launch."""
+    positions, lengths and counts may be None.  sections: pairs of each axis (None: one axis); offset: what is added to a token's place where positions are None.  One launch."""
     TENSOR_PARAMS = ["K", "K_cache", "Q", "Q_out", "V", "V_cache", "counts", "gamma_k", "gamma_q", "inv_freq", "lengths", "positions"]
 
-    def __init__(self, norm: bool = False, eps: float = 1e-6, interleaved: bool = False, sections=None):
+    offset = 0
+
+    def __init__(self, norm: bool = False, eps: float = 1e-6, interleaved: bool = False, sections=None, offset: int = 0):
         super().__init__()
-        self.norm, self.eps, self.interleaved, self.sections = norm, eps, interleaved, None if sections is None else list(sections)
+        self.norm, self.eps, self.interleaved, self.sections, self.offset = norm, eps, interleaved, None if sections is None else list(sections), offset
 
     def _native(self, host, ws, K, K_cache, Q, Q_out, V, V_cache, counts, gamma_k, gamma_q, inv_freq, lengths, positions):
         return host.cache_rope_append(self.norm, self.eps, self.interleaved, self.sections, K, K_cache, Q, Q_out, V, V_cache, counts, gamma_k, gamma_q, inv_freq,
-                                      lengths, positions)
+                                      lengths, positions, self.offset)
 
 
 class CachePrefixAttention(FusedModule):
@@ -704,7 +707,7 @@ class _CacheStep(FusedModule):
         self.head_dim, self.scale, self.norm, self.eps = head_dim, scale, norm, eps
         self.qk_norm, self.qk_eps, self.interleaved, self.sections = qk_norm, qk_eps, interleaved, None if sections is None else list(sections)
 
-    def _put(self, K_cache, O2, V_cache, WK, WQ, WV, X, counts, gamma_k, gamma_q, inv_freq, lengths, positions):
+    def _put(self, K_cache, O2, V_cache, WK, WQ, WV, X, counts, gamma_k, gamma_q, inv_freq, lengths, positions, offset=0):
         """The step's queries, and O2, as [B,Hq,M,D]."""
         D = self.head_dim
         if X.dim() != 3 or O2.dim() != 3 or WQ.dim() != 2 or WK.dim() != 2 or WQ.shape[1] % D or WK.shape[1] % D:
@@ -720,17 +723,32 @@ class _CacheStep(FusedModule):
         if B * M:
             ops.prenorm_qkv(X.view(B * M, N), None, WQ, WK, WV, *(t.view(B * M, h, D).permute(1, 0, 2) for t, h in parts), self.eps, self.norm)      # [head, token, D]
         q, k, v = (t.view(B, M, h, D).permute(0, 2, 1, 3) for t, h in parts)      # [B, H, M, D]
-        self._host.cache_rope_append(self.qk_norm, self.qk_eps, self.interleaved, self.sections, k, K_cache, q, q, v, V_cache, counts, gamma_k, gamma_q, inv_freq, lengths, positions)
+        self._host.cache_rope_append(self.qk_norm, self.qk_eps, self.interleaved, self.sections, k, K_cache, q, q, v, V_cache, counts, gamma_k, gamma_q, inv_freq, lengths, positions, offset)
         return q, O2.view(B, M, nq // D, D).permute(0, 2, 1, 3)
 
 
 class CacheStep(_CacheStep):
     """The decode-append step (ref_rms.py:45-83, 101-127, 197-231) on an fp16 cache of a batch whose sequences have lengths of their own, with positions, behind a prefix that they
-    share (K_prefix, V_prefix [Hkv,P,D]; P may be 0): X [B,M,N], O2 [B,M,Hq*D].  Three launches, or four with shares of the keys."""
+    share (K_prefix, V_prefix [Hkv,P,D]; P may be 0): X [B,M,N], O2 [B,M,Hq*D].  Three launches, or four with shares of the keys.
+
+    Where positions are None a token is rotated by its place in its sequence's own cache, to which after_prefix=True adds P: the prefix's keys are then those of the places 0..P-1, as the
+    append leaves them.  False: the prefix's keys are rotated by -P..-1, or by what the caller means.  Not said (None), the places are as with False, with a warning where that can matter."""
     TENSOR_PARAMS = ["K_cache", "K_prefix", "O2", "V_cache", "V_prefix", "WK", "WQ", "WV", "X", "counts", "gamma_k", "gamma_q", "inv_freq", "lengths", "positions"]
+    after_prefix: Optional[bool] = None
+
+    def __init__(self, head_dim: int, *args, after_prefix: Optional[bool] = None, **kw):
+        super().__init__(head_dim, *args, **kw)
+        self.after_prefix = after_prefix
 
     def _run(self, K_cache, K_prefix, O2, V_cache, V_prefix, WK, WQ, WV, X, counts, gamma_k, gamma_q, inv_freq, lengths, positions):
-        q, o = self._put(K_cache, O2, V_cache, WK, WQ, WV, X, counts, gamma_k, gamma_q, inv_freq, lengths, positions)
+        offset = 0
+        if positions is None and inv_freq is not None and isinstance(K_prefix, torch.Tensor) and K_prefix.dim() == 3 and K_prefix.shape[1]:
+            if self.after_prefix is None:
+                warnings.warn(f"{type(self).__name__}: positions count from 0 beside a prefix of {K_prefix.shape[1]} keys; after_prefix=True counts them from its end, after_prefix=False says that they are meant so",
+                              stacklevel=3)
+                self.after_prefix = False
+            offset = K_prefix.shape[1] if self.after_prefix else 0
+        q, o = self._put(K_cache, O2, V_cache, WK, WQ, WV, X, counts, gamma_k, gamma_q, inv_freq, lengths, positions, offset)
         self._host.cache_prefix_attention(self._hws, self.scale, True, K_cache, K_prefix, o, q, V_cache, V_prefix, counts, lengths)
 
 

@@ -429,13 +429,13 @@ def cache_evict_workspace_bytes(k, weights, keep: int) -> int:
 
 def cache_rope_append(q, k, v, q_out, k_cache, v_cache, inv_freq: Optional[torch.Tensor], lengths: Optional[torch.Tensor] = None,
                       counts: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None, gamma_q: Optional[torch.Tensor] = None,
-                      gamma_k: Optional[torch.Tensor] = None, norm: bool = False, eps: float = 1e-6, interleaved: bool = False, sections=None) -> None:
+                      gamma_k: Optional[torch.Tensor] = None, norm: bool = False, eps: float = 1e-6, interleaved: bool = False, sections=None, offset: int = 0) -> None:
     """New tokens q [B,Hq,M,D], k, v [B,Hkv,M,D] fp16 into q_out (or q itself) and caches [B,Hkv,S,D]: queries and keys RMS-normalised by head (norm=True;
     gamma_q, gamma_k fp16 [D] or None) and rotated by their positions, values as they are.  inv_freq float64 [pairs] (None: no rotation): pair p, elements p and
     p + pairs or, interleaved, 2p and 2p + 1, is turned by position * inv_freq[p].  lengths int32 [B]: the keys of each sequence with the new ones (None: S); counts int32
-    [B]: its new tokens (None: M).  Token i goes to position lengths[b] - counts[b] + i, which is what it is rotated by, unless positions int32 [axes,B,M] are
-    given: of several axes, sections[axis] pairs each, one after the other.  Rows from counts[b] on are padding: neither read nor written."""
-    _lib.host().cache_rope_append(norm, eps, interleaved, sections, k, k_cache, q, q_out, v, v_cache, counts, gamma_k, gamma_q, inv_freq, lengths, positions)
+    [B]: its new tokens (None: M).  Token i goes to the place lengths[b] - counts[b] + i; it is rotated by that plus offset (behind a shared prefix: the prefix's keys), unless
+    positions int32 [axes,B,M] are given: of several axes, sections[axis] pairs each, one after the other.  Rows from counts[b] on are padding: neither read nor written."""
+    _lib.host().cache_rope_append(norm, eps, interleaved, sections, k, k_cache, q, q_out, v, v_cache, counts, gamma_k, gamma_q, inv_freq, lengths, positions, offset)
 
 
 def _cache16_sizes(k) -> "_lib.Cache16":
