@@ -66,7 +66,7 @@ def _attend(q, k, v, scale, sees):
     """One head's queries over keys of which each sees some: outputs and how far they may be off.
 
     A score is off by (D + 4) 2^-24 of the sum of its products' magnitudes, times the scale s; a weight by as much again and 2^-21; weights enter the product with V as
-    fp16 (off by 2^-11, or by half of the smallest step next to a largest weight of 2^5 at least); numerator and sum: twice.  What does not matter (a key that no query
+    fp16 (off by 2^-11, or by half of the smallest step next to a largest weight of 2^7); numerator and sum: twice.  What does not matter (a key that no query
     sees) may be anything."""
     D = q.shape[1]
     out, tol = torch.zeros(q.shape, dtype=torch.float64), torch.zeros(q.shape, dtype=torch.float64)
@@ -83,7 +83,7 @@ def _attend(q, k, v, scale, sees):
         else:
             out[i] = p @ vv
         mag = p @ vv.abs()
-        tol[i] = mag * (HALF + 2 * (float(size.max()) * (D + 8) * EPS32 + 2.0 ** -21)) + out[i].abs() * HALF + TINY + vv.abs().sum(0) * float(p.max()) * 2.0 ** -30
+        tol[i] = mag * (HALF + 2 * (float(size.max()) * (D + 8) * EPS32 + 2.0 ** -21)) + out[i].abs() * HALF + TINY + vv.abs().sum(0) * float(p.max()) * 2.0 ** -32
     return out, tol
 
 

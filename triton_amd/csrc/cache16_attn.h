@@ -5,18 +5,18 @@
 //            joined in LDS.  For few rows, which memory bounds.
 //   wide     128 rows, 32 a wave; the waves share the keys in LDS, 32 at a time.  For many rows, which the matrix pipe bounds.
 // In both K and V come from memory straight into LDS, ahead of their use, scores are formed transposed, S^T = K Q^T, so that a lane's scores are the
-// operand P^T of O^T += V^T P^T as they are, and V is read transposing.  One pass with a running maximum m, taken anew only where a score exceeds it by 2^8 (wide: where a
-// tile's weights come to more than 2^10 in all, so that no maximum is formed), and sum l.
+// operand P^T of O^T += V^T P^T as they are, and V is read transposing.  One pass with a running maximum m, taken anew only where a score exceeds it by 2^15 (wide: where a
+// tile's weights come to more than 2^15 in all, so that no maximum is formed), and sum l.
 // A workgroup may have a share of a tile's keys: (m, l, O) of the shares of a row are joined by a second launch (cache16_join).
 #pragma once
 #include "cache16.h"
 
 namespace trn {
 
-// Weights enter their product with V in fp16, 2^(score - m), and m lies below the largest score: by 2^7 (narrow) or 2^5 (wide) in units of the weights when it is taken, so that they come to 2^15 at most.
-// A key that has nearly all of the weight (what all queries look at first, its value often next to nothing) leaves little to each of the others: of a weight w of the largest's 1 this keeps 2^-32 (two
-// numbers) or 2^-30 (one), where m at the largest score would keep 2^-25: keys of 2^-20 each are off by 0.03 % or 0.1 % at most, and would be by 3 %.
-constexpr float kBelowNarrow = 7.f, kBelowWide = 5.f;
+// Weights enter their product with V in fp16, 2^(score - m), and m lies 7 below the largest score when it is taken, so that they are 2^7 there and come to 2^15 at most.
+// A key that has nearly all of the weight (what all queries look at first, its value often next to nothing) leaves little to each of the others: with the largest weight as 1, one is off by
+// 2^-32 at most, or by its own rounding, where m at the largest score would make it 2^-25: keys of 2^-20 each are off by 0.03 % at most, and would be by 3 %.
+constexpr float kBelow = 7.f;
 
 // What became of a row's keys in one share: O unnormalised, and (m, l) with m in units of log2.  Row `row` of B Hkv M G has `slots` of them.
 struct Parts { float* o; float* ml; int slots; };
@@ -156,7 +156,7 @@ __device__ __forceinline__ void narrow_walk(Keys& keys, int t0, int t1, int t_ma
         if (__builtin_expect(__builtin_amdgcn_ballot_w64(due) != 0, 0)) {       // lazily: p stays below 2^15
 #pragma unroll
             for (int qb = 0; qb < NQ; ++qb) {
-                const float up = fmaxf(m[qb], quad_max(tm[qb]) - kBelowNarrow), alpha = up == -INFINITY ? 1.f : fast_exp2(m[qb] - up);
+                const float up = fmaxf(m[qb], quad_max(tm[qb]) - kBelow), alpha = up == -INFINITY ? 1.f : fast_exp2(m[qb] - up);
                 m[qb] = up;
                 l[qb] *= alpha;
 #pragma unroll
@@ -354,14 +354,14 @@ __device__ __forceinline__ void wide_walk(const Keys keys, int t0, int t1, int t
         };
         masked();
         float sum = weights();
-        // (their sum shows whether one exceeds 2^10, and `most` whether there was no maximum yet: only then scores are looked through, formed once more.  With a maximum of each tile 41.5 us in the place of
+        // (their sum shows whether one exceeds 2^15, and `most` whether there was no maximum yet: only then scores are looked through, formed once more.  With a maximum of each tile 41.5 us in the place of
         // 40.7 at head_dim 64, 145 in the place of 143 at 128: the chunks that cache_prefix_rows_kernel names)
         if (__builtin_expect(__builtin_amdgcn_ballot_w64(!(sum <= most)) != 0, 0)) {
             asm volatile("" ::: "memory");
 #pragma unroll
             for (int i = 0; i < NS; ++i) s = mfma32(*reinterpret_cast<const half8_t*>(in(Kt, kr[i])), qB[i], i == 0 ? zero : s);
             masked();
-            const float up = fmaxf(m, half_max(max16(s) * c) - kBelowWide), alpha = up == -INFINITY ? 1.f : fast_exp2(m - up);
+            const float up = fmaxf(m, half_max(max16(s) * c) - kBelow), alpha = up == -INFINITY ? 1.f : fast_exp2(m - up);
             m = up;
             l *= alpha;
             if (m != -INFINITY) { d = -m; most = 32768.f; }
