@@ -504,7 +504,8 @@ int trn_cache_rope_append_f16(const trn_cache16* cache, const trn_rope* rope, co
  * (strides {head, token}, as the cache's) are seen by every query and read once for all; of its own sequence a query sees, causal, the
  * keys j <= lengths[b] - counts[b] + i, otherwise all.  q, o [batch, n_q_heads, seq_q, head_dim] fp16, GQA / MQA, o on 8 bytes and apart from q; rows from counts[b] on are
  * neither read nor written.  prefix 0: attention over the cache alone.  A query that sees no key gets zeros; a channel in which it sees
- * an infinite value is infinite or NaN, whatever tokens hold that it does not see stays out.  Scores, sums and the joining of shares are in fp32.
+ * an infinite value is infinite or NaN, whatever tokens hold that it does not see stays out.  Scores, sums and the joining of shares are in fp32;
+ * weights enter the product with V as two fp16 numbers, as one where a sequence has more than 128 rows a KV head and more than 512 in all.
  *   workspace  trn_cache_prefix_attn_workspace_bytes(...) bytes, 256-byte aligned, no initial contents; TRN_E_SCRATCH if smaller.  One call at a time may use it.
  */
 typedef struct trn_prefix {

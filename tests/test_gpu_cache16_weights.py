@@ -10,13 +10,13 @@ pytestmark = pytest.mark.gpu
 DEV = "cuda"
 
 
-def _inputs(B, Hkv, M, P, S, D, G):
-    """Queries that look at one channel; there the first key is 16 and the others are 12 to 17 less; values about one, the first key's zero."""
+def _inputs(B, Hkv, M, P, S, D, G, spread=5.0):
+    """Queries that look at one channel; there the first key is 16 and the others are 12 to 12 + spread less; values about one, the first key's zero."""
     g = torch.Generator().manual_seed(31)
     q = torch.zeros(B, Hkv * G, M, D)
     q[..., 0] = 1.0 + torch.arange(Hkv * G)[:, None] / 128
     k, v = torch.randn(B, Hkv, P + S, D, generator=g), 1 + 0.5 * torch.randn(B, Hkv, P + S, D, generator=g)
-    k[..., 0] = 4.0 - 5.0 * torch.rand(B, Hkv, P + S, generator=g)
+    k[..., 0] = 4.0 - spread * torch.rand(B, Hkv, P + S, generator=g)
     if P:
         k[:, :, :P], v[:, :, :P] = k[:1, :, :P].clone(), v[:1, :, :P].clone()
     k[:, :, 0, 0], v[:, :, 0] = 16.0, 0.0
@@ -24,7 +24,7 @@ def _inputs(B, Hkv, M, P, S, D, G):
 
 
 def _check(o, q, k, v, sees, fine):
-    """How far a row may be off.  A weight: 2^-32 of the largest, or 2^-22 of itself, as two fp16 numbers; 2^-30 or 2^-11 as one.  Its exponent is below 2^5 and has three roundings of 2^-24
+    """How far a row may be off.  A weight: 2^-32 of the largest, or 2^-22 of itself, as two fp16 numbers; 2^-32 or 2^-11 as one.  Its exponent is below 2^5 and has three roundings of 2^-24
     (the scale, the product, the difference: 2^-18 times ln 2 in all, with those of the largest), the exponential 2^-22: 2^-17 for numerator and sum.  Additions one behind the other: a wave's tiles,
     and 64 for those of a tile, waves and shares, 2^-24 each, in both.  The output's rounding: 2^-11, or 2^-25."""
     G, N = q.shape[1] // k.shape[1], k.shape[2]
@@ -34,7 +34,7 @@ def _check(o, q, k, v, sees, fine):
     total = w.sum(-1, keepdim=True)
     want = w @ vv / total
     size = w @ vv.abs() / total
-    least, part = (2.0 ** -32, 2.0 ** -22) if fine else (2.0 ** -30, 2.0 ** -11)
+    least, part = 2.0 ** -32, 2.0 ** -22 if fine else 2.0 ** -11
     tol = (sees.double() @ vv.abs()) / total * least + size * (part + 2.0 ** -17 + 2 * (N / 32 + 64) * 2.0 ** -24) + want.abs() * 2.0 ** -11 + 2.0 ** -25
     off = (o.double().cpu() - want).abs() - tol
     assert float(off.max()) <= 0, f"{float(off.max())} past the bound, {float((o.double().cpu() - want).norm() / want.norm()):.2g} of the outputs' size"
@@ -57,6 +57,19 @@ def test_a_key_that_has_nearly_all_weight(B, M, P, S, fine, D):
     modules.get("prefix", "cache", scale=1.0).forward(kd[:, :, P:], kd[0, :, :P], o, q.to(DEV), vd[:, :, P:], vd[0, :, :P], None, None)
     sees = torch.arange(P + S) <= (P + S - M + torch.arange(M))[:, None]
     _check(o, q, k, v, sees.expand(B, Hkv * G, M, P + S), fine)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B, M, P, S, Hkv", [(1, 40, 0, 700, 2), (24, 40, 0, 700, 2), (24, 20, 900, 300, 2), (3, 64, 600, 200, 2), (5, 1, 600, 200, 2), (60, 5, 600, 200, 2), (1, 32, 100, 700, 8), (6, 32, 100, 700, 8)])
+def test_a_step_is_as_exact_in_any_batch(B, M, P, S, Hkv, D):
+    """Up to 512 rows of a sequence, or 128 of a KV head, alone or beside many: weights are two numbers.  They are equal, so that what one number would lose does not average out."""
+    G = 4
+    q, k, v = _inputs(B, Hkv, M, P, S, D, G, 0.0)
+    o = torch.empty(B, Hkv * G, M, D, dtype=torch.float16, device=DEV)
+    kd, vd = k.to(DEV), v.to(DEV)
+    modules.get("prefix", "cache", scale=1.0).forward(kd[:, :, P:], kd[0, :, :P], o, q.to(DEV), vd[:, :, P:], vd[0, :, :P], None, None)
+    sees = torch.arange(P + S) <= (P + S - M + torch.arange(M))[:, None]
+    _check(o, q, k, v, sees.expand(B, Hkv * G, M, P + S), True)
 
 
 @pytest.mark.parametrize("D", [64, 128])

@@ -11,7 +11,10 @@ inline int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 // sequence, in narrow ones of 16 nq rows, over its own keys.  n_rt row tiles and ns shares of their keys (_p, _o; one: _p); slots: results of a row to be joined (one: none);
 // first, second: workgroups of both parts; ml: offset of the statistics in the workspace, bytes: its size.
 // short_rt: row tiles of eight waves each that have all keys, where pitches allow.
-// fine: weights as two fp16 numbers in the first of these, where all heads together have up to 512 rows (else everywhere).
+// fine: weights as two fp16 numbers in the first of these too (elsewhere always), where a sequence has up to 128 rows a KV head or 512 in all: by its own rows, so that how exact its outputs are does not depend on
+// what else is in the batch.  The second number is half as much matrix work again, and the distance from 64 bits 1.0 in the place of 1.4 times that of a computation in 32 bits.  Steps, of a few tokens a
+// sequence, are as exact as single tokens; of prompts the matrix pipe is the bound.  us with one number / with two: 32 heads of 128 on 8, 4 x 500 rows behind 4000 keys 136 / 184, 4 x 32 on 4096
+// 32.2 / 33.8, 16 x 32 on 2048 40.6 / 43.6; 71 of 64 on 1, 16 x 5 behind 16001 45.7 / 56.4.
 struct PlanPrefix { bool one, wide, fine; int short_rt; int G, R, nq, n_rt_p, ns_p, n_rt_o, ns_o, slots; int64_t first, second, ml, bytes; };
 
 inline PlanPrefix plan_prefix(int batch, int n_kv_heads, int capacity, int head_dim, int prefix, int Hq, int Sq) {
@@ -19,9 +22,10 @@ inline PlanPrefix plan_prefix(int batch, int n_kv_heads, int capacity, int head_
     p.G = Hq / n_kv_heads;
     p.R = p.G * Sq;
     const int64_t heads = (int64_t)batch * n_kv_heads, rows_p = (int64_t)batch * p.R;
-    // (rows of all sequences fill tiles better than those of each: up to one tile of these, where the prefix is what there is to read)
+    // (rows of all sequences fill tiles better than those of each: up to one tile of these, where the prefix is what there is to read.  us by tiles of each / of all, 32 heads of 128 on 8: 16 x 20 rows, 200 keys behind
+    // 8192 92.0 / 83.1, 48 x 20, 100 behind 4000 149 / 113, 4 x 20, 500 behind 4000 26.4 / 27.9, 16 x 32 (whole tiles), 200 behind 8192 111 / 123; 71 of 64 on 1, 16 x 1, 200 behind 16000 26.1 / 22.8.)
     p.one = p.R > 64 && !(p.R <= 128 && prefix > 4 * (int64_t)capacity && batch > 1);
-    p.fine = heads * p.R <= 512;
+    p.fine = p.R <= 128 || (int64_t)Hq * Sq <= 512;
     const int64_t tiles16 = (p.R + 15) / 16;
     // (as long as a wave's tiles, one after the other, take less than a second launch.  One query of 32 heads of 128 on 8, us by shares / by eight waves: one sequence, 60 keys behind 200 9.2 / 6.4, behind
     // 1000 9.7 / 10.4; 8 sequences 12.7 / 10.6, 500 behind 1000 13.3 / 13.5; 32 (wide tiles) 26.8 / 17.0, 60 behind 3000 24.4 / 20.9 before those had shares of 128 keys, 18.7 with them; 16 heads of
