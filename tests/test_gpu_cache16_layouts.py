@@ -1,4 +1,4 @@
-"""Layouts of an fp16 cache that a view may give: strides of axes that have one entry."""
+"""Layouts of an fp16 cache: strides of axes that have one entry, and caches that have room for more than they hold."""
 import pytest
 import torch
 
@@ -37,4 +37,48 @@ def test_one_key_of_any_stride(B, M, P, S, pitch, D):
         assert torch.equal(bnd.cpu(), ref.bounds(k, torch.zeros(bnd.shape).half(), 64, [1] * B, [1] * B))
         modules.get("sparse", "cache", top=2).forward(dk, o, q.to(DEV), dv, bnd, None, None, sel)
         want, tol = ref.prefix_attention(q, k, v, kp[:, :0], vp[:, :0], torch.zeros_like(q), D ** -0.5, True, [1] * B, [M] * B)
+        assert ((o.cpu().double() - want).abs() <= tol).all()
+
+
+ROOMY = [
+    # B, Hq, Hkv, D, new, lengths, counts, prefix: in a cache of 9000 places.  Narrow shares; wide tiles on the prefix; two narrow row tiles; tiles of one sequence's rows, one number and two; no prefix;
+    # nothing there
+    (2, 8, 2, 128, 1, [5, 300], [1, 1], 700),
+    (12, 8, 2, 64, 1, list(range(1, 13)), [1] * 12, 900),
+    (25, 6, 2, 128, 4, [40 - i for i in range(25)], [1 + i % 4 for i in range(25)], 1500),
+    (1, 8, 1, 64, 4, [9], [4], 300),
+    (2, 8, 2, 128, 40, [200, 47], [40, 9], 333),
+    (2, 8, 2, 64, 150, [260, 150], [150, 97], 190),
+    (3, 8, 2, 128, 1, [33, 0, 70], [1, 0, 1], 0),
+    (2, 8, 2, 64, 80, [90, 80], [80, 3], 0),
+    (2, 4, 2, 64, 2, [0, 0], [2, 1], 100),
+]
+
+
+@pytest.mark.parametrize("case", ROOMY, ids=lambda c: f"B{c[0]}H{c[1]}_{c[2]}D{c[3]}M{c[4]}P{c[7]}")
+def test_caches_with_room(case):
+    """A cache much larger than what it holds, as a serving loop allocates it: what lies behind the sequences is NaN.  Selected blocks likewise, from few to all of what is there."""
+    B, Hq, Hkv, D, M, lengths, counts, P = case
+    S, far = max(max(lengths), 1), 9000
+    g = torch.Generator().manual_seed(42)
+    q, k, v = (torch.randn(B, h, s, D, generator=g).half() for h, s in ((Hq, M), (Hkv, S), (Hkv, S)))
+    kp, vp = (torch.randn(Hkv, P, D, generator=g).half() for _ in range(2))
+    for b, (n, c) in enumerate(zip(lengths, counts)):
+        k[b, :, n:], v[b, :, n:], q[b, :, c:] = float("nan"), float("nan"), float("nan")
+    dk, dv = (torch.full((B, Hkv, far, D), float("nan"), dtype=torch.float16, device=DEV) for _ in range(2))
+    dk[:, :, :S], dv[:, :, :S] = k.to(DEV), v.to(DEV)
+    ln, ct = (torch.tensor(x, dtype=torch.int32, device=DEV) for x in (lengths, counts))
+    was = torch.randn(q.shape, generator=g).half()
+    o = was.to(DEV)
+    want, tol = ref.prefix_attention(q, k, v, kp, vp, was, D ** -0.5, True, lengths, counts)
+    modules.get("prefix", "cache").forward(dk, kp.to(DEV), o, q.to(DEV), dv, vp.to(DEV), ct, ln)
+    assert ((o.cpu().double() - want).abs() <= tol).all()
+    for top in (1, 3, 300):
+        bnd, sel = torch.zeros(B, Hkv, -(-far // 32), 2, D, dtype=torch.float16, device=DEV), torch.full((B, Hkv, M, top), 7, dtype=torch.int32, device=DEV)
+        modules.get("bounds", "cache", block=32).forward(dk, bnd, None, ln)
+        o = was.to(DEV)
+        modules.get("sparse", "cache", top=top, block=32).forward(dk, o, q.to(DEV), dv, bnd, ct, ln, sel)
+        want_sel = ref.select(q, bnd.cpu(), torch.full(sel.shape, 7, dtype=torch.int32), 32, top, 0, 1, Hq // Hkv, lengths, counts, far)
+        assert torch.equal(sel.cpu(), want_sel)
+        want, tol = ref.sparse_attention(q, k, v, was, want_sel, 32, D ** -0.5, lengths, counts)
         assert ((o.cpu().double() - want).abs() <= tol).all()

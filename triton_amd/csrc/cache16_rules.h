@@ -57,7 +57,12 @@ inline PlanPrefix plan_prefix(int batch, int n_kv_heads, int capacity, int head_
             if (s > (keys + least - 1) / least) s = (keys + least - 1) / least;
             return (int)(keys == 0 ? 0 : s < 1 ? 1 : s > 64 ? 64 : s);
         };
-        p.ns_p = shares(cost ? 512 * cost_p / cost : 0, units_p, prefix, p.wide ? 128 : 256);
+        // (the capacity is what a sequence's own keys may come to: a cache that is to be filled step by step has few at first.  So the prefix's shares are taken as if it held an eighth of the prefix's keys at most;
+        // the own keys' divide the keys that are there.  One query of 32 heads of 128 on 8, us by the capacity itself / so: 32 sequences of 701 keys behind 8192, capacity 701 31.7 / 30.8, 2804 38.7 / 30.9, 22432
+        // 193.6 / 31.1, full 8192 219 / 206; 4 of 61 behind 1000, 16384 14.8 / 11.5, full 47.4 / 47.1; 1 of 500 behind 8192, 131072 24.5 / 17.2; 128 of 701 behind 4096, 4096 126 / 85; 8 of 4096 behind 8192,
+        // full, 34.0 / 35.2.)
+        const int64_t cost_least = units_o * (capacity < prefix / 8 ? capacity : prefix / 8);
+        p.ns_p = shares(cost_p ? 512 * cost_p / (cost_p + cost_least) : 0, units_p, prefix, p.wide ? 128 : 256);
         if (p.wide && p.ns_p > 1) {
             const int best = (int)std::sqrt(0.012 * prefix / (0.1 + (double)heads * p.R * head_dim * 2e-6));
             if (p.ns_p > best) p.ns_p = best < 1 ? 1 : best;
