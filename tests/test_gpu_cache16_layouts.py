@@ -82,3 +82,21 @@ def test_caches_with_room(case):
         assert torch.equal(sel.cpu(), want_sel)
         want, tol = ref.sparse_attention(q, k, v, was, want_sel, 32, D ** -0.5, lengths, counts)
         assert ((o.cpu().double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("B, Hq, Hkv, D, M, S, counts", [(1, 71, 1, 64, 40, 900, [40]), (2, 16, 2, 128, 100, 700, [100, 37]), (1, 8, 1, 64, 128, 500, [128]), (1, 8, 1, 128, 129, 500, [120])])
+def test_selection_of_many_heads_and_queries(B, Hq, Hkv, D, M, S, counts):
+    """Eight heads and more on a KV head, 12 queries and more: scores by heads up to 128 queries, by queries above."""
+    g = torch.Generator().manual_seed(43)
+    q, k, v = (torch.randn(B, h, s, D, generator=g).half() for h, s in ((Hq, M), (Hkv, S), (Hkv, S)))
+    for b, c in enumerate(counts):
+        q[b, :, c:] = float("nan")
+    bnd = torch.zeros(B, Hkv, -(-S // 32), 2, D, dtype=torch.float16, device=DEV)
+    sel = torch.full((B, Hkv, M, 4), 7, dtype=torch.int32, device=DEV)
+    o = torch.zeros(q.shape, dtype=torch.float16, device=DEV)
+    modules.get("bounds", "cache", block=32).forward(k.to(DEV), bnd, None, None)
+    modules.get("sparse", "cache", top=4, block=32).forward(k.to(DEV), o, q.to(DEV), v.to(DEV), bnd, torch.tensor(counts, dtype=torch.int32, device=DEV), None, sel)
+    want_sel = ref.select(q, bnd.cpu(), torch.full(sel.shape, 7, dtype=torch.int32), 32, 4, 0, 1, Hq // Hkv, [S] * B, counts, S)
+    assert torch.equal(sel.cpu(), want_sel)
+    want, tol = ref.sparse_attention(q, k, v, torch.zeros_like(q), want_sel, 32, D ** -0.5, [S] * B, counts)
+    assert ((o.cpu().double() - want).abs() <= tol).all()

@@ -773,7 +773,11 @@ extern "C" int trn_cache_sparse_attn_f16(const trn_cache16* c, const void* bound
     const int64_t groups = p.rows ? heads * (((int64_t)seq_q * p.n_rt + 3) / 4) : heads * seq_q * p.n_rt * p.ns;
     // (workgroups of 256, and as many threads in all as 32 bits number: of every launch, before the first one)
     const bool many = p.nb > kMostBlocks;
-    const bool by_heads = p.step < 12;
+    // Scores by a query's heads (a tile of 16 heads a query) or by queries (a tile of 16 queries a head).  us of the whole call by queries / by heads, 16 blocks of 64 keys taken: 32 heads of 128 on 8, 32768 keys, 2
+    // queries 19.5 / 17.8, 12 22.4 / 21.5, 32 25.4 / 25.8, 8 sequences of 16384 41.1 / 42.2 with 8 and 104 / 112 with 32; 16 heads of 64 on 16, 2 of 32768 18.4 / 18.7 with 4, 21.0 / 25.0 with 16; 8 heads of 128 on 1,
+    // 65536 22.3 / 17.9 with 16, 27.4 / 25.7 with 128, 29.3 / 30.5 with 256; 64 on 2, 4 of 16384 57.8 / 46.5 with 64, 100 / 111 with 256; 71 of 64 on 1, 65536 34.5 / 19.5 with 16, 57.7 / 34.8 with 128.
+    const bool by_heads = p.step < 12 || (p.G >= 8 && p.step <= 128);
+    // Several tiles of queries a wave once there are 2048 waves: 32 heads of 128 on 8, 256 queries on 32768 keys 46.5 us from 512 waves on, 41.8 to 41.9 from 1024 on and without; others do not change.
     const int64_t q_tiles = by_heads ? p.step : (p.step + 15) / 16, waves = heads * (p.nbp / (by_heads || many ? 16 : 32)) * q_tiles;
     const int steps = many ? (waves > 4096 ? 4 : 1) : (int)(waves <= 2048 ? 1 : waves / 2048 < 8 ? waves / 2048 : 8);
     const int per64 = 4 * 512 / c->head_dim * steps;
