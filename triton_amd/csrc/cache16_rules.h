@@ -37,7 +37,7 @@ inline PlanPrefix plan_prefix(int batch, int n_kv_heads, int capacity, int head_
         p.wide = true; p.nq = 2;
         p.n_rt_p = (p.R + 127) / 128;
         const int64_t units = heads * p.n_rt_p, tiles = ((int64_t)prefix + 63) / 64 + (capacity + 63) / 64;
-        int64_t ns = (head_dim == 128 ? 512 : 1024) / units;      // (two workgroups a compute unit, four of head_dim 64: 16 x 5 rows of 71 heads of 64 behind 16001 keys, 48 tiles, 46 to 48 us with 10 to 21 shares, 57 with 22)
+        int64_t ns = (head_dim == 128 ? 512 : 1024) / units;      // (two workgroups a compute unit, four of head_dim 64: 16 x 5 rows of 71 heads of 64 behind 16001 keys, 48 tiles, 46 to 48 us with 10 to 21 shares, 57 with 22; with weights as two numbers, of which three share one, 57.5 with 21 shares, 58.7 with 16, 60.0 with 10, 65.3 with 17)
         if (ns > tiles / 4) ns = tiles / 4;
         p.ns_p = (int)(ns < 1 ? 1 : ns > 32 ? 32 : ns);
         p.slots = p.ns_p;

@@ -61,8 +61,9 @@ __device__ __forceinline__ const half_t* query(const PrefixArgs& a, int b, int k
 }
 #endif
 
-// Tiles of 128 rows of one sequence, over the prefix and its own keys.  32 heads of 128 on 8, 4 chunks of up to 500 behind 4000 keys: 133 us, 840 TFLOP/s (a share of 1024
-// keys takes 53 us with one array for all stages, 32 so); 71 heads of 64 on 1, 16 of up to 5 behind 16001: 41 us, 490 TFLOP/s, where the exponentials bound it.
+// Tiles of 128 rows of one sequence, over the prefix and its own keys.  32 heads of 128 on 8, 4 chunks of up to 500 behind 4000 keys: 132 to 136 us back to back,
+// 830 to 850 TFLOP/s (151 under the profiler; a share of 1024 keys took 53 us with one array for all stages, 32 so); 71 heads of 64 on 1, 16 of up to 5 behind 16001: 53 us, 380 TFLOP/s, where the exponentials
+// bound it and the weights' second numbers take a fifth.
 template <int D, bool FINE>
 __global__ __launch_bounds__(256, D == 128 ? 2 : FINE ? 3 : 4) void cache_prefix_rows_kernel(const PrefixArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -132,7 +133,7 @@ __global__ __launch_bounds__(512, 1) void cache_prefix_short_kernel(const Prefix
 }
 
 // The rows of all sequences over shares of the prefix (the first workgroups), each sequence's rows over shares of its own keys (the others).  32 heads of 128 on 8: 32 sequences of up to 701 keys behind
-// 8192 (104 MB) 26 us, 4.0 TB/s; 4 of 61 behind 1000 6.9 us, of which memory's latency is most.
+// 8192 (104 MB) 28.5 us, 3.7 TB/s; 4 of 61 behind 1000 7.2 us, of which memory's latency is most.
 template <int D, int NQ, bool WIDE>
 __global__ __launch_bounds__(256, 2) void cache_prefix_parts_kernel(const PrefixArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)

@@ -6,7 +6,7 @@
 // such steps as its share of the token's heads: all have the same four angles a lane.  Those are formed once, one a lane: in 64 bits as far as the
 // fraction of a turn, whose sine and cosine are taken in 32 (the argument is then off by 2^-25 of a turn at most), and handed to the lanes that share them.
 //
-// 4 prompts of up to 2047 tokens, 32 heads of 128 on 8, norms (163 MB): 32.5 us, 5.0 TB/s (37.7 with loads and stores through the caches; 32.5 with eight pairs a lane); 48 single tokens: 5.1 us.
+// 4 prompts of up to 2047 tokens, 32 heads of 128 on 8, norms (163 MB): 32.5 us, 5.0 TB/s (37.7 with loads and stores through the caches; 32.5 with eight pairs a lane); 48 single tokens: 5.2 us.
 #include "cache16.h"
 
 namespace trn {

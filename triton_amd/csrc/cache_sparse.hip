@@ -635,7 +635,7 @@ __global__ __launch_bounds__(256, 2) void cache_sparse_attn_kernel(const SparseA
 }
 
 // Many queries: a wave has one query's row tile, all its keys, and nothing is joined.  All walk up the cache at the same pace, so that blocks which several of them selected are found in
-// the L2 of their XCD.  256 queries on 32756 keys, 32 heads of 128 on 8, 32 blocks each: 85 us, 25 TB/s from L2 (171 with a workgroup a query).
+// the L2 of their XCD.  256 queries on 32756 keys, 32 heads of 128 on 8, 32 blocks each: 90 us, 24 TB/s from L2 (171 with a workgroup a query).
 template <int D, int NQ>
 __global__ __launch_bounds__(256, 2) void cache_sparse_rows_kernel(const SparseArgs a) {
 #if defined(__HIP_DEVICE_COMPILE__)
