@@ -160,3 +160,33 @@ def test_positions_of_several_axes_in_a_step(variant, D):
         assert torch.equal(sel.cpu(), want_sel)
         want, tol = ref.sparse_attention(*args, torch.zeros_like(args[0]), want_sel, 32, D ** -0.5, lengths, counts)
     _within(o.view(B, M, Hq, D).permute(0, 2, 1, 3), want, tol)
+
+
+@pytest.mark.parametrize("form", ["cache8", "cache16"])
+def test_prompts_of_any_length_share_workspaces(form):
+    """Numbers of tokens that differ from call to call do not each leave a workspace behind, and a captured step of one keeps its results while others run."""
+    B, Hq, Hkv, N, S, D = 1, 8, 2, 192, 1500, 64
+    g = torch.Generator().manual_seed(55)
+    w = _weights(g, N, Hq, Hkv, D)
+    step = modules.get("vanilla" if form == "cache8" else "prefix", form, head_dim=D)
+    nothing = torch.zeros(Hkv, 0, D, dtype=torch.float16, device=DEV)
+    t = dict(w, gamma_q=None, gamma_k=None, K_cache=torch.zeros(B, Hkv, S, D, dtype=torch.float16, device=DEV), V_cache=torch.zeros(B, Hkv, S, D, dtype=torch.float16, device=DEV), K_prefix=nothing,
+             V_prefix=nothing, K8=torch.zeros(B, Hkv, S, D, dtype=torch.float8_e4m3fn, device=DEV), V8=torch.zeros(B, Hkv, S, D, dtype=torch.float8_e4m3fn, device=DEV),
+             K_scale=torch.ones(B, Hkv, -(-S // 64), device=DEV), V_scale=torch.ones(B, Hkv, -(-S // 64), device=DEV))
+    call = lambda m: dict(X=torch.randn(B, m, N, generator=torch.Generator().manual_seed(m)).half().to(DEV), O2=torch.zeros(B, m, Hq * D, dtype=torch.float16, device=DEV), lengths=_ints([m]))
+    seven = call(7)
+    _call(step, t, **seven)
+    want = seven["O2"].clone()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        _call(step, t, **seven)
+    for m in (1, 6, 30, 200, 333, 700, 701, 1400, 1499, 8):
+        _call(step, t, **call(m))
+        seven["O2"].zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(seven["O2"], want)
+    held = [x.numel() * x.element_size() for k, x in step._ws.items() if k[0] == "qkv"]
+    # (powers of two from 1 MiB on: the largest, 1499 x 12 x 64 x 2 bytes, takes 4 MiB, and all below it less than as much again)
+    assert len(held) <= 3 and sum(held) < 8 << 20

@@ -103,6 +103,11 @@ class FusedModule:
     def _workspace(self, name: str, shape, dtype, device) -> torch.Tensor:
         return _workspace_in(self._ws, type(self).__name__, name, shape, dtype, device)
 
+    def _rows(self, name: str, rows: int, cols: int, dtype, device) -> torch.Tensor:
+        """[rows, cols] in a workspace that numbers of rows share: a serving loop meets any number of them."""
+        kept = _kept_bytes(rows * cols * dtype.itemsize) // dtype.itemsize
+        return self._workspace(name, (kept,), dtype, device)[:rows * cols].view(rows, cols)
+
     def release(self) -> None:
         """Drop every cached workspace.  Graphs captured from this instance must not be replayed afterwards."""
         self._ws.clear()
@@ -626,7 +631,7 @@ class Cache8Step(FusedModule):
         nq, nkv = WQ.shape[1], WK.shape[1]
         if O2.shape != (B, M, nq):
             raise ValueError(f"O2 {tuple(O2.shape)}: expected {(B, M, nq)}")
-        qkv = self._workspace("qkv", (B * M, nq + 2 * nkv), X.dtype, X.device)
+        qkv = self._rows("qkv", B * M, nq + 2 * nkv, X.dtype, X.device)
         parts = [(t, t.shape[1] // D) for t in (qkv[:, :nq], qkv[:, nq:nq + nkv], qkv[:, nq + nkv:])]
         if B * M:
             ops.prenorm_qkv(X.view(B * M, N), None, WQ, WK, WV, *(t.view(B * M, h, D).permute(1, 0, 2) for t, h in parts), self.eps, self.norm)      # [head, token, D]
@@ -718,7 +723,7 @@ class _CacheStep(FusedModule):
         nq, nkv = WQ.shape[1], WK.shape[1]
         if O2.shape != (B, M, nq):
             raise ValueError(f"O2 {tuple(O2.shape)}: expected {(B, M, nq)}")
-        qkv = self._workspace("qkv", (B * M, nq + 2 * nkv), X.dtype, X.device)
+        qkv = self._rows("qkv", B * M, nq + 2 * nkv, X.dtype, X.device)
         parts = [(t, t.shape[1] // D) for t in (qkv[:, :nq], qkv[:, nq:nq + nkv], qkv[:, nq + nkv:])]
         if B * M:
             ops.prenorm_qkv(X.view(B * M, N), None, WQ, WK, WV, *(t.view(B * M, h, D).permute(1, 0, 2) for t, h in parts), self.eps, self.norm)      # [head, token, D]
